@@ -27,7 +27,7 @@ STATUS_NAMES = {
 EXPORTS = ('avey_fwd_v1', 'avey_fwd_plan', 'avey_fwd_workspace_size', 'avey_fwd_noalloc_v1',
            'avey_bwd_step_v1', 'avey_bwd_workspace_size',
            'avey_last_error', 'avey_device_status', 'avey_launch_count', 'avey_abi_version',
-           'avey_test_hooks_v1', 'avey_gemm_v1', 'avey_fwd_presummed_v1')
+           'avey_test_hooks_v1', 'avey_gemm_v1', 'avey_fwd_presummed_v1', 'avey_adamw_v1')
 BWD_PREP, BWD_SCORES, BWD_EPILOGUE, BWD_DSCORES, BWD_FINAL = range(5)
 NOALLOC_MAX_ROWS = 1 << 20
 ABI_VERSION = 5
@@ -150,6 +150,37 @@ class AveyGemmParams(ctypes.Structure):
     ]
 
 
+class AveyAdamWTensor(ctypes.Structure):
+    _fields_ = [
+        ('param', ctypes.c_void_p),
+        ('grad', ctypes.c_void_p),
+        ('exp_avg', ctypes.c_void_p),
+        ('exp_avg_sq', ctypes.c_void_p),
+        ('exp_avg_scale', ctypes.c_void_p),
+        ('exp_avg_sq_scale', ctypes.c_void_p),
+        ('master', ctypes.c_void_p),
+        ('numel', ctypes.c_int64),
+    ]
+
+
+class AveyAdamWParams(ctypes.Structure):
+    _fields_ = [
+        ('struct_size', ctypes.c_uint32),
+        ('dtype', ctypes.c_int32),
+        ('state_bits', ctypes.c_int32),
+        ('count', ctypes.c_int32),
+        ('tensors', ctypes.POINTER(AveyAdamWTensor)),
+        ('lr', ctypes.c_double),
+        ('beta1', ctypes.c_double),
+        ('beta2', ctypes.c_double),
+        ('eps', ctypes.c_double),
+        ('weight_decay', ctypes.c_double),
+        ('step', ctypes.c_int64),
+        ('seed', ctypes.c_uint64),
+        ('grad_scale', ctypes.c_void_p),
+    ]
+
+
 class AveyPlan(ctypes.Structure):
     _fields_ = [
         ('kernel', ctypes.c_int32),
@@ -222,6 +253,8 @@ def lib() -> ctypes.CDLL:
         dll.avey_fwd_presummed_v1.argtypes = [ctypes.POINTER(AveyFwdParams), ctypes.c_void_p,
                                               ctypes.c_int, ctypes.c_void_p]
         dll.avey_fwd_presummed_v1.restype = ctypes.c_int
+        dll.avey_adamw_v1.argtypes = [ctypes.POINTER(AveyAdamWParams), ctypes.c_void_p]
+        dll.avey_adamw_v1.restype = ctypes.c_int
         if dll.avey_abi_version() != ABI_VERSION:
             raise RuntimeError(f'{path}: ABI version {dll.avey_abi_version()} != {ABI_VERSION}')
         _lib = dll
@@ -252,6 +285,11 @@ def forward_presummed(params: AveyFwdParams, sumsq: int, planes: int, stream: in
     """avey_fwd_presummed_v1: forward with the row sums of squares supplied."""
     _check(lib().avey_fwd_presummed_v1(ctypes.byref(params), ctypes.c_void_p(sumsq), int(planes),
                                        ctypes.c_void_p(stream)))
+
+
+def adamw(params: AveyAdamWParams, stream: int) -> None:
+    """avey_adamw_v1: enqueue one AdamW step over the listed tensors on `stream`."""
+    _check(lib().avey_adamw_v1(ctypes.byref(params), ctypes.c_void_p(stream)))
 
 
 def plan(params: AveyFwdParams) -> AveyPlan:

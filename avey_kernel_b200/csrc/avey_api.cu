@@ -14,6 +14,7 @@
 #include <string>
 
 #include "avey_b200.h"
+#include "host_api.h"
 #include "common.cuh"
 #include "ptx.cuh"
 #include "norm_prepass.cuh"
@@ -950,12 +951,29 @@ int launch_gemm_out(const AveyGemmParams* p, cudaStream_t stream) {
 
 }  // namespace
 
-// Shared with the backward translation unit (avey_bwd.cu): one last-error
+// Shared with the other translation units (host_api.h): one last-error
 // string per thread and one launch counter for the whole library.
 namespace avey_host {
 int set_error(int code, const char* msg) { return fail(code, "%s", msg); }
 int clear_error() { return ok(); }
 void count_launches(int n) { g_launches.fetch_add(static_cast<uint64_t>(n), std::memory_order_relaxed); }
+int device_ok() { return device_arch_ok(nullptr); }
+int multiprocessors() { return sm_count(); }
+int encode_rows16(int dtype, const void* base, uint64_t inner, uint64_t rows, uint64_t batch, uint64_t row_bytes,
+                  uint64_t batch_bytes, int box_rows, CUtensorMap* map) {
+  auto fn = encode_fn();
+  if (!fn) return fail(AVEY_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
+  const cuuint64_t dims[3] = {inner, rows, batch};
+  const cuuint64_t strides[2] = {row_bytes, batch > 1 ? batch_bytes : row_bytes * rows};
+  const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(box_rows), 1};
+  const cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r = fn(map, dtype == AVEY_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                        3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(AVEY_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+  return AVEY_OK;
+}
 }  // namespace avey_host
 
 extern "C" {

@@ -1,7 +1,13 @@
-"""Build ``avey_kernel_b200/lib/libavey_b200.so`` with nvcc for sm_100a.
+"""Build the native code of the package, in-tree:
+
+* ``lib/libavey_b200.so``: the CUDA library, with nvcc for sm_100a. It exports
+  only the C ABI declared in ``include/avey_b200.h``. Each source is compiled
+  to an object of its own (in parallel, and only when it or a header changed)
+  and the objects are linked.
+* ``lib/_torch_binding.so``: the Python binding of the training and serving
+  operators (host C++ against PyTorch's headers; no device code).
 
 Usage: python -m avey_kernel_b200.csrc.build [--force] [--verbose]
-The library exports only the C ABI declared in ``include/avey_b200.h``.
 """
 
 from __future__ import annotations
@@ -11,23 +17,28 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 CSRC = Path(__file__).resolve().parent
 PKG = CSRC.parent
 ROOT = PKG.parent
 LIB_DIR = PKG / 'lib'
+OBJ_DIR = LIB_DIR / 'build'
 LIB = LIB_DIR / 'libavey_b200.so'
-SOURCES = ['avey_api.cu', 'avey_bwd.cu']
+BINDING = LIB_DIR / '_torch_binding.so'
+BINDING_SOURCE = 'torch_binding.cpp'
+SOURCES = ['avey_api.cu', 'avey_bwd.cu', 'avey_optim.cu']
 HEADERS = ['ptx.cuh', 'common.cuh', 'norm_prepass.cuh', 'simt_kernel.cuh', 'simt2_kernel.cuh',
-           'small_kernel.cuh', 'tc_kernel.cuh', 'tc_long.cuh', 'tc_tf32.cuh', 'tc_gemm.cuh', 'bwd_kernels.cuh']
+           'small_kernel.cuh', 'tc_kernel.cuh', 'tc_long.cuh', 'tc_tf32.cuh', 'tc_gemm.cuh', 'bwd_kernels.cuh',
+           'host_api.h', 'adamw_kernels.cuh']
 
 NVCC_FLAGS = [
     '-gencode', 'arch=compute_100a,code=sm_100a',
     '-O3', '-lineinfo', '-std=c++17',
     '-Xcompiler', '-fPIC', '-Xcompiler', '-fvisibility=hidden',
     '--expt-relaxed-constexpr',
-    '-shared',
 ]
 
 
@@ -42,33 +53,90 @@ def nvcc_path() -> str:
     return found
 
 
-def needs_build() -> bool:
-    if not LIB.exists():
+PUBLIC_HEADER = ROOT / 'include' / 'avey_b200.h'
+
+
+def _stale(target: Path, deps) -> bool:
+    if not target.exists():
         return True
-    mtime = LIB.stat().st_mtime
-    deps = [CSRC / s for s in SOURCES + HEADERS] + [ROOT / 'include' / 'avey_b200.h']
+    mtime = target.stat().st_mtime
     return any(p.stat().st_mtime > mtime for p in deps)
 
 
-def build(force: bool = False, verbose: bool = False, extra=()) -> Path:
-    """Build the library unless it is newer than every source."""
-    target = LIB
-    if not force and not needs_build():
-        return LIB
-    LIB_DIR.mkdir(exist_ok=True)
-    tmp = target.with_suffix('.so.tmp')
-    cmd = [nvcc_path(), *NVCC_FLAGS, *extra, '-I', str(ROOT / 'include'), '-I', str(CSRC),
-           *[str(CSRC / s) for s in SOURCES], '-o', str(tmp), '-lcudart']
+def _headers(source: str, seen=None) -> set:
+    """The package's headers that `source` includes, directly or through others."""
+    seen = set() if seen is None else seen
+    for line in (CSRC / source).read_text().splitlines():
+        if line.startswith('#include "'):
+            name = line.split('"')[1]
+            if name in HEADERS and name not in seen:
+                seen.add(name)
+                _headers(name, seen)
+    return seen
+
+
+def _deps(source: str) -> list:
+    return [CSRC / source, PUBLIC_HEADER, *[CSRC / h for h in _headers(source)]]
+
+
+def needs_build() -> bool:
+    deps = [CSRC / s for s in SOURCES + HEADERS] + [PUBLIC_HEADER]
+    return _stale(LIB, deps) or _stale(BINDING, [CSRC / BINDING_SOURCE, PUBLIC_HEADER])
+
+
+def _run(cmd, verbose: bool) -> None:
     if verbose:
-        print(' '.join(cmd), flush=True)
+        print(' '.join(map(str, cmd)), flush=True)
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         sys.stderr.write(res.stdout + res.stderr)
-        raise RuntimeError(f'nvcc failed with exit code {res.returncode}')
+        raise RuntimeError(f'{Path(str(cmd[0])).name} failed with exit code {res.returncode}')
     if verbose and (res.stdout or res.stderr):
         print(res.stdout + res.stderr)
-    os.replace(tmp, target)
-    return target
+
+
+def _compile(source: str, force: bool, verbose: bool, extra) -> Path:
+    obj = OBJ_DIR / (Path(source).stem + '.o')
+    if force or _stale(obj, _deps(source)):
+        tmp = obj.with_suffix('.o.tmp')
+        _run([nvcc_path(), *NVCC_FLAGS, *extra, '-I', str(ROOT / 'include'), '-I', str(CSRC), '-c',
+              str(CSRC / source), '-o', str(tmp)], verbose)
+        os.replace(tmp, obj)
+    return obj
+
+
+def _build_binding(force: bool, verbose: bool) -> None:
+    source = CSRC / BINDING_SOURCE
+    if not force and not _stale(BINDING, [source, PUBLIC_HEADER]):
+        return
+    import torch
+    inc = Path(torch.__file__).resolve().parent / 'include'
+    cuda = Path(nvcc_path()).resolve().parents[1] / 'include'
+    libs = Path(torch.__file__).resolve().parent / 'lib'
+    tmp = BINDING.with_suffix('.so.tmp')
+    _run(['g++', '-O2', '-std=c++17', '-fPIC', '-shared', '-fvisibility=hidden',
+          f'-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}',
+          '-I', str(ROOT / 'include'), '-I', str(CSRC), '-isystem', str(inc), '-isystem',
+          str(inc / 'torch' / 'csrc' / 'api' / 'include'), '-isystem', str(cuda), '-isystem',
+          sysconfig.get_paths()['include'], str(source), '-o', str(tmp), '-L', str(libs),
+          '-lc10', '-lc10_cuda', '-ltorch', '-ltorch_cpu', '-ltorch_cuda', '-ltorch_python'], verbose)
+    os.replace(tmp, BINDING)
+
+
+def build(force: bool = False, verbose: bool = False, extra=()) -> Path:
+    """Build the library and the binding unless they are newer than every source."""
+    if not force and not needs_build():
+        return LIB
+    OBJ_DIR.mkdir(parents=True, exist_ok=True)
+    with ThreadPoolExecutor(max_workers=len(SOURCES) + 1) as pool:
+        binding = pool.submit(_build_binding, force, verbose)
+        objs = list(pool.map(lambda s: _compile(s, force, verbose, extra), SOURCES))
+        binding.result()
+    if force or _stale(LIB, objs):
+        tmp = LIB.with_suffix('.so.tmp')
+        _run([nvcc_path(), *NVCC_FLAGS, '-shared', *map(str, objs), '-o', str(tmp), '-lcudart'], verbose)
+        os.replace(tmp, LIB)
+    return LIB
 
 
 def main():

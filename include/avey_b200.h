@@ -389,6 +389,65 @@ AVEY_API int avey_gemm_v1(const AveyGemmParams* params, void* stream);
 AVEY_API int avey_fwd_presummed_v1(const AveyFwdParams* params, const float* sumsq, int planes,
                                    void* stream);
 
+/*
+ * One AdamW step over many tensors (no counterpart in the reference, which
+ * leaves training to torch). For every element of every tensor, in fp32:
+ *
+ *   g = grad * (*grad_scale, or 1)
+ *   m = beta1 m + (1 - beta1) g
+ *   v = beta2 v + (1 - beta2) g^2
+ *   p = p (1 - lr weight_decay)
+ *         - lr / (1 - beta1^step) * m / (sqrt(v) / sqrt(1 - beta2^step) + eps)
+ *
+ * p is master where given (param is then its rounding to dtype), else param.
+ *
+ * state_bits 32: exp_avg and exp_avg_sq are floats (m and v).
+ *
+ * state_bits 8: exp_avg and exp_avg_sq are float8 e4m3 codes of m and of
+ * sqrt(v), in blocks of 256 consecutive elements (the last one of a tensor may
+ * be shorter) with one float per block in exp_avg_scale / exp_avg_sq_scale:
+ * value = code * scale, scale = max |value| / 448 (at least 2^-126). A new
+ * value x is rounded stochastically: r = |x| (1 / scale), to which 20 random
+ * bits are added below the last kept bit (r + 2^-6 in place of r below 2^-6,
+ * where e4m3 is evenly spaced), and the rest is cut off. The bits of element i
+ * of the call (tensors in order, each counted in whole blocks of 256) are
+ *   h = mix(low32(i) ^ key), noise = 16 (h mod 2^16) + 8 for m and
+ *   16 (h / 2^16) + 8 for sqrt(v),
+ *   key = mix2(seed + 0x9e3779b9 (step + high32(i))) (all mod 2^32),
+ * where mix is x ^= x >> 16; x *= 0x7feb352d; x ^= x >> 15; x *= 0x846ca68b;
+ * x ^= x >> 16 and mix2 is x = (x ^ x >> 16) * 0x7feb352d, x = (x ^ x >> 16) *
+ * 0x846ca68b. The same call gives the same bits. A block that gets a
+ * non-finite value has non-finite or undefined states from then on.
+ */
+#define AVEY_ADAMW_BLOCK 256
+
+typedef struct AveyAdamWTensor {
+  void* param;             /* dtype, numel elements */
+  const void* grad;        /* dtype */
+  void* exp_avg;           /* float, or e4m3 codes */
+  void* exp_avg_sq;        /* float, or e4m3 codes of the square root */
+  float* exp_avg_scale;    /* state_bits 8: ceil(numel / 256) floats */
+  float* exp_avg_sq_scale; /* state_bits 8: ceil(numel / 256) floats */
+  float* master;           /* numel floats, or NULL (for all tensors or none) */
+  int64_t numel;           /* >= 0 */
+} AveyAdamWTensor;
+
+typedef struct AveyAdamWParams {
+  uint32_t struct_size;   /* sizeof(AveyAdamWParams) */
+  int32_t dtype;          /* AVEY_F32, AVEY_F16 or AVEY_BF16: param and grad */
+  int32_t state_bits;     /* 32 or 8 */
+  int32_t count;          /* tensors */
+  const AveyAdamWTensor* tensors; /* host array */
+  double lr, beta1, beta2, eps, weight_decay;
+  int64_t step;           /* >= 1 */
+  uint64_t seed;          /* state_bits 8 (low 32 bits are used) */
+  const float* grad_scale; /* device float that multiplies every gradient, or NULL */
+} AveyAdamWParams;
+
+/* Enqueue the step on `stream`: one launch for every 400 tensors. The arrays
+ * of a call must not overlap. */
+AVEY_API int avey_adamw_v1(const AveyAdamWParams* params, void* stream);
+
 /* Bytes of `workspace` the backward steps need for these parameters. */
 AVEY_API int avey_bwd_workspace_size(const AveyBwdParams* params, uint64_t* bytes);
 
