@@ -18,7 +18,8 @@ import torch  # noqa: F401  (the binding links against its libraries)
 from . import _native
 
 BINDING_PATH = Path(__file__).resolve().parent / 'lib' / '_torch_binding.so'
-_FUNCTIONS = ('avey_adamw_v1',)
+_FUNCTIONS = ('avey_adamw_v1', 'avey_linear_fwd_v1', 'avey_linear_bwd_v1',
+              'avey_linear_workspace_size', 'avey_last_error')
 
 _lock = threading.Lock()
 _module = None

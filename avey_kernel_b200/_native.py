@@ -27,7 +27,9 @@ STATUS_NAMES = {
 EXPORTS = ('avey_fwd_v1', 'avey_fwd_plan', 'avey_fwd_workspace_size', 'avey_fwd_noalloc_v1',
            'avey_bwd_step_v1', 'avey_bwd_workspace_size',
            'avey_last_error', 'avey_device_status', 'avey_launch_count', 'avey_abi_version',
-           'avey_test_hooks_v1', 'avey_gemm_v1', 'avey_fwd_presummed_v1', 'avey_adamw_v1')
+           'avey_test_hooks_v1', 'avey_gemm_v1', 'avey_fwd_presummed_v1', 'avey_adamw_v1',
+           'avey_linear_fwd_v1', 'avey_linear_bwd_v1', 'avey_linear_workspace_size')
+LINEAR_AUTO, LINEAR_TCGEN05, LINEAR_FEW = 0, 1, 2
 BWD_PREP, BWD_SCORES, BWD_EPILOGUE, BWD_DSCORES, BWD_FINAL = range(5)
 NOALLOC_MAX_ROWS = 1 << 20
 ABI_VERSION = 5
@@ -150,6 +152,40 @@ class AveyGemmParams(ctypes.Structure):
     ]
 
 
+class AveyLinearParams(ctypes.Structure):
+    _fields_ = [
+        ('struct_size', ctypes.c_uint32),
+        ('dtype', ctypes.c_int32),
+        ('activation', ctypes.c_int32),
+        ('kernel', ctypes.c_int32),
+        ('rows', ctypes.c_int64),
+        ('d_in', ctypes.c_int64),
+        ('d_out', ctypes.c_int64),
+        ('groups', ctypes.c_int64),
+        ('offsets', ctypes.c_void_p),
+        ('x', ctypes.c_void_p),
+        ('x_ld', ctypes.c_int64),
+        ('weight', ctypes.c_void_p),
+        ('weight_ld', ctypes.c_int64),
+        ('weight_group_stride', ctypes.c_int64),
+        ('bias', ctypes.c_void_p),
+        ('bias_group_stride', ctypes.c_int64),
+        ('residual', ctypes.c_void_p),
+        ('residual_ld', ctypes.c_int64),
+        ('y', ctypes.c_void_p),
+        ('y_ld', ctypes.c_int64),
+        ('deriv', ctypes.c_void_p),
+        ('dy', ctypes.c_void_p),
+        ('dy_ld', ctypes.c_int64),
+        ('dx', ctypes.c_void_p),
+        ('dx_ld', ctypes.c_int64),
+        ('dweight', ctypes.c_void_p),
+        ('dbias', ctypes.c_void_p),
+        ('workspace', ctypes.c_void_p),
+        ('workspace_bytes', ctypes.c_uint64),
+    ]
+
+
 class AveyAdamWTensor(ctypes.Structure):
     _fields_ = [
         ('param', ctypes.c_void_p),
@@ -255,6 +291,12 @@ def lib() -> ctypes.CDLL:
         dll.avey_fwd_presummed_v1.restype = ctypes.c_int
         dll.avey_adamw_v1.argtypes = [ctypes.POINTER(AveyAdamWParams), ctypes.c_void_p]
         dll.avey_adamw_v1.restype = ctypes.c_int
+        for name in ('avey_linear_fwd_v1', 'avey_linear_bwd_v1'):
+            getattr(dll, name).argtypes = [ctypes.POINTER(AveyLinearParams), ctypes.c_void_p]
+            getattr(dll, name).restype = ctypes.c_int
+        dll.avey_linear_workspace_size.argtypes = [ctypes.POINTER(AveyLinearParams), ctypes.c_int,
+                                                   ctypes.POINTER(ctypes.c_uint64)]
+        dll.avey_linear_workspace_size.restype = ctypes.c_int
         if dll.avey_abi_version() != ABI_VERSION:
             raise RuntimeError(f'{path}: ABI version {dll.avey_abi_version()} != {ABI_VERSION}')
         _lib = dll
@@ -285,6 +327,18 @@ def forward_presummed(params: AveyFwdParams, sumsq: int, planes: int, stream: in
     """avey_fwd_presummed_v1: forward with the row sums of squares supplied."""
     _check(lib().avey_fwd_presummed_v1(ctypes.byref(params), ctypes.c_void_p(sumsq), int(planes),
                                        ctypes.c_void_p(stream)))
+
+
+def linear(params: AveyLinearParams, stream: int, backward: bool = False) -> None:
+    """avey_linear_fwd_v1 / avey_linear_bwd_v1: enqueue a linear layer or its gradients."""
+    call = lib().avey_linear_bwd_v1 if backward else lib().avey_linear_fwd_v1
+    _check(call(ctypes.byref(params), ctypes.c_void_p(stream)))
+
+
+def linear_workspace_size(params: AveyLinearParams, backward: bool = False) -> int:
+    out = ctypes.c_uint64(0)
+    _check(lib().avey_linear_workspace_size(ctypes.byref(params), int(backward), ctypes.byref(out)))
+    return int(out.value)
 
 
 def adamw(params: AveyAdamWParams, stream: int) -> None:

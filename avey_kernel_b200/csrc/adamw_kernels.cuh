@@ -248,9 +248,11 @@ __global__ void __launch_bounds__(kAwThreads) adamw_step(const __grid_constant__
     uint32_t mtop = 0, vtop = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
+      // Each product and sum of the states is rounded by itself, so that the
+      // stochastic codes are the same bits as the formula's in plain fp32.
       const float gi = g[i] * gs;
-      m[i] = fmaf(m[i], c.b1, gi * c.c1);
-      v[i] = fmaf(v[i], c.b2, gi * gi * c.c2);
+      m[i] = __fadd_rn(__fmul_rn(m[i], c.b1), __fmul_rn(gi, c.c1));
+      v[i] = __fadd_rn(__fmul_rn(v[i], c.b2), __fmul_rn(__fmul_rn(gi, gi), c.c2));
       root[i] = sqrtf(v[i]);
       const float upd = __fdividef(m[i], fmaf(root[i], c.inv_bc2, c.eps));
       p[i] = fmaf(p[i], c.decay, -c.step_size * upd);

@@ -1166,7 +1166,10 @@ int avey_device_status(uint32_t* flags, int clear) {
   unsigned int v = 0;
   e = cudaMemcpyFromSymbol(&v, avey::g_devflags, sizeof(v));
   if (e != cudaSuccess) return fail(AVEY_ERR_CUDA, "reading the status word: %s", cudaGetErrorString(e));
-  *flags = v;
+  unsigned int lin = 0;
+  e = static_cast<cudaError_t>(avey_host::linear_flags(&lin, clear != 0));
+  if (e != cudaSuccess) return fail(AVEY_ERR_CUDA, "reading the status word: %s", cudaGetErrorString(e));
+  *flags = v | lin;
   if (clear) {
     const unsigned int zero = 0;
     e = cudaMemcpyToSymbol(avey::g_devflags, &zero, sizeof(zero));
@@ -1181,6 +1184,8 @@ int avey_test_hooks_v1(long long wait_limit_cycles, int stall) {
   if (wait_limit_cycles <= 0) wait_limit_cycles = avey::kWaitLimitCycles;
   const cudaError_t e = cudaMemcpyToSymbol(avey::g_wait_limit, &wait_limit_cycles, sizeof(long long));
   if (e != cudaSuccess) return fail(AVEY_ERR_CUDA, "setting the wait limit: %s", cudaGetErrorString(e));
+  const cudaError_t l = static_cast<cudaError_t>(avey_host::linear_wait_limit(wait_limit_cycles));
+  if (l != cudaSuccess) return fail(AVEY_ERR_CUDA, "setting the wait limit: %s", cudaGetErrorString(l));
   g_test_stall.store(stall ? 1 : 0, std::memory_order_relaxed);
   return ok();
 }

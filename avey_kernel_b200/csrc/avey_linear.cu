@@ -1,0 +1,454 @@
+// C ABI of the linear layers (declared in include/avey_b200.h): argument checks,
+// tile and kernel choice, workspace layout and the launches of tc_linear.cuh and
+// linear_steps.cuh.
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cstdio>
+#include <mutex>
+
+#include "avey_b200.h"
+#include "host_api.h"
+#include "tc_linear.cuh"
+#include "linear_steps.cuh"
+
+namespace {
+
+int fail(int code, const char* msg) { return avey_host::set_error(code, msg); }
+
+constexpr int kMaxDevices = 64;
+
+// Opt kernel K into its shared memory, once per device; the outcome is kept.
+template <auto K>
+cudaError_t smem_opt_in() {
+  static std::once_flag once[kMaxDevices];
+  static cudaError_t err[kMaxDevices];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return cudaErrorInvalidDevice;
+  std::call_once(once[dev], [dev] {
+    err[dev] = cudaFuncSetAttribute(K, cudaFuncAttributeMaxDynamicSharedMemorySize, avey::kLnSmem);
+  });
+  return err[dev];
+}
+
+int launched(const char* what) {
+  const cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) {
+    char buf[256];
+    snprintf(buf, sizeof(buf), "%s launch: %s", what, cudaGetErrorString(e));
+    return fail(AVEY_ERR_LAUNCH, buf);
+  }
+  avey_host::count_launches(1);
+  return AVEY_OK;
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+// Rows that TMA and 16-byte accesses can read in place.
+bool whole_rows(const void* p, int64_t ld) { return aligned16(p) && ld % 8 == 0; }
+int64_t up8(int64_t x) { return (x + 7) / 8 * 8; }
+uint64_t up256(uint64_t x) { return (x + 255u) & ~uint64_t(255); }
+
+// Rows up to which AUTO takes the kernel for few rows.
+constexpr int64_t kFewRows = 64;
+
+int validate(const AveyLinearParams* p, bool backward) {
+  if (!p) return fail(AVEY_ERR_ARGUMENT, "params is NULL");
+  if (p->struct_size != sizeof(AveyLinearParams))
+    return fail(AVEY_ERR_ARGUMENT, "struct_size does not match sizeof(AveyLinearParams)");
+  if (p->dtype != AVEY_BF16 && p->dtype != AVEY_F16)
+    return fail(AVEY_ERR_ARGUMENT, "linear layers take bf16 or f16 operands");
+  if (p->activation < 0 || p->activation > 4) return fail(AVEY_ERR_ARGUMENT, "unknown activation");
+  if (p->kernel < AVEY_LINEAR_KERNEL_AUTO || p->kernel > AVEY_LINEAR_KERNEL_FEW)
+    return fail(AVEY_ERR_ARGUMENT, "unknown linear kernel");
+  if (p->rows < 0 || p->rows > (1 << 30) || p->d_in < 1 || p->d_in > (1 << 24) || p->d_out < 1 ||
+      p->d_out > (1 << 24) || p->groups < 1 || p->groups > 65535)
+    return fail(AVEY_ERR_ARGUMENT, "rows must be in [0, 2^30], d_in and d_out in [1, 2^24], groups in [1, 65535]");
+  if (!p->offsets && p->groups != 1) return fail(AVEY_ERR_ARGUMENT, "more than one group needs offsets");
+  if ((p->rows + 127) / 128 + p->groups > (1ll << 30) / ((std::max(p->d_in, p->d_out) + 63) / 64))
+    return fail(AVEY_ERR_ARGUMENT, "too many output tiles");
+  if (p->rows == 0 && !backward) return AVEY_OK;
+  if (p->rows > 0 && !p->x) return fail(AVEY_ERR_ARGUMENT, "x is required");
+  if (!p->weight) return fail(AVEY_ERR_ARGUMENT, "weight is required");
+  if (p->x_ld < p->d_in || p->weight_ld < p->d_in || p->bias_group_stride < 0 ||
+      (p->groups > 1 && p->weight_group_stride < (p->d_out - 1) * p->weight_ld + p->d_in))
+    return fail(AVEY_ERR_ARGUMENT, "strides must cover the rows");
+  if (!backward) {
+    if (!p->y || p->y_ld < p->d_out || (p->residual && p->residual_ld < p->d_out))
+      return fail(AVEY_ERR_ARGUMENT, "y is required and strides must cover the rows");
+    if (p->deriv && p->activation == AVEY_ACT_IDENTITY)
+      return fail(AVEY_ERR_ARGUMENT, "the identity has no derivative to keep");
+  } else if (p->rows > 0) {
+    if (!p->dy || p->dy_ld < p->d_out || (p->dx && p->dx_ld < p->d_in))
+      return fail(AVEY_ERR_ARGUMENT, "dy is required and strides must cover the rows");
+    if (!p->deriv && p->activation != AVEY_ACT_IDENTITY)
+      return fail(AVEY_ERR_ARGUMENT, "the backward pass needs deriv from the forward pass");
+  }
+  if (p->deriv && !aligned16(p->deriv)) return fail(AVEY_ERR_ARGUMENT, "deriv must be 16-byte aligned");
+  return AVEY_OK;
+}
+
+bool use_few(const AveyLinearParams* p) {
+  if (p->kernel != AVEY_LINEAR_KERNEL_AUTO) return p->kernel == AVEY_LINEAR_KERNEL_FEW;
+  return p->rows <= kFewRows;
+}
+
+// Row tiles of `tile` rows that the groups can come to.
+int64_t row_tiles(const AveyLinearParams* p, int tile) {
+  return p->offsets ? p->rows / tile + std::min(p->groups, p->rows) : (p->rows + tile - 1) / tile;
+}
+
+// Columns per tile: 256 wide tiles read the fewest bytes from shared memory for
+// their products; narrower ones are taken where 256 would leave SMs without one.
+int tile_cols(int64_t mt, int64_t n) {
+  const int sms = avey_host::multiprocessors();
+  for (int bn : {256, 128}) {
+    if (n <= bn / 2) continue;
+    if (mt * ((n + bn - 1) / bn) * 4 >= sms * 3) return bn;
+  }
+  return 64;
+}
+
+// K ranges per group of dW: as many as give every SM a tile, of four K blocks
+// at least.
+int dw_splits(const AveyLinearParams* p, int bn) {
+  const int64_t tiles = p->groups * ((p->d_out + 127) / 128) * ((p->d_in + bn - 1) / bn);
+  const int64_t blocks = (p->rows / p->groups + 63) / 64;
+  return static_cast<int>(
+      std::max<int64_t>(1, std::min<int64_t>({avey_host::multiprocessors() / tiles, blocks / 4, 64})));
+}
+int dw_cols(const AveyLinearParams* p) { return p->d_in <= 64 ? 64 : p->d_in <= 128 ? 128 : 256; }
+
+// Workspace: [packed x | packed W | dpre | bias partials | dW partials], the
+// parts that the call needs, each 256-byte aligned.
+struct Layout {
+  bool pack_x = false, pack_w = false, make_dpre = false, sums = false;
+  int splits = 1;
+  uint64_t x = 0, w = 0, dpre = 0, partial = 0, dw = 0, total = 0;
+};
+
+Layout layout(const AveyLinearParams* p, bool backward) {
+  Layout l;
+  uint64_t at = 0;
+  auto take = [&](uint64_t bytes) {
+    const uint64_t o = at;
+    at += up256(bytes);
+    return o;
+  };
+  if (p->rows == 0 || (!backward && use_few(p))) return l;
+  const bool want_x = !backward || p->dweight, want_w = !backward || p->dx;
+  l.pack_x = want_x && !whole_rows(p->x, p->x_ld);
+  l.pack_w = want_w && !(whole_rows(p->weight, p->weight_ld) && (p->weight_group_stride % 8 == 0 || p->groups == 1));
+  if (l.pack_x) l.x = take(static_cast<uint64_t>(p->rows) * up8(p->d_in) * 2);
+  if (l.pack_w) l.w = take(static_cast<uint64_t>(p->groups) * p->d_out * up8(p->d_in) * 2);
+  if (backward) {
+    l.make_dpre = (p->dx || p->dweight) &&
+                  (p->activation != AVEY_ACT_IDENTITY || !whole_rows(p->dy, p->dy_ld));
+    l.sums = p->dbias != nullptr;
+    if (l.make_dpre) l.dpre = take(static_cast<uint64_t>(p->rows) * up8(p->d_out) * 2);
+    if (l.sums) l.partial = take(static_cast<uint64_t>(row_tiles(p, avey::kLdRows)) * p->d_out * 4);
+    if (p->dweight) {
+      l.splits = dw_splits(p, dw_cols(p));
+      if (l.splits > 1)
+        l.dw = take(static_cast<uint64_t>(l.splits) * p->groups * p->d_out * ((p->d_in + 3) / 4 * 4) * 4);
+    }
+  }
+  l.total = at;
+  return l;
+}
+
+int pack(const void* src, int64_t ld, int64_t gs, int64_t per, int64_t rows, int64_t cols, void* dst,
+         cudaStream_t stream) {
+  const int64_t pieces = rows * (up8(cols) / 8);
+  const int grid = static_cast<int>(std::min<int64_t>((pieces + 255) / 256, avey_host::multiprocessors() * 16ll));
+  avey::ln_pack_rows<<<grid, 256, 0, stream>>>(static_cast<const uint16_t*>(src), ld, gs, per, rows,
+                                               static_cast<int>(cols), static_cast<uint16_t*>(dst), up8(cols));
+  return launched("row copy");
+}
+
+// The operands as the tensor cores read them.
+struct Rows {
+  const void* p;
+  int64_t ld, gs;
+};
+
+int pack_inputs(const AveyLinearParams* p, const Layout& l, Rows* x, Rows* w, cudaStream_t stream) {
+  char* ws = static_cast<char*>(p->workspace);
+  *x = {p->x, p->x_ld, 0};
+  *w = {p->weight, p->weight_ld, p->weight_group_stride};
+  if (l.pack_x) {
+    const int rc = pack(p->x, p->x_ld, 0, p->rows, p->rows, p->d_in, ws + l.x, stream);
+    if (rc != AVEY_OK) return rc;
+    *x = {ws + l.x, up8(p->d_in), 0};
+  }
+  if (l.pack_w) {
+    const int rc = pack(p->weight, p->weight_ld, p->weight_group_stride, p->d_out, p->groups * p->d_out, p->d_in,
+                        ws + l.w, stream);
+    if (rc != AVEY_OK) return rc;
+    *w = {ws + l.w, up8(p->d_in), p->d_out * up8(p->d_in)};
+  }
+  return AVEY_OK;
+}
+
+avey::LnGeom geom(const AveyLinearParams* p, int64_t n, int bn) {
+  avey::LnGeom q{};
+  q.groups = static_cast<int>(p->groups);
+  q.offsets = p->offsets;
+  q.rows = static_cast<int>(p->rows);
+  q.n = static_cast<int>(n);
+  q.bn = bn;
+  q.n_nt = static_cast<int>((n + bn - 1) / bn);
+  q.splits = 1;
+  q.stage_bytes = avey::kLnABytes + bn * avey::kLnBK * 2;
+  q.stages = avey::kLnRing / q.stage_bytes;
+  return q;
+}
+
+template <auto K>
+int launch_tc(const CUtensorMap& a, const CUtensorMap& b, const avey::LnGeom& q, int64_t tiles, cudaStream_t stream) {
+  const cudaError_t e = smem_opt_in<K>();
+  if (e != cudaSuccess) return fail(AVEY_ERR_CUDA, cudaGetErrorString(e));
+  const int grid = static_cast<int>(std::min<int64_t>(tiles, avey_host::multiprocessors()));
+  K<<<grid, avey::kLnThreads, avey::kLnSmem, stream>>>(a, b, q);
+  return launched("tc_linear");
+}
+
+template <typename T, int ACT>
+int forward_tc(const AveyLinearParams* p, cudaStream_t stream) {
+  const Layout l = layout(p, false);
+  if (l.total > 0 && (!p->workspace || p->workspace_bytes < l.total))
+    return fail(AVEY_ERR_ARGUMENT, "workspace is smaller than avey_linear_workspace_size");
+  Rows x, w;
+  int rc = pack_inputs(p, l, &x, &w, stream);
+  if (rc != AVEY_OK) return rc;
+  const int64_t mt = row_tiles(p, avey::kLnBM);
+  avey::LnGeom q = geom(p, p->d_out, tile_cols(mt, p->d_out));
+  q.kc = static_cast<int>(p->d_in);
+  q.out = p->y;
+  q.out_ld = p->y_ld;
+  q.out_vec = whole_rows(p->y, p->y_ld);
+  q.bias = p->bias;
+  q.bias_gs = p->bias_group_stride;
+  q.res = p->residual;
+  q.res_ld = p->residual_ld;
+  q.res_vec = p->residual && whole_rows(p->residual, p->residual_ld);
+  q.deriv = static_cast<uint16_t*>(p->deriv);
+  q.deriv_ld = up8(p->d_out);
+  CUtensorMap a, b;
+  rc = avey_host::encode_rows16(p->dtype, x.p, p->d_in, p->rows, 1, x.ld * 2, 0, avey::kLnBM, &a);
+  if (rc == AVEY_OK)
+    rc = avey_host::encode_rows16(p->dtype, w.p, p->d_in, p->d_out, p->groups, w.ld * 2, w.gs * 2, q.bn, &b);
+  if (rc != AVEY_OK) return rc;
+  // One more row tile than the groups': the rows past the last group.
+  const int64_t tiles = (mt + (p->offsets ? 1 : 0)) * q.n_nt;
+  if constexpr (ACT != AVEY_ACT_IDENTITY)
+    if (p->deriv) return launch_tc<avey::tc_linear<T, avey::kLnForward, ACT, true>>(a, b, q, tiles, stream);
+  return launch_tc<avey::tc_linear<T, avey::kLnForward, ACT, false>>(a, b, q, tiles, stream);
+}
+
+template <typename T, int ACT, bool DERIV>
+int launch_few(const avey::LnFew& q, cudaStream_t stream) {
+  const dim3 grid((q.n + avey::kLfOut - 1) / avey::kLfOut, q.offsets ? std::min(q.groups, q.rows) + 1 : 1);
+  // Rows of a product: the least that hold all rows in one pass over the weights.
+  if (q.rows <= 8)
+    avey::ln_few<T, ACT, DERIV, 1><<<grid, avey::kLfThreads, 0, stream>>>(q);
+  else if (q.rows <= 16)
+    avey::ln_few<T, ACT, DERIV, 2><<<grid, avey::kLfThreads, 0, stream>>>(q);
+  else if (q.rows <= 32)
+    avey::ln_few<T, ACT, DERIV, 4><<<grid, avey::kLfThreads, 0, stream>>>(q);
+  else
+    avey::ln_few<T, ACT, DERIV, 8><<<grid, avey::kLfThreads, 0, stream>>>(q);
+  return launched("ln_few");
+}
+
+template <typename T, int ACT>
+int forward_few(const AveyLinearParams* p, cudaStream_t stream) {
+  avey::LnFew q{};
+  q.offsets = p->offsets;
+  q.groups = static_cast<int>(p->groups);
+  q.rows = static_cast<int>(p->rows);
+  q.n = static_cast<int>(p->d_out);
+  q.k = static_cast<int>(p->d_in);
+  q.x = static_cast<const uint16_t*>(p->x);
+  q.w = static_cast<const uint16_t*>(p->weight);
+  q.bias = static_cast<const uint16_t*>(p->bias);
+  q.res = static_cast<const uint16_t*>(p->residual);
+  q.x_ld = p->x_ld;
+  q.w_ld = p->weight_ld;
+  q.w_gs = p->weight_group_stride;
+  q.bias_gs = p->bias_group_stride;
+  q.res_ld = p->residual_ld;
+  q.y = static_cast<uint16_t*>(p->y);
+  q.y_ld = p->y_ld;
+  q.deriv = static_cast<uint16_t*>(p->deriv);
+  q.deriv_ld = up8(p->d_out);
+  q.x_vec = whole_rows(p->x, p->x_ld);
+  q.w_vec = whole_rows(p->weight, p->weight_ld) && (p->weight_group_stride % 8 == 0 || p->groups == 1);
+  if constexpr (ACT != AVEY_ACT_IDENTITY)
+    if (p->deriv) return launch_few<T, ACT, true>(q, stream);
+  return launch_few<T, ACT, false>(q, stream);
+}
+
+template <typename T>
+int forward(const AveyLinearParams* p, cudaStream_t stream) {
+  const bool few = use_few(p);
+  switch (p->activation) {
+#define AVEY_CASE(A) \
+  case A: return few ? forward_few<T, A>(p, stream) : forward_tc<T, A>(p, stream)
+    AVEY_CASE(AVEY_ACT_RELU);
+    AVEY_CASE(AVEY_ACT_RELU2);
+    AVEY_CASE(AVEY_ACT_SILU);
+    AVEY_CASE(AVEY_ACT_GELU);
+    default: return few ? forward_few<T, AVEY_ACT_IDENTITY>(p, stream) : forward_tc<T, AVEY_ACT_IDENTITY>(p, stream);
+#undef AVEY_CASE
+  }
+}
+
+template <typename T>
+int launch_dpre(const avey::LnDpre& q, int activation, int64_t tiles, cudaStream_t stream) {
+  const dim3 grid(static_cast<unsigned>(tiles), (q.n + avey::kLdCols - 1) / avey::kLdCols);
+  switch (activation) {
+    case AVEY_ACT_IDENTITY: avey::ln_dpre<T, 0><<<grid, avey::kLdThreads, 0, stream>>>(q); break;
+    case AVEY_ACT_RELU2: avey::ln_dpre<T, 2><<<grid, avey::kLdThreads, 0, stream>>>(q); break;
+    default: avey::ln_dpre<T, 1><<<grid, avey::kLdThreads, 0, stream>>>(q); break;  // one code for the bounded ones
+  }
+  return launched("ln_dpre");
+}
+
+template <typename T>
+int backward(const AveyLinearParams* p, cudaStream_t stream) {
+  const Layout l = layout(p, true);
+  if (l.total > 0 && (!p->workspace || p->workspace_bytes < l.total))
+    return fail(AVEY_ERR_ARGUMENT, "workspace is smaller than avey_linear_workspace_size");
+  char* ws = static_cast<char*>(p->workspace);
+  Rows x, w, g{p->dy, p->dy_ld, 0};
+  int rc = pack_inputs(p, l, &x, &w, stream);
+  if (rc != AVEY_OK) return rc;
+  if (l.make_dpre || l.sums) {
+    avey::LnDpre q{};
+    q.offsets = p->offsets;
+    q.groups = static_cast<int>(p->groups);
+    q.rows = static_cast<int>(p->rows);
+    q.n = static_cast<int>(p->d_out);
+    q.dy = static_cast<const uint16_t*>(p->dy);
+    q.dy_ld = p->dy_ld;
+    q.dy_vec = whole_rows(p->dy, p->dy_ld);
+    q.deriv = static_cast<const uint16_t*>(p->deriv);
+    q.deriv_ld = up8(p->d_out);
+    if (l.make_dpre) {
+      q.dpre = reinterpret_cast<uint16_t*>(ws + l.dpre);
+      q.dpre_ld = up8(p->d_out);
+      g = {q.dpre, q.dpre_ld, 0};
+    }
+    if (l.sums) q.partial = reinterpret_cast<float*>(ws + l.partial);
+    rc = launch_dpre<T>(q, p->activation, row_tiles(p, avey::kLdRows), stream);
+    if (rc != AVEY_OK) return rc;
+    if (l.sums) {
+      const dim3 grid(static_cast<unsigned>((p->d_out + 31) / 32), static_cast<unsigned>(p->groups));
+      avey::ln_bias_sum<T><<<grid, 256, 0, stream>>>(p->offsets, q.groups, q.rows, q.n, q.partial,
+                                                     static_cast<T*>(p->dbias));
+      rc = launched("ln_bias_sum");
+      if (rc != AVEY_OK) return rc;
+    }
+  }
+  CUtensorMap a, b;
+  if (p->dx) {
+    const int64_t mt = row_tiles(p, avey::kLnBM);
+    avey::LnGeom q = geom(p, p->d_in, tile_cols(mt, p->d_in));
+    q.kc = static_cast<int>(p->d_out);
+    q.out = p->dx;
+    q.out_ld = p->dx_ld;
+    q.out_vec = whole_rows(p->dx, p->dx_ld);
+    rc = avey_host::encode_rows16(p->dtype, g.p, p->d_out, p->rows, 1, g.ld * 2, 0, avey::kLnBM, &a);
+    if (rc == AVEY_OK)
+      rc = avey_host::encode_rows16(p->dtype, w.p, p->d_in, p->d_out, p->groups, w.ld * 2, w.gs * 2, 64, &b);
+    if (rc != AVEY_OK) return rc;
+    const int64_t tiles = (mt + (p->offsets ? 1 : 0)) * q.n_nt;
+    rc = launch_tc<avey::tc_linear<T, avey::kLnGradX, 0, false>>(a, b, q, tiles, stream);
+    if (rc != AVEY_OK) return rc;
+  }
+  if (p->dweight) {
+    avey::LnGeom q = geom(p, p->d_in, dw_cols(p));
+    q.m = static_cast<int>(p->d_out);
+    q.n_mt = (q.m + avey::kLnBM - 1) / avey::kLnBM;
+    q.splits = l.splits;
+    const bool parts = l.splits > 1;
+    q.out = parts ? static_cast<void*>(ws + l.dw) : p->dweight;
+    q.out_ld = parts ? (p->d_in + 3) / 4 * 4 : p->d_in;
+    q.out_gs = p->d_out * q.out_ld;
+    q.out_vec = !parts && whole_rows(p->dweight, p->d_in);
+    rc = avey_host::encode_rows16(p->dtype, g.p, p->d_out, p->rows, 1, g.ld * 2, 0, 64, &a);
+    if (rc == AVEY_OK) rc = avey_host::encode_rows16(p->dtype, x.p, p->d_in, p->rows, 1, x.ld * 2, 0, 64, &b);
+    if (rc != AVEY_OK) return rc;
+    const int64_t tiles = p->groups * q.n_mt * q.n_nt * q.splits;
+    rc = parts ? launch_tc<avey::tc_linear<T, avey::kLnGradW, 0, true>>(a, b, q, tiles, stream)
+               : launch_tc<avey::tc_linear<T, avey::kLnGradW, 0, false>>(a, b, q, tiles, stream);
+    if (rc != AVEY_OK) return rc;
+    if (parts) {
+      const int64_t rows = p->groups * p->d_out, quads = rows * (q.out_ld / 4);
+      const int grid = static_cast<int>(std::min<int64_t>((quads + 255) / 256, avey_host::multiprocessors() * 8ll));
+      avey::ln_split_sum<T><<<grid, 256, 0, stream>>>(static_cast<const float*>(q.out), l.splits, rows,
+                                                      static_cast<int>(p->d_in), q.out_ld,
+                                                      static_cast<T*>(p->dweight));
+      rc = launched("ln_split_sum");
+      if (rc != AVEY_OK) return rc;
+    }
+  }
+  return avey_host::clear_error();
+}
+
+}  // namespace
+
+// The status word and the wait limit of this translation unit's kernels
+// (ptx.cuh), for avey_device_status and avey_test_hooks_v1.
+namespace avey_host {
+int linear_flags(unsigned int* flags, bool clear) {
+  cudaError_t e = cudaMemcpyFromSymbol(flags, avey::g_devflags, sizeof(*flags));
+  const unsigned int zero = 0;
+  if (e == cudaSuccess && clear) e = cudaMemcpyToSymbol(avey::g_devflags, &zero, sizeof(zero));
+  return e;
+}
+int linear_wait_limit(long long cycles) {
+  return cudaMemcpyToSymbol(avey::g_wait_limit, &cycles, sizeof(cycles));
+}
+}  // namespace avey_host
+
+extern "C" {
+
+int avey_linear_workspace_size(const AveyLinearParams* p, int backward, uint64_t* bytes) {
+  const int rc = validate(p, backward != 0);
+  if (rc != AVEY_OK) return rc;
+  if (!bytes) return fail(AVEY_ERR_ARGUMENT, "bytes is NULL");
+  *bytes = layout(p, backward != 0).total;
+  return avey_host::clear_error();
+}
+
+int avey_linear_fwd_v1(const AveyLinearParams* p, void* stream) {
+  int rc = validate(p, false);
+  if (rc != AVEY_OK) return rc;
+  if (p->rows == 0) return avey_host::clear_error();
+  rc = avey_host::device_ok();
+  if (rc != AVEY_OK) return rc;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  rc = p->dtype == AVEY_BF16 ? forward<__nv_bfloat16>(p, s) : forward<__half>(p, s);
+  return rc == AVEY_OK ? avey_host::clear_error() : rc;
+}
+
+int avey_linear_bwd_v1(const AveyLinearParams* p, void* stream) {
+  int rc = validate(p, true);
+  if (rc != AVEY_OK) return rc;
+  rc = avey_host::device_ok();
+  if (rc != AVEY_OK) return rc;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (p->rows == 0) {
+    // No rows: the weights' gradients are zero.
+    cudaError_t e = cudaSuccess;
+    if (p->dweight) e = cudaMemsetAsync(p->dweight, 0, static_cast<size_t>(p->groups) * p->d_out * p->d_in * 2, s);
+    if (e == cudaSuccess && p->dbias)
+      e = cudaMemsetAsync(p->dbias, 0, static_cast<size_t>(p->groups) * p->d_out * 2, s);
+    return e == cudaSuccess ? avey_host::clear_error() : fail(AVEY_ERR_CUDA, cudaGetErrorString(e));
+  }
+  return p->dtype == AVEY_BF16 ? backward<__nv_bfloat16>(p, s) : backward<__half>(p, s);
+}
+
+}  // extern "C"

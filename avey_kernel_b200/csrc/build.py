@@ -29,10 +29,11 @@ OBJ_DIR = LIB_DIR / 'build'
 LIB = LIB_DIR / 'libavey_b200.so'
 BINDING = LIB_DIR / '_torch_binding.so'
 BINDING_SOURCE = 'torch_binding.cpp'
-SOURCES = ['avey_api.cu', 'avey_bwd.cu', 'avey_optim.cu']
+SOURCES = ['avey_api.cu', 'avey_bwd.cu', 'avey_optim.cu', 'avey_linear.cu']
 HEADERS = ['ptx.cuh', 'common.cuh', 'norm_prepass.cuh', 'simt_kernel.cuh', 'simt2_kernel.cuh',
            'small_kernel.cuh', 'tc_kernel.cuh', 'tc_long.cuh', 'tc_tf32.cuh', 'tc_gemm.cuh', 'bwd_kernels.cuh',
-           'host_api.h', 'adamw_kernels.cuh']
+           'host_api.h', 'adamw_kernels.cuh',
+           'tc_linear.cuh', 'linear_steps.cuh']
 
 NVCC_FLAGS = [
     '-gencode', 'arch=compute_100a,code=sm_100a',

@@ -24,4 +24,9 @@ int multiprocessors();
 int encode_rows16(int dtype, const void* base, uint64_t inner, uint64_t rows, uint64_t batch, uint64_t row_bytes,
                   uint64_t batch_bytes, int box_rows, CUtensorMap* map);
 
+// The status word (read, and reset with `clear`) and the wait limit of the
+// kernels of avey_linear.cu, on the current device; a cudaError_t.
+int linear_flags(unsigned int* flags, bool clear);
+int linear_wait_limit(long long cycles);
+
 }  // namespace avey_host

@@ -1,0 +1,344 @@
+// The steps of the linear layers (avey_linear_*) around the products of
+// tc_linear.cuh: the kernel for few rows, dpre = dy act' with the bias
+// gradient's partial sums, the sums of partial results in a fixed order, and
+// the copy that lays rows out in whole 16-byte units.
+#pragma once
+
+#include "tc_linear.cuh"
+
+namespace avey {
+
+// ---------------------------------------------------------------- groups, by a warp
+
+struct LnSpan {
+  int g, lo, hi;  // group and its rows
+  int index;      // which of the group's tiles
+  int base, cnt;  // the group's first tile and its tiles
+};
+
+// Every lane of the warp: walk the groups 32 at a time, a group counting
+// count(lo, hi) items, and find the group that holds item t (t >= 0), or the
+// items of group `want` (t < 0). False when there is none.
+template <typename Count>
+__device__ __forceinline__ bool ln_find(const int32_t* offsets, int groups, int rows, int t, int want, Count count,
+                                        LnSpan& out) {
+  const int lane = threadIdx.x & 31;
+  int end_carry = 0, base = 0;
+  for (int g0 = 0; g0 < groups; g0 += 32) {
+    const int g = g0 + lane;
+    int hi = g < groups ? (offsets ? min(max(__ldg(offsets + g + 1), 0), rows) : rows) : 0;
+    hi = max(hi, end_carry);
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int o = __shfl_up_sync(0xFFFFFFFFu, hi, d);
+      if (lane >= d) hi = max(hi, o);
+    }
+    int lo = __shfl_up_sync(0xFFFFFFFFu, hi, 1);
+    if (lane == 0) lo = end_carry;
+    const int cnt = g < groups ? count(lo, hi) : 0;
+    int incl = cnt;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int o = __shfl_up_sync(0xFFFFFFFFu, incl, d);
+      if (lane >= d) incl += o;
+    }
+    const int excl = base + incl - cnt;
+    const bool mine = t >= 0 ? (t >= excl && t < excl + cnt) : g == want;
+    const unsigned hit = __ballot_sync(0xFFFFFFFFu, mine);
+    if (hit) {
+      const int src = __ffs(hit) - 1;
+      out.g = g0 + src;
+      out.lo = __shfl_sync(0xFFFFFFFFu, lo, src);
+      out.hi = __shfl_sync(0xFFFFFFFFu, hi, src);
+      out.base = __shfl_sync(0xFFFFFFFFu, excl, src);
+      out.cnt = __shfl_sync(0xFFFFFFFFu, cnt, src);
+      out.index = t - out.base;
+      return true;
+    }
+    end_carry = __shfl_sync(0xFFFFFFFFu, hi, 31);
+    base += __shfl_sync(0xFFFFFFFFu, incl, 31);
+  }
+  // Not found: the rows past the last group, and the items in all.
+  out.g = groups;
+  out.lo = end_carry;
+  out.hi = rows;
+  out.base = base;
+  out.cnt = 0;
+  out.index = t - base;
+  return false;
+}
+
+// Eight 16-bit values at p as four words; values at `left` and beyond are zero.
+__device__ __forceinline__ uint4 ln_load8(const uint16_t* p, int left, bool vec) {
+  if (vec && left >= 8) return __ldg(reinterpret_cast<const uint4*>(p));
+  uint32_t w[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if (j < left) w[j >> 1] |= static_cast<uint32_t>(__ldg(p + j)) << (16 * (j & 1));
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// ---------------------------------------------------------------- few rows
+
+// y for a few rows per group: the weights are read once, straight from global
+// memory into mma.sync fragments (bound: their bytes; the products are far
+// below any tensor rate, and 128-row tiles would leave most SMs without
+// work). W is the 16-row operand, up to 8 NT rows of x the 8-column one. The
+// order of k inside a product is free as long as both operands agree, so a
+// lane takes 8 consecutive k (16 bytes) of a 32-wide step for its fragments.
+// A CTA owns 16 outputs; its 8 warps take every eighth step of K, and their sums
+// are added in a fixed order.
+constexpr int kLfThreads = 256;
+constexpr int kLfOut = 16;
+
+struct LnFew {
+  const int32_t* offsets;
+  int groups, rows, n, k;
+  const uint16_t *x, *w, *bias, *res;
+  int64_t x_ld, w_ld, w_gs, bias_gs, res_ld, y_ld, deriv_ld;
+  uint16_t *y, *deriv;
+  int x_vec, w_vec;
+};
+
+template <typename T>
+__device__ __forceinline__ void ln_mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                       uint32_t b1) {
+  if constexpr (std::is_same<T, __half>::value)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+template <typename T, int ACT, bool DERIV, int NT>
+__global__ void __launch_bounds__(kLfThreads) ln_few(const LnFew q) {
+  __shared__ float red[8][8 * NT][kLfOut + 1];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int n0 = blockIdx.x * kLfOut;
+  LnSpan s{0, 0, q.rows, 0, 0, 1};
+  if (q.offsets) {
+    // Slot y: the y-th group that has rows; the slot after the last: the rest.
+    ln_find(q.offsets, q.groups, q.rows, blockIdx.y, 0, [](int lo, int hi) { return hi > lo ? 1 : 0; }, s);
+    if (s.g == q.groups && s.index != 0) return;
+  }
+  const bool zero = s.g == q.groups;
+  const uint16_t* w0 = q.w + static_cast<int64_t>(s.g) * q.w_gs;
+  const int o_lo = n0 + (lane >> 2), o_hi = o_lo + 8;
+  const uint16_t* wl = w0 + static_cast<int64_t>(o_lo) * q.w_ld;
+  const uint16_t* wh = w0 + static_cast<int64_t>(o_hi) * q.w_ld;
+  for (int r0 = s.lo; r0 < s.hi; r0 += 8 * NT) {
+    float acc[NT][4];
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[j][i] = 0.f;
+    if (!zero) {
+      constexpr int kUnroll = NT >= 4 ? 2 : 4;
+      const int steps = (q.k + 31) / 32;
+      for (int s0 = warp; s0 < steps; s0 += 8 * kUnroll) {
+        uint4 a[kUnroll], b[kUnroll], v[kUnroll][NT];
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+          const int k = (s0 + 8 * u) * 32 + (lane & 3) * 8;
+          const int left = q.k - k;
+          a[u] = b[u] = make_uint4(0u, 0u, 0u, 0u);
+          if (left > 0 && o_lo < q.n) a[u] = ln_load8(wl + k, left, q.w_vec);
+          if (left > 0 && o_hi < q.n) b[u] = ln_load8(wh + k, left, q.w_vec);
+#pragma unroll
+          for (int j = 0; j < NT; ++j) {
+            const int row = r0 + j * 8 + (lane >> 2);
+            v[u][j] = make_uint4(0u, 0u, 0u, 0u);
+            if (left > 0 && row < s.hi)
+              v[u][j] = ln_load8(q.x + static_cast<int64_t>(row) * q.x_ld + k, left, q.x_vec);
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u)
+#pragma unroll
+          for (int j = 0; j < NT; ++j) {
+            ln_mma<T>(acc[j], a[u].x, b[u].x, a[u].y, b[u].y, v[u][j].x, v[u][j].y);
+            ln_mma<T>(acc[j], a[u].z, b[u].z, a[u].w, b[u].w, v[u][j].z, v[u][j].w);
+          }
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        red[warp][j * 8 + (lane & 3) * 2 + (i & 1)][(lane >> 2) + (i >> 1) * 8] = acc[j][i];
+    __syncthreads();
+    for (int i = threadIdx.x; i < 8 * NT * kLfOut; i += kLfThreads) {
+      const int r = i / kLfOut, o = i % kLfOut;
+      const int row = r0 + r, col = n0 + o;
+      if (row >= s.hi || col >= q.n) continue;
+      float z = 0.f;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) z += red[k][r][o];
+      float y = 0.f, d;
+      if (!zero) {
+        if (q.bias) z += Elem<T>::to_f(reinterpret_cast<const T*>(q.bias)[static_cast<int64_t>(s.g) * q.bias_gs + col]);
+        y = ln_act<ACT, DERIV>(z, &d);
+        if (DERIV) q.deriv[static_cast<int64_t>(row) * q.deriv_ld + col] = static_cast<uint16_t>(ln_encode<T, ACT>(d));
+        if (q.res) y += Elem<T>::to_f(reinterpret_cast<const T*>(q.res)[static_cast<int64_t>(row) * q.res_ld + col]);
+      }
+      reinterpret_cast<T*>(q.y)[static_cast<int64_t>(row) * q.y_ld + col] = Elem<T>::from_f(y);
+    }
+  }
+}
+
+// ---------------------------------------------------------------- dpre
+
+// dpre = dy act' in the operand type, and the fp32 sums of dpre (before that
+// rounding) over every tile of 64 rows of a group. Bound by HBM: 6 bytes an
+// element. A warp reads rows of 512 bytes, a thread 8 columns of 8 rows at once.
+constexpr int kLdThreads = 256;
+constexpr int kLdRows = 64, kLdCols = 256;
+
+struct LnDpre {
+  const int32_t* offsets;
+  int groups, rows, n;
+  const uint16_t* dy;
+  int64_t dy_ld;
+  int dy_vec;
+  const uint16_t* deriv;  // null: the identity
+  int64_t deriv_ld;
+  uint16_t* dpre;  // null: only the sums are wanted
+  int64_t dpre_ld;
+  float* partial;  // [tiles][n], or null
+};
+
+template <typename T, int ACT>
+__global__ void __launch_bounds__(kLdThreads) ln_dpre(const LnDpre q) {
+  __shared__ float red[8][kLdCols];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  LnSpan s;
+  if (!ln_find(q.offsets, q.groups, q.rows, blockIdx.x, 0,
+               [](int lo, int hi) { return (hi - lo + kLdRows - 1) / kLdRows; }, s))
+    return;
+  const int row0 = s.lo + s.index * kLdRows, row1 = min(s.hi, row0 + kLdRows);
+  const int col = blockIdx.y * kLdCols + lane * 8;
+  const int left = q.n - col;
+  float sum[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) sum[j] = 0.f;
+  if (left > 0) {
+    uint4 g[8], d[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int row = row0 + warp + 8 * i;
+      g[i] = d[i] = make_uint4(0u, 0u, 0u, 0u);
+      if (row < row1) {
+        g[i] = ln_load8(q.dy + static_cast<int64_t>(row) * q.dy_ld + col, left, q.dy_vec);
+        if (ACT != 0) d[i] = ln_load8(q.deriv + static_cast<int64_t>(row) * q.deriv_ld + col, left, true);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int row = row0 + warp + 8 * i;
+      if (row >= row1) break;
+      const uint32_t gw[4] = {g[i].x, g[i].y, g[i].z, g[i].w}, dw[4] = {d[i].x, d[i].y, d[i].z, d[i].w};
+      uint32_t o[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float2 v = ln_unpack<T>(gw[j]);
+        if (ACT != 0) {
+          v.x *= ln_decode<T, ACT>(dw[j] & 0xFFFFu);
+          v.y *= ln_decode<T, ACT>(dw[j] >> 16);
+        }
+        sum[2 * j] += v.x;
+        sum[2 * j + 1] += v.y;
+        o[j] = ln_pack<T>(v.x, v.y);
+      }
+      if (q.dpre)  // rows of dpre are whole 16-byte units
+        *reinterpret_cast<uint4*>(q.dpre + static_cast<int64_t>(row) * q.dpre_ld + col) =
+            make_uint4(o[0], o[1], o[2], o[3]);
+    }
+  }
+  if (!q.partial) return;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) red[warp][lane * 8 + j] = sum[j];
+  __syncthreads();
+  const int c = blockIdx.y * kLdCols + threadIdx.x;
+  if (c < q.n) {
+    float t = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t += red[i][threadIdx.x];
+    q.partial[static_cast<int64_t>(blockIdx.x) * q.n + c] = t;
+  }
+}
+
+// db[g] = the sum of the group's partial rows (a fixed order: lane i of 8 takes
+// every eighth row, then the lanes in turn).
+template <typename T>
+__global__ void __launch_bounds__(256) ln_bias_sum(const int32_t* offsets, int groups, int rows, int n,
+                                                   const float* partial, T* db) {
+  __shared__ float red[8][33];
+  const int lane = threadIdx.x & 31, part = threadIdx.x >> 5;
+  LnSpan s;
+  ln_find(offsets, groups, rows, -1, blockIdx.y, [](int lo, int hi) { return (hi - lo + kLdRows - 1) / kLdRows; }, s);
+  const int c = blockIdx.x * 32 + lane;
+  float t = 0.f;
+  if (c < n)
+    for (int i = part; i < s.cnt; i += 8) t += partial[static_cast<int64_t>(s.base + i) * n + c];
+  red[part][lane] = t;
+  __syncthreads();
+  if (part == 0 && c < n) {
+    float z = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) z += red[i][lane];
+    db[static_cast<int64_t>(blockIdx.y) * n + c] = Elem<T>::from_f(z);
+  }
+}
+
+// out[row][c] = sum over the splits of partial[split][row][c], in split order;
+// rows of `partial` have `ld` floats (a multiple of 4), rows of `out` n values.
+template <typename T>
+__global__ void __launch_bounds__(256) ln_split_sum(const float* partial, int splits, int64_t rows, int n, int64_t ld,
+                                                    T* out) {
+  const int64_t per = ld / 4, total = rows * per, plane = rows * ld;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < total;
+       i += static_cast<int64_t>(gridDim.x) * 256) {
+    const int64_t row = i / per;
+    const int c = static_cast<int>(i - row * per) * 4;
+    const float* p = partial + row * ld + c;
+    float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int s = 0; s < splits; ++s) {
+      const float4 v = *reinterpret_cast<const float4*>(p + s * plane);
+      z.x += v.x;
+      z.y += v.y;
+      z.z += v.z;
+      z.w += v.w;
+    }
+    T* o = out + row * n + c;
+    if (c + 4 <= n && (n & 3) == 0) {
+      *reinterpret_cast<uint2*>(o) = make_uint2(ln_pack<T>(z.x, z.y), ln_pack<T>(z.z, z.w));
+    } else {
+      const float v[4] = {z.x, z.y, z.z, z.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (c + j < n) o[j] = Elem<T>::from_f(v[j]);
+    }
+  }
+}
+
+// Rows of `cols` 16-bit values (per rows of a group, groups gs apart) copied to
+// rows of ld values (a multiple of 8), zeros at the end: what TMA can read.
+__global__ void __launch_bounds__(256) ln_pack_rows(const uint16_t* src, int64_t src_ld, int64_t src_gs, int64_t per,
+                                                    int64_t rows, int cols, uint16_t* dst, int64_t ld) {
+  const int64_t pieces = ld / 8, total = rows * pieces;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < total;
+       i += static_cast<int64_t>(gridDim.x) * 256) {
+    const int64_t row = i / pieces, g = row / per;
+    const int c = static_cast<int>(i - row * pieces) * 8;
+    const uint16_t* p = src + g * src_gs + (row - g * per) * src_ld + c;
+    *reinterpret_cast<uint4*>(dst + row * ld + c) = ln_load8(p, cols - c, false);
+  }
+}
+
+}  // namespace avey

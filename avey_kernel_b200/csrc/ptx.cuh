@@ -7,15 +7,15 @@
 
 namespace avey {
 
-// Device status word shared by every kernel of the library (AVEY_DEVFLAG_*).
-// The library is a single translation unit, so the definition lives here.
-__device__ unsigned int g_devflags = 0u;
+// Device status word of the kernels of a translation unit (AVEY_DEVFLAG_*);
+// avey_device_status joins those of all.
+static __device__ unsigned int g_devflags = 0u;
 
 // ~2^31 SM cycles (about one second at 1.9 GHz) before a wait gives up.
 constexpr long long kWaitLimitCycles = 1ll << 31;
 // The limit in force: kWaitLimitCycles unless a test lowers it (test-only
 // entry point avey_test_hooks_v1). Read only on the slow path of a wait.
-__device__ long long g_wait_limit = kWaitLimitCycles;
+static __device__ long long g_wait_limit = kWaitLimitCycles;
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));

@@ -1,0 +1,668 @@
+// Linear layers on tcgen05, dense or grouped by expert (avey_linear_*):
+//
+//   forward   y  = act(x W_g^T + b_g) + r    (and a 16-bit code of act')
+//   dX        dx = dpre W_g
+//   dW        dW_g = dpre_g^T x_g            (fp32 partial sums when split over rows)
+//
+// where group g owns the rows [offsets[g], offsets[g + 1]) of x; a dense layer
+// is one group of all rows. The groups' sizes are known on the device only:
+// every role of the kernel walks the offsets itself, so nothing is read back to
+// the host, and rows past the last group give zeros.
+//
+// Bounds: 2 M N K flops on the tensor cores against reading x, W, r and
+// writing y once. Tiles are 128 rows x 256 columns (128 or 64 where 256 would
+// leave SMs without a tile), K in blocks of 64 through a TMA ring (128-byte
+// swizzle). Persistent CTAs, one per SM: warp 0 issues TMA, warp 1 issues
+// tcgen05.mma into one of two TMEM accumulators, warps 4-11 drain the other one,
+// so a tile's epilogue overlaps the next tile's products; warp 2 clears the
+// rows of a neighbouring group out of dW's last K block. Every wait is bounded.
+#pragma once
+
+#include <cuda.h>
+
+#include <type_traits>
+
+#include "common.cuh"
+#include "ptx.cuh"
+
+namespace avey {
+
+constexpr int kLnThreads = 384;
+constexpr int kLnBM = 128, kLnBK = 64;
+constexpr int kLnABytes = kLnBM * kLnBK * 2;  // 16 KB
+constexpr int kLnMnBox = 64 * kLnBK * 2;      // one {64 (m or n), 64 (k)} box: 8 KB
+constexpr int kLnStageTile = 4096;            // an epilogue warp's staging: two 32 x 32 16-bit tiles
+constexpr int kLnMaxStages = 8;
+constexpr int kLnCtrlBytes = 512;
+constexpr int kLnRing = 196608;  // bytes of the TMA ring: 4, 6 or 8 stages by tile width
+constexpr int kLnSmem = 1024 + kLnRing + 8 * kLnStageTile + kLnCtrlBytes;
+
+enum LnMode { kLnForward = 0, kLnGradX = 1, kLnGradW = 2 };
+
+struct LnGeom {
+  int groups;              // >= 1
+  const int32_t* offsets;  // [groups + 1], or null: one group of all rows
+  int rows;                // rows of x
+  int n;                   // output columns
+  int kc;                  // contraction length (forward, dX)
+  int bn;                  // columns per tile
+  int n_nt;                // column tiles
+  int m, n_mt, splits;     // dW: output rows, row tiles, K ranges per group
+  int stages, stage_bytes;
+  void* out;               // y, dx or dW (T), or dW's partial sums (float)
+  int64_t out_ld, out_gs;  // dW: group (and split) stride
+  int out_vec;             // rows of `out` are 16-byte aligned
+  const void* bias;        // [groups][n], or null
+  int64_t bias_gs;
+  const void* res;         // residual rows, or null
+  int64_t res_ld;
+  int res_vec;
+  uint16_t* deriv;         // codes of act' [rows][deriv_ld], or null
+  int64_t deriv_ld;        // a multiple of 8
+};
+
+// ---------------------------------------------------------------- activations
+
+__device__ __forceinline__ float ln_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float ln_rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// act(x) and, with D, its derivative. act(x)'s last product is kept from
+// joining a later sum (__fmul_rn), so that y is the same bits with and without
+// D.
+template <int ACT, bool D>
+__device__ __forceinline__ float ln_act(float x, float* d) {
+  if constexpr (ACT == 1) {
+    if (D) *d = x > 0.f ? 1.f : (x <= 0.f ? 0.f : x);
+    return x < 0.f ? 0.f : x;
+  } else if constexpr (ACT == 2) {
+    const float r = x < 0.f ? 0.f : x;
+    if (D) *d = 2.f * r;
+    return __fmul_rn(r, r);
+  } else if constexpr (ACT == 3) {
+    // s = 1 / (1 + 2^(-x log2 e)) by the hardware's base-2 exponential and
+    // reciprocal (about 2^-22 relative: far below a 16-bit result's rounding).
+    const float s = ln_rcp(1.f + ln_exp2(-1.4426950408889634f * x));
+    const float y = __fmul_rn(x, s);
+    if (D) *d = fmaf(y, 1.f - s, s);
+    return y;
+  } else if constexpr (ACT == 4) {
+    // x sigmoid(2 t), t = sqrt(2 / pi) (x + 0.044715 x^3); x^2 is capped where
+    // the sigmoid has long been 0 or 1, so that no infinity meets a zero.
+    const float u = fminf(x * x, 1e4f);
+    const float c0 = 1.5957691216057308f, c1 = 0.07135481282754853f;
+    const float z = x * fmaf(c1, u, c0);
+    const float s = ln_rcp(1.f + ln_exp2(-1.4426950408889634f * z));
+    const float y = __fmul_rn(x, s);
+    if (D) *d = fmaf(y * (1.f - s), fmaf(3.f * c1, u, c0), s);
+    return y;
+  } else {
+    if (D) *d = 1.f;
+    return x;
+  }
+}
+
+// 16-bit codes of act' kept for the backward pass. relu, silu and gelu have
+// derivatives in (-2, 2): fixed point in steps of 2^-14, which adds an eighth
+// of an f16 rounding to dpre (the pre-activation in 16 bits would add one or
+// more of the operand type's own). relu2's (2 relu(x)) is unbounded and not
+// negative: the fp32 bit pattern in equal steps from a base, which spreads 2^16
+// codes over 128 binades for bf16 (2^-62 .. 2^65, half steps of 2^-10) and
+// over 24 for f16 (2^-15 .. 2^9, where the square leaves f16's range; half
+// steps of 2^-12.4); zero below. The codes 0x8000 and 0xFFFF stand for a
+// derivative that is not finite or out of range.
+template <typename T>
+struct LnFloatCode {
+  static constexpr uint32_t kBinades = std::is_same<T, __half>::value ? 24 : 128;
+  static constexpr uint32_t kStep = kBinades * 128;  // 2^23 bit patterns a binade / 2^16 codes
+  static constexpr uint32_t kBase = (std::is_same<T, __half>::value ? 112u : 65u) << 23;
+};
+template <typename T, int ACT>
+__device__ __forceinline__ uint32_t ln_encode(float d) {
+  if constexpr (ACT == 2) {
+    using C = LnFloatCode<T>;
+    if (!(d >= __uint_as_float(C::kBase + C::kStep))) return d >= 0.f ? 0u : 0xFFFFu;
+    const uint32_t c = (__float_as_uint(d) - C::kBase + C::kStep / 2) / C::kStep;
+    return c < 0xFFFFu ? c : 0xFFFFu;
+  } else {
+    const int i = __float2int_rn(d * 16384.f);
+    return d == d ? static_cast<uint32_t>(i) & 0xFFFFu : 0x8000u;
+  }
+}
+template <typename T, int ACT>
+__device__ __forceinline__ float ln_decode(uint32_t c) {
+  if constexpr (ACT == 2) {
+    using C = LnFloatCode<T>;
+    if (c == 0xFFFFu) return __int_as_float(0x7f800000);
+    return c ? __uint_as_float(c * C::kStep + C::kBase) : 0.f;
+  } else {
+    const float d = static_cast<float>(static_cast<int16_t>(c)) * 0x1p-14f;
+    return c == 0x8000u ? __int_as_float(0x7fc00000) : d;
+  }
+}
+
+// ---------------------------------------------------------------- 16-bit pairs
+template <typename T>
+__device__ __forceinline__ uint32_t ln_pack(float lo, float hi) {
+  if constexpr (std::is_same<T, __half>::value) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+template <typename T>
+__device__ __forceinline__ float2 ln_unpack(uint32_t w) {
+  if constexpr (std::is_same<T, __half>::value) {
+    return __half22float2(*reinterpret_cast<const __half2*>(&w));
+  } else {
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+  }
+}
+
+__device__ __forceinline__ void ln_sts(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+  asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+__device__ __forceinline__ uint4 ln_lds(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ void ln_cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void ln_cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void ln_cp_wait0() { asm volatile("cp.async.wait_group 0;" ::: "memory"); }
+
+// ---------------------------------------------------------------- groups
+
+// The rows [lo, hi) of group g + 1 given group g's end: offsets out of order
+// or out of range are pulled into [lo, rows], so no value of theirs leads out
+// of the tensors.
+__device__ __forceinline__ int ln_group_end(const LnGeom& q, int g, int lo) {
+  if (!q.offsets) return q.rows;
+  return min(max(__ldg(q.offsets + g + 1), lo), q.rows);
+}
+
+struct LnTile {
+  int g;           // group (== groups: rows past the last group, zeros)
+  int lo, hi;      // its rows
+  int mt, nt;      // row and column tile
+  int row0;        // forward, dX: first row
+  int split;       // dW
+  int k0, nk;      // dW: first row of the K range; all: K blocks
+  int last;        // dW: rows in the last K block (kLnBK: whole, or past the tensor's end)
+};
+
+// Walks the groups' tiles in order; t must not decrease.
+template <int MODE>
+struct LnWalker {
+  int g = -1, lo = 0, hi = 0, base = 0, cnt = 0;
+  __device__ __forceinline__ bool seek(const LnGeom& q, int t, LnTile& c) {
+    const int total = MODE == kLnGradW ? q.groups : q.groups + 1;
+    while (t >= base + cnt) {
+      if (g + 1 >= total) return false;
+      ++g;
+      base += cnt;
+      lo = hi;
+      hi = g < q.groups ? ln_group_end(q, g, lo) : q.rows;
+      cnt = MODE == kLnGradW ? q.n_mt * q.n_nt * q.splits : (hi - lo + kLnBM - 1) / kLnBM * q.n_nt;
+    }
+    int r = t - base;
+    c.g = g;
+    c.lo = lo;
+    c.hi = hi;
+    if (MODE == kLnGradW) {
+      c.split = r % q.splits;
+      r /= q.splits;
+      c.nt = r % q.n_nt;
+      c.mt = r / q.n_nt;
+      c.row0 = c.mt * kLnBM;
+      const int blocks = (hi - lo + kLnBK - 1) / kLnBK;
+      const int b0 = static_cast<int>(static_cast<int64_t>(blocks) * c.split / q.splits);
+      const int b1 = static_cast<int>(static_cast<int64_t>(blocks) * (c.split + 1) / q.splits);
+      c.k0 = lo + b0 * kLnBK;
+      c.nk = b1 - b0;
+      const int end = c.k0 + c.nk * kLnBK;
+      c.last = c.nk > 0 && end > hi && hi < q.rows ? hi - (end - kLnBK) : kLnBK;
+    } else {
+      c.nt = r % q.n_nt;
+      c.mt = r / q.n_nt;
+      c.row0 = lo + c.mt * kLnBM;
+      c.split = 0;
+      c.k0 = 0;
+      c.nk = g < q.groups ? (q.kc + kLnBK - 1) / kLnBK : 0;
+      c.last = kLnBK;
+    }
+    return true;
+  }
+};
+
+struct LnCtrl {
+  uint64_t full[kLnMaxStages], empty[kLnMaxStages];
+  uint64_t acc_full[2], acc_empty[2];
+  uint64_t partial;  // dW: a last K block with rows of the next group has landed
+  uint64_t cleared;  // dW: warp 2 has cleared them
+  uint32_t tmem_base;
+};
+static_assert(sizeof(LnCtrl) <= kLnCtrlBytes, "control block too large");
+
+// ---------------------------------------------------------------- epilogue
+
+// A staging tile holds 32 rows of 64 bytes; 16-byte piece q of row r sits at
+// piece q ^ (r / 2 mod 4), so rows (lane = row) and whole lines (4 lanes per
+// row) are both read and written without bank conflicts.
+__device__ __forceinline__ uint32_t ln_piece(uint32_t tile, int r, int q) {
+  return tile + r * 64 + ((q ^ ((r >> 1) & 3)) << 4);
+}
+__device__ __forceinline__ void ln_put_row(uint32_t tile, int lane, const uint32_t (&w)[16]) {
+#pragma unroll
+  for (int q = 0; q < 4; ++q) ln_sts(ln_piece(tile, lane, q), w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
+}
+
+// Store a staged 32 x 32 16-bit tile to rows row0.. (below row_end) and
+// columns col0.. (below n) of `out`.
+__device__ __forceinline__ void ln_store_tile(uint32_t tile, int lane, uint16_t* out, int64_t ld, int row0,
+                                              int row_end, int col0, int n, bool vec) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = i * 8 + (lane >> 2), q = lane & 3;
+    const uint4 v = ln_lds(ln_piece(tile, r, q));
+    const int row = row0 + r, col = col0 + q * 8;
+    if (row >= row_end || col >= n) continue;
+    uint16_t* p = out + static_cast<int64_t>(row) * ld + col;
+    if (vec && col + 8 <= n) {
+      *reinterpret_cast<uint4*>(p) = v;
+    } else {
+      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (col + j < n) p[j] = static_cast<uint16_t>(w[j >> 1] >> (16 * (j & 1)));
+    }
+  }
+}
+
+// Bring a 32 x 32 tile of 16-bit values into a staging tile (cp.async where
+// rows are 16-byte aligned; the caller commits and waits).
+__device__ __forceinline__ void ln_fetch_tile(uint32_t tile, int lane, const uint16_t* src, int64_t ld, int row0,
+                                              int row_end, int col0, int n, bool vec) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = i * 8 + (lane >> 2), q = lane & 3;
+    const int row = row0 + r, col = col0 + q * 8;
+    if (row >= row_end || col >= n) continue;
+    const uint16_t* p = src + static_cast<int64_t>(row) * ld + col;
+    if (vec && col + 8 <= n) {
+      ln_cp_async16(ln_piece(tile, r, q), p);
+    } else {
+      uint32_t w[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (col + j < n) w[j >> 1] |= static_cast<uint32_t>(p[j]) << (16 * (j & 1));
+      ln_sts(ln_piece(tile, r, q), w[0], w[1], w[2], w[3]);
+    }
+  }
+}
+
+// Drain this warp's 32 rows x (bn / 2) columns of one accumulator and release
+// it. FLAG: the forward pass writes act' as well, or dW writes partial sums.
+template <typename T, int MODE, int ACT, bool FLAG>
+__device__ __forceinline__ void ln_drain(const LnGeom& q, const LnTile& c, uint32_t tb, int wq, int h, int lane,
+                                         uint32_t stage, uint32_t acc_full, uint32_t parity, uint32_t acc_empty,
+                                         bool& alive) {
+  constexpr bool F32 = MODE == kLnGradW && FLAG;
+  constexpr bool DERIV = MODE == kLnForward && FLAG;
+  const int row0 = c.row0 + wq * 32;
+  const int row_end = MODE == kLnGradW ? q.m : c.hi;
+  const int half = q.bn >> 1;
+  const int col0 = c.nt * q.bn + h * half;
+  const int nch = row0 < row_end ? max(0, min(half, q.n - col0) + 31) / 32 : 0;
+  const bool zero = c.nk == 0;
+  const bool plain = MODE != kLnForward || c.g >= q.groups;  // no epilogue: the product (or zeros) itself
+  const bool res = MODE == kLnForward && !plain && q.res;
+  const uint16_t* rp = static_cast<const uint16_t*>(q.res);
+  if (res && nch > 0) {
+    ln_fetch_tile(stage, lane, rp, q.res_ld, row0, row_end, col0, q.n, q.res_vec);
+    ln_cp_commit();
+  }
+  if (!mbar_wait(acc_full, parity)) {
+    alive = false;
+    if (res) ln_cp_wait0();
+    return;
+  }
+  tc_fence_after();
+  const T* bias = MODE == kLnForward && !plain && q.bias
+                      ? static_cast<const T*>(q.bias) + static_cast<int64_t>(c.g) * q.bias_gs
+                      : nullptr;
+  uint16_t* out16 = static_cast<uint16_t*>(q.out);
+  float* out32 = static_cast<float*>(q.out);
+  if (MODE == kLnGradW) {
+    const int64_t slot = F32 ? static_cast<int64_t>(c.split) * q.groups + c.g : c.g;
+    out16 += slot * q.out_gs;
+    out32 += slot * q.out_gs;
+  }
+
+  auto emit = [&](int ch, const uint32_t (&o)[32]) {
+    const int n0 = col0 + ch * 32;
+    if constexpr (F32) {
+      // 32 x 32 floats: rows of 128 bytes, 16-byte piece q of row r at q ^ (r mod 8).
+#pragma unroll
+      for (int p = 0; p < 8; ++p)
+        ln_sts(stage + lane * 128 + ((p ^ (lane & 7)) << 4), o[4 * p], o[4 * p + 1], o[4 * p + 2], o[4 * p + 3]);
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int r = i * 4 + (lane >> 3), p = lane & 7;
+        const uint4 v = ln_lds(stage + r * 128 + ((p ^ (r & 7)) << 4));
+        const int row = row0 + r, col = n0 + p * 4;
+        if (row < row_end && col < q.n)  // rows are padded to whole 16 bytes
+          *reinterpret_cast<uint4*>(out32 + static_cast<int64_t>(row) * q.out_ld + col) = v;
+      }
+      __syncwarp();
+    } else {
+      const uint32_t tile = stage + (ch & 1) * 2048;
+      uint32_t pk[16];
+      if (plain) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) pk[i] = ln_pack<T>(__uint_as_float(o[2 * i]), __uint_as_float(o[2 * i + 1]));
+      } else {
+        uint32_t rw[16];
+        if (res) {
+          // This chunk's residual has landed; start the next one's.
+          ln_cp_wait0();
+          __syncwarp();
+          if (ch + 1 < nch) {
+            ln_fetch_tile(stage + ((ch + 1) & 1) * 2048, lane, rp, q.res_ld, row0, row_end, n0 + 32, q.n, q.res_vec);
+            ln_cp_commit();
+          }
+#pragma unroll
+          for (int p = 0; p < 4; ++p) {
+            const uint4 v = ln_lds(ln_piece(tile, lane, p));
+            rw[4 * p] = v.x;
+            rw[4 * p + 1] = v.y;
+            rw[4 * p + 2] = v.z;
+            rw[4 * p + 3] = v.w;
+          }
+        }
+        const bool bias_vec = bias && n0 + 32 <= q.n && (reinterpret_cast<uintptr_t>(bias + n0) & 15u) == 0;
+        uint32_t dk[16];
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          uint32_t bw[4] = {0u, 0u, 0u, 0u};
+          if (bias_vec) {
+            const uint4 v = __ldg(reinterpret_cast<const uint4*>(bias + n0) + b);
+            bw[0] = v.x;
+            bw[1] = v.y;
+            bw[2] = v.z;
+            bw[3] = v.w;
+          } else if (bias) {
+            const uint16_t* bp = reinterpret_cast<const uint16_t*>(bias) + n0 + 8 * b;
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              if (n0 + 8 * b + j < q.n) bw[j >> 1] |= static_cast<uint32_t>(bp[j]) << (16 * (j & 1));
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int i = 4 * b + j;
+            const float2 bb = ln_unpack<T>(bw[j]);
+            float d0, d1;
+            float y0 = ln_act<ACT, DERIV>(__uint_as_float(o[2 * i]) + bb.x, &d0);
+            float y1 = ln_act<ACT, DERIV>(__uint_as_float(o[2 * i + 1]) + bb.y, &d1);
+            if (DERIV) dk[i] = ln_encode<T, ACT>(d0) | (ln_encode<T, ACT>(d1) << 16);
+            if (res) {
+              const float2 rr = ln_unpack<T>(rw[i]);
+              y0 += rr.x;
+              y1 += rr.y;
+            }
+            pk[i] = ln_pack<T>(y0, y1);
+          }
+        }
+        if (DERIV) {
+          __syncwarp();
+          ln_put_row(tile, lane, dk);
+          __syncwarp();
+          ln_store_tile(tile, lane, q.deriv, q.deriv_ld, row0, row_end, n0, q.n, true);
+          __syncwarp();
+        }
+      }
+      ln_put_row(tile, lane, pk);
+      __syncwarp();
+      ln_store_tile(tile, lane, out16, q.out_ld, row0, row_end, n0, q.n, q.out_vec);
+      __syncwarp();
+    }
+  };
+
+  if (!zero) {
+    // TMEM loads run one chunk ahead of the stores.
+    uint32_t oa[32], ob[32];
+    if (nch > 0) tmem_ld32(tb, oa);
+#pragma unroll 1
+    for (int ch = 0; ch < nch; ch += 2) {
+      tmem_wait_ld(oa);
+      const bool more = ch + 1 < nch;
+      if (more) tmem_ld32(tb + (ch + 1) * 32, ob);
+      emit(ch, oa);
+      if (more) {
+        tmem_wait_ld(ob);
+        if (ch + 2 < nch) tmem_ld32(tb + (ch + 2) * 32, oa);
+        emit(ch + 1, ob);
+      }
+    }
+  } else {
+    uint32_t z[32];
+#pragma unroll
+    for (int i = 0; i < 32; ++i) z[i] = 0u;
+#pragma unroll 1
+    for (int ch = 0; ch < nch; ++ch) emit(ch, z);
+  }
+  tc_fence_before();
+  __syncwarp();
+  if (lane == 0) mbar_arrive(acc_empty);
+}
+
+// ---------------------------------------------------------------- kernel
+
+template <typename T, int MODE, int ACT, bool FLAG>
+__global__ void __launch_bounds__(kLnThreads, 1)
+    tc_linear(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const LnGeom q) {
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t base = (raw + 1023u) & ~1023u;
+  const uint32_t staging = base + kLnRing;
+  LnCtrl* ctrl = reinterpret_cast<LnCtrl*>(smem_raw + (base - raw) + kLnRing + 8 * kLnStageTile);
+  constexpr bool kAMn = MODE == kLnGradW, kBMn = MODE != kLnForward;
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) {
+    for (int s = 0; s < q.stages; ++s) {
+      mbar_init(smem_u32(&ctrl->full[s]), 1);
+      mbar_init(smem_u32(&ctrl->empty[s]), 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_u32(&ctrl->acc_full[i]), 1);
+      mbar_init(smem_u32(&ctrl->acc_empty[i]), 8);
+    }
+    mbar_init(smem_u32(&ctrl->partial), 1);
+    mbar_init(smem_u32(&ctrl->cleared), 1);
+    fence_mbar_init();
+    tma_prefetch_desc(&map_a);
+    tma_prefetch_desc(&map_b);
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(&ctrl->tmem_base), 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = ctrl->tmem_base;
+
+  if (warp == 0) {
+    // ============================================================ TMA producer
+    if (lane == 0) {
+      const uint64_t keep = l2_policy_evict_last();  // operands are read again by other tiles
+      LnWalker<MODE> w;
+      LnTile c;
+      int st = 0, fills = 0;
+      uint32_t ph = 0;
+      bool alive = true;
+      for (int t = blockIdx.x; alive && w.seek(q, t, c); t += gridDim.x) {
+        for (int kk = 0; kk < c.nk; ++kk) {
+          if (fills >= q.stages && !mbar_wait(smem_u32(&ctrl->empty[st]), ph ^ 1u)) {
+            alive = false;
+            break;
+          }
+          const uint32_t full = smem_u32(&ctrl->full[st]);
+          const uint32_t sa = base + st * q.stage_bytes, sb = sa + kLnABytes;
+          const int kx = c.k0 + kk * kLnBK;
+          mbar_arrive_expect_tx(full, q.stage_bytes);
+          if (!kAMn) {
+            tma_load_3d_hint(sa, &map_a, full, kx, c.row0, 0, keep);
+          } else {
+            tma_load_3d_hint(sa, &map_a, full, c.row0, kx, 0, keep);
+            tma_load_3d_hint(sa + kLnMnBox, &map_a, full, c.row0 + 64, kx, 0, keep);
+          }
+          if (!kBMn) {
+            tma_load_3d_hint(sb, &map_b, full, kx, c.nt * q.bn, c.g, keep);
+          } else {
+            const int bz = MODE == kLnGradX ? c.g : 0;
+            for (int i = 0; i < q.bn / 64; ++i)
+              tma_load_3d_hint(sb + i * kLnMnBox, &map_b, full, c.nt * q.bn + i * 64, kx, bz, keep);
+          }
+          ++fills;
+          if (++st == q.stages) {
+            st = 0;
+            ph ^= 1u;
+          }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ============================================================ MMA issuer
+    if (lane == 0) {
+      const uint32_t idesc = idesc_f16(std::is_same<T, __nv_bfloat16>::value ? 1u : 0u, kLnBM,
+                                       static_cast<uint32_t>(q.bn), kAMn ? 1u : 0u, kBMn ? 1u : 0u);
+      // K-major: 16 k (32 bytes) per MMA inside the 128-byte swizzled rows;
+      // MN-major: 16 k rows (2 KB) per MMA, 64-wide m / n groups 8 KB apart.
+      const uint64_t da0 = kAMn ? smem_desc_sw128(base, kLnMnBox, 1024) : smem_desc_sw128(base, 16, 1024);
+      const uint64_t db0 = kBMn ? smem_desc_sw128(base + kLnABytes, kLnMnBox, 1024)
+                                : smem_desc_sw128(base + kLnABytes, 16, 1024);
+      constexpr uint32_t ka = kAMn ? (2048u >> 4) : 2u, kb = kBMn ? (2048u >> 4) : 2u;
+      LnWalker<MODE> w;
+      LnTile c;
+      int st = 0, it = 0;
+      uint32_t ph = 0, cleared = 0;
+      bool alive = true;
+      for (int t = blockIdx.x; alive && w.seek(q, t, c); t += gridDim.x, ++it) {
+        const int buf = it & 1;
+        if (it >= 2) {
+          if (!mbar_wait(smem_u32(&ctrl->acc_empty[buf]), ((it >> 1) - 1) & 1)) break;
+          tc_fence_after();
+        }
+        const uint32_t d_tmem = tmem + static_cast<uint32_t>(buf * 256);
+        for (int kk = 0; kk < c.nk; ++kk) {
+          int steps = kLnBK / 16;
+          bool ok = mbar_wait(smem_u32(&ctrl->full[st]), ph);
+          if (MODE == kLnGradW && ok && kk == c.nk - 1 && c.last < kLnBK) {
+            mbar_arrive(smem_u32(&ctrl->partial));
+            ok = mbar_wait(smem_u32(&ctrl->cleared), cleared);
+            cleared ^= 1u;
+            steps = (c.last + 15) / 16;
+          }
+          if (!ok) {
+            alive = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t adv = static_cast<uint32_t>(st * q.stage_bytes) >> 4;
+          if (MODE != kLnGradW || steps == kLnBK / 16) {
+#pragma unroll
+            for (int k = 0; k < kLnBK / 16; ++k)
+              tc_mma_f16(d_tmem, da0 + adv + ka * k, db0 + adv + kb * k, idesc, (kk != 0 || k != 0) ? 1u : 0u);
+          } else {
+            for (int k = 0; k < steps; ++k)
+              tc_mma_f16(d_tmem, da0 + adv + ka * k, db0 + adv + kb * k, idesc, (kk != 0 || k != 0) ? 1u : 0u);
+          }
+          tc_commit(smem_u32(&ctrl->empty[st]));
+          if (++st == q.stages) {
+            st = 0;
+            ph ^= 1u;
+          }
+        }
+        if (!alive) break;
+        if (c.nk == 0)
+          mbar_arrive(smem_u32(&ctrl->acc_full[buf]));  // empty K range: the tile is zero
+        else
+          tc_commit(smem_u32(&ctrl->acc_full[buf]));
+      }
+    }
+  } else if (warp == 2) {
+    // ============================================================ dW: rows of the next group
+    // The last K block of a group may hold rows of the next one. They are
+    // cleared in both operands (not only one: theirs may be infinite), up to
+    // the next multiple of 16 rows, where the products of the block stop.
+    if (MODE == kLnGradW) {
+      LnWalker<MODE> w;
+      LnTile c;
+      int64_t filled = 0;  // K blocks of this CTA before the tile
+      uint32_t turn = 0;
+      for (int t = blockIdx.x; w.seek(q, t, c); t += gridDim.x) {
+        if (c.nk > 0 && c.last < kLnBK) {
+          const int64_t f = filled + c.nk - 1;
+          const int st = static_cast<int>(f % q.stages);
+          // The MMA warp has seen the block and waits: the stage holds it until then.
+          if (!mbar_wait(smem_u32(&ctrl->partial), turn)) break;
+          turn ^= 1u;
+          if (!mbar_wait(smem_u32(&ctrl->full[st]), static_cast<uint32_t>(f / q.stages) & 1u)) break;
+          const int r1 = (c.last + 15) / 16 * 16;
+          const int boxes = (kLnBM + q.bn) / 64;
+          const int pieces = (r1 - c.last) * 8;
+          const uint32_t s0 = base + st * q.stage_bytes + c.last * 128;
+          for (int i = lane; i < boxes * pieces; i += 32) {
+            const int b = i / pieces, p = i - b * pieces;
+            ln_sts(s0 + b * kLnMnBox + p * 16, 0u, 0u, 0u, 0u);
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&ctrl->cleared));
+        }
+        filled += c.nk;
+      }
+    }
+  } else if (warp >= 4) {
+    // ============================================================ epilogue
+    const int h = (warp - 4) >> 2;  // column half of the tile
+    const int wq = warp & 3;        // TMEM lane quarter
+    const uint32_t lane_off = static_cast<uint32_t>(wq * 32) << 16;
+    const uint32_t stage = staging + static_cast<uint32_t>((warp - 4) * kLnStageTile);
+    LnWalker<MODE> w;
+    LnTile c;
+    int it = 0;
+    bool alive = true;
+    for (int t = blockIdx.x; alive && w.seek(q, t, c); t += gridDim.x, ++it) {
+      const int buf = it & 1;
+      ln_drain<T, MODE, ACT, FLAG>(q, c, tmem + lane_off + static_cast<uint32_t>(buf * 256 + h * (q.bn >> 1)), wq, h,
+                                  lane, stage, smem_u32(&ctrl->acc_full[buf]), (it >> 1) & 1,
+                                  smem_u32(&ctrl->acc_empty[buf]), alive);
+    }
+  }
+
+  // ---------------------------------------------------------------- teardown
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+}  // namespace avey

@@ -5,6 +5,7 @@
 // there is one loaded library in a process. Bad arguments raise ValueError;
 // a non-OK AveyStatus is returned and raised by the Python side.
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/extension.h>
 
 #include <ATen/cuda/CUDAContext.h>
@@ -21,6 +22,10 @@ using at::Tensor;
 
 struct Library {
   int (*adamw)(const AveyAdamWParams*, void*) = nullptr;
+  int (*linear_fwd)(const AveyLinearParams*, void*) = nullptr;
+  int (*linear_bwd)(const AveyLinearParams*, void*) = nullptr;
+  int (*linear_workspace)(const AveyLinearParams*, int, uint64_t*) = nullptr;
+  const char* (*last_error)() = nullptr;
 };
 Library lib;
 
@@ -167,10 +172,191 @@ int adamw_step(const py::object& params, const py::object& grads, const py::obje
   return lib.adamw(&a, at::cuda::getCurrentCUDAStream().stream());
 }
 
+// ------------------------------------------------------------ linear layers
+
+void check_status(int status) { TORCH_CHECK(status == AVEY_OK, "status ", status, ": ", lib.last_error()); }
+
+// t as rows of `cols` values with unit stride (a copy only where no view has that form).
+Tensor as_rows(const Tensor& t, int64_t cols) {
+  Tensor r = t.dim() == 2 ? t : t.reshape({-1, cols});
+  if ((cols > 1 && r.stride(1) != 1) || (r.size(0) > 1 && r.stride(0) < cols)) r = r.contiguous();
+  return r;
+}
+// Row stride; a single row may claim any.
+int64_t row_ld(const Tensor& r, int64_t cols) { return r.size(0) > 1 ? r.stride(0) : (cols + 7) / 8 * 8; }
+
+// The weights [d_out, d_in] or [groups, d_out, d_in] with unit stride along d_in.
+Tensor as_weight(const Tensor& w) {
+  const int64_t n = w.size(-2), k = w.size(-1);
+  const bool ok = (k == 1 || w.stride(-1) == 1) && (n == 1 || w.stride(-2) >= k) &&
+                  (w.dim() == 2 || w.size(0) == 1 || w.stride(0) >= (n > 1 ? (n - 1) * w.stride(-2) : 0) + k);
+  return ok ? w : w.contiguous();
+}
+
+// The parameter block of x, weight and the groups.
+AveyLinearParams linear_params(const Tensor& x, const Tensor& w, const std::optional<Tensor>& offsets, int64_t act) {
+  AveyLinearParams p{};
+  p.struct_size = sizeof(p);
+  p.dtype = dtype_id(x);
+  p.activation = static_cast<int32_t>(act);
+  p.rows = x.size(0);
+  p.d_in = w.size(-1);
+  p.d_out = w.size(-2);
+  p.groups = offsets ? w.size(0) : 1;
+  if (offsets) p.offsets = static_cast<const int32_t*>(offsets->const_data_ptr());
+  p.x = x.const_data_ptr();
+  p.x_ld = row_ld(x, p.d_in);
+  p.weight = w.const_data_ptr();
+  p.weight_ld = p.d_out > 1 ? w.stride(-2) : (p.d_in + 7) / 8 * 8;
+  p.weight_group_stride = p.groups > 1 ? w.stride(0) : 0;
+  return p;
+}
+
+Tensor workspace(AveyLinearParams& p, int backward, const Tensor& like) {
+  uint64_t bytes = 0;
+  check_status(lib.linear_workspace(&p, backward, &bytes));
+  if (bytes == 0) return {};
+  Tensor ws = at::empty({static_cast<int64_t>(bytes)}, like.options().dtype(at::kByte));
+  p.workspace = ws.data_ptr();
+  p.workspace_bytes = bytes;
+  return ws;
+}
+
+// y and, with want_deriv, the codes of act'.
+std::pair<Tensor, Tensor> linear_forward(const Tensor& x, const Tensor& weight, const std::optional<Tensor>& bias,
+                                         const std::optional<Tensor>& residual, const std::optional<Tensor>& offsets,
+                                         int64_t act, int64_t kernel, bool want_deriv) {
+  const c10::cuda::CUDAGuard guard(x.device());
+  const Tensor w = as_weight(weight), xr = as_rows(x, weight.size(-1));
+  AveyLinearParams p = linear_params(xr, w, offsets, act);
+  p.kernel = static_cast<int32_t>(kernel);
+  Tensor b, r, deriv;
+  if (bias) {
+    b = bias->contiguous();
+    p.bias = b.const_data_ptr();
+    p.bias_group_stride = p.d_out;
+  }
+  if (residual) {
+    r = as_rows(*residual, p.d_out);
+    p.residual = r.const_data_ptr();
+    p.residual_ld = row_ld(r, p.d_out);
+  }
+  auto shape = x.sizes().vec();
+  shape.back() = p.d_out;
+  Tensor y = at::empty(shape, x.options());
+  p.y = y.data_ptr();
+  p.y_ld = p.d_out;
+  if (want_deriv && act != AVEY_ACT_IDENTITY && p.rows > 0) {
+    deriv = at::empty({p.rows, (p.d_out + 7) / 8 * 8}, x.options().dtype(at::kShort));
+    p.deriv = deriv.data_ptr();
+  }
+  const Tensor ws = workspace(p, 0, x);
+  check_status(lib.linear_fwd(&p, at::cuda::getCurrentCUDAStream().stream()));
+  return {y, deriv};
+}
+
+class LinearFunction : public torch::autograd::Function<LinearFunction> {
+ public:
+  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const Tensor& weight,
+                        const std::optional<Tensor>& bias, const std::optional<Tensor>& residual,
+                        const std::optional<Tensor>& offsets, int64_t act, int64_t kernel) {
+    const bool want = x.requires_grad() || weight.requires_grad() || (bias && bias->requires_grad());
+    auto [y, deriv] = linear_forward(x, weight, bias, residual, offsets, act, kernel, want);
+    ctx->save_for_backward({x, weight, offsets ? *offsets : Tensor(), deriv});
+    ctx->saved_data["act"] = act;
+    ctx->saved_data["bias"] = bias ? (bias->dim() == 2 ? 2 : 1) : 0;
+    ctx->saved_data["residual"] = residual.has_value();
+    return y;
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    TORCH_CHECK(!at::GradMode::is_enabled(),
+                "the gradients of the native linear layers cannot be differentiated again (create_graph)");
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &x = saved[0], &weight = saved[1], &offs = saved[2], &deriv = saved[3];
+    const int64_t has_bias = ctx->saved_data["bias"].toInt();
+    torch::autograd::variable_list out(7);
+    const Tensor& dy = grads[0];
+    if (!dy.defined()) return out;
+    // needs_input_grad counts the tensors that were given.
+    const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1),
+               need_b = has_bias && ctx->needs_input_grad(2);
+    if (ctx->saved_data["residual"].toBool() && ctx->needs_input_grad(has_bias ? 3 : 2)) out[3] = dy;
+    if (!need_x && !need_w && !need_b) return out;
+    const c10::cuda::CUDAGuard guard(x.device());
+    const Tensor w = as_weight(weight), xr = as_rows(x, weight.size(-1));
+    AveyLinearParams p =
+        linear_params(xr, w, offs.defined() ? std::optional<Tensor>(offs) : std::nullopt, ctx->saved_data["act"].toInt());
+    const Tensor g = as_rows(dy, p.d_out);
+    p.dy = g.const_data_ptr();
+    p.dy_ld = row_ld(g, p.d_out);
+    if (deriv.defined()) p.deriv = deriv.data_ptr();
+    if (need_x) {
+      out[0] = at::empty(x.sizes(), x.options());
+      p.dx = out[0].data_ptr();
+      p.dx_ld = p.d_in;
+    }
+    if (need_w) {
+      out[1] = at::empty(weight.sizes(), weight.options());
+      p.dweight = out[1].data_ptr();
+    }
+    if (need_b) {
+      out[2] = has_bias == 2 ? at::empty({p.groups, p.d_out}, x.options()) : at::empty({p.d_out}, x.options());
+      p.dbias = out[2].data_ptr();
+    }
+    const Tensor ws = workspace(p, 1, x);
+    check_status(lib.linear_bwd(&p, at::cuda::getCurrentCUDAStream().stream()));
+    return out;
+  }
+};
+
+Tensor linear(const Tensor& x, const Tensor& weight, const std::optional<Tensor>& bias,
+              const std::optional<Tensor>& residual, const std::optional<Tensor>& offsets, int64_t act,
+              int64_t kernel) {
+  const auto dt = x.scalar_type();
+  const auto device = x.device();
+  TORCH_CHECK_VALUE(device.is_cuda() && (dt == at::kBFloat16 || dt == at::kHalf),
+                    "the native linear layers take bf16 / f16 CUDA tensors of one dtype");
+  TORCH_CHECK_VALUE(x.dim() >= 1 && weight.dim() == (offsets ? 3 : 2) && weight.size(-1) == x.size(-1) &&
+                        weight.size(-1) > 0 && weight.size(-2) > 0,
+                    "x must be [..., d_in] and weight ", offsets ? "[experts, d_out, d_in]" : "[d_out, d_in]");
+  for (const std::optional<Tensor>& t : {std::optional<Tensor>(weight), bias, residual})
+    TORCH_CHECK_VALUE(!t || (t->scalar_type() == dt && t->device() == device),
+                      "the native linear layers take bf16 / f16 CUDA tensors of one dtype");
+  if (bias) {
+    auto want = weight.sizes().vec();
+    want.pop_back();
+    TORCH_CHECK_VALUE(bias->sizes() == at::IntArrayRef(want), "bias must have shape ", at::IntArrayRef(want));
+  }
+  if (residual) {
+    auto want = x.sizes().vec();
+    want.back() = weight.size(-2);
+    TORCH_CHECK_VALUE(residual->sizes() == at::IntArrayRef(want), "residual must have shape ", at::IntArrayRef(want));
+  }
+  if (offsets) {
+    TORCH_CHECK_VALUE(x.dim() == 2, "x must be [rows, d_in]");
+    TORCH_CHECK_VALUE(weight.size(0) > 0, "weight must hold at least one expert");
+    TORCH_CHECK_VALUE(offsets->dim() == 1 && offsets->size(0) == weight.size(0) + 1 &&
+                          offsets->scalar_type() == at::kInt && offsets->device() == device &&
+                          offsets->is_contiguous(),
+                      "offsets must be ", weight.size(0) + 1, " contiguous int32 values on x's device");
+  }
+  if (at::GradMode::is_enabled() &&
+      (x.requires_grad() || weight.requires_grad() || (bias && bias->requires_grad()) ||
+       (residual && residual->requires_grad())))
+    return LinearFunction::apply(x, weight, bias, residual, offsets, act, kernel);
+  return linear_forward(x, weight, bias, residual, offsets, act, kernel, false).first;
+}
+
 // Entry points of the loaded library, by name.
 void bind(const py::dict& addresses) {
   auto at = [&](const char* name) { return addresses[name].cast<uintptr_t>(); };
   lib.adamw = reinterpret_cast<decltype(lib.adamw)>(at("avey_adamw_v1"));
+  lib.linear_fwd = reinterpret_cast<decltype(lib.linear_fwd)>(at("avey_linear_fwd_v1"));
+  lib.linear_bwd = reinterpret_cast<decltype(lib.linear_bwd)>(at("avey_linear_bwd_v1"));
+  lib.linear_workspace = reinterpret_cast<decltype(lib.linear_workspace)>(at("avey_linear_workspace_size"));
+  lib.last_error = reinterpret_cast<decltype(lib.last_error)>(at("avey_last_error"));
 }
 
 }  // namespace
@@ -178,4 +364,5 @@ void bind(const py::dict& addresses) {
 PYBIND11_MODULE(_torch_binding, m) {
   m.def("bind", &bind);
   m.def("adamw_step", &adamw_step);
+  m.def("linear", &linear);
 }

@@ -25,6 +25,11 @@ CUDA inputs run natively (bf16 / f16, 16-byte aligned rows) and raise
 contextualizer's CPU path. Inputs that require grad take PyTorch's
 ``F.linear`` / ``matmul`` for these layers (with autograd) and the native
 contextualizer and its native backward.
+
+* ``residual_linear``: ``act(x W^T + b) + residual``, native in both
+  directions (``avey_linear_fwd_v1``, ``avey_linear_bwd_v1``): bf16 / f16
+  inputs of any width and alignment, with or without grad. Its form grouped by
+  expert is ``experts.expert_linear``.
 """
 
 from __future__ import annotations
@@ -34,7 +39,7 @@ from typing import Optional, Tuple
 import torch
 import torch.nn.functional as F
 
-from . import _native, gemm, ops
+from . import _binding, _native, gemm, ops
 
 _ACT_IDS = _native.ACTIVATION_IDS
 _DT = {torch.bfloat16: _native.AVEY_BF16, torch.float16: _native.AVEY_F16}
@@ -230,3 +235,28 @@ def static_mix(z: torch.Tensor, weight: torch.Tensor, *, bias: Optional[torch.Te
     za = z if z.stride(-1) == 1 else z.contiguous()
     return _epilogue_gemm(wa, za, out, bias=bias, gate=gate, activation=activation,
                           mode=gemm.K_LOWER if causal else gemm.DENSE)
+
+
+def residual_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, *,
+                    activation: str = 'identity', residual: Optional[torch.Tensor] = None
+                    ) -> torch.Tensor:
+    """Linear layer with its epilogue, ``act(x W^T + bias) + residual``: x
+    ``[..., d_in]``, weight ``[d_out, d_in]``, bias ``[d_out]``, residual
+    ``[..., d_out]``.
+
+    bf16 / f16 CUDA tensors of one dtype run natively, forward and backward
+    (fp32 sums; y and the gradients are rounded once, the gradient at the
+    product is rounded to the operand type before its two products). A few rows
+    (64 at most: single tokens of a batch) read the weights once on a kernel of
+    their own. Views with any row stride are read in place. CPU tensors take
+    plain PyTorch."""
+    _check_act(activation)
+    if not x.is_cuda:
+        y = _act_torch(F.linear(x, weight, bias), activation)
+        if residual is None:
+            return y
+        if residual.shape != y.shape:
+            raise ValueError(f'residual must have shape {list(y.shape)}')
+        return y + residual
+    return _binding.module().linear(x, weight, bias, residual, None, _ACT_IDS[activation],
+                                    _native.LINEAR_AUTO)

@@ -390,6 +390,78 @@ AVEY_API int avey_fwd_presummed_v1(const AveyFwdParams* params, const float* sum
                                    void* stream);
 
 /*
+ * Linear layers with a fused epilogue, dense or grouped by expert, and their
+ * gradients (no counterpart in the reference, which leaves the layers around
+ * the contextualizer to torch.matmul):
+ *
+ *   forward   y  = act(x W_g^T + b_g) + residual
+ *   backward  dpre = dy (.) act'(x W_g^T + b_g)
+ *             dx = dpre W_g, dweight_g = dpre_g^T x_g, dbias_g = sum of dpre_g
+ *             (the residual's gradient is dy itself)
+ *
+ * on x [rows][d_in], W [groups][d_out][d_in], b [groups][d_out]. With offsets
+ * (device, groups + 1 values) group g owns the rows [offsets[g], offsets[g +
+ * 1]); offsets[0] is taken as 0, values out of order or out of range are pulled
+ * into [the group's start, rows], and rows from offsets[groups] on belong to no
+ * group: their y and dx are zero and they add to no gradient. Without offsets
+ * (groups == 1) every row belongs to the one group. Group sizes are never read
+ * back to the host.
+ *
+ * dtype is AVEY_BF16 or AVEY_F16 for every array; products and sums are fp32
+ * and each result is rounded once; dpre is rounded to dtype before the two
+ * products of the backward pass. The forward pass writes act' as 16-bit codes
+ * into deriv when it is given (d_out rounded up to 8 values a row; any
+ * activation but the identity), and the backward pass reads them. Gradients
+ * use fixed orders: results are bitwise reproducible.
+ *
+ * Last dimensions have stride 1; row strides (ld) and group strides are in
+ * elements. Any alignment is taken: rows that are not whole 16-byte units
+ * are copied into the workspace first where the tensor cores read them.
+ */
+typedef struct AveyLinearParams {
+  uint32_t struct_size; /* sizeof(AveyLinearParams) */
+  int32_t dtype;        /* AVEY_BF16 or AVEY_F16 */
+  int32_t activation;   /* AveyActivation */
+  int32_t kernel;       /* AVEY_LINEAR_KERNEL_* (forward) */
+  int64_t rows, d_in, d_out, groups;
+  const int32_t* offsets;
+  const void* x;
+  int64_t x_ld;
+  const void* weight;
+  int64_t weight_ld, weight_group_stride;
+  const void* bias; /* or NULL */
+  int64_t bias_group_stride;
+  const void* residual; /* [rows][d_out], or NULL */
+  int64_t residual_ld;
+  void* y;
+  int64_t y_ld;
+  void* deriv; /* 16-byte aligned; forward: or NULL */
+
+  /* Backward (y, residual and bias are not read). NULL: not wanted. */
+  const void* dy; /* [rows][d_out] */
+  int64_t dy_ld;
+  void* dx; /* [rows][d_in] */
+  int64_t dx_ld;
+  void* dweight; /* contiguous [groups][d_out][d_in] */
+  void* dbias;   /* contiguous [groups][d_out] */
+
+  void* workspace; /* 256-byte aligned, >= avey_linear_workspace_size() bytes */
+  uint64_t workspace_bytes;
+} AveyLinearParams;
+
+/* AUTO: the kernel for few rows up to 64 of them, which reads the weights
+ * once without filling 128-row tiles; tcgen05 tiles above. */
+#define AVEY_LINEAR_KERNEL_AUTO 0
+#define AVEY_LINEAR_KERNEL_TCGEN05 1
+#define AVEY_LINEAR_KERNEL_FEW 2
+
+AVEY_API int avey_linear_fwd_v1(const AveyLinearParams* params, void* stream);
+AVEY_API int avey_linear_bwd_v1(const AveyLinearParams* params, void* stream);
+
+/* Bytes of `workspace` of the forward (backward == 0) or backward call. */
+AVEY_API int avey_linear_workspace_size(const AveyLinearParams* params, int backward, uint64_t* bytes);
+
+/*
  * One AdamW step over many tensors (no counterpart in the reference, which
  * leaves training to torch). For every element of every tensor, in fp32:
  *
