@@ -180,11 +180,13 @@ __global__ void __launch_bounds__(kLfThreads) ln_few(const LnFew q) {
       float z = 0.f;
 #pragma unroll
       for (int k = 0; k < 8; ++k) z += red[k][r][o];
-      float y = 0.f, d;
+      float y = 0.f;
       if (!zero) {
         if (q.bias) z += Elem<T>::to_f(reinterpret_cast<const T*>(q.bias)[static_cast<int64_t>(s.g) * q.bias_gs + col]);
-        y = ln_act<ACT, DERIV>(z, &d);
-        if (DERIV) q.deriv[static_cast<int64_t>(row) * q.deriv_ld + col] = static_cast<uint16_t>(ln_encode<T, ACT>(d));
+        LnPair d;
+        y = ln_split(ln_act2<ACT, DERIV>(ln_pair(z), &d)).x;
+        if (DERIV)
+          q.deriv[static_cast<int64_t>(row) * q.deriv_ld + col] = static_cast<uint16_t>(ln_encode2<T, ACT>(d));
         if (q.res) y += Elem<T>::to_f(reinterpret_cast<const T*>(q.res)[static_cast<int64_t>(row) * q.res_ld + col]);
       }
       reinterpret_cast<T*>(q.y)[static_cast<int64_t>(row) * q.y_ld + col] = Elem<T>::from_f(y);

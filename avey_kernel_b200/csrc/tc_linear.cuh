@@ -13,9 +13,16 @@
 // writing y once. Tiles are 128 rows x 256 columns (128 or 64 where 256 would
 // leave SMs without a tile), K in blocks of 64 through a TMA ring (128-byte
 // swizzle). Persistent CTAs, one per SM: warp 0 issues TMA, warp 1 issues
-// tcgen05.mma into one of two TMEM accumulators, warps 4-11 drain the other one,
+// tcgen05.mma into one of two TMEM accumulators, warps 4-19 drain the other one,
 // so a tile's epilogue overlaps the next tile's products; warp 2 clears the
 // rows of a neighbouring group out of dW's last K block. Every wait is bounded.
+//
+// The epilogue has as long as the products take: at d_in = 768 3072 cycles for
+// 32768 elements, 12 issue slots each. silu and gelu take two special-function
+// results each (4096 cycles a tile), so they are computed on packed pairs
+// (fma.rn.f32x2) with the code of act' by a magic-number sum, and sixteen warps
+// cover one another's latencies: with eight warps and scalar sums the forward
+// pass of 32768 x 768 x 1536 with silu, residual and codes took 185 us.
 #pragma once
 
 #include <cuda.h>
@@ -27,15 +34,16 @@
 
 namespace avey {
 
-constexpr int kLnThreads = 384;
+constexpr int kLnEpiWarps = 16;
+constexpr int kLnThreads = 128 + 32 * kLnEpiWarps;
 constexpr int kLnBM = 128, kLnBK = 64;
 constexpr int kLnABytes = kLnBM * kLnBK * 2;  // 16 KB
 constexpr int kLnMnBox = 64 * kLnBK * 2;      // one {64 (m or n), 64 (k)} box: 8 KB
-constexpr int kLnStageTile = 4096;            // an epilogue warp's staging: two 32 x 32 16-bit tiles
+constexpr int kLnStageTile = 2048;            // an epilogue warp's staging: 32 x 32 16-bit (or 32 x 16 32-bit) values
 constexpr int kLnMaxStages = 8;
 constexpr int kLnCtrlBytes = 512;
 constexpr int kLnRing = 196608;  // bytes of the TMA ring: 4, 6 or 8 stages by tile width
-constexpr int kLnSmem = 1024 + kLnRing + 8 * kLnStageTile + kLnCtrlBytes;
+constexpr int kLnSmem = 1024 + kLnRing + kLnEpiWarps * kLnStageTile + kLnCtrlBytes;
 
 enum LnMode { kLnForward = 0, kLnGradX = 1, kLnGradW = 2 };
 
@@ -74,66 +82,111 @@ __device__ __forceinline__ float ln_rcp(float x) {
   return y;
 }
 
-// act(x) and, with D, its derivative. act(x)'s last product is kept from
-// joining a later sum (__fmul_rn), so that y is the same bits with and without
-// D.
+// Two fp32 values in one 64-bit register: every sum and product is rounded by
+// itself, as the scalar ones are.
+typedef unsigned long long LnPair;
+__device__ __forceinline__ LnPair ln_pair(float lo, float hi) {
+  LnPair r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ LnPair ln_pair(float x) { return ln_pair(x, x); }
+__device__ __forceinline__ float2 ln_split(LnPair p) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(p));
+  return r;
+}
+__device__ __forceinline__ LnPair ln_add2(LnPair a, LnPair b) {
+  LnPair r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ LnPair ln_mul2(LnPair a, LnPair b) {
+  LnPair r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ LnPair ln_fma2(LnPair a, LnPair b, LnPair c) {
+  LnPair r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+// 1 / (1 + 2^t) of both, by the hardware's base-2 exponential and reciprocal
+// (about 2^-22 relative: far below a 16-bit result's rounding).
+__device__ __forceinline__ LnPair ln_sigmoid2(LnPair t) {
+  const float2 a = ln_split(t);
+  const float2 q = ln_split(ln_add2(ln_pair(ln_exp2(a.x), ln_exp2(a.y)), ln_pair(1.f)));
+  return ln_pair(ln_rcp(q.x), ln_rcp(q.y));
+}
+
+// act(x) of a pair and, with D, its derivative.
 template <int ACT, bool D>
-__device__ __forceinline__ float ln_act(float x, float* d) {
+__device__ __forceinline__ LnPair ln_act2(LnPair x, LnPair* d) {
+  constexpr float kLog2e = 1.4426950408889634f;
   if constexpr (ACT == 1) {
-    if (D) *d = x > 0.f ? 1.f : (x <= 0.f ? 0.f : x);
-    return x < 0.f ? 0.f : x;
+    const float2 v = ln_split(x);
+    if (D)
+      *d = ln_pair(v.x > 0.f ? 1.f : (v.x <= 0.f ? 0.f : v.x), v.y > 0.f ? 1.f : (v.y <= 0.f ? 0.f : v.y));
+    return ln_pair(v.x < 0.f ? 0.f : v.x, v.y < 0.f ? 0.f : v.y);
   } else if constexpr (ACT == 2) {
-    const float r = x < 0.f ? 0.f : x;
-    if (D) *d = 2.f * r;
-    return __fmul_rn(r, r);
+    const float2 v = ln_split(x);
+    const LnPair r = ln_pair(v.x < 0.f ? 0.f : v.x, v.y < 0.f ? 0.f : v.y);
+    if (D) *d = ln_add2(r, r);
+    return ln_mul2(r, r);
   } else if constexpr (ACT == 3) {
-    // s = 1 / (1 + 2^(-x log2 e)) by the hardware's base-2 exponential and
-    // reciprocal (about 2^-22 relative: far below a 16-bit result's rounding).
-    const float s = ln_rcp(1.f + ln_exp2(-1.4426950408889634f * x));
-    const float y = __fmul_rn(x, s);
-    if (D) *d = fmaf(y, 1.f - s, s);
+    const LnPair s = ln_sigmoid2(ln_mul2(x, ln_pair(-kLog2e)));
+    const LnPair y = ln_mul2(x, s);
+    if (D) *d = ln_fma2(y, ln_fma2(s, ln_pair(-1.f), ln_pair(1.f)), s);
     return y;
   } else if constexpr (ACT == 4) {
     // x sigmoid(2 t), t = sqrt(2 / pi) (x + 0.044715 x^3); x^2 is capped where
     // the sigmoid has long been 0 or 1, so that no infinity meets a zero.
-    const float u = fminf(x * x, 1e4f);
-    const float c0 = 1.5957691216057308f, c1 = 0.07135481282754853f;
-    const float z = x * fmaf(c1, u, c0);
-    const float s = ln_rcp(1.f + ln_exp2(-1.4426950408889634f * z));
-    const float y = __fmul_rn(x, s);
-    if (D) *d = fmaf(y * (1.f - s), fmaf(3.f * c1, u, c0), s);
+    constexpr float c0 = 1.5957691216057308f, c1 = 0.07135481282754853f;
+    const float2 q = ln_split(ln_mul2(x, x));
+    const LnPair u = ln_pair(fminf(q.x, 1e4f), fminf(q.y, 1e4f));
+    const LnPair s = ln_sigmoid2(ln_mul2(x, ln_fma2(u, ln_pair(-kLog2e * c1), ln_pair(-kLog2e * c0))));
+    const LnPair y = ln_mul2(x, s);
+    if (D)
+      *d = ln_fma2(ln_mul2(y, ln_fma2(s, ln_pair(-1.f), ln_pair(1.f))), ln_fma2(u, ln_pair(3.f * c1), ln_pair(c0)), s);
     return y;
   } else {
-    if (D) *d = 1.f;
+    if (D) *d = ln_pair(1.f);
     return x;
   }
 }
 
 // 16-bit codes of act' kept for the backward pass. relu, silu and gelu have
-// derivatives in (-2, 2): fixed point in steps of 2^-14, which adds an eighth
-// of an f16 rounding to dpre (the pre-activation in 16 bits would add one or
-// more of the operand type's own). relu2's (2 relu(x)) is unbounded and not
-// negative: the fp32 bit pattern in equal steps from a base, which spreads 2^16
-// codes over 128 binades for bf16 (2^-62 .. 2^65, half steps of 2^-10) and
+// derivatives in (-0.2, 1.2): fixed point in steps of 2^-14 from -1/4, which adds
+// an eighth of an f16 rounding to dpre (the pre-activation in 16 bits would add
+// one or more of the operand type's own). relu2's (2 relu(x)) is unbounded and
+// not negative: the fp32 bit pattern in equal steps from a base, which spreads
+// 2^16 codes over 128 binades for bf16 (2^-62 .. 2^65, half steps of 2^-10) and
 // over 24 for f16 (2^-15 .. 2^9, where the square leaves f16's range; half
-// steps of 2^-12.4); zero below. The codes 0x8000 and 0xFFFF stand for a
-// derivative that is not finite or out of range.
+// steps of 2^-12.4); zero below. The code 0xFFFF stands for a derivative that is
+// not finite or out of range (a NaN gives it by itself in the fixed-point form).
 template <typename T>
 struct LnFloatCode {
   static constexpr uint32_t kBinades = std::is_same<T, __half>::value ? 24 : 128;
   static constexpr uint32_t kStep = kBinades * 128;  // 2^23 bit patterns a binade / 2^16 codes
   static constexpr uint32_t kBase = (std::is_same<T, __half>::value ? 112u : 65u) << 23;
 };
+template <typename T>
+__device__ __forceinline__ uint32_t ln_float_code(float d) {
+  using C = LnFloatCode<T>;
+  if (!(d >= __uint_as_float(C::kBase + C::kStep))) return d >= 0.f ? 0u : 0xFFFFu;
+  const uint32_t c = (__float_as_uint(d) - C::kBase + C::kStep / 2) / C::kStep;
+  return c < 0xFFFFu ? c : 0xFFFFu;
+}
+// The codes of a pair, the first in the low half.
 template <typename T, int ACT>
-__device__ __forceinline__ uint32_t ln_encode(float d) {
+__device__ __forceinline__ uint32_t ln_encode2(LnPair d) {
   if constexpr (ACT == 2) {
-    using C = LnFloatCode<T>;
-    if (!(d >= __uint_as_float(C::kBase + C::kStep))) return d >= 0.f ? 0u : 0xFFFFu;
-    const uint32_t c = (__float_as_uint(d) - C::kBase + C::kStep / 2) / C::kStep;
-    return c < 0xFFFFu ? c : 0xFFFFu;
+    const float2 v = ln_split(d);
+    return ln_float_code<T>(v.x) | (ln_float_code<T>(v.y) << 16);
   } else {
-    const int i = __float2int_rn(d * 16384.f);
-    return d == d ? static_cast<uint32_t>(i) & 0xFFFFu : 0x8000u;
+    // 2^23 + 2^22 + 2^12 + 2^14 d: the code is in the low 16 bits.
+    const float2 v = ln_split(ln_fma2(d, ln_pair(0x1p14f), ln_pair(0x1.8p23f + 0x1p12f)));
+    return __byte_perm(__float_as_uint(v.x), __float_as_uint(v.y), 0x5410);
   }
 }
 template <typename T, int ACT>
@@ -143,8 +196,9 @@ __device__ __forceinline__ float ln_decode(uint32_t c) {
     if (c == 0xFFFFu) return __int_as_float(0x7f800000);
     return c ? __uint_as_float(c * C::kStep + C::kBase) : 0.f;
   } else {
-    const float d = static_cast<float>(static_cast<int16_t>(c)) * 0x1p-14f;
-    return c == 0x8000u ? __int_as_float(0x7fc00000) : d;
+    // (2^23 + c) 2^-14 - 2^9 - 1/4, exactly.
+    const float d = fmaf(__uint_as_float(0x4B000000u | c), 0x1p-14f, -512.25f);
+    return c == 0xFFFFu ? __int_as_float(0x7fc00000) : d;
   }
 }
 
@@ -176,11 +230,6 @@ __device__ __forceinline__ uint4 ln_lds(uint32_t a) {
   asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
   return v;
 }
-__device__ __forceinline__ void ln_cp_async16(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void ln_cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-__device__ __forceinline__ void ln_cp_wait0() { asm volatile("cp.async.wait_group 0;" ::: "memory"); }
 
 // ---------------------------------------------------------------- groups
 
@@ -257,85 +306,87 @@ static_assert(sizeof(LnCtrl) <= kLnCtrlBytes, "control block too large");
 
 // ---------------------------------------------------------------- epilogue
 
-// A staging tile holds 32 rows of 64 bytes; 16-byte piece q of row r sits at
-// piece q ^ (r / 2 mod 4), so rows (lane = row) and whole lines (4 lanes per
+// A staging tile holds 32 rows of 64 bytes; 16-byte piece p of row r sits at
+// piece p ^ (r / 2 mod 4), so rows (lane = row) and whole lines (4 lanes per
 // row) are both read and written without bank conflicts.
-__device__ __forceinline__ uint32_t ln_piece(uint32_t tile, int r, int q) {
-  return tile + r * 64 + ((q ^ ((r >> 1) & 3)) << 4);
-}
-__device__ __forceinline__ void ln_put_row(uint32_t tile, int lane, const uint32_t (&w)[16]) {
-#pragma unroll
-  for (int q = 0; q < 4; ++q) ln_sts(ln_piece(tile, lane, q), w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
+__device__ __forceinline__ uint32_t ln_piece(uint32_t tile, int r, int p) {
+  return tile + r * 64 + ((p ^ ((r >> 1) & 3)) << 4);
 }
 
-// Store a staged 32 x 32 16-bit tile to rows row0.. (below row_end) and
-// columns col0.. (below n) of `out`.
-__device__ __forceinline__ void ln_store_tile(uint32_t tile, int lane, uint16_t* out, int64_t ld, int row0,
-                                              int row_end, int col0, int n, bool vec) {
+// Where a lane moves a tile's lines: rows row + 8 i, columns col..col + 7.
+struct LnLines {
+  int row, row_end, col, n;
+  __device__ __forceinline__ bool in(int i) const { return row + 8 * i < row_end; }
+};
+
+// Store a staged 32 x 32 16-bit tile to `out`.
+__device__ __forceinline__ void ln_store_tile(uint32_t tile, int lane, uint16_t* out, int64_t ld, const LnLines& l,
+                                              bool vec) {
+  if (l.col >= l.n) return;
+  uint16_t* p = out + static_cast<int64_t>(l.row) * ld + l.col;
+  if (vec && l.col + 8 <= l.n) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int r = i * 8 + (lane >> 2), q = lane & 3;
-    const uint4 v = ln_lds(ln_piece(tile, r, q));
-    const int row = row0 + r, col = col0 + q * 8;
-    if (row >= row_end || col >= n) continue;
-    uint16_t* p = out + static_cast<int64_t>(row) * ld + col;
-    if (vec && col + 8 <= n) {
-      *reinterpret_cast<uint4*>(p) = v;
-    } else {
+    for (int i = 0; i < 4; ++i) {
+      const uint4 v = ln_lds(ln_piece(tile, i * 8 + (lane >> 2), lane & 3));
+      if (l.in(i)) *reinterpret_cast<uint4*>(p + 8 * i * ld) = v;
+    }
+  } else {
+#pragma unroll 1
+    for (int i = 0; i < 4; ++i) {
+      const uint4 v = ln_lds(ln_piece(tile, i * 8 + (lane >> 2), lane & 3));
+      if (!l.in(i)) continue;
       const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        if (col + j < n) p[j] = static_cast<uint16_t>(w[j >> 1] >> (16 * (j & 1)));
+        if (l.col + j < l.n) p[8 * i * ld + j] = static_cast<uint16_t>(w[j >> 1] >> (16 * (j & 1)));
     }
   }
 }
 
-// Bring a 32 x 32 tile of 16-bit values into a staging tile (cp.async where
-// rows are 16-byte aligned; the caller commits and waits).
-__device__ __forceinline__ void ln_fetch_tile(uint32_t tile, int lane, const uint16_t* src, int64_t ld, int row0,
-                                              int row_end, int col0, int n, bool vec) {
+// This lane's pieces of a 32 x 32 tile of 16-bit values (outside: zeros).
+__device__ __forceinline__ void ln_load_tile(const uint16_t* src, int64_t ld, const LnLines& l, bool vec,
+                                             uint4 (&v)[4]) {
+  const uint16_t* p = src + static_cast<int64_t>(l.row) * ld + l.col;
+  if (vec && l.col + 8 <= l.n) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int r = i * 8 + (lane >> 2), q = lane & 3;
-    const int row = row0 + r, col = col0 + q * 8;
-    if (row >= row_end || col >= n) continue;
-    const uint16_t* p = src + static_cast<int64_t>(row) * ld + col;
-    if (vec && col + 8 <= n) {
-      ln_cp_async16(ln_piece(tile, r, q), p);
-    } else {
+    for (int i = 0; i < 4; ++i) {
+      v[i] = make_uint4(0u, 0u, 0u, 0u);
+      if (l.in(i)) v[i] = __ldg(reinterpret_cast<const uint4*>(p + 8 * i * ld));
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
       uint32_t w[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        if (col + j < n) w[j >> 1] |= static_cast<uint32_t>(p[j]) << (16 * (j & 1));
-      ln_sts(ln_piece(tile, r, q), w[0], w[1], w[2], w[3]);
+        if (l.in(i) && l.col + j < l.n) w[j >> 1] |= static_cast<uint32_t>(__ldg(p + 8 * i * ld + j)) << (16 * (j & 1));
+      v[i] = make_uint4(w[0], w[1], w[2], w[3]);
     }
   }
 }
 
-// Drain this warp's 32 rows x (bn / 2) columns of one accumulator and release
-// it. FLAG: the forward pass writes act' as well, or dW writes partial sums.
+// Drain this warp's 32 rows x max(32, bn / 4) columns of one accumulator and
+// release it. FLAG: the forward pass writes act' as well, or dW writes partial
+// sums.
 template <typename T, int MODE, int ACT, bool FLAG>
 __device__ __forceinline__ void ln_drain(const LnGeom& q, const LnTile& c, uint32_t tb, int wq, int h, int lane,
-                                         uint32_t stage, uint32_t acc_full, uint32_t parity, uint32_t acc_empty,
+                                         uint32_t tile, uint32_t acc_full, uint32_t parity, uint32_t acc_empty,
                                          bool& alive) {
   constexpr bool F32 = MODE == kLnGradW && FLAG;
   constexpr bool DERIV = MODE == kLnForward && FLAG;
   const int row0 = c.row0 + wq * 32;
   const int row_end = MODE == kLnGradW ? q.m : c.hi;
-  const int half = q.bn >> 1;
-  const int col0 = c.nt * q.bn + h * half;
-  const int nch = row0 < row_end ? max(0, min(half, q.n - col0) + 31) / 32 : 0;
+  const int part = max(32, q.bn >> 2);
+  const int col0 = c.nt * q.bn + h * part;
+  const int nch = row0 < row_end && h * part < q.bn ? max(0, min(part, q.n - col0) + 31) / 32 : 0;
   const bool zero = c.nk == 0;
   const bool plain = MODE != kLnForward || c.g >= q.groups;  // no epilogue: the product (or zeros) itself
   const bool res = MODE == kLnForward && !plain && q.res;
-  const uint16_t* rp = static_cast<const uint16_t*>(q.res);
-  if (res && nch > 0) {
-    ln_fetch_tile(stage, lane, rp, q.res_ld, row0, row_end, col0, q.n, q.res_vec);
-    ln_cp_commit();
-  }
+  LnLines l{row0 + (lane >> 2), row_end, col0 + (lane & 3) * 8, q.n};
+  uint4 rv[4];
+  if (res && nch > 0) ln_load_tile(static_cast<const uint16_t*>(q.res), q.res_ld, l, q.res_vec, rv);
   if (!mbar_wait(acc_full, parity)) {
     alive = false;
-    if (res) ln_cp_wait0();
     return;
   }
   tc_fence_after();
@@ -349,119 +400,119 @@ __device__ __forceinline__ void ln_drain(const LnGeom& q, const LnTile& c, uint3
     out16 += slot * q.out_gs;
     out32 += slot * q.out_gs;
   }
-
-  auto emit = [&](int ch, const uint32_t (&o)[32]) {
+#pragma unroll 1
+  for (int ch = 0; ch < nch; ++ch) {
     const int n0 = col0 + ch * 32;
+    uint32_t o[32];
+    if (!zero) {
+      tmem_ld32(tb + ch * 32, o);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) o[i] = 0u;
+    }
     if constexpr (F32) {
-      // 32 x 32 floats: rows of 128 bytes, 16-byte piece q of row r at q ^ (r mod 8).
+      if (!zero) tmem_wait_ld(o);
 #pragma unroll
-      for (int p = 0; p < 8; ++p)
-        ln_sts(stage + lane * 128 + ((p ^ (lane & 7)) << 4), o[4 * p], o[4 * p + 1], o[4 * p + 2], o[4 * p + 3]);
-      __syncwarp();
+      for (int hh = 0; hh < 2; ++hh) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int r = i * 4 + (lane >> 3), p = lane & 7;
-        const uint4 v = ln_lds(stage + r * 128 + ((p ^ (r & 7)) << 4));
-        const int row = row0 + r, col = n0 + p * 4;
-        if (row < row_end && col < q.n)  // rows are padded to whole 16 bytes
-          *reinterpret_cast<uint4*>(out32 + static_cast<int64_t>(row) * q.out_ld + col) = v;
+        for (int p = 0; p < 4; ++p)
+          ln_sts(ln_piece(tile, lane, p), o[16 * hh + 4 * p], o[16 * hh + 4 * p + 1], o[16 * hh + 4 * p + 2],
+                 o[16 * hh + 4 * p + 3]);
+        __syncwarp();
+        const int col = n0 + 16 * hh + (lane & 3) * 4;  // rows are padded to whole 16 bytes
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint4 v = ln_lds(ln_piece(tile, i * 8 + (lane >> 2), lane & 3));
+          if (l.in(i) && col < q.n)
+            *reinterpret_cast<uint4*>(out32 + static_cast<int64_t>(l.row + 8 * i) * q.out_ld + col) = v;
+        }
+        __syncwarp();
       }
+      continue;
+    }
+    if (plain) {
+      if (!zero) tmem_wait_ld(o);
+#pragma unroll
+      for (int p = 0; p < 4; ++p) {
+        uint32_t y[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          y[j] = ln_pack<T>(__uint_as_float(o[8 * p + 2 * j]), __uint_as_float(o[8 * p + 2 * j + 1]));
+        ln_sts(ln_piece(tile, lane, p), y[0], y[1], y[2], y[3]);
+      }
+      __syncwarp();
+      ln_store_tile(tile, lane, out16, q.out_ld, l, q.out_vec);
       __syncwarp();
     } else {
-      const uint32_t tile = stage + (ch & 1) * 2048;
-      uint32_t pk[16];
-      if (plain) {
+      if (res) {
+        // The residual's lines go through the staging tile to the lanes of their
+        // rows; the next chunk's are loaded meanwhile.
 #pragma unroll
-        for (int i = 0; i < 16; ++i) pk[i] = ln_pack<T>(__uint_as_float(o[2 * i]), __uint_as_float(o[2 * i + 1]));
-      } else {
-        uint32_t rw[16];
+        for (int i = 0; i < 4; ++i)
+          ln_sts(ln_piece(tile, i * 8 + (lane >> 2), lane & 3), rv[i].x, rv[i].y, rv[i].z, rv[i].w);
+        __syncwarp();
+        if (ch + 1 < nch) {
+          LnLines next = l;
+          next.col += 32;
+          ln_load_tile(static_cast<const uint16_t*>(q.res), q.res_ld, next, q.res_vec, rv);
+        }
+      }
+      const bool bias_vec = bias && n0 + 32 <= q.n && (reinterpret_cast<uintptr_t>(bias + n0) & 15u) == 0;
+      uint32_t dk[16];
+      if (!zero) tmem_wait_ld(o);
+#pragma unroll
+      for (int p = 0; p < 4; ++p) {
+        uint32_t bw[4] = {0u, 0u, 0u, 0u};
+        if (bias_vec) {
+          const uint4 v = __ldg(reinterpret_cast<const uint4*>(bias + n0) + p);
+          bw[0] = v.x;
+          bw[1] = v.y;
+          bw[2] = v.z;
+          bw[3] = v.w;
+        } else if (bias) {
+          const uint16_t* bp = reinterpret_cast<const uint16_t*>(bias) + n0 + 8 * p;
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (n0 + 8 * p + j < q.n) bw[j >> 1] |= static_cast<uint32_t>(__ldg(bp + j)) << (16 * (j & 1));
+        }
+        uint32_t y[4], rw[4] = {0u, 0u, 0u, 0u};
         if (res) {
-          // This chunk's residual has landed; start the next one's.
-          ln_cp_wait0();
-          __syncwarp();
-          if (ch + 1 < nch) {
-            ln_fetch_tile(stage + ((ch + 1) & 1) * 2048, lane, rp, q.res_ld, row0, row_end, n0 + 32, q.n, q.res_vec);
-            ln_cp_commit();
-          }
-#pragma unroll
-          for (int p = 0; p < 4; ++p) {
-            const uint4 v = ln_lds(ln_piece(tile, lane, p));
-            rw[4 * p] = v.x;
-            rw[4 * p + 1] = v.y;
-            rw[4 * p + 2] = v.z;
-            rw[4 * p + 3] = v.w;
-          }
+          const uint4 v = ln_lds(ln_piece(tile, lane, p));
+          rw[0] = v.x;
+          rw[1] = v.y;
+          rw[2] = v.z;
+          rw[3] = v.w;
         }
-        const bool bias_vec = bias && n0 + 32 <= q.n && (reinterpret_cast<uintptr_t>(bias + n0) & 15u) == 0;
-        uint32_t dk[16];
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          uint32_t bw[4] = {0u, 0u, 0u, 0u};
-          if (bias_vec) {
-            const uint4 v = __ldg(reinterpret_cast<const uint4*>(bias + n0) + b);
-            bw[0] = v.x;
-            bw[1] = v.y;
-            bw[2] = v.z;
-            bw[3] = v.w;
-          } else if (bias) {
-            const uint16_t* bp = reinterpret_cast<const uint16_t*>(bias) + n0 + 8 * b;
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-              if (n0 + 8 * b + j < q.n) bw[j >> 1] |= static_cast<uint32_t>(bp[j]) << (16 * (j & 1));
+        for (int j = 0; j < 4; ++j) {
+          const int i = 8 * p + 2 * j;
+          const float2 bb = ln_unpack<T>(bw[j]);
+          LnPair d;
+          LnPair v = ln_act2<ACT, DERIV>(
+              ln_add2(ln_pair(__uint_as_float(o[i]), __uint_as_float(o[i + 1])), ln_pair(bb.x, bb.y)), &d);
+          if (DERIV) dk[4 * p + j] = ln_encode2<T, ACT>(d);
+          if (res) {
+            const float2 rr = ln_unpack<T>(rw[j]);
+            v = ln_add2(v, ln_pair(rr.x, rr.y));
           }
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int i = 4 * b + j;
-            const float2 bb = ln_unpack<T>(bw[j]);
-            float d0, d1;
-            float y0 = ln_act<ACT, DERIV>(__uint_as_float(o[2 * i]) + bb.x, &d0);
-            float y1 = ln_act<ACT, DERIV>(__uint_as_float(o[2 * i + 1]) + bb.y, &d1);
-            if (DERIV) dk[i] = ln_encode<T, ACT>(d0) | (ln_encode<T, ACT>(d1) << 16);
-            if (res) {
-              const float2 rr = ln_unpack<T>(rw[i]);
-              y0 += rr.x;
-              y1 += rr.y;
-            }
-            pk[i] = ln_pack<T>(y0, y1);
-          }
+          const float2 z = ln_split(v);
+          y[j] = ln_pack<T>(z.x, z.y);
         }
-        if (DERIV) {
-          __syncwarp();
-          ln_put_row(tile, lane, dk);
-          __syncwarp();
-          ln_store_tile(tile, lane, q.deriv, q.deriv_ld, row0, row_end, n0, q.n, true);
-          __syncwarp();
-        }
+        ln_sts(ln_piece(tile, lane, p), y[0], y[1], y[2], y[3]);
       }
-      ln_put_row(tile, lane, pk);
       __syncwarp();
-      ln_store_tile(tile, lane, out16, q.out_ld, row0, row_end, n0, q.n, q.out_vec);
+      ln_store_tile(tile, lane, out16, q.out_ld, l, q.out_vec);
       __syncwarp();
-    }
-  };
-
-  if (!zero) {
-    // TMEM loads run one chunk ahead of the stores.
-    uint32_t oa[32], ob[32];
-    if (nch > 0) tmem_ld32(tb, oa);
-#pragma unroll 1
-    for (int ch = 0; ch < nch; ch += 2) {
-      tmem_wait_ld(oa);
-      const bool more = ch + 1 < nch;
-      if (more) tmem_ld32(tb + (ch + 1) * 32, ob);
-      emit(ch, oa);
-      if (more) {
-        tmem_wait_ld(ob);
-        if (ch + 2 < nch) tmem_ld32(tb + (ch + 2) * 32, oa);
-        emit(ch + 1, ob);
+      if (DERIV) {
+#pragma unroll
+        for (int p = 0; p < 4; ++p)
+          ln_sts(ln_piece(tile, lane, p), dk[4 * p], dk[4 * p + 1], dk[4 * p + 2], dk[4 * p + 3]);
+        __syncwarp();
+        ln_store_tile(tile, lane, q.deriv, q.deriv_ld, l, true);
+        __syncwarp();
       }
     }
-  } else {
-    uint32_t z[32];
-#pragma unroll
-    for (int i = 0; i < 32; ++i) z[i] = 0u;
-#pragma unroll 1
-    for (int ch = 0; ch < nch; ++ch) emit(ch, z);
+    l.col += 32;
   }
   tc_fence_before();
   __syncwarp();
@@ -477,7 +528,7 @@ __global__ void __launch_bounds__(kLnThreads, 1)
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
   const uint32_t staging = base + kLnRing;
-  LnCtrl* ctrl = reinterpret_cast<LnCtrl*>(smem_raw + (base - raw) + kLnRing + 8 * kLnStageTile);
+  LnCtrl* ctrl = reinterpret_cast<LnCtrl*>(smem_raw + (base - raw) + kLnRing + kLnEpiWarps * kLnStageTile);
   constexpr bool kAMn = MODE == kLnGradW, kBMn = MODE != kLnForward;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -488,7 +539,7 @@ __global__ void __launch_bounds__(kLnThreads, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(smem_u32(&ctrl->acc_full[i]), 1);
-      mbar_init(smem_u32(&ctrl->acc_empty[i]), 8);
+      mbar_init(smem_u32(&ctrl->acc_empty[i]), kLnEpiWarps);
     }
     mbar_init(smem_u32(&ctrl->partial), 1);
     mbar_init(smem_u32(&ctrl->cleared), 1);
@@ -639,7 +690,7 @@ __global__ void __launch_bounds__(kLnThreads, 1)
     }
   } else if (warp >= 4) {
     // ============================================================ epilogue
-    const int h = (warp - 4) >> 2;  // column half of the tile
+    const int h = (warp - 4) >> 2;  // column part of the tile
     const int wq = warp & 3;        // TMEM lane quarter
     const uint32_t lane_off = static_cast<uint32_t>(wq * 32) << 16;
     const uint32_t stage = staging + static_cast<uint32_t>((warp - 4) * kLnStageTile);
@@ -649,8 +700,8 @@ __global__ void __launch_bounds__(kLnThreads, 1)
     bool alive = true;
     for (int t = blockIdx.x; alive && w.seek(q, t, c); t += gridDim.x, ++it) {
       const int buf = it & 1;
-      ln_drain<T, MODE, ACT, FLAG>(q, c, tmem + lane_off + static_cast<uint32_t>(buf * 256 + h * (q.bn >> 1)), wq, h,
-                                  lane, stage, smem_u32(&ctrl->acc_full[buf]), (it >> 1) & 1,
+      ln_drain<T, MODE, ACT, FLAG>(q, c, tmem + lane_off + static_cast<uint32_t>(buf * 256 + h * max(32, q.bn >> 2)),
+                                   wq, h, lane, stage, smem_u32(&ctrl->acc_full[buf]), (it >> 1) & 1,
                                   smem_u32(&ctrl->acc_empty[buf]), alive);
     }
   }
