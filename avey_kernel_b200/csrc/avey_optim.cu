@@ -5,6 +5,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstring>
+#include <mutex>
 #include <type_traits>
 
 #include "avey_b200.h"
@@ -18,6 +19,21 @@ int fail(int code, const char* msg) { return avey_host::set_error(code, msg); }
 // Tensors per launch: 400 entries of 80 bytes fit the 32,764 bytes of kernel
 // parameters; calls of up to 48 tensors pass a table of that size instead.
 constexpr int kMany = 400, kFew = 48;
+
+constexpr int kMaxDevices = 64;
+
+// Opt kernel K into its shared memory, once per device; the outcome is kept.
+template <auto K>
+cudaError_t smem_opt_in(int bytes) {
+  static std::once_flag once[kMaxDevices];
+  static cudaError_t err[kMaxDevices];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return cudaErrorInvalidDevice;
+  std::call_once(once[dev], [dev, bytes] {
+    err[dev] = cudaFuncSetAttribute(K, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  });
+  return err[dev];
+}
 
 int validate(const AveyAdamWParams* p) {
   if (!p) return fail(AVEY_ERR_ARGUMENT, "params is NULL");
@@ -67,8 +83,17 @@ int launch(const AveyAdamWTensor* t, int count, int64_t* block0, const avey::AwS
     tab.chunks += (t[i].numel + avey::kAwChunk - 1) / avey::kAwChunk;
   }
   if (tab.chunks == 0) return AVEY_OK;
-  const int grid = static_cast<int>(std::min<int64_t>(tab.chunks, avey_host::multiprocessors() * 8ll));
-  avey::adamw_step<T, MASTER, Q8, N><<<grid, avey::kAwThreads, 0, stream>>>(tab, c);
+  const int64_t sms = avey_host::multiprocessors();
+  if constexpr (Q8) {
+    const int grid = static_cast<int>(std::min<int64_t>(tab.chunks, sms * avey::kAwCtas8));
+    constexpr int smem = avey::kAwStages * sizeof(avey::AwStage<T, MASTER>);
+    const cudaError_t attr = smem_opt_in<avey::adamw8_step<T, MASTER, N>>(smem);
+    if (attr != cudaSuccess) return fail(AVEY_ERR_CUDA, cudaGetErrorString(attr));
+    avey::adamw8_step<T, MASTER, N><<<grid, avey::kAwThreads, smem, stream>>>(tab, c);
+  } else {
+    const int grid = static_cast<int>(std::min<int64_t>(tab.chunks, sms * 8));
+    avey::adamw_step<T, MASTER, N><<<grid, avey::kAwThreads, 0, stream>>>(tab, c);
+  }
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return fail(AVEY_ERR_LAUNCH, cudaGetErrorString(e));
   avey_host::count_launches(1);
@@ -118,6 +143,16 @@ extern "C" int avey_adamw_v1(const AveyAdamWParams* p, void* stream) {
   c.step_size = static_cast<float>(p->lr / bc1);
   c.inv_bc2 = static_cast<float>(1.0 / std::sqrt(bc2));
   c.eps = static_cast<float>(p->eps);
+  auto twice = [](float x) { return make_float2(x, x); };
+  c.b1p = twice(c.b1);
+  c.c1p = twice(c.c1);
+  c.b2p = twice(c.b2);
+  c.c2p = twice(c.c2);
+  c.decayp = twice(c.decay);
+  c.minus_stepp = twice(-c.step_size);
+  c.inv_bc2p = twice(c.inv_bc2);
+  c.epsp = twice(c.eps);
+  c.minus_zerop = twice(-0.f);
   c.seed = static_cast<uint32_t>(p->seed);
   c.step = static_cast<uint32_t>(p->step);
   c.grad_scale = p->grad_scale;

@@ -90,6 +90,7 @@ def _check_cpu(p, g, m, v, w):
             raise ValueError('states must have the shape and strides of their parameter')
 
 
+@torch.no_grad()
 def _step_cpu(params, grads, exp_avgs, exp_avg_sqs, step, lr, beta1, beta2, eps, weight_decay,
               masters, avg_scales, sq_scales, seed, grad_scale):
     """The step in plain PyTorch (CPU tensors)."""
@@ -143,7 +144,6 @@ def _step_cpu(params, grads, exp_avgs, exp_avg_sqs, step, lr, beta1, beta2, eps,
         start += state_scales(p.numel()) * BLOCK
 
 
-@torch.no_grad()
 def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor],
                exp_avgs: Sequence[torch.Tensor], exp_avg_sqs: Sequence[torch.Tensor], *,
                step: int, lr: float, betas=(0.9, 0.999), eps: float = 1e-8,
