@@ -43,7 +43,8 @@ constexpr int kLnStageTile = 2048;            // an epilogue warp's staging: 32 
 constexpr int kLnMaxStages = 8;
 constexpr int kLnCtrlBytes = 512;
 constexpr int kLnRing = 196608;  // bytes of the TMA ring: 4, 6 or 8 stages by tile width
-constexpr int kLnSmem = 1024 + kLnRing + kLnEpiWarps * kLnStageTile + kLnCtrlBytes;
+constexpr int kLnBiasBytes = 64;  // an epilogue warp's 32 bias values
+constexpr int kLnSmem = 1024 + kLnRing + kLnEpiWarps * (kLnStageTile + kLnBiasBytes) + kLnCtrlBytes;
 
 enum LnMode { kLnForward = 0, kLnGradX = 1, kLnGradW = 2 };
 
@@ -82,8 +83,7 @@ __device__ __forceinline__ float ln_rcp(float x) {
   return y;
 }
 
-// Two fp32 values in one 64-bit register: every sum and product is rounded by
-// itself, as the scalar ones are.
+// Two fp32 values in one 64-bit register.
 typedef unsigned long long LnPair;
 __device__ __forceinline__ LnPair ln_pair(float lo, float hi) {
   LnPair r;
@@ -111,43 +111,45 @@ __device__ __forceinline__ LnPair ln_fma2(LnPair a, LnPair b, LnPair c) {
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
   return r;
 }
-// 1 / (1 + 2^t) of both, by the hardware's base-2 exponential and reciprocal
-// (about 2^-22 relative: far below a 16-bit result's rounding).
-__device__ __forceinline__ LnPair ln_sigmoid2(LnPair t) {
-  const float2 a = ln_split(t);
-  const float2 q = ln_split(ln_add2(ln_pair(ln_exp2(a.x), ln_exp2(a.y)), ln_pair(1.f)));
-  return ln_pair(ln_rcp(q.x), ln_rcp(q.y));
-}
+// 1 / (1 + 2^t) by the hardware's base-2 exponential and reciprocal (about
+// 2^-22 relative: far below a 16-bit result's rounding).
+__device__ __forceinline__ float ln_sigmoid(float t) { return ln_rcp(__fadd_rn(1.f, ln_exp2(t))); }
 
-// act(x) of a pair and, with D, its derivative.
+// act(x) of a pair and, with D, its derivative. Operations between values are
+// packed; those with a constant are scalar, where it is an immediate (a packed
+// one takes two moves each time: 24 against 15 instructions an element).
 template <int ACT, bool D>
 __device__ __forceinline__ LnPair ln_act2(LnPair x, LnPair* d) {
   constexpr float kLog2e = 1.4426950408889634f;
+  const float2 v = ln_split(x);
   if constexpr (ACT == 1) {
-    const float2 v = ln_split(x);
     if (D)
       *d = ln_pair(v.x > 0.f ? 1.f : (v.x <= 0.f ? 0.f : v.x), v.y > 0.f ? 1.f : (v.y <= 0.f ? 0.f : v.y));
     return ln_pair(v.x < 0.f ? 0.f : v.x, v.y < 0.f ? 0.f : v.y);
   } else if constexpr (ACT == 2) {
-    const float2 v = ln_split(x);
     const LnPair r = ln_pair(v.x < 0.f ? 0.f : v.x, v.y < 0.f ? 0.f : v.y);
     if (D) *d = ln_add2(r, r);
     return ln_mul2(r, r);
   } else if constexpr (ACT == 3) {
-    const LnPair s = ln_sigmoid2(ln_mul2(x, ln_pair(-kLog2e)));
+    const float s0 = ln_sigmoid(__fmul_rn(v.x, -kLog2e)), s1 = ln_sigmoid(__fmul_rn(v.y, -kLog2e));
+    const LnPair s = ln_pair(s0, s1);
     const LnPair y = ln_mul2(x, s);
-    if (D) *d = ln_fma2(y, ln_fma2(s, ln_pair(-1.f), ln_pair(1.f)), s);
+    if (D) *d = ln_fma2(y, ln_pair(__fsub_rn(1.f, s0), __fsub_rn(1.f, s1)), s);
     return y;
   } else if constexpr (ACT == 4) {
     // x sigmoid(2 t), t = sqrt(2 / pi) (x + 0.044715 x^3); x^2 is capped where
     // the sigmoid has long been 0 or 1, so that no infinity meets a zero.
     constexpr float c0 = 1.5957691216057308f, c1 = 0.07135481282754853f;
     const float2 q = ln_split(ln_mul2(x, x));
-    const LnPair u = ln_pair(fminf(q.x, 1e4f), fminf(q.y, 1e4f));
-    const LnPair s = ln_sigmoid2(ln_mul2(x, ln_fma2(u, ln_pair(-kLog2e * c1), ln_pair(-kLog2e * c0))));
+    const float u0 = fminf(q.x, 1e4f), u1 = fminf(q.y, 1e4f);
+    const float2 t = ln_split(
+        ln_mul2(x, ln_pair(fmaf(u0, -kLog2e * c1, -kLog2e * c0), fmaf(u1, -kLog2e * c1, -kLog2e * c0))));
+    const float s0 = ln_sigmoid(t.x), s1 = ln_sigmoid(t.y);
+    const LnPair s = ln_pair(s0, s1);
     const LnPair y = ln_mul2(x, s);
     if (D)
-      *d = ln_fma2(ln_mul2(y, ln_fma2(s, ln_pair(-1.f), ln_pair(1.f))), ln_fma2(u, ln_pair(3.f * c1), ln_pair(c0)), s);
+      *d = ln_fma2(ln_mul2(y, ln_pair(__fsub_rn(1.f, s0), __fsub_rn(1.f, s1))),
+                   ln_pair(fmaf(u0, 3.f * c1, c0), fmaf(u1, 3.f * c1, c0)), s);
     return y;
   } else {
     if (D) *d = ln_pair(1.f);
@@ -185,8 +187,9 @@ __device__ __forceinline__ uint32_t ln_encode2(LnPair d) {
     return ln_float_code<T>(v.x) | (ln_float_code<T>(v.y) << 16);
   } else {
     // 2^23 + 2^22 + 2^12 + 2^14 d: the code is in the low 16 bits.
-    const float2 v = ln_split(ln_fma2(d, ln_pair(0x1p14f), ln_pair(0x1.8p23f + 0x1p12f)));
-    return __byte_perm(__float_as_uint(v.x), __float_as_uint(v.y), 0x5410);
+    const float2 v = ln_split(d);
+    return __byte_perm(__float_as_uint(fmaf(v.x, 0x1p14f, 0x1.8p23f + 0x1p12f)),
+                       __float_as_uint(fmaf(v.y, 0x1p14f, 0x1.8p23f + 0x1p12f)), 0x5410);
   }
 }
 template <typename T, int ACT>
@@ -343,6 +346,22 @@ __device__ __forceinline__ void ln_store_tile(uint32_t tile, int lane, uint16_t*
   }
 }
 
+// 16 columns of this lane's accumulator row (zeros for an empty K range).
+__device__ __forceinline__ void ln_tmem_ld16(uint32_t taddr, bool zero, uint32_t (&o)[16]) {
+  if (zero) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[i] = 0u;
+    return;
+  }
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(o[0]), "=r"(o[1]), "=r"(o[2]), "=r"(o[3]), "=r"(o[4]), "=r"(o[5]), "=r"(o[6]), "=r"(o[7]), "=r"(o[8]),
+        "=r"(o[9]), "=r"(o[10]), "=r"(o[11]), "=r"(o[12]), "=r"(o[13]), "=r"(o[14]), "=r"(o[15])
+      : "r"(taddr)
+      : "memory");
+}
+
 // This lane's pieces of a 32 x 32 tile of 16-bit values (outside: zeros).
 __device__ __forceinline__ void ln_load_tile(const uint16_t* src, int64_t ld, const LnLines& l, bool vec,
                                              uint4 (&v)[4]) {
@@ -365,34 +384,52 @@ __device__ __forceinline__ void ln_load_tile(const uint16_t* src, int64_t ld, co
   }
 }
 
+// What an epilogue warp reads ahead for a 32 x 32 chunk: its residual lines and
+// the lane's bias value.
+struct LnAhead {
+  uint4 res[4];
+  uint16_t bias;
+};
+
+// The columns of an epilogue warp in a tile, from its part h.
+__device__ __forceinline__ int ln_part(const LnGeom& q) { return max(32, q.bn >> 2); }
+
+template <int MODE>
+__device__ __forceinline__ void ln_read_ahead(const LnGeom& q, const LnTile& c, int wq, int h, int ch, int lane,
+                                              LnAhead& a) {
+  if (MODE != kLnForward || c.g >= q.groups) return;
+  const int col = c.nt * q.bn + h * ln_part(q) + ch * 32;
+  if (q.res) {
+    const LnLines l{c.row0 + wq * 32 + (lane >> 2), c.hi, col + (lane & 3) * 8, q.n};
+    ln_load_tile(static_cast<const uint16_t*>(q.res), q.res_ld, l, q.res_vec, a.res);
+  }
+  a.bias = 0;
+  if (q.bias && col + lane < q.n)
+    a.bias = __ldg(static_cast<const uint16_t*>(q.bias) + static_cast<int64_t>(c.g) * q.bias_gs + col + lane);
+}
+
 // Drain this warp's 32 rows x max(32, bn / 4) columns of one accumulator and
 // release it. FLAG: the forward pass writes act' as well, or dW writes partial
-// sums.
+// sums. `a` holds the first chunk's residual and bias, and on return those of
+// the next tile's (`next`, when there is one): the loads of a chunk are a whole
+// chunk ahead of their use, across tiles too.
 template <typename T, int MODE, int ACT, bool FLAG>
-__device__ __forceinline__ void ln_drain(const LnGeom& q, const LnTile& c, uint32_t tb, int wq, int h, int lane,
-                                         uint32_t tile, uint32_t acc_full, uint32_t parity, uint32_t acc_empty,
-                                         bool& alive) {
+__device__ __forceinline__ bool ln_drain(const LnGeom& q, const LnTile& c, const LnTile& next, bool has_next,
+                                         uint32_t tb, int wq, int h, int lane, uint32_t tile, uint32_t bias_tile,
+                                         uint32_t acc_full, uint32_t parity, uint32_t acc_empty, LnAhead& a) {
   constexpr bool F32 = MODE == kLnGradW && FLAG;
   constexpr bool DERIV = MODE == kLnForward && FLAG;
   const int row0 = c.row0 + wq * 32;
   const int row_end = MODE == kLnGradW ? q.m : c.hi;
-  const int part = max(32, q.bn >> 2);
+  const int part = ln_part(q);
   const int col0 = c.nt * q.bn + h * part;
   const int nch = row0 < row_end && h * part < q.bn ? max(0, min(part, q.n - col0) + 31) / 32 : 0;
   const bool zero = c.nk == 0;
   const bool plain = MODE != kLnForward || c.g >= q.groups;  // no epilogue: the product (or zeros) itself
   const bool res = MODE == kLnForward && !plain && q.res;
   LnLines l{row0 + (lane >> 2), row_end, col0 + (lane & 3) * 8, q.n};
-  uint4 rv[4];
-  if (res && nch > 0) ln_load_tile(static_cast<const uint16_t*>(q.res), q.res_ld, l, q.res_vec, rv);
-  if (!mbar_wait(acc_full, parity)) {
-    alive = false;
-    return;
-  }
+  if (!mbar_wait(acc_full, parity)) return false;
   tc_fence_after();
-  const T* bias = MODE == kLnForward && !plain && q.bias
-                      ? static_cast<const T*>(q.bias) + static_cast<int64_t>(c.g) * q.bias_gs
-                      : nullptr;
   uint16_t* out16 = static_cast<uint16_t*>(q.out);
   float* out32 = static_cast<float*>(q.out);
   if (MODE == kLnGradW) {
@@ -400,26 +437,18 @@ __device__ __forceinline__ void ln_drain(const LnGeom& q, const LnTile& c, uint3
     out16 += slot * q.out_gs;
     out32 += slot * q.out_gs;
   }
+  if (nch == 0 && has_next) ln_read_ahead<MODE>(q, next, wq, h, 0, lane, a);
 #pragma unroll 1
   for (int ch = 0; ch < nch; ++ch) {
-    const int n0 = col0 + ch * 32;
-    uint32_t o[32];
-    if (!zero) {
-      tmem_ld32(tb + ch * 32, o);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 32; ++i) o[i] = 0u;
-    }
     if constexpr (F32) {
-      if (!zero) tmem_wait_ld(o);
 #pragma unroll
       for (int hh = 0; hh < 2; ++hh) {
+        uint32_t o[16];
+        ln_tmem_ld16(tb + ch * 32 + 16 * hh, zero, o);
 #pragma unroll
-        for (int p = 0; p < 4; ++p)
-          ln_sts(ln_piece(tile, lane, p), o[16 * hh + 4 * p], o[16 * hh + 4 * p + 1], o[16 * hh + 4 * p + 2],
-                 o[16 * hh + 4 * p + 3]);
+        for (int p = 0; p < 4; ++p) ln_sts(ln_piece(tile, lane, p), o[4 * p], o[4 * p + 1], o[4 * p + 2], o[4 * p + 3]);
         __syncwarp();
-        const int col = n0 + 16 * hh + (lane & 3) * 4;  // rows are padded to whole 16 bytes
+        const int col = col0 + ch * 32 + 16 * hh + (lane & 3) * 4;  // rows are padded to whole 16 bytes
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const uint4 v = ln_lds(ln_piece(tile, i * 8 + (lane >> 2), lane & 3));
@@ -428,77 +457,65 @@ __device__ __forceinline__ void ln_drain(const LnGeom& q, const LnTile& c, uint3
         }
         __syncwarp();
       }
-      continue;
-    }
-    if (plain) {
-      if (!zero) tmem_wait_ld(o);
+    } else if (plain) {
 #pragma unroll
-      for (int p = 0; p < 4; ++p) {
-        uint32_t y[4];
+      for (int hh = 0; hh < 2; ++hh) {
+        uint32_t o[16];
+        ln_tmem_ld16(tb + ch * 32 + 16 * hh, zero, o);
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          y[j] = ln_pack<T>(__uint_as_float(o[8 * p + 2 * j]), __uint_as_float(o[8 * p + 2 * j + 1]));
-        ln_sts(ln_piece(tile, lane, p), y[0], y[1], y[2], y[3]);
+        for (int p = 0; p < 2; ++p) {
+          uint32_t y[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            y[j] = ln_pack<T>(__uint_as_float(o[8 * p + 2 * j]), __uint_as_float(o[8 * p + 2 * j + 1]));
+          ln_sts(ln_piece(tile, lane, 2 * hh + p), y[0], y[1], y[2], y[3]);
+        }
       }
       __syncwarp();
       ln_store_tile(tile, lane, out16, q.out_ld, l, q.out_vec);
       __syncwarp();
     } else {
+      // The residual's lines go through the staging tile to the lanes of their
+      // rows, the bias to all lanes; the next chunk's are loaded meanwhile.
       if (res) {
-        // The residual's lines go through the staging tile to the lanes of their
-        // rows; the next chunk's are loaded meanwhile.
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          ln_sts(ln_piece(tile, i * 8 + (lane >> 2), lane & 3), rv[i].x, rv[i].y, rv[i].z, rv[i].w);
-        __syncwarp();
-        if (ch + 1 < nch) {
-          LnLines next = l;
-          next.col += 32;
-          ln_load_tile(static_cast<const uint16_t*>(q.res), q.res_ld, next, q.res_vec, rv);
-        }
+          ln_sts(ln_piece(tile, i * 8 + (lane >> 2), lane & 3), a.res[i].x, a.res[i].y, a.res[i].z, a.res[i].w);
       }
-      const bool bias_vec = bias && n0 + 32 <= q.n && (reinterpret_cast<uintptr_t>(bias + n0) & 15u) == 0;
+      asm volatile("st.shared.b16 [%0], %1;" ::"r"(bias_tile + 2 * lane), "h"(a.bias) : "memory");
+      __syncwarp();
+      if (ch + 1 < nch) ln_read_ahead<MODE>(q, c, wq, h, ch + 1, lane, a);
+      else if (has_next) ln_read_ahead<MODE>(q, next, wq, h, 0, lane, a);
       uint32_t dk[16];
-      if (!zero) tmem_wait_ld(o);
 #pragma unroll
-      for (int p = 0; p < 4; ++p) {
-        uint32_t bw[4] = {0u, 0u, 0u, 0u};
-        if (bias_vec) {
-          const uint4 v = __ldg(reinterpret_cast<const uint4*>(bias + n0) + p);
-          bw[0] = v.x;
-          bw[1] = v.y;
-          bw[2] = v.z;
-          bw[3] = v.w;
-        } else if (bias) {
-          const uint16_t* bp = reinterpret_cast<const uint16_t*>(bias) + n0 + 8 * p;
+      for (int hh = 0; hh < 2; ++hh) {
+        uint32_t o[16];
+        ln_tmem_ld16(tb + ch * 32 + 16 * hh, zero, o);
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if (n0 + 8 * p + j < q.n) bw[j >> 1] |= static_cast<uint32_t>(__ldg(bp + j)) << (16 * (j & 1));
-        }
-        uint32_t y[4], rw[4] = {0u, 0u, 0u, 0u};
-        if (res) {
-          const uint4 v = ln_lds(ln_piece(tile, lane, p));
-          rw[0] = v.x;
-          rw[1] = v.y;
-          rw[2] = v.z;
-          rw[3] = v.w;
-        }
+        for (int pp = 0; pp < 2; ++pp) {
+          const int p = 2 * hh + pp;
+          const uint4 bw = ln_lds(bias_tile + 16 * p);
+          uint4 rw = make_uint4(0u, 0u, 0u, 0u);
+          if (res) rw = ln_lds(ln_piece(tile, lane, p));
+          const uint32_t b4[4] = {bw.x, bw.y, bw.z, bw.w}, r4[4] = {rw.x, rw.y, rw.z, rw.w};
+          uint32_t y[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int i = 8 * p + 2 * j;
-          const float2 bb = ln_unpack<T>(bw[j]);
-          LnPair d;
-          LnPair v = ln_act2<ACT, DERIV>(
-              ln_add2(ln_pair(__uint_as_float(o[i]), __uint_as_float(o[i + 1])), ln_pair(bb.x, bb.y)), &d);
-          if (DERIV) dk[4 * p + j] = ln_encode2<T, ACT>(d);
-          if (res) {
-            const float2 rr = ln_unpack<T>(rw[j]);
-            v = ln_add2(v, ln_pair(rr.x, rr.y));
+          for (int j = 0; j < 4; ++j) {
+            const int i = 8 * pp + 2 * j;
+            const float2 bb = ln_unpack<T>(b4[j]);
+            LnPair d;
+            LnPair v = ln_act2<ACT, DERIV>(
+                ln_add2(ln_pair(__uint_as_float(o[i]), __uint_as_float(o[i + 1])), ln_pair(bb.x, bb.y)), &d);
+            if (DERIV) dk[4 * p + j] = ln_encode2<T, ACT>(d);
+            if (res) {
+              const float2 rr = ln_unpack<T>(r4[j]);
+              v = ln_add2(v, ln_pair(rr.x, rr.y));
+            }
+            const float2 z = ln_split(v);
+            y[j] = ln_pack<T>(z.x, z.y);
           }
-          const float2 z = ln_split(v);
-          y[j] = ln_pack<T>(z.x, z.y);
+          ln_sts(ln_piece(tile, lane, p), y[0], y[1], y[2], y[3]);
         }
-        ln_sts(ln_piece(tile, lane, p), y[0], y[1], y[2], y[3]);
       }
       __syncwarp();
       ln_store_tile(tile, lane, out16, q.out_ld, l, q.out_vec);
@@ -517,6 +534,7 @@ __device__ __forceinline__ void ln_drain(const LnGeom& q, const LnTile& c, uint3
   tc_fence_before();
   __syncwarp();
   if (lane == 0) mbar_arrive(acc_empty);
+  return true;
 }
 
 // ---------------------------------------------------------------- kernel
@@ -528,7 +546,8 @@ __global__ void __launch_bounds__(kLnThreads, 1)
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
   const uint32_t staging = base + kLnRing;
-  LnCtrl* ctrl = reinterpret_cast<LnCtrl*>(smem_raw + (base - raw) + kLnRing + kLnEpiWarps * kLnStageTile);
+  LnCtrl* ctrl =
+      reinterpret_cast<LnCtrl*>(smem_raw + (base - raw) + kLnRing + kLnEpiWarps * (kLnStageTile + kLnBiasBytes));
   constexpr bool kAMn = MODE == kLnGradW, kBMn = MODE != kLnForward;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -694,15 +713,25 @@ __global__ void __launch_bounds__(kLnThreads, 1)
     const int wq = warp & 3;        // TMEM lane quarter
     const uint32_t lane_off = static_cast<uint32_t>(wq * 32) << 16;
     const uint32_t stage = staging + static_cast<uint32_t>((warp - 4) * kLnStageTile);
+    const uint32_t bias_tile = staging + kLnEpiWarps * kLnStageTile + static_cast<uint32_t>((warp - 4) * kLnBiasBytes);
     LnWalker<MODE> w;
-    LnTile c;
-    int it = 0;
-    bool alive = true;
-    for (int t = blockIdx.x; alive && w.seek(q, t, c); t += gridDim.x, ++it) {
+    LnTile c, next;
+    LnAhead ahead{};
+    int it = 0, t = blockIdx.x;
+    bool more = w.seek(q, t, c);
+    if (more) ln_read_ahead<MODE>(q, c, wq, h, 0, lane, ahead);
+    while (more) {
+      t += gridDim.x;
+      const bool has_next = w.seek(q, t, next);
       const int buf = it & 1;
-      ln_drain<T, MODE, ACT, FLAG>(q, c, tmem + lane_off + static_cast<uint32_t>(buf * 256 + h * max(32, q.bn >> 2)),
-                                   wq, h, lane, stage, smem_u32(&ctrl->acc_full[buf]), (it >> 1) & 1,
-                                  smem_u32(&ctrl->acc_empty[buf]), alive);
+      const uint32_t tb = tmem + lane_off + static_cast<uint32_t>(buf * 256 + h * ln_part(q));
+      if (!ln_drain<T, MODE, ACT, FLAG>(q, c, next, has_next, tb, wq, h, lane, stage, bias_tile,
+                                        smem_u32(&ctrl->acc_full[buf]), (it >> 1) & 1,
+                                        smem_u32(&ctrl->acc_empty[buf]), ahead))
+        break;
+      more = has_next;
+      c = next;
+      ++it;
     }
   }
 
