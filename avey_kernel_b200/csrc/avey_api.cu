@@ -959,20 +959,34 @@ int clear_error() { return ok(); }
 void count_launches(int n) { g_launches.fetch_add(static_cast<uint64_t>(n), std::memory_order_relaxed); }
 int device_ok() { return device_arch_ok(nullptr); }
 int multiprocessors() { return sm_count(); }
-int encode_rows16(int dtype, const void* base, uint64_t inner, uint64_t rows, uint64_t batch, uint64_t row_bytes,
-                  uint64_t batch_bytes, int box_rows, CUtensorMap* map) {
+namespace {
+int encode_plain(int dtype, const void* base, uint64_t inner, uint64_t rows, uint64_t batch, uint64_t row_bytes,
+                 uint64_t batch_bytes, uint32_t box_cols, uint32_t box_rows, CUtensorMapSwizzle swizzle,
+                 CUtensorMap* map) {
   auto fn = encode_fn();
   if (!fn) return fail(AVEY_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
   const cuuint64_t dims[3] = {inner, rows, batch};
   const cuuint64_t strides[2] = {row_bytes, batch > 1 ? batch_bytes : row_bytes * rows};
-  const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(box_rows), 1};
+  const cuuint32_t box[3] = {box_cols, box_rows, 1};
   const cuuint32_t estr[3] = {1, 1, 1};
-  const CUresult r = fn(map, dtype == AVEY_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
-                        3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  const CUtensorMapDataType dt = dtype == AVEY_BF16  ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                 : dtype == AVEY_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                                     : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  const CUresult r = fn(map, dt, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(AVEY_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
   return AVEY_OK;
+}
+}  // namespace
+int encode_rows16(int dtype, const void* base, uint64_t inner, uint64_t rows, uint64_t batch, uint64_t row_bytes,
+                  uint64_t batch_bytes, int box_rows, CUtensorMap* map) {
+  return encode_plain(dtype, base, inner, rows, batch, row_bytes, batch_bytes, 64, static_cast<uint32_t>(box_rows),
+                      CU_TENSOR_MAP_SWIZZLE_128B, map);
+}
+int encode_tiles(int dtype, void* base, uint64_t inner, uint64_t rows, uint64_t batch, uint64_t row_bytes,
+                 uint64_t batch_bytes, CUtensorMap* map) {
+  return encode_plain(dtype, base, inner, rows, batch, row_bytes, batch_bytes, dtype == AVEY_F32 ? 16 : 32, 32,
+                      CU_TENSOR_MAP_SWIZZLE_64B, map);
 }
 }  // namespace avey_host
 

@@ -204,12 +204,18 @@ avey::LnGeom geom(const AveyLinearParams* p, int64_t n, int bn) {
   return q;
 }
 
+// Maps of a launch: the operands and the outputs (y / dx / dW, and the codes of
+// act'), which are left unset where they are not used.
+struct Maps {
+  CUtensorMap a{}, b{}, y{}, d{};
+};
+
 template <auto K>
-int launch_tc(const CUtensorMap& a, const CUtensorMap& b, const avey::LnGeom& q, int64_t tiles, cudaStream_t stream) {
+int launch_tc(const Maps& m, const avey::LnGeom& q, int64_t tiles, cudaStream_t stream) {
   const cudaError_t e = smem_opt_in<K>();
   if (e != cudaSuccess) return fail(AVEY_ERR_CUDA, cudaGetErrorString(e));
   const int grid = static_cast<int>(std::min<int64_t>(tiles, avey_host::multiprocessors()));
-  K<<<grid, avey::kLnThreads, avey::kLnSmem, stream>>>(a, b, q);
+  K<<<grid, avey::kLnThreads, avey::kLnSmem, stream>>>(m.a, m.b, m.y, m.d, q);
   return launched("tc_linear");
 }
 
@@ -234,16 +240,20 @@ int forward_tc(const AveyLinearParams* p, cudaStream_t stream) {
   q.res_vec = p->residual && whole_rows(p->residual, p->residual_ld);
   q.deriv = static_cast<uint16_t*>(p->deriv);
   q.deriv_ld = up8(p->d_out);
-  CUtensorMap a, b;
-  rc = avey_host::encode_rows16(p->dtype, x.p, p->d_in, p->rows, 1, x.ld * 2, 0, avey::kLnBM, &a);
+  Maps m;
+  rc = avey_host::encode_rows16(p->dtype, x.p, p->d_in, p->rows, 1, x.ld * 2, 0, avey::kLnBM, &m.a);
   if (rc == AVEY_OK)
-    rc = avey_host::encode_rows16(p->dtype, w.p, p->d_in, p->d_out, p->groups, w.ld * 2, w.gs * 2, q.bn, &b);
+    rc = avey_host::encode_rows16(p->dtype, w.p, p->d_in, p->d_out, p->groups, w.ld * 2, w.gs * 2, q.bn, &m.b);
+  if (rc == AVEY_OK && q.out_vec)
+    rc = avey_host::encode_tiles(p->dtype, p->y, p->d_out, p->rows, 1, p->y_ld * 2, 0, &m.y);
+  if (rc == AVEY_OK && q.out_vec && p->deriv)
+    rc = avey_host::encode_tiles(p->dtype, p->deriv, p->d_out, p->rows, 1, q.deriv_ld * 2, 0, &m.d);
   if (rc != AVEY_OK) return rc;
   // One more row tile than the groups': the rows past the last group.
   const int64_t tiles = (mt + (p->offsets ? 1 : 0)) * q.n_nt;
   if constexpr (ACT != AVEY_ACT_IDENTITY)
-    if (p->deriv) return launch_tc<avey::tc_linear<T, avey::kLnForward, ACT, true>>(a, b, q, tiles, stream);
-  return launch_tc<avey::tc_linear<T, avey::kLnForward, ACT, false>>(a, b, q, tiles, stream);
+    if (p->deriv) return launch_tc<avey::tc_linear<T, avey::kLnForward, ACT, true>>(m, q, tiles, stream);
+  return launch_tc<avey::tc_linear<T, avey::kLnForward, ACT, false>>(m, q, tiles, stream);
 }
 
 template <typename T, int ACT, bool DERIV>
@@ -351,7 +361,6 @@ int backward(const AveyLinearParams* p, cudaStream_t stream) {
       if (rc != AVEY_OK) return rc;
     }
   }
-  CUtensorMap a, b;
   if (p->dx) {
     const int64_t mt = row_tiles(p, avey::kLnBM);
     avey::LnGeom q = geom(p, p->d_in, tile_cols(mt, p->d_in));
@@ -359,12 +368,15 @@ int backward(const AveyLinearParams* p, cudaStream_t stream) {
     q.out = p->dx;
     q.out_ld = p->dx_ld;
     q.out_vec = whole_rows(p->dx, p->dx_ld);
-    rc = avey_host::encode_rows16(p->dtype, g.p, p->d_out, p->rows, 1, g.ld * 2, 0, avey::kLnBM, &a);
+    Maps m;
+    rc = avey_host::encode_rows16(p->dtype, g.p, p->d_out, p->rows, 1, g.ld * 2, 0, avey::kLnBM, &m.a);
     if (rc == AVEY_OK)
-      rc = avey_host::encode_rows16(p->dtype, w.p, p->d_in, p->d_out, p->groups, w.ld * 2, w.gs * 2, 64, &b);
+      rc = avey_host::encode_rows16(p->dtype, w.p, p->d_in, p->d_out, p->groups, w.ld * 2, w.gs * 2, 64, &m.b);
+    if (rc == AVEY_OK && q.out_vec)
+      rc = avey_host::encode_tiles(p->dtype, p->dx, p->d_in, p->rows, 1, p->dx_ld * 2, 0, &m.y);
     if (rc != AVEY_OK) return rc;
     const int64_t tiles = (mt + (p->offsets ? 1 : 0)) * q.n_nt;
-    rc = launch_tc<avey::tc_linear<T, avey::kLnGradX, 0, false>>(a, b, q, tiles, stream);
+    rc = launch_tc<avey::tc_linear<T, avey::kLnGradX, 0, false>>(m, q, tiles, stream);
     if (rc != AVEY_OK) return rc;
   }
   if (p->dweight) {
@@ -377,12 +389,16 @@ int backward(const AveyLinearParams* p, cudaStream_t stream) {
     q.out_ld = parts ? (p->d_in + 3) / 4 * 4 : p->d_in;
     q.out_gs = p->d_out * q.out_ld;
     q.out_vec = !parts && whole_rows(p->dweight, p->d_in);
-    rc = avey_host::encode_rows16(p->dtype, g.p, p->d_out, p->rows, 1, g.ld * 2, 0, 64, &a);
-    if (rc == AVEY_OK) rc = avey_host::encode_rows16(p->dtype, x.p, p->d_in, p->rows, 1, x.ld * 2, 0, 64, &b);
+    Maps m;
+    rc = avey_host::encode_rows16(p->dtype, g.p, p->d_out, p->rows, 1, g.ld * 2, 0, 64, &m.a);
+    if (rc == AVEY_OK) rc = avey_host::encode_rows16(p->dtype, x.p, p->d_in, p->rows, 1, x.ld * 2, 0, 64, &m.b);
+    if (rc == AVEY_OK && (parts || q.out_vec))
+      rc = avey_host::encode_tiles(parts ? AVEY_F32 : p->dtype, q.out, p->d_in, p->d_out, q.splits * p->groups,
+                                   q.out_ld * (parts ? 4 : 2), q.out_gs * (parts ? 4 : 2), &m.y);
     if (rc != AVEY_OK) return rc;
     const int64_t tiles = p->groups * q.n_mt * q.n_nt * q.splits;
-    rc = parts ? launch_tc<avey::tc_linear<T, avey::kLnGradW, 0, true>>(a, b, q, tiles, stream)
-               : launch_tc<avey::tc_linear<T, avey::kLnGradW, 0, false>>(a, b, q, tiles, stream);
+    rc = parts ? launch_tc<avey::tc_linear<T, avey::kLnGradW, 0, true>>(m, q, tiles, stream)
+               : launch_tc<avey::tc_linear<T, avey::kLnGradW, 0, false>>(m, q, tiles, stream);
     if (rc != AVEY_OK) return rc;
     if (parts) {
       const int64_t rows = p->groups * p->d_out, quads = rows * (q.out_ld / 4);

@@ -24,6 +24,11 @@ int multiprocessors();
 int encode_rows16(int dtype, const void* base, uint64_t inner, uint64_t rows, uint64_t batch, uint64_t row_bytes,
                   uint64_t batch_bytes, int box_rows, CUtensorMap* map);
 
+// The same for output tiles of 32 rows of 64 bytes (64-byte swizzle): 32 16-bit
+// or, with dtype AVEY_F32, 16 32-bit elements.
+int encode_tiles(int dtype, void* base, uint64_t inner, uint64_t rows, uint64_t batch, uint64_t row_bytes,
+                 uint64_t batch_bytes, CUtensorMap* map);
+
 // The status word (read, and reset with `clear`) and the wait limit of the
 // kernels of avey_linear.cu, on the current device; a cudaError_t.
 int linear_flags(unsigned int* flags, bool clear);
