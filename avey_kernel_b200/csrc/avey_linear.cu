@@ -259,12 +259,14 @@ int forward_tc(const AveyLinearParams* p, cudaStream_t stream) {
 template <typename T, int ACT, bool DERIV>
 int launch_few(const avey::LnFew& q, cudaStream_t stream) {
   const dim3 grid((q.n + avey::kLfOut - 1) / avey::kLfOut, q.offsets ? std::min(q.groups, q.rows) + 1 : 1);
-  // Rows of a product: the least that hold all rows in one pass over the weights.
-  if (q.rows <= 8)
+  // Rows of a pass over the weights: the least that hold all rows of a dense
+  // layer, or twice an expert's share.
+  const int rows = q.offsets ? std::max(1, 2 * q.rows / q.groups) : q.rows;
+  if (rows <= 8)
     avey::ln_few<T, ACT, DERIV, 1><<<grid, avey::kLfThreads, 0, stream>>>(q);
-  else if (q.rows <= 16)
+  else if (rows <= 16)
     avey::ln_few<T, ACT, DERIV, 2><<<grid, avey::kLfThreads, 0, stream>>>(q);
-  else if (q.rows <= 32)
+  else if (rows <= 32)
     avey::ln_few<T, ACT, DERIV, 4><<<grid, avey::kLfThreads, 0, stream>>>(q);
   else
     avey::ln_few<T, ACT, DERIV, 8><<<grid, avey::kLfThreads, 0, stream>>>(q);
