@@ -47,6 +47,7 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) ==
 // Rows that TMA and 16-byte accesses can read in place.
 bool whole_rows(const void* p, int64_t ld) { return aligned16(p) && ld % 8 == 0; }
 int64_t up8(int64_t x) { return (x + 7) / 8 * 8; }
+int64_t up16(int64_t x) { return (x + 15) / 16 * 16; }
 uint64_t up256(uint64_t x) { return (x + 255u) & ~uint64_t(255); }
 
 // Rows up to which AUTO takes the kernel for few rows.
@@ -84,7 +85,8 @@ int validate(const AveyLinearParams* p, bool backward) {
     if (!p->deriv && p->activation != AVEY_ACT_IDENTITY)
       return fail(AVEY_ERR_ARGUMENT, "the backward pass needs deriv from the forward pass");
   }
-  if (p->deriv && !aligned16(p->deriv)) return fail(AVEY_ERR_ARGUMENT, "deriv must be 16-byte aligned");
+  if (p->deriv && (reinterpret_cast<uintptr_t>(p->deriv) & 31u) != 0)
+    return fail(AVEY_ERR_ARGUMENT, "deriv must be 32-byte aligned");
   return AVEY_OK;
 }
 
@@ -204,10 +206,9 @@ avey::LnGeom geom(const AveyLinearParams* p, int64_t n, int bn) {
   return q;
 }
 
-// Maps of a launch: the operands and the outputs (y / dx / dW, and the codes of
-// act'), which are left unset where they are not used.
+// Maps of a launch: the operands, and the output where it is stored by TMA.
 struct Maps {
-  CUtensorMap a{}, b{}, y{}, d{};
+  CUtensorMap a{}, b{}, y{};
 };
 
 template <auto K>
@@ -215,7 +216,7 @@ int launch_tc(const Maps& m, const avey::LnGeom& q, int64_t tiles, cudaStream_t 
   const cudaError_t e = smem_opt_in<K>();
   if (e != cudaSuccess) return fail(AVEY_ERR_CUDA, cudaGetErrorString(e));
   const int grid = static_cast<int>(std::min<int64_t>(tiles, avey_host::multiprocessors()));
-  K<<<grid, avey::kLnThreads, avey::kLnSmem, stream>>>(m.a, m.b, m.y, m.d, q);
+  K<<<grid, avey::kLnThreads, avey::kLnSmem, stream>>>(m.a, m.b, m.y, q);
   return launched("tc_linear");
 }
 
@@ -239,15 +240,13 @@ int forward_tc(const AveyLinearParams* p, cudaStream_t stream) {
   q.res_ld = p->residual_ld;
   q.res_vec = p->residual && whole_rows(p->residual, p->residual_ld);
   q.deriv = static_cast<uint16_t*>(p->deriv);
-  q.deriv_ld = up8(p->d_out);
+  q.deriv_ld = up16(p->d_out);
   Maps m;
   rc = avey_host::encode_rows16(p->dtype, x.p, p->d_in, p->rows, 1, x.ld * 2, 0, avey::kLnBM, &m.a);
   if (rc == AVEY_OK)
     rc = avey_host::encode_rows16(p->dtype, w.p, p->d_in, p->d_out, p->groups, w.ld * 2, w.gs * 2, q.bn, &m.b);
   if (rc == AVEY_OK && q.out_vec)
     rc = avey_host::encode_tiles(p->dtype, p->y, p->d_out, p->rows, 1, p->y_ld * 2, 0, &m.y);
-  if (rc == AVEY_OK && q.out_vec && p->deriv)
-    rc = avey_host::encode_tiles(p->dtype, p->deriv, p->d_out, p->rows, 1, q.deriv_ld * 2, 0, &m.d);
   if (rc != AVEY_OK) return rc;
   // One more row tile than the groups': the rows past the last group.
   const int64_t tiles = (mt + (p->offsets ? 1 : 0)) * q.n_nt;
@@ -293,7 +292,7 @@ int forward_few(const AveyLinearParams* p, cudaStream_t stream) {
   q.y = static_cast<uint16_t*>(p->y);
   q.y_ld = p->y_ld;
   q.deriv = static_cast<uint16_t*>(p->deriv);
-  q.deriv_ld = up8(p->d_out);
+  q.deriv_ld = up16(p->d_out);
   q.x_vec = whole_rows(p->x, p->x_ld);
   q.w_vec = whole_rows(p->weight, p->weight_ld) && (p->weight_group_stride % 8 == 0 || p->groups == 1);
   if constexpr (ACT != AVEY_ACT_IDENTITY)
@@ -346,7 +345,7 @@ int backward(const AveyLinearParams* p, cudaStream_t stream) {
     q.dy_ld = p->dy_ld;
     q.dy_vec = whole_rows(p->dy, p->dy_ld);
     q.deriv = static_cast<const uint16_t*>(p->deriv);
-    q.deriv_ld = up8(p->d_out);
+    q.deriv_ld = up16(p->d_out);
     if (l.make_dpre) {
       q.dpre = reinterpret_cast<uint16_t*>(ws + l.dpre);
       q.dpre_ld = up8(p->d_out);

@@ -67,7 +67,7 @@ struct LnGeom {
   int64_t res_ld;
   int res_vec;
   uint16_t* deriv;         // codes of act' [rows][deriv_ld], or null
-  int64_t deriv_ld;        // a multiple of 8
+  int64_t deriv_ld;        // a multiple of 16
 };
 
 // ---------------------------------------------------------------- activations
@@ -430,6 +430,12 @@ __device__ __forceinline__ void ln_tma_tile(uint32_t tile, int lane, const CUten
     bulk_commit_group();
   }
 }
+// 32 bytes to 32-byte aligned global memory.
+__device__ __forceinline__ void ln_st32(void* p, const uint32_t (&w)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+               "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+               : "memory");
+}
 // Before the staging tile is written again.
 __device__ __forceinline__ void ln_tile_free(int lane) {
   if (lane == 0) bulk_wait_read_all();
@@ -504,8 +510,7 @@ __device__ __forceinline__ void ln_read_ahead(const LnGeom& q, const LnTile& c, 
 // the next tile's (`next`, when there is one): the loads of a chunk are a whole
 // chunk ahead of their use, across tiles too.
 template <typename T, int MODE, int ACT, bool FLAG>
-__device__ __forceinline__ bool ln_drain(const LnGeom& q, const CUtensorMap* map_y, const CUtensorMap* map_d,
-                                         uint64_t policy, const LnTile& c, const LnTile& next, bool has_next,
+__device__ __forceinline__ bool ln_drain(const LnGeom& q, const CUtensorMap* map_y, uint64_t policy, const LnTile& c, const LnTile& next, bool has_next,
                                          uint32_t tb, int wq, int h, int lane, uint32_t tile, uint32_t bias_tile,
                                          uint32_t acc_full, uint32_t parity, uint32_t acc_empty, LnAhead& a) {
   constexpr bool F32 = MODE == kLnGradW && FLAG;
@@ -574,10 +579,9 @@ __device__ __forceinline__ bool ln_drain(const LnGeom& q, const CUtensorMap* map
       __syncwarp();
       if (ch + 1 < nch) ln_read_ahead<MODE>(q, c, wq, h, ch + 1, lane, a);
       else if (has_next) ln_read_ahead<MODE>(q, next, wq, h, 0, lane, a);
-      uint32_t dk[16];
 #pragma unroll
       for (int hh = 0; hh < 2; ++hh) {
-        uint32_t o[16];
+        uint32_t o[16], dk[8];
         ln_tmem_ld16(tb + ch * 32 + 16 * hh, zero, o);
 #pragma unroll
         for (int pp = 0; pp < 2; ++pp) {
@@ -594,7 +598,7 @@ __device__ __forceinline__ bool ln_drain(const LnGeom& q, const CUtensorMap* map
             LnPair d;
             LnPair v = ln_act2<ACT, DERIV>(
                 ln_add2(ln_pair(__uint_as_float(o[i]), __uint_as_float(o[i + 1])), ln_pair(bb.x, bb.y)), &d);
-            if (DERIV) dk[4 * p + j] = ln_encode2<T, ACT>(d);
+            if (DERIV) dk[4 * pp + j] = ln_encode2<T, ACT>(d);
             if (res) {
               const float2 rr = ln_unpack<T>(r4[j]);
               v = ln_add2(v, ln_pair(rr.x, rr.y));
@@ -604,6 +608,10 @@ __device__ __forceinline__ bool ln_drain(const LnGeom& q, const CUtensorMap* map
           }
           ln_sts(ln_piece(tile, lane, p), y[0], y[1], y[2], y[3]);
         }
+        // The codes of 16 columns are one 32-byte sector of the lane's row.
+        const int dcol = col0 + ch * 32 + 16 * hh;
+        if (DERIV && row0 + lane < row_end && dcol < q.deriv_ld)
+          ln_st32(q.deriv + static_cast<int64_t>(row0 + lane) * q.deriv_ld + dcol, dk);
       }
       if (by_tma) {
         ln_tma_tile(tile, lane, map_y, col0 + ch * 32, row0, 0, policy);
@@ -611,19 +619,6 @@ __device__ __forceinline__ bool ln_drain(const LnGeom& q, const CUtensorMap* map
         __syncwarp();
         ln_store_tile(tile, lane, out16, q.out_ld, l, q.out_vec);
         __syncwarp();
-      }
-      if (DERIV) {
-        ln_tile_free(lane);
-#pragma unroll
-        for (int p = 0; p < 4; ++p)
-          ln_sts(ln_piece(tile, lane, p), dk[4 * p], dk[4 * p + 1], dk[4 * p + 2], dk[4 * p + 3]);
-        if (by_tma) {
-          ln_tma_tile(tile, lane, map_d, col0 + ch * 32, row0, 0, policy);
-        } else {
-          __syncwarp();
-          ln_store_tile(tile, lane, q.deriv, q.deriv_ld, l, true);
-          __syncwarp();
-        }
       }
     }
     l.col += 32;
@@ -639,7 +634,7 @@ __device__ __forceinline__ bool ln_drain(const LnGeom& q, const CUtensorMap* map
 template <typename T, int MODE, int ACT, bool FLAG>
 __global__ void __launch_bounds__(kLnThreads, 1)
     tc_linear(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
-              const __grid_constant__ CUtensorMap map_y, const __grid_constant__ CUtensorMap map_d, const LnGeom q) {
+              const __grid_constant__ CUtensorMap map_y, const LnGeom q) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
@@ -843,7 +838,7 @@ __global__ void __launch_bounds__(kLnThreads, 1)
       const bool has_next = ln_warp_tile<MODE>(q, ctrl, it + 1, next);
       const int buf = it & 1;
       const uint32_t tb = tmem + lane_off + static_cast<uint32_t>(buf * 256 + h * ln_part(q));
-      if (!ln_drain<T, MODE, ACT, FLAG>(q, &map_y, &map_d, policy, c, next, has_next, tb, wq, h, lane, stage, bias_tile,
+      if (!ln_drain<T, MODE, ACT, FLAG>(q, &map_y, policy, c, next, has_next, tb, wq, h, lane, stage, bias_tile,
                                         smem_u32(&ctrl->acc_full[buf]), (it >> 1) & 1,
                                         smem_u32(&ctrl->acc_empty[buf]), ahead))
         break;

@@ -247,7 +247,7 @@ std::pair<Tensor, Tensor> linear_forward(const Tensor& x, const Tensor& weight, 
   p.y = y.data_ptr();
   p.y_ld = p.d_out;
   if (want_deriv && act != AVEY_ACT_IDENTITY && p.rows > 0) {
-    deriv = at::empty({p.rows, (p.d_out + 7) / 8 * 8}, x.options().dtype(at::kShort));
+    deriv = at::empty({p.rows, (p.d_out + 15) / 16 * 16}, x.options().dtype(at::kShort));
     p.deriv = deriv.data_ptr();
   }
   const Tensor ws = workspace(p, 0, x);

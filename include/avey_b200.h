@@ -410,7 +410,7 @@ AVEY_API int avey_fwd_presummed_v1(const AveyFwdParams* params, const float* sum
  * dtype is AVEY_BF16 or AVEY_F16 for every array; products and sums are fp32
  * and each result is rounded once; dpre is rounded to dtype before the two
  * products of the backward pass. The forward pass writes act' as 16-bit codes
- * into deriv when it is given (d_out rounded up to 8 values a row; any
+ * into deriv when it is given (d_out rounded up to 16 values a row; any
  * activation but the identity), and the backward pass reads them. Gradients
  * use fixed orders: results are bitwise reproducible.
  *
@@ -435,7 +435,7 @@ typedef struct AveyLinearParams {
   int64_t residual_ld;
   void* y;
   int64_t y_ld;
-  void* deriv; /* 16-byte aligned; forward: or NULL */
+  void* deriv; /* 32-byte aligned; forward: or NULL */
 
   /* Backward (y, residual and bias are not read). NULL: not wanted. */
   const void* dy; /* [rows][d_out] */

@@ -504,7 +504,7 @@ def test_c_entry_rejects_bad_arguments_before_any_launch(field, value, match):
 
 @pytest.mark.parametrize('change,match', [
     (dict(dy=0), 'dy is required'), (dict(dx_ld=10), 'dy is required'),
-    (dict(activation=3), 'needs deriv'), (dict(activation=3, deriv=(1 << 21) + 2), '16-byte aligned')])
+    (dict(activation=3), 'needs deriv'), (dict(activation=3, deriv=(1 << 21) + 2), '32-byte aligned')])
 def test_c_backward_entry_rejects_bad_arguments(change, match):
     with pytest.raises(_native.NativeError, match=match):
         _native.linear(_params(**change), 0, backward=True)
