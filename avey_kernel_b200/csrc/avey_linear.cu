@@ -159,15 +159,6 @@ Layout layout(const AveyLinearParams* p, bool backward) {
   return l;
 }
 
-int pack(const void* src, int64_t ld, int64_t gs, int64_t per, int64_t rows, int64_t cols, void* dst,
-         cudaStream_t stream) {
-  const int64_t pieces = rows * (up8(cols) / 8);
-  const int grid = static_cast<int>(std::min<int64_t>((pieces + 255) / 256, avey_host::multiprocessors() * 16ll));
-  avey::ln_pack_rows<<<grid, 256, 0, stream>>>(static_cast<const uint16_t*>(src), ld, gs, per, rows,
-                                               static_cast<int>(cols), static_cast<uint16_t*>(dst), up8(cols));
-  return launched("row copy");
-}
-
 // The operands as the tensor cores read them.
 struct Rows {
   const void* p;
@@ -178,18 +169,30 @@ int pack_inputs(const AveyLinearParams* p, const Layout& l, Rows* x, Rows* w, cu
   char* ws = static_cast<char*>(p->workspace);
   *x = {p->x, p->x_ld, 0};
   *w = {p->weight, p->weight_ld, p->weight_group_stride};
+  if (!l.pack_x && !l.pack_w) return AVEY_OK;
+  avey::LnPack a{}, b{};
+  a.ld = b.ld = up8(p->d_in);
+  a.cols = b.cols = static_cast<int>(p->d_in);
   if (l.pack_x) {
-    const int rc = pack(p->x, p->x_ld, 0, p->rows, p->rows, p->d_in, ws + l.x, stream);
-    if (rc != AVEY_OK) return rc;
-    *x = {ws + l.x, up8(p->d_in), 0};
+    a.src = static_cast<const uint16_t*>(p->x);
+    a.src_ld = p->x_ld;
+    a.per = a.rows = p->rows;
+    a.dst = reinterpret_cast<uint16_t*>(ws + l.x);
+    *x = {a.dst, a.ld, 0};
   }
   if (l.pack_w) {
-    const int rc = pack(p->weight, p->weight_ld, p->weight_group_stride, p->d_out, p->groups * p->d_out, p->d_in,
-                        ws + l.w, stream);
-    if (rc != AVEY_OK) return rc;
-    *w = {ws + l.w, up8(p->d_in), p->d_out * up8(p->d_in)};
+    b.src = static_cast<const uint16_t*>(p->weight);
+    b.src_ld = p->weight_ld;
+    b.src_gs = p->weight_group_stride;
+    b.per = p->d_out;
+    b.rows = p->groups * p->d_out;
+    b.dst = reinterpret_cast<uint16_t*>(ws + l.w);
+    *w = {b.dst, b.ld, p->d_out * b.ld};
   }
-  return AVEY_OK;
+  const int64_t pieces = (a.rows + b.rows) * (a.ld / 8);
+  const int grid = static_cast<int>(std::min<int64_t>((pieces + 255) / 256, avey_host::multiprocessors() * 16ll));
+  avey::ln_pack_rows<<<grid, 256, 0, stream>>>(a, b);
+  return launched("row copy");
 }
 
 avey::LnGeom geom(const AveyLinearParams* p, int64_t n, int bn) {
@@ -356,7 +359,7 @@ int backward(const AveyLinearParams* p, cudaStream_t stream) {
     if (rc != AVEY_OK) return rc;
     if (l.sums) {
       const dim3 grid(static_cast<unsigned>((p->d_out + 31) / 32), static_cast<unsigned>(p->groups));
-      avey::ln_bias_sum<T><<<grid, 256, 0, stream>>>(p->offsets, q.groups, q.rows, q.n, q.partial,
+      avey::ln_bias_sum<T><<<grid, avey::kLbThreads, 0, stream>>>(p->offsets, q.groups, q.rows, q.n, q.partial,
                                                      static_cast<T*>(p->dbias));
       rc = launched("ln_bias_sum");
       if (rc != AVEY_OK) return rc;

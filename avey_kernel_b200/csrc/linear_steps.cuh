@@ -275,25 +275,27 @@ __global__ void __launch_bounds__(kLdThreads) ln_dpre(const LnDpre q) {
   }
 }
 
-// db[g] = the sum of the group's partial rows (a fixed order: lane i of 8 takes
-// every eighth row, then the lanes in turn).
+// db[g] = the sum of the group's partial rows (a fixed order: part i of 32 takes
+// every 32nd row, then the parts in turn).
+constexpr int kLbThreads = 1024;
 template <typename T>
-__global__ void __launch_bounds__(256) ln_bias_sum(const int32_t* offsets, int groups, int rows, int n,
-                                                   const float* partial, T* db) {
-  __shared__ float red[8][33];
+__global__ void __launch_bounds__(kLbThreads) ln_bias_sum(const int32_t* offsets, int groups, int rows, int n,
+                                                          const float* partial, T* db) {
+  __shared__ float red[32][33];
   const int lane = threadIdx.x & 31, part = threadIdx.x >> 5;
   LnSpan s;
   ln_find(offsets, groups, rows, -1, blockIdx.y, [](int lo, int hi) { return (hi - lo + kLdRows - 1) / kLdRows; }, s);
   const int c = blockIdx.x * 32 + lane;
   float t = 0.f;
   if (c < n)
-    for (int i = part; i < s.cnt; i += 8) t += partial[static_cast<int64_t>(s.base + i) * n + c];
+#pragma unroll 4
+    for (int i = part; i < s.cnt; i += 32) t += partial[static_cast<int64_t>(s.base + i) * n + c];
   red[part][lane] = t;
   __syncthreads();
   if (part == 0 && c < n) {
     float z = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) z += red[i][lane];
+    for (int i = 0; i < 32; ++i) z += red[i][lane];
     db[static_cast<int64_t>(blockIdx.y) * n + c] = Elem<T>::from_f(z);
   }
 }
@@ -329,17 +331,25 @@ __global__ void __launch_bounds__(256) ln_split_sum(const float* partial, int sp
   }
 }
 
-// Rows of `cols` 16-bit values (per rows of a group, groups gs apart) copied to
-// rows of ld values (a multiple of 8), zeros at the end: what TMA can read.
-__global__ void __launch_bounds__(256) ln_pack_rows(const uint16_t* src, int64_t src_ld, int64_t src_gs, int64_t per,
-                                                    int64_t rows, int cols, uint16_t* dst, int64_t ld) {
-  const int64_t pieces = ld / 8, total = rows * pieces;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < total;
+// Rows of `cols` 16-bit values (`per` rows of a group, groups gs apart) copied to
+// rows of ld values (a multiple of 8), zeros at the end: what TMA can read. Two
+// arrays a launch (rows 0: none).
+struct LnPack {
+  const uint16_t* src;
+  int64_t src_ld, src_gs, per, rows, ld;
+  int cols;
+  uint16_t* dst;
+};
+__global__ void __launch_bounds__(256) ln_pack_rows(const LnPack a, const LnPack b) {
+  const int64_t na = a.rows * (a.ld / 8), nb = b.rows * (b.ld / 8);
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < na + nb;
        i += static_cast<int64_t>(gridDim.x) * 256) {
-    const int64_t row = i / pieces, g = row / per;
-    const int c = static_cast<int>(i - row * pieces) * 8;
-    const uint16_t* p = src + g * src_gs + (row - g * per) * src_ld + c;
-    *reinterpret_cast<uint4*>(dst + row * ld + c) = ln_load8(p, cols - c, false);
+    const LnPack& k = i < na ? a : b;
+    const int64_t j = i < na ? i : i - na;
+    const int64_t pieces = k.ld / 8, row = j / pieces, g = row / k.per;
+    const int c = static_cast<int>(j - row * pieces) * 8;
+    const uint16_t* p = k.src + g * k.src_gs + (row - g * k.per) * k.src_ld + c;
+    *reinterpret_cast<uint4*>(k.dst + row * k.ld + c) = ln_load8(p, k.cols - c, false);
   }
 }
 

@@ -392,27 +392,54 @@ struct LnLines {
   __device__ __forceinline__ bool in(int i) const { return row + 8 * i < row_end; }
 };
 
+// Address of element (r, column k) of a staging tile.
+__device__ __forceinline__ uint32_t ln_element(uint32_t tile, int r, int k) {
+  return ln_piece(tile, r, k >> 3) + 2 * (k & 7);
+}
+
+// Store a staged tile row by row, a lane to a column: rows that are not whole
+// 16-byte units, and the last columns.
+__device__ __forceinline__ void ln_store_tile_by_column(uint32_t tile, int lane, uint16_t* out, int64_t ld,
+                                                        const LnLines& l) {
+  const int row0 = l.row - (lane >> 2), col = l.col - (lane & 3) * 8 + lane;
+  const int rows = min(32, l.row_end - row0);
+  uint16_t* p = out + static_cast<int64_t>(row0) * ld + col;
+  if (col < l.n) {
+#pragma unroll 8
+    for (int r = 0; r < rows; ++r) {
+      uint16_t v;
+      asm volatile("ld.shared.b16 %0, [%1];" : "=h"(v) : "r"(ln_element(tile, r, lane)));
+      p[r * ld] = v;
+    }
+  }
+}
+
+// Bring a tile into shared memory the same way (columns past the end: zeros).
+__device__ __forceinline__ void ln_fetch_tile_by_column(uint32_t tile, int lane, const uint16_t* src, int64_t ld,
+                                                        const LnLines& l) {
+  const int row0 = l.row - (lane >> 2), col = l.col - (lane & 3) * 8 + lane;
+  const int rows = min(32, l.row_end - row0);
+  const uint16_t* p = src + static_cast<int64_t>(row0) * ld + col;
+#pragma unroll 8
+  for (int r = 0; r < rows; ++r) {
+    const uint16_t v = col < l.n ? __ldg(p + r * ld) : static_cast<uint16_t>(0);
+    asm volatile("st.shared.b16 [%0], %1;" ::"r"(ln_element(tile, r, lane)), "h"(v) : "memory");
+  }
+}
+
 // Store a staged 32 x 32 16-bit tile to `out`.
 __device__ __forceinline__ void ln_store_tile(uint32_t tile, int lane, uint16_t* out, int64_t ld, const LnLines& l,
                                               bool vec) {
-  if (l.col >= l.n) return;
-  uint16_t* p = out + static_cast<int64_t>(l.row) * ld + l.col;
-  if (vec && l.col + 8 <= l.n) {
+  // The decision is the warp's: lane 31 has the tile's last columns.
+  if (vec && __shfl_sync(0xFFFFFFFFu, l.col, 31) + 8 <= l.n) {
+    uint16_t* p = out + static_cast<int64_t>(l.row) * ld + l.col;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const uint4 v = ln_lds(ln_piece(tile, i * 8 + (lane >> 2), lane & 3));
       if (l.in(i)) *reinterpret_cast<uint4*>(p + 8 * i * ld) = v;
     }
   } else {
-#pragma unroll 1
-    for (int i = 0; i < 4; ++i) {
-      const uint4 v = ln_lds(ln_piece(tile, i * 8 + (lane >> 2), lane & 3));
-      if (!l.in(i)) continue;
-      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (l.col + j < l.n) p[8 * i * ld + j] = static_cast<uint16_t>(w[j >> 1] >> (16 * (j & 1)));
-    }
+    ln_store_tile_by_column(tile, lane, out, ld, l);
   }
 }
 
@@ -458,11 +485,11 @@ __device__ __forceinline__ void ln_tmem_ld16(uint32_t taddr, bool zero, uint32_t
       : "memory");
 }
 
-// This lane's pieces of a 32 x 32 tile of 16-bit values (outside: zeros).
-__device__ __forceinline__ void ln_load_tile(const uint16_t* src, int64_t ld, const LnLines& l, bool vec,
-                                             uint4 (&v)[4]) {
+// This lane's pieces of a 32 x 32 tile of 16-bit values in 16-byte aligned rows
+// (outside: zeros; the last piece of a row may be cut).
+__device__ __forceinline__ void ln_load_tile(const uint16_t* src, int64_t ld, const LnLines& l, uint4 (&v)[4]) {
   const uint16_t* p = src + static_cast<int64_t>(l.row) * ld + l.col;
-  if (vec && l.col + 8 <= l.n) {
+  if (l.col + 8 <= l.n) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       v[i] = make_uint4(0u, 0u, 0u, 0u);
@@ -495,9 +522,9 @@ __device__ __forceinline__ void ln_read_ahead(const LnGeom& q, const LnTile& c, 
                                               LnAhead& a) {
   if (MODE != kLnForward || c.g >= q.groups) return;
   const int col = c.nt * q.bn + h * ln_part(q) + ch * 32;
-  if (q.res) {
+  if (q.res && q.res_vec) {
     const LnLines l{c.row0 + wq * 32 + (lane >> 2), c.hi, col + (lane & 3) * 8, q.n};
-    ln_load_tile(static_cast<const uint16_t*>(q.res), q.res_ld, l, q.res_vec, a.res);
+    ln_load_tile(static_cast<const uint16_t*>(q.res), q.res_ld, l, a.res);
   }
   a.bias = 0;
   if (q.bias && col + lane < q.n)
@@ -570,10 +597,12 @@ __device__ __forceinline__ bool ln_drain(const LnGeom& q, const CUtensorMap* map
       ln_tile_free(lane);
       // The residual's lines go through the staging tile to the lanes of their
       // rows, the bias to all lanes; the next chunk's are loaded meanwhile.
-      if (res) {
+      if (res && q.res_vec) {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           ln_sts(ln_piece(tile, i * 8 + (lane >> 2), lane & 3), a.res[i].x, a.res[i].y, a.res[i].z, a.res[i].w);
+      } else if (res) {
+        ln_fetch_tile_by_column(tile, lane, static_cast<const uint16_t*>(q.res), q.res_ld, l);
       }
       asm volatile("st.shared.b16 [%0], %1;" ::"r"(bias_tile + 2 * lane), "h"(a.bias) : "memory");
       __syncwarp();
