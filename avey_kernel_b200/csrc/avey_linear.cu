@@ -50,7 +50,7 @@ int64_t up8(int64_t x) { return (x + 7) / 8 * 8; }
 int64_t up16(int64_t x) { return (x + 15) / 16 * 16; }
 uint64_t up256(uint64_t x) { return (x + 255u) & ~uint64_t(255); }
 
-// Rows up to which AUTO takes the kernel for few rows.
+// Rows up to which AUTO may take the kernel for few rows.
 constexpr int64_t kFewRows = 64;
 
 int validate(const AveyLinearParams* p, bool backward) {
@@ -90,9 +90,15 @@ int validate(const AveyLinearParams* p, bool backward) {
   return AVEY_OK;
 }
 
+// AUTO: dense layers of 1 to 64 rows finish sooner there (64 rows, 768 -> 1536:
+// 5.3 against 7.9 us; 4096 -> 4096: 17.0 against 22.8), of 128 rows no longer
+// (4096 -> 4096: 30.7 against 23.0). Grouped ones too, while the weights that
+// the rows can touch stay below about 100 MB (64 rows of 8 experts, 768 -> 1536:
+// 8.3 against 12.7 us; 64 of 16, 1024 -> 2048: 13.0 against 12.8; 64 of 64: 45
+// against 36).
 bool use_few(const AveyLinearParams* p) {
   if (p->kernel != AVEY_LINEAR_KERNEL_AUTO) return p->kernel == AVEY_LINEAR_KERNEL_FEW;
-  return p->rows <= kFewRows;
+  return p->rows <= kFewRows && std::min(p->groups, p->rows) * p->d_in * p->d_out <= 48ll << 20;
 }
 
 // Row tiles of `tile` rows that the groups can come to.
@@ -258,21 +264,25 @@ int forward_tc(const AveyLinearParams* p, cudaStream_t stream) {
   return launch_tc<avey::tc_linear<T, avey::kLnForward, ACT, false>>(m, q, tiles, stream);
 }
 
+template <typename T, int ACT, bool DERIV, int NT>
+int launch_few_rows(const avey::LnFew& q, cudaStream_t stream) {
+  const dim3 grid((q.n + avey::kLfOut - 1) / avey::kLfOut, q.offsets ? std::min(q.groups, q.rows) + 1 : 1);
+  if (static_cast<int64_t>(grid.x) * grid.y <= avey_host::multiprocessors() && q.k >= 1024)
+    avey::ln_few<T, ACT, DERIV, NT, 16><<<grid, 512, 0, stream>>>(q);
+  else
+    avey::ln_few<T, ACT, DERIV, NT, 8><<<grid, 256, 0, stream>>>(q);
+  return launched("ln_few");
+}
+
 template <typename T, int ACT, bool DERIV>
 int launch_few(const avey::LnFew& q, cudaStream_t stream) {
-  const dim3 grid((q.n + avey::kLfOut - 1) / avey::kLfOut, q.offsets ? std::min(q.groups, q.rows) + 1 : 1);
   // Rows of a pass over the weights: the least that hold all rows of a dense
   // layer, or twice an expert's share.
   const int rows = q.offsets ? std::max(1, 2 * q.rows / q.groups) : q.rows;
-  if (rows <= 8)
-    avey::ln_few<T, ACT, DERIV, 1><<<grid, avey::kLfThreads, 0, stream>>>(q);
-  else if (rows <= 16)
-    avey::ln_few<T, ACT, DERIV, 2><<<grid, avey::kLfThreads, 0, stream>>>(q);
-  else if (rows <= 32)
-    avey::ln_few<T, ACT, DERIV, 4><<<grid, avey::kLfThreads, 0, stream>>>(q);
-  else
-    avey::ln_few<T, ACT, DERIV, 8><<<grid, avey::kLfThreads, 0, stream>>>(q);
-  return launched("ln_few");
+  if (rows <= 8) return launch_few_rows<T, ACT, DERIV, 1>(q, stream);
+  if (rows <= 16) return launch_few_rows<T, ACT, DERIV, 2>(q, stream);
+  if (rows <= 32) return launch_few_rows<T, ACT, DERIV, 4>(q, stream);
+  return launch_few_rows<T, ACT, DERIV, 8>(q, stream);
 }
 
 template <typename T, int ACT>
@@ -296,8 +306,12 @@ int forward_few(const AveyLinearParams* p, cudaStream_t stream) {
   q.y_ld = p->y_ld;
   q.deriv = static_cast<uint16_t*>(p->deriv);
   q.deriv_ld = up16(p->d_out);
-  q.x_vec = whole_rows(p->x, p->x_ld);
-  q.w_vec = whole_rows(p->weight, p->weight_ld) && (p->weight_group_stride % 8 == 0 || p->groups == 1);
+  auto vec = [](const void* base, int64_t ld, int64_t gs) {
+    const uint64_t all = reinterpret_cast<uintptr_t>(base) | static_cast<uint64_t>(ld) * 2 | static_cast<uint64_t>(gs) * 2;
+    return all % 32 == 0 ? 2 : all % 16 == 0 ? 1 : 0;
+  };
+  q.x_vec = vec(p->x, p->x_ld, 0);
+  q.w_vec = vec(p->weight, p->weight_ld, p->groups > 1 ? p->weight_group_stride : 0);
   if constexpr (ACT != AVEY_ACT_IDENTITY)
     if (p->deriv) return launch_few<T, ACT, true>(q, stream);
   return launch_few<T, ACT, false>(q, stream);

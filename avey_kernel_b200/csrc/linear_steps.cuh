@@ -78,6 +78,25 @@ __device__ __forceinline__ uint4 ln_load8(const uint16_t* p, int left, bool vec)
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+struct LnOct2 {
+  uint4 a, b;  // 16 consecutive values
+};
+// Sixteen 16-bit values at p; values at `left` and beyond are zero. `vec`: 32-byte
+// aligned (2), 16-byte aligned (1) or neither.
+__device__ __forceinline__ LnOct2 ln_load16(const uint16_t* p, int left, int vec) {
+  LnOct2 r;
+  if (vec == 2 && left >= 16) {
+    asm volatile("ld.global.nc.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(r.a.x), "=r"(r.a.y), "=r"(r.a.z), "=r"(r.a.w), "=r"(r.b.x), "=r"(r.b.y), "=r"(r.b.z),
+                   "=r"(r.b.w)
+                 : "l"(p));
+  } else {
+    r.a = ln_load8(p, left, vec != 0);
+    r.b = ln_load8(p + 8, left - 8, vec != 0);
+  }
+  return r;
+}
+
 // ---------------------------------------------------------------- few rows
 
 // y for a few rows per group: the weights are read once, straight from global
@@ -85,10 +104,12 @@ __device__ __forceinline__ uint4 ln_load8(const uint16_t* p, int left, bool vec)
 // below any tensor rate, and 128-row tiles would leave most SMs without
 // work). W is the 16-row operand, up to 8 NT rows of x the 8-column one. The
 // order of k inside a product is free as long as both operands agree, so a
-// lane takes 8 consecutive k (16 bytes) of a 32-wide step for its fragments.
-// A CTA owns 16 outputs; its 8 warps take every eighth step of K, and their sums
-// are added in a fixed order.
-constexpr int kLfThreads = 256;
+// lane takes 16 consecutive k (32 bytes) of a 64-wide step for its fragments:
+// four lanes read a whole line of a row (with 16 bytes a lane, half lines, 48
+// rows of 2048 -> 1024 took 8.8 us).
+// A CTA owns 16 outputs; its warps share the steps of K, and their sums are added
+// in a fixed order. Where there are no more CTAs than SMs and K is long, 16
+// warps share them instead of 8.
 constexpr int kLfOut = 16;
 
 struct LnFew {
@@ -97,7 +118,7 @@ struct LnFew {
   const uint16_t *x, *w, *bias, *res;
   int64_t x_ld, w_ld, w_gs, bias_gs, res_ld, y_ld, deriv_ld;
   uint16_t *y, *deriv;
-  int x_vec, w_vec;
+  int x_vec, w_vec;  // rows are 32-byte aligned (2), 16-byte aligned (1) or neither
 };
 
 template <typename T>
@@ -115,8 +136,9 @@ __device__ __forceinline__ void ln_mma(float (&c)[4], uint32_t a0, uint32_t a1, 
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-template <typename T, int ACT, bool DERIV, int NT>
-__global__ void __launch_bounds__(kLfThreads) ln_few(const LnFew q) {
+template <typename T, int ACT, bool DERIV, int NT, int WARPS>
+__global__ void __launch_bounds__(32 * WARPS) ln_few(const LnFew q) {
+  constexpr int kThreads = 32 * WARPS;
   __shared__ float red[8][8 * NT][kLfOut + 1];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int n0 = blockIdx.x * kLfOut;
@@ -138,42 +160,57 @@ __global__ void __launch_bounds__(kLfThreads) ln_few(const LnFew q) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) acc[j][i] = 0.f;
     if (!zero) {
-      constexpr int kUnroll = NT >= 4 ? 2 : 4;
-      const int steps = (q.k + 31) / 32;
-      for (int s0 = warp; s0 < steps; s0 += 8 * kUnroll) {
-        uint4 a[kUnroll], b[kUnroll], v[kUnroll][NT];
+      constexpr int kUnroll = NT >= 4 ? 1 : 2;
+      const int steps = (q.k + 63) / 64;
+      for (int s0 = warp; s0 < steps; s0 += WARPS * kUnroll) {
+        LnOct2 a[kUnroll], b[kUnroll], v[kUnroll][NT];
+        const LnOct2 none{make_uint4(0u, 0u, 0u, 0u), make_uint4(0u, 0u, 0u, 0u)};
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) {
-          const int k = (s0 + 8 * u) * 32 + (lane & 3) * 8;
+          const int k = (s0 + WARPS * u) * 64 + (lane & 3) * 16;
           const int left = q.k - k;
-          a[u] = b[u] = make_uint4(0u, 0u, 0u, 0u);
-          if (left > 0 && o_lo < q.n) a[u] = ln_load8(wl + k, left, q.w_vec);
-          if (left > 0 && o_hi < q.n) b[u] = ln_load8(wh + k, left, q.w_vec);
+          a[u] = b[u] = none;
+          if (left > 0 && o_lo < q.n) a[u] = ln_load16(wl + k, left, q.w_vec);
+          if (left > 0 && o_hi < q.n) b[u] = ln_load16(wh + k, left, q.w_vec);
 #pragma unroll
           for (int j = 0; j < NT; ++j) {
             const int row = r0 + j * 8 + (lane >> 2);
-            v[u][j] = make_uint4(0u, 0u, 0u, 0u);
+            v[u][j] = none;
             if (left > 0 && row < s.hi)
-              v[u][j] = ln_load8(q.x + static_cast<int64_t>(row) * q.x_ld + k, left, q.x_vec);
+              v[u][j] = ln_load16(q.x + static_cast<int64_t>(row) * q.x_ld + k, left, q.x_vec);
           }
         }
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u)
 #pragma unroll
           for (int j = 0; j < NT; ++j) {
-            ln_mma<T>(acc[j], a[u].x, b[u].x, a[u].y, b[u].y, v[u][j].x, v[u][j].y);
-            ln_mma<T>(acc[j], a[u].z, b[u].z, a[u].w, b[u].w, v[u][j].z, v[u][j].w);
+            ln_mma<T>(acc[j], a[u].a.x, b[u].a.x, a[u].a.y, b[u].a.y, v[u][j].a.x, v[u][j].a.y);
+            ln_mma<T>(acc[j], a[u].a.z, b[u].a.z, a[u].a.w, b[u].a.w, v[u][j].a.z, v[u][j].a.w);
+            ln_mma<T>(acc[j], a[u].b.x, b[u].b.x, a[u].b.y, b[u].b.y, v[u][j].b.x, v[u][j].b.y);
+            ln_mma<T>(acc[j], a[u].b.z, b[u].b.z, a[u].b.w, b[u].b.w, v[u][j].b.z, v[u][j].b.w);
           }
       }
     }
-    __syncthreads();
+    // The upper warps of 16 hand their sums to the lower ones.
+    auto put = [&](bool add) {
 #pragma unroll
-    for (int j = 0; j < NT; ++j)
+      for (int j = 0; j < NT; ++j)
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        red[warp][j * 8 + (lane & 3) * 2 + (i & 1)][(lane >> 2) + (i >> 1) * 8] = acc[j][i];
+        for (int i = 0; i < 4; ++i) {
+          float& z = red[warp & 7][j * 8 + (lane & 3) * 2 + (i & 1)][(lane >> 2) + (i >> 1) * 8];
+          z = add ? z + acc[j][i] : acc[j][i];
+        }
+    };
     __syncthreads();
-    for (int i = threadIdx.x; i < 8 * NT * kLfOut; i += kLfThreads) {
+    if (WARPS == 16) {
+      if (warp >= 8) put(false);
+      __syncthreads();
+      if (warp < 8) put(true);
+    } else {
+      put(false);
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < 8 * NT * kLfOut; i += kThreads) {
       const int r = i / kLfOut, o = i % kLfOut;
       const int row = r0 + r, col = n0 + o;
       if (row >= s.hi || col >= q.n) continue;
