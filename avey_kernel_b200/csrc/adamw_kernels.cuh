@@ -35,7 +35,8 @@ struct AwTensor {
   float* master;
   int64_t n;
   int64_t block0;  // number of the tensor's first block in the whole call
-  int64_t chunk0;  // first chunk of the launch
+  int32_t chunk0;  // first chunk of the launch
+  int32_t whole;   // 8-bit states: the first chunks that are whole and aligned
 };
 
 constexpr int kAwCtas8 = 3;   // CTAs per SM of the 8-bit step (at four, 64 registers a thread, it spills)
@@ -44,7 +45,7 @@ constexpr int kAwStages = 3;  // its blocks in flight per warp
 template <int N>
 struct AwTable {
   int count;
-  int64_t chunks;
+  int chunks;
   AwTensor t[N];
 };
 
@@ -59,6 +60,7 @@ struct AwScalars {
   float2 minus_zerop;  // -0 (see aw_prod2)
   uint32_t seed;
   uint32_t step;
+  uint32_t key;          // aw_key of the first 2^32 elements
   const float* grad_scale;
 };
 
@@ -70,7 +72,7 @@ __device__ __forceinline__ uint32_t aw_mix(uint32_t x) {
   return x ^ (x >> 16);
 }
 
-__device__ __forceinline__ uint32_t aw_key(uint32_t seed, uint32_t step, uint32_t hi) {
+__host__ __device__ __forceinline__ uint32_t aw_key(uint32_t seed, uint32_t step, uint32_t hi) {
   uint32_t x = seed + 0x9e3779b9u * (step + hi);
   x = (x ^ (x >> 16)) * 0x7feb352du;
   return (x ^ (x >> 16)) * 0x846ca68bu;
@@ -298,7 +300,7 @@ __device__ __forceinline__ void aw_block(const AwTensor& t, const AwScalars& c, 
 
 // The last tensor whose first chunk is at or before `chunk`.
 template <int N>
-__device__ __forceinline__ int aw_tensor_of(const AwTable<N>& tab, int64_t chunk) {
+__device__ __forceinline__ int aw_tensor_of(const AwTable<N>& tab, int chunk) {
   int lo = 0, hi = tab.count;
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
@@ -311,10 +313,9 @@ __device__ __forceinline__ int aw_tensor_of(const AwTable<N>& tab, int64_t chunk
 // States in fp32.
 template <typename T, bool MASTER, int N>
 __global__ void __launch_bounds__(kAwThreads) adamw_step(const __grid_constant__ AwTable<N> tab, const AwScalars c) {
-  int64_t chunk = blockIdx.x;
   const float gs = c.grad_scale ? *c.grad_scale : 1.f;
-  int ti = aw_tensor_of(tab, chunk);
-  for (; chunk < tab.chunks; chunk += gridDim.x) {
+  int ti = aw_tensor_of(tab, blockIdx.x);
+  for (int64_t chunk = blockIdx.x; chunk < tab.chunks; chunk += gridDim.x) {
     while (ti + 1 < tab.count && tab.t[ti + 1].chunk0 <= chunk) ++ti;
     const AwTensor& t = tab.t[ti];
     const int64_t at0 = (chunk - t.chunk0) * kAwChunk + (threadIdx.x >> 5) * kAwBlock;
@@ -449,16 +450,6 @@ __device__ __forceinline__ void aw_copy(void* dst, const void* src) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(d), "l"(src), "n"(BYTES) : "memory");
 }
 
-// Whether chunk `i` of a tensor takes the loop for whole blocks.
-template <typename T, bool MASTER>
-__device__ __forceinline__ bool aw_whole(const AwTensor& t, int64_t i) {
-  constexpr uintptr_t kMask = 8 * sizeof(T) - 1;
-  uintptr_t bad = ((reinterpret_cast<uintptr_t>(t.p) | reinterpret_cast<uintptr_t>(t.g)) & kMask) |
-                  ((reinterpret_cast<uintptr_t>(t.m) | reinterpret_cast<uintptr_t>(t.v)) & 7u);
-  if (MASTER) bad |= reinterpret_cast<uintptr_t>(t.master) & 31u;
-  return bad == 0 && (i + 1) * kAwChunk <= t.n;
-}
-
 template <typename T, bool MASTER, int N>
 __global__ void __launch_bounds__(kAwThreads, kAwCtas8) adamw8_step(const __grid_constant__ AwTable<N> tab, const AwScalars c) {
   using Stage = AwStage<T, MASTER>;
@@ -469,16 +460,16 @@ __global__ void __launch_bounds__(kAwThreads, kAwCtas8) adamw8_step(const __grid
   const float gs = c.grad_scale ? *c.grad_scale : 1.f;
   // CTAs take chunks round robin, so that all work on neighbouring memory. The
   // copies run kAwStages - 1 chunks ahead, into the next tensor too.
-  int ahead_ti = aw_tensor_of(tab, static_cast<int64_t>(blockIdx.x));
-  int64_t ahead = blockIdx.x;
+  int ahead_ti = aw_tensor_of(tab, blockIdx.x);
+  int ahead = blockIdx.x;
   auto copy = [&](int stage) {
     if (ahead < tab.chunks) {
       while (ahead_ti + 1 < tab.count && tab.t[ahead_ti + 1].chunk0 <= ahead) ++ahead_ti;
       const AwTensor& t = tab.t[ahead_ti];
-      const int64_t i = ahead - t.chunk0;
-      if (aw_whole<T, MASTER>(t, i)) {
+      const int i = ahead - t.chunk0;
+      if (i < t.whole) {
         Stage& d = stages[stage];
-        const int64_t at = i * kAwChunk;
+        const int64_t at = static_cast<int64_t>(i) * kAwChunk;
         const uint4* g = reinterpret_cast<const uint4*>(static_cast<const T*>(t.g) + at + off);
         const uint4* p = MASTER ? reinterpret_cast<const uint4*>(t.master + at + off)
                                 : reinterpret_cast<const uint4*>(static_cast<const T*>(t.p) + at + off);
@@ -492,12 +483,12 @@ __global__ void __launch_bounds__(kAwThreads, kAwCtas8) adamw8_step(const __grid
         aw_copy<4>(&d.vs[threadIdx.x], t.vs + at / kAwBlock + warp);
       }
     }
-    ahead += gridDim.x;
+    ahead = min(ahead, tab.chunks) + gridDim.x;
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
 #pragma unroll
   for (int i = 0; i < kAwStages - 1; ++i) copy(i);
-  int stage = 0, ti = aw_tensor_of(tab, static_cast<int64_t>(blockIdx.x));
+  int stage = 0, ti = aw_tensor_of(tab, blockIdx.x);
 #pragma unroll 1
   for (int64_t chunk = blockIdx.x; chunk < tab.chunks; chunk += gridDim.x) {
     // The stage read last takes the chunk kAwStages - 1 ahead.
@@ -507,13 +498,15 @@ __global__ void __launch_bounds__(kAwThreads, kAwCtas8) adamw8_step(const __grid
     stage = stage + 1 == kAwStages ? 0 : stage + 1;
     while (ti + 1 < tab.count && tab.t[ti + 1].chunk0 <= chunk) ++ti;
     const AwTensor& t = tab.t[ti];
-    const int64_t at = (chunk - t.chunk0) * kAwChunk;
-    if (!aw_whole<T, MASTER>(t, chunk - t.chunk0)) {
+    const int i = static_cast<int>(chunk) - t.chunk0;
+    const int64_t at = static_cast<int64_t>(i) * kAwChunk;
+    if (i >= t.whole) {
       if (at + warp * kAwBlock < t.n) aw_block<T, MASTER, true>(t, c, gs, at + warp * kAwBlock);
       continue;
     }
     const uint64_t e = static_cast<uint64_t>(t.block0) * kAwBlock + at;
-    const uint32_t idx = (static_cast<uint32_t>(e) + off) ^ aw_key(c.seed, c.step, static_cast<uint32_t>(e >> 32));
+    const uint32_t key = (e >> 32) == 0 ? c.key : aw_key(c.seed, c.step, static_cast<uint32_t>(e >> 32));
+    const uint32_t idx = (static_cast<uint32_t>(e) + off) ^ key;
     const float ms0 = in.ms[threadIdx.x], vs0 = in.vs[threadIdx.x];
     uint4 graw[Stage::kG / 16], praw[Stage::kP / 16];
 #pragma unroll

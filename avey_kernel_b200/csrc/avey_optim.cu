@@ -65,7 +65,7 @@ template <typename T, bool MASTER, bool Q8, int N>
 int launch(const AveyAdamWTensor* t, int count, int64_t* block0, const avey::AwScalars& c, cudaStream_t stream) {
   avey::AwTable<N> tab;
   tab.count = 0;
-  tab.chunks = 0;
+  int64_t chunks = 0;
   for (int i = 0; i < count; ++i) {
     if (t[i].numel == 0) continue;
     avey::AwTensor& e = tab.t[tab.count++];
@@ -78,10 +78,16 @@ int launch(const AveyAdamWTensor* t, int count, int64_t* block0, const avey::AwS
     e.master = t[i].master;
     e.n = t[i].numel;
     e.block0 = *block0;
-    e.chunk0 = tab.chunks;
+    e.chunk0 = static_cast<int32_t>(chunks);
+    uintptr_t at = (reinterpret_cast<uintptr_t>(e.p) | reinterpret_cast<uintptr_t>(e.g)) & (8 * sizeof(T) - 1);
+    at |= (reinterpret_cast<uintptr_t>(e.m) | reinterpret_cast<uintptr_t>(e.v)) & 7u;
+    if (MASTER) at |= reinterpret_cast<uintptr_t>(e.master) & 31u;
+    e.whole = at == 0 ? static_cast<int32_t>(t[i].numel / avey::kAwChunk) : 0;
     *block0 += (t[i].numel + avey::kAwBlock - 1) / avey::kAwBlock;
-    tab.chunks += (t[i].numel + avey::kAwChunk - 1) / avey::kAwChunk;
+    chunks += (t[i].numel + avey::kAwChunk - 1) / avey::kAwChunk;
+    if (chunks > (1 << 30)) return fail(AVEY_ERR_ARGUMENT, "more than 2^41 elements in a launch");
   }
+  tab.chunks = static_cast<int>(chunks);
   if (tab.chunks == 0) return AVEY_OK;
   const int64_t sms = avey_host::multiprocessors();
   if constexpr (Q8) {
@@ -155,6 +161,7 @@ extern "C" int avey_adamw_v1(const AveyAdamWParams* p, void* stream) {
   c.minus_zerop = twice(-0.f);
   c.seed = static_cast<uint32_t>(p->seed);
   c.step = static_cast<uint32_t>(p->step);
+  c.key = avey::aw_key(c.seed, c.step, 0);
   c.grad_scale = p->grad_scale;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   switch (p->dtype) {
