@@ -62,9 +62,9 @@ int validate(const AveyLinearParams* p, bool backward) {
   if (p->activation < 0 || p->activation > 4) return fail(AVEY_ERR_ARGUMENT, "unknown activation");
   if (p->kernel < AVEY_LINEAR_KERNEL_AUTO || p->kernel > AVEY_LINEAR_KERNEL_FEW)
     return fail(AVEY_ERR_ARGUMENT, "unknown linear kernel");
-  if (p->rows < 0 || p->rows > (1 << 30) || p->d_in < 1 || p->d_in > (1 << 24) || p->d_out < 1 ||
-      p->d_out > (1 << 24) || p->groups < 1 || p->groups > 65535)
-    return fail(AVEY_ERR_ARGUMENT, "rows must be in [0, 2^30], d_in and d_out in [1, 2^24], groups in [1, 65535]");
+  if (p->rows < 0 || p->rows > (1 << 30) || p->d_in < 1 || p->d_in > (1 << 22) || p->d_out < 1 ||
+      p->d_out > (1 << 22) || p->groups < 1 || p->groups > 65535)
+    return fail(AVEY_ERR_ARGUMENT, "rows must be in [0, 2^30], d_in and d_out in [1, 2^22], groups in [1, 65535]");
   if (!p->offsets && p->groups != 1) return fail(AVEY_ERR_ARGUMENT, "more than one group needs offsets");
   if ((p->rows + 127) / 128 + p->groups > (1ll << 30) / ((std::max(p->d_in, p->d_out) + 63) / 64))
     return fail(AVEY_ERR_ARGUMENT, "too many output tiles");

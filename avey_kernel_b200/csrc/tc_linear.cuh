@@ -368,6 +368,7 @@ __device__ __forceinline__ void ln_tile_taken(const LnGeom& q, LnCtrl* ctrl, int
 template <int MODE>
 __device__ __forceinline__ bool ln_warp_tile(const LnGeom& q, LnCtrl* ctrl, int i, LnTile& c) {
   const bool ok = __all_sync(0xFFFFFFFFu, ln_tile<MODE>(q, ctrl, i, c));
+  __syncwarp();  // every lane has read the slot
   if (ok && (threadIdx.x & 31) == 0) ln_tile_taken(q, ctrl, i);
   return ok;
 }

@@ -5,6 +5,7 @@
 // there is one loaded library in a process. Bad arguments raise ValueError;
 // a non-OK AveyStatus is returned and raised by the Python side.
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/autograd/variable.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/extension.h>
 
@@ -169,7 +170,11 @@ int adamw_step(const py::object& params, const py::object& grads, const py::obje
     a.grad_scale = static_cast<const float*>(grad_scale->const_data_ptr());
   }
   const c10::cuda::CUDAGuard guard(device);
-  return lib.adamw(&a, at::cuda::getCurrentCUDAStream().stream());
+  const int status = lib.adamw(&a, at::cuda::getCurrentCUDAStream().stream());
+  // Autograd sees that the parameters changed, as after any in-place operation.
+  if (status == AVEY_OK)
+    for (Py_ssize_t i = 0; i < n; ++i) torch::autograd::impl::bump_version(p[i]);
+  return status;
 }
 
 // ------------------------------------------------------------ linear layers

@@ -423,7 +423,7 @@ typedef struct AveyLinearParams {
   int32_t dtype;        /* AVEY_BF16 or AVEY_F16 */
   int32_t activation;   /* AveyActivation */
   int32_t kernel;       /* AVEY_LINEAR_KERNEL_* (forward) */
-  int64_t rows, d_in, d_out, groups;
+  int64_t rows, d_in, d_out, groups; /* up to 2^30, 2^22, 2^22 and 65535 */
   const int32_t* offsets;
   const void* x;
   int64_t x_ld;

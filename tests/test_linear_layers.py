@@ -278,6 +278,32 @@ def test_streams_and_graphs():
 
 
 @pytest.mark.gpu
+def test_arrays_past_2_to_the_31_elements():
+    rows, k, n = (1 << 21) + 77, 1032, 64  # x and dx hold 2^31 + 1.7 10^7 elements
+    w, b, dt = data(1, k, n, torch.bfloat16, 15)[1], None, torch.bfloat16
+    x = torch.zeros(rows, k, dtype=dt, device='cuda')
+    dy = torch.zeros(rows, n, dtype=dt, device='cuda')
+    last = data(200, k, n, dt, 16)
+    x[-200:], dy[-200:] = last[0], last[4]
+    y, (dx, dw, _, _) = run_linear(x, w, b, None, dy, 'silu')
+    want = reference(last[0], w, b, None, last[4], 'silu', dt)
+    close(y[-200:], want['y'], 'y')
+    close(dx[-200:], want['dx'], 'dx')
+    close(dw, want['dw'], 'dw')  # the other rows add nothing
+    assert not y[:-200].any() and not dx[:-200].any()
+
+
+@pytest.mark.gpu
+def test_compiled_functions_call_the_operators():
+    x, w, b, r, _ = data(100, 64, 72, torch.bfloat16, 17)
+
+    def f(x):
+        return layers.residual_linear(x * 2, w, b, activation='silu', residual=r) + 1
+
+    assert torch.equal(torch.compile(f)(x), f(x))
+
+
+@pytest.mark.gpu
 def test_empty_batches():
     x, w, b, r, dy = data(0, 64, 72, torch.bfloat16)
     y, (dx, dw, db, dr) = run_linear(x, w, b, r, dy, 'silu')

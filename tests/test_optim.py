@@ -311,6 +311,16 @@ def test_runs_on_the_current_stream_and_in_a_graph():
     assert torch.equal(s['params'][0], ref['params'][0]) and torch.equal(s['exp_avgs'][1], ref['exp_avgs'][1])
 
 
+@pytest.mark.parametrize('device', DEVICES)
+def test_autograd_notices_that_parameters_changed(device):
+    w = torch.nn.Parameter(torch.ones(4, device=device))
+    loss = (w * w).sum()
+    loss.backward(retain_graph=True)
+    optim.AdamW([w], lr=0.1).step()
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        loss.backward()
+
+
 def _train(device, steps, **kw):
     """A small least-squares fit; its loss after `steps` steps."""
     g = torch.Generator().manual_seed(0)
