@@ -21,13 +21,13 @@ constexpr int kMaxDevices = 64;
 
 // Opt kernel K into its shared memory, once per device; the outcome is kept.
 template <auto K>
-cudaError_t smem_opt_in() {
+cudaError_t smem_opt_in(int bytes = avey::kLnSmem) {
   static std::once_flag once[kMaxDevices];
   static cudaError_t err[kMaxDevices];
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return cudaErrorInvalidDevice;
-  std::call_once(once[dev], [dev] {
-    err[dev] = cudaFuncSetAttribute(K, cudaFuncAttributeMaxDynamicSharedMemorySize, avey::kLnSmem);
+  std::call_once(once[dev], [dev, bytes] {
+    err[dev] = cudaFuncSetAttribute(K, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
   });
   return err[dev];
 }
@@ -90,12 +90,12 @@ int validate(const AveyLinearParams* p, bool backward) {
   return AVEY_OK;
 }
 
-// AUTO: dense layers of 1 to 64 rows finish sooner there (64 rows, 768 -> 1536:
-// 5.3 against 7.9 us; 4096 -> 4096: 17.0 against 22.8), of 128 rows no longer
-// (4096 -> 4096: 30.7 against 23.0). Grouped ones too, while the weights that
-// the rows can touch stay below about 100 MB (64 rows of 8 experts, 768 -> 1536:
-// 8.3 against 12.7 us; 64 of 16, 1024 -> 2048: 13.0 against 12.8; 64 of 64: 45
-// against 36).
+// AUTO: dense layers of up to 64 rows finish sooner there or as soon (one row,
+// 768 -> 1536: 2.4 against 5.5 us; 64 rows: 5.2 against 5.9, 4096 -> 4096 17.0
+// against 16.9), of 128 rows later (8.9 against 6.9 us). Grouped ones too, while
+// the weights that the rows can touch stay below about 100 MB (64 rows of 8
+// experts, 768 -> 1536: 8.2 against 12.7 us; 64 of 16, 1024 -> 2048: 13.0 against
+// 12.9; 64 of 64: 45 against 36).
 bool use_few(const AveyLinearParams* p) {
   if (p->kernel != AVEY_LINEAR_KERNEL_AUTO) return p->kernel == AVEY_LINEAR_KERNEL_FEW;
   return p->rows <= kFewRows && std::min(p->groups, p->rows) * p->d_in * p->d_out <= 48ll << 20;
@@ -229,6 +229,44 @@ int launch_tc(const Maps& m, const avey::LnGeom& q, int64_t tiles, cudaStream_t 
   return launched("tc_linear");
 }
 
+// CTAs that share a 128 x 64 tile's K blocks (1: the persistent kernel): enough
+// for the SMs where such tiles are fewer than half of them, of two blocks each
+// at least. 128 rows, 2048 -> 1024: 8.9 us (8 CTAs a tile) against 13.6 by
+// one CTA a tile; 768 -> 1536: 6.9 (4 CTAs) against 7.7.
+int split_ctas(const AveyLinearParams* p) {
+  const int64_t tiles = (row_tiles(p, avey::kLnBM) + (p->offsets ? 1 : 0)) * ((p->d_out + avey::kLsBN - 1) / avey::kLsBN);
+  const int64_t blocks = (p->d_in + avey::kLnBK - 1) / avey::kLnBK;
+  int ctas = 1;
+  while (ctas < 8 && tiles * ctas * 2 <= avey_host::multiprocessors() && blocks >= 4 * ctas) ctas *= 2;
+  return ctas;
+}
+
+template <auto K>
+int launch_split(const CUtensorMap& a, const CUtensorMap& b, avey::LnGeom q, int64_t tiles, int ctas,
+                 cudaStream_t stream) {
+  q.bn = avey::kLsBN;
+  q.n_nt = (q.n + avey::kLsBN - 1) / avey::kLsBN;
+  q.stages = std::min<int>(avey::kLnMaxStages, ((q.kc + avey::kLnBK - 1) / avey::kLnBK + ctas - 1) / ctas);
+  const cudaError_t attr = smem_opt_in<K>(avey::ls_smem(avey::kLnMaxStages));
+  if (attr != cudaSuccess) return fail(AVEY_ERR_CUDA, cudaGetErrorString(attr));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(tiles * ctas));
+  cfg.blockDim = dim3(avey::kLsThreads);
+  cfg.dynamicSmemBytes = static_cast<size_t>(avey::ls_smem(q.stages));
+  cfg.stream = stream;
+  cudaLaunchAttribute cluster[1];
+  cluster[0].id = cudaLaunchAttributeClusterDimension;
+  cluster[0].val.clusterDim.x = static_cast<unsigned>(ctas);
+  cluster[0].val.clusterDim.y = 1;
+  cluster[0].val.clusterDim.z = 1;
+  cfg.attrs = cluster;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, K, a, b, q, ctas);
+  if (e != cudaSuccess) return fail(AVEY_ERR_LAUNCH, cudaGetErrorString(e));
+  avey_host::count_launches(1);
+  return AVEY_OK;
+}
+
 template <typename T, int ACT>
 int forward_tc(const AveyLinearParams* p, cudaStream_t stream) {
   const Layout l = layout(p, false);
@@ -238,7 +276,8 @@ int forward_tc(const AveyLinearParams* p, cudaStream_t stream) {
   int rc = pack_inputs(p, l, &x, &w, stream);
   if (rc != AVEY_OK) return rc;
   const int64_t mt = row_tiles(p, avey::kLnBM);
-  avey::LnGeom q = geom(p, p->d_out, tile_cols(mt, p->d_out));
+  const int ctas = split_ctas(p);
+  avey::LnGeom q = geom(p, p->d_out, ctas > 1 ? avey::kLsBN : tile_cols(mt, p->d_out));
   q.kc = static_cast<int>(p->d_in);
   q.out = p->y;
   q.out_ld = p->y_ld;
@@ -259,6 +298,11 @@ int forward_tc(const AveyLinearParams* p, cudaStream_t stream) {
   if (rc != AVEY_OK) return rc;
   // One more row tile than the groups': the rows past the last group.
   const int64_t tiles = (mt + (p->offsets ? 1 : 0)) * q.n_nt;
+  if (ctas > 1) {
+    if constexpr (ACT != AVEY_ACT_IDENTITY)
+      if (p->deriv) return launch_split<avey::tc_linear_split<T, ACT, true>>(m.a, m.b, q, tiles, ctas, stream);
+    return launch_split<avey::tc_linear_split<T, ACT, false>>(m.a, m.b, q, tiles, ctas, stream);
+  }
   if constexpr (ACT != AVEY_ACT_IDENTITY)
     if (p->deriv) return launch_tc<avey::tc_linear<T, avey::kLnForward, ACT, true>>(m, q, tiles, stream);
   return launch_tc<avey::tc_linear<T, avey::kLnForward, ACT, false>>(m, q, tiles, stream);

@@ -888,4 +888,177 @@ __global__ void __launch_bounds__(kLnThreads, 1)
   }
 }
 
+// ============================================================================
+// The forward pass where 128 x 64 tiles are too few for the SMs: a cluster of 2,
+// 4 or 8 CTAs shares one tile's K blocks. A CTA takes in only some 70 GB/s from
+// L2, so a tile alone takes 0.35 us a K block; each CTA of a cluster
+// accumulates its share in TMEM and lays it down in shared memory, and after a
+// cluster barrier every CTA finishes a part of the tile from the sums of all
+// (distributed shared memory, in the order of the CTAs). One tile a cluster.
+constexpr int kLsThreads = 256;
+constexpr int kLsBN = 64;
+constexpr int kLsStageBytes = kLnABytes + kLsBN * kLnBK * 2;  // 24 KB
+constexpr int kLsRow = kLsBN + 4;  // floats between rows of the sums: no bank conflicts
+constexpr int kLsSums = kLnBM * kLsRow * 4;
+constexpr int kLsCtrlBytes = 256;
+// Dynamic shared memory for a ring of `stages`; the sums reuse it.
+__host__ __device__ constexpr int ls_ring(int stages) {
+  return stages * kLsStageBytes > kLsSums ? stages * kLsStageBytes : kLsSums;
+}
+__host__ __device__ constexpr int ls_smem(int stages) { return 1024 + ls_ring(stages) + kLsCtrlBytes; }
+
+struct LsCtrl {
+  uint64_t full[kLnMaxStages], empty[kLnMaxStages];
+  uint64_t done;
+  uint32_t tmem_base;
+};
+static_assert(sizeof(LsCtrl) <= kLsCtrlBytes, "control block too large");
+
+__device__ __forceinline__ float4 ls_peer_ld(uint32_t addr, uint32_t rank) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(mapa_shared(addr, rank)));
+  return v;
+}
+
+template <typename T, int ACT, bool DERIV>
+__global__ void __launch_bounds__(kLsThreads)
+    tc_linear_split(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                    const LnGeom q, int ctas) {
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int rank = static_cast<int>(blockIdx.x) % ctas;
+  LnTile c;
+  {
+    const int t = static_cast<int>(blockIdx.x) / ctas;
+    if (q.offsets) {
+      LnWalker<kLnForward> w;
+      if (!w.seek(q, t, c)) return;  // the cluster's CTAs agree
+    } else {
+      ln_set_tile<kLnForward>(q, c, 0, 0, q.rows, t);
+    }
+  }
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t base = (raw + 1023u) & ~1023u;
+  LsCtrl* ctrl = reinterpret_cast<LsCtrl*>(smem_raw + (base - raw) + ls_ring(q.stages));
+  const int k0 = c.nk * rank / ctas, nk = c.nk * (rank + 1) / ctas - k0;
+  if (tid == 0) {
+    for (int s = 0; s < q.stages; ++s) {
+      mbar_init(smem_u32(&ctrl->full[s]), 1);
+      mbar_init(smem_u32(&ctrl->empty[s]), 1);
+    }
+    mbar_init(smem_u32(&ctrl->done), 1);
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(&ctrl->tmem_base), kLsBN);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = ctrl->tmem_base;
+  if (warp == 0 && lane == 0) {
+    const uint64_t keep = l2_policy_evict_last();
+    for (int kk = 0; kk < nk; ++kk) {
+      const int st = kk % q.stages;
+      if (kk >= q.stages && !mbar_wait(smem_u32(&ctrl->empty[st]), (kk / q.stages - 1) & 1)) break;
+      const uint32_t full = smem_u32(&ctrl->full[st]);
+      const uint32_t sa = base + st * kLsStageBytes;
+      mbar_arrive_expect_tx(full, kLsStageBytes);
+      tma_load_3d_hint(sa + kLnABytes, &map_b, full, (k0 + kk) * kLnBK, c.nt * kLsBN, c.g, keep);
+      tma_load_3d_hint(sa, &map_a, full, (k0 + kk) * kLnBK, c.row0, 0, keep);
+    }
+  } else if (warp == 1 && lane == 0) {
+    const uint32_t idesc = idesc_f16(std::is_same<T, __nv_bfloat16>::value ? 1u : 0u, kLnBM, kLsBN, 0u, 0u);
+    const uint64_t da0 = smem_desc_sw128(base, 16, 1024), db0 = smem_desc_sw128(base + kLnABytes, 16, 1024);
+    bool alive = true;
+    for (int kk = 0; alive && kk < nk; ++kk) {
+      const int st = kk % q.stages;
+      alive = mbar_wait(smem_u32(&ctrl->full[st]), (kk / q.stages) & 1);
+      if (!alive) break;
+      tc_fence_after();
+      const uint32_t adv = static_cast<uint32_t>(st * kLsStageBytes) >> 4;
+#pragma unroll
+      for (int k = 0; k < kLnBK / 16; ++k)
+        tc_mma_f16(tmem, da0 + adv + 2 * k, db0 + adv + 2 * k, idesc, (kk != 0 || k != 0) ? 1u : 0u);
+      tc_commit(smem_u32(&ctrl->empty[st]));
+    }
+    if (alive && nk > 0) tc_commit(smem_u32(&ctrl->done));
+    else mbar_arrive(smem_u32(&ctrl->done));
+  }
+  __syncwarp();
+  // Every product has read its operands when `done` completes: the ring is free.
+  ln_warp_wait(smem_u32(&ctrl->done), 0);
+  tc_fence_after();
+  const int wq = warp & 3, h = warp >> 2;
+  if (c.row0 + wq * 32 < c.hi) {
+    const uint32_t p = base + static_cast<uint32_t>((wq * 32 + lane) * kLsRow + h * 32) * 4;
+#pragma unroll
+    for (int hh = 0; hh < 2; ++hh) {
+      uint32_t o[16];
+      ln_tmem_ld16(tmem + (static_cast<uint32_t>(wq * 32) << 16) + static_cast<uint32_t>(h * 32 + hh * 16), nk == 0, o);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) ln_sts(p + hh * 64 + i * 16, o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+    }
+  }
+  tc_fence_before();
+  cluster_sync();  // all sums are in place (and this CTA's accumulator has been read)
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kLsBN);
+  }
+  const int rows = min(kLnBM, c.hi - c.row0);
+  const bool zero = c.g >= q.groups;
+  for (int i = rank * kLsThreads + tid; i < rows * (kLsBN / 4); i += ctas * kLsThreads) {
+    const int r = i / (kLsBN / 4), tc = i % (kLsBN / 4) * 4;
+    const int64_t row = c.row0 + r;
+    const int col = c.nt * kLsBN + tc;
+    if (col >= q.n) continue;
+    const uint32_t at = base + static_cast<uint32_t>(r * kLsRow + tc) * 4;
+    float z[4] = {0.f, 0.f, 0.f, 0.f};
+    if (!zero) {
+      for (int k = 0; k < ctas; ++k) {
+        const float4 v = ls_peer_ld(at, static_cast<uint32_t>(k));
+        z[0] += v.x;
+        z[1] += v.y;
+        z[2] += v.z;
+        z[3] += v.w;
+      }
+      const T* bias = q.bias ? static_cast<const T*>(q.bias) + static_cast<int64_t>(c.g) * q.bias_gs + col : nullptr;
+      const T* res = q.res ? static_cast<const T*>(q.res) + row * q.res_ld + col : nullptr;
+      uint32_t codes[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const bool one = col + 2 * j < q.n, two = col + 2 * j + 1 < q.n;
+        if (bias) {
+          if (one) z[2 * j] = __fadd_rn(z[2 * j], Elem<T>::to_f(bias[2 * j]));
+          if (two) z[2 * j + 1] = __fadd_rn(z[2 * j + 1], Elem<T>::to_f(bias[2 * j + 1]));
+        }
+        LnPair d;
+        const float2 y = ln_split(ln_act2<ACT, DERIV>(ln_pair(z[2 * j], z[2 * j + 1]), &d));
+        if (DERIV) codes[j] = ln_encode2<T, ACT>(d);
+        z[2 * j] = y.x;
+        z[2 * j + 1] = y.y;
+        if (res) {
+          if (one) z[2 * j] = __fadd_rn(z[2 * j], Elem<T>::to_f(res[2 * j]));
+          if (two) z[2 * j + 1] = __fadd_rn(z[2 * j + 1], Elem<T>::to_f(res[2 * j + 1]));
+        }
+      }
+      if (DERIV)  // rows of codes are whole 32-byte units: past n lies padding
+        *reinterpret_cast<uint2*>(q.deriv + row * q.deriv_ld + col) = make_uint2(codes[0], codes[1]);
+    }
+    T* out = static_cast<T*>(q.out) + row * q.out_ld + col;
+    if (q.out_vec && col + 4 <= q.n) {
+      *reinterpret_cast<uint2*>(out) = make_uint2(ln_pack<T>(z[0], z[1]), ln_pack<T>(z[2], z[3]));
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (col + j < q.n) out[j] = Elem<T>::from_f(z[j]);
+    }
+  }
+  cluster_sync();  // the peers have read this CTA's sums
+}
+
 }  // namespace avey
