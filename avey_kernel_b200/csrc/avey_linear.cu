@@ -396,6 +396,9 @@ int backward(const AveyLinearParams* p, cudaStream_t stream) {
   Rows x, w, g{p->dy, p->dy_ld, 0};
   int rc = pack_inputs(p, l, &x, &w, stream);
   if (rc != AVEY_OK) return rc;
+  // An idle warp of the dX kernel adds up the bias gradient where that hides
+  // behind the products (1024 partial rows take it about 20 us).
+  const bool sum_in_dx = l.sums && p->dx && p->rows <= 65536;
   if (l.make_dpre || l.sums) {
     avey::LnDpre q{};
     q.offsets = p->offsets;
@@ -415,10 +418,10 @@ int backward(const AveyLinearParams* p, cudaStream_t stream) {
     if (l.sums) q.partial = reinterpret_cast<float*>(ws + l.partial);
     rc = launch_dpre<T>(q, p->activation, row_tiles(p, avey::kLdRows), stream);
     if (rc != AVEY_OK) return rc;
-    if (l.sums) {
+    if (l.sums && !sum_in_dx) {
       const dim3 grid(static_cast<unsigned>((p->d_out + 31) / 32), static_cast<unsigned>(p->groups));
       avey::ln_bias_sum<T><<<grid, avey::kLbThreads, 0, stream>>>(p->offsets, q.groups, q.rows, q.n, q.partial,
-                                                     static_cast<T*>(p->dbias));
+                                                                  static_cast<T*>(p->dbias));
       rc = launched("ln_bias_sum");
       if (rc != AVEY_OK) return rc;
     }
@@ -430,6 +433,10 @@ int backward(const AveyLinearParams* p, cudaStream_t stream) {
     q.out = p->dx;
     q.out_ld = p->dx_ld;
     q.out_vec = whole_rows(p->dx, p->dx_ld);
+    if (sum_in_dx) {
+      q.bias_sums = reinterpret_cast<const float*>(ws + l.partial);
+      q.db = p->dbias;
+    }
     Maps m;
     rc = avey_host::encode_rows16(p->dtype, g.p, p->d_out, p->rows, 1, g.ld * 2, 0, avey::kLnBM, &m.a);
     if (rc == AVEY_OK)

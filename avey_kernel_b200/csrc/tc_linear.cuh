@@ -17,12 +17,20 @@
 // so a tile's epilogue overlaps the next tile's products; warp 2 clears the
 // rows of a neighbouring group out of dW's last K block. Every wait is bounded.
 //
-// The epilogue has as long as the products take: at d_in = 768 3072 cycles for
-// 32768 elements, 12 issue slots each. silu and gelu take two special-function
-// results each (4096 cycles a tile), so they are computed on packed pairs
-// (fma.rn.f32x2) with the code of act' by a magic-number sum, and sixteen warps
-// cover one another's latencies: with eight warps and scalar sums the forward
-// pass of 32768 x 768 x 1536 with silu, residual and codes took 185 us.
+// The epilogue has as long as the products take: at d_in = 768 6144 cycles for
+// 32768 elements, 24 issue slots each. silu and gelu take two special-function
+// results each (4096 cycles a tile), so they are computed on pairs (packed
+// fp32), with the code of act' by a magic-number sum, and sixteen warps cover one
+// another's latencies: with eight warps and scalar sums the forward pass of
+// 32768 x 768 x 1536 with silu, residual and codes took 185 us.
+//
+// Measured (bf16, one B200): 32768 x 768 x 1536 forward with bias and any
+// activation 70-74 us (1,050-1,110 TFLOP/s; torch.matmul 62-64), with residual 88,
+// for training with residual and codes 99-101 (350 MB moved, 3.5 TB/s); dX 66,
+// dW 67-69 and 4 for its partial sums; 8192 x 4096 x 4096 forward 183-191
+// (1,440-1,500 TFLOP/s; torch.matmul 179-207). Tiles of 128 columns instead of 256:
+// dX 89, dW 102 us, so what an SM takes in and reads back from shared memory for
+// its products is the bound of the bare product.
 #pragma once
 
 #include <cuda.h>
@@ -68,6 +76,8 @@ struct LnGeom {
   int res_vec;
   uint16_t* deriv;         // codes of act' [rows][deriv_ld], or null
   int64_t deriv_ld;        // a multiple of 16
+  const float* bias_sums;  // dX: partial sums of the bias gradient [tiles][kc], or null
+  void* db;                // its [groups][kc]
 };
 
 // ---------------------------------------------------------------- activations
@@ -245,6 +255,93 @@ struct LnTile {
   int k0, nk;      // dW: first row of the K range; all: K blocks
   int last;        // dW: rows in the last K block (kLnBK: whole, or past the tensor's end)
 };
+
+// ---------------------------------------------------------------- groups, by a warp
+
+struct LnSpan {
+  int g, lo, hi;  // group and its rows
+  int index;      // which of the group's tiles
+  int base, cnt;  // the group's first tile and its tiles
+};
+
+// Every lane of the warp: walk the groups 32 at a time, a group counting
+// count(lo, hi) items, and find the group that holds item t (t >= 0), or the
+// items of group `want` (t < 0). False when there is none.
+template <typename Count>
+__device__ __forceinline__ bool ln_find(const int32_t* offsets, int groups, int rows, int t, int want, Count count,
+                                        LnSpan& out) {
+  const int lane = threadIdx.x & 31;
+  int end_carry = 0, base = 0;
+  for (int g0 = 0; g0 < groups; g0 += 32) {
+    const int g = g0 + lane;
+    int hi = g < groups ? (offsets ? min(max(__ldg(offsets + g + 1), 0), rows) : rows) : 0;
+    hi = max(hi, end_carry);
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int o = __shfl_up_sync(0xFFFFFFFFu, hi, d);
+      if (lane >= d) hi = max(hi, o);
+    }
+    int lo = __shfl_up_sync(0xFFFFFFFFu, hi, 1);
+    if (lane == 0) lo = end_carry;
+    const int cnt = g < groups ? count(lo, hi) : 0;
+    int incl = cnt;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int o = __shfl_up_sync(0xFFFFFFFFu, incl, d);
+      if (lane >= d) incl += o;
+    }
+    const int excl = base + incl - cnt;
+    const bool mine = t >= 0 ? (t >= excl && t < excl + cnt) : g == want;
+    const unsigned hit = __ballot_sync(0xFFFFFFFFu, mine);
+    if (hit) {
+      const int src = __ffs(hit) - 1;
+      out.g = g0 + src;
+      out.lo = __shfl_sync(0xFFFFFFFFu, lo, src);
+      out.hi = __shfl_sync(0xFFFFFFFFu, hi, src);
+      out.base = __shfl_sync(0xFFFFFFFFu, excl, src);
+      out.cnt = __shfl_sync(0xFFFFFFFFu, cnt, src);
+      out.index = t - out.base;
+      return true;
+    }
+    end_carry = __shfl_sync(0xFFFFFFFFu, hi, 31);
+    base += __shfl_sync(0xFFFFFFFFu, incl, 31);
+  }
+  // Not found: the rows past the last group, and the items in all.
+  out.g = groups;
+  out.lo = end_carry;
+  out.hi = rows;
+  out.base = base;
+  out.cnt = 0;
+  out.index = t - base;
+  return false;
+}
+
+// Row tiles of ln_dpre, which writes the bias gradient's partial sums by them.
+constexpr int kLdRows = 64;
+__device__ __forceinline__ int ln_dpre_tiles(int lo, int hi) { return (hi - lo + kLdRows - 1) / kLdRows; }
+
+// db[g] for 32 columns from c0 by one warp: the sum of the group's partial rows in
+// a fixed order (part i of 32 takes every 32nd row, then the parts in turn).
+template <typename T>
+__device__ __forceinline__ void ln_bias_columns(const int32_t* offsets, int groups, int rows, int n,
+                                                const float* partial, T* db, int g, int c0) {
+  LnSpan s;
+  ln_find(offsets, groups, rows, -1, g, ln_dpre_tiles, s);
+  const int c = c0 + (threadIdx.x & 31);
+  if (c >= n) return;
+  float part[32];
+#pragma unroll
+  for (int j = 0; j < 32; ++j) part[j] = 0.f;
+  const float* p = partial + static_cast<int64_t>(s.base) * n + c;
+  for (int i = 0; i < s.cnt; i += 32)
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (i + j < s.cnt) part[j] += p[static_cast<int64_t>(i + j) * n];
+  float z = 0.f;
+#pragma unroll
+  for (int j = 0; j < 32; ++j) z += part[j];
+  db[static_cast<int64_t>(g) * n + c] = Elem<T>::from_f(z);
+}
 
 // Tiles of a group of the rows [lo, hi).
 template <int MODE>
@@ -807,6 +904,13 @@ __global__ void __launch_bounds__(kLnThreads, 1)
     // The last K block of a group may hold rows of the next one. They are
     // cleared in both operands (not only one: theirs may be infinite), up to
     // the next multiple of 16 rows, where the products of the block stop.
+    if (MODE == kLnGradX && q.bias_sums) {
+      // The bias gradient beside the products: a launch less.
+      const int cols = (q.kc + 31) / 32;
+      for (int64_t j = blockIdx.x; j < static_cast<int64_t>(cols) * q.groups; j += gridDim.x)
+        ln_bias_columns<T>(q.offsets, q.groups, q.rows, q.kc, q.bias_sums, static_cast<T*>(q.db),
+                           static_cast<int>(j / cols), static_cast<int>(j % cols) * 32);
+    }
     if (MODE == kLnGradW) {
       LnTile c;
       int64_t filled = 0;  // K blocks of this CTA before the tile
