@@ -959,6 +959,7 @@ int clear_error() { return ok(); }
 void count_launches(int n) { g_launches.fetch_add(static_cast<uint64_t>(n), std::memory_order_relaxed); }
 int device_ok() { return device_arch_ok(nullptr); }
 int multiprocessors() { return sm_count(); }
+bool test_stall() { return g_test_stall.load(std::memory_order_relaxed) != 0; }
 namespace {
 int encode_plain(int dtype, const void* base, uint64_t inner, uint64_t rows, uint64_t batch, uint64_t row_bytes,
                  uint64_t batch_bytes, uint32_t box_cols, uint32_t box_rows, CUtensorMapSwizzle swizzle,

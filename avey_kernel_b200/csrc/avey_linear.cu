@@ -212,6 +212,7 @@ avey::LnGeom geom(const AveyLinearParams* p, int64_t n, int bn) {
   q.splits = 1;
   q.stage_bytes = avey::kLnABytes + bn * avey::kLnBK * 2;
   q.stages = avey::kLnRing / q.stage_bytes;
+  q.test_stall = avey_host::test_stall();
   return q;
 }
 

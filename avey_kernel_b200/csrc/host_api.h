@@ -29,6 +29,9 @@ int encode_rows16(int dtype, const void* base, uint64_t inner, uint64_t rows, ui
 int encode_tiles(int dtype, void* base, uint64_t inner, uint64_t rows, uint64_t batch, uint64_t row_bytes,
                  uint64_t batch_bytes, CUtensorMap* map);
 
+// Test hook (avey_test_hooks_v1): launches are to stall.
+bool test_stall();
+
 // The status word (read, and reset with `clear`) and the wait limit of the
 // kernels of avey_linear.cu, on the current device; a cudaError_t.
 int linear_flags(unsigned int* flags, bool clear);

@@ -78,6 +78,7 @@ struct LnGeom {
   int64_t deriv_ld;        // a multiple of 16
   const float* bias_sums;  // dX: partial sums of the bias gradient [tiles][kc], or null
   void* db;                // its [groups][kc]
+  int test_stall;          // tests: the TMA lane asks for nothing
 };
 
 // ---------------------------------------------------------------- activations
@@ -436,6 +437,8 @@ struct LnCtrl {
   uint64_t acc_full[2], acc_empty[2];
   uint64_t partial;  // dW: a last K block with rows of the next group has landed
   uint64_t cleared;  // dW: warp 2 has cleared them
+  uint64_t settled;  // after a wait has given up: the products have ended
+  uint32_t failed;   // a wait of this CTA has given up
   uint32_t tmem_base;
 };
 static_assert(sizeof(LnCtrl) <= kLnCtrlBytes, "control block too large");
@@ -473,6 +476,19 @@ __device__ __forceinline__ bool ln_warp_tile(const LnGeom& q, LnCtrl* ctrl, int 
 // A wait by every lane of a warp: they go on, or give up, together.
 __device__ __forceinline__ bool ln_warp_wait(uint32_t bar, uint32_t parity) {
   return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity));
+}
+
+// Once a wait has given up: what is still under way, the products issued so far
+// and the TMA loads of the last `fills` K blocks, gets about a millisecond each to
+// end before the CTA's tensor memory and shared memory go.
+__device__ __forceinline__ void ln_settle(uint32_t bar, uint32_t parity) {
+  const long long start = clock64();
+  while (!mbar_try_wait(bar, parity) && clock64() - start < (1ll << 21)) {
+  }
+}
+__device__ __forceinline__ void ln_settle_loads(const uint64_t* full, int stages, int fills) {
+  for (int f = max(0, fills - stages); f < fills; ++f)
+    ln_settle(smem_u32(full + f % stages), static_cast<uint32_t>(f / stages) & 1u);
 }
 
 // ---------------------------------------------------------------- epilogue
@@ -787,6 +803,8 @@ __global__ void __launch_bounds__(kLnThreads, 1)
     }
     mbar_init(smem_u32(&ctrl->partial), 1);
     mbar_init(smem_u32(&ctrl->cleared), 1);
+    mbar_init(smem_u32(&ctrl->settled), 1);
+    ctrl->failed = 0;
     fence_mbar_init();
     tma_prefetch_desc(&map_a);
     tma_prefetch_desc(&map_b);
@@ -799,15 +817,16 @@ __global__ void __launch_bounds__(kLnThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = ctrl->tmem_base;
+  int fills = 0;  // K blocks that the TMA lane has asked for
 
   if (warp == 0) {
     // ============================================================ TMA producer
     if (lane == 0) {
       const uint64_t keep = l2_policy_evict_last();  // operands are read again by other tiles
       LnTile c;
-      int st = 0, fills = 0;
+      int st = 0;
       uint32_t ph = 0;
-      bool alive = true;
+      bool alive = !q.test_stall;
       for (int i = 0; alive && ln_tile<MODE>(q, ctrl, i, c); ++i) {
         ln_tile_taken(q, ctrl, i);
         for (int kk = 0; kk < c.nk; ++kk) {
@@ -859,7 +878,10 @@ __global__ void __launch_bounds__(kLnThreads, 1)
         ln_tile_taken(q, ctrl, it);
         const int buf = it & 1;
         if (it >= 2) {
-          if (!mbar_wait(smem_u32(&ctrl->acc_empty[buf]), ((it >> 1) - 1) & 1)) break;
+          if (!mbar_wait(smem_u32(&ctrl->acc_empty[buf]), ((it >> 1) - 1) & 1)) {
+            alive = false;
+            break;
+          }
           tc_fence_after();
         }
         const uint32_t d_tmem = tmem + static_cast<uint32_t>(buf * 256);
@@ -898,6 +920,7 @@ __global__ void __launch_bounds__(kLnThreads, 1)
         else
           tc_commit(smem_u32(&ctrl->acc_full[buf]));
       }
+      if (!alive) ctrl->failed = 1;
     }
   } else if (warp == 2) {
     // ============================================================ dW: rows of the next group
@@ -974,8 +997,10 @@ __global__ void __launch_bounds__(kLnThreads, 1)
       const uint32_t tb = tmem + lane_off + static_cast<uint32_t>(buf * 256 + h * ln_part(q));
       if (!ln_drain<T, MODE, ACT, FLAG>(q, &map_y, policy, c, next, has_next, tb, wq, h, lane, stage, bias_tile,
                                         smem_u32(&ctrl->acc_full[buf]), (it >> 1) & 1,
-                                        smem_u32(&ctrl->acc_empty[buf]), ahead))
+                                        smem_u32(&ctrl->acc_empty[buf]), ahead)) {
+        if (lane == 0) ctrl->failed = 1;
         break;
+      }
       more = has_next;
       c = next;
     }
@@ -986,6 +1011,14 @@ __global__ void __launch_bounds__(kLnThreads, 1)
   __syncwarp();
   tc_fence_before();
   __syncthreads();
+  if (ctrl->failed) {
+    if (tid == 0) ln_settle_loads(ctrl->full, q.stages, fills);
+    if (tid == 32) {  // the lane that issued the products
+      tc_commit(smem_u32(&ctrl->settled));
+      ln_settle(smem_u32(&ctrl->settled), 0);
+    }
+    __syncthreads();
+  }
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
@@ -1014,7 +1047,7 @@ __host__ __device__ constexpr int ls_smem(int stages) { return 1024 + ls_ring(st
 struct LsCtrl {
   uint64_t full[kLnMaxStages], empty[kLnMaxStages];
   uint64_t done;
-  uint32_t tmem_base;
+  uint32_t failed, tmem_base;
 };
 static_assert(sizeof(LsCtrl) <= kLsCtrlBytes, "control block too large");
 
@@ -1053,6 +1086,7 @@ __global__ void __launch_bounds__(kLsThreads)
       mbar_init(smem_u32(&ctrl->empty[s]), 1);
     }
     mbar_init(smem_u32(&ctrl->done), 1);
+    ctrl->failed = 0;
     fence_mbar_init();
   }
   if (warp == 1) {
@@ -1063,9 +1097,10 @@ __global__ void __launch_bounds__(kLsThreads)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = ctrl->tmem_base;
+  int fills = 0;
   if (warp == 0 && lane == 0) {
     const uint64_t keep = l2_policy_evict_last();
-    for (int kk = 0; kk < nk; ++kk) {
+    for (int kk = 0; kk < nk && !q.test_stall; ++kk, ++fills) {
       const int st = kk % q.stages;
       if (kk >= q.stages && !mbar_wait(smem_u32(&ctrl->empty[st]), (kk / q.stages - 1) & 1)) break;
       const uint32_t full = smem_u32(&ctrl->full[st]);
@@ -1089,12 +1124,15 @@ __global__ void __launch_bounds__(kLsThreads)
         tc_mma_f16(tmem, da0 + adv + 2 * k, db0 + adv + 2 * k, idesc, (kk != 0 || k != 0) ? 1u : 0u);
       tc_commit(smem_u32(&ctrl->empty[st]));
     }
-    if (alive && nk > 0) tc_commit(smem_u32(&ctrl->done));
+    if (!alive) ctrl->failed = 1;
+    if (nk > 0) tc_commit(smem_u32(&ctrl->done));  // when the products issued so far have ended
     else mbar_arrive(smem_u32(&ctrl->done));
   }
   __syncwarp();
   // Every product has read its operands when `done` completes: the ring is free.
-  ln_warp_wait(smem_u32(&ctrl->done), 0);
+  if (!ln_warp_wait(smem_u32(&ctrl->done), 0)) ln_settle(smem_u32(&ctrl->done), 0);
+  if (tid == 0 && ctrl->failed) ln_settle_loads(ctrl->full, q.stages, fills);
+  __syncwarp();
   tc_fence_after();
   const int wq = warp & 3, h = warp >> 2;
   if (c.row0 + wq * 32 < c.hi) {

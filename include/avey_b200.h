@@ -540,7 +540,8 @@ AVEY_API uint64_t avey_launch_count(void);
  * wait_limit_cycles: SM cycles after which a bounded wait on an mbarrier gives
  * up (<= 0 restores the default of about one second). stall != 0: later
  * launches of the fused tensor-core kernel start with their TMA and MMA warps
- * issuing nothing, so its compute warps' first wait runs out, the kernel
+ * issuing nothing, and those of the linear layers with their TMA lane issuing
+ * nothing, so the first wait for their work runs out, the kernel
  * raises AVEY_DEVFLAG_TIMEOUT, unwinds and returns (no trap, the context stays
  * usable). The wait limit applies to the current device; the stall flag to
  * the process. Not for production use. */

@@ -304,6 +304,33 @@ def test_compiled_functions_call_the_operators():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('rows', [100, 700])
+def test_a_wait_that_runs_out_sets_the_flag_and_the_next_call_is_right(rows):
+    """With the TMA lanes issuing nothing and a limit of 10^5 cycles, the products'
+    first wait runs out in every kernel (100 rows: the cluster kernel forward); the
+    calls return, the status word tells, and nothing is left behind."""
+    x, w, b, r, dy = data(rows, 256, 72, torch.bfloat16, 18)
+    off = torch.tensor([0, 30, rows - 10], device='cuda', dtype=torch.int32)
+    w2, b2 = torch.stack((w, w)), torch.stack((b, b))
+    want = run_linear(x, w, b, r, dy, 'silu')
+    want2 = run_experts(x, w2, off, b2, dy, 'silu')
+    assert _native.device_status(clear=True) == 0
+    try:
+        _native.test_hooks(100_000, stall=True)
+        run_linear(x, w, b, r, dy, 'silu')
+        assert _native.device_status(clear=True) & 1
+        run_experts(x, w2, off, b2, dy, 'silu')
+        assert _native.device_status(clear=True) & 1
+    finally:
+        _native.test_hooks()
+        _native.device_status(clear=True)
+    got, got2 = run_linear(x, w, b, r, dy, 'silu'), run_experts(x, w2, off, b2, dy, 'silu')
+    assert torch.equal(got[0], want[0]) and all(torch.equal(p, q) for p, q in zip(got[1], want[1]))
+    assert all(torch.equal(p, q) for p, q in zip(got2, want2))
+    assert _native.device_status() == 0
+
+
+@pytest.mark.gpu
 def test_empty_batches():
     x, w, b, r, dy = data(0, 64, 72, torch.bfloat16)
     y, (dx, dw, db, dr) = run_linear(x, w, b, r, dy, 'silu')
