@@ -296,6 +296,20 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
   return fn;
 }
 
+// A thread whose first CUDA call is a driver call has no current context yet (an
+// autograd worker, say): make the current device's primary one current and try
+// once more.
+template <typename F>
+CUresult with_context(F encode) {
+  CUresult r = encode();
+  if (r == CUDA_ERROR_INVALID_CONTEXT) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess && cudaFree(nullptr) == cudaSuccess)
+      r = encode();
+  }
+  return r;
+}
+
 // Encoded tensor maps, cached per process: a map is a pure function of its
 // encode arguments (device, base address, shape, strides, box, element type),
 // so callers that reuse buffers (training loops, graph warm-ups, benchmarks)
@@ -351,9 +365,10 @@ int encode_cached(int dtype, const void* base, const cuuint64_t (&dims)[3], cons
                                                      : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   cuuint64_t d[3] = {dims[0], dims[1], dims[2]};
   cuuint64_t st[2] = {strides[0], strides[1]};
-  const CUresult r = fn(map, dt, 3, const_cast<void*>(base), d, st, box, estr,
-                        CU_TENSOR_MAP_INTERLEAVE_NONE, swz,
-                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  const CUresult r = with_context([&] {
+    return fn(map, dt, 3, const_cast<void*>(base), d, st, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swz,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  });
   if (r != CUDA_SUCCESS) return fail(AVEY_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
   std::lock_guard<std::mutex> lock(c.mu);
   const int slot = c.used < MapCache::kEntries ? c.used++ : (c.next++ % MapCache::kEntries);
@@ -973,8 +988,10 @@ int encode_plain(int dtype, const void* base, uint64_t inner, uint64_t rows, uin
   const CUtensorMapDataType dt = dtype == AVEY_BF16  ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                  : dtype == AVEY_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                                                      : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-  const CUresult r = fn(map, dt, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                        swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  const CUresult r = with_context([&] {
+    return fn(map, dt, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  });
   if (r != CUDA_SUCCESS) return fail(AVEY_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
   return AVEY_OK;
 }

@@ -13,6 +13,7 @@ A relu's derivative may also flip where |pre| <= a. f16 adds 2^-25 to each
 rounding (half the spacing near zero)."""
 
 import ctypes
+import threading
 
 import pytest
 import torch
@@ -328,6 +329,27 @@ def test_a_wait_that_runs_out_sets_the_flag_and_the_next_call_is_right(rows):
     assert torch.equal(got[0], want[0]) and all(torch.equal(p, q) for p, q in zip(got[1], want[1]))
     assert all(torch.equal(p, q) for p, q in zip(got2, want2))
     assert _native.device_status() == 0
+
+
+@pytest.mark.gpu
+def test_the_first_call_of_a_thread():
+    """A layer without epilogue starts with tensor maps, a driver call, in a thread
+    that has no CUDA context yet; backward passes run in autograd's own threads."""
+    x, w, _, _, dy = data(200, 64, 72, torch.bfloat16, 19)
+    want, (dx, dw, _, _) = run_linear(x, w, None, None, dy, 'identity')
+    got = []
+
+    def call():
+        try:
+            got.append(run_linear(x, w, None, None, dy, 'identity'))
+        except Exception as e:  # seen by the assertions below
+            got.append(e)
+
+    t = threading.Thread(target=call)
+    t.start()
+    t.join()
+    y, grads = got[0]
+    assert torch.equal(y, want) and torch.equal(grads[0], dx) and torch.equal(grads[1], dw)
 
 
 @pytest.mark.gpu
