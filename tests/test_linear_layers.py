@@ -353,6 +353,15 @@ def test_the_first_call_of_a_thread():
 
 
 @pytest.mark.gpu
+def test_wide_layers_take_tiles_in_blocks_of_rows():
+    """More than 16 column tiles of 256 forward and in dX, with row tiles that do and
+    do not fill a block of 12."""
+    check_linear(1700, 72, 4200, torch.bfloat16, 'silu', seed=20)
+    check_linear(3000, 4200, 72, torch.bfloat16, 'identity', bias=False, residual=False, seed=21)
+    check_experts([1600, 0, 1541, 100], 40, 4360, torch.bfloat16, 'gelu', 50, seed=22)
+
+
+@pytest.mark.gpu
 def test_empty_batches():
     x, w, b, r, dy = data(0, 64, 72, torch.bfloat16)
     y, (dx, dw, db, dr) = run_linear(x, w, b, r, dy, 'silu')
