@@ -68,6 +68,15 @@ int validate(const AveyLinearParams* p, bool backward) {
   if (!p->offsets && p->groups != 1) return fail(AVEY_ERR_ARGUMENT, "more than one group needs offsets");
   if ((p->rows + 127) / 128 + p->groups > (1ll << 30) / ((std::max(p->d_in, p->d_out) + 63) / 64))
     return fail(AVEY_ERR_ARGUMENT, "too many output tiles");
+  if (p->kernel == AVEY_LINEAR_KERNEL_FEW && p->offsets && std::min(p->groups, p->rows) > 65534)
+    return fail(AVEY_ERR_ARGUMENT, "the kernel for few rows takes up to 65534 groups with rows");
+  uintptr_t odd = 0;
+  for (const void* a : {p->x, p->weight, p->bias, p->residual, p->dy, const_cast<const void*>(p->y),
+                        const_cast<const void*>(p->dx), const_cast<const void*>(p->dweight),
+                        const_cast<const void*>(p->dbias)})
+    odd |= reinterpret_cast<uintptr_t>(a) & 1u;
+  if (odd != 0 || (reinterpret_cast<uintptr_t>(p->offsets) & 3u) != 0)
+    return fail(AVEY_ERR_ARGUMENT, "arrays must be aligned to their elements");
   if (p->rows == 0 && !backward) return AVEY_OK;
   if (p->rows > 0 && !p->x) return fail(AVEY_ERR_ARGUMENT, "x is required");
   if (!p->weight) return fail(AVEY_ERR_ARGUMENT, "weight is required");
@@ -163,6 +172,15 @@ Layout layout(const AveyLinearParams* p, bool backward) {
   }
   l.total = at;
   return l;
+}
+
+int check_workspace(const AveyLinearParams* p, const Layout& l) {
+  if (l.total == 0) return AVEY_OK;
+  if (!p->workspace || p->workspace_bytes < l.total)
+    return fail(AVEY_ERR_ARGUMENT, "workspace is smaller than avey_linear_workspace_size");
+  if ((reinterpret_cast<uintptr_t>(p->workspace) & 255u) != 0)
+    return fail(AVEY_ERR_ARGUMENT, "workspace must be 256-byte aligned");
+  return AVEY_OK;
 }
 
 // The operands as the tensor cores read them.
@@ -271,10 +289,10 @@ int launch_split(const CUtensorMap& a, const CUtensorMap& b, avey::LnGeom q, int
 template <typename T, int ACT>
 int forward_tc(const AveyLinearParams* p, cudaStream_t stream) {
   const Layout l = layout(p, false);
-  if (l.total > 0 && (!p->workspace || p->workspace_bytes < l.total))
-    return fail(AVEY_ERR_ARGUMENT, "workspace is smaller than avey_linear_workspace_size");
+  int rc = check_workspace(p, l);
+  if (rc != AVEY_OK) return rc;
   Rows x, w;
-  int rc = pack_inputs(p, l, &x, &w, stream);
+  rc = pack_inputs(p, l, &x, &w, stream);
   if (rc != AVEY_OK) return rc;
   const int64_t mt = row_tiles(p, avey::kLnBM);
   const int ctas = split_ctas(p);
@@ -391,11 +409,11 @@ int launch_dpre(const avey::LnDpre& q, int activation, int64_t tiles, cudaStream
 template <typename T>
 int backward(const AveyLinearParams* p, cudaStream_t stream) {
   const Layout l = layout(p, true);
-  if (l.total > 0 && (!p->workspace || p->workspace_bytes < l.total))
-    return fail(AVEY_ERR_ARGUMENT, "workspace is smaller than avey_linear_workspace_size");
+  int rc = check_workspace(p, l);
+  if (rc != AVEY_OK) return rc;
   char* ws = static_cast<char*>(p->workspace);
   Rows x, w, g{p->dy, p->dy_ld, 0};
-  int rc = pack_inputs(p, l, &x, &w, stream);
+  rc = pack_inputs(p, l, &x, &w, stream);
   if (rc != AVEY_OK) return rc;
   // An idle warp of the dX kernel adds up the bias gradient where that hides
   // behind the products (1024 partial rows take it about 20 us).

@@ -57,6 +57,11 @@ int validate(const AveyAdamWParams* p) {
       return fail(AVEY_ERR_ARGUMENT, "param, grad, exp_avg and exp_avg_sq are required");
     if (p->state_bits == 8 && (!t.exp_avg_scale || !t.exp_avg_sq_scale))
       return fail(AVEY_ERR_ARGUMENT, "8-bit states need exp_avg_scale and exp_avg_sq_scale");
+    auto bits = [](const void* a) { return reinterpret_cast<uintptr_t>(a); };
+    const uintptr_t value = (bits(t.param) | bits(t.grad)) & (p->dtype == AVEY_F32 ? 3u : 1u);
+    uintptr_t word = bits(t.master) | bits(t.exp_avg_scale) | bits(t.exp_avg_sq_scale);
+    if (p->state_bits == 32) word |= bits(t.exp_avg) | bits(t.exp_avg_sq);
+    if (value != 0 || (word & 3u) != 0) return fail(AVEY_ERR_ARGUMENT, "arrays must be aligned to their elements");
   }
   return AVEY_OK;
 }

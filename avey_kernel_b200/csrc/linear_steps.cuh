@@ -284,6 +284,7 @@ template <typename T>
 __global__ void __launch_bounds__(256) ln_split_sum(const float* partial, int splits, int64_t rows, int n, int64_t ld,
                                                     T* out) {
   const int64_t per = ld / 4, total = rows * per, plane = rows * ld;
+  const bool vec = (n & 3) == 0 && (reinterpret_cast<uintptr_t>(out) & 7u) == 0;
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < total;
        i += static_cast<int64_t>(gridDim.x) * 256) {
     const int64_t row = i / per;
@@ -298,7 +299,7 @@ __global__ void __launch_bounds__(256) ln_split_sum(const float* partial, int sp
       z.w += v.w;
     }
     T* o = out + row * n + c;
-    if (c + 4 <= n && (n & 3) == 0) {
+    if (c + 4 <= n && vec) {
       *reinterpret_cast<uint2*>(o) = make_uint2(ln_pack<T>(z.x, z.y), ln_pack<T>(z.z, z.w));
     } else {
       const float v[4] = {z.x, z.y, z.z, z.w};

@@ -577,7 +577,8 @@ def _params(**kw):
     ('kernel', 3, 'kernel'), ('rows', -1, 'rows must'), ('d_in', 0, 'rows must'), ('groups', 0, 'rows must'),
     ('groups', 2, 'needs offsets'), ('x', 0, 'x is required'), ('weight', 0, 'weight is required'),
     ('x_ld', 63, 'strides'), ('weight_ld', 8, 'strides'), ('y', 0, 'y is required'), ('y_ld', 71, 'y is required'),
-    ('deriv', 1 << 21, 'identity has no derivative'), ('rows', 1 << 31, 'rows must')])
+    ('deriv', 1 << 21, 'identity has no derivative'), ('rows', 1 << 31, 'rows must'),
+    ('x', (1 << 20) + 1, 'aligned to their elements'), ('offsets', (1 << 20) + 2, 'aligned to their elements')])
 def test_c_entry_rejects_bad_arguments_before_any_launch(field, value, match):
     p = _params(**{field: value})
     before = _native.launch_count()
@@ -588,10 +589,45 @@ def test_c_entry_rejects_bad_arguments_before_any_launch(field, value, match):
 
 @pytest.mark.parametrize('change,match', [
     (dict(dy=0), 'dy is required'), (dict(dx_ld=10), 'dy is required'),
-    (dict(activation=3), 'needs deriv'), (dict(activation=3, deriv=(1 << 21) + 2), '32-byte aligned')])
+    (dict(activation=3), 'needs deriv'), (dict(activation=3, deriv=(1 << 21) + 2), '32-byte aligned'),
+    (dict(dweight=(1 << 21) + 1), 'aligned to their elements')])
 def test_c_backward_entry_rejects_bad_arguments(change, match):
     with pytest.raises(_native.NativeError, match=match):
         _native.linear(_params(**change), 0, backward=True)
+
+
+def test_few_row_kernel_refuses_more_groups_than_its_grid_has():
+    p = _params(kernel=_native.LINEAR_FEW, rows=65535, groups=65535, offsets=1 << 20, weight_group_stride=64 * 72)
+    with pytest.raises(_native.NativeError, match='up to 65534 groups'):
+        _native.linear(p, 0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('change,match', [
+    (dict(workspace=(1 << 21) + 128, workspace_bytes=1 << 20), '256-byte aligned'),
+    (dict(workspace=1 << 21, workspace_bytes=64), 'workspace is smaller'), (dict(), 'workspace is smaller')])
+def test_c_entry_rejects_a_workspace_before_any_launch(change, match):
+    p = _params(x=(1 << 20) + 2, **change)
+    before = _native.launch_count()
+    with pytest.raises(_native.NativeError, match=match):
+        _native.linear(p, 0)
+    assert _native.launch_count() == before
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('offset', [1, 2, 4])
+def test_c_backward_entry_takes_a_weight_gradient_at_any_alignment(offset):
+    """2000 rows split dW's contraction: the sums of its parts go to the array
+    as well as a whole tile's would."""
+    x, w, _, _, dy = data(2000, 64, 72, torch.bfloat16, 23)
+    _, (_, want, _, _) = run_linear(x, w, None, None, dy, 'identity')
+    room = torch.empty(72 * 64 + 8, dtype=torch.bfloat16, device='cuda')
+    p = _params(rows=2000, x=x.data_ptr(), weight=w.data_ptr(), dy=dy.data_ptr(), y=0, dx=0,
+                dweight=room.data_ptr() + 2 * offset)
+    ws = torch.empty(_native.linear_workspace_size(p, backward=True), dtype=torch.uint8, device='cuda')
+    p.workspace, p.workspace_bytes = ws.data_ptr(), ws.numel()
+    _native.linear(p, torch.cuda.current_stream().cuda_stream, backward=True)
+    assert torch.equal(room[offset:offset + 72 * 64].view(72, 64), want)
 
 
 def test_workspace_sizes():

@@ -467,6 +467,17 @@ def test_c_entry_rejects_bad_arguments_before_any_launch(field, value, match):
     assert info.value.status == -1 and _native.launch_count() == before
 
 
+@pytest.mark.parametrize('field,value,bits', [
+    ('param', (1 << 20) + 1, 32), ('grad', (2 << 20) + 1, 8), ('exp_avg', (3 << 20) + 2, 32),
+    ('exp_avg_scale', (5 << 20) + 2, 8), ('master', (6 << 20) + 2, 32)])
+def test_c_entry_wants_arrays_aligned_to_their_elements(field, value, bits):
+    p, t = _params(state_bits=bits)
+    t[0].exp_avg_scale = t[0].exp_avg_sq_scale = 5 << 20
+    setattr(t[0], field, value)
+    with pytest.raises(_native.NativeError, match='aligned to their elements'):
+        _native.adamw(p, 0)
+
+
 def test_c_entry_wants_masters_for_all_or_none():
     p, t = _params(count=2)
     two = (_native.AveyAdamWTensor * 2)(t[0], t[0])
