@@ -83,6 +83,9 @@ def _hash(start: int, n: int, seed: int, step: int) -> torch.Tensor:
 
 
 def _check_cpu(p, g, m, v, w):
+    # A dense tensor, and no other, gives its strides to empty_like.
+    if torch.empty_like(p, device='meta').stride() != p.stride() and p.numel() > 1:
+        raise ValueError('a parameter must be dense in memory')
     if g.shape != p.shape or g.dtype != p.dtype:
         raise ValueError('a gradient must have the shape and type of its parameter')
     for t in (m, v) if w is None else (m, v, w):
@@ -99,15 +102,18 @@ def _step_cpu(params, grads, exp_avgs, exp_avg_sqs, step, lr, beta1, beta2, eps,
     if any(len(x) != n for x in lists) or any(x is not None and len(x) != n
                                               for x in (masters, avg_scales, sq_scales)):
         raise ValueError('every list must hold one tensor for each parameter')
-    start = 0
+    quant = n > 0 and exp_avgs[0].dtype == torch.float8_e4m3fn
     for i, p in enumerate(params):
-        m, v = exp_avgs[i], exp_avg_sqs[i]
-        quant = m.dtype == torch.float8_e4m3fn
+        if any((x[i].dtype == torch.float8_e4m3fn) != quant for x in (exp_avgs, exp_avg_sqs)):
+            raise ValueError('the states of a step must have one type')
         if quant != (avg_scales is not None) or quant != (sq_scales is not None):
             raise ValueError('exp_avg_scales and exp_avg_sq_scales go with float8_e4m3fn states, '
                              'and only with them')
+        _check_cpu(p, grads[i], exp_avgs[i], exp_avg_sqs[i], None if masters is None else masters[i])
+    start = 0
+    for i, p in enumerate(params):
+        m, v = exp_avgs[i], exp_avg_sqs[i]
         w = None if masters is None else masters[i]
-        _check_cpu(p, grads[i], m, v, w)
         # Everything in the memory order of the parameter.
         g = torch.empty_like(p, dtype=torch.float32)
         g.copy_(grads[i])

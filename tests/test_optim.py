@@ -434,6 +434,14 @@ def test_step_rejects_what_it_cannot_take(change, match):
     assert _native.launch_count() == before
 
 
+@pytest.mark.parametrize('view', [lambda t: t[::2], lambda t: t[:, :3], lambda t: t[:1].expand(6, 8)])
+def test_cpu_step_refuses_parameters_that_are_not_dense(view):
+    p = view(torch.ones(6, 8))
+    m, v = (torch.empty_strided(p.shape, p.stride()).zero_() for _ in range(2))
+    with pytest.raises(ValueError, match='dense in memory'):
+        optim.adamw_step([p], [torch.ones(p.shape)], [m], [v], step=1, lr=0.1)
+
+
 @pytest.mark.gpu
 def test_8bit_states_need_the_right_scales():
     s = make([(600,)], torch.bfloat16, 'cuda', bits=8)
