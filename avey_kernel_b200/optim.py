@@ -261,14 +261,28 @@ class AdamW(torch.optim.Optimizer):
     def load_state_dict(self, state_dict):
         """As in torch, but the states keep their own types (torch casts them
         to the parameter's, which would round fp32 states of 16-bit
-        parameters and decode 8-bit ones)."""
+        parameters and decode 8-bit ones). States of a parameter whose layout in
+        memory has changed follow it; 8-bit ones, whose blocks go by that layout,
+        are rounded to the nearest codes of their new blocks."""
         super().load_state_dict(state_dict)
         ids = [i for g in state_dict['param_groups'] for i in g['params']]
         params = [p for g in self.param_groups for p in g['params']]
         for i, p in zip(ids, params):
-            for name, value in state_dict['state'].get(i, {}).items():
+            saved = state_dict['state'].get(i, {})
+            state = self.state[p]
+            for name, value in saved.items():
                 if isinstance(value, torch.Tensor):
-                    kept = value.detach().to(p.device, copy=True)
-                    if kept.shape == p.shape and kept.stride() != p.stride():
-                        kept = torch.empty_like(p, dtype=kept.dtype).copy_(kept)
-                    self.state[p][name] = kept
+                    state[name] = value.detach().to(p.device, copy=True)
+            for name in ('exp_avg', 'exp_avg_sq', 'master'):
+                old = state.get(name)
+                if old is None or old.stride() == p.stride() or old.shape != p.shape:
+                    continue
+                if old.dtype != torch.float8_e4m3fn:
+                    state[name] = torch.empty_like(p, dtype=old.dtype).copy_(old)
+                    continue
+                value = torch.empty_like(p, dtype=torch.float32)
+                value.copy_(dequantize(old, state[name + '_scale']))
+                half = torch.full((p.numel(),), 1 << 19, device=p.device)
+                codes, state[name + '_scale'] = _quantize(_memory_order(value), half)
+                state[name] = torch.empty_like(p, dtype=old.dtype)
+                _memory_order(state[name]).copy_(codes)

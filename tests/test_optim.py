@@ -390,6 +390,31 @@ def test_state_dict_round_trip_keeps_types_and_steps(bits, master, dtype):
         assert oa.state[p]['step'] == ob.state[q]['step'] == 4
 
 
+@pytest.mark.parametrize('bits', [32, 8])
+def test_state_dict_of_another_layout_follows_the_parameter(bits):
+    """8-bit values move by half a code at most: the codes of a block are 2^-3 of
+    their value or less apart, and 2^-9 of the block's maximum / 448 below 2^-6."""
+    g = torch.Generator().manual_seed(8)
+    w = torch.randn(40, 30, generator=g)
+    a, b = torch.nn.Parameter(w.clone()), torch.nn.Parameter(w.t().contiguous().t())
+    oa, ob = (optim.AdamW([p], lr=1e-2, state_bits=bits, seed=4) for p in (a, b))
+    a.grad = torch.randn(40, 30, generator=g)
+    oa.step()
+    ob.load_state_dict(oa.state_dict())
+    for name in ('exp_avg', 'exp_avg_sq'):
+        old, new = oa.state[a][name], ob.state[b][name]
+        assert new.dtype == old.dtype and new.stride() == b.stride()
+        if bits == 32:
+            assert torch.equal(new, old)
+            continue
+        want = optim.dequantize(old, oa.state[a][name + '_scale'])
+        got = optim.dequantize(new, ob.state[b][name + '_scale'])
+        top = want.abs().max() / 448
+        assert ((got - want).abs() <= want.abs() * 2.0 ** -4 * (1 + 2.0 ** -20) + top * 2.0 ** -10).all()
+    b.grad = a.grad.clone()
+    ob.step()
+
+
 def test_parameters_without_a_gradient_are_left_alone():
     p, q = torch.nn.Parameter(torch.ones(4)), torch.nn.Parameter(torch.ones(4))
     o = optim.AdamW([p, q], lr=0.1)
