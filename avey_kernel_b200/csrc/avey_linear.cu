@@ -239,13 +239,26 @@ struct Maps {
   CUtensorMap a{}, b{}, y{};
 };
 
+// `after`: the launch before this one on the stream is a step of the same call
+// that lets its dependents start early.
 template <auto K>
-int launch_tc(const Maps& m, const avey::LnGeom& q, int64_t tiles, cudaStream_t stream) {
-  const cudaError_t e = smem_opt_in<K>();
-  if (e != cudaSuccess) return fail(AVEY_ERR_CUDA, cudaGetErrorString(e));
-  const int grid = static_cast<int>(std::min<int64_t>(tiles, avey_host::multiprocessors()));
-  K<<<grid, avey::kLnThreads, avey::kLnSmem, stream>>>(m.a, m.b, m.y, q);
-  return launched("tc_linear");
+int launch_tc(const Maps& m, const avey::LnGeom& q, int64_t tiles, bool after, cudaStream_t stream) {
+  const cudaError_t attr = smem_opt_in<K>();
+  if (attr != cudaSuccess) return fail(AVEY_ERR_CUDA, cudaGetErrorString(attr));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(std::min<int64_t>(tiles, avey_host::multiprocessors())));
+  cfg.blockDim = dim3(avey::kLnThreads);
+  cfg.dynamicSmemBytes = avey::kLnSmem;
+  cfg.stream = stream;
+  cudaLaunchAttribute early[1];
+  early[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = early;
+  cfg.numAttrs = after ? 1 : 0;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, K, m.a, m.b, m.y, q);
+  if (e != cudaSuccess) return fail(AVEY_ERR_LAUNCH, cudaGetErrorString(e));
+  avey_host::count_launches(1);
+  return AVEY_OK;
 }
 
 // CTAs that share a 128 x 64 tile's K blocks (1: the persistent kernel): enough
@@ -261,7 +274,7 @@ int split_ctas(const AveyLinearParams* p) {
 }
 
 template <auto K>
-int launch_split(const CUtensorMap& a, const CUtensorMap& b, avey::LnGeom q, int64_t tiles, int ctas,
+int launch_split(const CUtensorMap& a, const CUtensorMap& b, avey::LnGeom q, int64_t tiles, int ctas, bool after,
                  cudaStream_t stream) {
   q.bn = avey::kLsBN;
   q.n_nt = (q.n + avey::kLsBN - 1) / avey::kLsBN;
@@ -273,13 +286,15 @@ int launch_split(const CUtensorMap& a, const CUtensorMap& b, avey::LnGeom q, int
   cfg.blockDim = dim3(avey::kLsThreads);
   cfg.dynamicSmemBytes = static_cast<size_t>(avey::ls_smem(q.stages));
   cfg.stream = stream;
-  cudaLaunchAttribute cluster[1];
+  cudaLaunchAttribute cluster[2];
   cluster[0].id = cudaLaunchAttributeClusterDimension;
   cluster[0].val.clusterDim.x = static_cast<unsigned>(ctas);
   cluster[0].val.clusterDim.y = 1;
   cluster[0].val.clusterDim.z = 1;
+  cluster[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  cluster[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = cluster;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = after ? 2 : 1;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, K, a, b, q, ctas);
   if (e != cudaSuccess) return fail(AVEY_ERR_LAUNCH, cudaGetErrorString(e));
   avey_host::count_launches(1);
@@ -317,14 +332,15 @@ int forward_tc(const AveyLinearParams* p, cudaStream_t stream) {
   if (rc != AVEY_OK) return rc;
   // One more row tile than the groups': the rows past the last group.
   const int64_t tiles = (mt + (p->offsets ? 1 : 0)) * q.n_nt;
+  const bool packed = l.pack_x || l.pack_w;
   if (ctas > 1) {
     if constexpr (ACT != AVEY_ACT_IDENTITY)
-      if (p->deriv) return launch_split<avey::tc_linear_split<T, ACT, true>>(m.a, m.b, q, tiles, ctas, stream);
-    return launch_split<avey::tc_linear_split<T, ACT, false>>(m.a, m.b, q, tiles, ctas, stream);
+      if (p->deriv) return launch_split<avey::tc_linear_split<T, ACT, true>>(m.a, m.b, q, tiles, ctas, packed, stream);
+    return launch_split<avey::tc_linear_split<T, ACT, false>>(m.a, m.b, q, tiles, ctas, packed, stream);
   }
   if constexpr (ACT != AVEY_ACT_IDENTITY)
-    if (p->deriv) return launch_tc<avey::tc_linear<T, avey::kLnForward, ACT, true>>(m, q, tiles, stream);
-  return launch_tc<avey::tc_linear<T, avey::kLnForward, ACT, false>>(m, q, tiles, stream);
+    if (p->deriv) return launch_tc<avey::tc_linear<T, avey::kLnForward, ACT, true>>(m, q, tiles, packed, stream);
+  return launch_tc<avey::tc_linear<T, avey::kLnForward, ACT, false>>(m, q, tiles, packed, stream);
 }
 
 template <typename T, int ACT, bool DERIV, int NT>
@@ -417,6 +433,7 @@ int backward(const AveyLinearParams* p, cudaStream_t stream) {
   if (rc != AVEY_OK) return rc;
   // An idle warp of the dX kernel adds up the bias gradient where that hides
   // behind the products (1024 partial rows take it about 20 us).
+  bool after = l.pack_x || l.pack_w;
   const bool sum_in_dx = l.sums && p->dx && p->rows <= 65536;
   if (l.make_dpre || l.sums) {
     avey::LnDpre q{};
@@ -437,6 +454,7 @@ int backward(const AveyLinearParams* p, cudaStream_t stream) {
     if (l.sums) q.partial = reinterpret_cast<float*>(ws + l.partial);
     rc = launch_dpre<T>(q, p->activation, row_tiles(p, avey::kLdRows), stream);
     if (rc != AVEY_OK) return rc;
+    after = !(l.sums && !sum_in_dx);
     if (l.sums && !sum_in_dx) {
       const dim3 grid(static_cast<unsigned>((p->d_out + 31) / 32), static_cast<unsigned>(p->groups));
       avey::ln_bias_sum<T><<<grid, avey::kLbThreads, 0, stream>>>(p->offsets, q.groups, q.rows, q.n, q.partial,
@@ -464,8 +482,10 @@ int backward(const AveyLinearParams* p, cudaStream_t stream) {
       rc = avey_host::encode_tiles(p->dtype, p->dx, p->d_in, p->rows, 1, p->dx_ld * 2, 0, &m.y);
     if (rc != AVEY_OK) return rc;
     const int64_t tiles = (mt + (p->offsets ? 1 : 0)) * q.n_nt;
-    rc = launch_tc<avey::tc_linear<T, avey::kLnGradX, 0, false>>(m, q, tiles, stream);
+    q.lets_next = p->dweight != nullptr;
+    rc = launch_tc<avey::tc_linear<T, avey::kLnGradX, 0, false>>(m, q, tiles, after, stream);
     if (rc != AVEY_OK) return rc;
+    after = true;
   }
   if (p->dweight) {
     avey::LnGeom q = geom(p, p->d_in, dw_cols(p));
@@ -473,6 +493,7 @@ int backward(const AveyLinearParams* p, cudaStream_t stream) {
     q.n_mt = (q.m + avey::kLnBM - 1) / avey::kLnBM;
     q.splits = l.splits;
     const bool parts = l.splits > 1;
+    q.beside = p->dx != nullptr;
     q.out = parts ? static_cast<void*>(ws + l.dw) : p->dweight;
     q.out_ld = parts ? (p->d_in + 3) / 4 * 4 : p->d_in;
     q.out_gs = p->d_out * q.out_ld;
@@ -485,8 +506,8 @@ int backward(const AveyLinearParams* p, cudaStream_t stream) {
                                    q.out_ld * (parts ? 4 : 2), q.out_gs * (parts ? 4 : 2), &m.y);
     if (rc != AVEY_OK) return rc;
     const int64_t tiles = p->groups * q.n_mt * q.n_nt * q.splits;
-    rc = parts ? launch_tc<avey::tc_linear<T, avey::kLnGradW, 0, true>>(m, q, tiles, stream)
-               : launch_tc<avey::tc_linear<T, avey::kLnGradW, 0, false>>(m, q, tiles, stream);
+    rc = parts ? launch_tc<avey::tc_linear<T, avey::kLnGradW, 0, true>>(m, q, tiles, after, stream)
+               : launch_tc<avey::tc_linear<T, avey::kLnGradW, 0, false>>(m, q, tiles, after, stream);
     if (rc != AVEY_OK) return rc;
     if (parts) {
       const int64_t rows = p->groups * p->d_out, quads = rows * (q.out_ld / 4);

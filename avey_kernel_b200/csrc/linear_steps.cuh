@@ -197,6 +197,7 @@ template <typename T, int ACT>
 __global__ void __launch_bounds__(kLdThreads) ln_dpre(const LnDpre q) {
   __shared__ float red[8][kLdCols];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  griddep_launch_dependents();  // the products are set up meanwhile
   LnSpan s;
   if (!ln_find(q.offsets, q.groups, q.rows, blockIdx.x, 0, ln_dpre_tiles, s)) return;
   const int row0 = s.lo + s.index * kLdRows, row1 = min(s.hi, row0 + kLdRows);
@@ -320,6 +321,7 @@ struct LnPack {
   uint16_t* dst;
 };
 __global__ void __launch_bounds__(256) ln_pack_rows(const LnPack a, const LnPack b) {
+  griddep_launch_dependents();  // the products are set up meanwhile
   const int64_t na = a.rows * (a.ld / 8), nb = b.rows * (b.ld / 8);
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < na + nb;
        i += static_cast<int64_t>(gridDim.x) * 256) {

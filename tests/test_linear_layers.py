@@ -216,6 +216,37 @@ def test_only_the_wanted_gradients():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('grouped', [False, True])
+@pytest.mark.parametrize('act,k', [('silu', 520), ('identity', 520), ('gelu', 389)])
+def test_passes_in_a_row_give_what_each_gives_alone(grouped, act, k):
+    """dX is set up beside the step before it and dW starts beside dX: calls in a
+    row, each on the workspace of the one before it, against single gradients."""
+    rows, n, f = 9000, 712, torch.bfloat16
+    x = torch.randn(rows, k, generator=torch.Generator('cuda').manual_seed(4), device='cuda').to(f)
+    w = (torch.randn(5, n, k, device='cuda') * k ** -0.5).to(f)
+    offsets = torch.tensor([0, 3000, 3000, 3100, 8000, 8990], dtype=torch.int32, device='cuda')
+    x, w = x.requires_grad_(True), (w if grouped else w[0]).requires_grad_(True)
+    b = torch.randn(w.shape[:-1], device='cuda').to(f).requires_grad_(True)
+
+    def layer():
+        if grouped:
+            return experts.expert_linear(x, w, offsets, b, activation=act)
+        return layers.residual_linear(x, w, b, activation=act)
+
+    dys = [torch.randn(rows, n, device='cuda').to(f) for _ in range(3)]
+    alone = []
+    for dy in dys:
+        grads = []
+        for t in (x, w, b):
+            grads += torch.autograd.grad(layer(), t, dy)
+            torch.cuda.synchronize()
+        alone.append(grads)
+    for i in [0, 1, 2] * 10:
+        got = torch.autograd.grad(layer(), (x, w, b), dys[i])
+        assert all(torch.equal(a, c) for a, c in zip(got, alone[i]))
+
+
+@pytest.mark.gpu
 def test_gradients_against_differences_of_the_formula():
     """A step h along a direction moves <dy, y> by h <grad, direction> + O(h^3)."""
     x, w, b, r, dy = data(150, 48, 56, torch.bfloat16, 7)
