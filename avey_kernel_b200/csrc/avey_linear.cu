@@ -50,7 +50,7 @@ int64_t up8(int64_t x) { return (x + 7) / 8 * 8; }
 int64_t up16(int64_t x) { return (x + 15) / 16 * 16; }
 uint64_t up256(uint64_t x) { return (x + 255u) & ~uint64_t(255); }
 
-// Rows up to which AUTO may take the kernel for few rows.
+// Rows up to which AUTO takes the kernel for few rows.
 constexpr int64_t kFewRows = 64;
 
 int validate(const AveyLinearParams* p, bool backward) {
@@ -99,15 +99,15 @@ int validate(const AveyLinearParams* p, bool backward) {
   return AVEY_OK;
 }
 
-// AUTO: dense layers of up to 64 rows finish sooner there or as soon (one row,
-// 768 -> 1536: 2.4 against 5.5 us; 64 rows: 5.2 against 5.9, 4096 -> 4096 17.0
-// against 16.9), of 128 rows later (8.9 against 6.9 us). Grouped ones too, while
-// the weights that the rows can touch stay below about 100 MB (64 rows of 8
-// experts, 768 -> 1536: 8.2 against 12.7 us; 64 of 16, 1024 -> 2048: 13.0 against
-// 12.9; 64 of 64: 45 against 36).
+// AUTO: up to 64 rows finish sooner there or as soon (one row, 768 -> 1536: 2.5
+// against 6.0 us; 64 rows: 5.2 against 6.2, 4096 -> 4096 17.5 against 17.5; 128
+// rows, 768 -> 1536: 8.9 against 6.9). Grouped ones too (64 rows of 16 experts,
+// 1024 -> 2048: 15.3 against 18.4 us, of 64: 32.2 against 36.3, of 128: 41.7 against
+// 40.3); more rows finish sooner here or there by the number of experts (128 rows
+// of 32: 26.2 against 29.7; of 128, 768 -> 1536: 49.8 against 38.2) and take tiles.
 bool use_few(const AveyLinearParams* p) {
   if (p->kernel != AVEY_LINEAR_KERNEL_AUTO) return p->kernel == AVEY_LINEAR_KERNEL_FEW;
-  return p->rows <= kFewRows && std::min(p->groups, p->rows) * p->d_in * p->d_out <= 48ll << 20;
+  return p->rows <= kFewRows;
 }
 
 // Row tiles of `tile` rows that the groups can come to.
@@ -346,10 +346,13 @@ int forward_tc(const AveyLinearParams* p, cudaStream_t stream) {
 template <typename T, int ACT, bool DERIV, int NT>
 int launch_few_rows(const avey::LnFew& q, cudaStream_t stream) {
   const dim3 grid((q.n + avey::kLfOut - 1) / avey::kLfOut, q.offsets ? std::min(q.groups, q.rows) + 1 : 1);
-  if (static_cast<int64_t>(grid.x) * grid.y <= avey_host::multiprocessors() && q.k >= 1024)
+  const int64_t ctas = static_cast<int64_t>(grid.x) * (q.offsets ? grid.y - 1 : 1), sms = avey_host::multiprocessors();
+  if (ctas <= sms && q.k >= 1024)
     avey::ln_few<T, ACT, DERIV, NT, 16><<<grid, 512, 0, stream>>>(q);
-  else
+  else if (ctas < 3 * sms)
     avey::ln_few<T, ACT, DERIV, NT, 8><<<grid, 256, 0, stream>>>(q);
+  else
+    avey::ln_few<T, ACT, DERIV, NT, 4><<<grid, 128, 0, stream>>>(q);
   return launched("ln_few");
 }
 

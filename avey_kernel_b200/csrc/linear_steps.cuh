@@ -48,8 +48,11 @@ __device__ __forceinline__ LnOct2 ln_load16(const uint16_t* p, int left, int vec
 // four lanes read a whole line of a row (with 16 bytes a lane, half lines, 48
 // rows of 2048 -> 1024 took 8.8 us).
 // A CTA owns 16 outputs; its warps share the steps of K, and their sums are added
-// in a fixed order. Where there are no more CTAs than SMs and K is long, 16
-// warps share them instead of 8.
+// in a fixed order: 8 warps; 16 where there are no more CTAs than SMs and K is
+// long (48 rows of 2048 -> 1024: 7.5 against 8.2 us); 4 where there are three CTAs
+// an SM and more, which then come and go more evenly (16 rows of 16 experts, 1024
+// -> 2048, from HBM: 11.2 against 13.9 us, 3.9 TB/s; 4 rows of 2048 -> 8192: 9.5
+// against 10.3; but 384 CTAs of 1536 -> 6144: 7.0 against 6.3).
 constexpr int kLfOut = 16;
 
 struct LnFew {
@@ -79,7 +82,8 @@ __device__ __forceinline__ void ln_mma(float (&c)[4], uint32_t a0, uint32_t a1, 
 template <typename T, int ACT, bool DERIV, int NT, int WARPS>
 __global__ void __launch_bounds__(32 * WARPS) ln_few(const LnFew q) {
   constexpr int kThreads = 32 * WARPS;
-  __shared__ float red[8][8 * NT][kLfOut + 1];
+  constexpr int kParts = WARPS < 8 ? WARPS : 8;
+  __shared__ float red[kParts][8 * NT][kLfOut + 1];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int n0 = blockIdx.x * kLfOut;
   LnSpan s{0, 0, q.rows, 0, 0, 1};
@@ -137,7 +141,7 @@ __global__ void __launch_bounds__(32 * WARPS) ln_few(const LnFew q) {
       for (int j = 0; j < NT; ++j)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          float& z = red[warp & 7][j * 8 + (lane & 3) * 2 + (i & 1)][(lane >> 2) + (i >> 1) * 8];
+          float& z = red[warp % kParts][j * 8 + (lane & 3) * 2 + (i & 1)][(lane >> 2) + (i >> 1) * 8];
           z = add ? z + acc[j][i] : acc[j][i];
         }
     };
@@ -156,7 +160,7 @@ __global__ void __launch_bounds__(32 * WARPS) ln_few(const LnFew q) {
       if (row >= s.hi || col >= q.n) continue;
       float z = 0.f;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) z += red[k][r][o];
+      for (int k = 0; k < kParts; ++k) z += red[k][r][o];
       float y = 0.f;
       if (!zero) {
         if (q.bias) z += Elem<T>::to_f(reinterpret_cast<const T*>(q.bias)[static_cast<int64_t>(s.g) * q.bias_gs + col]);

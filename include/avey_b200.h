@@ -449,9 +449,8 @@ typedef struct AveyLinearParams {
   uint64_t workspace_bytes;
 } AveyLinearParams;
 
-/* AUTO: the kernel for few rows up to 64 of them (grouped: while the experts'
- * weights that so many rows can touch stay below 48 Mi elements), which reads
- * the weights without filling 128-row tiles; tcgen05 tiles above. */
+/* AUTO: the kernel for few rows up to 64 of them, which reads the weights
+ * without filling 128-row tiles; tcgen05 tiles above. */
 #define AVEY_LINEAR_KERNEL_AUTO 0
 #define AVEY_LINEAR_KERNEL_TCGEN05 1
 #define AVEY_LINEAR_KERNEL_FEW 2
