@@ -310,6 +310,35 @@ def test_streams_and_graphs():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('k', [389, 520])
+def test_a_captured_training_step(k):
+    """All steps of both directions, with what follows them on the stream, in a
+    graph: replays with new inputs against calls as they come."""
+    x, w, b, r, dy = data(3000, k, 712, torch.bfloat16, 24)
+    leaves = [t.detach().clone().requires_grad_(True) for t in (x, w, b)]
+
+    def step():
+        y = layers.residual_linear(*leaves, activation='gelu', residual=r)
+        return [y.detach()] + [g + 1 for g in torch.autograd.grad(y, leaves, dy)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for scale in (1.0, 0.5, -2.0, 0.25):
+        dy.mul_(scale)
+        leaves[0].data.mul_(scale)
+        for _ in range(3):
+            graph.replay()
+        got = [t.clone() for t in out]
+        assert all(torch.equal(p, q) for p, q in zip(got, step()))
+
+
+@pytest.mark.gpu
 def test_arrays_past_2_to_the_31_elements():
     rows, k, n = (1 << 21) + 77, 1032, 64  # x and dx hold 2^31 + 1.7 10^7 elements
     w, b, dt = data(1, k, n, torch.bfloat16, 15)[1], None, torch.bfloat16
