@@ -50,9 +50,6 @@ int64_t up8(int64_t x) { return (x + 7) / 8 * 8; }
 int64_t up16(int64_t x) { return (x + 15) / 16 * 16; }
 uint64_t up256(uint64_t x) { return (x + 255u) & ~uint64_t(255); }
 
-// Rows up to which AUTO takes the kernel for few rows.
-constexpr int64_t kFewRows = 64;
-
 int validate(const AveyLinearParams* p, bool backward) {
   if (!p) return fail(AVEY_ERR_ARGUMENT, "params is NULL");
   if (p->struct_size != sizeof(AveyLinearParams))
@@ -99,15 +96,30 @@ int validate(const AveyLinearParams* p, bool backward) {
   return AVEY_OK;
 }
 
-// AUTO: up to 64 rows finish sooner there or as soon (one row, 768 -> 1536: 2.5
-// against 6.0 us; 64 rows: 5.2 against 6.2, 4096 -> 4096 17.5 against 17.5; 128
-// rows, 768 -> 1536: 8.9 against 6.9). Grouped ones too (64 rows of 16 experts,
-// 1024 -> 2048: 15.3 against 18.4 us, of 64: 32.2 against 36.3, of 128: 41.7 against
-// 40.3); more rows finish sooner here or there by the number of experts (128 rows
-// of 32: 26.2 against 29.7; of 128, 768 -> 1536: 49.8 against 38.2) and take tiles.
+// Whether TMA can read x and the weights in place.
+bool whole_x(const AveyLinearParams* p) { return whole_rows(p->x, p->x_ld); }
+bool whole_w(const AveyLinearParams* p) {
+  return whole_rows(p->weight, p->weight_ld) && (p->weight_group_stride % 8 == 0 || p->groups == 1);
+}
+
+// AUTO, dense layers: the kernel for few rows costs as its rows x d_in x d_out,
+// tiles as their number. 8 rows at most finish sooner there at any size (768 ->
+// 1536: 2.5 against 6.0 us, 8192 -> 16384: 43 against 50-70); up to 32 rows to 2^29
+// (32 of 2048 -> 8192: 13.0 against 14.7; past it 16 of 4096 -> 14336: 29.8 against
+// 27.3); up to 256 to 2^28 (64 of 1024 -> 4096: 8.1 against 9.2; 256 of 768 -> 768:
+// 6.4 against 6.9; past it 64 of 1536 -> 6144: 15.6 against 12.3; 256 of 768 -> 1536:
+// 11.1 against 8.5). Rows that are not whole 16-byte units it reads value by value,
+// four times as dear (128 of 389 -> 771: 7.1 against 8.8; 256: 10.9 against 9.1).
+// Grouped ones: up to 64 rows (of 16 experts, 1024 -> 2048: 15.3 against 18.4 us, of
+// 64: 32.2 against 36.3, of 128: 41.7 against 40.3); more finish sooner here or there
+// by the number of experts (128 rows of 32: 26.2 against 29.7; of 128, 768 -> 1536:
+// 49.8 against 38.2) and take tiles.
 bool use_few(const AveyLinearParams* p) {
   if (p->kernel != AVEY_LINEAR_KERNEL_AUTO) return p->kernel == AVEY_LINEAR_KERNEL_FEW;
-  return p->rows <= kFewRows;
+  if (p->offsets) return p->rows <= 64;
+  if (p->rows <= 8) return true;
+  const int64_t most = (p->rows <= 32 ? 1ll << 29 : 1ll << 28) / (whole_x(p) && whole_w(p) ? 1 : 4);
+  return p->rows <= 256 && p->rows * p->d_in * p->d_out <= most;
 }
 
 // Row tiles of `tile` rows that the groups can come to.
@@ -154,8 +166,8 @@ Layout layout(const AveyLinearParams* p, bool backward) {
   };
   if (p->rows == 0 || (!backward && use_few(p))) return l;
   const bool want_x = !backward || p->dweight, want_w = !backward || p->dx;
-  l.pack_x = want_x && !whole_rows(p->x, p->x_ld);
-  l.pack_w = want_w && !(whole_rows(p->weight, p->weight_ld) && (p->weight_group_stride % 8 == 0 || p->groups == 1));
+  l.pack_x = want_x && !whole_x(p);
+  l.pack_w = want_w && !whole_w(p);
   if (l.pack_x) l.x = take(static_cast<uint64_t>(p->rows) * up8(p->d_in) * 2);
   if (l.pack_w) l.w = take(static_cast<uint64_t>(p->groups) * p->d_out * up8(p->d_in) * 2);
   if (backward) {
@@ -344,9 +356,9 @@ int forward_tc(const AveyLinearParams* p, cudaStream_t stream) {
 }
 
 template <typename T, int ACT, bool DERIV, int NT>
-int launch_few_rows(const avey::LnFew& q, cudaStream_t stream) {
-  const dim3 grid((q.n + avey::kLfOut - 1) / avey::kLfOut, q.offsets ? std::min(q.groups, q.rows) + 1 : 1);
-  const int64_t ctas = static_cast<int64_t>(grid.x) * (q.offsets ? grid.y - 1 : 1), sms = avey_host::multiprocessors();
+int launch_few_rows(const avey::LnFew& q, int passes, cudaStream_t stream) {
+  const dim3 grid((q.n + avey::kLfOut - 1) / avey::kLfOut, q.offsets ? std::min(q.groups, q.rows) + 1 : passes);
+  const int64_t ctas = static_cast<int64_t>(grid.x) * (q.offsets ? grid.y - 1 : grid.y), sms = avey_host::multiprocessors();
   if (ctas <= sms && q.k >= 1024)
     avey::ln_few<T, ACT, DERIV, NT, 16><<<grid, 512, 0, stream>>>(q);
   else if (ctas < 3 * sms)
@@ -358,13 +370,21 @@ int launch_few_rows(const avey::LnFew& q, cudaStream_t stream) {
 
 template <typename T, int ACT, bool DERIV>
 int launch_few(const avey::LnFew& q, cudaStream_t stream) {
-  // Rows of a pass over the weights: the least that hold all rows of a dense
-  // layer, or twice an expert's share.
-  const int rows = q.offsets ? std::max(1, 2 * q.rows / q.groups) : q.rows;
-  if (rows <= 8) return launch_few_rows<T, ACT, DERIV, 1>(q, stream);
-  if (rows <= 16) return launch_few_rows<T, ACT, DERIV, 2>(q, stream);
-  if (rows <= 32) return launch_few_rows<T, ACT, DERIV, 4>(q, stream);
-  return launch_few_rows<T, ACT, DERIV, 8>(q, stream);
+  // Rows of a pass over the weights: twice an expert's share, or the least that hold
+  // all rows of a dense layer. Those share its rows among CTAs while there are no
+  // more than two an SM: the weights come from L2 for all but one of them, and a CTA
+  // takes in fewer rows of x, which is most of what it reads (48 rows of 2048 ->
+  // 1024: 5.5 us by two passes, 7.2 by one; 64 of 768 -> 768: 3.2 by four, 5.2; with
+  // up to three CTAs an SM 64 of 1536 -> 1536 take 8.0 us instead of 6.3).
+  int passes = 1;
+  if (!q.offsets)
+    while (q.rows > 8 * passes && (q.n + avey::kLfOut - 1) / avey::kLfOut * passes <= avey_host::multiprocessors())
+      passes *= 2;
+  const int rows = q.offsets ? std::max(1, 2 * q.rows / q.groups) : (q.rows + passes - 1) / passes;
+  if (rows <= 8) return launch_few_rows<T, ACT, DERIV, 1>(q, passes, stream);
+  if (rows <= 16) return launch_few_rows<T, ACT, DERIV, 2>(q, passes, stream);
+  if (rows <= 32) return launch_few_rows<T, ACT, DERIV, 4>(q, passes, stream);
+  return launch_few_rows<T, ACT, DERIV, 8>(q, passes, stream);
 }
 
 template <typename T, int ACT>

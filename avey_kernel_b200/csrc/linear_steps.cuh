@@ -49,7 +49,7 @@ __device__ __forceinline__ LnOct2 ln_load16(const uint16_t* p, int left, int vec
 // rows of 2048 -> 1024 took 8.8 us).
 // A CTA owns 16 outputs; its warps share the steps of K, and their sums are added
 // in a fixed order: 8 warps; 16 where there are no more CTAs than SMs and K is
-// long (48 rows of 2048 -> 1024: 7.5 against 8.2 us); 4 where there are three CTAs
+// long (48 rows of 2048 -> 1024 by 64 CTAs: 7.5 against 8.2 us); 4 where there are three CTAs
 // an SM and more, which then come and go more evenly (16 rows of 16 experts, 1024
 // -> 2048, from HBM: 11.2 against 13.9 us, 3.9 TB/s; 4 rows of 2048 -> 8192: 9.5
 // against 10.3; but 384 CTAs of 1536 -> 6144: 7.0 against 6.3).
@@ -97,7 +97,9 @@ __global__ void __launch_bounds__(32 * WARPS) ln_few(const LnFew q) {
   const int o_lo = n0 + (lane >> 2), o_hi = o_lo + 8;
   const uint16_t* wl = w0 + static_cast<int64_t>(o_lo) * q.w_ld;
   const uint16_t* wh = w0 + static_cast<int64_t>(o_hi) * q.w_ld;
-  for (int r0 = s.lo; r0 < s.hi; r0 += 8 * NT) {
+  // Dense layers: the passes of 8 NT rows are shared by the grid's second dimension.
+  const int pass0 = q.offsets ? 0 : blockIdx.y, passes = q.offsets ? 1 : gridDim.y;
+  for (int r0 = s.lo + pass0 * 8 * NT; r0 < s.hi; r0 += passes * 8 * NT) {
     float acc[NT][4];
 #pragma unroll
     for (int j = 0; j < NT; ++j)

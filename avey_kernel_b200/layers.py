@@ -247,9 +247,9 @@ def residual_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.
     bf16 / f16 CUDA tensors of one dtype run natively, forward and backward
     (fp32 sums; y and the gradients are rounded once, the gradient at the
     product is rounded to the operand type before its two products, so in f16
-    it is infinite past f16's range, as in torch's). A few rows
-    (64 at most: single tokens of a batch) read the weights once on a kernel of
-    their own. Views with any row stride are read in place. CPU tensors take
+    it is infinite past f16's range, as in torch's). Few rows
+    (single tokens of a batch; up to 256 where the layer is small) have a kernel
+    of their own. Views with any row stride are read in place. CPU tensors take
     plain PyTorch."""
     _check_act(activation)
     if not x.is_cuda:

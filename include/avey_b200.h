@@ -449,8 +449,9 @@ typedef struct AveyLinearParams {
   uint64_t workspace_bytes;
 } AveyLinearParams;
 
-/* AUTO: the kernel for few rows up to 64 of them, which reads the weights
- * without filling 128-row tiles; tcgen05 tiles above. */
+/* AUTO: the kernel for few rows, which reads the weights without filling
+ * 128-row tiles, up to 8 rows, up to 256 by the size of the product (2^28
+ * multiplications and about), and up to 64 grouped ones; tcgen05 tiles above. */
 #define AVEY_LINEAR_KERNEL_AUTO 0
 #define AVEY_LINEAR_KERNEL_TCGEN05 1
 #define AVEY_LINEAR_KERNEL_FEW 2

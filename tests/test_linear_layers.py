@@ -134,6 +134,16 @@ def test_linear_and_its_gradients(rows, k, n, dt, act):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('act', ACTS)
+@pytest.mark.parametrize('dt', DTYPES)
+@pytest.mark.parametrize('rows,k,n', [(65, 128, 264), (150, 520, 72), (33, 1032, 40), (250, 72, 4200)])
+@pytest.mark.parametrize('kernel', [_native.LINEAR_TCGEN05, _native.LINEAR_FEW])
+def test_both_kernels_between_few_rows_and_many(rows, k, n, dt, act, kernel):
+    """Clusters that share K, and rows shared by CTAs; many CTAs of few rows."""
+    check_linear(rows, k, n, dt, act, kernel=kernel, seed=n)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize('kernel', [_native.LINEAR_TCGEN05, _native.LINEAR_FEW])
 @pytest.mark.parametrize('rows', [1, 7, 8, 9, 16, 31, 33, 63, 64, 65, 127, 128, 129, 257])
 def test_row_counts_on_both_kernels(rows, kernel):
@@ -373,19 +383,20 @@ def test_a_wait_that_runs_out_sets_the_flag_and_the_next_call_is_right(rows):
     x, w, b, r, dy = data(rows, 256, 72, torch.bfloat16, 18)
     off = torch.tensor([0, 30, rows - 10], device='cuda', dtype=torch.int32)
     w2, b2 = torch.stack((w, w)), torch.stack((b, b))
-    want = run_linear(x, w, b, r, dy, 'silu')
-    want2 = run_experts(x, w2, off, b2, dy, 'silu')
+    tiles = _native.LINEAR_TCGEN05
+    want = run_linear(x, w, b, r, dy, 'silu', tiles)
+    want2 = run_experts(x, w2, off, b2, dy, 'silu', tiles)
     assert _native.device_status(clear=True) == 0
     try:
         _native.test_hooks(100_000, stall=True)
-        run_linear(x, w, b, r, dy, 'silu')
+        run_linear(x, w, b, r, dy, 'silu', tiles)
         assert _native.device_status(clear=True) & 1
-        run_experts(x, w2, off, b2, dy, 'silu')
+        run_experts(x, w2, off, b2, dy, 'silu', tiles)
         assert _native.device_status(clear=True) & 1
     finally:
         _native.test_hooks()
         _native.device_status(clear=True)
-    got, got2 = run_linear(x, w, b, r, dy, 'silu'), run_experts(x, w2, off, b2, dy, 'silu')
+    got, got2 = run_linear(x, w, b, r, dy, 'silu', tiles), run_experts(x, w2, off, b2, dy, 'silu', tiles)
     assert torch.equal(got[0], want[0]) and all(torch.equal(p, q) for p, q in zip(got[1], want[1]))
     assert all(torch.equal(p, q) for p, q in zip(got2, want2))
     assert _native.device_status() == 0
