@@ -516,7 +516,6 @@ int backward(const AveyLinearParams* p, cudaStream_t stream) {
     q.n_mt = (q.m + avey::kLnBM - 1) / avey::kLnBM;
     q.splits = l.splits;
     const bool parts = l.splits > 1;
-    q.beside = p->dx != nullptr;
     q.out = parts ? static_cast<void*>(ws + l.dw) : p->dweight;
     q.out_ld = parts ? (p->d_in + 3) / 4 * 4 : p->d_in;
     q.out_gs = p->d_out * q.out_ld;

@@ -81,7 +81,6 @@ struct LnGeom {
   const float* bias_sums;  // dX: partial sums of the bias gradient [tiles][kc], or null
   void* db;                // its [groups][kc]
   int lets_next;           // dX: dW is launched as its dependent
-  int beside;              // dW: launched beside dX, whose operands it does not wait for
   int test_stall;          // tests: the TMA lane asks for nothing
 };
 
@@ -839,12 +838,11 @@ __global__ void __launch_bounds__(kLnThreads, 1)
     // ============================================================ TMA producer
     if (lane == 0) {
       const uint64_t keep = l2_policy_evict_last();  // operands are read again by other tiles
-      // The CTA is set up beside the end of the step before (a copy of rows, dpre),
-      // and its operands are read after it. dW's CTAs come up as dX's leave their
-      // SMs: its operands are complete once every CTA of dX has waited for them.
-      // (Training steps of 32768 rows of 8 experts 768 -> 1536: 300 -> 288 us, dense
-      // 311.5 -> 308; a forward pass with a copy of rows: 0.5-1.5 us less.)
-      if (!(MODE == kLnGradW && q.beside)) griddep_wait();
+      // The CTA is set up beside the end of the step before (a copy of rows, dpre, dX),
+      // and its operands are read after it. dW's too, though its operands are older
+      // than dX: what an earlier grid has written is promised to a grid that waits for
+      // the one before it, and to no other.
+      griddep_wait();
       if (MODE == kLnGradX && q.lets_next) griddep_launch_dependents();
       LnTile c;
       int st = 0;
@@ -1047,8 +1045,6 @@ __global__ void __launch_bounds__(kLnThreads, 1)
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
-  // dW ends after dX, so what follows it on the stream follows both.
-  if (MODE == kLnGradW && q.beside) griddep_wait();
 }
 
 // ============================================================================

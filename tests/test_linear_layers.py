@@ -13,7 +13,9 @@ A relu's derivative may also flip where |pre| <= a. f16 adds 2^-25 to each
 rounding (half the spacing near zero)."""
 
 import ctypes
+import re
 import threading
+from pathlib import Path
 
 import pytest
 import torch
@@ -711,3 +713,14 @@ def test_workspace_sizes():
     sums = 5 * 72 * 4
     assert _native.linear_workspace_size(p, backward=True) == 43264 + (sums + 255) // 256 * 256  # dpre: 300 x 72 x 2
     assert _native.linear_workspace_size(_params(), backward=True) == 0
+
+
+def test_operands_are_loaded_after_the_wait_for_the_grid_before():
+    """The kernels of the products may be launched while the step before them runs:
+    in each, the wait for it stands before the first load, under no condition."""
+    source = (Path(_native.__file__).parent / 'csrc' / 'tc_linear.cuh').read_text()
+    kernels = source.split('__global__')[1:]
+    assert len(kernels) == 2
+    for body in kernels:
+        before = body[:body.index('tma_load_3d_hint(')]
+        assert re.search(r'^ *griddep_wait\(\);', before, re.M)
