@@ -176,13 +176,15 @@ __device__ __forceinline__ LnPair ln_act2(LnPair x, LnPair* d) {
 // an eighth of an f16 rounding to dpre (the pre-activation in 16 bits would add
 // one or more of the operand type's own). relu2's (2 relu(x)) is unbounded and
 // not negative: the fp32 bit pattern in equal steps from a base, which spreads
-// 2^16 codes over 128 binades for bf16 (2^-62 .. 2^65, half steps of 2^-10) and
-// over 24 for f16 (2^-15 .. 2^9, where the square leaves f16's range; half
-// steps of 2^-12.4); zero below. The code 0xFFFF stands for a derivative that is
+// 2^16 codes over 128 binades for bf16 (2^-62 .. 2^66, half steps of 2^-10) and
+// over 25 for f16 (2^-15 .. 2^10, half steps of 2^-12.3); zero below. Both hold
+// the derivative of every finite y: bf16's square leaves fp32's range at 2^64; f16's
+// y is the square and a residual of -65504 at the least, rounded together, so
+// the pre-activation stays below 362. The code 0xFFFF stands for a derivative that is
 // not finite or out of range (a NaN gives it by itself in the fixed-point form).
 template <typename T>
 struct LnFloatCode {
-  static constexpr uint32_t kBinades = std::is_same<T, __half>::value ? 24 : 128;
+  static constexpr uint32_t kBinades = std::is_same<T, __half>::value ? 25 : 128;
   static constexpr uint32_t kStep = kBinades * 128;  // 2^23 bit patterns a binade / 2^16 codes
   static constexpr uint32_t kBase = (std::is_same<T, __half>::value ? 112u : 65u) << 23;
 };

@@ -724,3 +724,36 @@ def test_operands_are_loaded_after_the_wait_for_the_grid_before():
     for body in kernels:
         before = body[:body.index('tma_load_3d_hint(')]
         assert re.search(r'^ *griddep_wait\(\);', before, re.M)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('rows,kernel', [(5, _native.LINEAR_FEW), (70, _native.LINEAR_FEW), (70, _native.LINEAR_TCGEN05),
+                                         (3000, _native.LINEAR_TCGEN05)])
+def test_f16_relu2_has_its_gradient_wherever_y_is_finite(rows, kernel):
+    """Squares past f16's range that a residual brings back into it, and without one
+    the last pre-activation whose square rounds to 65504; rows without a gradient."""
+    k, n = 16, 40
+    g = torch.Generator(device='cuda').manual_seed(rows)
+    x = torch.full((rows, k), 1.0, device='cuda').half()
+    x[:, 1:] = 0
+    x[:, 0] = (16 + 6.5 * torch.rand(rows, generator=g, device='cuda')).half()  # 16 x: 256 to 360
+    w = (0.1 * torch.randn(n, k, generator=g, device='cuda')).half()
+    w[:, 0] = 16
+    pre = x.double() @ w.double().t()
+    r = (200 * torch.rand(rows, n, generator=g, device='cuda').double() - pre ** 2).clamp(min=-65504).half()
+    dy = (2.0 ** -6 * torch.randn(rows, n, generator=g, device='cuda')).half()
+    dy[::3] = 0
+    b = torch.zeros(n, device='cuda').half()
+    want = reference(x, w, b, r, dy, 'relu2', x.dtype)
+    y, (dx, dw, db, _) = run_linear(x, w, b, r, dy, 'relu2', kernel)
+    assert pre.max() > 355 and y.isfinite().all()
+    for name, got in (('y', y), ('dx', dx), ('dw', dw), ('db', db)):
+        close(got, want[name], name)
+    assert not dx[::3].any()
+    x[:, 0], x[:, 1], w[:, 1:] = 15.9921875, 1, 0
+    w[:, 1] = 0.078125  # the pre-activation is 255.953125
+    want = reference(x, w, None, None, dy, 'relu2', x.dtype)
+    y, (dx, dw, _, _) = run_linear(x, w, None, None, dy, 'relu2', kernel)
+    assert y.isfinite().all()
+    for name, got in (('y', y), ('dx', dx), ('dw', dw)):
+        close(got, want[name], name)
