@@ -746,7 +746,7 @@ def test_f16_relu2_has_its_gradient_wherever_y_is_finite(rows, kernel):
     b = torch.zeros(n, device='cuda').half()
     want = reference(x, w, b, r, dy, 'relu2', x.dtype)
     y, (dx, dw, db, _) = run_linear(x, w, b, r, dy, 'relu2', kernel)
-    assert pre.max() > 355 and y.isfinite().all()
+    assert pre.max() > 300 and y.isfinite().all()  # act' past 600
     for name, got in (('y', y), ('dx', dx), ('dw', dw), ('db', db)):
         close(got, want[name], name)
     assert not dx[::3].any()
