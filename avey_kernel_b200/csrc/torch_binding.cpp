@@ -7,9 +7,13 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/autograd/variable.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/forward_grad.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
 #include <ATen/cuda/CUDAContext.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAGuard.h>
 
 #include <algorithm>
@@ -37,6 +41,24 @@ int dtype_id(const Tensor& t) {
     case at::kBFloat16: return AVEY_BF16;
     default: return -1;
   }
+}
+
+// The operators work on the memory of their tensors, which torch does not see: a
+// forward-mode derivative would be lost and a trace would hold their outputs as
+// they were allocated, so both are refused. `visit(f)` calls f for each tensor.
+template <typename Visit>
+void refuse_unseen(Visit visit) {
+  const bool traced =
+      torch::jit::tracer::isTracing() || c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::PreDispatch) ||
+      (c10::impl::TorchDispatchModeTLS::any_modes_set() &&
+       c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value());
+  TORCH_CHECK(!traced, "the native operators cannot be traced (torch.jit.trace, make_fx)");
+  // Tangents exist within a level of forward-mode differentiation only; there is one at most.
+  if (!torch::autograd::ForwardADLevel::try_get_by_idx(0)) return;
+  visit([](const Tensor& t) {
+    TORCH_CHECK(!t.defined() || !t._fw_grad(0).defined(),
+                "the native operators have no forward-mode derivative (a tensor has a tangent)");
+  });
 }
 
 // ------------------------------------------------------------------- AdamW
@@ -86,6 +108,11 @@ int adamw_step(const py::object& params, const py::object& grads, const py::obje
   v.need(n);
   if (w.given()) w.need(n);
   if (n == 0) return AVEY_OK;
+  refuse_unseen([&](auto f) {
+    for (const TensorList* l : {&p, &g, &m, &v, &w, &ms, &vs})
+      for (Py_ssize_t i = 0; i < l->size(); ++i) f((*l)[i]);
+    if (grad_scale) f(*grad_scale);
+  });
   const auto device = p[0].device();
   const auto dt = p[0].scalar_type();
   const auto state_type = m[0].scalar_type();
@@ -284,6 +311,7 @@ class LinearFunction : public torch::autograd::Function<LinearFunction> {
     torch::autograd::variable_list out(7);
     const Tensor& dy = grads[0];
     if (!dy.defined()) return out;
+    refuse_unseen([&](auto f) { f(dy); });
     // needs_input_grad counts the tensors that were given.
     const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1),
                need_b = has_bias && ctx->needs_input_grad(2);
@@ -319,6 +347,12 @@ class LinearFunction : public torch::autograd::Function<LinearFunction> {
 Tensor linear(const Tensor& x, const Tensor& weight, const std::optional<Tensor>& bias,
               const std::optional<Tensor>& residual, const std::optional<Tensor>& offsets, int64_t act,
               int64_t kernel) {
+  refuse_unseen([&](auto f) {
+    f(x);
+    f(weight);
+    for (const std::optional<Tensor>* t : {&bias, &residual})
+      if (*t) f(**t);
+  });
   const auto dt = x.scalar_type();
   const auto device = x.device();
   TORCH_CHECK_VALUE(device.is_cuda() && (dt == at::kBFloat16 || dt == at::kHalf),

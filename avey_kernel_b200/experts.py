@@ -57,8 +57,8 @@ def expert_linear(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor,
     (``offsets[0] = 0``, rising; an expert may have no row), bias ``[experts,
     d_out]``. Rows from ``offsets[-1]`` on belong to no expert: they give
     zeros and get zero gradients. The gradients of experts without rows are
-    zero. bf16 / f16 CUDA tensors of one dtype run natively; CPU tensors take
-    plain PyTorch."""
+    zero. bf16 / f16 CUDA tensors of one dtype run natively (forward-mode tangents
+    and traces raise); CPU tensors take plain PyTorch."""
     _check_act(activation)
     if x.is_cuda:
         return _binding.module().linear(x, weight, bias, None, offsets, _ACT_IDS[activation],

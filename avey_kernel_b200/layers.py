@@ -249,8 +249,9 @@ def residual_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.
     product is rounded to the operand type before its two products, so in f16
     it is infinite past f16's range, as in torch's). Few rows
     (single tokens of a batch; up to 256 where the layer is small) have a kernel
-    of their own. Views with any row stride are read in place. CPU tensors take
-    plain PyTorch."""
+    of their own. Views with any row stride are read in place. Tensors with
+    forward-mode tangents and calls under a trace (``torch.jit.trace``, ``make_fx``)
+    raise: torch does not see the native calls. CPU tensors take plain PyTorch."""
     _check_act(activation)
     if not x.is_cuda:
         y = _act_torch(F.linear(x, weight, bias), activation)

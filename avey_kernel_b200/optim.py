@@ -166,7 +166,8 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor],
     masters: fp32 copies that carry the update of 16-bit parameters. step: 1
     for the first. grad_scale: one fp32 value on the device that multiplies
     every gradient (a clip factor, the inverse of a loss scale). step, lr and
-    seed are host numbers: a captured CUDA graph repeats those of its capture."""
+    seed are host numbers: a captured CUDA graph repeats those of its capture.
+    CUDA tensors with forward-mode tangents and calls under a trace raise."""
     if type(step) is not int or step < 1:
         raise ValueError('step must be a whole number, 1 or more')
     beta1, beta2 = betas

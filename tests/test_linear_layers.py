@@ -20,6 +20,8 @@ from pathlib import Path
 import pytest
 import torch
 import torch.nn.functional as F
+from torch.autograd import forward_ad
+from torch.fx.experimental.proxy_tensor import make_fx
 
 from avey_kernel_b200 import _binding, _native, experts, layers
 
@@ -757,3 +759,37 @@ def test_f16_relu2_has_its_gradient_wherever_y_is_finite(rows, kernel):
     assert y.isfinite().all()
     for name, got in (('y', y), ('dx', dx), ('dw', dw)):
         close(got, want[name], name)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('which', range(5))
+def test_a_tangent_is_refused(which):
+    """Forward-mode derivatives of x, weight, bias, residual and dy would be lost."""
+    tensors = list(data(20, 64, 72, torch.bfloat16, 25))
+    x, w, b, r, dy = tensors
+    y = layers.residual_linear(x.detach().requires_grad_(True), w, b, residual=r)
+    with forward_ad.dual_level():
+        layers.residual_linear(x, w, b, residual=r)  # a level without a tangent takes nothing away
+        tensors[which] = forward_ad.make_dual(tensors[which], torch.ones_like(tensors[which]))
+        x, w, b, r, dy = tensors
+        with pytest.raises(RuntimeError, match='forward-mode'):
+            if which == 4:
+                y.backward(dy)
+            else:
+                layers.residual_linear(x, w, b, residual=r)
+    off = torch.tensor([0, 5, 20], device='cuda', dtype=torch.int32)
+    with forward_ad.dual_level(), pytest.raises(RuntimeError, match='forward-mode'):
+        experts.expert_linear(forward_ad.make_dual(tensors[0].detach(), tensors[0].detach()), tensors[1].expand(2, 72, 64), off)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('grad', [False, True])
+@pytest.mark.parametrize('trace', [lambda f, x: make_fx(f)(x), lambda f, x: make_fx(f, pre_dispatch=True)(x),
+                                   lambda f, x: torch.jit.trace(f, (x,), check_trace=False)])
+def test_a_trace_is_refused(trace, grad):
+    """It would hold the output as it was allocated."""
+    x, w, b, _, _ = data(20, 64, 72, torch.bfloat16, 26)
+    w.requires_grad_(grad)
+    with pytest.raises(RuntimeError, match='traced'):
+        trace(lambda t: layers.residual_linear(t, w, b, activation='silu'), x)
+    layers.residual_linear(x, w, b)

@@ -12,6 +12,8 @@ import math
 import numpy as np
 import pytest
 import torch
+from torch.autograd import forward_ad
+from torch.fx.experimental.proxy_tensor import make_fx
 
 from avey_kernel_b200 import _native, optim
 
@@ -518,3 +520,30 @@ def test_c_entry_wants_masters_for_all_or_none():
     p.tensors = two
     with pytest.raises(_native.NativeError, match='for all tensors or for none'):
         _native.adamw(p, 0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('name', ['params', 'grads', 'exp_avgs', 'exp_avg_sqs', 'masters'])
+def test_native_step_refuses_tangents(name):
+    """The step would leave the tangents as they were."""
+    s = make([(40,), (8, 12)], torch.bfloat16, 'cuda', master=True)
+    with forward_ad.dual_level():
+        call(s)
+        before = clone(s)
+        s[name][1] = forward_ad.make_dual(s[name][1], torch.ones_like(s[name][1]))
+        with pytest.raises(RuntimeError, match='forward-mode'):
+            call(s)
+    assert torch.equal(s['params'][0], before['params'][0])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('trace', [lambda f, x: make_fx(f)(x), lambda f, x: torch.jit.trace(f, (x,), check_trace=False)])
+def test_native_step_refuses_to_be_traced(trace):
+    s = make([(40,)], torch.float32, 'cuda')
+
+    def step(g):
+        call(dict(s, grads=[g]))
+        return s['params'][0] + 1
+
+    with pytest.raises(RuntimeError, match='traced'):
+        trace(step, s['grads'][0])
