@@ -217,7 +217,8 @@ class AdamW(torch.optim.Optimizer):
         if group['state_bits'] == 8:
             for name in ('exp_avg', 'exp_avg_sq'):
                 state[name] = torch.zeros_like(p, dtype=torch.float8_e4m3fn)
-                state[name + '_scale'] = torch.zeros(state_scales(p.numel()), device=p.device)
+                state[name + '_scale'] = torch.zeros(state_scales(p.numel()), device=p.device,
+                                                      dtype=torch.float32)
         else:
             for name in ('exp_avg', 'exp_avg_sq'):
                 state[name] = torch.zeros_like(p, dtype=torch.float32)

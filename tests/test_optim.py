@@ -547,3 +547,26 @@ def test_native_step_refuses_to_be_traced(trace):
 
     with pytest.raises(RuntimeError, match='traced'):
         trace(step, s['grads'][0])
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('default', [torch.bfloat16, torch.float64])
+def test_8bit_states_do_not_go_by_the_default_type(default, device):
+    """Their scales are fp32, and exact, under any default type."""
+    def run():
+        p = torch.nn.Parameter(torch.ones(700, device=device, dtype=torch.float32))
+        p.grad = torch.linspace(-1, 1, 700, device=device, dtype=torch.float32)
+        opt = optim.AdamW([p], lr=0.1, state_bits=8, seed=3)
+        for _ in range(2):
+            opt.step()
+        return p.detach(), opt.state[p]
+
+    want, state = run()
+    torch.set_default_dtype(default)
+    try:
+        got, other = run()
+    finally:
+        torch.set_default_dtype(torch.float32)
+    assert torch.equal(got, want)
+    for name in ('exp_avg_scale', 'exp_avg_sq_scale'):
+        assert other[name].dtype == torch.float32 and torch.equal(other[name], state[name])
