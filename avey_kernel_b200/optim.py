@@ -82,15 +82,23 @@ def _hash(start: int, n: int, seed: int, step: int) -> torch.Tensor:
     return x ^ (x >> 16)
 
 
-def _check_cpu(p, g, m, v, w):
+def _check_cpu(i, p, g, m, v, w, scales):
     # A dense tensor, and no other, gives its strides to empty_like.
     if torch.empty_like(p, device='meta').stride() != p.stride() and p.numel() > 1:
         raise ValueError('a parameter must be dense in memory')
     if g.shape != p.shape or g.dtype != p.dtype:
         raise ValueError('a gradient must have the shape and type of its parameter')
+    if any(t.dtype != (torch.float8_e4m3fn if scales else torch.float32) for t in (m, v)):
+        raise ValueError('states must be float32 or float8_e4m3fn')
+    if w is not None and w.dtype != torch.float32:
+        raise ValueError(f'masters[{i}] must be float32')
     for t in (m, v) if w is None else (m, v, w):
         if t.shape != p.shape or (t.stride() != p.stride() and p.numel() > 1):
             raise ValueError('states must have the shape and strides of their parameter')
+    blocks = state_scales(p.numel())
+    for t in scales:
+        if t.dtype != torch.float32 or t.numel() != blocks or not t.is_contiguous():
+            raise ValueError(f'scales of parameter {i} must be {blocks} contiguous float32 values')
 
 
 @torch.no_grad()
@@ -109,7 +117,8 @@ def _step_cpu(params, grads, exp_avgs, exp_avg_sqs, step, lr, beta1, beta2, eps,
         if quant != (avg_scales is not None) or quant != (sq_scales is not None):
             raise ValueError('exp_avg_scales and exp_avg_sq_scales go with float8_e4m3fn states, '
                              'and only with them')
-        _check_cpu(p, grads[i], exp_avgs[i], exp_avg_sqs[i], None if masters is None else masters[i])
+        _check_cpu(i, p, grads[i], exp_avgs[i], exp_avg_sqs[i], None if masters is None else masters[i],
+                   (avg_scales[i], sq_scales[i]) if quant else ())
     start = 0
     for i, p in enumerate(params):
         m, v = exp_avgs[i], exp_avg_sqs[i]

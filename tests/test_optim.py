@@ -570,3 +570,21 @@ def test_8bit_states_do_not_go_by_the_default_type(default, device):
     assert torch.equal(got, want)
     for name in ('exp_avg_scale', 'exp_avg_sq_scale'):
         assert other[name].dtype == torch.float32 and torch.equal(other[name], state[name])
+
+
+@pytest.mark.parametrize('bits,change,match', [
+    (32, dict(exp_avgs=torch.Tensor.bfloat16), 'float32 or float8'),
+    (32, dict(exp_avg_sqs=torch.Tensor.double), 'float32 or float8'),
+    (32, dict(masters=torch.Tensor.bfloat16), 'masters.1. must be float32'),
+    (8, dict(exp_avg_scales=torch.Tensor.bfloat16), 'scales of parameter 1 must be 1 contiguous'),
+    (8, dict(exp_avg_sq_scales=lambda t: torch.cat((t, t))), 'scales of parameter 1 must be 1 contiguous'),
+    (8, dict(exp_avg_scales=lambda t: t[:0]), 'scales of parameter 1 must be 1 contiguous')])
+@pytest.mark.parametrize('device', DEVICES)
+def test_states_of_another_type_or_size_are_refused_before_any_change(bits, change, match, device):
+    s = make([(600,), (8, 12)], torch.bfloat16, device, bits=bits, master=True)
+    for name, f in change.items():
+        s[name][1] = f(s[name][1])
+    before = clone(s)
+    with pytest.raises(ValueError, match=match + '|one type'):
+        call(s)
+    assert torch.equal(s['params'][0], before['params'][0])
