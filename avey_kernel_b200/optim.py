@@ -70,9 +70,9 @@ def _quantize(x: torch.Tensor, noise: torch.Tensor):
     return code.view(-1)[:n].to(torch.uint8).view(torch.float8_e4m3fn), scale.view(-1)
 
 
-def _hash(start: int, n: int, seed: int, step: int) -> torch.Tensor:
+def _hash(start: int, n: int, seed: int, step: int, device) -> torch.Tensor:
     """The 32-bit hashes of elements start .. start + n - 1 of a call."""
-    i = torch.arange(start, start + n)
+    i = torch.arange(start, start + n, device=device)
     key = (seed + 0x9e3779b9 * (step + (i >> 32))) & _MASK
     for mul in (0x7feb352d, 0x846ca68b):
         key = ((key ^ (key >> 16)) * mul) & _MASK
@@ -142,7 +142,7 @@ def _step_cpu(params, grads, exp_avgs, exp_avg_sqs, step, lr, beta1, beta2, eps,
         upd = m32 / (root * (1 / math.sqrt(1 - beta2 ** step)) + eps)
         new = target.float() * (1 - lr * weight_decay) - upd * (lr / (1 - beta1 ** step))
         if quant:
-            h = _hash(start, p.numel(), seed, step)
+            h = _hash(start, p.numel(), seed, step, p.device)
             for x, codes, scales, noise in (
                     (m32, fm, avg_scales[i], ((h & 0xffff) << 4) + 8),
                     (root, fv, sq_scales[i], ((h >> 16) << 4) + 8)):

@@ -588,3 +588,16 @@ def test_states_of_another_type_or_size_are_refused_before_any_change(bits, chan
     with pytest.raises(ValueError, match=match + '|one type'):
         call(s)
     assert torch.equal(s['params'][0], before['params'][0])
+
+
+def test_cpu_step_does_not_go_by_the_default_device():
+    a = make([(600,), (8, 12)], torch.bfloat16, 'cpu', bits=8)
+    b = clone(a)
+    call(a, seed=7)
+    torch.set_default_device('meta')
+    try:
+        call(b, seed=7)
+    finally:
+        torch.set_default_device(None)
+    for name in ('params', 'exp_avgs', 'exp_avg_sqs'):
+        assert all(torch.equal(p.float(), q.float()) for p, q in zip(a[name], b[name]))
