@@ -254,8 +254,7 @@ class AdamW(torch.optim.Optimizer):
                 state = self.state[p]
                 if not state:
                     self._init_state(p, group)
-                state['step'] += 1
-                key = (p.device, p.dtype, state['step'])
+                key = (p.device, p.dtype, state['step'] + 1)
                 calls.setdefault(key, []).append((p, state))
             for (_, _, count), members in calls.items():
                 def column(name, members=members):
@@ -267,6 +266,8 @@ class AdamW(torch.optim.Optimizer):
                            exp_avg_scales=column('exp_avg_scale'),
                            exp_avg_sq_scales=column('exp_avg_sq_scale'),
                            seed=group['seed'] + 0x632be5ab * number, grad_scale=grad_scale)
+                for _, state in members:  # once the step has been taken
+                    state['step'] = count
                 number += 1
         return loss
 

@@ -601,3 +601,29 @@ def test_cpu_step_does_not_go_by_the_default_device():
         torch.set_default_device(None)
     for name in ('params', 'exp_avgs', 'exp_avg_sqs'):
         assert all(torch.equal(p.float(), q.float()) for p, q in zip(a[name], b[name]))
+
+
+@pytest.mark.parametrize('device', DEVICES)
+def test_a_step_that_raises_is_not_counted(device):
+    """Neither for the parameters before the bad one nor for it; the next step is
+    what it would have been."""
+    p, q, r = (torch.nn.Parameter(torch.full((4,), 2.0, device=device)) for _ in range(3))
+    opt, ref = optim.AdamW([p, q], lr=0.1), optim.AdamW([r], lr=0.1)
+    for t in (p, q, r):
+        t.grad = torch.ones_like(t)
+    opt.step()
+    ref.step()
+    good, q.grad = q.grad, torch.ones(4, device=device).to_sparse()
+    with pytest.raises(ValueError, match='sparse'):
+        opt.step()
+    with pytest.raises(ValueError, match='lr'):
+        q.grad = good
+        opt.param_groups[0]['lr'] = float('nan')
+        opt.step()
+    opt.param_groups[0]['lr'] = 0.1
+    p.grad.mul_(-1)
+    r.grad.mul_(-1)
+    opt.step()
+    ref.step()
+    assert opt.state[p]['step'] == opt.state[q]['step'] == 2
+    assert torch.equal(p, r)
