@@ -793,3 +793,67 @@ def test_a_trace_is_refused(trace, grad):
     with pytest.raises(RuntimeError, match='traced'):
         trace(lambda t: layers.residual_linear(t, w, b, activation='silu'), x)
     layers.residual_linear(x, w, b)
+
+
+# ------------------------------------------------------------------ exact sums
+
+# Whole numbers from -2 to 2: every product and sum is exact in fp32, in any order,
+# and each result is the exact sum rounded once. A lost or doubled row shows where a
+# bound on rounding errors, which grows with the rows, would not see it.
+
+def whole_numbers(rows, k, n, dt, device, seed=0, groups=()):
+    g = torch.Generator(device=device).manual_seed(seed)
+
+    def draw(*s):
+        return torch.randint(-2, 3, s, generator=g, device=device).to(dt)
+
+    return draw(rows, k), draw(*groups, n, k), draw(*groups, n), draw(rows, n)
+
+
+def exact_gradients(x, w, b, dy, act):
+    x, w, dy = x.double(), w.double(), dy.double()
+    pre = x @ w.t() + b.double()
+    if act == 'relu':
+        dy = dy * (pre > 0)
+    return [pre.clamp(min=0) if act == 'relu' else pre, dy @ w, dy.t() @ x, dy.sum(0)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dt', DTYPES)
+@pytest.mark.parametrize('act', ['identity', 'relu'])
+@pytest.mark.parametrize('rows,k,n', [(20000, 128, 128), (3001, 72, 264), (65537, 64, 40), (9000, 389, 77)])
+def test_no_row_is_lost_or_doubled_in_long_sums(rows, k, n, act, dt):
+    x, w, b, dy = whole_numbers(rows, k, n, dt, 'cuda', rows)
+    y, (dx, dw, db, _) = run_linear(x, w, b, None, dy, act)
+    for name, got, want in zip(('y', 'dx', 'dw', 'db'), (y, dx, dw, db), exact_gradients(x, w, b, dy, act)):
+        assert torch.equal(got, want.to(dt)), name
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('act', ['identity', 'relu'])
+@pytest.mark.parametrize('sizes', [[5000, 1, 63, 64, 65, 9000, 0, 127, 2000], [15, 17, 4000, 4033, 33], [66000, 500]], ids=str)
+def test_no_row_is_lost_or_doubled_between_experts(sizes, act):
+    k, n, tail = 72, 136, 50
+    x, w, b, dy = whole_numbers(sum(sizes) + tail, k, n, torch.bfloat16, 'cuda', len(sizes), (len(sizes),))
+    off = torch.tensor([0] + sizes, device='cuda').cumsum(0).to(torch.int32)
+    y, dx, dw, db = run_experts(x, w, off, b, dy, act)
+    start = 0
+    for i, c in enumerate(sizes):
+        s = slice(start, start + c)
+        start += c
+        want = exact_gradients(x[s], w[i], b[i], dy[s], act)
+        for name, got, v in zip(('y', 'dx', 'dw', 'db'), (y[s], dx[s], dw[i], db[i]), want):
+            assert torch.equal(got, v.to(x.dtype)), f'expert {i} {name}'
+    assert not y[start:].any() and not dx[start:].any()
+
+
+def test_exact_sums_show_a_lost_row():
+    """One row less in the 64-bit sums, or a block of rows twice, changes dW and db
+    as they are compared above."""
+    x, w, b, dy = whole_numbers(20000, 128, 128, torch.bfloat16, 'cpu', 1)
+    _, _, dw, db = exact_gradients(x, w, b, dy, 'identity')
+    for first, rows, sign in [(0, 1, -1), (77, 1, -1), (19999, 1, 1), (64 * 100, 64, -1), (64 * 200, 64, 1), (19968, 32, -1)]:
+        s = slice(first, first + rows)
+        _, _, part_w, part_b = exact_gradients(x[s], w, b, dy[s], 'identity')
+        assert not torch.equal((dw + sign * part_w).bfloat16(), dw.bfloat16())
+        assert not torch.equal((db + sign * part_b).bfloat16(), db.bfloat16())
