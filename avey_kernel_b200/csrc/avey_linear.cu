@@ -434,6 +434,45 @@ int forward(const AveyLinearParams* p, cudaStream_t stream) {
   }
 }
 
+// The bias gradient is summed by 32 columns of a group at a time, in one of three
+// places, with the same bits. An idle warp of each CTA of the dX kernel takes 1.2 us
+// for one, 0.25 to walk past 32 groups and 1.5 for each 32 partial rows after the
+// first; that is free where the CTA lasts as long: 5 us and 0.4 a K block. (Steps in
+// a graph, with db in dX / by a launch of its own / without db: 4096 x 1024 -> 1024
+// 46.0 / 48.1 / 45.7 us, 16 x 1024 -> 8192 50.8 / 53.2 / 50.5, 32768 x 768 -> 1536 324
+// / 333 / 320; but 64 x 64 -> 4096 187.6 / 33.6 / 31.5, 65536 x 256 -> 256 128 / 92 / 84.)
+bool bias_in_dx(const AveyLinearParams* p) {
+  if (!p->dx) return false;
+  const int64_t mt = row_tiles(p, avey::kLnBM), sms = avey_host::multiprocessors();
+  const int64_t tiles = (mt + (p->offsets ? 1 : 0)) * ((p->d_in + tile_cols(mt, p->d_in) - 1) / tile_cols(mt, p->d_in));
+  const int64_t ctas = std::min(tiles, sms), items = (p->d_out + 31) / 32 * p->groups;
+  const int64_t partial = p->rows / p->groups / avey::kLdRows + 1;
+  const double sums = static_cast<double>((items + ctas - 1) / ctas) *
+                      (1.2 + 0.25 * static_cast<double>((p->groups + 31) / 32) + 1.5 * static_cast<double>(partial / 32));
+  const double lasts = 5 + 0.4 * static_cast<double>((tiles + ctas - 1) / ctas) * static_cast<double>((p->d_out + 63) / 64);
+  return sums <= lasts;
+}
+
+// A launch of its own: a CTA for 32 columns of a group, or a warp where that would
+// be more than four CTAs an SM, of groups with up to 64 partial rows (steps in a graph:
+// 512 rows of 16 experts, 768 -> 768: 31.2 against 30.0 us; 64 rows of 64, 64 -> 1536:
+// 58.3 against 46.4; 1000 of 1000, 64 -> 512: 765 against 256; 4096 dense rows, 1024 ->
+// 1024: 48.1 against 58.5).
+template <typename T>
+int launch_bias_sum(const AveyLinearParams* p, const float* partial, cudaStream_t stream) {
+  const int groups = static_cast<int>(p->groups), rows = static_cast<int>(p->rows), n = static_cast<int>(p->d_out);
+  T* db = static_cast<T*>(p->dbias);
+  const int64_t cols = (p->d_out + 31) / 32, items = cols * p->groups;
+  if (items > 4 * avey_host::multiprocessors() && p->rows / p->groups <= 64 * avey::kLdRows) {
+    const dim3 grid(static_cast<unsigned>((items + avey::kLbWarps - 1) / avey::kLbWarps));
+    avey::ln_bias_groups<T><<<grid, 32 * avey::kLbWarps, 0, stream>>>(p->offsets, groups, rows, n, partial, db);
+  } else {
+    const dim3 grid(static_cast<unsigned>(cols), static_cast<unsigned>(p->groups));
+    avey::ln_bias_sum<T><<<grid, avey::kLbThreads, 0, stream>>>(p->offsets, groups, rows, n, partial, db);
+  }
+  return launched("bias sum");
+}
+
 template <typename T>
 int launch_dpre(const avey::LnDpre& q, int activation, int64_t tiles, cudaStream_t stream) {
   const dim3 grid(static_cast<unsigned>(tiles), (q.n + avey::kLdCols - 1) / avey::kLdCols);
@@ -454,10 +493,9 @@ int backward(const AveyLinearParams* p, cudaStream_t stream) {
   Rows x, w, g{p->dy, p->dy_ld, 0};
   rc = pack_inputs(p, l, &x, &w, stream);
   if (rc != AVEY_OK) return rc;
-  // An idle warp of the dX kernel adds up the bias gradient where that hides
-  // behind the products (1024 partial rows take it about 20 us).
   bool after = l.pack_x || l.pack_w;
-  const bool sum_in_dx = l.sums && p->dx && p->rows <= 65536;
+  const bool sum_in_dx = l.sums && bias_in_dx(p);
+  const float* partial = reinterpret_cast<const float*>(ws + l.partial);
   if (l.make_dpre || l.sums) {
     avey::LnDpre q{};
     q.offsets = p->offsets;
@@ -477,14 +515,7 @@ int backward(const AveyLinearParams* p, cudaStream_t stream) {
     if (l.sums) q.partial = reinterpret_cast<float*>(ws + l.partial);
     rc = launch_dpre<T>(q, p->activation, row_tiles(p, avey::kLdRows), stream);
     if (rc != AVEY_OK) return rc;
-    after = !(l.sums && !sum_in_dx);
-    if (l.sums && !sum_in_dx) {
-      const dim3 grid(static_cast<unsigned>((p->d_out + 31) / 32), static_cast<unsigned>(p->groups));
-      avey::ln_bias_sum<T><<<grid, avey::kLbThreads, 0, stream>>>(p->offsets, q.groups, q.rows, q.n, q.partial,
-                                                                  static_cast<T*>(p->dbias));
-      rc = launched("ln_bias_sum");
-      if (rc != AVEY_OK) return rc;
-    }
+    after = true;
   }
   if (p->dx) {
     const int64_t mt = row_tiles(p, avey::kLnBM);
@@ -494,7 +525,7 @@ int backward(const AveyLinearParams* p, cudaStream_t stream) {
     q.out_ld = p->dx_ld;
     q.out_vec = whole_rows(p->dx, p->dx_ld);
     if (sum_in_dx) {
-      q.bias_sums = reinterpret_cast<const float*>(ws + l.partial);
+      q.bias_sums = partial;
       q.db = p->dbias;
     }
     Maps m;
@@ -540,6 +571,10 @@ int backward(const AveyLinearParams* p, cudaStream_t stream) {
       rc = launched("ln_split_sum");
       if (rc != AVEY_OK) return rc;
     }
+  }
+  if (l.sums && !sum_in_dx) {
+    rc = launch_bias_sum<T>(p, partial, stream);
+    if (rc != AVEY_OK) return rc;
   }
   return avey_host::clear_error();
 }

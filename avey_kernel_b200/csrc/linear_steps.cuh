@@ -258,9 +258,9 @@ __global__ void __launch_bounds__(kLdThreads) ln_dpre(const LnDpre q) {
   }
 }
 
-// db where the dX kernel does not sum it (no dX wanted, or many rows): the same
-// order as ln_bias_columns, by 32 warps (512 tiles of 1536 columns: 5.2 us; by 8
-// warps 7.6).
+// db where the dX kernel does not sum it: the same order as ln_bias_columns, by 32
+// warps for 32 columns of a group (512 tiles of 1536 columns: 5.2 us; by 8 warps
+// 7.6).
 constexpr int kLbThreads = 1024;
 template <typename T>
 __global__ void __launch_bounds__(kLbThreads) ln_bias_sum(const int32_t* offsets, int groups, int rows, int n,
@@ -282,6 +282,19 @@ __global__ void __launch_bounds__(kLbThreads) ln_bias_sum(const int32_t* offsets
     for (int i = 0; i < 32; ++i) z += red[i][lane];
     db[static_cast<int64_t>(blockIdx.y) * n + c] = Elem<T>::from_f(z);
   }
+}
+
+// The same for many groups of few tiles, where 32 warps each would mostly wait for
+// the walk to their group: one warp for 32 columns of a group.
+constexpr int kLbWarps = 8;
+template <typename T>
+__global__ void __launch_bounds__(32 * kLbWarps) ln_bias_groups(const int32_t* offsets, int groups, int rows, int n,
+                                                                const float* partial, T* db) {
+  const int cols = (n + 31) / 32;
+  const int64_t j = static_cast<int64_t>(blockIdx.x) * kLbWarps + (threadIdx.x >> 5);
+  if (j < static_cast<int64_t>(cols) * groups)
+    ln_bias_columns<T>(offsets, groups, rows, n, partial, db, static_cast<int>(j / cols),
+                       static_cast<int>(j % cols) * 32);
 }
 
 // out[row][c] = sum over the splits of partial[split][row][c], in split order

@@ -847,6 +847,41 @@ def test_no_row_is_lost_or_doubled_between_experts(sizes, act):
     assert not y[start:].any() and not dx[start:].any()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize('rows,k,n,count,alone', [
+    (64, 64, 4096, 0, 1), (64, 64, 1536, 64, 1), (300, 40, 300, 300, 1), (20000, 64, 72, 0, 1), (1024, 1024, 1024, 0, 0),
+    (300, 392, 520, 7, 0), (16384, 256, 256, 0, 1), (9000, 64, 20000, 0, 0)])
+def test_bias_sums_go_where_they_take_least(rows, k, n, count, alone):
+    """An idle warp of the dX kernel takes them where they hide behind its products;
+    elsewhere (one CTA would take 128 of them in turn, say) they are a launch."""
+    x, w, b, dy = whole_numbers(rows, k, n, torch.bfloat16, 'cuda', rows + n, (count,) if count else ())
+    off = None
+    if count:
+        sizes = [rows // count + (i < rows % count) for i in range(count)]
+        off = torch.tensor([0] + sizes, device='cuda').cumsum(0).to(torch.int32)
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+
+    def grads(wanted):
+        y = _binding.module().linear(*leaves, None, off, layers._ACT_IDS['relu'], _native.LINEAR_AUTO)
+        before = _native.launch_count()
+        out = torch.autograd.grad(y, wanted, dy)
+        return out, _native.launch_count() - before
+
+    (dx, dw, db), with_bias = grads(leaves)
+    (dx2, dw2), without = grads(leaves[:2])
+    (alone_db,), _ = grads(leaves[2:])
+    assert with_bias - without == alone
+    assert torch.equal(dx, dx2) and torch.equal(dw, dw2) and torch.equal(db, alone_db)
+    if not count:
+        pre = x.detach().double() @ w.detach().double().t() + b.detach().double()
+        assert torch.equal(db, (dy.double() * (pre > 0)).sum(0).to(db.dtype))
+    else:
+        for i in range(0, count, 7):
+            s = slice(off[i].item(), off[i + 1].item())
+            want = exact_gradients(x.detach()[s], w.detach()[i], b.detach()[i], dy[s], 'relu')[3]
+            assert torch.equal(db[i], want.to(db.dtype))
+
+
 def test_exact_sums_show_a_lost_row():
     """One row less in the 64-bit sums, or a block of rows twice, changes dW and db
     as they are compared above."""
