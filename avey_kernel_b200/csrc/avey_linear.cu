@@ -110,13 +110,17 @@ bool whole_w(const AveyLinearParams* p) {
 // 6.4 against 6.9; past it 64 of 1536 -> 6144: 15.6 against 12.3; 256 of 768 -> 1536:
 // 11.1 against 8.5). Rows that are not whole 16-byte units it reads value by value,
 // four times as dear (128 of 389 -> 771: 7.1 against 8.8; 256: 10.9 against 9.1).
-// Grouped ones: up to 64 rows (of 16 experts, 1024 -> 2048: 15.3 against 18.4 us, of
-// 64: 32.2 against 36.3, of 128: 41.7 against 40.3); more finish sooner here or there
-// by the number of experts (128 rows of 32: 26.2 against 29.7; of 128, 768 -> 1536:
-// 49.8 against 38.2) and take tiles.
+// Grouped ones: up to 64 rows (of 16 experts, 1024 -> 2048: 14.3 against 18.4 us, of
+// 64: 48.0 against 50.3; 64 rows of 16, 4096 -> 14336: 276 against 308), but those of
+// more than 8 rows an expert to 2^28 (64 rows of 4, 2048 -> 2048: 12.1 against 15.3;
+// past it 64 of 4, 2048 -> 8192: 33.7 against 28.7, 64 of 2, 4096 -> 14336: 90.8 against
+// 46.1; odd rows alike to 2^27: 64 of 4, 1021 -> 2047: 18.7 against 19.7); more rows
+// finish sooner here or there by the number of experts (128 rows of 32: 26.2 against
+// 29.7; of 128, 768 -> 1536: 49.8 against 38.2) and take tiles.
 bool use_few(const AveyLinearParams* p) {
   if (p->kernel != AVEY_LINEAR_KERNEL_AUTO) return p->kernel == AVEY_LINEAR_KERNEL_FEW;
-  if (p->offsets) return p->rows <= 64;
+  if (p->offsets)
+    return p->rows <= 64 && (p->rows <= 8 * p->groups || p->rows * p->d_in * p->d_out <= 1ll << 28);
   if (p->rows <= 8) return true;
   const int64_t most = (p->rows <= 32 ? 1ll << 29 : 1ll << 28) / (whole_x(p) && whole_w(p) ? 1 : 4);
   return p->rows <= 256 && p->rows * p->d_in * p->d_out <= most;

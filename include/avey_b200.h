@@ -451,7 +451,8 @@ typedef struct AveyLinearParams {
 
 /* AUTO: the kernel for few rows, which reads the weights without filling
  * 128-row tiles, up to 8 rows, up to 256 by the size of the product (2^28
- * multiplications and about), and up to 64 grouped ones; tcgen05 tiles above. */
+ * multiplications and about), and up to 64 grouped ones (by the size too where a
+ * group has more than 8 rows on average); tcgen05 tiles above. */
 #define AVEY_LINEAR_KERNEL_AUTO 0
 #define AVEY_LINEAR_KERNEL_TCGEN05 1
 #define AVEY_LINEAR_KERNEL_FEW 2

@@ -892,3 +892,14 @@ def test_exact_sums_show_a_lost_row():
         _, _, part_w, part_b = exact_gradients(x[s], w, b, dy[s], 'identity')
         assert not torch.equal((dw + sign * part_w).bfloat16(), dw.bfloat16())
         assert not torch.equal((db + sign * part_b).bfloat16(), db.bfloat16())
+
+
+@pytest.mark.parametrize('rows,groups,k,n,few', [
+    (64, 2, 4096, 14336, False), (64, 4, 2048, 8192, False), (32, 2, 2048, 8192, False), (64, 4, 2048, 2048, True),
+    (64, 8, 4096, 14336, True), (16, 2, 4096, 14336, True), (64, 16, 4096, 14336, True), (8, 1, 4096, 14336, True),
+    (65, 16, 64, 64, False)])
+def test_grouped_rows_go_by_the_size_of_the_product(rows, groups, k, n, few):
+    """Only the kernel of tiles needs a workspace, for rows that it cannot read in place."""
+    p = _params(rows=rows, groups=groups, d_in=k, d_out=n, offsets=1 << 20, x=(1 << 20) + 2, x_ld=k, weight_ld=k,
+                weight_group_stride=n * k, y_ld=n)
+    assert (_native.linear_workspace_size(p) == 0) == few
