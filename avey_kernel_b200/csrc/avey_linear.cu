@@ -75,8 +75,8 @@ int validate(const AveyLinearParams* p, bool backward) {
   if (odd != 0 || (reinterpret_cast<uintptr_t>(p->offsets) & 3u) != 0)
     return fail(AVEY_ERR_ARGUMENT, "arrays must be aligned to their elements");
   if (p->rows == 0 && !backward) return AVEY_OK;
-  if (p->rows > 0 && !p->x) return fail(AVEY_ERR_ARGUMENT, "x is required");
-  if (!p->weight) return fail(AVEY_ERR_ARGUMENT, "weight is required");
+  if (p->rows > 0 && !p->x && (!backward || p->dweight)) return fail(AVEY_ERR_ARGUMENT, "x is required");
+  if (!p->weight && (!backward || p->dx)) return fail(AVEY_ERR_ARGUMENT, "weight is required");
   if (p->x_ld < p->d_in || p->weight_ld < p->d_in || p->bias_group_stride < 0 ||
       (p->groups > 1 && p->weight_group_stride < (p->d_out - 1) * p->weight_ld + p->d_in))
     return fail(AVEY_ERR_ARGUMENT, "strides must cover the rows");

@@ -225,23 +225,32 @@ Tensor as_weight(const Tensor& w) {
   return ok ? w : w.contiguous();
 }
 
-// The parameter block of x, weight and the groups.
-AveyLinearParams linear_params(const Tensor& x, const Tensor& w, const std::optional<Tensor>& offsets, int64_t act) {
+// The parameter block but for the operands, from the shapes of x and the weights;
+// `like` has their type.
+AveyLinearParams linear_params(at::IntArrayRef x, at::IntArrayRef w, const Tensor* offsets, const Tensor& like,
+                               int64_t act) {
   AveyLinearParams p{};
   p.struct_size = sizeof(p);
-  p.dtype = dtype_id(x);
+  p.dtype = dtype_id(like);
   p.activation = static_cast<int32_t>(act);
-  p.rows = x.size(0);
-  p.d_in = w.size(-1);
-  p.d_out = w.size(-2);
-  p.groups = offsets ? w.size(0) : 1;
+  p.d_in = w[w.size() - 1];
+  p.d_out = w[w.size() - 2];
+  p.rows = 1;
+  for (size_t i = 0; i + 1 < x.size(); ++i) p.rows *= x[i];
+  p.groups = offsets ? w[0] : 1;
   if (offsets) p.offsets = static_cast<const int32_t*>(offsets->const_data_ptr());
+  p.x_ld = p.weight_ld = p.d_in;
+  if (p.groups > 1) p.weight_group_stride = p.d_out * p.d_in;
+  return p;
+}
+void set_x(AveyLinearParams& p, const Tensor& x) {
   p.x = x.const_data_ptr();
   p.x_ld = row_ld(x, p.d_in);
+}
+void set_weight(AveyLinearParams& p, const Tensor& w) {
   p.weight = w.const_data_ptr();
   p.weight_ld = p.d_out > 1 ? w.stride(-2) : (p.d_in + 7) / 8 * 8;
-  p.weight_group_stride = p.groups > 1 ? w.stride(0) : 0;
-  return p;
+  if (p.groups > 1) p.weight_group_stride = w.stride(0);
 }
 
 Tensor workspace(AveyLinearParams& p, int backward, const Tensor& like) {
@@ -260,7 +269,9 @@ std::pair<Tensor, Tensor> linear_forward(const Tensor& x, const Tensor& weight, 
                                          int64_t act, int64_t kernel, bool want_deriv) {
   const c10::cuda::CUDAGuard guard(x.device());
   const Tensor w = as_weight(weight), xr = as_rows(x, weight.size(-1));
-  AveyLinearParams p = linear_params(xr, w, offsets, act);
+  AveyLinearParams p = linear_params(x.sizes(), w.sizes(), offsets ? &*offsets : nullptr, x, act);
+  set_x(p, xr);
+  set_weight(p, w);
   p.kernel = static_cast<int32_t>(kernel);
   Tensor b, r, deriv;
   if (bias) {
@@ -294,10 +305,16 @@ class LinearFunction : public torch::autograd::Function<LinearFunction> {
                         const std::optional<Tensor>& offsets, int64_t act, int64_t kernel) {
     const bool want = x.requires_grad() || weight.requires_grad() || (bias && bias->requires_grad());
     auto [y, deriv] = linear_forward(x, weight, bias, residual, offsets, act, kernel, want);
-    ctx->save_for_backward({x, weight, offsets ? *offsets : Tensor(), deriv});
-    ctx->saved_data["act"] = act;
-    ctx->saved_data["bias"] = bias ? (bias->dim() == 2 ? 2 : 1) : 0;
-    ctx->saved_data["residual"] = residual.has_value();
+    // x goes into dW and the weights into dx only: what is not needed is neither
+    // held nor has to stay as it is.
+    ctx->save_for_backward({weight.requires_grad() ? x : Tensor(), x.requires_grad() ? weight : Tensor(),
+                            offsets ? *offsets : Tensor(), deriv});
+    // The call's numbers: activation, the bias's dimensions, whether there is a
+    // residual, the dimensions of x, and the sizes of x and the weights.
+    std::vector<int64_t> call{act, bias ? bias->dim() : 0, residual.has_value(), x.dim()};
+    call.insert(call.end(), x.sizes().begin(), x.sizes().end());
+    call.insert(call.end(), weight.sizes().begin(), weight.sizes().end());
+    ctx->saved_data["call"] = std::move(call);
     return y;
   }
 
@@ -307,7 +324,10 @@ class LinearFunction : public torch::autograd::Function<LinearFunction> {
                 "the gradients of the native linear layers cannot be differentiated again (create_graph)");
     const auto saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &weight = saved[1], &offs = saved[2], &deriv = saved[3];
-    const int64_t has_bias = ctx->saved_data["bias"].toInt();
+    const std::vector<int64_t> call = ctx->saved_data["call"].toIntVector();
+    const at::IntArrayRef sizes = at::IntArrayRef(call).slice(4), x_sizes = sizes.slice(0, call[3]),
+                          w_sizes = sizes.slice(call[3]);
+    const int64_t has_bias = call[1];
     torch::autograd::variable_list out(7);
     const Tensor& dy = grads[0];
     if (!dy.defined()) return out;
@@ -315,30 +335,31 @@ class LinearFunction : public torch::autograd::Function<LinearFunction> {
     // needs_input_grad counts the tensors that were given.
     const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1),
                need_b = has_bias && ctx->needs_input_grad(2);
-    if (ctx->saved_data["residual"].toBool() && ctx->needs_input_grad(has_bias ? 3 : 2)) out[3] = dy;
+    if (call[2] && ctx->needs_input_grad(has_bias ? 3 : 2)) out[3] = dy;
     if (!need_x && !need_w && !need_b) return out;
-    const c10::cuda::CUDAGuard guard(x.device());
-    const Tensor w = as_weight(weight), xr = as_rows(x, weight.size(-1));
-    AveyLinearParams p =
-        linear_params(xr, w, offs.defined() ? std::optional<Tensor>(offs) : std::nullopt, ctx->saved_data["act"].toInt());
+    const c10::cuda::CUDAGuard guard(dy.device());
+    AveyLinearParams p = linear_params(x_sizes, w_sizes, offs.defined() ? &offs : nullptr, dy, call[0]);
+    Tensor w, xr;
+    if (need_x) set_weight(p, w = as_weight(weight));
+    if (need_w) set_x(p, xr = as_rows(x, p.d_in));
     const Tensor g = as_rows(dy, p.d_out);
     p.dy = g.const_data_ptr();
     p.dy_ld = row_ld(g, p.d_out);
     if (deriv.defined()) p.deriv = deriv.data_ptr();
     if (need_x) {
-      out[0] = at::empty(x.sizes(), x.options());
+      out[0] = at::empty(x_sizes, dy.options());
       p.dx = out[0].data_ptr();
       p.dx_ld = p.d_in;
     }
     if (need_w) {
-      out[1] = at::empty(weight.sizes(), weight.options());
+      out[1] = at::empty(w_sizes, dy.options());
       p.dweight = out[1].data_ptr();
     }
     if (need_b) {
-      out[2] = has_bias == 2 ? at::empty({p.groups, p.d_out}, x.options()) : at::empty({p.d_out}, x.options());
+      out[2] = has_bias == 2 ? at::empty({p.groups, p.d_out}, dy.options()) : at::empty({p.d_out}, dy.options());
       p.dbias = out[2].data_ptr();
     }
-    const Tensor ws = workspace(p, 1, x);
+    const Tensor ws = workspace(p, 1, dy);
     check_status(lib.linear_bwd(&p, at::cuda::getCurrentCUDAStream().stream()));
     return out;
   }

@@ -437,7 +437,8 @@ typedef struct AveyLinearParams {
   int64_t y_ld;
   void* deriv; /* 32-byte aligned; forward: or NULL */
 
-  /* Backward (y, residual and bias are not read). NULL: not wanted. */
+  /* Backward (y, residual and bias are not read, x for dweight only and weight
+   * for dx only). NULL: not wanted. */
   const void* dy; /* [rows][d_out] */
   int64_t dy_ld;
   void* dx; /* [rows][d_in] */

@@ -903,3 +903,43 @@ def test_grouped_rows_go_by_the_size_of_the_product(rows, groups, k, n, few):
     p = _params(rows=rows, groups=groups, d_in=k, d_out=n, offsets=1 << 20, x=(1 << 20) + 2, x_ld=k, weight_ld=k,
                 weight_group_stride=n * k, y_ld=n)
     assert (_native.linear_workspace_size(p) == 0) == few
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('grouped', [False, True])
+def test_only_what_a_gradient_needs_has_to_stay_as_it_was(grouped):
+    """Frozen weights need no x for the backward pass, constant inputs no weights, a
+    bias neither: those may change in place in between, as with torch's layers."""
+    x, w, b, _, dy = data(130, 64, 72, torch.bfloat16, 27, (2,) if grouped else ())
+    off = torch.tensor([0, 50, 130], device='cuda', dtype=torch.int32)
+
+    def layer(x, w, b):
+        return (experts.expert_linear(x, w, off, b, activation='silu') if grouped else
+                layers.residual_linear(x, w, b, activation='silu'))
+
+    full = [t.detach().requires_grad_(True) for t in (x, w, b)]
+    want = torch.autograd.grad(layer(*full), full, dy)
+    for i, spoiled in ((0, (0, 2)), (1, (1, 2)), (2, (0, 1, 2))):
+        leaves = [t.clone().requires_grad_(j == i) for j, t in enumerate((x, w, b))]
+        y = layer(*leaves)
+        with torch.no_grad():
+            for j in spoiled:
+                leaves[j].zero_()
+        (got,) = torch.autograd.grad(y, leaves[i], dy)
+        assert torch.equal(got, want[i])
+    for i, needed in ((0, 1), (1, 0)):  # and what is needed is still guarded
+        leaves = [t.clone().requires_grad_(j == i) for j, t in enumerate((x, w, b))]
+        y = layer(*leaves)
+        with torch.no_grad():
+            leaves[needed].zero_()
+        with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+            torch.autograd.grad(y, leaves[i], dy)
+
+
+@pytest.mark.parametrize('change,match', [
+    (dict(x=0, dweight=6 << 20), 'x is required'), (dict(weight=0), 'weight is required')])
+def test_c_backward_entry_wants_the_operands_of_what_is_wanted(change, match):
+    with pytest.raises(_native.NativeError, match=match):
+        _native.linear(_params(**change), 0, backward=True)
+    _native.linear_workspace_size(_params(x=0), backward=True)
+    _native.linear_workspace_size(_params(weight=0, dx=0, dweight=6 << 20), backward=True)
