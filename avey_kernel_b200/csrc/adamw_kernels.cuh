@@ -66,6 +66,8 @@ struct AwScalars {
   const float* grad_scale;
 };
 
+// A 32-bit mix of two products, constants from C. Wellons, "Prospecting for hash
+// functions" (2018).
 __device__ __forceinline__ uint32_t aw_mix(uint32_t x) {
   x ^= x >> 16;
   x *= 0x7feb352du;
@@ -330,13 +332,12 @@ __global__ void __launch_bounds__(kAwThreads) adamw_step(const __grid_constant__
 // At 10 bytes an element HBM leaves about 55 instructions an element, so the
 // whole blocks of aligned tensors take a loop of their own: two values to an
 // instruction (f32x2), three-input minima and maxima, one square root step for
-// a pair, and the next chunks' loads in flight (cp.async): 58 instructions. 64 M
-// bf16 parameters take 174 us (3.85 TB/s) against 224 us by the general code on
-// every block (87 instructions an element). The same loop without its arithmetic
-// takes 123 us (5.5 TB/s); the arithmetic is spread over decoding, the root, the
-// hash and the two roundings (leaving out the hash and roundings 152 us, the
-// exact root 165 us), and four CTAs per SM, two stages or ranges of consecutive
-// chunks per CTA changed it by less than 5%.
+// a pair, and the next chunks' loads in flight (cp.async). 64 M bf16 parameters
+// take 168 us (4.0 TB/s) with 65 instructions an element. Counters of that
+// launch: issue slots 73% busy, the pipe of integer products and fp32 pairs 60%,
+// the one of logic and comparisons 50%; of 6.9 warps a scheduler, 1.7 stand ready
+// behind another, 1.6 wait out an instruction's latency, 1.1 for a pipe and 0.1 for
+// memory. So the arithmetic bounds it, through no single pipe.
 
 typedef unsigned long long AwPair;
 __device__ __forceinline__ AwPair aw_pair(float lo, float hi) {
@@ -386,10 +387,13 @@ __device__ __forceinline__ float aw_rsqrt(float x) {
   asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// sqrt(v) of a pair, correctly rounded for v in [2^-100, 2^100]: with y about
-// 1 / sqrt(v) and s = v y, the residual v - s^2 is exact in one fused operation
-// and s + (residual) y / 2 rounds correctly (P. Markstein, "Computation of
-// elementary functions on the IBM RISC System/6000 processor", 1990).
+// sqrt(v) of a pair for v in [2^-100, 2^100]: with y about 1 / sqrt(v) and s = v y,
+// the residual v - s^2 is exact in one fused operation and s + (residual) y / 2 is
+// within 2^-20 of a unit in the last place before its rounding (P. Markstein,
+// "Computation of elementary functions on the IBM RISC System/6000 processor",
+// 1990). That gives the nearest value but for the few mantissas whose root is as
+// close to the middle of two (3.72775697 gives 1.93073797 for 1.93073809 unless y is
+// the nearest value itself): far below the 20 bits that round it to a code.
 __device__ __forceinline__ AwPair aw_sqrt2(AwPair v) {
   const float2 a = aw_split(v);
   const AwPair y = aw_pair(aw_rsqrt(a.x), aw_rsqrt(a.y));
@@ -405,7 +409,7 @@ __device__ __forceinline__ float aw_rcp(float x) {
 }
 
 // The codes of eight m and sqrt(v) of the elements `idx` ^ 0..7 (element number
-// and key). FAST: none is below 2^-6 of its scale but zeros.
+// and key). FAST: none is below 2^-6 of its scale, and none is zero.
 template <bool FAST>
 __device__ __forceinline__ void aw_codes(const AwPair (&m)[4], const AwPair (&u)[4], float mi, float vi, uint32_t idx,
                                          AwRaw<8>& mc, AwRaw<8>& vc) {
@@ -583,8 +587,8 @@ __global__ void __launch_bounds__(kAwThreads, kAwCtas8) adamw8_step(const __grid
 #pragma unroll
     for (int i = 0; i < 8; ++i) reinterpret_cast<T*>(&po)[i] = aw_from_f<T>(pn[i]);
     aw_st<8 * sizeof(T)>(static_cast<T*>(t.p) + at + off, po);
-    // Codes. Values below 2^-6 (1 / 28672 of the block's maximum) are rare: a
-    // block that has none takes the short rounding.
+    // Codes. Values below 2^-6 (1 / 28672 of the block's maximum) and zeros are rare:
+    // a block that has none takes the short rounding.
     AwRaw<8> mc{}, vc{};
     if (!__any_sync(0xFFFFFFFFu, mmin * mi < 0x1p-6f || sqrtf(vmin) * vi < 0x1p-6f))
       aw_codes<true>(m, u, mi, vi, idx, mc, vc);

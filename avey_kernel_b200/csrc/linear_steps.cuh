@@ -180,8 +180,11 @@ __global__ void __launch_bounds__(32 * WARPS) ln_few(const LnFew q) {
 // ---------------------------------------------------------------- dpre
 
 // dpre = dy act' in the operand type, and the fp32 sums of dpre (before that
-// rounding) over every tile of 64 rows of a group. Bound by HBM: 6 bytes an
-// element. A warp reads rows of 512 bytes, a thread 8 columns of 8 rows at once,
+// rounding) over every tile of 64 rows of a group. The rounding is what 16-bit
+// operands of the two products take: it makes the error of dx and dW against 64
+// bits 1.41 times that of an fp32 dpre (2.3 10^-3 of their norm in bf16, 2.9 10^-4 in
+// f16; the results' own rounding is the rest), and a second 16-bit part for what it
+// cuts off would double both products. Bound by HBM: 6 bytes an element. A warp reads rows of 512 bytes, a thread 8 columns of 8 rows at once,
 // all loads before the first product (32768 x 1536: 54 us, 5.6 TB/s).
 constexpr int kLdThreads = 256;
 constexpr int kLdCols = 256;

@@ -27,7 +27,7 @@
 // Measured (bf16, one B200): 32768 x 768 x 1536 forward with bias and any
 // activation 70-74 us (1,050-1,110 TFLOP/s; torch.matmul 62-64), with residual 88,
 // for training with residual and codes 99-101 (350 MB moved, 3.5 TB/s); dX 66,
-// dW 67-69 and 4 for its partial sums; 8192 x 4096 x 4096 forward 183-191
+// dW 67-69 (77 with the set-up beside dX's end) and 4 for its partial sums; 8192 x 4096 x 4096 forward 183-191
 // (1,440-1,500 TFLOP/s; torch.matmul 179-207). Tiles of 128 columns instead of 256:
 // dX 89, dW 102 us, so what an SM takes in and reads back from shared memory for
 // its products is the bound of the bare product.
@@ -172,9 +172,11 @@ __device__ __forceinline__ LnPair ln_act2(LnPair x, LnPair* d) {
 }
 
 // 16-bit codes of act' kept for the backward pass. relu, silu and gelu have
-// derivatives in (-0.2, 1.2): fixed point in steps of 2^-14 from -1/4, which adds
-// an eighth of an f16 rounding to dpre (the pre-activation in 16 bits would add
-// one or more of the operand type's own). relu2's (2 relu(x)) is unbounded and
+// derivatives in (-0.2, 1.2): fixed point in steps of 2^-14 from -1/4, which moves
+// dpre by at most 2^-15 |dy|. That is an eighth of an f16 rounding where the
+// derivative is near 1 (the pre-activation in 16 bits would add one or more of the
+// operand type's own), and more of a small one: one below 2^-15, of a unit far on
+// its flat side, becomes 0. relu2's (2 relu(x)) is unbounded and
 // not negative: the fp32 bit pattern in equal steps from a base, which spreads
 // 2^16 codes over 128 binades for bf16 (2^-62 .. 2^66, half steps of 2^-10) and
 // over 25 for f16 (2^-15 .. 2^10, half steps of 2^-12.3); zero below. Both hold

@@ -247,7 +247,8 @@ def residual_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.
     bf16 / f16 CUDA tensors of one dtype run natively, forward and backward
     (fp32 sums; y and the gradients are rounded once, the gradient at the
     product is rounded to the operand type before its two products, so in f16
-    it is infinite past f16's range, as in torch's). Few rows
+    it is infinite past f16's range, as in torch's; silu' and gelu' are kept to
+    2^-15, relu2' to 2^-10 or, in f16, 2^-12 of itself). Few rows
     (single tokens of a batch; up to 256 where the layer is small) have a kernel
     of their own. Views with any row stride are read in place. Tensors with
     forward-mode tangents and calls under a trace (``torch.jit.trace``, ``make_fx``)

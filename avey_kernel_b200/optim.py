@@ -71,7 +71,8 @@ def _quantize(x: torch.Tensor, noise: torch.Tensor):
 
 
 def _hash(start: int, n: int, seed: int, step: int, device) -> torch.Tensor:
-    """The 32-bit hashes of elements start .. start + n - 1 of a call."""
+    """The 32-bit hashes of elements start .. start + n - 1 of a call (constants from
+    C. Wellons, "Prospecting for hash functions", 2018)."""
     i = torch.arange(start, start + n, device=device)
     key = (seed + 0x9e3779b9 * (step + (i >> 32))) & _MASK
     for mul in (0x7feb352d, 0x846ca68b):

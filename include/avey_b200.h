@@ -411,7 +411,9 @@ AVEY_API int avey_fwd_presummed_v1(const AveyFwdParams* params, const float* sum
  * and each result is rounded once; dpre is rounded to dtype before the two
  * products of the backward pass. The forward pass writes act' as 16-bit codes
  * into deriv when it is given (d_out rounded up to 16 values a row; any
- * activation but the identity), and the backward pass reads them. Gradients
+ * activation but the identity), and the backward pass reads them: relu exactly,
+ * silu and gelu to 2^-15, relu2 to 2^-10 (bf16, up to 2^66) or 2^-12 (f16, up to
+ * 2^10) of itself, which holds wherever y is finite. Gradients
  * use fixed orders: results are bitwise reproducible.
  *
  * Last dimensions have stride 1; row strides (ld) and group strides are in
@@ -491,7 +493,8 @@ AVEY_API int avey_linear_workspace_size(const AveyLinearParams* params, int back
  *   key = mix2(seed + 0x9e3779b9 (step + high32(i))) (all mod 2^32),
  * where mix is x ^= x >> 16; x *= 0x7feb352d; x ^= x >> 15; x *= 0x846ca68b;
  * x ^= x >> 16 and mix2 is x = (x ^ x >> 16) * 0x7feb352d, x = (x ^ x >> 16) *
- * 0x846ca68b. The same call gives the same bits. A block that gets a
+ * 0x846ca68b (constants from C. Wellons, "Prospecting for hash functions", 2018).
+ * The same call gives the same bits. A block that gets a
  * non-finite value has non-finite or undefined states from then on.
  */
 #define AVEY_ADAMW_BLOCK 256
