@@ -412,8 +412,8 @@ AVEY_API int avey_fwd_presummed_v1(const AveyFwdParams* params, const float* sum
  * products of the backward pass. The forward pass writes act' as 16-bit codes
  * into deriv when it is given (d_out rounded up to 16 values a row; any
  * activation but the identity), and the backward pass reads them: relu exactly,
- * silu and gelu to 2^-15, relu2 to 2^-10 (bf16, up to 2^66) or 2^-12 (f16, up to
- * 2^10) of itself, which holds wherever y is finite. Gradients
+ * silu and gelu to 2^-15, relu2 to 2^-10 of itself from 2^-62 to 2^66 (bf16) or
+ * 2^-12 from 2^-15 to 2^10 (f16) and as 0 below, so wherever y is finite. Gradients
  * use fixed orders: results are bitwise reproducible.
  *
  * Last dimensions have stride 1; row strides (ld) and group strides are in
