@@ -28,7 +28,9 @@ EXPORTS = ('avey_fwd_v1', 'avey_fwd_plan', 'avey_fwd_workspace_size', 'avey_fwd_
            'avey_bwd_step_v1', 'avey_bwd_workspace_size',
            'avey_last_error', 'avey_device_status', 'avey_launch_count', 'avey_abi_version',
            'avey_test_hooks_v1', 'avey_gemm_v1', 'avey_fwd_presummed_v1', 'avey_adamw_v1',
-           'avey_linear_fwd_v1', 'avey_linear_bwd_v1', 'avey_linear_workspace_size')
+           'avey_linear_fwd_v1', 'avey_linear_bwd_v1', 'avey_linear_workspace_size',
+           'avey_loss_fwd_v1', 'avey_loss_bwd_v1', 'avey_loss_workspace_size')
+REDUCTION_IDS = {'none': 0, 'sum': 1, 'mean': 2}
 LINEAR_AUTO, LINEAR_TCGEN05, LINEAR_FEW = 0, 1, 2
 BWD_PREP, BWD_SCORES, BWD_EPILOGUE, BWD_DSCORES, BWD_FINAL = range(5)
 NOALLOC_MAX_ROWS = 1 << 20
@@ -186,6 +188,35 @@ class AveyLinearParams(ctypes.Structure):
     ]
 
 
+class AveyLossParams(ctypes.Structure):
+    _fields_ = [
+        ('struct_size', ctypes.c_uint32),
+        ('dtype', ctypes.c_int32),
+        ('target_bits', ctypes.c_int32),
+        ('reduction', ctypes.c_int32),
+        ('rows', ctypes.c_int64),
+        ('width', ctypes.c_int64),
+        ('vocab', ctypes.c_int64),
+        ('x', ctypes.c_void_p),
+        ('x_ld', ctypes.c_int64),
+        ('weight', ctypes.c_void_p),
+        ('weight_ld', ctypes.c_int64),
+        ('targets', ctypes.c_void_p),
+        ('target_stride', ctypes.c_int64),
+        ('ignore_index', ctypes.c_int64),
+        ('z_loss', ctypes.c_double),
+        ('loss', ctypes.c_void_p),
+        ('saved', ctypes.c_void_p),
+        ('dloss', ctypes.c_void_p),
+        ('dloss_stride', ctypes.c_int64),
+        ('dx', ctypes.c_void_p),
+        ('dx_ld', ctypes.c_int64),
+        ('dweight', ctypes.c_void_p),
+        ('workspace', ctypes.c_void_p),
+        ('workspace_bytes', ctypes.c_uint64),
+    ]
+
+
 class AveyAdamWTensor(ctypes.Structure):
     _fields_ = [
         ('param', ctypes.c_void_p),
@@ -297,6 +328,12 @@ def lib() -> ctypes.CDLL:
         dll.avey_linear_workspace_size.argtypes = [ctypes.POINTER(AveyLinearParams), ctypes.c_int,
                                                    ctypes.POINTER(ctypes.c_uint64)]
         dll.avey_linear_workspace_size.restype = ctypes.c_int
+        for name in ('avey_loss_fwd_v1', 'avey_loss_bwd_v1'):
+            getattr(dll, name).argtypes = [ctypes.POINTER(AveyLossParams), ctypes.c_void_p]
+            getattr(dll, name).restype = ctypes.c_int
+        dll.avey_loss_workspace_size.argtypes = [ctypes.POINTER(AveyLossParams), ctypes.c_int,
+                                                 ctypes.POINTER(ctypes.c_uint64)]
+        dll.avey_loss_workspace_size.restype = ctypes.c_int
         if dll.avey_abi_version() != ABI_VERSION:
             raise RuntimeError(f'{path}: ABI version {dll.avey_abi_version()} != {ABI_VERSION}')
         _lib = dll
@@ -338,6 +375,18 @@ def linear(params: AveyLinearParams, stream: int, backward: bool = False) -> Non
 def linear_workspace_size(params: AveyLinearParams, backward: bool = False) -> int:
     out = ctypes.c_uint64(0)
     _check(lib().avey_linear_workspace_size(ctypes.byref(params), int(backward), ctypes.byref(out)))
+    return int(out.value)
+
+
+def loss(params: AveyLossParams, stream: int, backward: bool = False) -> None:
+    """avey_loss_fwd_v1 / avey_loss_bwd_v1: enqueue a cross entropy or its gradients."""
+    call = lib().avey_loss_bwd_v1 if backward else lib().avey_loss_fwd_v1
+    _check(call(ctypes.byref(params), ctypes.c_void_p(stream)))
+
+
+def loss_workspace_size(params: AveyLossParams, backward: bool = False) -> int:
+    out = ctypes.c_uint64(0)
+    _check(lib().avey_loss_workspace_size(ctypes.byref(params), int(backward), ctypes.byref(out)))
     return int(out.value)
 
 

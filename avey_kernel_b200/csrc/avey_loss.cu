@@ -1,0 +1,485 @@
+// C ABI of the cross entropy over a vocabulary (declared in include/avey_b200.h):
+// argument checks, tile choice, workspace layout and the launches of tc_loss.cuh.
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cstdio>
+#include <mutex>
+
+#include "avey_b200.h"
+#include "host_api.h"
+#include "tc_loss.cuh"
+#include "linear_steps.cuh"
+
+namespace {
+
+int fail(int code, const char* msg) { return avey_host::set_error(code, msg); }
+
+constexpr int kMaxDevices = 64;
+
+template <auto K>
+cudaError_t smem_opt_in() {
+  static std::once_flag once[kMaxDevices];
+  static cudaError_t err[kMaxDevices];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return cudaErrorInvalidDevice;
+  std::call_once(once[dev], [dev] {
+    err[dev] = cudaFuncSetAttribute(K, cudaFuncAttributeMaxDynamicSharedMemorySize, avey::kCeSmem);
+  });
+  return err[dev];
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+bool whole_rows(const void* p, int64_t ld) { return aligned16(p) && ld % 8 == 0; }
+int64_t up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
+
+int validate(const AveyLossParams* p, bool backward) {
+  if (!p) return fail(AVEY_ERR_ARGUMENT, "params is NULL");
+  if (p->struct_size != sizeof(AveyLossParams))
+    return fail(AVEY_ERR_ARGUMENT, "struct_size does not match sizeof(AveyLossParams)");
+  if (p->dtype != AVEY_BF16 && p->dtype != AVEY_F16)
+    return fail(AVEY_ERR_ARGUMENT, "the cross entropy takes bf16 or f16 operands");
+  if (p->target_bits != 32 && p->target_bits != 64) return fail(AVEY_ERR_ARGUMENT, "targets have 32 or 64 bits");
+  if (p->reduction < AVEY_LOSS_NONE || p->reduction > AVEY_LOSS_MEAN)
+    return fail(AVEY_ERR_ARGUMENT, "unknown reduction");
+  if (p->rows < 0 || p->rows > (1 << 30) || p->width < 1 || p->width > (1 << 22) || p->vocab < 1 ||
+      p->vocab > (1 << 30))
+    return fail(AVEY_ERR_ARGUMENT, "rows must be in [0, 2^30], width in [1, 2^22], vocab in [1, 2^30]");
+  if ((p->rows / 256 + 1) > (1ll << 30) / (p->vocab / 64 + 1) ||
+      (std::max(p->rows, p->vocab) / 256 + 1) > (1ll << 30) / (p->width / 64 + 1))
+    return fail(AVEY_ERR_ARGUMENT, "too many tiles");
+  if (!(p->z_loss > -1e30 && p->z_loss < 1e30)) return fail(AVEY_ERR_ARGUMENT, "z_loss must be finite");
+  uintptr_t odd = 0;
+  for (const void* a : {p->x, p->weight, const_cast<const void*>(p->dx), const_cast<const void*>(p->dweight)})
+    odd |= reinterpret_cast<uintptr_t>(a) & 1u;
+  for (const void* a : {static_cast<const void*>(p->loss), static_cast<const void*>(p->saved),
+                        static_cast<const void*>(p->dloss)})
+    odd |= reinterpret_cast<uintptr_t>(a) & 3u;
+  if (odd != 0 || (reinterpret_cast<uintptr_t>(p->targets) & (p->target_bits / 8 - 1)) != 0)
+    return fail(AVEY_ERR_ARGUMENT, "arrays must be aligned to their elements");
+  if (!backward && !p->loss && (p->rows > 0 || p->reduction != AVEY_LOSS_NONE))
+    return fail(AVEY_ERR_ARGUMENT, "loss is required");
+  if (p->rows > 0 && (!p->x || !p->targets)) return fail(AVEY_ERR_ARGUMENT, "x and targets are required");
+  if (p->rows > 0 && !p->weight) return fail(AVEY_ERR_ARGUMENT, "weight is required");
+  if (p->x_ld < p->width || p->weight_ld < p->width || p->target_stride < 0)
+    return fail(AVEY_ERR_ARGUMENT, "strides must cover the rows");
+  if (backward && p->rows > 0) {
+    if (!p->saved || !p->dloss) return fail(AVEY_ERR_ARGUMENT, "saved and dloss are required");
+    if ((p->dx && p->dx_ld < p->width) || p->dloss_stride < 0)
+      return fail(AVEY_ERR_ARGUMENT, "strides must cover the rows");
+  }
+  return AVEY_OK;
+}
+
+int pairs() { return avey_host::multiprocessors() / 2; }
+
+// Columns of a tile of the logits: 256 read the fewest bytes for their products;
+// narrower ones are taken where those would leave the last wave of pairs half empty.
+int logit_cols(int64_t rows, int64_t n) {
+  const int64_t mt = (rows + avey::kCeBM - 1) / avey::kCeBM;
+  for (int bn : {256, 128})
+    if (mt * ((n + bn - 1) / bn) >= 4 * pairs()) return bn;
+  return 64;
+}
+// Of a gradient's product over `width` columns (boxes of 64 for each CTA).
+int grad_cols(int64_t m, int64_t width) {
+  const int64_t mt = (m + avey::kCeBM - 1) / avey::kCeBM;
+  return width > 128 && mt * ((width + 255) / 256) * 4 >= pairs() * 3 ? 256 : 128;
+}
+
+// Workspace of a call, each part 256-byte aligned.
+struct Layout {
+  bool pack_x = false, pack_w = false;
+  uint64_t x = 0, w = 0;
+  // forward
+  int bn = 0, seg = 0;
+  int64_t n_nt = 0, segments = 0;
+  uint64_t partial = 0, picked = 0, each = 0;
+  // backward
+  int64_t piece = 0, pieces = 0;  // columns of dz at a time
+  uint64_t coef = 0, largest = 0, dirty = 0, copy = 0, dz = 0, sums = 0;
+  uint64_t total = 0;
+};
+
+// Bytes of dz kept at a time: 512 MB, or columns of four times the width where
+// that is more, so that dx's sums, read and written for every piece, stay small
+// beside its products.
+int64_t piece_columns(const AveyLossParams* p) {
+  const int64_t most = std::max<int64_t>((512ll << 20) / (2 * p->rows), 4 * p->width);
+  const int64_t tiles = (p->vocab + 255) / 256;
+  int64_t per = std::max<int64_t>(1, most / 256);
+  // dW's tiles in whole waves of pairs, where there is a wave.
+  const int64_t n_nt = (p->width + 255) / 256, waves = per * n_nt / pairs();
+  if (waves > 0) per = std::max<int64_t>(1, waves * pairs() / n_nt);
+  if (per >= tiles) return up(p->vocab, 8);
+  return per * 256;
+}
+
+Layout layout(const AveyLossParams* p, bool backward) {
+  Layout l;
+  uint64_t at = 0;
+  auto take = [&](uint64_t bytes) {
+    const uint64_t o = at;
+    at += (bytes + 255u) & ~uint64_t(255);
+    return o;
+  };
+  if (p->rows == 0) return l;
+  l.pack_x = !whole_rows(p->x, p->x_ld);
+  l.pack_w = !whole_rows(p->weight, p->weight_ld);
+  const uint64_t row = up(p->width, 8) * 2;
+  if (l.pack_x) l.x = take(p->rows * row);
+  if (l.pack_w) l.w = take(p->vocab * row);
+  if (!backward) {
+    l.bn = logit_cols(p->rows, p->vocab);
+    l.n_nt = (p->vocab + l.bn - 1) / l.bn;
+    const int64_t mt = (p->rows + avey::kCeBM - 1) / avey::kCeBM;
+    // Units of more than one tile where there are enough for the pairs to end together.
+    l.seg = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(avey::kCeMaxSeg, mt * l.n_nt / (16 * pairs()))));
+    l.segments = (l.n_nt + l.seg - 1) / l.seg;
+    l.partial = take(l.segments * p->rows * 8);
+    l.picked = take(p->rows * 4);
+    if (p->reduction != AVEY_LOSS_NONE) l.each = take(p->rows * 4);
+  } else {
+    l.piece = piece_columns(p);
+    l.pieces = (p->vocab + l.piece - 1) / l.piece;
+    l.coef = take(p->rows * 8);
+    l.largest = take(4);
+    if (p->dweight) {
+      l.dirty = take((p->rows + 63) / 64);
+      l.copy = take(p->rows * row);
+    }
+    l.dz = take(p->rows * l.piece * 2);
+    if (p->dx && l.pieces > 1) l.sums = take(p->rows * up(p->width, 4) * 4);
+  }
+  l.total = at;
+  return l;
+}
+
+int check_workspace(const AveyLossParams* p, const Layout& l) {
+  if (l.total == 0) return AVEY_OK;
+  if (!p->workspace || p->workspace_bytes < l.total)
+    return fail(AVEY_ERR_ARGUMENT, "workspace is smaller than avey_loss_workspace_size");
+  if ((reinterpret_cast<uintptr_t>(p->workspace) & 255u) != 0)
+    return fail(AVEY_ERR_ARGUMENT, "workspace must be 256-byte aligned");
+  return AVEY_OK;
+}
+
+// Launches of a call: all but the first may be set up beside the end of the one
+// before (each waits for it ahead of its first read).
+struct Chain {
+  cudaStream_t stream;
+  bool after = false;
+
+  template <typename... Params, typename... Args>
+  int launch(const char* what, void (*kernel)(Params...), int64_t grid, int block, int smem, int cluster,
+             Args... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(grid));
+    cfg.blockDim = dim3(static_cast<unsigned>(block));
+    cfg.dynamicSmemBytes = static_cast<size_t>(smem);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    int n = 0;
+    if (cluster > 1) {
+      attr[n].id = cudaLaunchAttributeClusterDimension;
+      attr[n].val.clusterDim.x = static_cast<unsigned>(cluster);
+      attr[n].val.clusterDim.y = 1;
+      attr[n].val.clusterDim.z = 1;
+      ++n;
+    }
+    if (after) {
+      attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+      attr[n].val.programmaticStreamSerializationAllowed = 1;
+      ++n;
+    }
+    cfg.attrs = attr;
+    cfg.numAttrs = static_cast<unsigned>(n);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
+    if (e != cudaSuccess) {
+      char buf[256];
+      snprintf(buf, sizeof(buf), "%s launch: %s", what, cudaGetErrorString(e));
+      return fail(AVEY_ERR_LAUNCH, buf);
+    }
+    avey_host::count_launches(1);
+    after = true;
+    return AVEY_OK;
+  }
+};
+
+struct Rows {
+  const void* p;
+  int64_t ld;
+};
+
+int pack_inputs(const AveyLossParams* p, const Layout& l, Rows* x, Rows* w, Chain& chain) {
+  char* ws = static_cast<char*>(p->workspace);
+  *x = {p->x, p->x_ld};
+  *w = {p->weight, p->weight_ld};
+  if (!l.pack_x && !l.pack_w) return AVEY_OK;
+  avey::LnPack a{}, b{};
+  a.ld = b.ld = up(p->width, 8);
+  a.cols = b.cols = static_cast<int>(p->width);
+  if (l.pack_x) {
+    a.src = static_cast<const uint16_t*>(p->x);
+    a.src_ld = p->x_ld;
+    a.per = a.rows = p->rows;
+    a.dst = reinterpret_cast<uint16_t*>(ws + l.x);
+    *x = {a.dst, a.ld};
+  }
+  if (l.pack_w) {
+    b.src = static_cast<const uint16_t*>(p->weight);
+    b.src_ld = p->weight_ld;
+    b.per = b.rows = p->vocab;
+    b.dst = reinterpret_cast<uint16_t*>(ws + l.w);
+    *w = {b.dst, b.ld};
+  }
+  const int64_t pieces = (a.rows + b.rows) * (a.ld / 8);
+  const int64_t grid = std::min<int64_t>((pieces + 255) / 256, avey_host::multiprocessors() * 16ll);
+  return chain.launch("row copy", avey::ln_pack_rows, grid, 256, 0, 1, a, b);
+}
+
+struct Maps {
+  CUtensorMap a{}, b{}, b2{}, y{};
+};
+
+template <auto K>
+int launch_product(const Maps& m, const avey::CeGeom& q, Chain& chain) {
+  const cudaError_t attr = smem_opt_in<K>();
+  if (attr != cudaSuccess) return fail(AVEY_ERR_CUDA, cudaGetErrorString(attr));
+  return chain.launch("cross entropy product", K, 2ll * std::min<int64_t>(q.units, pairs()), avey::kCeThreads,
+                      avey::kCeSmem, 2, m.a, m.b, m.b2, m.y, q);
+}
+
+avey::CeGeom geom(const AveyLossParams* p, int64_t m, int64_t n, int64_t k, int bn) {
+  avey::CeGeom q{};
+  q.m = static_cast<int>(m);
+  q.n = static_cast<int>(n);
+  q.k = static_cast<int>(k);
+  q.bn = bn;
+  q.n_mt = static_cast<int>((m + avey::kCeBM - 1) / avey::kCeBM);
+  q.n_nt = static_cast<int>((n + bn - 1) / bn);
+  q.seg = 1;
+  q.units = q.n_mt * q.n_nt;
+  q.stage_bytes = avey::kCeHalfA + bn * avey::kLnBK;
+  q.stages = std::min(avey::kCeMaxStages, avey::kCeRing / q.stage_bytes);
+  q.rows = static_cast<int>(p->rows);
+  q.vocab = static_cast<int>(p->vocab);
+  q.targets = p->targets;
+  q.target_stride = p->target_stride;
+  q.target64 = p->target_bits == 64;
+  q.ignore = p->ignore_index;
+  q.test_stall = avey_host::test_stall();
+  return q;
+}
+
+avey::CeRows rows_of(const AveyLossParams* p) {
+  avey::CeRows q{};
+  q.rows = static_cast<int>(p->rows);
+  q.vocab = static_cast<int>(p->vocab);
+  q.targets = p->targets;
+  q.target_stride = p->target_stride;
+  q.target64 = p->target_bits == 64;
+  q.ignore = p->ignore_index;
+  q.z_loss = static_cast<float>(p->z_loss);
+  return q;
+}
+
+template <typename T>
+int forward(const AveyLossParams* p, cudaStream_t stream) {
+  const Layout l = layout(p, false);
+  int rc = check_workspace(p, l);
+  if (rc != AVEY_OK) return rc;
+  char* ws = static_cast<char*>(p->workspace);
+  Chain chain{stream};
+  Rows x, w;
+  rc = pack_inputs(p, l, &x, &w, chain);
+  if (rc != AVEY_OK) return rc;
+  avey::CeGeom q = geom(p, p->rows, p->vocab, p->width, l.bn);
+  q.seg = l.seg;
+  q.units = static_cast<int>(l.segments) * q.n_mt;
+  q.partial = reinterpret_cast<float2*>(ws + l.partial);
+  q.picked = reinterpret_cast<float*>(ws + l.picked);
+  Maps m;
+  rc = avey_host::encode_rows16(p->dtype, x.p, p->width, p->rows, 1, x.ld * 2, 0, 128, &m.a);
+  if (rc == AVEY_OK) rc = avey_host::encode_rows16(p->dtype, w.p, p->width, p->vocab, 1, w.ld * 2, 0, l.bn / 2, &m.b);
+  if (rc != AVEY_OK) return rc;
+  rc = launch_product<avey::ce_product<T, avey::kCeStats, false>>(m, q, chain);
+  if (rc != AVEY_OK) return rc;
+  avey::CeRows r = rows_of(p);
+  r.segments = static_cast<int>(l.segments);
+  r.partial = q.partial;
+  r.picked = q.picked;
+  const bool none = p->reduction == AVEY_LOSS_NONE;
+  r.each = none ? p->loss : reinterpret_cast<float*>(ws + l.each);
+  r.lse = p->saved;
+  r.per = 32;
+  while (r.per > 1 && r.per / 2 >= p->rows) r.per /= 2;
+  rc = chain.launch("cross entropy rows", avey::ce_rows, (p->rows + r.per - 1) / r.per, 256, 0, 1, r);
+  if (rc != AVEY_OK || none) return rc;
+  return chain.launch("cross entropy total", avey::ce_total, 1, 1024, 0, 1, r, p->reduction == AVEY_LOSS_MEAN ? 1 : 0,
+                      p->loss, p->saved ? p->saved + p->rows : nullptr);
+}
+
+template <typename T>
+int backward(const AveyLossParams* p, cudaStream_t stream) {
+  const Layout l = layout(p, true);
+  int rc = check_workspace(p, l);
+  if (rc != AVEY_OK) return rc;
+  char* ws = static_cast<char*>(p->workspace);
+  Chain chain{stream};
+  uint32_t* largest = nullptr;
+  if (p->dtype == AVEY_F16) {
+    largest = reinterpret_cast<uint32_t*>(ws + l.largest);
+    const cudaError_t e = cudaMemsetAsync(largest, 0, 4, stream);
+    if (e != cudaSuccess) return fail(AVEY_ERR_CUDA, cudaGetErrorString(e));
+  }
+  Rows x, w;
+  rc = pack_inputs(p, l, &x, &w, chain);
+  if (rc != AVEY_OK) return rc;
+  avey::CeCoef k{};
+  k.rows = static_cast<int>(p->rows);
+  k.vocab = static_cast<int>(p->vocab);
+  k.width = static_cast<int>(p->width);
+  k.targets = p->targets;
+  k.target_stride = p->target_stride;
+  k.target64 = p->target_bits == 64;
+  k.ignore = p->ignore_index;
+  k.lse = p->saved;
+  k.count = p->reduction == AVEY_LOSS_MEAN ? p->saved + p->rows : nullptr;
+  k.dy = p->dloss;
+  k.dy_stride = p->reduction == AVEY_LOSS_NONE ? p->dloss_stride : 0;
+  k.z_loss = static_cast<float>(p->z_loss);
+  k.coef = reinterpret_cast<float2*>(ws + l.coef);
+  k.largest = largest;
+  if (p->dweight) {
+    k.x = static_cast<const uint16_t*>(x.p);
+    k.x_ld = x.ld;
+    k.copy = reinterpret_cast<uint16_t*>(ws + l.copy);
+    k.copy_ld = up(p->width, 8);
+    k.dirty = reinterpret_cast<uint8_t*>(ws + l.dirty);
+  }
+  rc = chain.launch("cross entropy coefficients", avey::ce_coef<T>, (p->rows + 63) / 64, 256, 0, 1, k);
+  if (rc != AVEY_OK) return rc;
+  char* dz = ws + l.dz;
+  const int64_t sums_ld = up(p->width, 4);
+  float* sums = reinterpret_cast<float*>(ws + l.sums);
+  const bool planes = l.pieces > 1;
+  for (int64_t v0 = 0; v0 < p->vocab; v0 += l.piece) {
+    const int64_t n = std::min(l.piece, p->vocab - v0), ld = up(n, 8);
+    const char* wp = static_cast<const char*>(w.p) + v0 * w.ld * 2;
+    {
+      const int bn = logit_cols(p->rows, n);
+      avey::CeGeom q = geom(p, p->rows, n, p->width, bn);
+      q.seg = static_cast<int>(std::max<int64_t>(
+          1, std::min<int64_t>(avey::kCeMaxSeg, static_cast<int64_t>(q.n_mt) * q.n_nt / (16 * pairs()))));
+      q.units = (q.n_nt + q.seg - 1) / q.seg * q.n_mt;
+      q.col0 = static_cast<int>(v0);
+      q.lse = p->saved;
+      q.coef = k.coef;
+      q.largest = largest;
+      Maps m;
+      rc = avey_host::encode_rows16(p->dtype, x.p, p->width, p->rows, 1, x.ld * 2, 0, 128, &m.a);
+      if (rc == AVEY_OK) rc = avey_host::encode_rows16(p->dtype, wp, p->width, n, 1, w.ld * 2, 0, bn / 2, &m.b);
+      if (rc == AVEY_OK) rc = avey_host::encode_tiles(p->dtype, dz, n, p->rows, 1, ld * 2, 0, &m.y);
+      if (rc == AVEY_OK) rc = launch_product<avey::ce_product<T, avey::kCeGrad, false>>(m, q, chain);
+      if (rc != AVEY_OK) return rc;
+    }
+    if (p->dx) {
+      const int bn = grad_cols(p->rows, p->width);
+      avey::CeGeom q = geom(p, p->rows, p->width, n, bn);
+      q.largest = largest;
+      q.out = p->dx;
+      q.out_ld = p->dx_ld;
+      q.out_vec = whole_rows(p->dx, p->dx_ld);
+      q.add = v0 > 0;
+      Maps m;
+      rc = avey_host::encode_rows16(p->dtype, dz, n, p->rows, 1, ld * 2, 0, 128, &m.a);
+      if (rc == AVEY_OK) rc = avey_host::encode_rows16(p->dtype, wp, p->width, n, 1, w.ld * 2, 0, 64, &m.b);
+      if (rc == AVEY_OK && planes) rc = avey_host::encode_tiles(AVEY_F32, sums, p->width, p->rows, 1, sums_ld * 4, 0, &m.y);
+      if (rc == AVEY_OK && !planes && q.out_vec)
+        rc = avey_host::encode_tiles(p->dtype, p->dx, p->width, p->rows, 1, p->dx_ld * 2, 0, &m.y);
+      if (rc == AVEY_OK)
+        rc = planes ? launch_product<avey::ce_product<T, avey::kCeDx, true>>(m, q, chain)
+                    : launch_product<avey::ce_product<T, avey::kCeDx, false>>(m, q, chain);
+      if (rc != AVEY_OK) return rc;
+    }
+    if (p->dweight) {
+      char* dw = static_cast<char*>(p->dweight) + v0 * p->width * 2;
+      const int bn = grad_cols(n, p->width);
+      avey::CeGeom q = geom(p, n, p->width, p->rows, bn);
+      q.largest = largest;
+      q.out = dw;
+      q.out_ld = p->width;
+      q.out_vec = whole_rows(dw, p->width);
+      q.dirty = k.dirty;
+      Maps m;
+      rc = avey_host::encode_rows16(p->dtype, dz, n, p->rows, 1, ld * 2, 0, 64, &m.a);
+      if (rc == AVEY_OK) rc = avey_host::encode_rows16(p->dtype, x.p, p->width, p->rows, 1, x.ld * 2, 0, 64, &m.b);
+      if (rc == AVEY_OK) rc = avey_host::encode_rows16(p->dtype, k.copy, p->width, p->rows, 1, k.copy_ld * 2, 0, 64, &m.b2);
+      if (rc == AVEY_OK && q.out_vec) rc = avey_host::encode_tiles(p->dtype, dw, p->width, n, 1, p->width * 2, 0, &m.y);
+      if (rc == AVEY_OK) rc = launch_product<avey::ce_product<T, avey::kCeDw, false>>(m, q, chain);
+      if (rc != AVEY_OK) return rc;
+    }
+  }
+  if (p->dx && planes) {
+    const int64_t quads = p->rows * (sums_ld / 4);
+    const int64_t grid = std::min<int64_t>((quads + 255) / 256, avey_host::multiprocessors() * 8ll);
+    rc = chain.launch("dx rounding", avey::ce_finish<T>, grid, 256, 0, 1, sums, sums_ld, p->rows, p->width, largest,
+                      static_cast<T*>(p->dx), p->dx_ld);
+  }
+  return rc;
+}
+
+// Sum and mean of no row, and the gradient of a weight without rows.
+int empty(const AveyLossParams* p, bool backward, cudaStream_t stream) {
+  cudaError_t e = cudaSuccess;
+  if (!backward) {
+    // 0, or the NaN of all ones for 0 / 0.
+    if (p->reduction != AVEY_LOSS_NONE)
+      e = cudaMemsetAsync(p->loss, p->reduction == AVEY_LOSS_MEAN ? 0xFF : 0, 4, stream);
+    if (e == cudaSuccess && p->saved) e = cudaMemsetAsync(p->saved, 0, 4, stream);
+  } else if (p->dweight) {
+    e = cudaMemsetAsync(p->dweight, 0, static_cast<size_t>(p->vocab) * p->width * 2, stream);
+  }
+  return e == cudaSuccess ? AVEY_OK : fail(AVEY_ERR_CUDA, cudaGetErrorString(e));
+}
+
+int run(const AveyLossParams* p, bool back, void* stream) {
+  int rc = validate(p, back);
+  if (rc != AVEY_OK) return rc;
+  rc = avey_host::device_ok();
+  if (rc != AVEY_OK) return rc;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (p->rows == 0) rc = empty(p, back, s);
+  else if (!back) rc = p->dtype == AVEY_BF16 ? forward<__nv_bfloat16>(p, s) : forward<__half>(p, s);
+  else if (p->dx || p->dweight) rc = p->dtype == AVEY_BF16 ? backward<__nv_bfloat16>(p, s) : backward<__half>(p, s);
+  return rc == AVEY_OK ? avey_host::clear_error() : rc;
+}
+
+}  // namespace
+
+namespace avey_host {
+int loss_flags(unsigned int* flags, bool clear) {
+  cudaError_t e = cudaMemcpyFromSymbol(flags, avey::g_devflags, sizeof(*flags));
+  const unsigned int zero = 0;
+  if (e == cudaSuccess && clear) e = cudaMemcpyToSymbol(avey::g_devflags, &zero, sizeof(zero));
+  return e;
+}
+int loss_wait_limit(long long cycles) { return cudaMemcpyToSymbol(avey::g_wait_limit, &cycles, sizeof(cycles)); }
+}  // namespace avey_host
+
+extern "C" {
+
+int avey_loss_workspace_size(const AveyLossParams* p, int backward, uint64_t* bytes) {
+  const int rc = validate(p, backward != 0);
+  if (rc != AVEY_OK) return rc;
+  if (!bytes) return fail(AVEY_ERR_ARGUMENT, "bytes is NULL");
+  *bytes = layout(p, backward != 0).total;
+  return avey_host::clear_error();
+}
+
+int avey_loss_fwd_v1(const AveyLossParams* p, void* stream) { return run(p, false, stream); }
+int avey_loss_bwd_v1(const AveyLossParams* p, void* stream) { return run(p, true, stream); }
+
+}  // extern "C"

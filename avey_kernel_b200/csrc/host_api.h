@@ -36,5 +36,8 @@ bool test_stall();
 // kernels of avey_linear.cu, on the current device; a cudaError_t.
 int linear_flags(unsigned int* flags, bool clear);
 int linear_wait_limit(long long cycles);
+// The same for avey_loss.cu.
+int loss_flags(unsigned int* flags, bool clear);
+int loss_wait_limit(long long cycles);
 
 }  // namespace avey_host

@@ -1,0 +1,699 @@
+// Softmax cross entropy of z = x W^T over a vocabulary, and its gradients, on
+// tcgen05 CTA pairs (avey_loss_*), without keeping z:
+//
+//   stats  (c, s) of every row over a segment of the vocabulary, where
+//          s = sum_j 2^(z_j log2 e - c), and the target's z
+//   grad   dz_ij = a_i 2^(z_ij log2 e - lse_i) - b_i [j = t_i] for a piece of the
+//          vocabulary, z computed again
+//   dX     dx (+)= dz W over the piece       dW    dW = dz^T x for the piece
+//
+// c is the running maximum, so every power is at most 1; lse_i = c + log2 s is
+// kept in base 2, as the hardware's exponential takes it. a_i and b_i hold the
+// gradient that comes in, the z loss's factor and, for f16, a power of two that
+// brings the largest of them to 2^14 (a probability of 1e-5 times 1 / rows is
+// below f16's range); dX and dW divide by it. dz is rounded to the operand type
+// once, as the tensor cores need it; all sums are fp32.
+//
+// Bounds: 2 M V d flops for the loss and 6 M V d for the gradients on the tensor
+// cores. A cluster of two CTAs computes 256 x 256 tiles (cta_group::2): per K
+// block of 64 a CTA takes in 32 KB for 512 cycles of products, just what an SM
+// can (64 bytes a cycle); a CTA alone on a 128 x 256 tile would take in 48 KB.
+// Warp 0 issues TMA, warp 1 of the even CTA tcgen05.mma into one of two TMEM
+// accumulators, warps 4-19 of each CTA drain the other one. Every wait is bounded.
+//
+// stats and grad take the tiles in units of up to 4 column tiles of one row
+// tile, rows first, so that the pairs at work share W's rows in L2 and a row's
+// (c, s) stay in registers over a unit.
+#pragma once
+
+#include "tc_linear.cuh"
+
+namespace avey {
+
+constexpr int kCeThreads = kLnThreads;
+constexpr int kCeBM = 256;                  // rows of a pair's tile
+constexpr int kCeHalfA = 128 * kLnBK * 2;   // a CTA's 128 rows of A: 16 KB
+constexpr int kCeMaxSeg = 4;                // column tiles of a unit
+constexpr int kCeMaxStages = 8;
+constexpr int kCeRing = 196608;
+constexpr int kCeStaging = kLnEpiWarps * kLnStageTile;
+constexpr int kCeCtrlBytes = 512;
+constexpr int kCeSmem = 1024 + kCeRing + kCeStaging + kCeCtrlBytes;
+
+enum CeMode { kCeStats = 0, kCeGrad = 1, kCeDx = 2, kCeDw = 3 };
+
+struct CeGeom {
+  int m, n, k;             // output rows and columns, contraction
+  int bn, n_mt, n_nt;      // columns of a tile, tiles
+  int seg, units;          // column tiles of a unit, units
+  int stages, stage_bytes;
+  int rows;                // tokens
+  int vocab;
+  int col0;                // grad: the piece's first column
+  const void* targets;
+  int64_t target_stride;
+  int target64;
+  int64_t ignore;
+  float2* partial;         // stats: [segments][rows]
+  float* picked;           // stats: the target's z, [rows]
+  const float* lse;        // grad: [rows], base 2
+  const float2* coef;      // grad: (a, b) of every row
+  const uint32_t* largest; // f16: bits of the largest |a|, |b|; null: no scale
+  void* out;               // dX, dW (16 bits), where rows are not stored by TMA
+  int64_t out_ld;
+  int out_vec;
+  int add;                 // dX: sums are added to the fp32 plane
+  const uint8_t* dirty;    // dW: K blocks whose rows come from the second map
+  int test_stall;
+};
+
+// The target of a row: its column, -1 for a row that is ignored, -2 for a
+// target outside the vocabulary.
+__device__ __forceinline__ int ce_target(const void* targets, int64_t stride, int wide, int64_t ignore, int vocab,
+                                         int row) {
+  const int64_t t = wide ? __ldg(static_cast<const long long*>(targets) + row * stride)
+                         : static_cast<int64_t>(__ldg(static_cast<const int32_t*>(targets) + row * stride));
+  if (t == ignore) return -1;
+  return t >= 0 && t < vocab ? static_cast<int>(t) : -2;
+}
+
+// f16: the power of two that brings the largest coefficient into [2^13, 2^14), or
+// its inverse (1 without one; a largest coefficient of zero leaves zeros).
+__device__ __forceinline__ float ce_scale(const uint32_t* largest, bool inverse) {
+  if (!largest) return 1.f;
+  const int e = static_cast<int>(__ldg(largest) >> 23);  // 2^(e - 127) <= largest < 2^(e - 126)
+  int k = e ? 127 + 13 - e : 0;
+  k = max(-126, min(126, k));
+  return __uint_as_float(static_cast<uint32_t>(127 + (inverse ? -k : k)) << 23);
+}
+
+struct CeCtrl {
+  uint64_t full[kCeMaxStages], empty[kCeMaxStages];
+  uint64_t acc_full[2], acc_empty[2];
+  uint64_t settled;
+  uint32_t failed;
+  uint32_t tmem_base;
+};
+static_assert(sizeof(CeCtrl) <= kCeCtrlBytes, "control block too large");
+
+__device__ __forceinline__ void tma_reduce_add_3d(const void* tmap, uint32_t src, int x, int y, int z) {
+  asm volatile(
+      "cp.reduce.async.bulk.tensor.3d.global.shared::cta.add.tile.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(
+          reinterpret_cast<uint64_t>(tmap)),
+      "r"(x), "r"(y), "r"(z), "r"(src)
+      : "memory");
+}
+
+// A pair's i-th tile.
+struct CeTile {
+  int mt, nt;
+  bool first, last;  // of its unit
+  int seg;
+};
+// Walks a pair's tiles in order.
+template <int MODE>
+struct CeWalker {
+  int unit, step, stop;
+  __device__ __forceinline__ CeWalker(int pair, int pairs) : unit(pair), step(pairs), stop(0) {}
+  int nt = 0, mt = 0, sg = 0;
+  __device__ __forceinline__ bool next(const CeGeom& q, CeTile& c) {
+    if (nt >= stop) {
+      if (unit >= q.units) return false;
+      if (MODE == kCeStats || MODE == kCeGrad) {
+        sg = unit / q.n_mt;
+        mt = unit - sg * q.n_mt;
+        nt = sg * q.seg;
+        stop = min(q.n_nt, nt + q.seg);
+      } else {
+        mt = unit / q.n_nt;
+        nt = unit - mt * q.n_nt;
+        stop = nt + 1;
+      }
+      unit += step;
+      c.first = true;
+    } else {
+      c.first = false;
+    }
+    c.mt = mt;
+    c.nt = nt++;
+    c.last = nt >= stop;
+    c.seg = sg;
+    return true;
+  }
+};
+
+// What an epilogue lane holds of its row.
+struct CeRow {
+  int target;
+  float lse, a, b;  // grad
+  float c, s;       // stats
+};
+
+// (c, s) of two parts of a row.
+__device__ __forceinline__ void ce_join(float& c, float& s, float c2, float s2) {
+  const float top = fmaxf(c, c2);
+  // A part without a column, or of infinite negative logits, has c = -inf and adds nothing.
+  const float base = top == -INFINITY ? 0.f : top;
+  s = s * ln_exp2(c - base) + s2 * ln_exp2(c2 - base);
+  c = top;
+}
+
+// 32 columns of a row from column col on: the running maximum and sum.
+template <bool EDGE>
+__device__ __forceinline__ void ce_stats32(uint32_t (&o)[32], int left, CeRow& r) {
+  constexpr float kLog2e = 1.4426950408889634f;
+  if (EDGE) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (j >= left) o[j] = 0xFF800000u;
+  }
+  float top = __uint_as_float(o[0]);
+#pragma unroll
+  for (int j = 1; j < 32; ++j) top = fmaxf(top, __uint_as_float(o[j]));
+  const float c = fmaxf(r.c, top * kLog2e);
+  const float base = c == -INFINITY ? 0.f : c;
+  float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+  for (int j = 0; j < 32; j += 2) {
+    s0 += ln_exp2(fmaf(__uint_as_float(o[j]), kLog2e, -base));
+    s1 += ln_exp2(fmaf(__uint_as_float(o[j + 1]), kLog2e, -base));
+  }
+  r.s = r.s * ln_exp2(r.c - base) + (s0 + s1);
+  r.c = c;
+}
+
+// 32 columns of dz into a staging tile.
+template <typename T, bool HIT>
+__device__ __forceinline__ void ce_grad32(const uint32_t (&o)[32], int at, const CeRow& r, uint32_t tile, int lane) {
+  constexpr float kLog2e = 1.4426950408889634f;
+#pragma unroll
+  for (int p = 0; p < 4; ++p) {
+    uint32_t y[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int i = 8 * p + 2 * j;
+      float d0 = r.a * ln_exp2(fmaf(__uint_as_float(o[i]), kLog2e, -r.lse));
+      float d1 = r.a * ln_exp2(fmaf(__uint_as_float(o[i + 1]), kLog2e, -r.lse));
+      if (HIT) {
+        if (i == at) d0 -= r.b;
+        if (i + 1 == at) d1 -= r.b;
+      }
+      y[j] = r.target == -1 ? 0u : ln_pack<T>(d0, d1);
+    }
+    ln_sts(ln_piece(tile, lane, p), y[0], y[1], y[2], y[3]);
+  }
+}
+
+template <typename T, int MODE, bool F32>
+__global__ void __launch_bounds__(kCeThreads, 1)
+    ce_product(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+               const __grid_constant__ CUtensorMap map_b2, const __grid_constant__ CUtensorMap map_y, const CeGeom q) {
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t base = (raw + 1023u) & ~1023u;
+  const uint32_t staging = base + kCeRing;
+  CeCtrl* ctrl = reinterpret_cast<CeCtrl*>(smem_raw + (base - raw) + kCeRing + kCeStaging);
+  constexpr bool kAMn = MODE == kCeDw, kBMn = MODE == kCeDx || MODE == kCeDw;
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t rank = cluster_rank();
+  const bool leader = rank == 0;
+  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  if (tid == 0) {
+    for (int s = 0; s < q.stages; ++s) {
+      mbar_init(smem_u32(&ctrl->full[s]), 1);
+      mbar_init(smem_u32(&ctrl->empty[s]), 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_u32(&ctrl->acc_full[i]), 1);
+      mbar_init(smem_u32(&ctrl->acc_empty[i]), 2 * kLnEpiWarps);  // the epilogue warps of both CTAs
+    }
+    mbar_init(smem_u32(&ctrl->settled), 1);
+    ctrl->failed = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&map_a);
+    tma_prefetch_desc(&map_b);
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(smem_u32(&ctrl->tmem_base), 512);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();  // both CTAs' barriers and tensor memory are set up
+  tc_fence_after();
+  const uint32_t tmem = ctrl->tmem_base;
+  int fills = 0;
+  // The set-up ran beside the end of the step before; what that wrote is read from here on.
+  griddep_launch_dependents();
+  griddep_wait();
+
+  if (warp == 0) {
+    // ============================================================ TMA producer (both CTAs)
+    if (lane == 0) {
+      const uint64_t keep = l2_policy_evict_last();
+      const int half = q.bn / 2;  // this CTA's columns of B
+      const int nk = (q.k + kLnBK - 1) / kLnBK;
+      int st = 0;
+      uint32_t ph = 0;
+      bool alive = !q.test_stall;
+      CeWalker<MODE> w(pair, pairs);
+      CeTile c;
+      while (alive && w.next(q, c)) {
+        const int arow = c.mt * kCeBM + static_cast<int>(rank) * 128;
+        const int bcol = c.nt * q.bn + static_cast<int>(rank) * half;
+        for (int kk = 0; kk < nk; ++kk) {
+          if (fills >= q.stages && !mbar_wait(smem_u32(&ctrl->empty[st]), ph ^ 1u)) {
+            alive = false;
+            break;
+          }
+          const uint32_t full = mapa_shared(smem_u32(&ctrl->full[st]), 0);
+          const uint32_t sa = base + st * q.stage_bytes, sb = sa + kCeHalfA;
+          const int kx = kk * kLnBK;
+          if (leader) mbar_arrive_expect_tx(smem_u32(&ctrl->full[st]), 2 * q.stage_bytes);
+          if (!kAMn) {
+            tma_load_3d_pair(sa, &map_a, full, kx, arow, 0, keep);
+          } else {
+            tma_load_3d_pair(sa, &map_a, full, arow, kx, 0, keep);
+            tma_load_3d_pair(sa + kLnMnBox, &map_a, full, arow + 64, kx, 0, keep);
+          }
+          if (!kBMn) {
+            tma_load_3d_pair(sb, &map_b, full, kx, bcol, 0, keep);
+          } else {
+            const CUtensorMap* mb = MODE == kCeDw && q.dirty && q.dirty[kk] ? &map_b2 : &map_b;
+            for (int j = 0; j < half / 64; ++j)
+              tma_load_3d_pair(sb + j * kLnMnBox, mb, full, bcol + j * 64, kx, 0, keep);
+          }
+          ++fills;
+          if (++st == q.stages) {
+            st = 0;
+            ph ^= 1u;
+          }
+        }
+      }
+      // Until the leader's commits have released every stage that this CTA filled:
+      // no signal of theirs may come after the CTA is gone.
+      for (int f = max(0, fills - q.stages); alive && f < fills; ++f)
+        alive = mbar_wait(smem_u32(&ctrl->empty[f % q.stages]), static_cast<uint32_t>(f / q.stages) & 1u);
+      if (!alive) ctrl->failed = 1;
+    }
+  } else if (warp == 1) {
+    // ============================================================ MMA issuer (even CTA)
+    if (lane == 0 && leader) {
+      const uint32_t idesc = idesc_f16(std::is_same<T, __nv_bfloat16>::value ? 1u : 0u, kCeBM,
+                                       static_cast<uint32_t>(q.bn), kAMn ? 1u : 0u, kBMn ? 1u : 0u);
+      const uint64_t da0 = kAMn ? smem_desc_sw128(base, kLnMnBox, 1024) : smem_desc_sw128(base, 16, 1024);
+      const uint64_t db0 =
+          kBMn ? smem_desc_sw128(base + kCeHalfA, kLnMnBox, 1024) : smem_desc_sw128(base + kCeHalfA, 16, 1024);
+      constexpr uint32_t ka = kAMn ? (2048u >> 4) : 2u, kb = kBMn ? (2048u >> 4) : 2u;
+      const int nk = (q.k + kLnBK - 1) / kLnBK;
+      int st = 0, it = 0;
+      uint32_t ph = 0;
+      bool alive = true;
+      CeWalker<MODE> w(pair, pairs);
+      CeTile c;
+      for (; alive && w.next(q, c); ++it) {
+        const int buf = it & 1;
+        if (it >= 2) {
+          if (!mbar_wait(smem_u32(&ctrl->acc_empty[buf]), ((it >> 1) - 1) & 1)) {
+            alive = false;
+            break;
+          }
+          tc_fence_after();
+        }
+        const uint32_t d_tmem = tmem + static_cast<uint32_t>(buf * 256);
+        for (int kk = 0; kk < nk; ++kk) {
+          if (!mbar_wait(smem_u32(&ctrl->full[st]), ph)) {
+            alive = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t adv = static_cast<uint32_t>(st * q.stage_bytes) >> 4;
+#pragma unroll
+          for (int k = 0; k < kLnBK / 16; ++k)
+            tc_mma_f16_pair(d_tmem, da0 + adv + ka * k, db0 + adv + kb * k, idesc, (kk != 0 || k != 0) ? 1u : 0u);
+          tc_commit_pair(smem_u32(&ctrl->empty[st]));
+          tc_commit_pair(mapa_shared(smem_u32(&ctrl->empty[st]), 1));
+          if (++st == q.stages) {
+            st = 0;
+            ph ^= 1u;
+          }
+        }
+        if (!alive) break;
+        tc_commit_pair(smem_u32(&ctrl->acc_full[buf]));
+        tc_commit_pair(mapa_shared(smem_u32(&ctrl->acc_full[buf]), 1));
+      }
+      if (!alive) ctrl->failed = 1;
+    }
+  } else if (warp >= 4) {
+    // ============================================================ epilogue (both CTAs)
+    const int h = (warp - 4) >> 2;  // column part of the tile
+    const int wq = warp & 3;        // TMEM lane quarter
+    const int part = max(32, q.bn >> 2);
+    const uint32_t lane_off = static_cast<uint32_t>(wq * 32) << 16;
+    const uint32_t tile = staging + static_cast<uint32_t>((warp - 4) * kLnStageTile);
+    const uint32_t freed0 = mapa_shared(smem_u32(&ctrl->acc_empty[0]), 0);
+    const uint32_t freed1 = mapa_shared(smem_u32(&ctrl->acc_empty[1]), 0);
+    const uint64_t policy = l2_policy_evict_normal();
+    const float scale = MODE == kCeGrad ? ce_scale(q.largest, false) : MODE == kCeStats ? 1.f : ce_scale(q.largest, true);
+    CeWalker<MODE> w(pair, pairs);
+    CeTile c;
+    CeRow r{};
+    bool alive = true;  // a warp that gave up still meets the others at their barriers
+    for (int it = 0; w.next(q, c); ++it) {
+      const int buf = it & 1;
+      const int row0 = c.mt * kCeBM + static_cast<int>(rank) * 128 + wq * 32, row = row0 + lane;
+      const int col0 = c.nt * q.bn + h * part;
+      const int nch = row0 < q.m && h * part < q.bn ? max(0, min(part, q.n - col0) + 31) / 32 : 0;
+      if ((MODE == kCeStats || MODE == kCeGrad) && c.first) {
+        r.target = row < q.m ? ce_target(q.targets, q.target_stride, q.target64, q.ignore, q.vocab, row) : -1;
+        if (MODE == kCeGrad) {
+          const float2 ab = row < q.m ? __ldg(q.coef + row) : make_float2(0.f, 0.f);
+          r.a = ab.x * scale;
+          r.b = ab.y * scale;
+          r.lse = row < q.m ? __ldg(q.lse + row) : 0.f;
+        }
+        r.c = -INFINITY;
+        r.s = 0.f;
+      }
+      if (alive && !ln_warp_wait(smem_u32(&ctrl->acc_full[buf]), (it >> 1) & 1)) {
+        if (lane == 0) ctrl->failed = 1;
+        alive = false;
+      }
+      if (!alive && MODE != kCeStats) break;
+      tc_fence_after();
+      const uint32_t tb = tmem + lane_off + static_cast<uint32_t>(buf * 256 + h * part);
+#pragma unroll 1
+      for (int ch = 0; ch < nch && alive; ++ch) {
+        const int col = col0 + ch * 32;
+        if constexpr (MODE == kCeStats || MODE == kCeGrad) {
+          uint32_t o[32];
+          tmem_ld32(tb + ch * 32, o);
+          tmem_wait_ld(o);
+          const int at = r.target - q.col0 - col;  // the target's place among the 32
+          const bool hit = __any_sync(0xFFFFFFFFu, r.target >= 0 && at >= 0 && at < 32);
+          if constexpr (MODE == kCeStats) {
+            if (hit) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                if (j == at && r.target >= 0) q.picked[row] = __uint_as_float(o[j]);
+            }
+            if (col + 32 <= q.n) ce_stats32<false>(o, 32, r);
+            else ce_stats32<true>(o, q.n - col, r);
+          } else {
+            ln_tile_free(lane);
+            if (hit) ce_grad32<T, true>(o, r.target >= 0 ? at : -1, r, tile, lane);
+            else ce_grad32<T, false>(o, -1, r, tile, lane);
+            ln_tma_tile(tile, lane, &map_y, col, row0, 0, policy);
+          }
+        } else if constexpr (F32) {
+#pragma unroll
+          for (int hh = 0; hh < 2; ++hh) {
+            uint32_t o[16];
+            ln_tmem_ld16(tb + ch * 32 + 16 * hh, false, o);
+            ln_tile_free(lane);
+#pragma unroll
+            for (int p = 0; p < 4; ++p)
+              ln_sts(ln_piece(tile, lane, p), o[4 * p], o[4 * p + 1], o[4 * p + 2], o[4 * p + 3]);
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              if (q.add) tma_reduce_add_3d(&map_y, tile, col + 16 * hh, row0, 0);
+              else tma_store_3d(&map_y, tile, col + 16 * hh, row0, 0, policy);
+              bulk_commit_group();
+            }
+          }
+        } else {
+          ln_tile_free(lane);
+#pragma unroll
+          for (int hh = 0; hh < 2; ++hh) {
+            uint32_t o[16];
+            ln_tmem_ld16(tb + ch * 32 + 16 * hh, false, o);
+#pragma unroll
+            for (int p = 0; p < 2; ++p) {
+              uint32_t y[4];
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                y[j] = ln_pack<T>(__uint_as_float(o[8 * p + 2 * j]) * scale, __uint_as_float(o[8 * p + 2 * j + 1]) * scale);
+              ln_sts(ln_piece(tile, lane, 2 * hh + p), y[0], y[1], y[2], y[3]);
+            }
+          }
+          if (q.out_vec) {
+            ln_tma_tile(tile, lane, &map_y, col, row0, 0, policy);
+          } else {
+            const LnLines l{row0 + (lane >> 2), q.m, col + (lane & 3) * 8, q.n};
+            __syncwarp();
+            ln_store_tile_by_column(tile, lane, static_cast<uint16_t*>(q.out), q.out_ld, l);
+            __syncwarp();
+          }
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0 && alive) mbar_arrive_cluster(buf ? freed1 : freed0);
+      if (MODE == kCeStats && c.last) {
+        // The four parts of a row meet in shared memory.
+        const uint32_t meet = staging + static_cast<uint32_t>(wq * 32 + lane) * 8;
+        if (h > 0)
+          asm volatile("st.shared.v2.f32 [%0], {%1,%2};" ::"r"(meet + h * 1024), "f"(r.c), "f"(r.s) : "memory");
+        named_bar_sync(1 + wq, 128);
+        if (h == 0) {
+#pragma unroll
+          for (int i = 1; i < 4; ++i) {
+            float c2, s2;
+            asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(c2), "=f"(s2) : "r"(meet + i * 1024));
+            ce_join(r.c, r.s, c2, s2);
+          }
+          if (row < q.m) q.partial[static_cast<int64_t>(c.seg) * q.rows + row] = make_float2(r.c, r.s);
+        }
+        named_bar_sync(1 + wq, 128);  // read before the next unit's
+      }
+    }
+    if (lane == 0) bulk_wait_read_all();
+  }
+
+  // ---------------------------------------------------------------- teardown
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (ctrl->failed) {
+    // The even CTA's barriers count the loads of both CTAs.
+    if (tid == 0 && leader) ln_settle_loads(ctrl->full, q.stages, fills);
+    if (tid == 32 && leader) {
+      tc_commit_pair(smem_u32(&ctrl->settled));
+      ln_settle(smem_u32(&ctrl->settled), 0);
+    }
+    __syncthreads();
+  }
+  cluster_sync();  // no signal goes to either CTA, and no product reads it, after this
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem, 512);
+  }
+}
+
+// ---------------------------------------------------------------- steps around the products
+
+struct CeRows {
+  int rows, vocab, segments;
+  const void* targets;
+  int64_t target_stride;
+  int target64;
+  int64_t ignore;
+  const float2* partial;   // [segments][rows]
+  const float* picked;
+  float z_loss;
+  float* each;             // losses of the rows
+  float* lse;              // [rows], base 2
+  int per;                 // rows of a block, a power of two up to 32
+};
+
+// The rows' log sums from their segments' parts, and their losses. A block takes
+// `per` rows, 256 / per threads a row share its segments; parts are joined in a fixed
+// order.
+__global__ void __launch_bounds__(256) ce_rows(const CeRows q) {
+  __shared__ float2 part[256];
+  griddep_launch_dependents();
+  griddep_wait();
+  const int r = threadIdx.x & (q.per - 1), y = threadIdx.x / q.per, ny = 256 / q.per;
+  const int row = blockIdx.x * q.per + r;
+  float c = -INFINITY, s = 0.f;
+  if (row < q.rows) {
+    const float2* p = q.partial + row;
+    int i = y;
+    for (; i + 3 * ny < q.segments; i += 4 * ny) {
+      float2 v[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = __ldg(p + static_cast<int64_t>(i + j * ny) * q.rows);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) ce_join(c, s, v[j].x, v[j].y);
+    }
+    for (; i < q.segments; i += ny) {
+      const float2 v = __ldg(p + static_cast<int64_t>(i) * q.rows);
+      ce_join(c, s, v.x, v.y);
+    }
+  }
+  part[threadIdx.x] = make_float2(c, s);
+  __syncthreads();
+  for (int step = ny / 2; step > 0; step >>= 1) {
+    if (y < step) {
+      const float2 o = part[threadIdx.x + step * q.per];
+      float2 mine = part[threadIdx.x];
+      ce_join(mine.x, mine.y, o.x, o.y);
+      part[threadIdx.x] = mine;
+    }
+    __syncthreads();
+  }
+  if (y != 0 || row >= q.rows) return;
+  constexpr float kLn2 = 0.6931471805599453f;
+  const float2 v = part[threadIdx.x];
+  const float lse2 = v.x + log2f(v.y), lse = lse2 * kLn2;
+  const int t = ce_target(q.targets, q.target_stride, q.target64, q.ignore, q.vocab, row);
+  float loss = 0.f;
+  if (t >= 0) {
+    loss = lse - q.picked[row];
+    if (q.z_loss != 0.f) loss = fmaf(q.z_loss * lse, lse, loss);
+  } else if (t == -2) {
+    loss = __int_as_float(0x7fc00000);
+  }
+  q.each[row] = loss;
+  if (q.lse) q.lse[row] = lse2;
+}
+
+// The sum or mean of the rows' losses, in 64 bits and a fixed order; *count: the
+// rows that are not ignored.
+__global__ void __launch_bounds__(1024) ce_total(const CeRows q, int mean, float* loss, float* count) {
+  __shared__ double sums[32];
+  __shared__ int counts[32];
+  griddep_launch_dependents();
+  griddep_wait();
+  double s = 0.0;
+  int n = 0;
+  for (int i = threadIdx.x; i < q.rows; i += 1024) {
+    s += static_cast<double>(q.each[i]);
+    n += ce_target(q.targets, q.target_stride, q.target64, q.ignore, q.vocab, i) != -1;
+  }
+#pragma unroll
+  for (int d = 16; d; d >>= 1) {
+    s += __shfl_xor_sync(0xFFFFFFFFu, s, d);
+    n += __shfl_xor_sync(0xFFFFFFFFu, n, d);
+  }
+  if ((threadIdx.x & 31) == 0) {
+    sums[threadIdx.x >> 5] = s;
+    counts[threadIdx.x >> 5] = n;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    s = 0.0;
+    n = 0;
+    for (int i = 0; i < 32; ++i) {
+      s += sums[i];
+      n += counts[i];
+    }
+    *loss = static_cast<float>(mean ? s / n : s);  // the mean of no row is 0 / 0
+    if (count) *count = __int_as_float(n);
+  }
+}
+
+struct CeCoef {
+  int rows, vocab, width;
+  const void* targets;
+  int64_t target_stride;
+  int target64;
+  int64_t ignore;
+  const float* lse;
+  const float* count;      // mean: the bits of the number of rows, else null
+  const float* dy;
+  int64_t dy_stride;       // 0: one value
+  float z_loss;
+  float2* coef;
+  uint32_t* largest;       // f16: zero before, or null
+  const uint16_t* x;
+  int64_t x_ld;
+  uint16_t* copy;          // rows of ignored targets that are not finite, as zeros
+  int64_t copy_ld;
+  uint8_t* dirty;          // [ceil(rows / 64)], or null: dW is not wanted
+};
+
+constexpr int kCeCoefRows = kLnBK;
+
+// a and b of 64 rows. dW multiplies every row of x by its dz, which is zero for
+// an ignored row, but padding may hold infinities and NaN: a block of 64 rows
+// with such a row is copied with those rows as zeros, and dW reads the copy there.
+template <typename T>
+__global__ void __launch_bounds__(256) ce_coef(const CeCoef q) {
+  __shared__ uint8_t skip[kCeCoefRows];
+  griddep_launch_dependents();
+  griddep_wait();
+  constexpr float kLn2 = 0.6931471805599453f;
+  const int row0 = blockIdx.x * kCeCoefRows, tid = threadIdx.x, row = row0 + tid;
+  const int here = min(kCeCoefRows, q.rows - row0);
+  if (tid < kCeCoefRows) {
+    float a = 0.f, b = 0.f;
+    bool out = true;
+    if (tid < here) {
+      const int t = ce_target(q.targets, q.target_stride, q.target64, q.ignore, q.vocab, row);
+      out = t == -1;
+      if (!out) {
+        float g = __ldg(q.dy + row * q.dy_stride);
+        if (q.count) g /= static_cast<float>(__float_as_int(*q.count));
+        if (t == -2) g = __int_as_float(0x7fc00000);
+        b = g;
+        a = q.z_loss != 0.f ? g * fmaf(2.f * q.z_loss, __ldg(q.lse + row) * kLn2, 1.f) : g;
+      }
+      q.coef[row] = make_float2(a, b);
+    }
+    skip[tid] = out;
+    if (q.largest) {
+      // The largest finite one; the order of the maxima does not matter.
+      float top = fmaxf(fabsf(a), fabsf(b));
+      if (!(top < INFINITY)) top = 0.f;
+      const uint32_t all = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(top));
+      if ((tid & 31) == 0 && all) atomicMax(q.largest, all);
+    }
+  }
+  if (!q.dirty) return;
+  __syncthreads();
+  constexpr uint16_t kTop = std::is_same<T, __half>::value ? 0x7C00 : 0x7F80;
+  bool bad = false;
+  for (int i = 0; i < here; ++i) {
+    if (!skip[i]) continue;
+    const uint16_t* p = q.x + static_cast<int64_t>(row0 + i) * q.x_ld;
+    for (int j = tid; j < q.width; j += 256) bad |= (p[j] & kTop) == kTop;
+  }
+  bad = __syncthreads_or(bad);
+  if (tid == 0) q.dirty[blockIdx.x] = bad;
+  if (!bad) return;
+  for (int i = 0; i < here; ++i) {
+    const uint16_t* p = q.x + static_cast<int64_t>(row0 + i) * q.x_ld;
+    uint16_t* o = q.copy + static_cast<int64_t>(row0 + i) * q.copy_ld;
+    for (int j = tid; j < q.width; j += 256) o[j] = skip[i] ? static_cast<uint16_t>(0) : p[j];
+  }
+}
+
+// dx from its fp32 sums over all pieces.
+template <typename T>
+__global__ void __launch_bounds__(256) ce_finish(const float* sums, int64_t ld, int rows, int width,
+                                                 const uint32_t* largest, T* dx, int64_t dx_ld) {
+  griddep_wait();
+  const float scale = ce_scale(largest, true);
+  const int64_t per = ld / 4, total = rows * per;
+  const bool vec = width % 4 == 0 && dx_ld % 4 == 0 && (reinterpret_cast<uintptr_t>(dx) & 7u) == 0;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < total;
+       i += static_cast<int64_t>(gridDim.x) * 256) {
+    const int64_t row = i / per;
+    const int col = static_cast<int>(i - row * per) * 4;
+    const float4 v = __ldcs(reinterpret_cast<const float4*>(sums + row * ld + col));
+    T* o = dx + row * dx_ld + col;
+    if (vec) {
+      *reinterpret_cast<uint2*>(o) = make_uint2(ln_pack<T>(v.x * scale, v.y * scale), ln_pack<T>(v.z * scale, v.w * scale));
+    } else {
+      const float f[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (col + j < width) o[j] = Elem<T>::from_f(f[j] * scale);
+    }
+  }
+}
+
+}  // namespace avey

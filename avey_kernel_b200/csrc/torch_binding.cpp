@@ -30,6 +30,9 @@ struct Library {
   int (*linear_fwd)(const AveyLinearParams*, void*) = nullptr;
   int (*linear_bwd)(const AveyLinearParams*, void*) = nullptr;
   int (*linear_workspace)(const AveyLinearParams*, int, uint64_t*) = nullptr;
+  int (*loss_fwd)(const AveyLossParams*, void*) = nullptr;
+  int (*loss_bwd)(const AveyLossParams*, void*) = nullptr;
+  int (*loss_workspace)(const AveyLossParams*, int, uint64_t*) = nullptr;
   const char* (*last_error)() = nullptr;
 };
 Library lib;
@@ -409,6 +412,128 @@ Tensor linear(const Tensor& x, const Tensor& weight, const std::optional<Tensor>
   return linear_forward(x, weight, bias, residual, offsets, act, kernel, false).first;
 }
 
+// ------------------------------------------------------------ cross entropy
+
+// The parameter block but for the operands, and for `targets` [rows].
+AveyLossParams loss_params(const Tensor& like, int64_t rows, int64_t width, int64_t vocab, const Tensor& targets,
+                           int64_t ignore, int64_t reduction, double z_loss) {
+  AveyLossParams p{};
+  p.struct_size = sizeof(p);
+  p.dtype = dtype_id(like);
+  p.target_bits = targets.scalar_type() == at::kLong ? 64 : 32;
+  p.reduction = static_cast<int32_t>(reduction);
+  p.rows = rows;
+  p.width = width;
+  p.vocab = vocab;
+  p.targets = targets.const_data_ptr();
+  p.target_stride = rows > 1 ? targets.stride(0) : 1;
+  p.ignore_index = ignore;
+  p.z_loss = z_loss;
+  return p;
+}
+
+Tensor loss_workspace(AveyLossParams& p, int backward, const Tensor& like) {
+  uint64_t bytes = 0;
+  check_status(lib.loss_workspace(&p, backward, &bytes));
+  if (bytes == 0) return {};
+  Tensor ws = at::empty({static_cast<int64_t>(bytes)}, like.options().dtype(at::kByte));
+  p.workspace = ws.data_ptr();
+  p.workspace_bytes = bytes;
+  return ws;
+}
+
+// The operands of a call, as the library takes them: rows with unit stride.
+struct LossRows {
+  Tensor x, w, t;
+  LossRows(AveyLossParams& p, const Tensor& x_, const Tensor& w_) : x(as_rows(x_, p.width)), w(as_weight(w_)) {
+    p.x = x.const_data_ptr();
+    p.x_ld = row_ld(x, p.width);
+    p.weight = w.const_data_ptr();
+    p.weight_ld = p.vocab > 1 ? w.stride(0) : (p.width + 7) / 8 * 8;
+  }
+};
+
+// The loss and, with keep, what the backward pass needs of it.
+std::pair<Tensor, Tensor> loss_forward(const Tensor& x, const Tensor& weight, const Tensor& targets, int64_t ignore,
+                                       int64_t reduction, double z_loss, bool keep) {
+  const c10::cuda::CUDAGuard guard(x.device());
+  const Tensor t = targets.reshape({-1});
+  AveyLossParams p = loss_params(x, t.size(0), weight.size(1), weight.size(0), t, ignore, reduction, z_loss);
+  const LossRows rows(p, x, weight);
+  const auto f32 = x.options().dtype(at::kFloat);
+  Tensor loss = reduction == AVEY_LOSS_NONE ? at::empty(targets.sizes(), f32) : at::empty({}, f32), saved;
+  p.loss = loss.data_ptr<float>();
+  if (keep) {
+    saved = at::empty({p.rows + 1}, f32);
+    p.saved = saved.data_ptr<float>();
+  }
+  const Tensor ws = loss_workspace(p, 0, x);
+  check_status(lib.loss_fwd(&p, at::cuda::getCurrentCUDAStream().stream()));
+  return {loss, saved};
+}
+
+class LossFunction : public torch::autograd::Function<LossFunction> {
+ public:
+  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const Tensor& weight,
+                        const Tensor& targets, int64_t ignore, int64_t reduction, double z_loss) {
+    auto [loss, saved] = loss_forward(x, weight, targets, ignore, reduction, z_loss, true);
+    ctx->save_for_backward({x, weight, targets, saved});
+    ctx->saved_data["call"] = std::vector<int64_t>{ignore, reduction};
+    ctx->saved_data["z_loss"] = z_loss;
+    return loss;
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    TORCH_CHECK(!at::GradMode::is_enabled(),
+                "the gradients of the native cross entropy cannot be differentiated again (create_graph)");
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &x = saved[0], &weight = saved[1];
+    const std::vector<int64_t> call = ctx->saved_data["call"].toIntVector();
+    torch::autograd::variable_list out(6);
+    if (!grads[0].defined()) return out;
+    refuse_unseen([&](auto f) { f(grads[0]); });
+    const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1);
+    if (!need_x && !need_w) return out;
+    const c10::cuda::CUDAGuard guard(x.device());
+    const Tensor t = saved[2].reshape({-1}), g = grads[0].reshape({-1});
+    AveyLossParams p = loss_params(x, t.size(0), weight.size(1), weight.size(0), t, call[0], call[1],
+                                   ctx->saved_data["z_loss"].toDouble());
+    const LossRows rows(p, x, weight);
+    p.saved = saved[3].data_ptr<float>();
+    p.dloss = g.const_data_ptr<float>();
+    p.dloss_stride = g.size(0) > 1 ? g.stride(0) : 1;
+    if (need_x) {
+      out[0] = at::empty(x.sizes(), x.options());
+      p.dx = out[0].data_ptr();
+      p.dx_ld = p.width;
+    }
+    if (need_w) {
+      out[1] = at::empty(weight.sizes(), weight.options());
+      p.dweight = out[1].data_ptr();
+    }
+    const Tensor ws = loss_workspace(p, 1, x);
+    check_status(lib.loss_bwd(&p, at::cuda::getCurrentCUDAStream().stream()));
+    return out;
+  }
+};
+
+Tensor cross_entropy(const Tensor& x, const Tensor& weight, const Tensor& targets, int64_t ignore, int64_t reduction,
+                     double z_loss) {
+  refuse_unseen([&](auto f) {
+    f(x);
+    f(weight);
+  });
+  const auto dt = x.scalar_type();
+  TORCH_CHECK_VALUE(x.is_cuda() && (dt == at::kBFloat16 || dt == at::kHalf) && weight.scalar_type() == dt &&
+                        weight.device() == x.device(),
+                    "the native cross entropy takes bf16 / f16 CUDA tensors of one dtype");
+  TORCH_CHECK_VALUE(targets.device() == x.device(), "targets must be on x's device");
+  if (at::GradMode::is_enabled() && (x.requires_grad() || weight.requires_grad()))
+    return LossFunction::apply(x, weight, targets, ignore, reduction, z_loss);
+  return loss_forward(x, weight, targets, ignore, reduction, z_loss, false).first;
+}
+
 // Entry points of the loaded library, by name.
 void bind(const py::dict& addresses) {
   auto at = [&](const char* name) { return addresses[name].cast<uintptr_t>(); };
@@ -416,6 +541,9 @@ void bind(const py::dict& addresses) {
   lib.linear_fwd = reinterpret_cast<decltype(lib.linear_fwd)>(at("avey_linear_fwd_v1"));
   lib.linear_bwd = reinterpret_cast<decltype(lib.linear_bwd)>(at("avey_linear_bwd_v1"));
   lib.linear_workspace = reinterpret_cast<decltype(lib.linear_workspace)>(at("avey_linear_workspace_size"));
+  lib.loss_fwd = reinterpret_cast<decltype(lib.loss_fwd)>(at("avey_loss_fwd_v1"));
+  lib.loss_bwd = reinterpret_cast<decltype(lib.loss_bwd)>(at("avey_loss_bwd_v1"));
+  lib.loss_workspace = reinterpret_cast<decltype(lib.loss_workspace)>(at("avey_loss_workspace_size"));
   lib.last_error = reinterpret_cast<decltype(lib.last_error)>(at("avey_last_error"));
 }
 
@@ -425,4 +553,5 @@ PYBIND11_MODULE(_torch_binding, m) {
   m.def("bind", &bind);
   m.def("adamw_step", &adamw_step);
   m.def("linear", &linear);
+  m.def("cross_entropy", &cross_entropy);
 }

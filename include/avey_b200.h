@@ -467,6 +467,75 @@ AVEY_API int avey_linear_bwd_v1(const AveyLinearParams* params, void* stream);
 AVEY_API int avey_linear_workspace_size(const AveyLinearParams* params, int backward, uint64_t* bytes);
 
 /*
+ * Softmax cross entropy of z = x W^T over a vocabulary, without keeping z, and
+ * its gradients (no counterpart in the reference, which leaves the loss to
+ * torch). For row i with the target t_i:
+ *
+ *   lse_i  = log sum_j exp(z_ij)
+ *   loss_i = lse_i - z_{i,t_i} + z_loss lse_i^2, or 0 where t_i = ignore_index
+ *   loss   = loss_i (NONE), their sum (SUM), or the sum over the number of rows
+ *            that are not ignored (MEAN; of none: NaN)
+ *
+ * on x [rows][width] and W [vocab][width]. A target outside [0, vocab) that is not
+ * ignore_index makes its row's loss, and what depends on it, NaN. Ignored rows
+ * have no part in anything, whatever x holds there, and their dx is zero.
+ *
+ * The forward call writes `saved` (rows + 1 floats: lse_i / log 2, and the bits of
+ * the number of rows that count) for the backward call, which computes z again in
+ * pieces of the vocabulary, from dloss (rows values dloss_stride apart for NONE, else
+ * one):
+ *
+ *   dz_ij = g_i ((1 + 2 z_loss lse_i) exp(z_ij - lse_i) - [j = t_i])
+ *   dx = dz W, dweight = dz^T x
+ *
+ * Products and sums are fp32; dz is rounded to dtype before its products (scaled by
+ * a power of two in f16, so that small probabilities are not lost) and each result
+ * once. Sums are taken in fixed orders: results are bitwise reproducible.
+ *
+ * Last dimensions have stride 1; x_ld, weight_ld, dx_ld and target_stride are in
+ * elements (target_stride >= 0). Any alignment is taken: rows that are not whole
+ * 16-byte units are copied into the workspace first.
+ */
+#define AVEY_LOSS_NONE 0
+#define AVEY_LOSS_SUM 1
+#define AVEY_LOSS_MEAN 2
+
+typedef struct AveyLossParams {
+  uint32_t struct_size; /* sizeof(AveyLossParams) */
+  int32_t dtype;        /* AVEY_BF16 or AVEY_F16: x, weight, dx, dweight */
+  int32_t target_bits;  /* 32 or 64: signed targets */
+  int32_t reduction;    /* AVEY_LOSS_* */
+  int64_t rows, width, vocab; /* up to 2^30, 2^22 and 2^30 */
+  const void* x;
+  int64_t x_ld;
+  const void* weight;
+  int64_t weight_ld;
+  const void* targets;
+  int64_t target_stride;
+  int64_t ignore_index;
+  double z_loss;
+  float* loss;  /* forward: [rows] (NONE) or one value */
+  float* saved; /* [rows + 1]; forward: or NULL */
+
+  /* Backward. NULL: not wanted. */
+  const float* dloss;
+  int64_t dloss_stride;
+  void* dx;
+  int64_t dx_ld;
+  void* dweight; /* contiguous [vocab][width] */
+
+  void* workspace; /* 256-byte aligned, >= avey_loss_workspace_size() bytes */
+  uint64_t workspace_bytes;
+} AveyLossParams;
+
+AVEY_API int avey_loss_fwd_v1(const AveyLossParams* params, void* stream);
+AVEY_API int avey_loss_bwd_v1(const AveyLossParams* params, void* stream);
+
+/* Bytes of `workspace` of the forward (backward == 0) or backward call: about 512
+ * MB at most beside a share of the operands' size, whatever rows x vocab is. */
+AVEY_API int avey_loss_workspace_size(const AveyLossParams* params, int backward, uint64_t* bytes);
+
+/*
  * One AdamW step over many tensors (no counterpart in the reference, which
  * leaves training to torch). For every element of every tensor, in fp32:
  *
