@@ -82,11 +82,13 @@ int logit_cols(int64_t rows, int64_t n) {
     if (mt * ((n + bn - 1) / bn) >= 4 * pairs()) return bn;
   return 64;
 }
-// Of a gradient's product over `width` columns (boxes of 64 for each CTA).
-int grad_cols(int64_t m, int64_t width) {
-  const int64_t mt = (m + avey::kCeBM - 1) / avey::kCeBM;
-  return width > 128 && mt * ((width + 255) / 256) * 4 >= pairs() * 3 ? 256 : 128;
+// Column tiles of a unit of logits: more than one where there are enough for the
+// pairs to end together.
+int unit_tiles(int64_t mt, int64_t nt) {
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(avey::kCeMaxSeg, mt * nt / (16 * pairs()))));
 }
+// Of a gradient's product over `width` columns (boxes of 64 for each CTA).
+int grad_cols(int64_t width) { return width > 128 ? 256 : 128; }
 
 // Workspace of a call, each part 256-byte aligned.
 struct Layout {
@@ -98,22 +100,34 @@ struct Layout {
   uint64_t partial = 0, picked = 0, each = 0;
   // backward
   int64_t piece = 0, pieces = 0;  // columns of dz at a time
-  uint64_t coef = 0, largest = 0, dirty = 0, copy = 0, dz = 0, sums = 0;
+  uint64_t coef = 0, counters = 0, dirty = 0, copy = 0, dz = 0, dz_bytes = 0, sums = 0, parts = 0;
   uint64_t total = 0;
 };
 
-// Bytes of dz kept at a time: 512 MB, or columns of four times the width where
-// that is more, so that dx's sums, read and written for every piece, stay small
-// beside its products.
+// Columns of dz kept at a time, twice where there is more than one piece: 256 MB, or
+// four times the width where that is more, so that dx's sums, read and written for
+// every piece, stay small beside its products.
 int64_t piece_columns(const AveyLossParams* p) {
-  const int64_t most = std::max<int64_t>((512ll << 20) / (2 * p->rows), 4 * p->width);
-  const int64_t tiles = (p->vocab + 255) / 256;
-  int64_t per = std::max<int64_t>(1, most / 256);
-  // dW's tiles in whole waves of pairs, where there is a wave.
-  const int64_t n_nt = (p->width + 255) / 256, waves = per * n_nt / pairs();
-  if (waves > 0) per = std::max<int64_t>(1, waves * pairs() / n_nt);
-  if (per >= tiles) return up(p->vocab, 8);
-  return per * 256;
+  const int64_t most = std::max<int64_t>((256ll << 20) / (2 * p->rows), 4 * p->width);
+  const int64_t tiles = (p->vocab + 255) / 256, per = std::max<int64_t>(1, most / 256);
+  if (2 * per >= tiles) return up(p->vocab, 8);
+  const int64_t pieces = (tiles + per - 1) / per;
+  return (tiles + pieces - 1) / pieces * 256;
+}
+
+int64_t tiles_of(int64_t m, int64_t n, int bn) { return (m + avey::kCeBM - 1) / avey::kCeBM * ((n + bn - 1) / bn); }
+
+// K ranges of a tile of dX: more than one where a tile would last longer than a
+// pair's share of the launch (with dW over `n` columns), of eight K blocks at least.
+int dx_splits(const AveyLossParams* p, int64_t n) {
+  const int bn = grad_cols(p->width);
+  const int64_t nk = (n + 63) / 64, tiles = tiles_of(p->rows, p->width, bn);
+  const int64_t dw = p->dweight ? tiles_of(n, p->width, bn) * ((p->rows + 63) / 64) : 0;
+  const int64_t share = (tiles * nk + dw + pairs() - 1) / pairs();
+  int64_t s = (nk + share - 1) / share;
+  // Without dW's tiles to fill it, the last wave of dX's is cut finer too.
+  if (!p->dweight && tiles % pairs() != 0 && tiles < 4 * pairs()) s = std::max<int64_t>(s, 4);
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(s, nk / 8)));
 }
 
 Layout layout(const AveyLossParams* p, bool backward) {
@@ -134,8 +148,7 @@ Layout layout(const AveyLossParams* p, bool backward) {
     l.bn = logit_cols(p->rows, p->vocab);
     l.n_nt = (p->vocab + l.bn - 1) / l.bn;
     const int64_t mt = (p->rows + avey::kCeBM - 1) / avey::kCeBM;
-    // Units of more than one tile where there are enough for the pairs to end together.
-    l.seg = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(avey::kCeMaxSeg, mt * l.n_nt / (16 * pairs()))));
+    l.seg = unit_tiles(mt, l.n_nt);
     l.segments = (l.n_nt + l.seg - 1) / l.seg;
     l.partial = take(l.segments * p->rows * 8);
     l.picked = take(p->rows * 4);
@@ -144,13 +157,21 @@ Layout layout(const AveyLossParams* p, bool backward) {
     l.piece = piece_columns(p);
     l.pieces = (p->vocab + l.piece - 1) / l.piece;
     l.coef = take(p->rows * 8);
-    l.largest = take(4);
+    l.counters = take(4 * (l.pieces + 2));
     if (p->dweight) {
       l.dirty = take((p->rows + 63) / 64);
       l.copy = take(p->rows * row);
     }
-    l.dz = take(p->rows * l.piece * 2);
-    if (p->dx && l.pieces > 1) l.sums = take(p->rows * up(p->width, 4) * 4);
+    l.dz_bytes = static_cast<uint64_t>(p->rows) * l.piece * 2;
+    l.dz = take(l.dz_bytes * (l.pieces > 1 ? 2 : 1));
+    if (p->dx) {
+      if (l.pieces > 1) l.sums = take(p->rows * up(p->width, 4) * 4);
+      const int bn = grad_cols(p->width);
+      int splits = 1;
+      for (int64_t n : {std::min(l.piece, p->vocab), p->vocab - (l.pieces - 1) * l.piece})
+        splits = std::max(splits, dx_splits(p, n));
+      if (splits > 1) l.parts = take(splits * tiles_of(p->rows, p->width, bn) * avey::kCeBM * bn * 4);
+    }
   }
   l.total = at;
   return l;
@@ -239,30 +260,18 @@ int pack_inputs(const AveyLossParams* p, const Layout& l, Rows* x, Rows* w, Chai
   return chain.launch("row copy", avey::ln_pack_rows, grid, 256, 0, 1, a, b);
 }
 
-struct Maps {
-  CUtensorMap a{}, b{}, b2{}, y{};
-};
-
 template <auto K>
-int launch_product(const Maps& m, const avey::CeGeom& q, Chain& chain) {
+int launch_product(const avey::CeMaps& m, avey::CeGeom& q, Chain& chain) {
   const cudaError_t attr = smem_opt_in<K>();
   if (attr != cudaSuccess) return fail(AVEY_ERR_CUDA, cudaGetErrorString(attr));
-  return chain.launch("cross entropy product", K, 2ll * std::min<int64_t>(q.units, pairs()), avey::kCeThreads,
-                      avey::kCeSmem, 2, m.a, m.b, m.b2, m.y, q);
+  q.units = 0;
+  for (const avey::CeJob& j : q.job) q.units += j.units;
+  return chain.launch("cross entropy product", K, 2ll * std::min(q.units, pairs()), avey::kCeThreads,
+                      avey::kCeSmem, 2, m, q);
 }
 
-avey::CeGeom geom(const AveyLossParams* p, int64_t m, int64_t n, int64_t k, int bn) {
+avey::CeGeom geom(const AveyLossParams* p) {
   avey::CeGeom q{};
-  q.m = static_cast<int>(m);
-  q.n = static_cast<int>(n);
-  q.k = static_cast<int>(k);
-  q.bn = bn;
-  q.n_mt = static_cast<int>((m + avey::kCeBM - 1) / avey::kCeBM);
-  q.n_nt = static_cast<int>((n + bn - 1) / bn);
-  q.seg = 1;
-  q.units = q.n_mt * q.n_nt;
-  q.stage_bytes = avey::kCeHalfA + bn * avey::kLnBK;
-  q.stages = std::min(avey::kCeMaxStages, avey::kCeRing / q.stage_bytes);
   q.rows = static_cast<int>(p->rows);
   q.vocab = static_cast<int>(p->vocab);
   q.targets = p->targets;
@@ -271,6 +280,28 @@ avey::CeGeom geom(const AveyLossParams* p, int64_t m, int64_t n, int64_t k, int 
   q.ignore = p->ignore_index;
   q.test_stall = avey_host::test_stall();
   return q;
+}
+
+avey::CeJob job(int kind, int64_t m, int64_t n, int64_t k, int bn) {
+  avey::CeJob j{};
+  j.kind = kind;
+  j.m = static_cast<int>(m);
+  j.n = static_cast<int>(n);
+  j.nk = static_cast<int>((k + avey::kLnBK - 1) / avey::kLnBK);
+  j.bn = bn;
+  j.n_mt = static_cast<int>((m + avey::kCeBM - 1) / avey::kCeBM);
+  j.n_nt = static_cast<int>((n + bn - 1) / bn);
+  j.seg = 1;
+  j.units = j.n_mt * j.n_nt;
+  return j;
+}
+
+// The ring of a launch: stages for its widest tiles.
+void set_ring(avey::CeGeom& q) {
+  int bn = 0;
+  for (const avey::CeJob& j : q.job) bn = std::max(bn, j.units ? j.bn : 0);
+  q.stage_bytes = avey::kCeHalfA + bn * avey::kLnBK;
+  q.stages = std::min(avey::kCeMaxStages, avey::kCeRing / q.stage_bytes);
 }
 
 avey::CeRows rows_of(const AveyLossParams* p) {
@@ -295,16 +326,18 @@ int forward(const AveyLossParams* p, cudaStream_t stream) {
   Rows x, w;
   rc = pack_inputs(p, l, &x, &w, chain);
   if (rc != AVEY_OK) return rc;
-  avey::CeGeom q = geom(p, p->rows, p->vocab, p->width, l.bn);
-  q.seg = l.seg;
-  q.units = static_cast<int>(l.segments) * q.n_mt;
+  avey::CeGeom q = geom(p);
+  q.job[0] = job(avey::kCeStats, p->rows, p->vocab, p->width, l.bn);
+  q.job[0].seg = l.seg;
+  q.job[0].units = static_cast<int>(l.segments) * q.job[0].n_mt;
+  set_ring(q);
   q.partial = reinterpret_cast<float2*>(ws + l.partial);
   q.picked = reinterpret_cast<float*>(ws + l.picked);
-  Maps m;
-  rc = avey_host::encode_rows16(p->dtype, x.p, p->width, p->rows, 1, x.ld * 2, 0, 128, &m.a);
-  if (rc == AVEY_OK) rc = avey_host::encode_rows16(p->dtype, w.p, p->width, p->vocab, 1, w.ld * 2, 0, l.bn / 2, &m.b);
+  avey::CeMaps m{};
+  rc = avey_host::encode_rows16(p->dtype, x.p, p->width, p->rows, 1, x.ld * 2, 0, 128, &m.x);
+  if (rc == AVEY_OK) rc = avey_host::encode_rows16(p->dtype, w.p, p->width, p->vocab, 1, w.ld * 2, 0, l.bn / 2, &m.w);
   if (rc != AVEY_OK) return rc;
-  rc = launch_product<avey::ce_product<T, avey::kCeStats, false>>(m, q, chain);
+  rc = launch_product<avey::ce_product<T, true>>(m, q, chain);
   if (rc != AVEY_OK) return rc;
   avey::CeRows r = rows_of(p);
   r.segments = static_cast<int>(l.segments);
@@ -328,12 +361,10 @@ int backward(const AveyLossParams* p, cudaStream_t stream) {
   if (rc != AVEY_OK) return rc;
   char* ws = static_cast<char*>(p->workspace);
   Chain chain{stream};
-  uint32_t* largest = nullptr;
-  if (p->dtype == AVEY_F16) {
-    largest = reinterpret_cast<uint32_t*>(ws + l.largest);
-    const cudaError_t e = cudaMemsetAsync(largest, 0, 4, stream);
-    if (e != cudaSuccess) return fail(AVEY_ERR_CUDA, cudaGetErrorString(e));
-  }
+  uint32_t* counters = reinterpret_cast<uint32_t*>(ws + l.counters);
+  const cudaError_t zeroed = cudaMemsetAsync(counters, 0, 4 * (l.pieces + 2), stream);
+  if (zeroed != cudaSuccess) return fail(AVEY_ERR_CUDA, cudaGetErrorString(zeroed));
+  uint32_t* largest = p->dtype == AVEY_F16 ? counters + l.pieces + 1 : nullptr;
   Rows x, w;
   rc = pack_inputs(p, l, &x, &w, chain);
   if (rc != AVEY_OK) return rc;
@@ -361,64 +392,97 @@ int backward(const AveyLossParams* p, cudaStream_t stream) {
   }
   rc = chain.launch("cross entropy coefficients", avey::ce_coef<T>, (p->rows + 63) / 64, 256, 0, 1, k);
   if (rc != AVEY_OK) return rc;
-  char* dz = ws + l.dz;
   const int64_t sums_ld = up(p->width, 4);
   float* sums = reinterpret_cast<float*>(ws + l.sums);
+  float* parts = reinterpret_cast<float*>(ws + l.parts);
   const bool planes = l.pieces > 1;
-  for (int64_t v0 = 0; v0 < p->vocab; v0 += l.piece) {
-    const int64_t n = std::min(l.piece, p->vocab - v0), ld = up(n, 8);
-    const char* wp = static_cast<const char*>(w.p) + v0 * w.ld * 2;
-    {
-      const int bn = logit_cols(p->rows, n);
-      avey::CeGeom q = geom(p, p->rows, n, p->width, bn);
-      q.seg = static_cast<int>(std::max<int64_t>(
-          1, std::min<int64_t>(avey::kCeMaxSeg, static_cast<int64_t>(q.n_mt) * q.n_nt / (16 * pairs()))));
-      q.units = (q.n_nt + q.seg - 1) / q.seg * q.n_mt;
+  const int bn = grad_cols(p->width);
+  // Launch i makes dz of piece i and the gradients' products of piece i - 1.
+  for (int64_t i = 0; i <= l.pieces; ++i) {
+    avey::CeGeom q = geom(p);
+    avey::CeMaps m{};
+    if (i > 0) q.claimed = counters + i;  // dz alone: units of one kind
+    q.largest = largest;
+    q.lse = p->saved;
+    q.coef = k.coef;
+    int jobs = 0, splits = 1;
+    if (i > 0) {
+      const int64_t v0 = (i - 1) * l.piece, n = std::min(l.piece, p->vocab - v0), ld = up(n, 8);
+      const char* dz = ws + l.dz + (i - 1) % 2 * l.dz_bytes;
+      const char* wp = static_cast<const char*>(w.p) + v0 * w.ld * 2;
+      if (p->dx) {
+        splits = dx_splits(p, n);
+        avey::CeJob j = job(avey::kCeDx, p->rows, p->width, n, bn);
+        j.seg = splits;
+        j.units *= splits;
+        q.job[jobs++] = j;
+        q.dx = planes ? nullptr : p->dx;
+        q.dx_ld = p->dx_ld;
+        q.dx_vec = whole_rows(p->dx, p->dx_ld);
+        q.dx_add = i > 1;
+        rc = avey_host::encode_rows16(p->dtype, dz, n, p->rows, 1, ld * 2, 0, 128, &m.dz_x);
+        if (rc == AVEY_OK) rc = avey_host::encode_rows16(p->dtype, wp, p->width, n, 1, w.ld * 2, 0, 64, &m.w_x);
+        if (rc == AVEY_OK && splits > 1)
+          rc = avey_host::encode_tiles(AVEY_F32, parts, bn, static_cast<uint64_t>(j.units) * avey::kCeBM, 1, bn * 4, 0,
+                                       &m.parts);
+        else if (rc == AVEY_OK && planes)
+          rc = avey_host::encode_tiles(AVEY_F32, sums, p->width, p->rows, 1, sums_ld * 4, 0, &m.y_dx);
+        else if (rc == AVEY_OK && q.dx_vec)
+          rc = avey_host::encode_tiles(p->dtype, p->dx, p->width, p->rows, 1, p->dx_ld * 2, 0, &m.y_dx);
+        if (rc != AVEY_OK) return rc;
+      }
+      if (p->dweight) {
+        q.job[jobs++] = job(avey::kCeDw, n, p->width, p->rows, bn);
+        char* dw = static_cast<char*>(p->dweight) + v0 * p->width * 2;
+        q.dw = dw;
+        q.dw_ld = p->width;
+        q.dw_vec = whole_rows(dw, p->width);
+        q.dirty = k.dirty;
+        rc = avey_host::encode_rows16(p->dtype, dz, n, p->rows, 1, ld * 2, 0, 64, &m.dz_w);
+        if (rc == AVEY_OK) rc = avey_host::encode_rows16(p->dtype, x.p, p->width, p->rows, 1, x.ld * 2, 0, 64, &m.x_w);
+        if (rc == AVEY_OK)
+          rc = avey_host::encode_rows16(p->dtype, k.copy, p->width, p->rows, 1, k.copy_ld * 2, 0, 64, &m.x2);
+        if (rc == AVEY_OK && q.dw_vec)
+          rc = avey_host::encode_tiles(p->dtype, dw, p->width, n, 1, p->width * 2, 0, &m.y_dw);
+        if (rc != AVEY_OK) return rc;
+        if (jobs == 2 && q.job[1].nk > q.job[0].nk / splits) std::swap(q.job[0], q.job[1]);  // the longest first
+      }
+    }
+    if (i < l.pieces) {
+      const int64_t v0 = i * l.piece, n = std::min(l.piece, p->vocab - v0), ld = up(n, 8);
+      const int cols = logit_cols(p->rows, n);
+      q.job[jobs] = job(avey::kCeGrad, p->rows, n, p->width, cols);
+      q.job[jobs].seg = unit_tiles(q.job[jobs].n_mt, q.job[jobs].n_nt);
+      q.job[jobs].units = (q.job[jobs].n_nt + q.job[jobs].seg - 1) / q.job[jobs].seg * q.job[jobs].n_mt;
+      ++jobs;
       q.col0 = static_cast<int>(v0);
-      q.lse = p->saved;
-      q.coef = k.coef;
-      q.largest = largest;
-      Maps m;
-      rc = avey_host::encode_rows16(p->dtype, x.p, p->width, p->rows, 1, x.ld * 2, 0, 128, &m.a);
-      if (rc == AVEY_OK) rc = avey_host::encode_rows16(p->dtype, wp, p->width, n, 1, w.ld * 2, 0, bn / 2, &m.b);
-      if (rc == AVEY_OK) rc = avey_host::encode_tiles(p->dtype, dz, n, p->rows, 1, ld * 2, 0, &m.y);
-      if (rc == AVEY_OK) rc = launch_product<avey::ce_product<T, avey::kCeGrad, false>>(m, q, chain);
-      if (rc != AVEY_OK) return rc;
-    }
-    if (p->dx) {
-      const int bn = grad_cols(p->rows, p->width);
-      avey::CeGeom q = geom(p, p->rows, p->width, n, bn);
-      q.largest = largest;
-      q.out = p->dx;
-      q.out_ld = p->dx_ld;
-      q.out_vec = whole_rows(p->dx, p->dx_ld);
-      q.add = v0 > 0;
-      Maps m;
-      rc = avey_host::encode_rows16(p->dtype, dz, n, p->rows, 1, ld * 2, 0, 128, &m.a);
-      if (rc == AVEY_OK) rc = avey_host::encode_rows16(p->dtype, wp, p->width, n, 1, w.ld * 2, 0, 64, &m.b);
-      if (rc == AVEY_OK && planes) rc = avey_host::encode_tiles(AVEY_F32, sums, p->width, p->rows, 1, sums_ld * 4, 0, &m.y);
-      if (rc == AVEY_OK && !planes && q.out_vec)
-        rc = avey_host::encode_tiles(p->dtype, p->dx, p->width, p->rows, 1, p->dx_ld * 2, 0, &m.y);
+      rc = avey_host::encode_rows16(p->dtype, x.p, p->width, p->rows, 1, x.ld * 2, 0, 128, &m.x);
       if (rc == AVEY_OK)
-        rc = planes ? launch_product<avey::ce_product<T, avey::kCeDx, true>>(m, q, chain)
-                    : launch_product<avey::ce_product<T, avey::kCeDx, false>>(m, q, chain);
+        rc = avey_host::encode_rows16(p->dtype, static_cast<const char*>(w.p) + v0 * w.ld * 2, p->width, n, 1, w.ld * 2,
+                                      0, cols / 2, &m.w);
+      if (rc == AVEY_OK)
+        rc = avey_host::encode_tiles(p->dtype, ws + l.dz + i % 2 * l.dz_bytes, n, p->rows, 1, ld * 2, 0, &m.dz_out);
       if (rc != AVEY_OK) return rc;
     }
-    if (p->dweight) {
-      char* dw = static_cast<char*>(p->dweight) + v0 * p->width * 2;
-      const int bn = grad_cols(n, p->width);
-      avey::CeGeom q = geom(p, n, p->width, p->rows, bn);
-      q.largest = largest;
-      q.out = dw;
-      q.out_ld = p->width;
-      q.out_vec = whole_rows(dw, p->width);
-      q.dirty = k.dirty;
-      Maps m;
-      rc = avey_host::encode_rows16(p->dtype, dz, n, p->rows, 1, ld * 2, 0, 64, &m.a);
-      if (rc == AVEY_OK) rc = avey_host::encode_rows16(p->dtype, x.p, p->width, p->rows, 1, x.ld * 2, 0, 64, &m.b);
-      if (rc == AVEY_OK) rc = avey_host::encode_rows16(p->dtype, k.copy, p->width, p->rows, 1, k.copy_ld * 2, 0, 64, &m.b2);
-      if (rc == AVEY_OK && q.out_vec) rc = avey_host::encode_tiles(p->dtype, dw, p->width, n, 1, p->width * 2, 0, &m.y);
-      if (rc == AVEY_OK) rc = launch_product<avey::ce_product<T, avey::kCeDw, false>>(m, q, chain);
+    set_ring(q);
+    rc = launch_product<avey::ce_product<T, false>>(m, q, chain);
+    if (rc != AVEY_OK) return rc;
+    if (splits > 1) {
+      avey::CeParts j{};
+      j.parts = parts;
+      j.m = static_cast<int>(p->rows);
+      j.n = static_cast<int>(p->width);
+      j.bn = bn;
+      j.n_nt = static_cast<int>((p->width + bn - 1) / bn);
+      j.tiles = static_cast<int>(tiles_of(p->rows, p->width, bn));
+      j.splits = splits;
+      j.largest = largest;
+      j.out = planes ? static_cast<void*>(sums) : p->dx;
+      j.out_ld = planes ? sums_ld : p->dx_ld;
+      j.add = i > 1;
+      const int64_t grid = static_cast<int64_t>(j.tiles) * (avey::kCeBM / avey::kCeJoinRows);
+      rc = planes ? chain.launch("cross entropy parts", avey::ce_join_parts<T, true>, grid, 256, 0, 1, j)
+                  : chain.launch("cross entropy parts", avey::ce_join_parts<T, false>, grid, 256, 0, 1, j);
       if (rc != AVEY_OK) return rc;
     }
   }

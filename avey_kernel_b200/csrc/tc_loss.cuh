@@ -21,9 +21,13 @@
 // Warp 0 issues TMA, warp 1 of the even CTA tcgen05.mma into one of two TMEM
 // accumulators, warps 4-19 of each CTA drain the other one. Every wait is bounded.
 //
-// stats and grad take the tiles in units of up to 4 column tiles of one row
-// tile, rows first, so that the pairs at work share W's rows in L2 and a row's
-// (c, s) stay in registers over a unit.
+// The pairs claim units of work from a counter, the longest first, so that they end
+// together: a unit is up to 4 column tiles of one row tile for the statistics and dz (a
+// row's numbers stay in registers over it), else one tile. The gradients' launches
+// hold three kinds: dX and dW of one piece and dz of the next (in the other half of
+// dz), whose short units fill what the long ones leave of the last wave. (With a
+// launch for each kind 48 tiles of dX on 74 pairs took 370 us instead of 150.) Who
+// takes a unit does not change its result.
 #pragma once
 
 #include "tc_linear.cuh"
@@ -40,15 +44,25 @@ constexpr int kCeStaging = kLnEpiWarps * kLnStageTile;
 constexpr int kCeCtrlBytes = 512;
 constexpr int kCeSmem = 1024 + kCeRing + kCeStaging + kCeCtrlBytes;
 
-enum CeMode { kCeStats = 0, kCeGrad = 1, kCeDx = 2, kCeDw = 3 };
+enum CeKind { kCeStats = 0, kCeGrad = 1, kCeDx = 2, kCeDw = 3 };
+template <int K>
+using CeKindOf = std::integral_constant<int, K>;
+
+// Units of one kind in a launch.
+struct CeJob {
+  int kind, units;
+  int m, n, nk;            // output rows and columns, K blocks
+  int bn, n_mt, n_nt;      // columns of a tile, tiles
+  int seg;                 // stats, grad: column tiles of a unit; dX: K ranges of a tile
+};
+constexpr int kCeJobs = 3;
 
 struct CeGeom {
-  int m, n, k;             // output rows and columns, contraction
-  int bn, n_mt, n_nt;      // columns of a tile, tiles
-  int seg, units;          // column tiles of a unit, units
+  CeJob job[kCeJobs];
+  int units;               // of all kinds
   int stages, stage_bytes;
-  int rows;                // tokens
-  int vocab;
+  unsigned int* claimed;   // the next unit, zero before; or null
+  int rows, vocab;
   int col0;                // grad: the piece's first column
   const void* targets;
   int64_t target_stride;
@@ -59,10 +73,12 @@ struct CeGeom {
   const float* lse;        // grad: [rows], base 2
   const float2* coef;      // grad: (a, b) of every row
   const uint32_t* largest; // f16: bits of the largest |a|, |b|; null: no scale
-  void* out;               // dX, dW (16 bits), where rows are not stored by TMA
-  int64_t out_ld;
-  int out_vec;
-  int add;                 // dX: sums are added to the fp32 plane
+  void* dx;                // 16 bits; null: fp32 sums by map_dx
+  int64_t dx_ld;
+  int dx_vec, dx_add;      // rows stored by TMA; sums are added to
+  void* dw;
+  int64_t dw_ld;
+  int dw_vec;
   const uint8_t* dirty;    // dW: K blocks whose rows come from the second map
   int test_stall;
 };
@@ -87,14 +103,102 @@ __device__ __forceinline__ float ce_scale(const uint32_t* largest, bool inverse)
   return __uint_as_float(static_cast<uint32_t>(127 + (inverse ? -k : k)) << 23);
 }
 
+constexpr int kCeAhead = 4;  // units that the scheduler may be ahead of the last reader
+
 struct CeCtrl {
   uint64_t full[kCeMaxStages], empty[kCeMaxStages];
+  uint64_t unit_full[kCeAhead], unit_empty[kCeAhead];
+  uint64_t want;               // the even CTA's TMA lane is near the end of its unit
   uint64_t acc_full[2], acc_empty[2];
+  uint64_t met[4], joined[4];  // stats: a row quarter's parts have been written, and read
   uint64_t settled;
+  int unit[kCeAhead];
   uint32_t failed;
   uint32_t tmem_base;
 };
 static_assert(sizeof(CeCtrl) <= kCeCtrlBytes, "control block too large");
+
+// Arrive on an mbarrier of either CTA. Nothing in memory is handed over with it (the
+// reads of tensor memory before it are ordered by their wait and fence), so it is
+// relaxed: a release for the cluster makes each warp wait for a fence.
+__device__ __forceinline__ void ce_arrive(uint32_t cluster_bar) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
+}
+
+// The scheduler (a lane of the even CTA) hands unit u, the i-th of the pair, to every
+// role of both CTAs: the store counts as 4 bytes on the barrier beside it.
+__device__ __forceinline__ bool ce_hand(CeCtrl* ctrl, int i, int u) {
+  const int slot = i % kCeAhead;
+  if (i >= kCeAhead && !mbar_wait(smem_u32(&ctrl->unit_empty[slot]), (i / kCeAhead - 1) & 1)) return false;
+#pragma unroll
+  for (uint32_t cta = 0; cta < 2; ++cta)
+    asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.u32 [%0], %1, [%2];" ::"r"(
+                     mapa_shared(smem_u32(&ctrl->unit[slot]), cta)),
+                 "r"(u), "r"(mapa_shared(smem_u32(&ctrl->unit_full[slot]), cta))
+                 : "memory");
+  return true;
+}
+// The pair's i-th unit (-1: none is left, or a wait gave up). Without a counter (units
+// of one kind) a pair takes every pairs-th one.
+__device__ __forceinline__ int ce_unit(const CeGeom& q, CeCtrl* ctrl, int i) {
+  if (!q.claimed) {
+    const int64_t u = (blockIdx.x >> 1) + static_cast<int64_t>(i) * (gridDim.x >> 1);
+    return u < q.units ? static_cast<int>(u) : -1;
+  }
+  const int slot = i % kCeAhead;
+  if (!mbar_wait(smem_u32(&ctrl->unit_full[slot]), (i / kCeAhead) & 1)) return -1;
+  return *reinterpret_cast<volatile int*>(&ctrl->unit[slot]);
+}
+// By one lane of each role once it has been read.
+__device__ __forceinline__ void ce_unit_read(const CeGeom& q, CeCtrl* ctrl, int i) {
+  if (q.claimed) ce_arrive(mapa_shared(smem_u32(&ctrl->unit_empty[i % kCeAhead]), 0));
+}
+// The same for a whole warp.
+__device__ __forceinline__ int ce_warp_unit(const CeGeom& q, CeCtrl* ctrl, int i) {
+  const int u = __reduce_min_sync(0xFFFFFFFFu, ce_unit(q, ctrl, i));
+  if (u >= 0 && (threadIdx.x & 31) == 0) ce_unit_read(q, ctrl, i);
+  return u;
+}
+
+// A unit's tiles: `count` column tiles from (mt, nt) on, K blocks k0 to k1 of them.
+struct CeUnit {
+  int job, mt, nt, count, k0, k1;
+  int part;  // stats: the segment; dX: where the sums of a cut tile go, or -1
+};
+template <bool STATS>
+__device__ __forceinline__ CeUnit ce_set_unit(const CeGeom& q, int u) {
+  CeUnit c;
+  c.job = 0;
+  if (!STATS) {
+#pragma unroll
+    for (int j = 0; j < kCeJobs - 1; ++j)
+      if (c.job == j && u >= q.job[j].units) {
+        u -= q.job[j].units;
+        c.job = j + 1;
+      }
+  }
+  const CeJob& b = q.job[c.job];
+  c.k0 = 0;
+  c.k1 = b.nk;
+  c.count = 1;
+  c.part = -1;
+  if (STATS || b.kind == kCeGrad) {
+    c.part = u / b.n_mt;  // rows first: the pairs at work share W's rows in L2
+    c.mt = u - c.part * b.n_mt;
+    c.nt = c.part * b.seg;
+    c.count = min(b.seg, b.n_nt - c.nt);
+  } else {
+    const int tiles = b.n_mt * b.n_nt, split = u / tiles, t = u - split * tiles;
+    c.mt = t / b.n_nt;
+    c.nt = t - c.mt * b.n_nt;
+    if (b.seg > 1) {
+      c.k0 = static_cast<int>(static_cast<int64_t>(b.nk) * split / b.seg);
+      c.k1 = static_cast<int>(static_cast<int64_t>(b.nk) * (split + 1) / b.seg);
+      c.part = u;
+    }
+  }
+  return c;
+}
 
 __device__ __forceinline__ void tma_reduce_add_3d(const void* tmap, uint32_t src, int x, int y, int z) {
   asm volatile(
@@ -103,44 +207,6 @@ __device__ __forceinline__ void tma_reduce_add_3d(const void* tmap, uint32_t src
       "r"(x), "r"(y), "r"(z), "r"(src)
       : "memory");
 }
-
-// A pair's i-th tile.
-struct CeTile {
-  int mt, nt;
-  bool first, last;  // of its unit
-  int seg;
-};
-// Walks a pair's tiles in order.
-template <int MODE>
-struct CeWalker {
-  int unit, step, stop;
-  __device__ __forceinline__ CeWalker(int pair, int pairs) : unit(pair), step(pairs), stop(0) {}
-  int nt = 0, mt = 0, sg = 0;
-  __device__ __forceinline__ bool next(const CeGeom& q, CeTile& c) {
-    if (nt >= stop) {
-      if (unit >= q.units) return false;
-      if (MODE == kCeStats || MODE == kCeGrad) {
-        sg = unit / q.n_mt;
-        mt = unit - sg * q.n_mt;
-        nt = sg * q.seg;
-        stop = min(q.n_nt, nt + q.seg);
-      } else {
-        mt = unit / q.n_nt;
-        nt = unit - mt * q.n_nt;
-        stop = nt + 1;
-      }
-      unit += step;
-      c.first = true;
-    } else {
-      c.first = false;
-    }
-    c.mt = mt;
-    c.nt = nt++;
-    c.last = nt >= stop;
-    c.seg = sg;
-    return true;
-  }
-};
 
 // What an epilogue lane holds of its row.
 struct CeRow {
@@ -204,35 +270,166 @@ __device__ __forceinline__ void ce_grad32(const uint32_t (&o)[32], int at, const
   }
 }
 
-template <typename T, int MODE, bool F32>
+struct CeMaps {
+  CUtensorMap x, w;           // the logits' operands, K-major
+  CUtensorMap dz_out, y_dx;   // where dz and dX go (dX: 16 bits or fp32 sums)
+  CUtensorMap dz_x, w_x;      // dX's operands
+  CUtensorMap dz_w, x_w, x2;  // dW's operands, and the copy of x's blocks that hold ignored rows
+  CUtensorMap y_dw, parts;
+};
+
+// Arrive on the barrier at this offset in both CTAs when the products issued so far are done.
+__device__ __forceinline__ void ce_commit_both(uint32_t bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+      "h"(static_cast<uint16_t>(3))
+      : "memory");
+}
+
+// The ring as a producing or consuming lane walks it.
+struct CeRingAt {
+  int st = 0;
+  uint32_t ph = 0;
+  __device__ __forceinline__ void next(int stages) {
+    if (++st == stages) {
+      st = 0;
+      ph ^= 1u;
+    }
+  }
+};
+
+// One CTA's loads for a unit (`half` columns of B a tile from bcol on). The next unit
+// is asked for eight K blocks before the end: late, so that the pairs end together, and
+// early enough for its number to arrive in time. The loops of the TMA and MMA lanes are
+// compiled for each kind: with the kind looked up in them dX and dW of 4096 x 32768
+// (width 768) took 689,000 cycles instead of 458,000.
+template <int KIND>
+__device__ __forceinline__ bool ce_load_unit(const CeMaps& maps, const CeGeom& q, const CeUnit& c, CeCtrl* ctrl,
+                                             uint32_t base, bool leader, int arow, int bcol, int bn, int half,
+                                             CeRingAt& at, int& fills, uint64_t keep) {
+  const uint32_t bytes = 2u * (kCeHalfA + half * kLnBK * 2);
+  const int stages = q.stages, stage_bytes = q.stage_bytes, k0 = c.k0, k1 = c.k1;
+  const int count = KIND == kCeStats || KIND == kCeGrad ? c.count : 1;
+  const int ask = max(k0, k1 - 8);
+  for (int t = 0; t < count; ++t, bcol += bn) {
+#pragma unroll 1
+    for (int kk = k0; kk < k1; ++kk) {
+      if (kk == ask && leader && t == count - 1 && q.claimed) mbar_arrive(smem_u32(&ctrl->want));
+      if (fills >= stages && !mbar_wait(smem_u32(&ctrl->empty[at.st]), at.ph ^ 1u)) return false;
+      const uint32_t mine = smem_u32(&ctrl->full[at.st]), full = mapa_shared(mine, 0);
+      const uint32_t sa = base + at.st * stage_bytes, sb = sa + kCeHalfA;
+      const int kx = kk * kLnBK;
+      if (leader) mbar_arrive_expect_tx(mine, bytes);
+      if constexpr (KIND == kCeStats || KIND == kCeGrad) {
+        tma_load_3d_pair(sa, &maps.x, full, kx, arow, 0, keep);
+        tma_load_3d_pair(sb, &maps.w, full, kx, bcol, 0, keep);
+      } else if constexpr (KIND == kCeDx) {
+        tma_load_3d_pair(sa, &maps.dz_x, full, kx, arow, 0, keep);
+        tma_load_3d_pair(sb, &maps.w_x, full, bcol, kx, 0, keep);
+        if (half > 64) tma_load_3d_pair(sb + kLnMnBox, &maps.w_x, full, bcol + 64, kx, 0, keep);
+      } else {
+        tma_load_3d_pair(sa, &maps.dz_w, full, arow, kx, 0, keep);
+        tma_load_3d_pair(sa + kLnMnBox, &maps.dz_w, full, arow + 64, kx, 0, keep);
+        const CUtensorMap* mb = __ldg(q.dirty + kk) ? &maps.x2 : &maps.x_w;
+        tma_load_3d_pair(sb, mb, full, bcol, kx, 0, keep);
+        if (half > 64) tma_load_3d_pair(sb + kLnMnBox, mb, full, bcol + 64, kx, 0, keep);
+      }
+      ++fills;
+      at.next(stages);
+    }
+  }
+  return true;
+}
+
+// The products of a unit.
+template <int KIND, uint32_t FMT>
+__device__ __forceinline__ bool ce_multiply_unit(const CeGeom& q, const CeUnit& c, CeCtrl* ctrl, uint32_t base,
+                                                 uint32_t tmem, int bn, CeRingAt& at, int& it) {
+  constexpr bool kAMn = KIND == kCeDw, kBMn = KIND == kCeDx || KIND == kCeDw;
+  const uint32_t idesc = idesc_f16(FMT, kCeBM, static_cast<uint32_t>(bn), kAMn ? 1u : 0u, kBMn ? 1u : 0u);
+  const uint64_t da0 = kAMn ? smem_desc_sw128(base, kLnMnBox, 1024) : smem_desc_sw128(base, 16, 1024);
+  const uint64_t db0 =
+      kBMn ? smem_desc_sw128(base + kCeHalfA, kLnMnBox, 1024) : smem_desc_sw128(base + kCeHalfA, 16, 1024);
+  constexpr uint32_t ka = kAMn ? (2048u >> 4) : 2u, kb = kBMn ? (2048u >> 4) : 2u;
+  const int stages = q.stages, stage_bytes = q.stage_bytes, blocks = c.k1 - c.k0;
+  const int count = KIND == kCeStats || KIND == kCeGrad ? c.count : 1;
+  for (int t = 0; t < count; ++t, ++it) {
+    const int buf = it & 1;
+    if (it >= 2) {
+      if (!mbar_wait(smem_u32(&ctrl->acc_empty[buf]), ((it >> 1) - 1) & 1)) return false;
+      tc_fence_after();
+    }
+    const uint32_t d_tmem = tmem + static_cast<uint32_t>(buf * 256);
+#pragma unroll 1
+    for (int kk = 0; kk < blocks; ++kk) {
+      if (!mbar_wait(smem_u32(&ctrl->full[at.st]), at.ph)) return false;
+      tc_fence_after();
+      const uint32_t adv = static_cast<uint32_t>(at.st * stage_bytes) >> 4;
+#pragma unroll
+      for (int k = 0; k < kLnBK / 16; ++k)
+        tc_mma_f16_pair(d_tmem, da0 + adv + ka * k, db0 + adv + kb * k, idesc, (kk != 0 || k != 0) ? 1u : 0u);
+      ce_commit_both(smem_u32(&ctrl->empty[at.st]));
+      at.next(stages);
+    }
+    ce_commit_both(smem_u32(&ctrl->acc_full[buf]));
+  }
+  return true;
+}
+
+// Store a warp's 32 x 32 fp32 sums (from TMEM) at column x, row y of a map.
+__device__ __forceinline__ void ce_store_f32(uint32_t tb, uint32_t tile, int lane, const CUtensorMap* map, int x, int y,
+                                             bool add, uint64_t policy) {
+#pragma unroll
+  for (int hh = 0; hh < 2; ++hh) {
+    uint32_t o[16];
+    ln_tmem_ld16(tb + 16 * hh, false, o);
+    ln_tile_free(lane);
+#pragma unroll
+    for (int p = 0; p < 4; ++p) ln_sts(ln_piece(tile, lane, p), o[4 * p], o[4 * p + 1], o[4 * p + 2], o[4 * p + 3]);
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+      if (add) tma_reduce_add_3d(map, tile, x + 16 * hh, y, 0);
+      else tma_store_3d(map, tile, x + 16 * hh, y, 0, policy);
+      bulk_commit_group();
+    }
+  }
+}
+
+template <typename T, bool STATS>
 __global__ void __launch_bounds__(kCeThreads, 1)
-    ce_product(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
-               const __grid_constant__ CUtensorMap map_b2, const __grid_constant__ CUtensorMap map_y, const CeGeom q) {
+    ce_product(const __grid_constant__ CeMaps maps, const __grid_constant__ CeGeom q) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
   const uint32_t staging = base + kCeRing;
   CeCtrl* ctrl = reinterpret_cast<CeCtrl*>(smem_raw + (base - raw) + kCeRing + kCeStaging);
-  constexpr bool kAMn = MODE == kCeDw, kBMn = MODE == kCeDx || MODE == kCeDw;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t rank = cluster_rank();
   const bool leader = rank == 0;
-  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
   if (tid == 0) {
     for (int s = 0; s < q.stages; ++s) {
       mbar_init(smem_u32(&ctrl->full[s]), 1);
       mbar_init(smem_u32(&ctrl->empty[s]), 1);
     }
+    for (int i = 0; i < kCeAhead; ++i) {
+      mbar_init(smem_u32(&ctrl->unit_full[i]), 1);
+      // Both CTAs' TMA lanes and epilogue warps, and the MMA lane.
+      mbar_init(smem_u32(&ctrl->unit_empty[i]), 2 * (1 + kLnEpiWarps) + 1);
+    }
     for (int i = 0; i < 2; ++i) {
       mbar_init(smem_u32(&ctrl->acc_full[i]), 1);
-      mbar_init(smem_u32(&ctrl->acc_empty[i]), 2 * kLnEpiWarps);  // the epilogue warps of both CTAs
+      mbar_init(smem_u32(&ctrl->acc_empty[i]), 2 * kLnEpiWarps);
     }
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(smem_u32(&ctrl->met[i]), 3);
+      mbar_init(smem_u32(&ctrl->joined[i]), 1);
+    }
+    mbar_init(smem_u32(&ctrl->want), 1);
     mbar_init(smem_u32(&ctrl->settled), 1);
     ctrl->failed = 0;
     fence_mbar_init();
-    tma_prefetch_desc(&map_a);
-    tma_prefetch_desc(&map_b);
   }
   if (warp == 1) {
     tmem_alloc_pair(smem_u32(&ctrl->tmem_base), 512);
@@ -252,44 +449,26 @@ __global__ void __launch_bounds__(kCeThreads, 1)
     // ============================================================ TMA producer (both CTAs)
     if (lane == 0) {
       const uint64_t keep = l2_policy_evict_last();
-      const int half = q.bn / 2;  // this CTA's columns of B
-      const int nk = (q.k + kLnBK - 1) / kLnBK;
-      int st = 0;
-      uint32_t ph = 0;
+      CeRingAt at;
       bool alive = !q.test_stall;
-      CeWalker<MODE> w(pair, pairs);
-      CeTile c;
-      while (alive && w.next(q, c)) {
+      for (int i = 0; alive; ++i) {
+        // The lane that expects the unit's four bytes.
+        if (q.claimed) mbar_arrive_expect_tx(smem_u32(&ctrl->unit_full[i % kCeAhead]), 4);
+        const int u = ce_unit(q, ctrl, i);
+        if (u < 0) break;
+        ce_unit_read(q, ctrl, i);
+        const CeUnit c = ce_set_unit<STATS>(q, u);
+        const CeJob& b = q.job[c.job];
+        const int bn = b.bn, half = bn / 2, kind = b.kind;  // half: this CTA's columns of B
         const int arow = c.mt * kCeBM + static_cast<int>(rank) * 128;
-        const int bcol = c.nt * q.bn + static_cast<int>(rank) * half;
-        for (int kk = 0; kk < nk; ++kk) {
-          if (fills >= q.stages && !mbar_wait(smem_u32(&ctrl->empty[st]), ph ^ 1u)) {
-            alive = false;
-            break;
-          }
-          const uint32_t full = mapa_shared(smem_u32(&ctrl->full[st]), 0);
-          const uint32_t sa = base + st * q.stage_bytes, sb = sa + kCeHalfA;
-          const int kx = kk * kLnBK;
-          if (leader) mbar_arrive_expect_tx(smem_u32(&ctrl->full[st]), 2 * q.stage_bytes);
-          if (!kAMn) {
-            tma_load_3d_pair(sa, &map_a, full, kx, arow, 0, keep);
-          } else {
-            tma_load_3d_pair(sa, &map_a, full, arow, kx, 0, keep);
-            tma_load_3d_pair(sa + kLnMnBox, &map_a, full, arow + 64, kx, 0, keep);
-          }
-          if (!kBMn) {
-            tma_load_3d_pair(sb, &map_b, full, kx, bcol, 0, keep);
-          } else {
-            const CUtensorMap* mb = MODE == kCeDw && q.dirty && q.dirty[kk] ? &map_b2 : &map_b;
-            for (int j = 0; j < half / 64; ++j)
-              tma_load_3d_pair(sb + j * kLnMnBox, mb, full, bcol + j * 64, kx, 0, keep);
-          }
-          ++fills;
-          if (++st == q.stages) {
-            st = 0;
-            ph ^= 1u;
-          }
-        }
+        const int bcol = c.nt * bn + static_cast<int>(rank) * half;
+        auto load = [&](auto k) {
+          return ce_load_unit<decltype(k)::value>(maps, q, c, ctrl, base, leader, arow, bcol, bn, half, at, fills, keep);
+        };
+        if constexpr (STATS) alive = load(CeKindOf<kCeStats>{});
+        else if (kind == kCeGrad) alive = load(CeKindOf<kCeGrad>{});
+        else if (kind == kCeDx) alive = load(CeKindOf<kCeDx>{});
+        else alive = load(CeKindOf<kCeDw>{});
       }
       // Until the leader's commits have released every stage that this CTA filled:
       // no signal of theirs may come after the CTA is gone.
@@ -300,173 +479,159 @@ __global__ void __launch_bounds__(kCeThreads, 1)
   } else if (warp == 1) {
     // ============================================================ MMA issuer (even CTA)
     if (lane == 0 && leader) {
-      const uint32_t idesc = idesc_f16(std::is_same<T, __nv_bfloat16>::value ? 1u : 0u, kCeBM,
-                                       static_cast<uint32_t>(q.bn), kAMn ? 1u : 0u, kBMn ? 1u : 0u);
-      const uint64_t da0 = kAMn ? smem_desc_sw128(base, kLnMnBox, 1024) : smem_desc_sw128(base, 16, 1024);
-      const uint64_t db0 =
-          kBMn ? smem_desc_sw128(base + kCeHalfA, kLnMnBox, 1024) : smem_desc_sw128(base + kCeHalfA, 16, 1024);
-      constexpr uint32_t ka = kAMn ? (2048u >> 4) : 2u, kb = kBMn ? (2048u >> 4) : 2u;
-      const int nk = (q.k + kLnBK - 1) / kLnBK;
-      int st = 0, it = 0;
-      uint32_t ph = 0;
+      constexpr uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+      CeRingAt at;
+      int it = 0, u;
       bool alive = true;
-      CeWalker<MODE> w(pair, pairs);
-      CeTile c;
-      for (; alive && w.next(q, c); ++it) {
-        const int buf = it & 1;
-        if (it >= 2) {
-          if (!mbar_wait(smem_u32(&ctrl->acc_empty[buf]), ((it >> 1) - 1) & 1)) {
-            alive = false;
-            break;
-          }
-          tc_fence_after();
-        }
-        const uint32_t d_tmem = tmem + static_cast<uint32_t>(buf * 256);
-        for (int kk = 0; kk < nk; ++kk) {
-          if (!mbar_wait(smem_u32(&ctrl->full[st]), ph)) {
-            alive = false;
-            break;
-          }
-          tc_fence_after();
-          const uint32_t adv = static_cast<uint32_t>(st * q.stage_bytes) >> 4;
-#pragma unroll
-          for (int k = 0; k < kLnBK / 16; ++k)
-            tc_mma_f16_pair(d_tmem, da0 + adv + ka * k, db0 + adv + kb * k, idesc, (kk != 0 || k != 0) ? 1u : 0u);
-          tc_commit_pair(smem_u32(&ctrl->empty[st]));
-          tc_commit_pair(mapa_shared(smem_u32(&ctrl->empty[st]), 1));
-          if (++st == q.stages) {
-            st = 0;
-            ph ^= 1u;
-          }
-        }
-        if (!alive) break;
-        tc_commit_pair(smem_u32(&ctrl->acc_full[buf]));
-        tc_commit_pair(mapa_shared(smem_u32(&ctrl->acc_full[buf]), 1));
+      for (int i = 0; alive && (u = ce_unit(q, ctrl, i)) >= 0; ++i) {
+        ce_unit_read(q, ctrl, i);
+        const CeUnit c = ce_set_unit<STATS>(q, u);
+        const CeJob& b = q.job[c.job];
+        const int bn = b.bn, kind = b.kind;
+        auto multiply = [&](auto k) {
+          return ce_multiply_unit<decltype(k)::value, fmt>(q, c, ctrl, base, tmem, bn, at, it);
+        };
+        if constexpr (STATS) alive = multiply(CeKindOf<kCeStats>{});
+        else if (kind == kCeGrad) alive = multiply(CeKindOf<kCeGrad>{});
+        else if (kind == kCeDx) alive = multiply(CeKindOf<kCeDx>{});
+        else alive = multiply(CeKindOf<kCeDw>{});
       }
       if (!alive) ctrl->failed = 1;
+    }
+  } else if (warp == 3) {
+    // ============================================================ scheduler (even CTA)
+    if (lane == 0 && leader && q.claimed) {
+      for (int i = 0, u = 0; u >= 0; ++i) {
+        if (i > 0 && !mbar_wait(smem_u32(&ctrl->want), (i - 1) & 1)) break;
+        const unsigned int claim = atomicAdd(q.claimed, 1u);
+        u = claim < static_cast<unsigned int>(q.units) ? static_cast<int>(claim) : -1;
+        if (!ce_hand(ctrl, i, u)) break;
+      }
     }
   } else if (warp >= 4) {
     // ============================================================ epilogue (both CTAs)
     const int h = (warp - 4) >> 2;  // column part of the tile
     const int wq = warp & 3;        // TMEM lane quarter
-    const int part = max(32, q.bn >> 2);
     const uint32_t lane_off = static_cast<uint32_t>(wq * 32) << 16;
     const uint32_t tile = staging + static_cast<uint32_t>((warp - 4) * kLnStageTile);
     const uint32_t freed0 = mapa_shared(smem_u32(&ctrl->acc_empty[0]), 0);
     const uint32_t freed1 = mapa_shared(smem_u32(&ctrl->acc_empty[1]), 0);
     const uint64_t policy = l2_policy_evict_normal();
-    const float scale = MODE == kCeGrad ? ce_scale(q.largest, false) : MODE == kCeStats ? 1.f : ce_scale(q.largest, true);
-    CeWalker<MODE> w(pair, pairs);
-    CeTile c;
+    const float scale = STATS ? 1.f : ce_scale(q.largest, false), unscale = STATS ? 1.f : ce_scale(q.largest, true);
     CeRow r{};
-    bool alive = true;  // a warp that gave up still meets the others at their barriers
-    for (int it = 0; w.next(q, c); ++it) {
-      const int buf = it & 1;
+    bool alive = true;
+    int it = 0, u;
+    for (int i = 0; alive && (u = ce_warp_unit(q, ctrl, i)) >= 0; ++i) {
+      const CeUnit c = ce_set_unit<STATS>(q, u);
+      const CeJob b = q.job[c.job];
+      const int part = max(32, b.bn >> 2);
       const int row0 = c.mt * kCeBM + static_cast<int>(rank) * 128 + wq * 32, row = row0 + lane;
-      const int col0 = c.nt * q.bn + h * part;
-      const int nch = row0 < q.m && h * part < q.bn ? max(0, min(part, q.n - col0) + 31) / 32 : 0;
-      if ((MODE == kCeStats || MODE == kCeGrad) && c.first) {
-        r.target = row < q.m ? ce_target(q.targets, q.target_stride, q.target64, q.ignore, q.vocab, row) : -1;
-        if (MODE == kCeGrad) {
-          const float2 ab = row < q.m ? __ldg(q.coef + row) : make_float2(0.f, 0.f);
+      const bool logits = STATS || b.kind == kCeGrad;
+      if (logits) {
+        r.target = row < b.m ? ce_target(q.targets, q.target_stride, q.target64, q.ignore, q.vocab, row) : -1;
+        if (!STATS) {
+          const float2 ab = row < b.m ? __ldg(q.coef + row) : make_float2(0.f, 0.f);
           r.a = ab.x * scale;
           r.b = ab.y * scale;
-          r.lse = row < q.m ? __ldg(q.lse + row) : 0.f;
+          r.lse = row < b.m ? __ldg(q.lse + row) : 0.f;
         }
         r.c = -INFINITY;
         r.s = 0.f;
       }
-      if (alive && !ln_warp_wait(smem_u32(&ctrl->acc_full[buf]), (it >> 1) & 1)) {
-        if (lane == 0) ctrl->failed = 1;
-        alive = false;
-      }
-      if (!alive && MODE != kCeStats) break;
-      tc_fence_after();
-      const uint32_t tb = tmem + lane_off + static_cast<uint32_t>(buf * 256 + h * part);
+      for (int t = 0; t < c.count; ++t, ++it) {
+        const int buf = it & 1;
+        const int col0 = (c.nt + t) * b.bn + h * part;
+        const int nch = row0 < b.m && h * part < b.bn ? max(0, min(part, b.n - col0) + 31) / 32 : 0;
+        if (alive && !ln_warp_wait(smem_u32(&ctrl->acc_full[buf]), (it >> 1) & 1)) {
+          if (lane == 0) ctrl->failed = 1;
+          alive = false;
+        }
+        if (!alive) break;
+        tc_fence_after();
+        const uint32_t tb = tmem + lane_off + static_cast<uint32_t>(buf * 256 + h * part);
 #pragma unroll 1
-      for (int ch = 0; ch < nch && alive; ++ch) {
-        const int col = col0 + ch * 32;
-        if constexpr (MODE == kCeStats || MODE == kCeGrad) {
-          uint32_t o[32];
-          tmem_ld32(tb + ch * 32, o);
-          tmem_wait_ld(o);
-          const int at = r.target - q.col0 - col;  // the target's place among the 32
-          const bool hit = __any_sync(0xFFFFFFFFu, r.target >= 0 && at >= 0 && at < 32);
-          if constexpr (MODE == kCeStats) {
-            if (hit) {
+        for (int ch = 0; ch < nch; ++ch) {
+          const int col = col0 + ch * 32;
+          if (logits) {
+            uint32_t o[32];
+            tmem_ld32(tb + ch * 32, o);
+            tmem_wait_ld(o);
+            const int at = r.target - q.col0 - col;  // the target's place among the 32
+            const bool hit = __any_sync(0xFFFFFFFFu, r.target >= 0 && at >= 0 && at < 32);
+            if constexpr (STATS) {
+              if (hit) {
 #pragma unroll
-              for (int j = 0; j < 32; ++j)
-                if (j == at && r.target >= 0) q.picked[row] = __uint_as_float(o[j]);
+                for (int j = 0; j < 32; ++j)
+                  if (j == at && r.target >= 0) q.picked[row] = __uint_as_float(o[j]);
+              }
+              if (col + 32 <= b.n) ce_stats32<false>(o, 32, r);
+              else ce_stats32<true>(o, b.n - col, r);
+            } else {
+              ln_tile_free(lane);
+              if (hit) ce_grad32<T, true>(o, r.target >= 0 ? at : -1, r, tile, lane);
+              else ce_grad32<T, false>(o, -1, r, tile, lane);
+              ln_tma_tile(tile, lane, &maps.dz_out, col, row0, 0, policy);
             }
-            if (col + 32 <= q.n) ce_stats32<false>(o, 32, r);
-            else ce_stats32<true>(o, q.n - col, r);
-          } else {
-            ln_tile_free(lane);
-            if (hit) ce_grad32<T, true>(o, r.target >= 0 ? at : -1, r, tile, lane);
-            else ce_grad32<T, false>(o, -1, r, tile, lane);
-            ln_tma_tile(tile, lane, &map_y, col, row0, 0, policy);
-          }
-        } else if constexpr (F32) {
+          } else if constexpr (!STATS) {
+            if (c.part >= 0) {
+              ce_store_f32(tb + ch * 32, tile, lane, &maps.parts, col - c.nt * b.bn,
+                           c.part * kCeBM + (row0 - c.mt * kCeBM), false, policy);
+            } else if (b.kind == kCeDx && !q.dx) {
+              ce_store_f32(tb + ch * 32, tile, lane, &maps.y_dx, col, row0, q.dx_add, policy);
+            } else {
+              ln_tile_free(lane);
 #pragma unroll
-          for (int hh = 0; hh < 2; ++hh) {
-            uint32_t o[16];
-            ln_tmem_ld16(tb + ch * 32 + 16 * hh, false, o);
-            ln_tile_free(lane);
+              for (int hh = 0; hh < 2; ++hh) {
+                uint32_t o[16];
+                ln_tmem_ld16(tb + ch * 32 + 16 * hh, false, o);
 #pragma unroll
-            for (int p = 0; p < 4; ++p)
-              ln_sts(ln_piece(tile, lane, p), o[4 * p], o[4 * p + 1], o[4 * p + 2], o[4 * p + 3]);
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) {
-              if (q.add) tma_reduce_add_3d(&map_y, tile, col + 16 * hh, row0, 0);
-              else tma_store_3d(&map_y, tile, col + 16 * hh, row0, 0, policy);
-              bulk_commit_group();
+                for (int p = 0; p < 2; ++p) {
+                  uint32_t y[4];
+#pragma unroll
+                  for (int j = 0; j < 4; ++j)
+                    y[j] = ln_pack<T>(__uint_as_float(o[8 * p + 2 * j]) * unscale,
+                                      __uint_as_float(o[8 * p + 2 * j + 1]) * unscale);
+                  ln_sts(ln_piece(tile, lane, 2 * hh + p), y[0], y[1], y[2], y[3]);
+                }
+              }
+              const bool dx = b.kind == kCeDx;
+              if (dx ? q.dx_vec : q.dw_vec) {
+                ln_tma_tile(tile, lane, dx ? &maps.y_dx : &maps.y_dw, col, row0, 0, policy);
+              } else {
+                const LnLines l{row0 + (lane >> 2), b.m, col + (lane & 3) * 8, b.n};
+                __syncwarp();
+                ln_store_tile_by_column(tile, lane, static_cast<uint16_t*>(dx ? q.dx : q.dw), dx ? q.dx_ld : q.dw_ld, l);
+                __syncwarp();
+              }
             }
-          }
-        } else {
-          ln_tile_free(lane);
-#pragma unroll
-          for (int hh = 0; hh < 2; ++hh) {
-            uint32_t o[16];
-            ln_tmem_ld16(tb + ch * 32 + 16 * hh, false, o);
-#pragma unroll
-            for (int p = 0; p < 2; ++p) {
-              uint32_t y[4];
-#pragma unroll
-              for (int j = 0; j < 4; ++j)
-                y[j] = ln_pack<T>(__uint_as_float(o[8 * p + 2 * j]) * scale, __uint_as_float(o[8 * p + 2 * j + 1]) * scale);
-              ln_sts(ln_piece(tile, lane, 2 * hh + p), y[0], y[1], y[2], y[3]);
-            }
-          }
-          if (q.out_vec) {
-            ln_tma_tile(tile, lane, &map_y, col, row0, 0, policy);
-          } else {
-            const LnLines l{row0 + (lane >> 2), q.m, col + (lane & 3) * 8, q.n};
-            __syncwarp();
-            ln_store_tile_by_column(tile, lane, static_cast<uint16_t*>(q.out), q.out_ld, l);
-            __syncwarp();
           }
         }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) ce_arrive(buf ? freed1 : freed0);
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0 && alive) mbar_arrive_cluster(buf ? freed1 : freed0);
-      if (MODE == kCeStats && c.last) {
+      if constexpr (STATS) {
+        if (!alive) break;
         // The four parts of a row meet in shared memory.
         const uint32_t meet = staging + static_cast<uint32_t>(wq * 32 + lane) * 8;
-        if (h > 0)
+        if (h > 0) {
+          alive = i == 0 || ln_warp_wait(smem_u32(&ctrl->joined[wq]), (i - 1) & 1);
           asm volatile("st.shared.v2.f32 [%0], {%1,%2};" ::"r"(meet + h * 1024), "f"(r.c), "f"(r.s) : "memory");
-        named_bar_sync(1 + wq, 128);
-        if (h == 0) {
+          __syncwarp();
+          if (lane == 0 && alive) mbar_arrive(smem_u32(&ctrl->met[wq]));
+        } else {
+          alive = ln_warp_wait(smem_u32(&ctrl->met[wq]), i & 1);
 #pragma unroll
-          for (int i = 1; i < 4; ++i) {
+          for (int j = 1; j < 4; ++j) {
             float c2, s2;
-            asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(c2), "=f"(s2) : "r"(meet + i * 1024));
+            asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(c2), "=f"(s2) : "r"(meet + j * 1024) : "memory");
             ce_join(r.c, r.s, c2, s2);
           }
-          if (row < q.m) q.partial[static_cast<int64_t>(c.seg) * q.rows + row] = make_float2(r.c, r.s);
+          if (row < b.m && alive) q.partial[static_cast<int64_t>(c.part) * q.rows + row] = make_float2(r.c, r.s);
+          __syncwarp();
+          if (lane == 0 && alive) mbar_arrive(smem_u32(&ctrl->joined[wq]));
         }
-        named_bar_sync(1 + wq, 128);  // read before the next unit's
+        if (!alive && lane == 0) ctrl->failed = 1;
       }
     }
     if (lane == 0) bulk_wait_read_all();
@@ -668,6 +833,63 @@ __global__ void __launch_bounds__(256) ce_coef(const CeCoef q) {
     const uint16_t* p = q.x + static_cast<int64_t>(row0 + i) * q.x_ld;
     uint16_t* o = q.copy + static_cast<int64_t>(row0 + i) * q.copy_ld;
     for (int j = tid; j < q.width; j += 256) o[j] = skip[i] ? static_cast<uint16_t>(0) : p[j];
+  }
+}
+
+struct CeParts {
+  const float* parts;      // [splits][tiles][256][bn]
+  int m, n, bn, n_nt, tiles, splits;
+  const uint32_t* largest;
+  void* out;               // 16 bits, or fp32 sums to add to (`add`) or to set
+  int64_t out_ld;
+  int add;
+};
+
+// The sums of dX's tiles whose K blocks were shared, in the order of the blocks. A
+// block takes 16 rows of a tile.
+constexpr int kCeJoinRows = 16;
+template <typename T, bool F32>
+__global__ void __launch_bounds__(256) ce_join_parts(const CeParts q) {
+  griddep_launch_dependents();
+  griddep_wait();
+  constexpr int kBlocks = kCeBM / kCeJoinRows;
+  const int t = blockIdx.x / kBlocks, r0 = blockIdx.x % kBlocks * kCeJoinRows;
+  const int mt = t / q.n_nt, nt = t - mt * q.n_nt;
+  const float scale = F32 ? 1.f : ce_scale(q.largest, true);
+  const int per = q.bn / 4;
+  for (int j = threadIdx.x; j < kCeJoinRows * per; j += 256) {
+    const int r = r0 + j / per, c = j % per * 4;
+    const int row = mt * kCeBM + r, col = nt * q.bn + c;
+    if (row >= q.m || col >= q.n) continue;
+    const float* p = q.parts + (static_cast<int64_t>(t) * kCeBM + r) * q.bn + c;
+    const int64_t plane = static_cast<int64_t>(q.tiles) * kCeBM * q.bn;
+    float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int k = 0; k < q.splits; ++k) {
+      const float4 v = __ldcg(reinterpret_cast<const float4*>(p + k * plane));
+      z.x += v.x;
+      z.y += v.y;
+      z.z += v.z;
+      z.w += v.w;
+    }
+    if constexpr (F32) {  // rows of whole 16 bytes
+      float4* o = reinterpret_cast<float4*>(static_cast<float*>(q.out) + row * q.out_ld + col);
+      if (q.add) {
+        const float4 v = *o;
+        z = make_float4(z.x + v.x, z.y + v.y, z.z + v.z, z.w + v.w);
+      }
+      *o = z;
+    } else {
+      const float f[4] = {z.x * scale, z.y * scale, z.z * scale, z.w * scale};
+      T* o = static_cast<T*>(q.out) + row * q.out_ld + col;
+      if (col + 4 <= q.n && (reinterpret_cast<uintptr_t>(o) & 7u) == 0) {
+        *reinterpret_cast<uint2*>(o) = make_uint2(ln_pack<T>(f[0], f[1]), ln_pack<T>(f[2], f[3]));
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (col + k < q.n) o[k] = Elem<T>::from_f(f[k]);
+      }
+    }
   }
 }
 
