@@ -29,7 +29,12 @@ EXPORTS = ('avey_fwd_v1', 'avey_fwd_plan', 'avey_fwd_workspace_size', 'avey_fwd_
            'avey_last_error', 'avey_device_status', 'avey_launch_count', 'avey_abi_version',
            'avey_test_hooks_v1', 'avey_gemm_v1', 'avey_fwd_presummed_v1', 'avey_adamw_v1',
            'avey_linear_fwd_v1', 'avey_linear_bwd_v1', 'avey_linear_workspace_size',
-           'avey_loss_fwd_v1', 'avey_loss_bwd_v1', 'avey_loss_workspace_size')
+           'avey_loss_fwd_v1', 'avey_loss_bwd_v1', 'avey_loss_workspace_size',
+           'avey_route_fwd_v1', 'avey_route_bwd_v1', 'avey_arrange_v1', 'avey_arrange_workspace_size',
+           'avey_dispatch_v1', 'avey_combine_v1', 'avey_combine_bwd_v1', 'avey_embedding_fwd_v1',
+           'avey_embedding_bwd_v1', 'avey_embedding_workspace_size')
+SCORE_IDS = {'softmax': 0, 'sigmoid': 1}
+MAX_EXPERTS, MAX_CHOICES, MAX_GROUPS = 1024, 32, 32
 REDUCTION_IDS = {'none': 0, 'sum': 1, 'mean': 2}
 LINEAR_AUTO, LINEAR_TCGEN05, LINEAR_FEW = 0, 1, 2
 BWD_PREP, BWD_SCORES, BWD_EPILOGUE, BWD_DSCORES, BWD_FINAL = range(5)
@@ -217,6 +222,86 @@ class AveyLossParams(ctypes.Structure):
     ]
 
 
+class AveyRouteParams(ctypes.Structure):
+    _fields_ = [
+        ('struct_size', ctypes.c_uint32),
+        ('dtype', ctypes.c_int32),
+        ('score', ctypes.c_int32),
+        ('renormalize', ctypes.c_int32),
+        ('k', ctypes.c_int32),
+        ('groups', ctypes.c_int32),
+        ('top_groups', ctypes.c_int32),
+        ('group_best', ctypes.c_int32),
+        ('tokens', ctypes.c_int64),
+        ('experts', ctypes.c_int64),
+        ('scale', ctypes.c_double),
+        ('logits', ctypes.c_void_p),
+        ('logits_ld', ctypes.c_int64),
+        ('bias', ctypes.c_void_p),
+        ('weights', ctypes.c_void_p),
+        ('chosen', ctypes.c_void_p),
+        ('dweights', ctypes.c_void_p),
+        ('dlogits', ctypes.c_void_p),
+    ]
+
+
+class AveyArrangeParams(ctypes.Structure):
+    _fields_ = [
+        ('struct_size', ctypes.c_uint32),
+        ('index_bits', ctypes.c_int32),
+        ('count', ctypes.c_int64),
+        ('experts', ctypes.c_int64),
+        ('chosen', ctypes.c_void_p),
+        ('slots', ctypes.c_void_p),
+        ('offsets', ctypes.c_void_p),
+        ('workspace', ctypes.c_void_p),
+        ('workspace_bytes', ctypes.c_uint64),
+    ]
+
+
+class AveyRowsParams(ctypes.Structure):
+    _fields_ = [
+        ('struct_size', ctypes.c_uint32),
+        ('dtype', ctypes.c_int32),
+        ('k', ctypes.c_int32),
+        ('reserved', ctypes.c_int32),
+        ('tokens', ctypes.c_int64),
+        ('width', ctypes.c_int64),
+        ('slots', ctypes.c_void_p),
+        ('x', ctypes.c_void_p),
+        ('x_ld', ctypes.c_int64),
+        ('rows', ctypes.c_void_p),
+        ('rows_ld', ctypes.c_int64),
+        ('weights', ctypes.c_void_p),
+        ('out', ctypes.c_void_p),
+        ('drows', ctypes.c_void_p),
+        ('dweights', ctypes.c_void_p),
+    ]
+
+
+class AveyEmbeddingParams(ctypes.Structure):
+    _fields_ = [
+        ('struct_size', ctypes.c_uint32),
+        ('dtype', ctypes.c_int32),
+        ('index_bits', ctypes.c_int32),
+        ('reserved', ctypes.c_int32),
+        ('count', ctypes.c_int64),
+        ('width', ctypes.c_int64),
+        ('vocab', ctypes.c_int64),
+        ('padding', ctypes.c_int64),
+        ('scale', ctypes.c_double),
+        ('tokens', ctypes.c_void_p),
+        ('table', ctypes.c_void_p),
+        ('table_ld', ctypes.c_int64),
+        ('out', ctypes.c_void_p),
+        ('dy', ctypes.c_void_p),
+        ('dy_ld', ctypes.c_int64),
+        ('dtable', ctypes.c_void_p),
+        ('workspace', ctypes.c_void_p),
+        ('workspace_bytes', ctypes.c_uint64),
+    ]
+
+
 class AveyAdamWTensor(ctypes.Structure):
     _fields_ = [
         ('param', ctypes.c_void_p),
@@ -334,6 +419,18 @@ def lib() -> ctypes.CDLL:
         dll.avey_loss_workspace_size.argtypes = [ctypes.POINTER(AveyLossParams), ctypes.c_int,
                                                  ctypes.POINTER(ctypes.c_uint64)]
         dll.avey_loss_workspace_size.restype = ctypes.c_int
+        for names, params in (
+                (('avey_route_fwd_v1', 'avey_route_bwd_v1'), AveyRouteParams),
+                (('avey_arrange_v1',), AveyArrangeParams),
+                (('avey_dispatch_v1', 'avey_combine_v1', 'avey_combine_bwd_v1'), AveyRowsParams),
+                (('avey_embedding_fwd_v1', 'avey_embedding_bwd_v1'), AveyEmbeddingParams)):
+            for name in names:
+                getattr(dll, name).argtypes = [ctypes.POINTER(params), ctypes.c_void_p]
+                getattr(dll, name).restype = ctypes.c_int
+        for name, params in (('avey_arrange_workspace_size', AveyArrangeParams),
+                             ('avey_embedding_workspace_size', AveyEmbeddingParams)):
+            getattr(dll, name).argtypes = [ctypes.POINTER(params), ctypes.POINTER(ctypes.c_uint64)]
+            getattr(dll, name).restype = ctypes.c_int
         if dll.avey_abi_version() != ABI_VERSION:
             raise RuntimeError(f'{path}: ABI version {dll.avey_abi_version()} != {ABI_VERSION}')
         _lib = dll

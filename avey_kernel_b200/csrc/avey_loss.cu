@@ -9,10 +9,13 @@
 
 #include "avey_b200.h"
 #include "host_api.h"
+#include "launch_chain.h"
 #include "tc_loss.cuh"
 #include "linear_steps.cuh"
 
 namespace {
+
+using avey_host::Chain;
 
 int fail(int code, const char* msg) { return avey_host::set_error(code, msg); }
 
@@ -74,14 +77,10 @@ int validate(const AveyLossParams* p, bool backward) {
 
 int pairs() { return avey_host::multiprocessors() / 2; }
 
-// Columns of a tile of the logits: 256 read the fewest bytes for their products;
-// narrower ones are taken where those would leave the last wave of pairs half empty.
-int logit_cols(int64_t rows, int64_t n) {
-  const int64_t mt = (rows + avey::kCeBM - 1) / avey::kCeBM;
-  for (int bn : {256, 128})
-    if (mt * ((n + bn - 1) / bn) >= 4 * pairs()) return bn;
-  return 64;
-}
+// Columns of a tile of the logits. A K block takes nearly as long for 64 columns as for
+// 256 (33 rows, 32768 x 768: 49 us with tiles of 64, 31 of 128, 23 of 256), so narrower
+// tiles are for smaller vocabularies only.
+int logit_cols(int64_t n) { return n > 128 ? 256 : n > 64 ? 128 : 64; }
 // Column tiles of a unit of logits: more than one where there are enough for the
 // pairs to end together.
 int unit_tiles(int64_t mt, int64_t nt) {
@@ -90,9 +89,20 @@ int unit_tiles(int64_t mt, int64_t nt) {
 // Of a gradient's product over `width` columns (boxes of 64 for each CTA).
 int grad_cols(int64_t width) { return width > 128 ? 256 : 128; }
 
+// Rows up to which the statistics take the kernel for few rows (8 rows, 32768 x 768: 22
+// us against 26 by tiles, 131072 x 1024: 65 against 80, 50021 x 389: 39 against 43; 16
+// rows, which would be two passes of its products: 29, 90 and 76).
+constexpr int64_t kFewRows = 8;
+bool use_few(const AveyLossParams* p) { return p->rows <= kFewRows; }
+// Its CTAs: a warp for 16 rows of W, up to four CTAs an SM.
+int64_t few_grid(const AveyLossParams* p) {
+  const int64_t groups = (p->vocab + 15) / 16;
+  return std::min<int64_t>((groups + avey::kCfWarps - 1) / avey::kCfWarps, avey_host::multiprocessors() * 4ll);
+}
+
 // Workspace of a call, each part 256-byte aligned.
 struct Layout {
-  bool pack_x = false, pack_w = false;
+  bool few = false, pack_x = false, pack_w = false;
   uint64_t x = 0, w = 0;
   // forward
   int bn = 0, seg = 0;
@@ -139,17 +149,18 @@ Layout layout(const AveyLossParams* p, bool backward) {
     return o;
   };
   if (p->rows == 0) return l;
-  l.pack_x = !whole_rows(p->x, p->x_ld);
-  l.pack_w = !whole_rows(p->weight, p->weight_ld);
+  l.few = !backward && use_few(p);
+  l.pack_x = !l.few && !whole_rows(p->x, p->x_ld);
+  l.pack_w = !l.few && !whole_rows(p->weight, p->weight_ld);
   const uint64_t row = up(p->width, 8) * 2;
   if (l.pack_x) l.x = take(p->rows * row);
   if (l.pack_w) l.w = take(p->vocab * row);
   if (!backward) {
-    l.bn = logit_cols(p->rows, p->vocab);
+    l.bn = logit_cols(p->vocab);
     l.n_nt = (p->vocab + l.bn - 1) / l.bn;
     const int64_t mt = (p->rows + avey::kCeBM - 1) / avey::kCeBM;
     l.seg = unit_tiles(mt, l.n_nt);
-    l.segments = (l.n_nt + l.seg - 1) / l.seg;
+    l.segments = l.few ? few_grid(p) : (l.n_nt + l.seg - 1) / l.seg;
     l.partial = take(l.segments * p->rows * 8);
     l.picked = take(p->rows * 4);
     if (p->reduction != AVEY_LOSS_NONE) l.each = take(p->rows * 4);
@@ -186,48 +197,6 @@ int check_workspace(const AveyLossParams* p, const Layout& l) {
   return AVEY_OK;
 }
 
-// Launches of a call: all but the first may be set up beside the end of the one
-// before (each waits for it ahead of its first read).
-struct Chain {
-  cudaStream_t stream;
-  bool after = false;
-
-  template <typename... Params, typename... Args>
-  int launch(const char* what, void (*kernel)(Params...), int64_t grid, int block, int smem, int cluster,
-             Args... args) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(grid));
-    cfg.blockDim = dim3(static_cast<unsigned>(block));
-    cfg.dynamicSmemBytes = static_cast<size_t>(smem);
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[2];
-    int n = 0;
-    if (cluster > 1) {
-      attr[n].id = cudaLaunchAttributeClusterDimension;
-      attr[n].val.clusterDim.x = static_cast<unsigned>(cluster);
-      attr[n].val.clusterDim.y = 1;
-      attr[n].val.clusterDim.z = 1;
-      ++n;
-    }
-    if (after) {
-      attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-      attr[n].val.programmaticStreamSerializationAllowed = 1;
-      ++n;
-    }
-    cfg.attrs = attr;
-    cfg.numAttrs = static_cast<unsigned>(n);
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
-    if (e != cudaSuccess) {
-      char buf[256];
-      snprintf(buf, sizeof(buf), "%s launch: %s", what, cudaGetErrorString(e));
-      return fail(AVEY_ERR_LAUNCH, buf);
-    }
-    avey_host::count_launches(1);
-    after = true;
-    return AVEY_OK;
-  }
-};
-
 struct Rows {
   const void* p;
   int64_t ld;
@@ -257,7 +226,7 @@ int pack_inputs(const AveyLossParams* p, const Layout& l, Rows* x, Rows* w, Chai
   }
   const int64_t pieces = (a.rows + b.rows) * (a.ld / 8);
   const int64_t grid = std::min<int64_t>((pieces + 255) / 256, avey_host::multiprocessors() * 16ll);
-  return chain.launch("row copy", avey::ln_pack_rows, grid, 256, 0, 1, a, b);
+  return chain.launch("row copy", avey::ln_pack_rows, dim3(static_cast<unsigned>(grid)), 256, 0, 1, a, b);
 }
 
 template <auto K>
@@ -266,7 +235,7 @@ int launch_product(const avey::CeMaps& m, avey::CeGeom& q, Chain& chain) {
   if (attr != cudaSuccess) return fail(AVEY_ERR_CUDA, cudaGetErrorString(attr));
   q.units = 0;
   for (const avey::CeJob& j : q.job) q.units += j.units;
-  return chain.launch("cross entropy product", K, 2ll * std::min(q.units, pairs()), avey::kCeThreads,
+  return chain.launch("cross entropy product", K, dim3(2 * static_cast<unsigned>(std::min<int64_t>(q.units, pairs()))), avey::kCeThreads,
                       avey::kCeSmem, 2, m, q);
 }
 
@@ -317,14 +286,36 @@ avey::CeRows rows_of(const AveyLossParams* p) {
 }
 
 template <typename T>
-int forward(const AveyLossParams* p, cudaStream_t stream) {
-  const Layout l = layout(p, false);
-  int rc = check_workspace(p, l);
-  if (rc != AVEY_OK) return rc;
+int stats_few(const AveyLossParams* p, const Layout& l, Chain& chain) {
   char* ws = static_cast<char*>(p->workspace);
-  Chain chain{stream};
+  auto vec = [](const void* base, int64_t ld) {
+    const uint64_t all = reinterpret_cast<uintptr_t>(base) | static_cast<uint64_t>(ld) * 2;
+    return all % 32 == 0 ? 2 : all % 16 == 0 ? 1 : 0;
+  };
+  avey::CeFew q{};
+  q.rows = static_cast<int>(p->rows);
+  q.vocab = static_cast<int>(p->vocab);
+  q.width = static_cast<int>(p->width);
+  q.x = static_cast<const uint16_t*>(p->x);
+  q.w = static_cast<const uint16_t*>(p->weight);
+  q.x_ld = p->x_ld;
+  q.w_ld = p->weight_ld;
+  q.x_vec = vec(p->x, p->rows > 1 ? p->x_ld : 0);
+  q.w_vec = vec(p->weight, p->weight_ld);
+  q.targets = p->targets;
+  q.target_stride = p->target_stride;
+  q.target64 = p->target_bits == 64;
+  q.ignore = p->ignore_index;
+  q.partial = reinterpret_cast<float2*>(ws + l.partial);
+  q.picked = reinterpret_cast<float*>(ws + l.picked);
+  return chain.launch("cross entropy of few rows", avey::ce_few<T>, dim3(static_cast<unsigned>(l.segments)), 32 * avey::kCfWarps, 0, 1, q);
+}
+
+template <typename T>
+int stats_tiles(const AveyLossParams* p, const Layout& l, Chain& chain) {
+  char* ws = static_cast<char*>(p->workspace);
   Rows x, w;
-  rc = pack_inputs(p, l, &x, &w, chain);
+  int rc = pack_inputs(p, l, &x, &w, chain);
   if (rc != AVEY_OK) return rc;
   avey::CeGeom q = geom(p);
   q.job[0] = job(avey::kCeStats, p->rows, p->vocab, p->width, l.bn);
@@ -336,21 +327,30 @@ int forward(const AveyLossParams* p, cudaStream_t stream) {
   avey::CeMaps m{};
   rc = avey_host::encode_rows16(p->dtype, x.p, p->width, p->rows, 1, x.ld * 2, 0, 128, &m.x);
   if (rc == AVEY_OK) rc = avey_host::encode_rows16(p->dtype, w.p, p->width, p->vocab, 1, w.ld * 2, 0, l.bn / 2, &m.w);
+  return rc == AVEY_OK ? launch_product<avey::ce_product<T, true>>(m, q, chain) : rc;
+}
+
+template <typename T>
+int forward(const AveyLossParams* p, cudaStream_t stream) {
+  const Layout l = layout(p, false);
+  int rc = check_workspace(p, l);
   if (rc != AVEY_OK) return rc;
-  rc = launch_product<avey::ce_product<T, true>>(m, q, chain);
+  char* ws = static_cast<char*>(p->workspace);
+  Chain chain{stream};
+  rc = l.few ? stats_few<T>(p, l, chain) : stats_tiles<T>(p, l, chain);
   if (rc != AVEY_OK) return rc;
   avey::CeRows r = rows_of(p);
   r.segments = static_cast<int>(l.segments);
-  r.partial = q.partial;
-  r.picked = q.picked;
+  r.partial = reinterpret_cast<const float2*>(ws + l.partial);
+  r.picked = reinterpret_cast<const float*>(ws + l.picked);
   const bool none = p->reduction == AVEY_LOSS_NONE;
   r.each = none ? p->loss : reinterpret_cast<float*>(ws + l.each);
   r.lse = p->saved;
   r.per = 32;
   while (r.per > 1 && r.per / 2 >= p->rows) r.per /= 2;
-  rc = chain.launch("cross entropy rows", avey::ce_rows, (p->rows + r.per - 1) / r.per, 256, 0, 1, r);
+  rc = chain.launch("cross entropy rows", avey::ce_rows, dim3(static_cast<unsigned>((p->rows + r.per - 1) / r.per)), 256, 0, 1, r);
   if (rc != AVEY_OK || none) return rc;
-  return chain.launch("cross entropy total", avey::ce_total, 1, 1024, 0, 1, r, p->reduction == AVEY_LOSS_MEAN ? 1 : 0,
+  return chain.launch("cross entropy total", avey::ce_total, dim3(1), 1024, 0, 1, r, p->reduction == AVEY_LOSS_MEAN ? 1 : 0,
                       p->loss, p->saved ? p->saved + p->rows : nullptr);
 }
 
@@ -390,7 +390,7 @@ int backward(const AveyLossParams* p, cudaStream_t stream) {
     k.copy_ld = up(p->width, 8);
     k.dirty = reinterpret_cast<uint8_t*>(ws + l.dirty);
   }
-  rc = chain.launch("cross entropy coefficients", avey::ce_coef<T>, (p->rows + 63) / 64, 256, 0, 1, k);
+  rc = chain.launch("cross entropy coefficients", avey::ce_coef<T>, dim3(static_cast<unsigned>((p->rows + 63) / 64)), 256, 0, 1, k);
   if (rc != AVEY_OK) return rc;
   const int64_t sums_ld = up(p->width, 4);
   float* sums = reinterpret_cast<float*>(ws + l.sums);
@@ -450,7 +450,7 @@ int backward(const AveyLossParams* p, cudaStream_t stream) {
     }
     if (i < l.pieces) {
       const int64_t v0 = i * l.piece, n = std::min(l.piece, p->vocab - v0), ld = up(n, 8);
-      const int cols = logit_cols(p->rows, n);
+      const int cols = logit_cols(n);
       q.job[jobs] = job(avey::kCeGrad, p->rows, n, p->width, cols);
       q.job[jobs].seg = unit_tiles(q.job[jobs].n_mt, q.job[jobs].n_nt);
       q.job[jobs].units = (q.job[jobs].n_nt + q.job[jobs].seg - 1) / q.job[jobs].seg * q.job[jobs].n_mt;
@@ -480,7 +480,7 @@ int backward(const AveyLossParams* p, cudaStream_t stream) {
       j.out = planes ? static_cast<void*>(sums) : p->dx;
       j.out_ld = planes ? sums_ld : p->dx_ld;
       j.add = i > 1;
-      const int64_t grid = static_cast<int64_t>(j.tiles) * (avey::kCeBM / avey::kCeJoinRows);
+      const dim3 grid(static_cast<unsigned>(j.tiles * (avey::kCeBM / avey::kCeJoinRows)));
       rc = planes ? chain.launch("cross entropy parts", avey::ce_join_parts<T, true>, grid, 256, 0, 1, j)
                   : chain.launch("cross entropy parts", avey::ce_join_parts<T, false>, grid, 256, 0, 1, j);
       if (rc != AVEY_OK) return rc;
@@ -488,7 +488,7 @@ int backward(const AveyLossParams* p, cudaStream_t stream) {
   }
   if (p->dx && planes) {
     const int64_t quads = p->rows * (sums_ld / 4);
-    const int64_t grid = std::min<int64_t>((quads + 255) / 256, avey_host::multiprocessors() * 8ll);
+    const dim3 grid(static_cast<unsigned>(std::min<int64_t>((quads + 255) / 256, avey_host::multiprocessors() * 8ll)));
     rc = chain.launch("dx rounding", avey::ce_finish<T>, grid, 256, 0, 1, sums, sums_ld, p->rows, p->width, largest,
                       static_cast<T*>(p->dx), p->dx_ld);
   }

@@ -1,0 +1,455 @@
+// C ABI of the operators that route and move tokens (declared in include/avey_b200.h):
+// argument checks, workspace layout and the launches of route_kernels.cuh,
+// sort_kernels.cuh and rows_kernels.cuh.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+
+#include "avey_b200.h"
+#include "host_api.h"
+#include "launch_chain.h"
+#include "rows_kernels.cuh"
+#include "route_kernels.cuh"
+#include "sort_kernels.cuh"
+
+namespace {
+
+using avey_host::Chain;
+
+int fail(int code, const char* msg) { return avey_host::set_error(code, msg); }
+int done(int rc) { return rc == AVEY_OK ? avey_host::clear_error() : rc; }
+
+uint64_t up256(uint64_t x) { return (x + 255u) & ~uint64_t(255); }
+uintptr_t address(const void* p) { return reinterpret_cast<uintptr_t>(p); }
+int size_of(int dtype) { return dtype == AVEY_F32 ? 4 : 2; }
+bool known(int dtype) { return dtype == AVEY_F32 || dtype == AVEY_F16 || dtype == AVEY_BF16; }
+
+int check_workspace(const void* ws, uint64_t have, uint64_t need) {
+  if (need == 0) return AVEY_OK;
+  if (!ws || have < need) return fail(AVEY_ERR_ARGUMENT, "workspace is smaller than the call's workspace size");
+  if ((address(ws) & 255u) != 0) return fail(AVEY_ERR_ARGUMENT, "workspace must be 256-byte aligned");
+  return AVEY_OK;
+}
+
+unsigned blocks_for(int64_t items, int per) {
+  return static_cast<unsigned>(
+      std::max<int64_t>(1, std::min<int64_t>((items + per - 1) / per, avey_host::multiprocessors() * 32ll)));
+}
+
+// ------------------------------------------------------------------ routing
+
+int validate(const AveyRouteParams* p, bool backward) {
+  if (!p) return fail(AVEY_ERR_ARGUMENT, "params is NULL");
+  if (p->struct_size != sizeof(AveyRouteParams))
+    return fail(AVEY_ERR_ARGUMENT, "struct_size does not match sizeof(AveyRouteParams)");
+  if (!known(p->dtype)) return fail(AVEY_ERR_ARGUMENT, "logits are f32, f16 or bf16");
+  if (p->score != AVEY_SCORE_SOFTMAX && p->score != AVEY_SCORE_SIGMOID) return fail(AVEY_ERR_ARGUMENT, "unknown score");
+  if (p->tokens < 0 || p->tokens > (1 << 30) || p->experts < 1 || p->experts > avey::kRtMaxExperts)
+    return fail(AVEY_ERR_ARGUMENT, "tokens must be in [0, 2^30] and experts in [1, 1024]");
+  if (p->groups < 1 || p->groups > avey::kRtMaxGroups || p->experts % p->groups != 0 || p->top_groups < 1 ||
+      p->top_groups > p->groups || (p->group_best != 1 && p->group_best != 2))
+    return fail(AVEY_ERR_ARGUMENT,
+                "groups must divide the experts and be in [1, 32], top_groups in [1, groups], group_best 1 or 2");
+  if (p->k < 1 || p->k > avey::kRtMaxK || p->k > p->experts / p->groups * p->top_groups)
+    return fail(AVEY_ERR_ARGUMENT, "k must be in [1, 32] and no more than the experts of top_groups groups");
+  if (!(p->scale > -1e30 && p->scale < 1e30)) return fail(AVEY_ERR_ARGUMENT, "scale must be finite");
+  const uintptr_t element = size_of(p->dtype) - 1;
+  if (((address(p->logits) | address(p->dlogits)) & element) != 0 ||
+      ((address(p->bias) | address(p->weights) | address(p->chosen) | address(p->dweights)) & 3u) != 0)
+    return fail(AVEY_ERR_ARGUMENT, "arrays must be aligned to their elements");
+  if (p->tokens == 0) return AVEY_OK;
+  if (!p->logits || !p->weights || !p->chosen) return fail(AVEY_ERR_ARGUMENT, "logits, weights and chosen are required");
+  if (p->logits_ld < p->experts) return fail(AVEY_ERR_ARGUMENT, "strides must cover the rows");
+  if (backward && (!p->dweights || !p->dlogits))
+    return fail(AVEY_ERR_ARGUMENT, "dweights and dlogits are required");
+  return AVEY_OK;
+}
+
+template <typename T, int R>
+int launch_route(const avey::RtArgs& q, bool backward, Chain& chain) {
+  const dim3 grid(static_cast<unsigned>((q.tokens + avey::kRtWarps - 1) / avey::kRtWarps));
+  if (!backward) return chain.launch("route", avey::route_forward<T, R>, grid, 32 * avey::kRtWarps, 0, 1, q);
+  return chain.launch("route gradient", avey::route_backward<T, R>, grid, 32 * avey::kRtWarps,
+                      avey::kRtWarps * 32 * R * 4, 1, q);
+}
+
+template <typename T>
+int route(const AveyRouteParams* p, bool backward, cudaStream_t stream) {
+  avey::RtArgs q{};
+  q.tokens = p->tokens;
+  q.experts = static_cast<int>(p->experts);
+  q.k = p->k;
+  q.groups = p->groups;
+  q.top_groups = p->top_groups;
+  q.group_best = p->group_best;
+  q.softmax = p->score == AVEY_SCORE_SOFTMAX;
+  q.renormalize = p->renormalize != 0;
+  q.scale = static_cast<float>(p->scale);
+  q.logits = p->logits;
+  q.ld = p->logits_ld;
+  q.vec = ((address(p->logits) | static_cast<uint64_t>(p->logits_ld) * sizeof(T)) & 15u) == 0;
+  q.bias = p->bias;
+  q.weights = p->weights;
+  q.chosen = p->chosen;
+  q.dweights = p->dweights;
+  q.dlogits = p->dlogits;
+  q.dvec = ((address(p->dlogits) | static_cast<uint64_t>(p->experts) * sizeof(T)) & 15u) == 0;
+  Chain chain{stream};
+  const int per = (q.experts + 31) / 32;
+  if (per <= 1) return launch_route<T, 1>(q, backward, chain);
+  if (per <= 2) return launch_route<T, 2>(q, backward, chain);
+  if (per <= 4) return launch_route<T, 4>(q, backward, chain);
+  if (per <= 8) return launch_route<T, 8>(q, backward, chain);
+  if (per <= 16) return launch_route<T, 16>(q, backward, chain);
+  return launch_route<T, 32>(q, backward, chain);
+}
+
+int run_route(const AveyRouteParams* p, bool backward, void* stream) {
+  int rc = validate(p, backward);
+  if (rc != AVEY_OK) return rc;
+  rc = avey_host::device_ok();
+  if (rc != AVEY_OK || p->tokens == 0) return done(rc);
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return done(p->dtype == AVEY_F32   ? route<float>(p, backward, s)
+              : p->dtype == AVEY_F16 ? route<__half>(p, backward, s)
+                                     : route<__nv_bfloat16>(p, backward, s));
+}
+
+// ------------------------------------------------------------------ sorting
+
+// Blocks of a pass over n entries, and the entries of each (whole warps' steps).
+int64_t sort_run(int64_t n) {
+  if (n <= avey::kStOneBlock) return n;
+  const int64_t share = (n + avey_host::multiprocessors() - 1) / avey_host::multiprocessors();
+  return std::max<int64_t>(avey::kStRun, (share + 255) / 256 * 256);
+}
+int64_t sort_blocks(int64_t n) {
+  const int64_t run = sort_run(n);
+  return n ? (n + run - 1) / run : 1;
+}
+uint64_t count_bytes(int64_t n, int buckets) {
+  const int64_t b = sort_blocks(n);
+  return b > 1 ? up256(static_cast<uint64_t>(b) * buckets * 4) : 0;
+}
+
+int launch_pass(avey::StArgs& q, Chain& chain) {
+  q.run = std::max<int64_t>(1, sort_run(q.n));
+  q.blocks = static_cast<int>(sort_blocks(q.n));
+  const int smem = avey::kStWarps * q.buckets * 4;
+  if (q.blocks > 1) {
+    const int rc = chain.launch("sort counts", avey::st_count, dim3(q.blocks), avey::kStThreads, smem, 1, q);
+    if (rc != AVEY_OK) return rc;
+  }
+  return chain.launch("sort", avey::st_place, dim3(q.blocks), avey::kStThreads, smem + q.buckets * 4, 1, q);
+}
+
+int validate(const AveyArrangeParams* p) {
+  if (!p) return fail(AVEY_ERR_ARGUMENT, "params is NULL");
+  if (p->struct_size != sizeof(AveyArrangeParams))
+    return fail(AVEY_ERR_ARGUMENT, "struct_size does not match sizeof(AveyArrangeParams)");
+  if (p->index_bits != 32 && p->index_bits != 64) return fail(AVEY_ERR_ARGUMENT, "expert numbers have 32 or 64 bits");
+  if (p->count < 0 || p->count > (1ll << 30) || p->experts < 1 || p->experts > avey::kRtMaxExperts)
+    return fail(AVEY_ERR_ARGUMENT, "count must be in [0, 2^30] and experts in [1, 1024]");
+  if ((address(p->chosen) & (p->index_bits / 8 - 1)) != 0 || ((address(p->slots) | address(p->offsets)) & 3u) != 0)
+    return fail(AVEY_ERR_ARGUMENT, "arrays must be aligned to their elements");
+  if (!p->offsets || (p->count > 0 && (!p->chosen || !p->slots)))
+    return fail(AVEY_ERR_ARGUMENT, "chosen, slots and offsets are required");
+  return AVEY_OK;
+}
+
+// ------------------------------------------------------------------ rows
+
+int validate(const AveyRowsParams* p, int what) {
+  if (!p) return fail(AVEY_ERR_ARGUMENT, "params is NULL");
+  if (p->struct_size != sizeof(AveyRowsParams))
+    return fail(AVEY_ERR_ARGUMENT, "struct_size does not match sizeof(AveyRowsParams)");
+  if (!known(p->dtype)) return fail(AVEY_ERR_ARGUMENT, "rows are f32, f16 or bf16");
+  if (p->tokens < 0 || p->k < 1 || p->k > avey::kRwMaxK || p->tokens > (1ll << 30) / p->k || p->width < 1 ||
+      p->width > (1 << 22))
+    return fail(AVEY_ERR_ARGUMENT, "k must be in [1, 32], tokens x k up to 2^30 and width in [1, 2^22]");
+  const uintptr_t element = size_of(p->dtype) - 1;
+  if (((address(p->x) | address(p->rows) | address(p->out) | address(p->drows)) & element) != 0 ||
+      ((address(p->slots) | address(p->weights) | address(p->dweights)) & 3u) != 0)
+    return fail(AVEY_ERR_ARGUMENT, "arrays must be aligned to their elements");
+  if (p->tokens == 0) return AVEY_OK;
+  if (!p->slots) return fail(AVEY_ERR_ARGUMENT, "slots is required");
+  if ((p->x && p->x_ld < p->width) || (p->rows && p->rows_ld < p->width))
+    return fail(AVEY_ERR_ARGUMENT, "strides must cover the rows");
+  if (what == 0 && (!p->x || !p->rows)) return fail(AVEY_ERR_ARGUMENT, "x and rows are required");
+  if (what == 1 && (!p->rows || !p->out)) return fail(AVEY_ERR_ARGUMENT, "rows and out are required");
+  if (what == 2 && (!p->x || !p->weights || (p->dweights && !p->rows)))
+    return fail(AVEY_ERR_ARGUMENT, "x (the gradient of out), weights and, for dweights, rows are required");
+  return AVEY_OK;
+}
+
+// Bytes of an access that all rows are whole multiples of.
+int access_bytes(int size, int64_t width, std::initializer_list<const void*> bases,
+                 std::initializer_list<int64_t> strides) {
+  uint64_t all = static_cast<uint64_t>(width) * size;
+  for (const void* b : bases) all |= address(b);
+  for (int64_t s : strides) all |= static_cast<uint64_t>(s) * size;
+  return (all & 15u) == 0 ? 16 : (all & 3u) == 0 ? 4 : size;
+}
+
+template <typename T, int N>
+int launch_rows(const avey::RwArgs& q, int what, Chain& chain) {
+  const unsigned grid = blocks_for(q.tokens * (q.width / N), 256);
+  if (what == 0) return chain.launch("dispatch", avey::rw_dispatch<T, N>, dim3(grid), 256, 0, 1, q);
+  if (what == 1) return chain.launch("combine", avey::rw_combine<T, N>, dim3(grid), 256, 0, 1, q);
+  const dim3 warps(static_cast<unsigned>((q.tokens + avey::kRwWarps - 1) / avey::kRwWarps));
+  return chain.launch("combine gradient", avey::rw_combine_backward<T, N>, warps, 32 * avey::kRwWarps, 0, 1, q);
+}
+
+// what: 0 dispatch, 1 combine, 2 combine's backward.
+int run_rows(const AveyRowsParams* p, int what, void* stream) {
+  int rc = validate(p, what);
+  if (rc != AVEY_OK) return rc;
+  rc = avey_host::device_ok();
+  if (rc != AVEY_OK || p->tokens == 0) return done(rc);
+  avey::RwArgs q{};
+  q.tokens = p->tokens;
+  q.k = p->k;
+  q.width = static_cast<int>(p->width);
+  q.slots = p->slots;
+  q.x = p->x;
+  q.x_ld = p->x_ld;
+  q.rows = p->rows;
+  q.rows_ld = p->rows_ld;
+  q.weights = p->weights;
+  q.out = what == 2 ? p->drows : p->out;
+  q.dweights = p->dweights;
+  Chain chain{static_cast<cudaStream_t>(stream)};
+  const int size = size_of(p->dtype);
+  const int bytes = access_bytes(size, p->width, {p->x, p->rows, q.out},
+                                 {p->x ? p->x_ld : 0, p->rows ? p->rows_ld : 0});
+  if (p->dtype == AVEY_F32)
+    rc = bytes == 16 ? launch_rows<float, 4>(q, what, chain) : launch_rows<float, 1>(q, what, chain);
+  else if (p->dtype == AVEY_F16)
+    rc = bytes == 16  ? launch_rows<__half, 8>(q, what, chain)
+         : bytes == 4 ? launch_rows<__half, 2>(q, what, chain)
+                      : launch_rows<__half, 1>(q, what, chain);
+  else
+    rc = bytes == 16  ? launch_rows<__nv_bfloat16, 8>(q, what, chain)
+         : bytes == 4 ? launch_rows<__nv_bfloat16, 2>(q, what, chain)
+                      : launch_rows<__nv_bfloat16, 1>(q, what, chain);
+  return done(rc);
+}
+
+// ------------------------------------------------------------------ embedding
+
+int validate(const AveyEmbeddingParams* p, bool backward) {
+  if (!p) return fail(AVEY_ERR_ARGUMENT, "params is NULL");
+  if (p->struct_size != sizeof(AveyEmbeddingParams))
+    return fail(AVEY_ERR_ARGUMENT, "struct_size does not match sizeof(AveyEmbeddingParams)");
+  if (!known(p->dtype)) return fail(AVEY_ERR_ARGUMENT, "the table is f32, f16 or bf16");
+  if (p->index_bits != 32 && p->index_bits != 64) return fail(AVEY_ERR_ARGUMENT, "tokens have 32 or 64 bits");
+  if (p->count < 0 || p->count > (1 << 30) || p->width < 1 || p->width > (1 << 22) || p->vocab < 1 ||
+      p->vocab > (1 << 30))
+    return fail(AVEY_ERR_ARGUMENT, "count must be in [0, 2^30], width in [1, 2^22], vocab in [1, 2^30]");
+  if (!(p->scale > -1e30 && p->scale < 1e30)) return fail(AVEY_ERR_ARGUMENT, "scale must be finite");
+  const uintptr_t element = size_of(p->dtype) - 1;
+  if (((address(p->table) | address(p->out) | address(p->dy) | address(p->dtable)) & element) != 0 ||
+      (address(p->tokens) & (p->index_bits / 8 - 1)) != 0)
+    return fail(AVEY_ERR_ARGUMENT, "arrays must be aligned to their elements");
+  if (p->count > 0 && !p->tokens) return fail(AVEY_ERR_ARGUMENT, "tokens is required");
+  if (!backward && p->count > 0 && (!p->table || !p->out || p->table_ld < p->width))
+    return fail(AVEY_ERR_ARGUMENT, "table and out are required and strides must cover the rows");
+  if (backward && (!p->dtable || (p->count > 0 && (!p->dy || p->dy_ld < p->width))))
+    return fail(AVEY_ERR_ARGUMENT, "dy and dtable are required and strides must cover the rows");
+  return AVEY_OK;
+}
+
+avey::EmArgs embedding_args(const AveyEmbeddingParams* p) {
+  avey::EmArgs q{};
+  q.n = p->count;
+  q.width = static_cast<int>(p->width);
+  q.vocab = p->vocab;
+  q.tokens = p->tokens;
+  q.tokens64 = p->index_bits == 64;
+  q.table = p->table;
+  q.table_ld = p->table_ld;
+  q.scale = static_cast<float>(p->scale);
+  q.out = p->out;
+  q.dy = p->dy;
+  q.dy_ld = p->dy_ld;
+  q.dtable = p->dtable;
+  return q;
+}
+
+// Workspace of the backward call: [keys, ids] twice, counts, tokens seen, parts.
+struct EmLayout {
+  int passes = 0;
+  uint64_t keys[2] = {}, ids[2] = {}, counts = 0, seen = 0, parts = 0, total = 0;
+};
+EmLayout embedding_layout(const AveyEmbeddingParams* p) {
+  EmLayout l;
+  if (p->count == 0) return l;
+  uint64_t at = 0;
+  auto take = [&](uint64_t bytes) {
+    const uint64_t o = at;
+    at += up256(bytes);
+    return o;
+  };
+  int bits = 1;
+  while (bits < 31 && (1ll << bits) <= p->vocab) ++bits;  // keys up to vocab itself
+  l.passes = (bits + 9) / 10;
+  for (int i = 0; i < 2; ++i) {
+    l.keys[i] = take(p->count * 4);
+    l.ids[i] = take(p->count * 4);
+  }
+  l.counts = take(count_bytes(p->count, 1024));
+  l.seen = take(p->vocab + 1);
+  l.parts = take(static_cast<uint64_t>((p->count + avey::kEmChunk - 1) / avey::kEmChunk) * 2 * p->width * 4);
+  l.total = at;
+  return l;
+}
+
+template <typename T, int N>
+int launch_sums(const avey::EmArgs& q, Chain& chain) {
+  const int threads = static_cast<int>(std::min<int64_t>(256, (q.width / N + 31) / 32 * 32));
+  const int64_t zeros = (q.vocab + avey::kEmZeroRows - 1) / avey::kEmZeroRows;
+  int rc = chain.launch("embedding sums", avey::em_sum<T, N>, dim3(static_cast<unsigned>(q.chunks + zeros)), threads, 0,
+                        1, q);
+  if (rc != AVEY_OK || q.chunks < 2) return rc;
+  const unsigned slabs = static_cast<unsigned>(std::min<int64_t>(4, (q.width + avey::kEmCols - 1) / avey::kEmCols));
+  return chain.launch("embedding parts", avey::em_finish<T>, dim3(static_cast<unsigned>(q.chunks), slabs),
+                      avey::kEmGroups * avey::kEmCols, 0, 1, q);
+}
+
+int embedding_backward(const AveyEmbeddingParams* p, cudaStream_t stream) {
+  const int size = size_of(p->dtype);
+  if (p->count == 0) {
+    const cudaError_t e = cudaMemsetAsync(p->dtable, 0, static_cast<size_t>(p->vocab) * p->width * size, stream);
+    return e == cudaSuccess ? AVEY_OK : fail(AVEY_ERR_CUDA, cudaGetErrorString(e));
+  }
+  const EmLayout l = embedding_layout(p);
+  int rc = check_workspace(p->workspace, p->workspace_bytes, l.total);
+  if (rc != AVEY_OK) return rc;
+  char* ws = static_cast<char*>(p->workspace);
+  uint8_t* seen = reinterpret_cast<uint8_t*>(ws + l.seen);
+  const cudaError_t e = cudaMemsetAsync(seen, 0, p->vocab + 1, stream);
+  if (e != cudaSuccess) return fail(AVEY_ERR_CUDA, cudaGetErrorString(e));
+  Chain chain{stream};
+  for (int pass = 0; pass < l.passes; ++pass) {
+    avey::StArgs q{};
+    q.n = p->count;
+    q.buckets = 1024;
+    q.shift = 10 * pass;
+    q.mask = 1023;
+    q.limit = p->vocab;
+    q.skip = p->padding >= 0 ? p->padding : -1;
+    if (pass == 0) {
+      q.raw = p->tokens;
+      q.raw64 = p->index_bits == 64;
+      q.seen = seen;
+    } else {
+      q.keys = reinterpret_cast<uint32_t*>(ws + l.keys[(pass - 1) & 1]);
+      q.ids = reinterpret_cast<uint32_t*>(ws + l.ids[(pass - 1) & 1]);
+    }
+    q.counts = reinterpret_cast<uint32_t*>(ws + l.counts);
+    q.keys_out = reinterpret_cast<uint32_t*>(ws + l.keys[pass & 1]);
+    q.ids_out = reinterpret_cast<uint32_t*>(ws + l.ids[pass & 1]);
+    rc = launch_pass(q, chain);
+    if (rc != AVEY_OK) return rc;
+  }
+  avey::EmArgs q = embedding_args(p);
+  q.keys = reinterpret_cast<uint32_t*>(ws + l.keys[(l.passes - 1) & 1]);
+  q.ids = reinterpret_cast<uint32_t*>(ws + l.ids[(l.passes - 1) & 1]);
+  q.seen = seen;
+  q.parts = reinterpret_cast<float*>(ws + l.parts);
+  q.chunks = (p->count + avey::kEmChunk - 1) / avey::kEmChunk;
+  const int bytes = access_bytes(size, p->width, {p->dy, p->dtable}, {p->dy_ld});
+  if (p->dtype == AVEY_F32) return bytes == 16 ? launch_sums<float, 4>(q, chain) : launch_sums<float, 1>(q, chain);
+  if (p->dtype == AVEY_F16)
+    return bytes == 16  ? launch_sums<__half, 8>(q, chain)
+           : bytes == 4 ? launch_sums<__half, 2>(q, chain)
+                        : launch_sums<__half, 1>(q, chain);
+  return bytes == 16  ? launch_sums<__nv_bfloat16, 8>(q, chain)
+         : bytes == 4 ? launch_sums<__nv_bfloat16, 2>(q, chain)
+                      : launch_sums<__nv_bfloat16, 1>(q, chain);
+}
+
+template <typename T, int N>
+int launch_lookup(const avey::EmArgs& q, Chain& chain) {
+  return chain.launch("embedding", avey::em_forward<T, N>, dim3(blocks_for(q.n * (q.width / N), 256)), 256, 0, 1, q);
+}
+
+int embedding_forward(const AveyEmbeddingParams* p, cudaStream_t stream) {
+  if (p->count == 0) return AVEY_OK;
+  const avey::EmArgs q = embedding_args(p);
+  Chain chain{stream};
+  const int bytes = access_bytes(size_of(p->dtype), p->width, {p->table, p->out}, {p->table_ld});
+  if (p->dtype == AVEY_F32) return bytes == 16 ? launch_lookup<float, 4>(q, chain) : launch_lookup<float, 1>(q, chain);
+  if (p->dtype == AVEY_F16)
+    return bytes == 16  ? launch_lookup<__half, 8>(q, chain)
+           : bytes == 4 ? launch_lookup<__half, 2>(q, chain)
+                        : launch_lookup<__half, 1>(q, chain);
+  return bytes == 16  ? launch_lookup<__nv_bfloat16, 8>(q, chain)
+         : bytes == 4 ? launch_lookup<__nv_bfloat16, 2>(q, chain)
+                      : launch_lookup<__nv_bfloat16, 1>(q, chain);
+}
+
+}  // namespace
+
+extern "C" {
+
+int avey_route_fwd_v1(const AveyRouteParams* p, void* stream) { return run_route(p, false, stream); }
+int avey_route_bwd_v1(const AveyRouteParams* p, void* stream) { return run_route(p, true, stream); }
+
+int avey_arrange_workspace_size(const AveyArrangeParams* p, uint64_t* bytes) {
+  const int rc = validate(p);
+  if (rc != AVEY_OK) return rc;
+  if (!bytes) return fail(AVEY_ERR_ARGUMENT, "bytes is NULL");
+  *bytes = count_bytes(p->count, static_cast<int>(p->experts) + 1);
+  return avey_host::clear_error();
+}
+
+int avey_arrange_v1(const AveyArrangeParams* p, void* stream) {
+  int rc = validate(p);
+  if (rc != AVEY_OK) return rc;
+  rc = avey_host::device_ok();
+  if (rc != AVEY_OK) return rc;
+  avey::StArgs q{};
+  q.n = p->count;
+  q.buckets = static_cast<int>(p->experts) + 1;  // the last: of no expert
+  q.mask = -1;
+  q.raw = p->chosen;
+  q.raw64 = p->index_bits == 64;
+  q.limit = p->experts;
+  q.skip = -1;
+  q.slots = p->slots;
+  q.offsets = p->offsets;
+  rc = check_workspace(p->workspace, p->workspace_bytes, count_bytes(q.n, q.buckets));
+  if (rc != AVEY_OK) return rc;
+  q.counts = static_cast<uint32_t*>(p->workspace);
+  Chain chain{static_cast<cudaStream_t>(stream)};
+  return done(launch_pass(q, chain));
+}
+
+int avey_dispatch_v1(const AveyRowsParams* p, void* stream) { return run_rows(p, 0, stream); }
+int avey_combine_v1(const AveyRowsParams* p, void* stream) { return run_rows(p, 1, stream); }
+int avey_combine_bwd_v1(const AveyRowsParams* p, void* stream) { return run_rows(p, 2, stream); }
+
+int avey_embedding_workspace_size(const AveyEmbeddingParams* p, uint64_t* bytes) {
+  const int rc = validate(p, true);
+  if (rc != AVEY_OK) return rc;
+  if (!bytes) return fail(AVEY_ERR_ARGUMENT, "bytes is NULL");
+  *bytes = embedding_layout(p).total;
+  return avey_host::clear_error();
+}
+
+int avey_embedding_fwd_v1(const AveyEmbeddingParams* p, void* stream) {
+  int rc = validate(p, false);
+  if (rc != AVEY_OK) return rc;
+  rc = avey_host::device_ok();
+  return done(rc == AVEY_OK ? embedding_forward(p, static_cast<cudaStream_t>(stream)) : rc);
+}
+
+int avey_embedding_bwd_v1(const AveyEmbeddingParams* p, void* stream) {
+  int rc = validate(p, true);
+  if (rc != AVEY_OK) return rc;
+  rc = avey_host::device_ok();
+  return done(rc == AVEY_OK ? embedding_backward(p, static_cast<cudaStream_t>(stream)) : rc);
+}
+
+}  // extern "C"

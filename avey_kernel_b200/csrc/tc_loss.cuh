@@ -30,7 +30,7 @@
 // takes a unit does not change its result.
 #pragma once
 
-#include "tc_linear.cuh"
+#include "linear_steps.cuh"
 
 namespace avey {
 
@@ -654,6 +654,103 @@ __global__ void __launch_bounds__(kCeThreads, 1)
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc_pair(tmem, 512);
+  }
+}
+
+// ---------------------------------------------------------------- few rows
+
+// The statistics of a few rows: W is read once, straight from global memory into
+// mma.sync fragments (16 rows of it by up to 8 of x; bound: its bytes). A lane takes 16 consecutive k (32 bytes) of a 64-wide step for its fragments, so that four
+// lanes read a whole line; the order of k inside a product is free as long as both
+// operands agree. A warp takes 16 rows of W at a time and keeps (c, s) of the rows of x;
+// a CTA's warps are joined at the end. 131072 x 1024: 59 us, 4.5 TB/s.
+constexpr int kCfWarps = 8, kCfRows = 8;
+struct CeFew {
+  int rows, vocab, width;
+  const uint16_t* x;
+  const uint16_t* w;
+  int64_t x_ld, w_ld;
+  int x_vec, w_vec;
+  const void* targets;
+  int64_t target_stride;
+  int target64;
+  int64_t ignore;
+  float2* partial;  // [gridDim.x][rows]
+  float* picked;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(32 * kCfWarps) ce_few(const CeFew q) {
+  constexpr float kLog2e = 1.4426950408889634f;
+  __shared__ float2 meet[kCfWarps][kCfRows];
+  griddep_launch_dependents();
+  griddep_wait();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, tg = lane & 3;
+  int target[2];
+  float c[2], s[2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int row = 2 * tg + j;
+    target[j] = row < q.rows ? ce_target(q.targets, q.target_stride, q.target64, q.ignore, q.vocab, row) : -1;
+    c[j] = -INFINITY;
+    s[j] = 0.f;
+  }
+  const int groups = (q.vocab + 15) / 16;
+  for (int group = blockIdx.x * kCfWarps + warp; group < groups; group += gridDim.x * kCfWarps) {
+    const int v0 = group * 16 + g, v1 = v0 + 8;
+    const uint16_t* w0 = q.w + v0 * q.w_ld;
+    const uint16_t* w1 = q.w + v1 * q.w_ld;
+    const bool in0 = v0 < q.vocab, in1 = v1 < q.vocab;
+    float z[4] = {};
+#pragma unroll 2
+    for (int k0 = 0; k0 < q.width; k0 += 128) {
+      LnOct2 a[2], b[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int k = k0 + 64 * h + 16 * tg, left = q.width - k;
+        a[h] = ln_load16(w0 + k, in0 ? left : 0, q.w_vec);
+        b[h] = ln_load16(w1 + k, in1 ? left : 0, q.w_vec);
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int k = k0 + 64 * h + 16 * tg, left = q.width - k;
+        const uint32_t wa[8] = {a[h].a.x, a[h].a.y, a[h].a.z, a[h].a.w, a[h].b.x, a[h].b.y, a[h].b.z, a[h].b.w};
+        const uint32_t wb[8] = {b[h].a.x, b[h].a.y, b[h].a.z, b[h].a.w, b[h].b.x, b[h].b.y, b[h].b.z, b[h].b.w};
+        const LnOct2 xv = ln_load16(q.x + g * q.x_ld + k, g < q.rows ? left : 0, q.x_vec);
+        const uint32_t xw[8] = {xv.a.x, xv.a.y, xv.a.z, xv.a.w, xv.b.x, xv.b.y, xv.b.z, xv.b.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          ln_mma<T>(z, wa[2 * i], wb[2 * i], wa[2 * i + 1], wb[2 * i + 1], xw[2 * i], xw[2 * i + 1]);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const float z0 = in0 ? z[j] : -INFINITY, z1 = in1 ? z[j + 2] : -INFINITY;
+      if (target[j] >= 0) {
+        if (target[j] == v0) q.picked[2 * tg + j] = z0;
+        if (target[j] == v1) q.picked[2 * tg + j] = z1;
+      }
+      const float top = fmaxf(c[j], fmaxf(z0, z1) * kLog2e), base = top == -INFINITY ? 0.f : top;
+      s[j] = s[j] * ln_exp2(c[j] - base) + (ln_exp2(fmaf(z0, kLog2e, -base)) + ln_exp2(fmaf(z1, kLog2e, -base)));
+      c[j] = top;
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+#pragma unroll
+    for (int d = 4; d < 32; d <<= 1) {
+      const float c2 = __shfl_xor_sync(0xFFFFFFFFu, c[j], d), s2 = __shfl_xor_sync(0xFFFFFFFFu, s[j], d);
+      ce_join(c[j], s[j], c2, s2);
+    }
+    if (g == 0) meet[warp][2 * tg + j] = make_float2(c[j], s[j]);
+  }
+  __syncthreads();
+  const int row = threadIdx.x;
+  if (row < q.rows) {
+    float2 v = meet[0][row];
+    for (int i = 1; i < kCfWarps; ++i) ce_join(v.x, v.y, meet[i][row].x, meet[i][row].y);
+    q.partial[static_cast<int64_t>(blockIdx.x) * q.rows + row] = v;
   }
 }
 

@@ -33,6 +33,16 @@ struct Library {
   int (*loss_fwd)(const AveyLossParams*, void*) = nullptr;
   int (*loss_bwd)(const AveyLossParams*, void*) = nullptr;
   int (*loss_workspace)(const AveyLossParams*, int, uint64_t*) = nullptr;
+  int (*route_fwd)(const AveyRouteParams*, void*) = nullptr;
+  int (*route_bwd)(const AveyRouteParams*, void*) = nullptr;
+  int (*arrange)(const AveyArrangeParams*, void*) = nullptr;
+  int (*arrange_workspace)(const AveyArrangeParams*, uint64_t*) = nullptr;
+  int (*dispatch)(const AveyRowsParams*, void*) = nullptr;
+  int (*combine)(const AveyRowsParams*, void*) = nullptr;
+  int (*combine_bwd)(const AveyRowsParams*, void*) = nullptr;
+  int (*embedding_fwd)(const AveyEmbeddingParams*, void*) = nullptr;
+  int (*embedding_bwd)(const AveyEmbeddingParams*, void*) = nullptr;
+  int (*embedding_workspace)(const AveyEmbeddingParams*, uint64_t*) = nullptr;
   const char* (*last_error)() = nullptr;
 };
 Library lib;
@@ -534,6 +544,354 @@ Tensor cross_entropy(const Tensor& x, const Tensor& weight, const Tensor& target
   return loss_forward(x, weight, targets, ignore, reduction, z_loss, false).first;
 }
 
+// ------------------------------------------------------------ routing
+
+void check_floating(const Tensor& t, const char* name) {
+  TORCH_CHECK_VALUE(t.is_cuda() && dtype_id(t) >= 0, name, " must be a CUDA tensor of float32, float16 or bfloat16");
+}
+Tensor byte_workspace(uint64_t bytes, const Tensor& like) {
+  return bytes ? at::empty({static_cast<int64_t>(bytes)}, like.options().dtype(at::kByte)) : Tensor();
+}
+void* stream_of() { return at::cuda::getCurrentCUDAStream().stream(); }
+
+// The numbers of a call, as they are kept for the backward pass.
+struct RouteCall {
+  int64_t k, score, groups, top_groups, group_best, renormalize;
+  double scale;
+};
+AveyRouteParams route_params(const Tensor& rows, const RouteCall& call) {
+  AveyRouteParams p{};
+  p.struct_size = sizeof(p);
+  p.dtype = dtype_id(rows);
+  p.score = static_cast<int32_t>(call.score);
+  p.renormalize = static_cast<int32_t>(call.renormalize);
+  p.k = static_cast<int32_t>(call.k);
+  p.groups = static_cast<int32_t>(call.groups);
+  p.top_groups = static_cast<int32_t>(call.top_groups);
+  p.group_best = static_cast<int32_t>(call.group_best);
+  p.tokens = rows.size(0);
+  p.experts = rows.size(1);
+  p.scale = call.scale;
+  p.logits = rows.const_data_ptr();
+  p.logits_ld = row_ld(rows, p.experts);
+  return p;
+}
+
+std::pair<Tensor, Tensor> route_forward(const Tensor& logits, const std::optional<Tensor>& bias, const RouteCall& call) {
+  const c10::cuda::CUDAGuard guard(logits.device());
+  const Tensor rows = as_rows(logits, logits.size(-1));
+  AveyRouteParams p = route_params(rows, call);
+  auto shape = logits.sizes().vec();
+  shape.back() = call.k;
+  Tensor weights = at::empty(shape, logits.options().dtype(at::kFloat));
+  Tensor chosen = at::empty(shape, logits.options().dtype(at::kInt));
+  Tensor b;
+  if (bias) {
+    b = bias->contiguous();
+    p.bias = b.const_data_ptr<float>();
+  }
+  p.weights = weights.data_ptr<float>();
+  p.chosen = chosen.data_ptr<int32_t>();
+  check_status(lib.route_fwd(&p, stream_of()));
+  return {weights, chosen};
+}
+
+class RouteFunction : public torch::autograd::Function<RouteFunction> {
+ public:
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& logits,
+                                                const std::optional<Tensor>& bias, int64_t k, int64_t score,
+                                                int64_t groups, int64_t top_groups, int64_t group_best,
+                                                int64_t renormalize, double scale) {
+    const RouteCall call{k, score, groups, top_groups, group_best, renormalize, scale};
+    auto [weights, chosen] = route_forward(logits, bias, call);
+    ctx->save_for_backward({logits, weights, chosen});
+    ctx->mark_non_differentiable({chosen});
+    ctx->saved_data["call"] = std::vector<int64_t>{k, score, groups, top_groups, group_best, renormalize};
+    ctx->saved_data["scale"] = scale;
+    return {weights, chosen};
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    TORCH_CHECK(!at::GradMode::is_enabled(),
+                "the gradients of the native routing cannot be differentiated again (create_graph)");
+    const auto saved = ctx->get_saved_variables();
+    torch::autograd::variable_list out(9);
+    const Tensor &logits = saved[0], &dw = grads[0];
+    if (!dw.defined()) return out;
+    refuse_unseen([&](auto f) { f(dw); });
+    const std::vector<int64_t> c = ctx->saved_data["call"].toIntVector();
+    const RouteCall call{c[0], c[1], c[2], c[3], c[4], c[5], ctx->saved_data["scale"].toDouble()};
+    const c10::cuda::CUDAGuard guard(logits.device());
+    const Tensor rows = as_rows(logits, logits.size(-1)), g = dw.contiguous();
+    AveyRouteParams p = route_params(rows, call);
+    p.weights = saved[1].data_ptr<float>();
+    p.chosen = saved[2].data_ptr<int32_t>();
+    p.dweights = g.const_data_ptr<float>();
+    out[0] = at::empty(logits.sizes(), logits.options());
+    p.dlogits = out[0].data_ptr();
+    check_status(lib.route_bwd(&p, stream_of()));
+    return out;
+  }
+};
+
+std::pair<Tensor, Tensor> route(const Tensor& logits, const std::optional<Tensor>& bias, int64_t k, int64_t score,
+                                int64_t groups, int64_t top_groups, int64_t group_best, bool renormalize,
+                                double scale) {
+  refuse_unseen([&](auto f) {
+    f(logits);
+    if (bias) f(*bias);
+  });
+  check_floating(logits, "logits");
+  if (bias)
+    TORCH_CHECK_VALUE(bias->scalar_type() == at::kFloat && bias->device() == logits.device(),
+                      "bias must be float32 on the logits' device");
+  if (at::GradMode::is_enabled() && logits.requires_grad()) {
+    auto out = RouteFunction::apply(logits, bias, k, score, groups, top_groups, group_best,
+                                    static_cast<int64_t>(renormalize), scale);
+    return {out[0], out[1]};
+  }
+  return route_forward(logits, bias, {k, score, groups, top_groups, group_best, renormalize, scale});
+}
+
+std::pair<Tensor, Tensor> arrange(const Tensor& chosen, int64_t experts) {
+  refuse_unseen([](auto) {});
+  const c10::cuda::CUDAGuard guard(chosen.device());
+  const Tensor c = chosen.contiguous();
+  const auto i32 = chosen.options().dtype(at::kInt);
+  Tensor slots = at::empty(chosen.sizes(), i32), offsets = at::empty({experts + 1}, i32);
+  AveyArrangeParams p{};
+  p.struct_size = sizeof(p);
+  p.index_bits = c.scalar_type() == at::kLong ? 64 : 32;
+  p.count = c.numel();
+  p.experts = experts;
+  p.chosen = c.const_data_ptr();
+  p.slots = slots.data_ptr<int32_t>();
+  p.offsets = offsets.data_ptr<int32_t>();
+  uint64_t bytes = 0;
+  check_status(lib.arrange_workspace(&p, &bytes));
+  const Tensor ws = byte_workspace(bytes, c);
+  if (bytes) p.workspace = ws.data_ptr();
+  p.workspace_bytes = bytes;
+  check_status(lib.arrange(&p, stream_of()));
+  return {slots, offsets};
+}
+
+// ------------------------------------------------------------ rows of tokens
+
+AveyRowsParams rows_params(const Tensor& like, const Tensor& slots, int64_t width) {
+  AveyRowsParams p{};
+  p.struct_size = sizeof(p);
+  p.dtype = dtype_id(like);
+  p.tokens = slots.size(0);
+  p.k = static_cast<int32_t>(slots.size(1));
+  p.width = width;
+  p.slots = slots.const_data_ptr<int32_t>();
+  return p;
+}
+void set_rows(AveyRowsParams& p, const Tensor& rows) {
+  p.rows = const_cast<void*>(rows.const_data_ptr());
+  p.rows_ld = row_ld(rows, p.width);
+}
+void set_tokens(AveyRowsParams& p, const Tensor& x) {
+  p.x = x.const_data_ptr();
+  p.x_ld = row_ld(x, p.width);
+}
+
+Tensor dispatch_rows(const Tensor& x, const Tensor& slots) {
+  const c10::cuda::CUDAGuard guard(x.device());
+  const Tensor xr = as_rows(x, x.size(1)), s = slots.contiguous();
+  AveyRowsParams p = rows_params(x, s, x.size(1));
+  Tensor rows = at::empty({slots.numel(), x.size(1)}, x.options());
+  set_tokens(p, xr);
+  p.rows = rows.data_ptr();
+  p.rows_ld = p.width;
+  check_status(lib.dispatch(&p, stream_of()));
+  return rows;
+}
+
+Tensor combine_rows(const Tensor& rows, const Tensor& slots, const std::optional<Tensor>& weights,
+                    const std::optional<Tensor>& residual) {
+  const c10::cuda::CUDAGuard guard(rows.device());
+  const Tensor r = as_rows(rows, rows.size(1)), s = slots.contiguous();
+  AveyRowsParams p = rows_params(rows, s, rows.size(1));
+  set_rows(p, r);
+  Tensor w, res, out = at::empty({slots.size(0), rows.size(1)}, rows.options());
+  if (weights) {
+    w = weights->contiguous();
+    p.weights = w.const_data_ptr<float>();
+  }
+  if (residual) set_tokens(p, res = as_rows(*residual, p.width));
+  p.out = out.data_ptr();
+  check_status(lib.combine(&p, stream_of()));
+  return out;
+}
+
+class DispatchFunction : public torch::autograd::Function<DispatchFunction> {
+ public:
+  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const Tensor& slots) {
+    ctx->save_for_backward({slots});
+    return dispatch_rows(x, slots);
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    TORCH_CHECK(!at::GradMode::is_enabled(),
+                "the gradients of the native dispatch cannot be differentiated again (create_graph)");
+    if (!grads[0].defined()) return {Tensor(), Tensor()};
+    refuse_unseen([&](auto f) { f(grads[0]); });
+    return {combine_rows(grads[0], ctx->get_saved_variables()[0], std::nullopt, std::nullopt), Tensor()};
+  }
+};
+
+class CombineFunction : public torch::autograd::Function<CombineFunction> {
+ public:
+  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& rows, const Tensor& slots,
+                        const Tensor& weights, const std::optional<Tensor>& residual) {
+    // The rows go into the weights' gradient only.
+    ctx->save_for_backward({weights.requires_grad() ? rows : Tensor(), slots, weights});
+    ctx->saved_data["residual"] = residual.has_value();
+    return combine_rows(rows, slots, weights, residual);
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    TORCH_CHECK(!at::GradMode::is_enabled(),
+                "the gradients of the native combine cannot be differentiated again (create_graph)");
+    torch::autograd::variable_list out(4);
+    const Tensor& dy = grads[0];
+    if (!dy.defined()) return out;
+    refuse_unseen([&](auto f) { f(dy); });
+    const auto saved = ctx->get_saved_variables();
+    // needs_input_grad counts the tensors that were given: rows, slots, weights, residual.
+    const bool need_rows = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(2);
+    if (ctx->saved_data["residual"].toBool() && ctx->needs_input_grad(3)) out[3] = dy;
+    if (!need_rows && !need_w) return out;
+    const c10::cuda::CUDAGuard guard(dy.device());
+    const Tensor g = as_rows(dy, dy.size(1)), s = saved[1].contiguous(), w = saved[2].contiguous();
+    AveyRowsParams p = rows_params(dy, s, dy.size(1));
+    set_tokens(p, g);
+    p.weights = w.const_data_ptr<float>();
+    Tensor rows;
+    if (need_w) {
+      set_rows(p, rows = as_rows(saved[0], p.width));
+      out[2] = at::empty(s.sizes(), w.options());
+      p.dweights = out[2].data_ptr<float>();
+    }
+    if (need_rows) {
+      out[0] = at::empty({s.numel(), p.width}, dy.options());
+      p.drows = out[0].data_ptr();
+    }
+    check_status(lib.combine_bwd(&p, stream_of()));
+    return out;
+  }
+};
+
+void check_slots(const Tensor& slots, const Tensor& like) {
+  TORCH_CHECK_VALUE(slots.dim() == 2 && slots.scalar_type() == at::kInt && slots.device() == like.device(),
+                    "slots must be [tokens, k] int32 on the rows' device");
+}
+
+Tensor dispatch(const Tensor& x, const Tensor& slots) {
+  refuse_unseen([&](auto f) { f(x); });
+  check_floating(x, "x");
+  check_slots(slots, x);
+  if (at::GradMode::is_enabled() && x.requires_grad()) return DispatchFunction::apply(x, slots);
+  return dispatch_rows(x, slots);
+}
+
+Tensor combine(const Tensor& rows, const Tensor& slots, const Tensor& weights, const std::optional<Tensor>& residual) {
+  refuse_unseen([&](auto f) {
+    f(rows);
+    f(weights);
+    if (residual) f(*residual);
+  });
+  check_floating(rows, "rows");
+  check_slots(slots, rows);
+  TORCH_CHECK_VALUE(weights.scalar_type() == at::kFloat && weights.device() == rows.device(),
+                    "weights must be float32 on the rows' device");
+  if (residual)
+    TORCH_CHECK_VALUE(residual->scalar_type() == rows.scalar_type() && residual->device() == rows.device(),
+                      "residual must have the rows' type and device");
+  if (at::GradMode::is_enabled() &&
+      (rows.requires_grad() || weights.requires_grad() || (residual && residual->requires_grad())))
+    return CombineFunction::apply(rows, slots, weights, residual);
+  return combine_rows(rows, slots, weights, residual);
+}
+
+// ------------------------------------------------------------ embedding
+
+AveyEmbeddingParams embedding_params(const Tensor& like, const Tensor& tokens, int64_t vocab, int64_t width,
+                                     double scale, int64_t padding) {
+  AveyEmbeddingParams p{};
+  p.struct_size = sizeof(p);
+  p.dtype = dtype_id(like);
+  p.index_bits = tokens.scalar_type() == at::kLong ? 64 : 32;
+  p.count = tokens.numel();
+  p.width = width;
+  p.vocab = vocab;
+  p.padding = padding;
+  p.scale = scale;
+  p.tokens = tokens.const_data_ptr();
+  return p;
+}
+
+Tensor embedding_forward(const Tensor& tokens, const Tensor& weight, double scale, int64_t padding) {
+  const c10::cuda::CUDAGuard guard(weight.device());
+  const Tensor t = tokens.contiguous(), w = as_weight(weight);
+  AveyEmbeddingParams p = embedding_params(weight, t, weight.size(0), weight.size(1), scale, padding);
+  auto shape = tokens.sizes().vec();
+  shape.push_back(p.width);
+  Tensor out = at::empty(shape, weight.options());
+  p.table = w.const_data_ptr();
+  p.table_ld = p.vocab > 1 ? w.stride(0) : p.width;
+  p.out = out.data_ptr();
+  check_status(lib.embedding_fwd(&p, stream_of()));
+  return out;
+}
+
+class EmbeddingFunction : public torch::autograd::Function<EmbeddingFunction> {
+ public:
+  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& tokens, const Tensor& weight, double scale,
+                        int64_t padding) {
+    ctx->save_for_backward({tokens});
+    ctx->saved_data["call"] = std::vector<int64_t>{weight.size(0), weight.size(1), padding};
+    ctx->saved_data["scale"] = scale;
+    return embedding_forward(tokens, weight, scale, padding);
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    TORCH_CHECK(!at::GradMode::is_enabled(),
+                "the gradient of the native embedding cannot be differentiated again (create_graph)");
+    torch::autograd::variable_list out(4);
+    const Tensor& dy = grads[0];
+    if (!dy.defined()) return out;
+    refuse_unseen([&](auto f) { f(dy); });
+    const std::vector<int64_t> call = ctx->saved_data["call"].toIntVector();
+    const c10::cuda::CUDAGuard guard(dy.device());
+    const Tensor t = ctx->get_saved_variables()[0].contiguous(), g = as_rows(dy, call[1]);
+    AveyEmbeddingParams p = embedding_params(dy, t, call[0], call[1], ctx->saved_data["scale"].toDouble(), call[2]);
+    p.dy = g.const_data_ptr();
+    p.dy_ld = row_ld(g, p.width);
+    out[1] = at::empty({p.vocab, p.width}, dy.options());
+    p.dtable = out[1].data_ptr();
+    uint64_t bytes = 0;
+    check_status(lib.embedding_workspace(&p, &bytes));
+    const Tensor ws = byte_workspace(bytes, dy);
+    if (bytes) p.workspace = ws.data_ptr();
+    p.workspace_bytes = bytes;
+    check_status(lib.embedding_bwd(&p, stream_of()));
+    return out;
+  }
+};
+
+Tensor embedding(const Tensor& tokens, const Tensor& weight, double scale, int64_t padding) {
+  refuse_unseen([&](auto f) { f(weight); });
+  check_floating(weight, "weight");
+  TORCH_CHECK_VALUE(tokens.device() == weight.device(), "tokens must be on the weight's device");
+  if (at::GradMode::is_enabled() && weight.requires_grad())
+    return EmbeddingFunction::apply(tokens, weight, scale, padding);
+  return embedding_forward(tokens, weight, scale, padding);
+}
+
 // Entry points of the loaded library, by name.
 void bind(const py::dict& addresses) {
   auto at = [&](const char* name) { return addresses[name].cast<uintptr_t>(); };
@@ -544,6 +902,16 @@ void bind(const py::dict& addresses) {
   lib.loss_fwd = reinterpret_cast<decltype(lib.loss_fwd)>(at("avey_loss_fwd_v1"));
   lib.loss_bwd = reinterpret_cast<decltype(lib.loss_bwd)>(at("avey_loss_bwd_v1"));
   lib.loss_workspace = reinterpret_cast<decltype(lib.loss_workspace)>(at("avey_loss_workspace_size"));
+  lib.route_fwd = reinterpret_cast<decltype(lib.route_fwd)>(at("avey_route_fwd_v1"));
+  lib.route_bwd = reinterpret_cast<decltype(lib.route_bwd)>(at("avey_route_bwd_v1"));
+  lib.arrange = reinterpret_cast<decltype(lib.arrange)>(at("avey_arrange_v1"));
+  lib.arrange_workspace = reinterpret_cast<decltype(lib.arrange_workspace)>(at("avey_arrange_workspace_size"));
+  lib.dispatch = reinterpret_cast<decltype(lib.dispatch)>(at("avey_dispatch_v1"));
+  lib.combine = reinterpret_cast<decltype(lib.combine)>(at("avey_combine_v1"));
+  lib.combine_bwd = reinterpret_cast<decltype(lib.combine_bwd)>(at("avey_combine_bwd_v1"));
+  lib.embedding_fwd = reinterpret_cast<decltype(lib.embedding_fwd)>(at("avey_embedding_fwd_v1"));
+  lib.embedding_bwd = reinterpret_cast<decltype(lib.embedding_bwd)>(at("avey_embedding_bwd_v1"));
+  lib.embedding_workspace = reinterpret_cast<decltype(lib.embedding_workspace)>(at("avey_embedding_workspace_size"));
   lib.last_error = reinterpret_cast<decltype(lib.last_error)>(at("avey_last_error"));
 }
 
@@ -554,4 +922,9 @@ PYBIND11_MODULE(_torch_binding, m) {
   m.def("adamw_step", &adamw_step);
   m.def("linear", &linear);
   m.def("cross_entropy", &cross_entropy);
+  m.def("route", &route);
+  m.def("arrange", &arrange);
+  m.def("dispatch", &dispatch);
+  m.def("combine", &combine);
+  m.def("embedding", &embedding);
 }

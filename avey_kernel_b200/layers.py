@@ -30,10 +30,14 @@ contextualizer and its native backward.
   directions (``avey_linear_fwd_v1``, ``avey_linear_bwd_v1``): bf16 / f16
   inputs of any width and alignment, with or without grad. Its form grouped by
   expert is ``experts.expert_linear``.
+* ``embedding``: the rows of a table, scaled, native in both directions
+  (``avey_embedding_fwd_v1``, ``avey_embedding_bwd_v1``). The other end of a language
+  model is ``losses.linear_cross_entropy``.
 """
 
 from __future__ import annotations
 
+import math
 from typing import Optional, Tuple
 
 import torch
@@ -263,3 +267,29 @@ def residual_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.
         return y + residual
     return _binding.module().linear(x, weight, bias, residual, None, _ACT_IDS[activation],
                                     _native.LINEAR_AUTO)
+
+
+def embedding(tokens: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0,
+              padding_idx: Optional[int] = None) -> torch.Tensor:
+    """``scale * weight[tokens]``, rounded once: tokens of any shape (int64 or int32),
+    weight ``[vocab, width]`` (fp32, bf16 or f16), result ``[..., width]``.
+
+    ``padding_idx`` names a token whose row gets no gradient. A token outside the
+    vocabulary gives a row of NaN and no gradient. CUDA tensors run natively, forward
+    and backward: the gradient sorts the tokens and adds each one's rows up in fp32 in
+    one order, so it is bitwise reproducible and needs no array in fp32 of the table's size.
+    Forward-mode tangents, traces and second differentiation raise. CPU tensors take
+    plain PyTorch."""
+    if weight.ndim != 2 or 0 in weight.shape:
+        raise ValueError('weight must be [vocab, width]')
+    if tokens.dtype not in (torch.int32, torch.int64):
+        raise ValueError('tokens must be int32 or int64')
+    if padding_idx is not None and not 0 <= padding_idx < weight.shape[0]:
+        raise ValueError('padding_idx must be a token of the vocabulary')
+    if not math.isfinite(scale):
+        raise ValueError('scale must be finite')
+    if weight.is_cuda:
+        return _binding.module().embedding(tokens, weight, scale, -1 if padding_idx is None else padding_idx)
+    inside = (tokens >= 0) & (tokens < weight.shape[0])
+    out = F.embedding(torch.where(inside, tokens, 0), weight.float(), padding_idx) * scale
+    return torch.where(inside.unsqueeze(-1), out, math.nan).to(weight.dtype)

@@ -536,6 +536,138 @@ AVEY_API int avey_loss_bwd_v1(const AveyLossParams* params, void* stream);
 AVEY_API int avey_loss_workspace_size(const AveyLossParams* params, int backward, uint64_t* bytes);
 
 /*
+ * Routing of tokens to experts (no counterpart in the reference). For each token, with z
+ * its logits:
+ *
+ *   s = softmax(z) or sigmoid(z);   rank = z without a bias, else s + bias
+ *   a group of experts / groups consecutive experts ranks by the sum of the ranks of its
+ *   best group_best experts (1 or 2; without a bias by z for 1, by s for 2), and the
+ *   experts of the best top_groups groups are chosen from
+ *   chosen = the k of them that rank best, from the best on
+ *   weights = scale s, or with renormalize scale s / (sum of s over the chosen)
+ *
+ * Ties go to the lowest index. The order is that of the formula in exact arithmetic:
+ * where ranks in fp32 are too near to tell they are computed again in 64 bits. A logit
+ * of -inf ranks its expert below every other, whatever its bias, and gives the weight 0
+ * (also where all are -inf); a NaN ranks last and makes the softmax, or its own
+ * sigmoid, NaN. The weights' gradient goes to the logits; the choice and the bias have none.
+ */
+#define AVEY_SCORE_SOFTMAX 0
+#define AVEY_SCORE_SIGMOID 1
+
+typedef struct AveyRouteParams {
+  uint32_t struct_size; /* sizeof(AveyRouteParams) */
+  int32_t dtype;        /* logits and dlogits: AVEY_F32, AVEY_F16 or AVEY_BF16 */
+  int32_t score;        /* AVEY_SCORE_* */
+  int32_t renormalize;
+  int32_t k;            /* 1..32 */
+  int32_t groups;       /* 1..32, a divisor of experts */
+  int32_t top_groups;   /* 1..groups */
+  int32_t group_best;   /* 1 or 2 */
+  int64_t tokens, experts; /* up to 2^30 and 1024 */
+  double scale;
+  const void* logits;
+  int64_t logits_ld;
+  const float* bias;    /* [experts], or NULL */
+  float* weights;       /* [tokens][k] (backward: as the forward call wrote it) */
+  int32_t* chosen;      /* [tokens][k] (the same) */
+  const float* dweights; /* backward: [tokens][k] */
+  void* dlogits;         /* backward: contiguous [tokens][experts] */
+} AveyRouteParams;
+
+AVEY_API int avey_route_fwd_v1(const AveyRouteParams* params, void* stream);
+AVEY_API int avey_route_bwd_v1(const AveyRouteParams* params, void* stream);
+
+/*
+ * Places of choices sorted by expert: slots[i] is the place of entry i among all entries
+ * in the order of their experts (entries of one expert in their given order), and
+ * expert e's entries hold the places [offsets[e], offsets[e + 1]). Entries with a number
+ * outside [0, experts) hold the places from offsets[experts] on: they belong to no
+ * expert (avey_linear_* gives zeros there).
+ */
+typedef struct AveyArrangeParams {
+  uint32_t struct_size; /* sizeof(AveyArrangeParams) */
+  int32_t index_bits;   /* 32 or 64: signed expert numbers */
+  int64_t count, experts; /* up to 2^30 and 1024 */
+  const void* chosen;   /* [count] */
+  int32_t* slots;       /* [count] */
+  int32_t* offsets;     /* [experts + 1] */
+  void* workspace;      /* 256-byte aligned, >= avey_arrange_workspace_size() bytes */
+  uint64_t workspace_bytes;
+} AveyArrangeParams;
+
+AVEY_API int avey_arrange_v1(const AveyArrangeParams* params, void* stream);
+AVEY_API int avey_arrange_workspace_size(const AveyArrangeParams* params, uint64_t* bytes);
+
+/*
+ * Rows of tokens to the places of their choices and back, with slots [tokens][k] that
+ * hold each place in [0, tokens k) once (a slot outside it stands for no place: its choice
+ * is left out; a place that no slot names is not written):
+ *
+ *   dispatch      rows[slots[t][j]] = x[t]
+ *   combine       out[t] = x[t] (the residual, or 0 where x is NULL)
+ *                          + sum_j weights[t][j] rows[slots[t][j]]  (weights NULL: 1)
+ *   combine_bwd   drows[slots[t][j]] = weights[t][j] x[t], dweights[t][j] =
+ *                 <x[t], rows[slots[t][j]]>, with x the gradient of out
+ *
+ * dispatch's gradient is combine without weights and residual. Sums are fp32, in the
+ * order of j, and rounded once.
+ */
+typedef struct AveyRowsParams {
+  uint32_t struct_size; /* sizeof(AveyRowsParams) */
+  int32_t dtype;        /* x, rows, out, drows: AVEY_F32, AVEY_F16 or AVEY_BF16 */
+  int32_t k;            /* 1..32 */
+  int32_t reserved;
+  int64_t tokens, width; /* tokens x k up to 2^30, width up to 2^22 */
+  const int32_t* slots;
+  const void* x;
+  int64_t x_ld;
+  void* rows;           /* dispatch writes them */
+  int64_t rows_ld;
+  const float* weights; /* contiguous [tokens][k] */
+  void* out;            /* combine: contiguous [tokens][width] */
+  void* drows;          /* combine_bwd: contiguous [tokens k][width], or NULL */
+  float* dweights;      /* combine_bwd: contiguous [tokens][k], or NULL */
+} AveyRowsParams;
+
+AVEY_API int avey_dispatch_v1(const AveyRowsParams* params, void* stream);
+AVEY_API int avey_combine_v1(const AveyRowsParams* params, void* stream);
+AVEY_API int avey_combine_bwd_v1(const AveyRowsParams* params, void* stream);
+
+/*
+ * Embedding: out[i] = scale table[tokens[i]], rounded once (a token outside [0, vocab)
+ * gives a row of NaN), and the table's gradient
+ *
+ *   dtable[v] = scale * (sum of dy[i] over the i with tokens[i] = v, in fp32)
+ *
+ * for every v, with zeros for tokens that do not occur, for `padding` (when it is not
+ * negative) and for tokens outside the vocabulary. The tokens are sorted and each
+ * sum is taken in one order: results are bitwise reproducible.
+ */
+typedef struct AveyEmbeddingParams {
+  uint32_t struct_size; /* sizeof(AveyEmbeddingParams) */
+  int32_t dtype;        /* table, out, dy, dtable: AVEY_F32, AVEY_F16 or AVEY_BF16 */
+  int32_t index_bits;   /* 32 or 64: signed tokens */
+  int32_t reserved;
+  int64_t count, width, vocab; /* up to 2^30, 2^22 and 2^30 */
+  int64_t padding;      /* a token without a gradient, or negative */
+  double scale;
+  const void* tokens;   /* [count] */
+  const void* table;    /* forward */
+  int64_t table_ld;
+  void* out;            /* forward: contiguous [count][width] */
+  const void* dy;       /* backward */
+  int64_t dy_ld;
+  void* dtable;         /* backward: contiguous [vocab][width] */
+  void* workspace;      /* backward: 256-byte aligned, >= avey_embedding_workspace_size() bytes */
+  uint64_t workspace_bytes;
+} AveyEmbeddingParams;
+
+AVEY_API int avey_embedding_fwd_v1(const AveyEmbeddingParams* params, void* stream);
+AVEY_API int avey_embedding_bwd_v1(const AveyEmbeddingParams* params, void* stream);
+AVEY_API int avey_embedding_workspace_size(const AveyEmbeddingParams* params, uint64_t* bytes);
+
+/*
  * One AdamW step over many tensors (no counterpart in the reference, which
  * leaves training to torch). For every element of every tensor, in fp32:
  *
