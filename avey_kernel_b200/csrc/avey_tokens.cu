@@ -4,6 +4,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <mutex>
 
 #include "avey_b200.h"
 #include "host_api.h"
@@ -68,7 +69,10 @@ int validate(const AveyRouteParams* p, bool backward) {
 template <typename T, int R>
 int launch_route(const avey::RtArgs& q, bool backward, Chain& chain) {
   const dim3 grid(static_cast<unsigned>((q.tokens + avey::kRtWarps - 1) / avey::kRtWarps));
-  if (!backward) return chain.launch("route", avey::route_forward<T, R>, grid, 32 * avey::kRtWarps, 0, 1, q);
+  if (!backward) {
+    const dim3 some(std::min<unsigned>(grid.x, avey_host::multiprocessors() * 8u));
+    return chain.launch("route", avey::route_forward<T, R>, some, 32 * avey::kRtWarps, 0, 1, q);
+  }
   return chain.launch("route gradient", avey::route_backward<T, R>, grid, 32 * avey::kRtWarps,
                       avey::kRtWarps * 32 * R * 4, 1, q);
 }
@@ -121,7 +125,7 @@ int run_route(const AveyRouteParams* p, bool backward, void* stream) {
 int64_t sort_run(int64_t n) {
   if (n <= avey::kStOneBlock) return n;
   const int64_t share = (n + avey_host::multiprocessors() - 1) / avey_host::multiprocessors();
-  return std::max<int64_t>(avey::kStRun, (share + 255) / 256 * 256);
+  return std::max<int64_t>(avey::kStRun, (share + 511) / 512 * 512);
 }
 int64_t sort_blocks(int64_t n) {
   const int64_t run = sort_run(n);
@@ -132,7 +136,25 @@ uint64_t count_bytes(int64_t n, int buckets) {
   return b > 1 ? up256(static_cast<uint64_t>(b) * buckets * 4) : 0;
 }
 
+// The kernels' shared memory, past what a launch has by itself, once per device.
+int sort_opt_in() {
+  constexpr int kMaxDevices = 64;
+  static std::once_flag once[kMaxDevices];
+  static cudaError_t err[kMaxDevices];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices)
+    return fail(AVEY_ERR_CUDA, "no current device");
+  std::call_once(once[dev], [dev] {
+    err[dev] = cudaFuncSetAttribute(avey::st_count, cudaFuncAttributeMaxDynamicSharedMemorySize, avey::kStSmem);
+    if (err[dev] == cudaSuccess)
+      err[dev] = cudaFuncSetAttribute(avey::st_place, cudaFuncAttributeMaxDynamicSharedMemorySize, avey::kStSmem);
+  });
+  return err[dev] == cudaSuccess ? AVEY_OK : fail(AVEY_ERR_CUDA, cudaGetErrorString(err[dev]));
+}
+
 int launch_pass(avey::StArgs& q, Chain& chain) {
+  const int opted = sort_opt_in();
+  if (opted != AVEY_OK) return opted;
   q.run = std::max<int64_t>(1, sort_run(q.n));
   q.blocks = static_cast<int>(sort_blocks(q.n));
   const int smem = avey::kStWarps * q.buckets * 4;
@@ -191,13 +213,24 @@ int access_bytes(int size, int64_t width, std::initializer_list<const void*> bas
   return (all & 15u) == 0 ? 16 : (all & 3u) == 0 ? 4 : size;
 }
 
+// Lanes that take a row: as many as it has accesses, up to a warp.
+int part_lanes(int64_t width, int per) {
+  int lanes = 1;
+  while (lanes < 32 && lanes * per < width) lanes *= 2;
+  return lanes;
+}
+
 template <typename T, int N>
 int launch_rows(const avey::RwArgs& q, int what, Chain& chain) {
-  const unsigned grid = blocks_for(q.tokens * (q.width / N), 256);
-  if (what == 0) return chain.launch("dispatch", avey::rw_dispatch<T, N>, dim3(grid), 256, 0, 1, q);
-  if (what == 1) return chain.launch("combine", avey::rw_combine<T, N>, dim3(grid), 256, 0, 1, q);
-  const dim3 warps(static_cast<unsigned>((q.tokens + avey::kRwWarps - 1) / avey::kRwWarps));
-  return chain.launch("combine gradient", avey::rw_combine_backward<T, N>, warps, 32 * avey::kRwWarps, 0, 1, q);
+  if (what == 0)
+    return chain.launch("dispatch", avey::rw_dispatch<T, N>, dim3(blocks_for(q.tokens * (q.width / N), 256)), 256, 0, 1,
+                        q);
+  const int lanes = part_lanes(q.width, N);
+  const int64_t tokens = avey::kRwThreads / lanes;
+  const dim3 grid(static_cast<unsigned>(
+      std::min<int64_t>((q.tokens + tokens - 1) / tokens, avey_host::multiprocessors() * 3ll)));
+  if (what == 1) return chain.launch("combine", avey::rw_combine<T, N>, grid, avey::kRwThreads, 0, 1, q, lanes);
+  return chain.launch("combine gradient", avey::rw_combine_backward<T, N>, grid, avey::kRwThreads, 0, 1, q, lanes);
 }
 
 // what: 0 dispatch, 1 combine, 2 combine's backward.
@@ -276,10 +309,10 @@ avey::EmArgs embedding_args(const AveyEmbeddingParams* p) {
   return q;
 }
 
-// Workspace of the backward call: [keys, ids] twice, counts, tokens seen, parts.
+// Workspace of the backward call: [keys, ids] twice, counts, edges, tokens seen, parts.
 struct EmLayout {
   int passes = 0;
-  uint64_t keys[2] = {}, ids[2] = {}, counts = 0, seen = 0, parts = 0, total = 0;
+  uint64_t keys[2] = {}, ids[2] = {}, counts = 0, edges = 0, seen = 0, parts = 0, total = 0;
 };
 EmLayout embedding_layout(const AveyEmbeddingParams* p) {
   EmLayout l;
@@ -298,8 +331,10 @@ EmLayout embedding_layout(const AveyEmbeddingParams* p) {
     l.ids[i] = take(p->count * 4);
   }
   l.counts = take(count_bytes(p->count, 1024));
+  const uint64_t chunks = (p->count + avey::kEmChunk - 1) / avey::kEmChunk;
+  l.edges = take((1 + chunks) * 4);
   l.seen = take(p->vocab + 1);
-  l.parts = take(static_cast<uint64_t>((p->count + avey::kEmChunk - 1) / avey::kEmChunk) * 2 * p->width * 4);
+  l.parts = take(chunks * 2 * p->width * 4);
   l.total = at;
   return l;
 }
@@ -311,9 +346,12 @@ int launch_sums(const avey::EmArgs& q, Chain& chain) {
   int rc = chain.launch("embedding sums", avey::em_sum<T, N>, dim3(static_cast<unsigned>(q.chunks + zeros)), threads, 0,
                         1, q);
   if (rc != AVEY_OK || q.chunks < 2) return rc;
-  const unsigned slabs = static_cast<unsigned>(std::min<int64_t>(4, (q.width + avey::kEmCols - 1) / avey::kEmCols));
-  return chain.launch("embedding parts", avey::em_finish<T>, dim3(static_cast<unsigned>(q.chunks), slabs),
-                      avey::kEmGroups * avey::kEmCols, 0, 1, q);
+  constexpr int V = N > 1 && sizeof(T) * N == 16 ? 4 : 1;  // width is a multiple of 4
+  const int slabs = (q.width + avey::kEmLanes * V - 1) / (avey::kEmLanes * V);
+  const unsigned grid = static_cast<unsigned>(
+      std::min<int64_t>(avey_host::multiprocessors() * 8ll, q.chunks * static_cast<int64_t>(slabs)));
+  return chain.launch("embedding parts", avey::em_finish<T, V>, dim3(grid), avey::kEmGroups * avey::kEmLanes, 0, 1, q,
+                      slabs);
 }
 
 int embedding_backward(const AveyEmbeddingParams* p, cudaStream_t stream) {
@@ -327,7 +365,7 @@ int embedding_backward(const AveyEmbeddingParams* p, cudaStream_t stream) {
   if (rc != AVEY_OK) return rc;
   char* ws = static_cast<char*>(p->workspace);
   uint8_t* seen = reinterpret_cast<uint8_t*>(ws + l.seen);
-  const cudaError_t e = cudaMemsetAsync(seen, 0, p->vocab + 1, stream);
+  const cudaError_t e = cudaMemsetAsync(ws + l.edges, 0, l.parts - l.edges, stream);
   if (e != cudaSuccess) return fail(AVEY_ERR_CUDA, cudaGetErrorString(e));
   Chain chain{stream};
   for (int pass = 0; pass < l.passes; ++pass) {
@@ -357,6 +395,7 @@ int embedding_backward(const AveyEmbeddingParams* p, cudaStream_t stream) {
   q.ids = reinterpret_cast<uint32_t*>(ws + l.ids[(l.passes - 1) & 1]);
   q.seen = seen;
   q.parts = reinterpret_cast<float*>(ws + l.parts);
+  q.edges = reinterpret_cast<uint32_t*>(ws + l.edges);
   q.chunks = (p->count + avey::kEmChunk - 1) / avey::kEmChunk;
   const int bytes = access_bytes(size, p->width, {p->dy, p->dtable}, {p->dy_ld});
   if (p->dtype == AVEY_F32) return bytes == 16 ? launch_sums<float, 4>(q, chain) : launch_sums<float, 1>(q, chain);
@@ -371,7 +410,10 @@ int embedding_backward(const AveyEmbeddingParams* p, cudaStream_t stream) {
 
 template <typename T, int N>
 int launch_lookup(const avey::EmArgs& q, Chain& chain) {
-  return chain.launch("embedding", avey::em_forward<T, N>, dim3(blocks_for(q.n * (q.width / N), 256)), 256, 0, 1, q);
+  const int lanes = part_lanes(q.width, N);
+  const int64_t rows = avey::kRwThreads / lanes;
+  return chain.launch("embedding", avey::em_forward<T, N>, dim3(static_cast<unsigned>((q.n + rows - 1) / rows)),
+                      avey::kRwThreads, 0, 1, q, lanes);
 }
 
 int embedding_forward(const AveyEmbeddingParams* p, cudaStream_t stream) {

@@ -108,86 +108,6 @@ __device__ __forceinline__ void rt_scores(const float (&z)[R], bool softmax, S (
   }
 }
 
-// The warp's best value and the lowest expert that has it; `there` marks what may be taken.
-struct RtBest64 {
-  double value;
-  int expert;  // -1: none
-};
-template <int R>
-__device__ __forceinline__ RtBest64 rt_best64(const double (&r)[R], uint32_t there, int e0) {
-  RtBest64 b{-CUDART_INF, -1};
-#pragma unroll
-  for (int i = 0; i < R; ++i)
-    if ((there >> i & 1u) && (b.expert < 0 || r[i] > b.value)) b = {r[i], e0 + i};
-#pragma unroll
-  for (int d = 16; d; d >>= 1) {
-    const double v = __shfl_xor_sync(0xFFFFFFFFu, b.value, d);
-    const int e = __shfl_xor_sync(0xFFFFFFFFu, b.expert, d);
-    if (e >= 0 && (b.expert < 0 || v > b.value || (v == b.value && e < b.expert))) b = {v, e};
-  }
-  return b;
-}
-
-// Lane j's expert is the j-th chosen one. In 64 bits; of NaN and -inf ranks as the header says.
-template <int R>
-__device__ __noinline__ int rt_choose64(const RtArgs& q, const float (&z)[R], int lane) {
-  const int e0 = lane * R;
-  double r[R];
-  if (q.bias || (q.groups > 1 && q.group_best == 2)) rt_scores<double, R>(z, q.softmax, r);
-  double by[R];  // what groups rank by
-  uint32_t there = 0, dead = 0;
-#pragma unroll
-  for (int i = 0; i < R; ++i) {
-    if (e0 + i >= q.experts) continue;
-    there |= 1u << i;
-    if (q.bias) by[i] = r[i] += static_cast<double>(__ldg(q.bias + e0 + i));
-    else if (q.groups > 1 && q.group_best == 2) by[i] = r[i], r[i] = z[i];
-    else by[i] = r[i] = z[i];
-    if (r[i] != r[i] || z[i] != z[i]) r[i] = by[i] = -CUDART_INF, dead |= 1u << i;
-    else if (z[i] == -CUDART_INF_F) r[i] = by[i] = -CUDART_INF;
-  }
-  if (q.groups > 1) {
-    const int size = q.experts / q.groups;
-    double merit = -CUDART_INF;  // lane g: of group g
-    for (int g = 0; g < q.groups; ++g) {
-      uint32_t in = 0;
-#pragma unroll
-      for (int i = 0; i < R; ++i)
-        if ((there >> i & 1u) && (e0 + i) / size == g) in |= 1u << i;
-      const RtBest64 a = rt_best64<R>(by, in, e0);
-      double m = a.value;
-      if (q.group_best == 2 && a.value > -CUDART_INF) {
-#pragma unroll
-        for (int i = 0; i < R; ++i)
-          if (e0 + i == a.expert) in &= ~(1u << i);
-        const RtBest64 b = rt_best64<R>(by, in, e0);
-        if (b.expert >= 0 && b.value > -CUDART_INF) m += b.value;
-      }
-      if (lane == g) merit = m;
-    }
-    uint32_t open = lane < q.groups, keep = 0;
-    for (int n = 0; n < q.top_groups; ++n) {
-      const double one[1] = {merit};
-      const RtBest64 b = rt_best64<1>(one, open, lane);
-      keep |= 1u << b.expert;
-      if (lane == b.expert) open = 0;
-    }
-#pragma unroll
-    for (int i = 0; i < R; ++i)
-      if ((there >> i & 1u) && !(keep >> ((e0 + i) / size) & 1u)) there &= ~(1u << i);
-  }
-  int mine = 0;
-  for (int j = 0; j < q.k; ++j) {
-    RtBest64 b = rt_best64<R>(r, there & ~dead, e0);
-    if (b.expert < 0) b = rt_best64<R>(r, there, e0);  // only NaN are left
-#pragma unroll
-    for (int i = 0; i < R; ++i)
-      if (e0 + i == b.expert) there &= ~(1u << i);
-    if (lane == j) mine = b.expert;
-  }
-  return mine;
-}
-
 // The warp's largest key, and the lowest expert that has it.
 template <int R>
 __device__ __forceinline__ uint32_t rt_best(const uint32_t (&key)[R], int e0, int& expert) {
@@ -204,9 +124,107 @@ __device__ __forceinline__ uint32_t rt_best(const uint32_t (&key)[R], int e0, in
   return all;
 }
 
-// The same choice in 32 bits; false where two that matter are too near to tell.
+// The same for 64-bit keys, which order doubles: NaN at 1, 0 stands for "not there".
+__device__ __forceinline__ unsigned long long rt_key64(double x) {
+  if (x != x) return 1ull;
+  const unsigned long long b = static_cast<unsigned long long>(__double_as_longlong(x + 0.0));
+  return b >> 63 ? ~b : b | (1ull << 63);
+}
+__device__ __forceinline__ double rt_value64(unsigned long long key) {
+  if (key <= 1ull) return -CUDART_INF;
+  return __longlong_as_double(static_cast<long long>(key >> 63 ? key ^ (1ull << 63) : ~key));
+}
 template <int R>
-__device__ __forceinline__ bool rt_choose(const RtArgs& q, const float (&z)[R], int lane, int& mine) {
+__device__ __forceinline__ unsigned long long rt_best64(const unsigned long long (&key)[R], int e0, int& expert) {
+  unsigned long long top = key[0];
+#pragma unroll
+  for (int i = 1; i < R; ++i) top = max(top, key[i]);
+  const uint32_t hi = __reduce_max_sync(0xFFFFFFFFu, static_cast<uint32_t>(top >> 32));
+  const uint32_t lo = __reduce_max_sync(0xFFFFFFFFu, top >> 32 == hi ? static_cast<uint32_t>(top) : 0u);
+  const unsigned long long all = static_cast<unsigned long long>(hi) << 32 | lo;
+  int at = 0;
+#pragma unroll
+  for (int i = R - 1; i >= 0; --i)
+    if (key[i] == all) at = i;
+  const int src = __ffs(__ballot_sync(0xFFFFFFFFu, top == all)) - 1;
+  expert = __shfl_sync(0xFFFFFFFFu, e0 + at, src);
+  return all;
+}
+
+// Which groups are chosen from: lane g has group g's merit. A group's place is the number
+// of better ones (and of those as good before it). `in`, `out`: the last one kept and the
+// first one not.
+template <typename S>
+__device__ __forceinline__ uint32_t rt_keep(const RtArgs& q, S merit, int lane, int& in, int& out) {
+  int place = 0;
+  for (int g = 0; g < q.groups; ++g) {
+    const S other = __shfl_sync(0xFFFFFFFFu, merit, g);
+    place += other > merit || (other == merit && g < lane);
+  }
+  const bool there = lane < q.groups;
+  in = __ffs(__ballot_sync(0xFFFFFFFFu, there && place == q.top_groups - 1)) - 1;
+  out = __ffs(__ballot_sync(0xFFFFFFFFu, there && place == q.top_groups)) - 1;
+  return __ballot_sync(0xFFFFFFFFu, there && place < q.top_groups);
+}
+
+// Lane j's expert is the j-th chosen one, by scores in 64 bits.
+template <int R>
+__device__ __noinline__ int rt_choose64(const RtArgs& q, const float (&z)[R], int lane) {
+  const int e0 = lane * R;
+  const bool scored = q.bias || (q.groups > 1 && q.group_best == 2);
+  double r[R];
+  if (scored) rt_scores<double, R>(z, q.softmax, r);
+  unsigned long long key[R], by[R];  // by: what groups rank by
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    key[i] = by[i] = 0ull;
+    if (e0 + i >= q.experts) continue;
+    const double own = scored ? r[i] : static_cast<double>(z[i]);
+    const double rank = q.bias ? own + static_cast<double>(__ldg(q.bias + e0 + i)) : own;
+    by[i] = z[i] == -CUDART_INF_F ? rt_key64(-CUDART_INF) : z[i] != z[i] ? 1ull : rt_key64(rank);
+    key[i] = q.bias ? by[i] : rt_key64(static_cast<double>(z[i]));
+  }
+  if (q.groups > 1) {
+    const int size = q.experts / q.groups;
+    double merit = -CUDART_INF;
+    for (int g = 0; g < q.groups; ++g) {
+      unsigned long long mine[R];
+#pragma unroll
+      for (int i = 0; i < R; ++i) mine[i] = (e0 + i) / size == g ? by[i] : 0ull;
+      int e;
+      double m = rt_value64(rt_best64<R>(mine, e0, e));
+      if (q.group_best == 2 && m > -CUDART_INF) {
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+          if (e0 + i == e) mine[i] = 0ull;
+        const double second = rt_value64(rt_best64<R>(mine, e0, e));
+        if (second > -CUDART_INF) m += second;
+      }
+      if (lane == g) merit = m;
+    }
+    int in, out;
+    const uint32_t keep = rt_keep(q, merit, lane, in, out);
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+      if (!(keep >> (min((e0 + i) / size, 31)) & 1u)) key[i] = 0ull;
+  }
+  int mine = 0;
+  for (int j = 0; j < q.k; ++j) {
+    int e;
+    rt_best64<R>(key, e0, e);
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+      if (e0 + i == e) key[i] = 0ull;
+    if (lane == j) mine = e;
+  }
+  return mine;
+}
+
+// The same choice in 32 bits, and the chosen logits; false where two ranks that matter are
+// too near to tell. `most`: the largest |bias|.
+template <int R>
+__device__ __forceinline__ bool rt_choose(const RtArgs& q, const float (&z)[R], float most, int lane, int& mine,
+                                          float& mz) {
   const int e0 = lane * R;
   const bool by_logit = !q.bias, sums = q.groups > 1 && q.group_best == 2;
   // Bounds of the errors of two ranks relative to their terms: the exponential and the
@@ -214,98 +232,108 @@ __device__ __forceinline__ bool rt_choose(const RtArgs& q, const float (&z)[R], 
   // addition of the bias (2^-24).
   const float tol = q.softmax ? 4e-6f : 1e-6f;
   uint32_t key[R];
-  float s[R];
-  if (!by_logit || sums) rt_scores<float, R>(z, q.softmax, s);
   bool sure = true;
-  auto rank = [&](int i) {  // of this lane's i-th expert, where the choice is not by the logit
-    const float r = q.bias ? s[i] + __ldg(q.bias + e0 + i) : s[i];
-    return z[i] == -CUDART_INF_F ? -CUDART_INF_F : z[i] != z[i] ? z[i] : r;
-  };
-  if (sums || !by_logit) {
-#pragma unroll
-    for (int i = 0; i < R; ++i) key[i] = e0 + i < q.experts ? rt_key(rank(i)) : 0u;
-  } else {
+  if (by_logit && !sums) {
 #pragma unroll
     for (int i = 0; i < R; ++i) key[i] = e0 + i < q.experts ? rt_key(z[i]) : 0u;
+  } else {
+    float s[R];
+    rt_scores<float, R>(z, q.softmax, s);
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      key[i] = 0u;
+      if (e0 + i >= q.experts) continue;
+      const float r = q.bias ? s[i] + __ldg(q.bias + e0 + i) : s[i];
+      key[i] = z[i] == -CUDART_INF_F ? rt_key(-CUDART_INF_F) : z[i] != z[i] ? 1u : rt_key(r);
+    }
   }
   if (q.groups > 1) {
     const int size = q.experts / q.groups;
-    float merit = -CUDART_INF_F;  // lane g: of group g
-    float bound = 0.f;            // of its terms' sizes
-    for (int g = 0; g < q.groups; ++g) {
-      uint32_t in[R];
+    float first = -CUDART_INF_F, second = -CUDART_INF_F;  // lane g: of group g
+    const int span = size / R;
+    if (size % R == 0 && (span & (span - 1)) == 0) {
+      // A group is `span` whole lanes, a power of two: all groups at once.
+      float a = -CUDART_INF_F, b = -CUDART_INF_F;
 #pragma unroll
-      for (int i = 0; i < R; ++i) in[i] = (e0 + i) / size == g ? key[i] : 0u;
-      int e;
-      float m = rt_value(rt_best<R>(in, e0, e));
-      float terms = fabsf(m) + (q.bias ? fabsf(__ldg(q.bias + e)) : 0.f);
-      if (sums && m > -CUDART_INF_F) {
+      for (int i = 0; i < R; ++i) {
+        const float r = rt_value(key[i]);
+        b = fmaxf(b, fminf(a, r));
+        a = fmaxf(a, r);
+      }
+      for (int d = 1; d < span; d <<= 1) {
+        const float a2 = __shfl_xor_sync(0xFFFFFFFFu, a, d), b2 = __shfl_xor_sync(0xFFFFFFFFu, b, d);
+        b = fmaxf(fminf(a, a2), fmaxf(b, b2));
+        a = fmaxf(a, a2);
+      }
+      const int src = min(lane * span, 31);
+      first = __shfl_sync(0xFFFFFFFFu, a, src);
+      second = __shfl_sync(0xFFFFFFFFu, b, src);
+    } else {
+      for (int g = 0; g < q.groups; ++g) {
+        uint32_t in[R];
+#pragma unroll
+        for (int i = 0; i < R; ++i) in[i] = (e0 + i) / size == g ? key[i] : 0u;
+        int e;
+        const float a = rt_value(rt_best<R>(in, e0, e));
 #pragma unroll
         for (int i = 0; i < R; ++i)
           if (e0 + i == e) in[i] = 0u;
-        const float second = rt_value(rt_best<R>(in, e0, e));
-        if (second > -CUDART_INF_F) {
-          m += second;
-          terms += fabsf(second) + (q.bias ? fabsf(__ldg(q.bias + e)) : 0.f);
+        const float b = rt_value(rt_best<R>(in, e0, e));
+        if (lane == g) {
+          first = a;
+          second = b;
         }
       }
-      if (lane == g) {
-        merit = m;
-        bound = terms;
-      }
     }
-    const uint32_t one[1] = {lane < q.groups ? rt_key(merit) : 0u};
-    uint32_t open[1] = {one[0]};
-    uint32_t keep = 0;
-    int last = 0;
-    for (int n = 0; n < q.top_groups; ++n) {
-      rt_best<1>(open, lane, last);
-      keep |= 1u << last;
-      if (lane == last) open[0] = 0u;
-    }
-    if (q.top_groups < q.groups && (sums || !by_logit)) {
-      // The last group in and the first one out.
-      int first = 0;
-      const float out = rt_value(rt_best<1>(open, lane, first));
-      const float in = __shfl_sync(0xFFFFFFFFu, merit, last);
-      const float e = tol * (__shfl_sync(0xFFFFFFFFu, bound, last) + __shfl_sync(0xFFFFFFFFu, bound, first));
-      sure = !(in - out <= e) || out == -CUDART_INF_F;
+    const bool two = q.group_best == 2 && second > -CUDART_INF_F;
+    const float merit = two ? first + second : first;
+    int in, out;
+    const uint32_t keep = rt_keep(q, merit, lane, in, out);
+    if (q.top_groups < q.groups && !(by_logit && !sums)) {
+      const float terms = fabsf(first) + (two ? fabsf(second) : 0.f) + 2.f * most;
+      const float bound = tol * (__shfl_sync(0xFFFFFFFFu, terms, in) + __shfl_sync(0xFFFFFFFFu, terms, out));
+      const float m_in = __shfl_sync(0xFFFFFFFFu, merit, in), m_out = __shfl_sync(0xFFFFFFFFu, merit, out);
+      sure = m_out == -CUDART_INF_F || !(m_in - m_out <= bound);
     }
 #pragma unroll
     for (int i = 0; i < R; ++i) {
       if (by_logit && sums && key[i]) key[i] = rt_key(z[i]);
-      if (!(keep >> ((e0 + i) / size) & 1u)) key[i] = 0u;
+      if (!(keep >> (min((e0 + i) / size, 31)) & 1u)) key[i] = 0u;
     }
   }
-  // The chosen, and the next one, from the best on.
-  uint32_t before = 0u;
+  // The chosen, and with a bias the next one, from the best on.
+  float before = 0.f;
   int before_e = 0;
   const int rounds = by_logit ? q.k : min(q.k + 1, q.top_groups * (q.experts / q.groups));
   for (int j = 0; j < rounds; ++j) {
     int e;
     const uint32_t top = rt_best<R>(key, e0, e);
-    if (!by_logit && j > 0) {
-      const float a = rt_value(before), b = rt_value(top);
-      const float ba = __ldg(q.bias + before_e), bb = __ldg(q.bias + e);
-      if (b > -CUDART_INF_F && a - b <= tol * (fabsf(a) + fabsf(b) + fabsf(ba) + fabsf(bb))) {
-        // Too near, unless they are alike.
-        float za = 0.f, zb = 0.f;
-#pragma unroll
-        for (int i = 0; i < R; ++i) {
-          if (e0 + i == before_e) za = z[i];
-          if (e0 + i == e) zb = z[i];
-        }
-        za = __shfl_sync(0xFFFFFFFFu, za, before_e / R);
-        zb = __shfl_sync(0xFFFFFFFFu, zb, e / R);
-        sure = sure && za == zb && ba == bb;
-      }
-    }
+    float own = 0.f;
 #pragma unroll
     for (int i = 0; i < R; ++i)
-      if (e0 + i == e) key[i] = 0u;
-    if (lane == j && j < q.k) mine = e;
-    before = top;
-    before_e = e;
+      if (e0 + i == e) {
+        key[i] = 0u;
+        own = z[i];
+      }
+    if (!by_logit) {
+      const float r = rt_value(top);
+      if (j > 0 && r > -CUDART_INF_F && before - r <= tol * (fabsf(before) + fabsf(r) + 2.f * most)) {
+        // Too near, unless they are alike.
+        float other = 0.f;
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+          if (e0 + i == before_e) other = z[i];
+        sure = sure && __shfl_sync(0xFFFFFFFFu, other, before_e / R) == __shfl_sync(0xFFFFFFFFu, own, e / R) &&
+               __ldg(q.bias + before_e) == __ldg(q.bias + e);
+      }
+      before = r;
+      before_e = e;
+    }
+    own = __shfl_sync(0xFFFFFFFFu, own, e / R);
+    if (lane == j && j < q.k) {
+      mine = e;
+      mz = own;
+    }
   }
   return sure;
 }
@@ -331,46 +359,64 @@ __device__ __forceinline__ float rt_renormalized(float z, bool softmax, bool in)
 
 template <typename T, int R>
 __global__ void __launch_bounds__(32 * kRtWarps) route_forward(const RtArgs q) {
-  const int lane = threadIdx.x & 31;
-  const int64_t t = static_cast<int64_t>(blockIdx.x) * kRtWarps + (threadIdx.x >> 5);
-  if (t >= q.tokens) return;
-  const T* row = static_cast<const T*>(q.logits) + t * q.ld;
-  float z[R];
-  rt_load<T, R>(row, lane * R, q.experts, q.vec, z);
-  int mine = 0;
-  if (!rt_choose<R>(q, z, lane, mine)) mine = rt_choose64<R>(q, z, lane);
-  const bool in = lane < q.k;
-  const float mz = in ? Elem<T>::load(row + mine) : 0.f;
-  float w;
-  if (q.softmax) {
-    // A NaN or +inf anywhere in the row makes the softmax NaN.
-    float top = -CUDART_INF_F;
-    bool bad = false;
+  const int lane = threadIdx.x & 31, e0 = lane * R;
+  float most = 0.f;  // the largest |bias|
+  if (q.bias) {
+    for (int e = lane; e < q.experts; e += 32) most = fmaxf(most, fabsf(__ldg(q.bias + e)));
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-      top = fmaxf(top, z[i]);
-      bad |= !(z[i] < CUDART_INF_F);
+    for (int d = 16; d; d >>= 1) most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, d));
+  }
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kRtWarps;
+  int64_t t = static_cast<int64_t>(blockIdx.x) * kRtWarps + (threadIdx.x >> 5);
+  float next[R];
+  if (t < q.tokens) rt_load<T, R>(static_cast<const T*>(q.logits) + t * q.ld, e0, q.experts, q.vec, next);
+  for (; t < q.tokens; t += step) {
+    float z[R];
+#pragma unroll
+    for (int i = 0; i < R; ++i) z[i] = next[i];
+    if (t + step < q.tokens)  // the next token's logits are under way meanwhile
+      rt_load<T, R>(static_cast<const T*>(q.logits) + (t + step) * q.ld, e0, q.experts, q.vec, next);
+    int mine = 0;
+    float mz = 0.f;
+    if (!rt_choose<R>(q, z, most, lane, mine, mz)) {
+      mine = rt_choose64<R>(q, z, lane);
+      for (int j = 0; j < q.k; ++j) {
+        const int e = __shfl_sync(0xFFFFFFFFu, mine, j);
+        float own = 0.f;
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+          if (e0 + i == e) own = z[i];
+        own = __shfl_sync(0xFFFFFFFFu, own, e / R);
+        if (lane == j) mz = own;
+      }
     }
-    bad = __any_sync(0xFFFFFFFFu, bad);
-    if (q.renormalize) {
-      w = rt_renormalized(mz, true, in);
-    } else {
+    const bool in = lane < q.k;
+    float w;
+    if (q.softmax && !q.renormalize) {
+      float top = z[0];
 #pragma unroll
-      for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
+      for (int i = 1; i < R; ++i) top = fmaxf(top, z[i]);
+      top = rt_value(__reduce_max_sync(0xFFFFFFFFu, rt_key(top)));
       const float base = top == -CUDART_INF_F ? 0.f : top;
       float sum = 0.f;
 #pragma unroll
       for (int i = 0; i < R; ++i) sum += expf(z[i] - base);
-      sum = rt_warp_sum(sum);
+      sum = rt_warp_sum(sum);  // NaN where a logit is NaN or +inf
       w = sum == 0.f ? 0.f : expf(mz - base) / sum;
+    } else if (q.softmax) {
+      // A NaN or +inf anywhere in the row makes the softmax NaN.
+      bool bad = false;
+#pragma unroll
+      for (int i = 0; i < R; ++i) bad |= !(z[i] < CUDART_INF_F);
+      w = rt_renormalized(mz, true, in);
+      if (__any_sync(0xFFFFFFFFu, bad)) w = CUDART_NAN_F;
+    } else {
+      w = q.renormalize ? rt_renormalized(mz, false, in) : 1.f / (1.f + expf(-mz));
     }
-    if (bad) w = CUDART_NAN_F;
-  } else {
-    w = q.renormalize ? rt_renormalized(mz, false, in) : 1.f / (1.f + expf(-mz));
-  }
-  if (in) {
-    q.weights[t * q.k + lane] = w * q.scale;
-    q.chosen[t * q.k + lane] = mine;
+    if (in) {
+      q.weights[t * q.k + lane] = w * q.scale;
+      q.chosen[t * q.k + lane] = mine;
+    }
   }
 }
 

@@ -6,9 +6,11 @@
 //   embedding  out_i = scale table[token_i]
 //   and the embedding's gradient by sorted tokens.
 //
-// Bound: the rows' bytes, each read and written once; a thread moves 16 bytes of a row
-// (less where rows are not whole 16-byte units), with all k rows of a token under way
-// together. Sums are fp32, in the order of the choices, or of the tokens.
+// Bound: the rows' bytes, each read and written once. A lane moves 16 bytes of a row at a
+// time (less where rows are not whole 16-byte units); a token's rows belong to one warp
+// (or a part of one, for narrow rows), which has up to eight accesses a lane under way and
+// the next token's slots read ahead.
+// Sums are fp32, in the order of the choices, or of the tokens.
 #pragma once
 
 #include <math_constants.h>
@@ -20,24 +22,74 @@
 
 namespace avey {
 
-// N values of type T as one access.
+// N values of type T as one access of 16, 4 or 2 bytes, held as words (as an array of T
+// the compiler kept what is loaded under a condition in local memory: 101 -> 170 us for
+// the sums of combine).
 template <typename T, int N>
-struct alignas(sizeof(T) * N) RwVec {
-  T v[N];
+struct RwVec {
+  static constexpr int kBytes = static_cast<int>(sizeof(T)) * N, kWords = kBytes < 4 ? 1 : kBytes / 4;
+  uint32_t w[kWords];
 };
+template <typename T, int N>
+__device__ __forceinline__ RwVec<T, N> rw_zero() {
+  RwVec<T, N> r;
+#pragma unroll
+  for (int i = 0; i < RwVec<T, N>::kWords; ++i) r.w[i] = 0u;
+  return r;
+}
 template <typename T, int N>
 __device__ __forceinline__ RwVec<T, N> rw_load(const T* p) {
   RwVec<T, N> r;
-  constexpr int kBytes = sizeof(T) * N;
-  if constexpr (kBytes == 16) *reinterpret_cast<uint4*>(&r) = __ldg(reinterpret_cast<const uint4*>(p));
-  else if constexpr (kBytes == 8) *reinterpret_cast<uint2*>(&r) = __ldg(reinterpret_cast<const uint2*>(p));
-  else if constexpr (kBytes == 4) *reinterpret_cast<uint32_t*>(&r) = __ldg(reinterpret_cast<const uint32_t*>(p));
-  else *reinterpret_cast<uint16_t*>(&r) = __ldg(reinterpret_cast<const uint16_t*>(p));
+  if constexpr (RwVec<T, N>::kBytes == 16) {
+    const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
+    r.w[0] = v.x;
+    r.w[1] = v.y;
+    r.w[2] = v.z;
+    r.w[3] = v.w;
+  } else if constexpr (RwVec<T, N>::kBytes == 4) {
+    r.w[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
+  } else {
+    r.w[0] = __ldg(reinterpret_cast<const uint16_t*>(p));
+  }
   return r;
 }
 template <typename T, int N>
 __device__ __forceinline__ void rw_store(T* p, const RwVec<T, N>& r) {
-  *reinterpret_cast<RwVec<T, N>*>(p) = r;
+  if constexpr (RwVec<T, N>::kBytes == 16) *reinterpret_cast<uint4*>(p) = make_uint4(r.w[0], r.w[1], r.w[2], r.w[3]);
+  else if constexpr (RwVec<T, N>::kBytes == 4) *reinterpret_cast<uint32_t*>(p) = r.w[0];
+  else *reinterpret_cast<uint16_t*>(p) = static_cast<uint16_t>(r.w[0]);
+}
+// The n-th value, and values rounded to T.
+template <typename T, int N>
+__device__ __forceinline__ float rw_get(const RwVec<T, N>& r, int n) {
+  if constexpr (sizeof(T) == 4) {
+    return __uint_as_float(r.w[n]);
+  } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    return __uint_as_float((n & 1) ? r.w[n / 2] & 0xFFFF0000u : r.w[n / 2] << 16);
+  } else {
+    return __half2float(__ushort_as_half(static_cast<unsigned short>((n & 1) ? r.w[n / 2] >> 16 : r.w[n / 2])));
+  }
+}
+template <typename T, int N>
+__device__ __forceinline__ RwVec<T, N> rw_pack(const float (&z)[N]) {
+  RwVec<T, N> r;
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) r.w[n] = __float_as_uint(z[n]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < RwVec<T, N>::kWords; ++i) {
+      const float lo = z[2 * i], hi = 2 * i + 1 < N ? z[2 * i + 1] : 0.f;
+      if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+        r.w[i] = *reinterpret_cast<const uint32_t*>(&h);
+      } else {
+        const __half2 h = __floats2half2_rn(lo, hi);
+        r.w[i] = *reinterpret_cast<const uint32_t*>(&h);
+      }
+    }
+  }
+  return r;
 }
 
 constexpr int kRwMaxK = 32;
@@ -71,111 +123,144 @@ __global__ void __launch_bounds__(256) rw_dispatch(const RwArgs q) {
   }
 }
 
+// A part of a warp for a token: 32 lanes, or the least power of two that holds a row.
+// The parts take every gridDim-th token.
+constexpr int kRwThreads = 256;
+constexpr int kRwHold = 2;   // accesses of a row under way for a lane,
+constexpr int kRwRows = 4;   // of so many rows
+struct RwPart {
+  int64_t t, step;
+  int lane;
+};
+__device__ __forceinline__ RwPart rw_part(int lanes) {
+  const int parts = kRwThreads / lanes;
+  return {static_cast<int64_t>(blockIdx.x) * parts + threadIdx.x / lanes, static_cast<int64_t>(gridDim.x) * parts,
+          static_cast<int>(threadIdx.x) & (lanes - 1)};
+}
+// Slots and weights of up to kRwRows choices of a token from j0 on (past its last: no row).
+struct RwSlots {
+  int32_t s[kRwRows];
+  float w[kRwRows];
+};
+__device__ __forceinline__ RwSlots rw_slots(const RwArgs& q, int64_t t, int j0) {
+  RwSlots r;
+#pragma unroll
+  for (int j = 0; j < kRwRows; ++j) {
+    const bool in = t < q.tokens && j0 + j < q.k;
+    r.s[j] = in ? __ldg(q.slots + t * q.k + j0 + j) : -1;
+    r.w[j] = in && q.weights ? __ldg(q.weights + t * q.k + j0 + j) : 1.f;
+  }
+  return r;
+}
+
 template <typename T, int N>
-__global__ void __launch_bounds__(256) rw_combine(const RwArgs q) {
-  const int per = q.width / N;
-  const int64_t total = q.tokens * per, places = q.tokens * q.k;
+__global__ void __launch_bounds__(kRwThreads, 3) rw_combine(const RwArgs q, int lanes) {
+  const RwPart at = rw_part(lanes);
+  const int64_t places = q.tokens * q.k;
   const T* rows = static_cast<const T*>(q.rows);
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < total;
-       i += static_cast<int64_t>(gridDim.x) * 256) {
-    const int64_t t = i / per;
-    const int c = static_cast<int>(i - t * per) * N;
-    float z[N];
-    if (q.x) {
-      const RwVec<T, N> v = rw_load<T, N>(static_cast<const T*>(q.x) + t * q.x_ld + c);
+  const int span = lanes * N;
+  RwSlots ahead = rw_slots(q, at.t, 0);
+  for (int64_t t = at.t; t < q.tokens; t += at.step) {
+    const RwSlots first = ahead;
+    ahead = rw_slots(q, t + at.step, 0);
+    for (int c0 = at.lane * N; c0 < q.width; c0 += span * kRwHold) {
+      RwVec<T, N> r[kRwHold];
 #pragma unroll
-      for (int n = 0; n < N; ++n) z[n] = Elem<T>::to_f(v.v[n]);
-    } else {
+      for (int h = 0; h < kRwHold; ++h)
+        r[h] = q.x && c0 + h * span < q.width ? rw_load<T, N>(static_cast<const T*>(q.x) + t * q.x_ld + c0 + h * span)
+                                              : rw_zero<T, N>();
+      float z[kRwHold][N];
+      for (int j0 = 0; j0 < q.k; j0 += kRwRows) {
+        const RwSlots sl = j0 == 0 ? first : rw_slots(q, t, j0);
+        RwVec<T, N> v[kRwRows][kRwHold];
 #pragma unroll
-      for (int n = 0; n < N; ++n) z[n] = 0.f;
-    }
-    for (int j0 = 0; j0 < q.k; j0 += 4) {
-      RwVec<T, N> v[4];
-      float w[4];
-      bool in[4];
+        for (int j = 0; j < kRwRows; ++j)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int64_t s = j0 + j < q.k ? __ldg(q.slots + t * q.k + j0 + j) : -1;
-        in[j] = s >= 0 && s < places;
-        if (in[j]) {
-          v[j] = rw_load<T, N>(rows + s * q.rows_ld + c);
-          w[j] = q.weights ? __ldg(q.weights + t * q.k + j0 + j) : 1.f;
+          for (int h = 0; h < kRwHold; ++h)
+            v[j][h] = sl.s[j] >= 0 && sl.s[j] < places && c0 + h * span < q.width
+                          ? rw_load<T, N>(rows + static_cast<int64_t>(sl.s[j]) * q.rows_ld + c0 + h * span)
+                          : rw_zero<T, N>();
+        if (j0 == 0) {
+#pragma unroll
+          for (int h = 0; h < kRwHold; ++h)
+#pragma unroll
+            for (int n = 0; n < N; ++n) z[h][n] = rw_get(r[h], n);
         }
+#pragma unroll
+        for (int j = 0; j < kRwRows; ++j)
+          if (sl.s[j] >= 0 && sl.s[j] < places) {  // (its weight may be infinite where there is no row)
+#pragma unroll
+            for (int h = 0; h < kRwHold; ++h)
+#pragma unroll
+              for (int n = 0; n < N; ++n) z[h][n] = fmaf(sl.w[j], rw_get(v[j][h], n), z[h][n]);
+          }
       }
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (in[j]) {
-#pragma unroll
-          for (int n = 0; n < N; ++n) z[n] = fmaf(w[j], Elem<T>::to_f(v[j].v[n]), z[n]);
-        }
+      for (int h = 0; h < kRwHold; ++h) {
+        if (c0 + h * span < q.width)
+          rw_store<T, N>(static_cast<T*>(q.out) + t * q.width + c0 + h * span, rw_pack<T, N>(z[h]));
+      }
     }
-    RwVec<T, N> o;
-#pragma unroll
-    for (int n = 0; n < N; ++n) o.v[n] = Elem<T>::from_f(z[n]);
-    rw_store<T, N>(static_cast<T*>(q.out) + t * q.width + c, o);
   }
 }
 
-// combine's backward: a warp takes a token; drows[slot_tj] = w_tj dout_t (q.out: drows, contiguous)
-// and dw_tj = <dout_t, rows[slot_tj]>. Lane j keeps the j-th sum.
-constexpr int kRwWarps = 8;
+// combine's backward: drows[slot_tj] = w_tj dout_t (q.out: drows, contiguous) and dw_tj =
+// <dout_t, rows[slot_tj]>.
 template <typename T, int N>
-__global__ void __launch_bounds__(32 * kRwWarps) rw_combine_backward(const RwArgs q) {
-  const int lane = threadIdx.x & 31;
-  const int64_t t = static_cast<int64_t>(blockIdx.x) * kRwWarps + (threadIdx.x >> 5);
-  if (t >= q.tokens) return;
-  constexpr int kHold = 16 / (N * static_cast<int>(sizeof(T)) >= 16 ? 4 : N * static_cast<int>(sizeof(T)) >= 8 ? 2 : 1);
+__global__ void __launch_bounds__(kRwThreads, 3) rw_combine_backward(const RwArgs q, int lanes) {
+  const RwPart at = rw_part(lanes);
+  const unsigned mask = lanes == 32 ? 0xFFFFFFFFu : ((1u << lanes) - 1) << (threadIdx.x & 31 & ~(lanes - 1));
   const int64_t places = q.tokens * q.k;
-  const T* dout = static_cast<const T*>(q.x) + t * q.x_ld;
-  const int64_t my_slot = lane < q.k ? __ldg(q.slots + t * q.k + lane) : -1;
-  const float my_weight = lane < q.k ? __ldg(q.weights + t * q.k + lane) : 0.f;
-  float dw = 0.f;
-  for (int c0 = 0; c0 < q.width; c0 += 32 * N * kHold) {
-    RwVec<T, N> d[kHold];
+  const T* rows = static_cast<const T*>(q.rows);
+  const int span = lanes * N;
+  RwSlots ahead = rw_slots(q, at.t, 0);
+  for (int64_t t = at.t; t < q.tokens; t += at.step) {
+    const T* dout = static_cast<const T*>(q.x) + t * q.x_ld;
+    const RwSlots first = ahead;
+    ahead = rw_slots(q, t + at.step, 0);
+    for (int j0 = 0; j0 < q.k; j0 += kRwRows) {
+      const RwSlots sl = j0 == 0 ? first : rw_slots(q, t, j0);
+      float sum[kRwRows] = {};
+      for (int c0 = at.lane * N; c0 < q.width; c0 += span * kRwHold) {
+        RwVec<T, N> d[kRwHold], v[kRwRows][kRwHold];
 #pragma unroll
-    for (int h = 0; h < kHold; ++h) {
-      const int c = c0 + (h * 32 + lane) * N;
-      if (c < q.width) d[h] = rw_load<T, N>(dout + c);
-    }
-    for (int j = 0; j < q.k; ++j) {
-      const int64_t s = __shfl_sync(0xFFFFFFFFu, my_slot, j);
-      const float w = __shfl_sync(0xFFFFFFFFu, my_weight, j);
-      if (s < 0 || s >= places) continue;
-      if (q.out) {
-        T* o = static_cast<T*>(q.out) + s * q.width;
+        for (int h = 0; h < kRwHold; ++h)
+          d[h] = c0 + h * span < q.width ? rw_load<T, N>(dout + c0 + h * span) : rw_zero<T, N>();
 #pragma unroll
-        for (int h = 0; h < kHold; ++h) {
-          const int c = c0 + (h * 32 + lane) * N;
-          if (c >= q.width) continue;
-          RwVec<T, N> y;
+        for (int j = 0; j < kRwRows; ++j)
 #pragma unroll
-          for (int n = 0; n < N; ++n) y.v[n] = Elem<T>::from_f(w * Elem<T>::to_f(d[h].v[n]));
-          rw_store<T, N>(o + c, y);
+          for (int h = 0; h < kRwHold; ++h)
+            v[j][h] = q.dweights && sl.s[j] >= 0 && sl.s[j] < places && c0 + h * span < q.width
+                          ? rw_load<T, N>(rows + static_cast<int64_t>(sl.s[j]) * q.rows_ld + c0 + h * span)
+                          : rw_zero<T, N>();
+#pragma unroll
+        for (int j = 0; j < kRwRows; ++j) {
+          if (sl.s[j] < 0 || sl.s[j] >= places) continue;
+#pragma unroll
+          for (int h = 0; h < kRwHold; ++h) {
+            if (q.out && c0 + h * span < q.width) {
+              float y[N];
+#pragma unroll
+              for (int n = 0; n < N; ++n) y[n] = sl.w[j] * rw_get(d[h], n);
+              rw_store<T, N>(static_cast<T*>(q.out) + static_cast<int64_t>(sl.s[j]) * q.width + c0 + h * span,
+                             rw_pack<T, N>(y));
+            }
+            if (c0 + h * span < q.width) {
+#pragma unroll
+              for (int n = 0; n < N; ++n) sum[j] = fmaf(rw_get(d[h], n), rw_get(v[j][h], n), sum[j]);
+            }
+          }
         }
       }
       if (q.dweights) {
-        const T* r = static_cast<const T*>(q.rows) + s * q.rows_ld;
-        RwVec<T, N> v[kHold];
 #pragma unroll
-        for (int h = 0; h < kHold; ++h) {
-          const int c = c0 + (h * 32 + lane) * N;
-          if (c < q.width) v[h] = rw_load<T, N>(r + c);
+        for (int j = 0; j < kRwRows; ++j) {
+          for (int m = lanes / 2; m; m >>= 1) sum[j] += __shfl_xor_sync(mask, sum[j], m);
+          if (at.lane == 0 && j0 + j < q.k) q.dweights[t * q.k + j0 + j] = sum[j];
         }
-        float sum = 0.f;
-#pragma unroll
-        for (int h = 0; h < kHold; ++h) {
-          const int c = c0 + (h * 32 + lane) * N;
-          if (c >= q.width) continue;
-#pragma unroll
-          for (int n = 0; n < N; ++n) sum = fmaf(Elem<T>::to_f(d[h].v[n]), Elem<T>::to_f(v[h].v[n]), sum);
-        }
-#pragma unroll
-        for (int m = 16; m; m >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, m);
-        if (lane == j) dw += sum;
       }
     }
   }
-  if (q.dweights && lane < q.k) q.dweights[t * q.k + lane] = dw;
 }
 
 // ---------------------------------------------------------------- embedding
@@ -197,33 +282,39 @@ struct EmArgs {
   const uint32_t* ids;
   const uint8_t* seen;    // [vocab]
   float* parts;           // [chunks][2][width]
+  uint32_t* edges;        // chunks where a run begins that goes on: their number, zero before, and they
   int64_t chunks;
   void* dtable;           // [vocab], contiguous
 };
 
-// A token outside the vocabulary gives a row of NaN.
+// A token outside the vocabulary gives a row of NaN. A part of a warp takes a row.
 template <typename T, int N>
-__global__ void __launch_bounds__(256) em_forward(const EmArgs q) {
-  const int per = q.width / N;
-  const int64_t total = q.n * per;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < total;
-       i += static_cast<int64_t>(gridDim.x) * 256) {
-    const int64_t r = i / per;
-    const int c = static_cast<int>(i - r * per) * N;
-    const int64_t t = q.tokens64 ? __ldg(static_cast<const long long*>(q.tokens) + r)
-                                 : static_cast<int64_t>(__ldg(static_cast<const int32_t*>(q.tokens) + r));
-    RwVec<T, N> v;
-    if (t >= 0 && t < q.vocab) {
-      v = rw_load<T, N>(static_cast<const T*>(q.table) + t * q.table_ld + c);
-      if (q.scale != 1.f) {
+__global__ void __launch_bounds__(kRwThreads) em_forward(const EmArgs q, int lanes) {
+  const RwPart at = rw_part(lanes);
+  if (at.t >= q.n) return;
+  const int64_t t = q.tokens64 ? __ldg(static_cast<const long long*>(q.tokens) + at.t)
+                               : static_cast<int64_t>(__ldg(static_cast<const int32_t*>(q.tokens) + at.t));
+  const bool in = t >= 0 && t < q.vocab;
+  const T* row = static_cast<const T*>(q.table) + t * q.table_ld;
+  T* out = static_cast<T*>(q.out) + at.t * q.width;
+  const int span = lanes * N;
+  constexpr int kHold = 4;
+  for (int c0 = at.lane * N; c0 < q.width; c0 += span * kHold) {
+    RwVec<T, N> v[kHold];
 #pragma unroll
-        for (int n = 0; n < N; ++n) v.v[n] = Elem<T>::from_f(Elem<T>::to_f(v.v[n]) * q.scale);
+    for (int h = 0; h < kHold; ++h)
+      v[h] = in && c0 + h * span < q.width ? rw_load<T, N>(row + c0 + h * span) : rw_zero<T, N>();
+#pragma unroll
+    for (int h = 0; h < kHold; ++h) {
+      if (c0 + h * span >= q.width) continue;
+      if (!in || q.scale != 1.f) {
+        float z[N];
+#pragma unroll
+        for (int n = 0; n < N; ++n) z[n] = in ? rw_get(v[h], n) * q.scale : CUDART_NAN_F;
+        v[h] = rw_pack<T, N>(z);
       }
-    } else {
-#pragma unroll
-      for (int n = 0; n < N; ++n) v.v[n] = Elem<T>::from_f(CUDART_NAN_F);
+      rw_store<T, N>(out + c0 + h * span, v[h]);
     }
-    rw_store<T, N>(static_cast<T*>(q.out) + r * q.width + c, v);
   }
 }
 
@@ -231,18 +322,19 @@ __global__ void __launch_bounds__(256) em_forward(const EmArgs q) {
 // and adds up the rows of each run of one token. A run inside the block's places is
 // finished there; the parts of one that goes over their edge are kept: slot 0 of a
 // chunk for the run that comes in, slot 1 for one that begins there and goes on. (A frequent
-// token's rows are so shared by many blocks.) em_finish adds the parts up. Blocks past the
-// chunks write the zeros of tokens that do not occur.
+// token's rows are so shared by many blocks.) em_finish adds the parts up: of the runs that
+// em_sum lists, whose order does not matter. Blocks past the chunks write the zeros of
+// tokens that do not occur.
 constexpr int kEmChunk = 32;
 constexpr int kEmAhead = 8;  // rows under way for each thread
 constexpr int kEmZeroRows = 32;
 
 template <typename T, int N>
 __device__ __forceinline__ void em_put(const EmArgs& q, uint32_t token, int c, const float (&z)[N]) {
-  RwVec<T, N> o;
+  float y[N];
 #pragma unroll
-  for (int n = 0; n < N; ++n) o.v[n] = Elem<T>::from_f(z[n] * q.scale);
-  rw_store<T, N>(static_cast<T*>(q.dtable) + static_cast<int64_t>(token) * q.width + c, o);
+  for (int n = 0; n < N; ++n) y[n] = z[n] * q.scale;
+  rw_store<T, N>(static_cast<T*>(q.dtable) + static_cast<int64_t>(token) * q.width + c, rw_pack<T, N>(y));
 }
 
 template <typename T, int N>
@@ -253,11 +345,11 @@ __global__ void __launch_bounds__(256) em_sum(const EmArgs q) {
   const int threads = blockDim.x;
   if (blockIdx.x >= q.chunks) {
     const int64_t r0 = (blockIdx.x - q.chunks) * kEmZeroRows;
-    RwVec<T, N> zero;
-#pragma unroll
-    for (int n = 0; n < N; ++n) zero.v[n] = Elem<T>::from_f(0.f);
+    const RwVec<T, N> zero = rw_zero<T, N>();
+    const int64_t mine = r0 + (threadIdx.x & 31);
+    const unsigned seen = __ballot_sync(0xFFFFFFFFu, mine < q.vocab && q.seen[mine]);
     for (int64_t r = r0; r < min(r0 + kEmZeroRows, q.vocab); ++r) {
-      if (q.seen[r]) continue;
+      if (seen >> (r - r0) & 1u) continue;
       for (int c = threadIdx.x * N; c < q.width; c += threads * N)
         rw_store<T, N>(static_cast<T*>(q.dtable) + r * q.width + c, zero);
     }
@@ -271,6 +363,9 @@ __global__ void __launch_bounds__(256) em_sum(const EmArgs q) {
   }
   __syncthreads();
   const bool enters = p0 > 0 && __ldg(q.keys + p0 - 1) == keys[0];
+  if (threadIdx.x == 0 && here == kEmChunk && keys[here] == keys[here - 1] && keys[here] < q.vocab &&
+      !(enters && keys[0] == keys[here]))
+    q.edges[1 + atomicAdd(q.edges, 1u)] = blockIdx.x;
   for (int c = threadIdx.x * N; c < q.width; c += threads * N) {
     float z[N];
 #pragma unroll
@@ -280,14 +375,15 @@ __global__ void __launch_bounds__(256) em_sum(const EmArgs q) {
       RwVec<T, N> v[kEmAhead];
 #pragma unroll
       for (int j = 0; j < kEmAhead; ++j)
-        if (i0 + j < here && keys[i0 + j] < q.vocab)
-          v[j] = rw_load<T, N>(static_cast<const T*>(q.dy) + static_cast<int64_t>(ids[i0 + j]) * q.dy_ld + c);
+        v[j] = i0 + j < here && keys[i0 + j] < q.vocab
+                   ? rw_load<T, N>(static_cast<const T*>(q.dy) + static_cast<int64_t>(ids[i0 + j]) * q.dy_ld + c)
+                   : rw_zero<T, N>();
 #pragma unroll
       for (int j = 0; j < kEmAhead; ++j) {
         const int i = i0 + j;
         if (i >= here || keys[i] >= q.vocab) continue;
 #pragma unroll
-        for (int n = 0; n < N; ++n) z[n] += Elem<T>::to_f(v[j].v[n]);
+        for (int n = 0; n < N; ++n) z[n] += rw_get(v[j], n);
         const bool on = i + 1 == here && keys[here] == keys[i];  // the run goes on in the next chunk
         if (keys[i + 1] != keys[i] || on) {
           if (!came && !on) {
@@ -306,47 +402,59 @@ __global__ void __launch_bounds__(256) em_sum(const EmArgs q) {
   }
 }
 
-// The runs that go over a chunk's edge: the block of the chunk where one begins adds its
-// parts up, eight groups of threads a share of the chunks each, then the groups in turn.
-constexpr int kEmGroups = 8, kEmCols = 32;
-template <typename T>
-__global__ void __launch_bounds__(kEmGroups * kEmCols) em_finish(const EmArgs q) {
-  __shared__ float sums[kEmGroups][kEmCols];
-  __shared__ int64_t end;
+// The runs that go over a chunk's edge. A block takes a run and 64 V of its columns: four
+// groups of threads a share of its chunks each, then the groups in turn.
+constexpr int kEmGroups = 4, kEmLanes = 64;
+template <typename T, int V>
+__global__ void __launch_bounds__(kEmGroups * kEmLanes) em_finish(const EmArgs q, int slabs) {
+  __shared__ float sums[kEmGroups][kEmLanes * V];
+  __shared__ int64_t last;
   griddep_wait();
-  const int64_t b = blockIdx.x, p0 = b * kEmChunk, next = p0 + kEmChunk;
-  if (next >= q.n) return;
-  const uint32_t token = __ldg(q.keys + next);
-  if (token >= q.vocab || __ldg(q.keys + next - 1) != token) return;  // no run over this edge
-  if (__ldg(q.keys + p0) == token && p0 > 0 && __ldg(q.keys + p0 - 1) == token) return;  // it began before
-  // The first chunk after b that the run does not reach.
-  if (threadIdx.x == 0) {
-    int64_t lo = b + 1, hi = q.chunks;
-    while (lo < hi) {
-      const int64_t mid = (lo + hi) / 2;
-      if (__ldg(q.keys + mid * kEmChunk) == token) lo = mid + 1;
-      else hi = mid;
+  const int g = threadIdx.x / kEmLanes, l = threadIdx.x % kEmLanes;
+  const int64_t items = static_cast<int64_t>(*q.edges) * slabs;
+  for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+    const int64_t b = q.edges[1 + item / slabs];
+    const uint32_t token = __ldg(q.keys + b * kEmChunk + kEmChunk);
+    // The last chunk that the run reaches: looked at 256 at a time.
+    if (threadIdx.x == 0) last = b;
+    __syncthreads();
+    for (int64_t c0 = b + 1;; c0 += kEmGroups * kEmLanes) {
+      const int64_t c = c0 + threadIdx.x;
+      const bool in = c < q.chunks && __ldg(q.keys + c * kEmChunk) == token;
+      const int n = __syncthreads_count(in);
+      if (threadIdx.x == 0) last = c0 - 1 + n;
+      if (n < kEmGroups * kEmLanes) break;
     }
-    end = lo;
-  }
-  __syncthreads();
-  const int g = threadIdx.x / kEmCols, l = threadIdx.x % kEmCols;
-  const int64_t count = end - (b + 1), share = (count + kEmGroups - 1) / kEmGroups;
-  const int64_t c0 = b + 1 + g * share, c1 = min(end, c0 + share);
-  for (int col0 = blockIdx.y * kEmCols; col0 < q.width; col0 += gridDim.y * kEmCols) {
-    const int col = col0 + l;
-    float z = 0.f;
+    __syncthreads();
+    const int64_t count = last - b, share = (count + kEmGroups - 1) / kEmGroups;
+    const int64_t c0 = b + 1 + g * share, c1 = min(last + 1, c0 + share);
+    const int col = static_cast<int>(item % slabs) * kEmLanes * V + l * V;
+    float z[V];
+#pragma unroll
+    for (int n = 0; n < V; ++n) z[n] = 0.f;
     if (col < q.width) {
-      if (g == 0) z = __ldcg(q.parts + (b * 2 + 1) * q.width + col);
+      if (g == 0) {
+        const RwVec<float, V> v = rw_load<float, V>(q.parts + (b * 2 + 1) * q.width + col);
+#pragma unroll
+        for (int n = 0; n < V; ++n) z[n] = rw_get(v, n);
+      }
 #pragma unroll 8
-      for (int64_t c = c0; c < c1; ++c) z += __ldcg(q.parts + c * 2 * q.width + col);
+      for (int64_t c = c0; c < c1; ++c) {
+        const RwVec<float, V> v = rw_load<float, V>(q.parts + c * 2 * q.width + col);
+#pragma unroll
+        for (int n = 0; n < V; ++n) z[n] += rw_get(v, n);
+      }
     }
-    sums[g][l] = z;
+#pragma unroll
+    for (int n = 0; n < V; ++n) sums[g][l * V + n] = z[n];
     __syncthreads();
     if (g == 0 && col < q.width) {
 #pragma unroll
-      for (int j = 1; j < kEmGroups; ++j) z += sums[j][l];
-      static_cast<T*>(q.dtable)[static_cast<int64_t>(token) * q.width + col] = Elem<T>::from_f(z * q.scale);
+      for (int n = 0; n < V; ++n) {
+#pragma unroll
+        for (int j = 1; j < kEmGroups; ++j) z[n] += sums[j][l * V + n];
+        static_cast<T*>(q.dtable)[static_cast<int64_t>(token) * q.width + col + n] = Elem<T>::from_f(z[n] * q.scale);
+      }
     }
     __syncthreads();
   }

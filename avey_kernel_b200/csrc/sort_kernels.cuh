@@ -5,19 +5,23 @@
 // Blocks take consecutive runs of the entries, warps consecutive parts of a run: so an
 // entry's place is the number of entries with a lower digit, of those with its own in
 // earlier blocks and warps, and of those before it in its warp (found 32 at a time by
-// matching digits over the warp). No atomics but on counts, whose order does not matter:
-// the same input gives the same order. Up to 4096 entries one block does it all; more
-// take a launch that counts and one that places.
+// matching digits over the warp). No atomics: the same input gives the same order. Up to
+// 8192 entries one block does it all; more take a launch that counts and one that places.
+//
+// Bound: latency, of a few dependent reads a launch: so a warp's keys are loaded eight
+// steps at a time, and the counts of all blocks 16 at a time.
 #pragma once
 
 #include "ptx.cuh"
 
 namespace avey {
 
-constexpr int kStWarps = 8, kStThreads = 32 * kStWarps;
+constexpr int kStWarps = 16, kStThreads = 32 * kStWarps;
 constexpr int kStMaxBuckets = 1025;
-constexpr int kStRun = 2048;       // entries of a block at least
-constexpr int kStOneBlock = 4096;  // entries that one block takes
+constexpr int kStRun = 4096;       // entries of a block at least
+constexpr int kStOneBlock = 8192;  // entries that one block takes
+constexpr int kStSteps = 8;        // keys a lane holds
+constexpr int kStSmem = (kStWarps + 1) * kStMaxBuckets * 4;
 
 struct StArgs {
   int64_t n;
@@ -49,22 +53,44 @@ __device__ __forceinline__ uint32_t st_digit(const StArgs& q, uint32_t key) {
   return (key >> q.shift) & static_cast<uint32_t>(q.mask);
 }
 
+// A warp's part of a block's entries [lo, hi): whole steps of 32.
+struct StPart {
+  int64_t w0, w1;
+};
+__device__ __forceinline__ StPart st_part(int64_t lo, int64_t hi) {
+  const int64_t part = (hi - lo + kStThreads - 1) / kStThreads * 32;
+  const int64_t w0 = min(hi, lo + (threadIdx.x >> 5) * part);
+  return {w0, min(hi, w0 + part)};
+}
+// Eight steps' keys from i0 on (past the end: none).
+__device__ __forceinline__ void st_keys(const StArgs& q, int64_t i0, int64_t w1, uint32_t (&key)[kStSteps]) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int s = 0; s < kStSteps; ++s) {
+    const int64_t i = i0 + 32 * s + lane;
+    key[s] = i < w1 ? st_key(q, i) : 0xFFFFFFFFu;
+  }
+}
+
 // The digits of a block's entries, counted for each warp: hist [warps][buckets].
-__device__ __forceinline__ void st_count_block(const StArgs& q, uint32_t* hist, int64_t lo, int64_t hi) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+__device__ __forceinline__ void st_count_block(const StArgs& q, uint32_t* hist, const StPart& part) {
+  const int lane = threadIdx.x & 31;
   for (int i = threadIdx.x; i < kStWarps * q.buckets; i += kStThreads) hist[i] = 0;
   __syncthreads();
-  const int64_t part = (hi - lo + kStWarps * 32 - 1) / (kStWarps * 32) * 32;
-  const int64_t w0 = lo + warp * part, w1 = min(hi, w0 + part);
-  uint32_t* mine = hist + warp * q.buckets;
-  for (int64_t i = w0; i < w1; i += 32) {
-    const bool in = i + lane < w1;
-    const uint32_t key = in ? st_key(q, i + lane) : 0u;
-    const uint32_t d = in ? st_digit(q, key) : 0xFFFFFFFFu;
-    if (in && q.seen) q.seen[key] = 1;
-    const unsigned peers = __match_any_sync(0xFFFFFFFFu, d);
-    if (in && (peers & ((1u << lane) - 1)) == 0) mine[d] += __popc(peers);
-    __syncwarp();
+  uint32_t* mine = hist + (threadIdx.x >> 5) * q.buckets;
+  for (int64_t i0 = part.w0; i0 < part.w1; i0 += 32 * kStSteps) {
+    uint32_t key[kStSteps];
+    st_keys(q, i0, part.w1, key);
+#pragma unroll
+    for (int s = 0; s < kStSteps; ++s) {
+      if (i0 + 32 * s >= part.w1) break;
+      const bool in = key[s] != 0xFFFFFFFFu;
+      const uint32_t d = in ? st_digit(q, key[s]) : 0xFFFFFFFFu;
+      if (in && q.seen) q.seen[key[s]] = 1;
+      const unsigned peers = __match_any_sync(0xFFFFFFFFu, d);
+      if (in && (peers & ((1u << lane) - 1)) == 0) mine[d] += __popc(peers);
+      __syncwarp();
+    }
   }
   __syncthreads();
 }
@@ -74,7 +100,7 @@ __global__ void __launch_bounds__(kStThreads) st_count(const StArgs q) {
   griddep_launch_dependents();
   griddep_wait();
   const int64_t lo = blockIdx.x * q.run, hi = min(q.n, lo + q.run);
-  st_count_block(q, hist, lo, hi);
+  st_count_block(q, hist, st_part(lo, hi));
   for (int d = threadIdx.x; d < q.buckets; d += kStThreads) {
     uint32_t sum = 0;
 #pragma unroll
@@ -88,31 +114,47 @@ __global__ void __launch_bounds__(kStThreads) st_place(const StArgs q) {
   __shared__ uint32_t warp_sums[kStWarps];
   griddep_launch_dependents();
   griddep_wait();
-  uint32_t* start = hist + kStWarps * q.buckets;
+  uint32_t* totals = hist + kStWarps * q.buckets;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int64_t lo = blockIdx.x * q.run, hi = min(q.n, lo + q.run);
-  st_count_block(q, hist, lo, hi);
-  // Entries with a lower digit: an exclusive sum over the digits' totals, `per`
-  // consecutive digits a thread.
+  const StPart part = st_part(lo, hi);
+  st_count_block(q, hist, part);
+  // The digits' totals, and how many of them are in earlier blocks.
   constexpr int kPer = (kStMaxBuckets + kStThreads - 1) / kStThreads;
-  uint32_t total[kPer], before[kPer], sum = 0;
+  uint32_t before[kPer];
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) {
+    const int d = j * kStThreads + tid;
+    before[j] = 0;
+    if (d >= q.buckets) continue;
+    uint32_t total = 0;
+    if (q.blocks > 1) {
+      const uint32_t* c = q.counts + d;
+      for (int b0 = 0; b0 < q.blocks; b0 += 16) {
+        uint32_t v[16];
+#pragma unroll
+        for (int b = 0; b < 16; ++b)
+          v[b] = b0 + b < q.blocks ? __ldcg(c + static_cast<int64_t>(b0 + b) * q.buckets) : 0u;
+#pragma unroll
+        for (int b = 0; b < 16; ++b) {
+          total += v[b];
+          if (b0 + b < static_cast<int>(blockIdx.x)) before[j] += v[b];
+        }
+      }
+    } else {
+#pragma unroll
+      for (int w = 0; w < kStWarps; ++w) total += hist[w * q.buckets + d];
+    }
+    totals[d] = total;
+  }
+  __syncthreads();
+  // Entries with a lower digit: an exclusive sum, kPer consecutive digits a thread.
+  uint32_t mine[kPer], sum = 0;
 #pragma unroll
   for (int j = 0; j < kPer; ++j) {
     const int d = tid * kPer + j;
-    total[j] = before[j] = 0;
-    if (d >= q.buckets) continue;
-    if (q.blocks > 1) {
-      const uint32_t* c = q.counts + d;
-#pragma unroll 8
-      for (int b = 0; b < q.blocks; ++b) {
-        const uint32_t v = __ldcg(c + static_cast<int64_t>(b) * q.buckets);
-        total[j] += v;
-        if (b < static_cast<int>(blockIdx.x)) before[j] += v;
-      }
-    } else {
-      for (int w = 0; w < kStWarps; ++w) total[j] += hist[w * q.buckets + d];
-    }
-    sum += total[j];
+    mine[j] = d < q.buckets ? totals[d] : 0u;
+    sum += mine[j];
   }
   uint32_t incl = sum;
 #pragma unroll
@@ -128,14 +170,17 @@ __global__ void __launch_bounds__(kStThreads) st_place(const StArgs q) {
   for (int j = 0; j < kPer; ++j) {
     const int d = tid * kPer + j;
     if (d >= q.buckets) continue;
-    start[d] = at + before[j];
+    totals[d] = at;
     if (q.offsets && blockIdx.x == 0) q.offsets[d] = static_cast<int32_t>(at);
-    at += total[j];
+    at += mine[j];
   }
   __syncthreads();
   // The first place of each warp's entries of each digit.
-  for (int d = tid; d < q.buckets; d += kStThreads) {
-    uint32_t p = start[d];
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) {
+    const int d = j * kStThreads + tid;
+    if (d >= q.buckets) continue;
+    uint32_t p = totals[d] + before[j];
 #pragma unroll
     for (int w = 0; w < kStWarps; ++w) {
       const uint32_t c = hist[w * q.buckets + d];
@@ -144,26 +189,34 @@ __global__ void __launch_bounds__(kStThreads) st_place(const StArgs q) {
     }
   }
   __syncthreads();
-  const int64_t part = (hi - lo + kStWarps * 32 - 1) / (kStWarps * 32) * 32;
-  const int64_t w0 = lo + warp * part, w1 = min(hi, w0 + part);
-  uint32_t* mine = hist + warp * q.buckets;
-  for (int64_t i = w0; i < w1; i += 32) {
-    const bool in = i + lane < w1;
-    const uint32_t key = in ? st_key(q, i + lane) : 0u;
-    const uint32_t d = in ? st_digit(q, key) : 0xFFFFFFFFu;
-    const unsigned peers = __match_any_sync(0xFFFFFFFFu, d);
-    const unsigned lower = peers & ((1u << lane) - 1);
-    uint32_t p = 0;
-    if (in) p = mine[d] + __popc(lower);
-    __syncwarp();
-    if (in && lower == 0) mine[d] += __popc(peers);
-    __syncwarp();
-    if (!in) continue;
-    if (q.slots) {
-      q.slots[i + lane] = static_cast<int32_t>(p);
-    } else {
-      q.keys_out[p] = key;
-      q.ids_out[p] = q.ids ? __ldg(q.ids + i + lane) : static_cast<uint32_t>(i + lane);
+  uint32_t* place = hist + warp * q.buckets;
+  for (int64_t i0 = part.w0; i0 < part.w1; i0 += 32 * kStSteps) {
+    uint32_t key[kStSteps], id[kStSteps];
+    st_keys(q, i0, part.w1, key);
+#pragma unroll
+    for (int s = 0; s < kStSteps; ++s) {
+      const int64_t i = i0 + 32 * s + lane;
+      id[s] = q.ids && i < part.w1 ? __ldg(q.ids + i) : static_cast<uint32_t>(i);
+    }
+#pragma unroll
+    for (int s = 0; s < kStSteps; ++s) {
+      if (i0 + 32 * s >= part.w1) break;
+      const bool in = key[s] != 0xFFFFFFFFu;
+      const uint32_t d = in ? st_digit(q, key[s]) : 0xFFFFFFFFu;
+      const unsigned peers = __match_any_sync(0xFFFFFFFFu, d);
+      const unsigned lower = peers & ((1u << lane) - 1);
+      uint32_t p = 0;
+      if (in) p = place[d] + __popc(lower);
+      __syncwarp();
+      if (in && lower == 0) place[d] += __popc(peers);
+      __syncwarp();
+      if (!in) continue;
+      if (q.slots) {
+        q.slots[i0 + 32 * s + lane] = static_cast<int32_t>(p);
+      } else {
+        q.keys_out[p] = key[s];
+        q.ids_out[p] = id[s];
+      }
     }
   }
 }

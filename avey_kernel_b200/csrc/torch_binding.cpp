@@ -606,6 +606,7 @@ class RouteFunction : public torch::autograd::Function<RouteFunction> {
     auto [weights, chosen] = route_forward(logits, bias, call);
     ctx->save_for_backward({logits, weights, chosen});
     ctx->mark_non_differentiable({chosen});
+    ctx->set_materialize_grads(false);
     ctx->saved_data["call"] = std::vector<int64_t>{k, score, groups, top_groups, group_best, renormalize};
     ctx->saved_data["scale"] = scale;
     return {weights, chosen};
