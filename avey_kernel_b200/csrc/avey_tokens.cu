@@ -152,17 +152,18 @@ int sort_opt_in() {
   return err[dev] == cudaSuccess ? AVEY_OK : fail(AVEY_ERR_CUDA, cudaGetErrorString(err[dev]));
 }
 
-int launch_pass(avey::StArgs& q, Chain& chain) {
+// `counted`: the pass before has counted for this one; `zero_blocks` more write zeros.
+int launch_pass(avey::StArgs& q, Chain& chain, bool counted = false, int zero_blocks = 0) {
   const int opted = sort_opt_in();
   if (opted != AVEY_OK) return opted;
   q.run = std::max<int64_t>(1, sort_run(q.n));
   q.blocks = static_cast<int>(sort_blocks(q.n));
   const int smem = avey::kStWarps * q.buckets * 4;
-  if (q.blocks > 1) {
+  if (q.blocks > 1 && !counted) {
     const int rc = chain.launch("sort counts", avey::st_count, dim3(q.blocks), avey::kStThreads, smem, 1, q);
     if (rc != AVEY_OK) return rc;
   }
-  return chain.launch("sort", avey::st_place, dim3(q.blocks), avey::kStThreads, smem + q.buckets * 4, 1, q);
+  return chain.launch("sort", avey::st_place, dim3(q.blocks + zero_blocks), avey::kStThreads, smem + q.buckets * 4, 1, q);
 }
 
 int validate(const AveyArrangeParams* p) {
@@ -312,7 +313,7 @@ avey::EmArgs embedding_args(const AveyEmbeddingParams* p) {
 // Workspace of the backward call: [keys, ids] twice, counts, edges, tokens seen, parts.
 struct EmLayout {
   int passes = 0;
-  uint64_t keys[2] = {}, ids[2] = {}, counts = 0, edges = 0, seen = 0, parts = 0, total = 0;
+  uint64_t keys[2] = {}, ids[2] = {}, counts[2] = {}, edges = 0, seen = 0, parts = 0, total = 0;
 };
 EmLayout embedding_layout(const AveyEmbeddingParams* p) {
   EmLayout l;
@@ -330,7 +331,9 @@ EmLayout embedding_layout(const AveyEmbeddingParams* p) {
     l.keys[i] = take(p->count * 4);
     l.ids[i] = take(p->count * 4);
   }
-  l.counts = take(count_bytes(p->count, 1024));
+  l.counts[0] = take(count_bytes(p->count, 1024));
+  // From here on zero before the first launch, up to `parts`.
+  l.counts[1] = take(count_bytes(p->count, 1024) * (l.passes - 1));
   const uint64_t chunks = (p->count + avey::kEmChunk - 1) / avey::kEmChunk;
   l.edges = take((1 + chunks) * 4);
   l.seen = take(p->vocab + 1);
@@ -342,9 +345,7 @@ EmLayout embedding_layout(const AveyEmbeddingParams* p) {
 template <typename T, int N>
 int launch_sums(const avey::EmArgs& q, Chain& chain) {
   const int threads = static_cast<int>(std::min<int64_t>(256, (q.width / N + 31) / 32 * 32));
-  const int64_t zeros = (q.vocab + avey::kEmZeroRows - 1) / avey::kEmZeroRows;
-  int rc = chain.launch("embedding sums", avey::em_sum<T, N>, dim3(static_cast<unsigned>(q.chunks + zeros)), threads, 0,
-                        1, q);
+  int rc = chain.launch("embedding sums", avey::em_sum<T, N>, dim3(static_cast<unsigned>(q.chunks)), threads, 0, 1, q);
   if (rc != AVEY_OK || q.chunks < 2) return rc;
   constexpr int V = N > 1 && sizeof(T) * N == 16 ? 4 : 1;  // width is a multiple of 4
   const int slabs = (q.width + avey::kEmLanes * V - 1) / (avey::kEmLanes * V);
@@ -365,7 +366,7 @@ int embedding_backward(const AveyEmbeddingParams* p, cudaStream_t stream) {
   if (rc != AVEY_OK) return rc;
   char* ws = static_cast<char*>(p->workspace);
   uint8_t* seen = reinterpret_cast<uint8_t*>(ws + l.seen);
-  const cudaError_t e = cudaMemsetAsync(ws + l.edges, 0, l.parts - l.edges, stream);
+  const cudaError_t e = cudaMemsetAsync(ws + l.counts[1], 0, l.parts - l.counts[1], stream);
   if (e != cudaSuccess) return fail(AVEY_ERR_CUDA, cudaGetErrorString(e));
   Chain chain{stream};
   for (int pass = 0; pass < l.passes; ++pass) {
@@ -384,16 +385,43 @@ int embedding_backward(const AveyEmbeddingParams* p, cudaStream_t stream) {
       q.keys = reinterpret_cast<uint32_t*>(ws + l.keys[(pass - 1) & 1]);
       q.ids = reinterpret_cast<uint32_t*>(ws + l.ids[(pass - 1) & 1]);
     }
-    q.counts = reinterpret_cast<uint32_t*>(ws + l.counts);
+    const uint64_t pass_bytes = count_bytes(p->count, 1024);
+    const bool many = pass_bytes > 0;  // blocks
+    q.counts = reinterpret_cast<uint32_t*>(pass == 0 ? ws + l.counts[0] : ws + l.counts[1] + (pass - 1) * pass_bytes);
+    if (many && pass + 1 < l.passes) q.next_counts = reinterpret_cast<uint32_t*>(ws + l.counts[1] + pass * pass_bytes);
     q.keys_out = reinterpret_cast<uint32_t*>(ws + l.keys[pass & 1]);
     q.ids_out = reinterpret_cast<uint32_t*>(ws + l.ids[pass & 1]);
-    rc = launch_pass(q, chain);
+    // The zeros, once the tokens that occur are known: beside every pass that follows
+    // the first count.
+    const int parts = many ? l.passes : l.passes - 1, part = many ? pass : pass - 1;
+    int zero_blocks = 0;
+    if (part >= 0 && parts > 0) {
+      q.seen = seen;
+      q.table = static_cast<uint8_t*>(p->dtable);
+      q.row_bytes = p->width * size;
+      q.row0 = p->vocab * part / parts;
+      q.row1 = p->vocab * (part + 1) / parts;
+      q.access = access_bytes(size, p->width, {p->dtable}, {});
+      zero_blocks = static_cast<int>(std::min<int64_t>((q.row1 - q.row0 + 511) / 512, avey_host::multiprocessors() * 2));
+    }
+    rc = launch_pass(q, chain, many && pass > 0, zero_blocks);
+    if (rc != AVEY_OK) return rc;
+  }
+  if (l.passes == 1 && count_bytes(p->count, 1024) == 0) {
+    // One block has sorted by one digit: the zeros by a launch of their own.
+    avey::StArgs q{};
+    q.seen = seen;
+    q.table = static_cast<uint8_t*>(p->dtable);
+    q.row_bytes = p->width * size;
+    q.row1 = p->vocab;
+    q.access = access_bytes(size, p->width, {p->dtable}, {});
+    rc = chain.launch("embedding zeros", avey::st_zeros, dim3(static_cast<unsigned>((p->vocab + 511) / 512)),
+                      avey::kStThreads, 0, 1, q);
     if (rc != AVEY_OK) return rc;
   }
   avey::EmArgs q = embedding_args(p);
   q.keys = reinterpret_cast<uint32_t*>(ws + l.keys[(l.passes - 1) & 1]);
   q.ids = reinterpret_cast<uint32_t*>(ws + l.ids[(l.passes - 1) & 1]);
-  q.seen = seen;
   q.parts = reinterpret_cast<float*>(ws + l.parts);
   q.edges = reinterpret_cast<uint32_t*>(ws + l.edges);
   q.chunks = (p->count + avey::kEmChunk - 1) / avey::kEmChunk;

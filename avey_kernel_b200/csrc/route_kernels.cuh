@@ -104,7 +104,11 @@ __device__ __forceinline__ void rt_scores(const float (&z)[R], bool softmax, S (
     for (int i = 0; i < R; ++i) s[i] *= inv;
   } else {
 #pragma unroll
-    for (int i = 0; i < R; ++i) s[i] = S(1) / (S(1) + rt_exp(-S(z[i])));
+    for (int i = 0; i < R; ++i) {
+      const S e = S(1) + rt_exp(-S(z[i]));
+      if constexpr (sizeof(S) == 8) s[i] = S(1) / e;
+      else s[i] = __fdividef(1.f, e);  // 0 past 2^126, as far as any order goes
+    }
   }
 }
 
@@ -123,6 +127,61 @@ __device__ __forceinline__ uint32_t rt_best(const uint32_t (&key)[R], int e0, in
   expert = __shfl_sync(0xFFFFFFFFu, e0 + at, src);
   return all;
 }
+
+// A warp's keys from the best on, ties by the lowest expert. Up to eight a lane are sorted
+// first, so that a round compares one key of each lane (a round over eight unsorted ones
+// takes 70 instructions, a sorted one 30 after 140 for the sort).
+template <int R>
+struct RtPool {
+  static constexpr bool kSorted = R <= 8;
+  uint32_t key[R];
+  int index[R];
+
+  __device__ __forceinline__ void fill(const uint32_t (&k)[R], int e0) {
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      key[i] = k[i];
+      index[i] = e0 + i;
+    }
+    if constexpr (kSorted) {
+      // Neighbours change places only for a larger key, so equal ones keep their order.
+#pragma unroll
+      for (int n = R - 1; n > 0; --n)
+#pragma unroll
+        for (int i = 0; i < n; ++i) {
+          const bool swap = key[i + 1] > key[i];
+          const uint32_t hi = swap ? key[i + 1] : key[i], lo = swap ? key[i] : key[i + 1];
+          const int hi_e = swap ? index[i + 1] : index[i], lo_e = swap ? index[i] : index[i + 1];
+          key[i] = hi;
+          key[i + 1] = lo;
+          index[i] = hi_e;
+          index[i + 1] = lo_e;
+        }
+    }
+  }
+  __device__ __forceinline__ uint32_t next(int lane, int& expert) {
+    if constexpr (kSorted) {
+      const uint32_t all = __reduce_max_sync(0xFFFFFFFFu, key[0]);
+      const int src = __ffs(__ballot_sync(0xFFFFFFFFu, key[0] == all)) - 1;
+      expert = __shfl_sync(0xFFFFFFFFu, index[0], src);
+      if (lane == src) {
+#pragma unroll
+        for (int i = 0; i + 1 < R; ++i) {
+          key[i] = key[i + 1];
+          index[i] = index[i + 1];
+        }
+        key[R - 1] = 0u;
+      }
+      return all;
+    } else {
+      const uint32_t all = rt_best<R>(key, index[0], expert);
+#pragma unroll
+      for (int i = 0; i < R; ++i)
+        if (index[0] + i == expert) key[i] = 0u;
+      return all;
+    }
+  }
+};
 
 // The same for 64-bit keys, which order doubles: NaN at 1, 0 stands for "not there".
 __device__ __forceinline__ unsigned long long rt_key64(double x) {
@@ -167,10 +226,13 @@ __device__ __forceinline__ uint32_t rt_keep(const RtArgs& q, S merit, int lane, 
   return __ballot_sync(0xFFFFFFFFu, there && place < q.top_groups);
 }
 
-// Lane j's expert is the j-th chosen one, by scores in 64 bits.
-template <int R>
-__device__ __noinline__ int rt_choose64(const RtArgs& q, const float (&z)[R], int lane) {
+// Lane j's expert is the j-th chosen one, by scores in 64 bits. (It reads the logits again:
+// given them, it would have them kept in local memory by every token.)
+template <typename T, int R>
+__device__ __noinline__ int rt_choose64(const RtArgs& q, int64_t t, int lane) {
   const int e0 = lane * R;
+  float z[R];
+  rt_load<T, R>(static_cast<const T*>(q.logits) + t * q.ld, e0, q.experts, q.vec, z);
   const bool scored = q.bias || (q.groups > 1 && q.group_best == 2);
   double r[R];
   if (scored) rt_scores<double, R>(z, q.softmax, r);
@@ -220,45 +282,47 @@ __device__ __noinline__ int rt_choose64(const RtArgs& q, const float (&z)[R], in
   return mine;
 }
 
-// The same choice in 32 bits, and the chosen logits; false where two ranks that matter are
-// too near to tell. `most`: the largest |bias|.
-template <int R>
-__device__ __forceinline__ bool rt_choose(const RtArgs& q, const float (&z)[R], float most, int lane, int& mine,
-                                          float& mz) {
+// The same choice in 32 bits; false where two ranks that matter are too near to tell.
+// `most`: the largest |bias|; `row`: the logits, to compare two that are near.
+template <typename T, int R>
+__device__ __forceinline__ bool rt_choose(const RtArgs& q, const T* row, const float (&z)[R], float most, int lane,
+                                          int& mine, float& mz) {
   const int e0 = lane * R;
   const bool by_logit = !q.bias, sums = q.groups > 1 && q.group_best == 2;
   // Bounds of the errors of two ranks relative to their terms: the exponential and the
-  // division (2^-22), the softmax's common sum of up to 32 + 5 additions (37 2^-24), the
+  // division (2^-21), the softmax's common sum of up to 32 + 5 additions (37 2^-24), the
   // addition of the bias (2^-24).
   const float tol = q.softmax ? 4e-6f : 1e-6f;
+  float r[R];
   uint32_t key[R];
   bool sure = true;
   if (by_logit && !sums) {
 #pragma unroll
-    for (int i = 0; i < R; ++i) key[i] = e0 + i < q.experts ? rt_key(z[i]) : 0u;
+    for (int i = 0; i < R; ++i) r[i] = z[i];
   } else {
-    float s[R];
-    rt_scores<float, R>(z, q.softmax, s);
+    rt_scores<float, R>(z, q.softmax, r);
 #pragma unroll
     for (int i = 0; i < R; ++i) {
-      key[i] = 0u;
-      if (e0 + i >= q.experts) continue;
-      const float r = q.bias ? s[i] + __ldg(q.bias + e0 + i) : s[i];
-      key[i] = z[i] == -CUDART_INF_F ? rt_key(-CUDART_INF_F) : z[i] != z[i] ? 1u : rt_key(r);
+      if (q.bias && e0 + i < q.experts) r[i] += __ldg(q.bias + e0 + i);
+      if (z[i] == -CUDART_INF_F) r[i] = -CUDART_INF_F;
+      if (z[i] != z[i]) r[i] = z[i];
     }
   }
+#pragma unroll
+  for (int i = 0; i < R; ++i) key[i] = e0 + i < q.experts ? rt_key(by_logit ? z[i] : r[i]) : 0u;
   if (q.groups > 1) {
-    const int size = q.experts / q.groups;
+    const int size = q.experts / q.groups, span = size / R;
+    const bool lanes = size % R == 0 && (span & (span - 1)) == 0;
     float first = -CUDART_INF_F, second = -CUDART_INF_F;  // lane g: of group g
-    const int span = size / R;
-    if (size % R == 0 && (span & (span - 1)) == 0) {
-      // A group is `span` whole lanes, a power of two: all groups at once.
+    if (lanes) {
+      // A group is `span` whole lanes, a power of two: all groups at once (and none has
+      // lanes past the experts; a NaN counts as -inf).
       float a = -CUDART_INF_F, b = -CUDART_INF_F;
 #pragma unroll
       for (int i = 0; i < R; ++i) {
-        const float r = rt_value(key[i]);
-        b = fmaxf(b, fminf(a, r));
-        a = fmaxf(a, r);
+        const float v = e0 + i < q.experts ? fmaxf(r[i], -CUDART_INF_F) : -CUDART_INF_F;
+        b = fmaxf(b, fminf(a, v));
+        a = fmaxf(a, v);
       }
       for (int d = 1; d < span; d <<= 1) {
         const float a2 = __shfl_xor_sync(0xFFFFFFFFu, a, d), b2 = __shfl_xor_sync(0xFFFFFFFFu, b, d);
@@ -272,7 +336,8 @@ __device__ __forceinline__ bool rt_choose(const RtArgs& q, const float (&z)[R], 
       for (int g = 0; g < q.groups; ++g) {
         uint32_t in[R];
 #pragma unroll
-        for (int i = 0; i < R; ++i) in[i] = (e0 + i) / size == g ? key[i] : 0u;
+        for (int i = 0; i < R; ++i)
+          in[i] = e0 + i >= g * size && e0 + i < (g + 1) * size ? rt_key(r[i]) : 0u;
         int e;
         const float a = rt_value(rt_best<R>(in, e0, e));
 #pragma unroll
@@ -295,46 +360,42 @@ __device__ __forceinline__ bool rt_choose(const RtArgs& q, const float (&z)[R], 
       const float m_in = __shfl_sync(0xFFFFFFFFu, merit, in), m_out = __shfl_sync(0xFFFFFFFFu, merit, out);
       sure = m_out == -CUDART_INF_F || !(m_in - m_out <= bound);
     }
+    if (lanes) {
+      if (!(keep >> min(lane / span, 31) & 1u)) {
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-      if (by_logit && sums && key[i]) key[i] = rt_key(z[i]);
-      if (!(keep >> (min((e0 + i) / size, 31)) & 1u)) key[i] = 0u;
+        for (int i = 0; i < R; ++i) key[i] = 0u;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < R; ++i)
+        if (!(keep >> min((e0 + i) / size, 31) & 1u)) key[i] = 0u;
     }
   }
   // The chosen, and with a bias the next one, from the best on.
+  RtPool<R> pool;
+  pool.fill(key, e0);
   float before = 0.f;
   int before_e = 0;
   const int rounds = by_logit ? q.k : min(q.k + 1, q.top_groups * (q.experts / q.groups));
+  uint32_t mine_key = 0u;
   for (int j = 0; j < rounds; ++j) {
     int e;
-    const uint32_t top = rt_best<R>(key, e0, e);
-    float own = 0.f;
-#pragma unroll
-    for (int i = 0; i < R; ++i)
-      if (e0 + i == e) {
-        key[i] = 0u;
-        own = z[i];
-      }
+    const uint32_t top = pool.next(lane, e);
     if (!by_logit) {
-      const float r = rt_value(top);
-      if (j > 0 && r > -CUDART_INF_F && before - r <= tol * (fabsf(before) + fabsf(r) + 2.f * most)) {
-        // Too near, unless they are alike.
-        float other = 0.f;
-#pragma unroll
-        for (int i = 0; i < R; ++i)
-          if (e0 + i == before_e) other = z[i];
-        sure = sure && __shfl_sync(0xFFFFFFFFu, other, before_e / R) == __shfl_sync(0xFFFFFFFFu, own, e / R) &&
+      const float v = rt_value(top);
+      // Too near, unless they are alike.
+      if (j > 0 && v > -CUDART_INF_F && before - v <= tol * (fabsf(before) + fabsf(v) + 2.f * most))
+        sure = sure && Elem<T>::load(row + before_e) == Elem<T>::load(row + e) &&
                __ldg(q.bias + before_e) == __ldg(q.bias + e);
-      }
-      before = r;
+      before = v;
       before_e = e;
     }
-    own = __shfl_sync(0xFFFFFFFFu, own, e / R);
     if (lane == j && j < q.k) {
       mine = e;
-      mz = own;
+      mine_key = top;
     }
   }
+  if (lane < q.k) mz = by_logit ? (mine_key == 1u ? CUDART_NAN_F : rt_value(mine_key)) : Elem<T>::load(row + mine);
   return sure;
 }
 
@@ -354,11 +415,11 @@ __device__ __forceinline__ float rt_renormalized(float z, bool softmax, bool in)
   for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
   const float e = top == -CUDART_INF_F && l == l ? 0.f : expf(l - top);
   const float sum = rt_warp_sum(e);
-  return sum == 0.f ? 0.f : e / sum;
+  return sum == 0.f ? 0.f : __fdividef(e, sum);  // a sum of up to 32 terms, of at most 1 each
 }
 
 template <typename T, int R>
-__global__ void __launch_bounds__(32 * kRtWarps) route_forward(const RtArgs q) {
+__global__ void __launch_bounds__(32 * kRtWarps, R <= 4 ? 3 : R <= 8 ? 2 : 1) route_forward(const __grid_constant__ RtArgs q) {
   const int lane = threadIdx.x & 31, e0 = lane * R;
   float most = 0.f;  // the largest |bias|
   if (q.bias) {
@@ -378,17 +439,10 @@ __global__ void __launch_bounds__(32 * kRtWarps) route_forward(const RtArgs q) {
       rt_load<T, R>(static_cast<const T*>(q.logits) + (t + step) * q.ld, e0, q.experts, q.vec, next);
     int mine = 0;
     float mz = 0.f;
-    if (!rt_choose<R>(q, z, most, lane, mine, mz)) {
-      mine = rt_choose64<R>(q, z, lane);
-      for (int j = 0; j < q.k; ++j) {
-        const int e = __shfl_sync(0xFFFFFFFFu, mine, j);
-        float own = 0.f;
-#pragma unroll
-        for (int i = 0; i < R; ++i)
-          if (e0 + i == e) own = z[i];
-        own = __shfl_sync(0xFFFFFFFFu, own, e / R);
-        if (lane == j) mz = own;
-      }
+    const T* row = static_cast<const T*>(q.logits) + t * q.ld;
+    if (!rt_choose<T, R>(q, row, z, most, lane, mine, mz)) {
+      mine = rt_choose64<T, R>(q, t, lane);
+      if (lane < q.k) mz = Elem<T>::load(row + mine);
     }
     const bool in = lane < q.k;
     float w;
@@ -402,7 +456,7 @@ __global__ void __launch_bounds__(32 * kRtWarps) route_forward(const RtArgs q) {
 #pragma unroll
       for (int i = 0; i < R; ++i) sum += expf(z[i] - base);
       sum = rt_warp_sum(sum);  // NaN where a logit is NaN or +inf
-      w = sum == 0.f ? 0.f : expf(mz - base) / sum;
+      w = sum == 0.f ? 0.f : __fdividef(expf(mz - base), sum);
     } else if (q.softmax) {
       // A NaN or +inf anywhere in the row makes the softmax NaN.
       bool bad = false;

@@ -280,7 +280,6 @@ struct EmArgs {
   int64_t dy_ld;
   const uint32_t* keys;   // sorted tokens (vocab: no row of the table), and their numbers
   const uint32_t* ids;
-  const uint8_t* seen;    // [vocab]
   float* parts;           // [chunks][2][width]
   uint32_t* edges;        // chunks where a run begins that goes on: their number, zero before, and they
   int64_t chunks;
@@ -323,11 +322,10 @@ __global__ void __launch_bounds__(kRwThreads) em_forward(const EmArgs q, int lan
 // finished there; the parts of one that goes over their edge are kept: slot 0 of a
 // chunk for the run that comes in, slot 1 for one that begins there and goes on. (A frequent
 // token's rows are so shared by many blocks.) em_finish adds the parts up: of the runs that
-// em_sum lists, whose order does not matter. Blocks past the chunks write the zeros of
-// tokens that do not occur.
+// em_sum lists, whose order does not matter. The rows of tokens that do not occur are
+// written beside the sort (st_place), which leaves most of the GPU idle.
 constexpr int kEmChunk = 32;
 constexpr int kEmAhead = 8;  // rows under way for each thread
-constexpr int kEmZeroRows = 32;
 
 template <typename T, int N>
 __device__ __forceinline__ void em_put(const EmArgs& q, uint32_t token, int c, const float (&z)[N]) {
@@ -343,18 +341,6 @@ __global__ void __launch_bounds__(256) em_sum(const EmArgs q) {
   griddep_launch_dependents();
   griddep_wait();
   const int threads = blockDim.x;
-  if (blockIdx.x >= q.chunks) {
-    const int64_t r0 = (blockIdx.x - q.chunks) * kEmZeroRows;
-    const RwVec<T, N> zero = rw_zero<T, N>();
-    const int64_t mine = r0 + (threadIdx.x & 31);
-    const unsigned seen = __ballot_sync(0xFFFFFFFFu, mine < q.vocab && q.seen[mine]);
-    for (int64_t r = r0; r < min(r0 + kEmZeroRows, q.vocab); ++r) {
-      if (seen >> (r - r0) & 1u) continue;
-      for (int c = threadIdx.x * N; c < q.width; c += threads * N)
-        rw_store<T, N>(static_cast<T*>(q.dtable) + r * q.width + c, zero);
-    }
-    return;
-  }
   const int64_t p0 = blockIdx.x * static_cast<int64_t>(kEmChunk);
   const int here = static_cast<int>(min(static_cast<int64_t>(kEmChunk), q.n - p0));
   for (int i = threadIdx.x; i <= here; i += threads) {

@@ -5,8 +5,10 @@
 // Blocks take consecutive runs of the entries, warps consecutive parts of a run: so an
 // entry's place is the number of entries with a lower digit, of those with its own in
 // earlier blocks and warps, and of those before it in its warp (found 32 at a time by
-// matching digits over the warp). No atomics: the same input gives the same order. Up to
-// 8192 entries one block does it all; more take a launch that counts and one that places.
+// matching digits over the warp). No atomics but on counts: the same input gives the same
+// order. Up to
+// 8192 entries one block does it all; more take a launch that counts and one that places,
+// which counts for the next digit.
 //
 // Bound: latency, of a few dependent reads a launch: so a warp's keys are loaded eight
 // steps at a time, and the counts of all blocks 16 at a time.
@@ -41,7 +43,34 @@ struct StArgs {
   uint32_t* ids_out;
   int32_t* slots;         // the place of every entry
   int32_t* offsets;       // [buckets]: entries with a lower digit; or null
+  uint32_t* next_counts;  // the next pass's [blocks][buckets], zero before: counted while placing; or null
+  // Blocks past `blocks` write zeros to the rows of a table whose keys do not occur.
+  uint8_t* table;
+  int64_t row_bytes, row0, row1;
+  int access;             // 16, 4 or 2 bytes
 };
+
+// Zeros for the rows [row0, row1) that are not seen, a warp 32 rows at a time.
+template <typename W>
+__device__ __forceinline__ void st_zero_row(uint8_t* row, int64_t bytes) {
+  W zero{};
+  for (int64_t i = (threadIdx.x & 31) * static_cast<int64_t>(sizeof(W)); i < bytes; i += 32 * sizeof(W))
+    *reinterpret_cast<W*>(row + i) = zero;
+}
+__device__ __forceinline__ void st_zero_rows(const StArgs& q, int64_t warp, int64_t warps) {
+  const int lane = threadIdx.x & 31;
+  for (int64_t r0 = q.row0 + warp * 32; r0 < q.row1; r0 += warps * 32) {
+    const bool seen = r0 + lane >= q.row1 || q.seen[r0 + lane];
+    unsigned todo = __ballot_sync(0xFFFFFFFFu, !seen);
+    while (todo) {
+      uint8_t* row = q.table + (r0 + __ffs(todo) - 1) * q.row_bytes;
+      todo &= todo - 1;
+      if (q.access == 16) st_zero_row<uint4>(row, q.row_bytes);
+      else if (q.access == 4) st_zero_row<uint32_t>(row, q.row_bytes);
+      else st_zero_row<uint16_t>(row, q.row_bytes);
+    }
+  }
+}
 
 __device__ __forceinline__ uint32_t st_key(const StArgs& q, int64_t i) {
   if (!q.raw) return __ldg(q.keys + i);
@@ -73,7 +102,7 @@ __device__ __forceinline__ void st_keys(const StArgs& q, int64_t i0, int64_t w1,
 }
 
 // The digits of a block's entries, counted for each warp: hist [warps][buckets].
-__device__ __forceinline__ void st_count_block(const StArgs& q, uint32_t* hist, const StPart& part) {
+__device__ __forceinline__ void st_count_block(const StArgs& q, uint32_t* hist, const StPart& part, uint8_t* seen) {
   const int lane = threadIdx.x & 31;
   for (int i = threadIdx.x; i < kStWarps * q.buckets; i += kStThreads) hist[i] = 0;
   __syncthreads();
@@ -86,7 +115,7 @@ __device__ __forceinline__ void st_count_block(const StArgs& q, uint32_t* hist, 
       if (i0 + 32 * s >= part.w1) break;
       const bool in = key[s] != 0xFFFFFFFFu;
       const uint32_t d = in ? st_digit(q, key[s]) : 0xFFFFFFFFu;
-      if (in && q.seen) q.seen[key[s]] = 1;
+      if (in && seen) seen[key[s]] = 1;
       const unsigned peers = __match_any_sync(0xFFFFFFFFu, d);
       if (in && (peers & ((1u << lane) - 1)) == 0) mine[d] += __popc(peers);
       __syncwarp();
@@ -100,7 +129,7 @@ __global__ void __launch_bounds__(kStThreads) st_count(const StArgs q) {
   griddep_launch_dependents();
   griddep_wait();
   const int64_t lo = blockIdx.x * q.run, hi = min(q.n, lo + q.run);
-  st_count_block(q, hist, st_part(lo, hi));
+  st_count_block(q, hist, st_part(lo, hi), q.seen);
   for (int d = threadIdx.x; d < q.buckets; d += kStThreads) {
     uint32_t sum = 0;
 #pragma unroll
@@ -114,11 +143,16 @@ __global__ void __launch_bounds__(kStThreads) st_place(const StArgs q) {
   __shared__ uint32_t warp_sums[kStWarps];
   griddep_launch_dependents();
   griddep_wait();
+  if (static_cast<int>(blockIdx.x) >= q.blocks) {
+    st_zero_rows(q, (blockIdx.x - q.blocks) * static_cast<int64_t>(kStWarps) + (threadIdx.x >> 5),
+                 (gridDim.x - q.blocks) * static_cast<int64_t>(kStWarps));
+    return;
+  }
   uint32_t* totals = hist + kStWarps * q.buckets;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int64_t lo = blockIdx.x * q.run, hi = min(q.n, lo + q.run);
   const StPart part = st_part(lo, hi);
-  st_count_block(q, hist, part);
+  st_count_block(q, hist, part, q.blocks == 1 && q.raw ? q.seen : nullptr);
   // The digits' totals, and how many of them are in earlier blocks.
   constexpr int kPer = (kStMaxBuckets + kStThreads - 1) / kStThreads;
   uint32_t before[kPer];
@@ -216,9 +250,18 @@ __global__ void __launch_bounds__(kStThreads) st_place(const StArgs q) {
       } else {
         q.keys_out[p] = key[s];
         q.ids_out[p] = id[s];
+        if (q.next_counts)
+          atomicAdd(q.next_counts + p / static_cast<uint32_t>(q.run) * q.buckets + ((key[s] >> (q.shift + 10)) & static_cast<uint32_t>(q.mask)),
+                    1u);
       }
     }
   }
+}
+
+__global__ void __launch_bounds__(kStThreads) st_zeros(const StArgs q) {
+  griddep_launch_dependents();
+  griddep_wait();
+  st_zero_rows(q, blockIdx.x * static_cast<int64_t>(kStWarps) + (threadIdx.x >> 5), gridDim.x * static_cast<int64_t>(kStWarps));
 }
 
 }  // namespace avey
