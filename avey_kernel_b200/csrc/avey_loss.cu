@@ -168,7 +168,7 @@ Layout layout(const AveyLossParams* p, bool backward) {
     l.piece = piece_columns(p);
     l.pieces = (p->vocab + l.piece - 1) / l.piece;
     l.coef = take(p->rows * 8);
-    l.counters = take(4 * (l.pieces + 2));
+    l.counters = take(4 * (l.pieces + 3));
     if (p->dweight) {
       l.dirty = take((p->rows + 63) / 64);
       l.copy = take(p->rows * row);
@@ -362,9 +362,9 @@ int backward(const AveyLossParams* p, cudaStream_t stream) {
   char* ws = static_cast<char*>(p->workspace);
   Chain chain{stream};
   uint32_t* counters = reinterpret_cast<uint32_t*>(ws + l.counters);
-  const cudaError_t zeroed = cudaMemsetAsync(counters, 0, 4 * (l.pieces + 2), stream);
+  const cudaError_t zeroed = cudaMemsetAsync(counters, 0, 4 * (l.pieces + 3), stream);
   if (zeroed != cudaSuccess) return fail(AVEY_ERR_CUDA, cudaGetErrorString(zeroed));
-  uint32_t* largest = p->dtype == AVEY_F16 ? counters + l.pieces + 1 : nullptr;
+  uint32_t* largest = counters + l.pieces + 1;
   Rows x, w;
   rc = pack_inputs(p, l, &x, &w, chain);
   if (rc != AVEY_OK) return rc;

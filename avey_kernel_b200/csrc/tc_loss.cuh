@@ -9,10 +9,9 @@
 //
 // c is the running maximum, so every power is at most 1; lse_i = c + log2 s is
 // kept in base 2, as the hardware's exponential takes it. a_i and b_i hold the
-// gradient that comes in, the z loss's factor and, for f16, a power of two that
-// brings the largest of them to 2^14 (a probability of 1e-5 times 1 / rows is
-// below f16's range); dX and dW divide by it. dz is rounded to the operand type
-// once, as the tensor cores need it; all sums are fp32.
+// gradient that comes in, the z loss's factor and a scale that dX and dW divide by
+// (CeScale). dz is rounded to the operand type once, as the tensor cores need it; all
+// sums are fp32.
 //
 // Bounds: 2 M V d flops for the loss and 6 M V d for the gradients on the tensor
 // cores. A cluster of two CTAs computes 256 x 256 tiles (cta_group::2): per K
@@ -72,7 +71,7 @@ struct CeGeom {
   float* picked;           // stats: the target's z, [rows]
   const float* lse;        // grad: [rows], base 2
   const float2* coef;      // grad: (a, b) of every row
-  const uint32_t* largest; // f16: bits of the largest |a|, |b|; null: no scale
+  const uint32_t* largest; // bits of the largest |b| and |a|
   void* dx;                // 16 bits; null: fp32 sums by map_dx
   int64_t dx_ld;
   int dx_vec, dx_add;      // rows stored by TMA; sums are added to
@@ -93,14 +92,22 @@ __device__ __forceinline__ int ce_target(const void* targets, int64_t stride, in
   return t >= 0 && t < vocab ? static_cast<int>(t) : -2;
 }
 
-// f16: the power of two that brings the largest coefficient into [2^13, 2^14), or
-// its inverse (1 without one; a largest coefficient of zero leaves zeros).
-__device__ __forceinline__ float ce_scale(const uint32_t* largest, bool inverse) {
-  if (!largest) return 1.f;
-  const int e = static_cast<int>(__ldg(largest) >> 23);  // 2^(e - 127) <= largest < 2^(e - 126)
-  int k = e ? 127 + 13 - e : 0;
-  k = max(-126, min(126, k));
-  return __uint_as_float(static_cast<uint32_t>(127 + (inverse ? -k : k)) << 23);
+// What dz is multiplied by before it is rounded, and its inverse. A row's b is its share
+// of the gradient that comes in: divided by the largest |b| (largest[0]) it is exactly 1
+// where all rows count alike, so that a target's dz, p - 1, keeps small p's to bf16's
+// eight bits below 1 (dz = (p - 1) / rows, rounded, gave dx and dW twice the error). f16's
+// range starts at 2^-14: the power of two brings the largest |a| and |b| (largest[1]: |a|)
+// to between 2^12 and 2^13.
+struct CeScale {
+  float apply, undo;
+};
+__device__ __forceinline__ CeScale ce_scale(const uint32_t* largest) {
+  // (Below 2^-100 the inverse would leave fp32's range: rows that small count less than 1.)
+  const float b = fmaxf(__uint_as_float(__ldg(largest)), 0x1p-100f);
+  const float ratio = fmaxf(1.f, __fdiv_rn(__uint_as_float(__ldg(largest + 1)), b));
+  const int e = min(static_cast<int>(__float_as_uint(ratio) >> 23) - 127, 100);  // 2^e <= ratio < 2^(e + 1)
+  const float up = __uint_as_float(static_cast<uint32_t>(127 + 12 - e) << 23);
+  return {__fdiv_rn(up, b), __fdiv_rn(b, up)};
 }
 
 constexpr int kCeAhead = 4;  // units that the scheduler may be ahead of the last reader
@@ -517,7 +524,7 @@ __global__ void __launch_bounds__(kCeThreads, 1)
     const uint32_t freed0 = mapa_shared(smem_u32(&ctrl->acc_empty[0]), 0);
     const uint32_t freed1 = mapa_shared(smem_u32(&ctrl->acc_empty[1]), 0);
     const uint64_t policy = l2_policy_evict_normal();
-    const float scale = STATS ? 1.f : ce_scale(q.largest, false), unscale = STATS ? 1.f : ce_scale(q.largest, true);
+    const CeScale scale = STATS ? CeScale{1.f, 1.f} : ce_scale(q.largest);
     CeRow r{};
     bool alive = true;
     int it = 0, u;
@@ -531,8 +538,8 @@ __global__ void __launch_bounds__(kCeThreads, 1)
         r.target = row < b.m ? ce_target(q.targets, q.target_stride, q.target64, q.ignore, q.vocab, row) : -1;
         if (!STATS) {
           const float2 ab = row < b.m ? __ldg(q.coef + row) : make_float2(0.f, 0.f);
-          r.a = ab.x * scale;
-          r.b = ab.y * scale;
+          r.a = ab.x * scale.apply;
+          r.b = ab.y * scale.apply;
           r.lse = row < b.m ? __ldg(q.lse + row) : 0.f;
         }
         r.c = -INFINITY;
@@ -589,8 +596,8 @@ __global__ void __launch_bounds__(kCeThreads, 1)
                   uint32_t y[4];
 #pragma unroll
                   for (int j = 0; j < 4; ++j)
-                    y[j] = ln_pack<T>(__uint_as_float(o[8 * p + 2 * j]) * unscale,
-                                      __uint_as_float(o[8 * p + 2 * j + 1]) * unscale);
+                    y[j] = ln_pack<T>(__uint_as_float(o[8 * p + 2 * j]) * scale.undo,
+                                      __uint_as_float(o[8 * p + 2 * j + 1]) * scale.undo);
                   ln_sts(ln_piece(tile, lane, 2 * hh + p), y[0], y[1], y[2], y[3]);
                 }
               }
@@ -869,7 +876,7 @@ struct CeCoef {
   int64_t dy_stride;       // 0: one value
   float z_loss;
   float2* coef;
-  uint32_t* largest;       // f16: zero before, or null
+  uint32_t* largest;       // bits of the largest |b| and |a|, zero before
   const uint16_t* x;
   int64_t x_ld;
   uint16_t* copy;          // rows of ignored targets that are not finite, as zeros
@@ -906,12 +913,13 @@ __global__ void __launch_bounds__(256) ce_coef(const CeCoef q) {
       q.coef[row] = make_float2(a, b);
     }
     skip[tid] = out;
-    if (q.largest) {
-      // The largest finite one; the order of the maxima does not matter.
-      float top = fmaxf(fabsf(a), fabsf(b));
-      if (!(top < INFINITY)) top = 0.f;
-      const uint32_t all = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(top));
-      if ((tid & 31) == 0 && all) atomicMax(q.largest, all);
+    // The largest finite ones; the order of the maxima does not matter.
+    const float top_b = fabsf(b) < INFINITY ? fabsf(b) : 0.f, top_a = fabsf(a) < INFINITY ? fabsf(a) : 0.f;
+    const uint32_t all_b = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(top_b));
+    const uint32_t all_a = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(top_a));
+    if ((tid & 31) == 0) {
+      if (all_b) atomicMax(q.largest, all_b);
+      if (all_a) atomicMax(q.largest + 1, all_a);
     }
   }
   if (!q.dirty) return;
@@ -952,7 +960,7 @@ __global__ void __launch_bounds__(256) ce_join_parts(const CeParts q) {
   constexpr int kBlocks = kCeBM / kCeJoinRows;
   const int t = blockIdx.x / kBlocks, r0 = blockIdx.x % kBlocks * kCeJoinRows;
   const int mt = t / q.n_nt, nt = t - mt * q.n_nt;
-  const float scale = F32 ? 1.f : ce_scale(q.largest, true);
+  const float scale = F32 ? 1.f : ce_scale(q.largest).undo;
   const int per = q.bn / 4;
   for (int j = threadIdx.x; j < kCeJoinRows * per; j += 256) {
     const int r = r0 + j / per, c = j % per * 4;
@@ -995,7 +1003,7 @@ template <typename T>
 __global__ void __launch_bounds__(256) ce_finish(const float* sums, int64_t ld, int rows, int width,
                                                  const uint32_t* largest, T* dx, int64_t dx_ld) {
   griddep_wait();
-  const float scale = ce_scale(largest, true);
+  const float scale = ce_scale(largest).undo;
   const int64_t per = ld / 4, total = rows * per;
   const bool vec = width % 4 == 0 && dx_ld % 4 == 0 && (reinterpret_cast<uintptr_t>(dx) & 7u) == 0;
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < total;

@@ -37,8 +37,8 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, targets: torch.T
 
     bf16 / f16 CUDA tensors of one dtype run natively, forward and backward, with
     any row strides: fp32 sums, the gradient at the logits rounded to the operand
-    type before its two products (in f16 after a scaling by a power of two), and
-    each result rounded once. Tensors with forward-mode tangents, calls under a trace
+    type before its two products (relative to the largest gradient that comes in, so
+    that f16 keeps small probabilities), and each result rounded once. Tensors with forward-mode tangents, calls under a trace
     (``torch.jit.trace``, ``make_fx``) and second differentiation raise. CPU tensors
     take plain PyTorch."""
     if x.ndim < 1 or weight.ndim != 2 or weight.shape[1] != x.shape[-1] or 0 in weight.shape:

@@ -488,9 +488,9 @@ AVEY_API int avey_linear_workspace_size(const AveyLinearParams* params, int back
  *   dz_ij = g_i ((1 + 2 z_loss lse_i) exp(z_ij - lse_i) - [j = t_i])
  *   dx = dz W, dweight = dz^T x
  *
- * Products and sums are fp32; dz is rounded to dtype before its products (scaled by
- * a power of two in f16, so that small probabilities are not lost) and each result
- * once. Sums are taken in fixed orders: results are bitwise reproducible.
+ * Products and sums are fp32; dz is rounded to dtype before its products (divided by the
+ * largest |g_i| and scaled by a power of two, so that f16 does not lose small
+ * probabilities) and each result once. Sums are taken in fixed orders: results are bitwise reproducible.
  *
  * Last dimensions have stride 1; x_ld, weight_ld, dx_ld and target_stride are in
  * elements (target_stride >= 0). Any alignment is taken: rows that are not whole
