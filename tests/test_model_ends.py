@@ -1,0 +1,73 @@
+"""The example's model, from tokens to the loss and back to all of its weights, against the same
+model written in plain torch in 64 bits."""
+
+import importlib.util
+from pathlib import Path
+
+import pytest
+import torch
+import torch.nn.functional as F
+
+from avey_kernel_b200 import _native
+
+PATH = Path(__file__).resolve().parents[1] / 'examples' / 'train_block.py'
+spec = importlib.util.spec_from_file_location('train_block', PATH)
+train_block = importlib.util.module_from_spec(spec)
+spec.loader.exec_module(train_block)
+
+
+def plain(p, tokens, targets, chosen):
+    """The loss of the model with the parameters p (by name), whose every token takes all experts
+    (`chosen` of them: the renormalised weights are the softmax of the router's logits)."""
+    x = p['embed'][tokens]
+    blocks = 1 + max(int(name.split('.')[1]) for name in p if name.startswith('blocks'))
+    for i in range(blocks):
+        q = {name.split('.')[2]: t for name, t in p.items() if name.startswith(f'blocks.{i}.')}
+        width, context = x.shape[-1], x.shape[1]
+        e = F.silu(F.layer_norm(x, (width,)) @ q['enrich_w'].t() + q['enrich_b'])
+        head, tail = e[..., :width], e[..., width:]
+        unit = F.normalize(tail, dim=-1)
+        s = (unit @ unit.transpose(1, 2)) * q['mix'].tril()
+        assert s.shape[-1] == context
+        x = (s @ tail) * head @ q['fuse_w'].t() + q['fuse_b'] + x
+        h = F.layer_norm(x, (width,))
+        weights = torch.softmax(h @ q['route_w'].t(), -1)
+        assert chosen == weights.shape[-1]
+        for k in range(chosen):
+            up = torch.relu(h @ q['up_w'][k].t() + q['up_b'][k]).square()
+            x = x + weights[..., k:k + 1] * (up @ q['down_w'][k].t() + q['down_b'][k])
+    z = F.layer_norm(x, (x.shape[-1],)) @ p['head'].t()
+    return F.cross_entropy(z.flatten(0, 1), targets.flatten())
+
+
+@pytest.mark.parametrize('device,dt', [('cpu', torch.float32), pytest.param('cuda', torch.bfloat16, marks=pytest.mark.gpu),
+                                       pytest.param('cuda', torch.float16, marks=pytest.mark.gpu)])
+def test_gradients_of_the_example_model(device, dt):
+    """On the way to a weight's gradient some 24 tensors are rounded to the operands' type, each by
+    at most u = 2^-24, 2^-8 or 2^-11 of itself, and a layer passes on relative errors of its
+    inputs at about their size (norms and weights of the order of one): 24 u of the norm. (fp32: 2^-15, as
+    sums of some hundred terms add 2^-17 each.)"""
+    torch.manual_seed(0)
+    model = train_block.Model(vocab=50, context=24, width=64, num_experts=2, chosen=2, blocks=2)
+    for name, t in model.named_parameters():
+        if name.endswith('_b'):
+            torch.nn.init.normal_(t, std=0.1)
+    model = model.to(device, dt)
+    gen = torch.Generator().manual_seed(1)
+    seq = torch.randint(0, 50, (6, 25), generator=gen).to(device)
+    loss = model(seq[:, :-1], seq[:, 1:])
+    loss.backward()
+    p = {name: t.detach().double().requires_grad_(True) for name, t in model.named_parameters()}
+    want = plain(p, seq[:, :-1], seq[:, 1:], 2)
+    want.backward()
+    u = {torch.float32: 2.0 ** -15 / 24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}[dt]
+    assert abs(float(loss.detach() - want.detach())) <= 24 * u * float(want.detach())
+    for name, t in model.named_parameters():
+        off = float((t.grad.double() - p[name].grad).norm() / p[name].grad.norm())
+        assert off <= 24 * u, (name, off)
+    if device == 'cuda':
+        first = [t.grad.clone() for t in model.parameters()]
+        model.zero_grad()
+        model(seq[:, :-1], seq[:, 1:]).backward()
+        assert all(torch.equal(a, t.grad) for a, t in zip(first, model.parameters()))
+        assert _native.device_status(clear=True) == 0
