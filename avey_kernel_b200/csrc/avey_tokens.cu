@@ -148,22 +148,33 @@ int sort_opt_in() {
     err[dev] = cudaFuncSetAttribute(avey::st_count, cudaFuncAttributeMaxDynamicSharedMemorySize, avey::kStSmem);
     if (err[dev] == cudaSuccess)
       err[dev] = cudaFuncSetAttribute(avey::st_place, cudaFuncAttributeMaxDynamicSharedMemorySize, avey::kStSmem);
+    if (err[dev] == cudaSuccess)
+      err[dev] = cudaFuncSetAttribute(avey::st_sort, cudaFuncAttributeMaxDynamicSharedMemorySize, avey::kStSmem);
   });
   return err[dev] == cudaSuccess ? AVEY_OK : fail(AVEY_ERR_CUDA, cudaGetErrorString(err[dev]));
 }
 
-// `counted`: the pass before has counted for this one; `zero_blocks` more write zeros.
-int launch_pass(avey::StArgs& q, Chain& chain, bool counted = false, int zero_blocks = 0) {
+int sort_smem(int buckets) { return (avey::kStWarps + 1) * buckets * 4; }
+// Blocks beside a sort's that write `bytes` of zeros.
+int zero_blocks(int64_t bytes) {
+  return static_cast<int>(std::min<int64_t>((bytes + 65535) / 65536, avey_host::multiprocessors() * 2ll));
+}
+
+// One pass over many blocks. `counted`: the pass before has counted for this one.
+int launch_pass(avey::StArgs& q, Chain& chain, bool counted = false) {
   const int opted = sort_opt_in();
   if (opted != AVEY_OK) return opted;
   q.run = std::max<int64_t>(1, sort_run(q.n));
   q.blocks = static_cast<int>(sort_blocks(q.n));
-  const int smem = avey::kStWarps * q.buckets * 4;
+  const dim3 grid(static_cast<unsigned>(q.blocks + zero_blocks(q.zero_bytes)));
   if (q.blocks > 1 && !counted) {
-    const int rc = chain.launch("sort counts", avey::st_count, dim3(q.blocks), avey::kStThreads, smem, 1, q);
+    avey::StArgs c = q;
+    c.zero_bytes = 0;
+    const int rc = chain.launch("sort counts", avey::st_count, dim3(q.blocks), avey::kStThreads, sort_smem(q.buckets),
+                                1, c);
     if (rc != AVEY_OK) return rc;
   }
-  return chain.launch("sort", avey::st_place, dim3(q.blocks + zero_blocks), avey::kStThreads, smem + q.buckets * 4, 1, q);
+  return chain.launch("sort", avey::st_place, grid, avey::kStThreads, sort_smem(q.buckets), 1, q);
 }
 
 int validate(const AveyArrangeParams* p) {
@@ -310,10 +321,14 @@ avey::EmArgs embedding_args(const AveyEmbeddingParams* p) {
   return q;
 }
 
-// Workspace of the backward call: [keys, ids] twice, counts, edges, tokens seen, parts.
+// Places of a chunk of em_sum.
+int64_t chunk_places(int64_t n) {
+  return n >= avey::kEmChunk * 4ll * avey_host::multiprocessors() ? avey::kEmChunk : avey::kEmSmallChunk;
+}
+// Workspace of the backward call: [keys, ids] twice, counts, edges, parts.
 struct EmLayout {
   int passes = 0;
-  uint64_t keys[2] = {}, ids[2] = {}, counts[2] = {}, edges = 0, seen = 0, parts = 0, total = 0;
+  uint64_t keys[2] = {}, ids[2] = {}, counts[2] = {}, edges = 0, parts = 0, total = 0;
 };
 EmLayout embedding_layout(const AveyEmbeddingParams* p) {
   EmLayout l;
@@ -332,11 +347,11 @@ EmLayout embedding_layout(const AveyEmbeddingParams* p) {
     l.ids[i] = take(p->count * 4);
   }
   l.counts[0] = take(count_bytes(p->count, 1024));
-  // From here on zero before the first launch, up to `parts`.
+  // Zero before the first launch, where there is more than one block: the later passes'
+  // counts and the number of edges.
   l.counts[1] = take(count_bytes(p->count, 1024) * (l.passes - 1));
-  const uint64_t chunks = (p->count + avey::kEmChunk - 1) / avey::kEmChunk;
+  const uint64_t chunk = chunk_places(p->count), chunks = (p->count + chunk - 1) / chunk;
   l.edges = take((1 + chunks) * 4);
-  l.seen = take(p->vocab + 1);
   l.parts = take(chunks * 2 * p->width * 4);
   l.total = at;
   return l;
@@ -344,8 +359,11 @@ EmLayout embedding_layout(const AveyEmbeddingParams* p) {
 
 template <typename T, int N>
 int launch_sums(const avey::EmArgs& q, Chain& chain) {
-  const int threads = static_cast<int>(std::min<int64_t>(256, (q.width / N + 31) / 32 * 32));
-  int rc = chain.launch("embedding sums", avey::em_sum<T, N>, dim3(static_cast<unsigned>(q.chunks)), threads, 0, 1, q);
+  const int64_t columns = q.width / N;
+  const int threads = static_cast<int>(std::min<int64_t>(256, (columns + 31) / 32 * 32));
+  const unsigned slices = static_cast<unsigned>(std::min<int64_t>((columns + threads - 1) / threads, 64));
+  int rc = chain.launch("embedding sums", avey::em_sum<T, N>, dim3(static_cast<unsigned>(q.chunks), slices), threads, 0,
+                        1, q);
   if (rc != AVEY_OK || q.chunks < 2) return rc;
   constexpr int V = N > 1 && sizeof(T) * N == 16 ? 4 : 1;  // width is a multiple of 4
   const int slabs = (q.width + avey::kEmLanes * V - 1) / (avey::kEmLanes * V);
@@ -365,66 +383,67 @@ int embedding_backward(const AveyEmbeddingParams* p, cudaStream_t stream) {
   int rc = check_workspace(p->workspace, p->workspace_bytes, l.total);
   if (rc != AVEY_OK) return rc;
   char* ws = static_cast<char*>(p->workspace);
-  uint8_t* seen = reinterpret_cast<uint8_t*>(ws + l.seen);
-  const cudaError_t e = cudaMemsetAsync(ws + l.counts[1], 0, l.parts - l.counts[1], stream);
-  if (e != cudaSuccess) return fail(AVEY_ERR_CUDA, cudaGetErrorString(e));
+  const uint64_t pass_bytes = count_bytes(p->count, 1024), table = static_cast<uint64_t>(p->vocab) * p->width * size;
+  uint32_t* edges = reinterpret_cast<uint32_t*>(ws + l.edges);
+  auto words = [&](uint64_t at) { return reinterpret_cast<uint32_t*>(ws + at); };
+  const int last = (l.passes - 1) & 1;
   Chain chain{stream};
-  for (int pass = 0; pass < l.passes; ++pass) {
-    avey::StArgs q{};
-    q.n = p->count;
-    q.buckets = 1024;
-    q.shift = 10 * pass;
-    q.mask = 1023;
-    q.limit = p->vocab;
-    q.skip = p->padding >= 0 ? p->padding : -1;
-    if (pass == 0) {
-      q.raw = p->tokens;
-      q.raw64 = p->index_bits == 64;
-      q.seen = seen;
-    } else {
-      q.keys = reinterpret_cast<uint32_t*>(ws + l.keys[(pass - 1) & 1]);
-      q.ids = reinterpret_cast<uint32_t*>(ws + l.ids[(pass - 1) & 1]);
-    }
-    const uint64_t pass_bytes = count_bytes(p->count, 1024);
-    const bool many = pass_bytes > 0;  // blocks
-    q.counts = reinterpret_cast<uint32_t*>(pass == 0 ? ws + l.counts[0] : ws + l.counts[1] + (pass - 1) * pass_bytes);
-    if (many && pass + 1 < l.passes) q.next_counts = reinterpret_cast<uint32_t*>(ws + l.counts[1] + pass * pass_bytes);
-    q.keys_out = reinterpret_cast<uint32_t*>(ws + l.keys[pass & 1]);
-    q.ids_out = reinterpret_cast<uint32_t*>(ws + l.ids[pass & 1]);
-    // The zeros, once the tokens that occur are known: beside every pass that follows
-    // the first count.
-    const int parts = many ? l.passes : l.passes - 1, part = many ? pass : pass - 1;
-    int zero_blocks = 0;
-    if (part >= 0 && parts > 0) {
-      q.seen = seen;
-      q.table = static_cast<uint8_t*>(p->dtable);
-      q.row_bytes = p->width * size;
-      q.row0 = p->vocab * part / parts;
-      q.row1 = p->vocab * (part + 1) / parts;
-      q.access = access_bytes(size, p->width, {p->dtable}, {});
-      zero_blocks = static_cast<int>(std::min<int64_t>((q.row1 - q.row0 + 511) / 512, avey_host::multiprocessors() * 2));
-    }
-    rc = launch_pass(q, chain, many && pass > 0, zero_blocks);
+  avey::StArgs first{};
+  first.n = p->count;
+  first.buckets = 1024;
+  first.mask = 1023;
+  first.limit = p->vocab;
+  first.skip = p->padding >= 0 ? p->padding : -1;
+  first.raw = p->tokens;
+  first.raw64 = p->index_bits == 64;
+  if (pass_bytes == 0) {  // one block
+    rc = sort_opt_in();
     if (rc != AVEY_OK) return rc;
-  }
-  if (l.passes == 1 && count_bytes(p->count, 1024) == 0) {
-    // One block has sorted by one digit: the zeros by a launch of their own.
-    avey::StArgs q{};
-    q.seen = seen;
-    q.table = static_cast<uint8_t*>(p->dtable);
-    q.row_bytes = p->width * size;
-    q.row1 = p->vocab;
-    q.access = access_bytes(size, p->width, {p->dtable}, {});
-    rc = chain.launch("embedding zeros", avey::st_zeros, dim3(static_cast<unsigned>((p->vocab + 511) / 512)),
-                      avey::kStThreads, 0, 1, q);
+    avey::StArgs q = first;
+    q.run = p->count;
+    q.blocks = 1;
+    q.passes = l.passes;
+    q.keys_out = words(l.keys[last]);
+    q.ids_out = words(l.ids[last]);
+    q.more_keys = words(l.keys[last ^ 1]);
+    q.more_ids = words(l.ids[last ^ 1]);
+    q.clear = edges;
+    q.zeros = static_cast<uint8_t*>(p->dtable);
+    q.zero_bytes = static_cast<int64_t>(table);
+    rc = chain.launch("sort", avey::st_sort, dim3(1u + zero_blocks(q.zero_bytes)), avey::kStThreads,
+                      sort_smem(q.buckets), 1, q);
     if (rc != AVEY_OK) return rc;
+  } else {
+    const cudaError_t e = cudaMemsetAsync(ws + l.counts[1], 0, l.edges + 4 - l.counts[1], stream);
+    if (e != cudaSuccess) return fail(AVEY_ERR_CUDA, cudaGetErrorString(e));
+    for (int pass = 0; pass < l.passes; ++pass) {
+      avey::StArgs q = first;
+      q.shift = 10 * pass;
+      if (pass > 0) {
+        q.raw = nullptr;
+        q.keys = words(l.keys[(pass - 1) & 1]);
+        q.ids = words(l.ids[(pass - 1) & 1]);
+      }
+      q.counts = words(pass == 0 ? l.counts[0] : l.counts[1] + (pass - 1) * pass_bytes);
+      if (pass + 1 < l.passes) q.next_counts = words(l.counts[1] + pass * pass_bytes);
+      q.keys_out = words(l.keys[pass & 1]);
+      q.ids_out = words(l.ids[pass & 1]);
+      // A share of the table's zeros beside each pass, in whole 256 bytes.
+      const uint64_t z0 = table / l.passes / 256 * 256 * pass;
+      const uint64_t z1 = pass + 1 == l.passes ? table : table / l.passes / 256 * 256 * (pass + 1);
+      q.zeros = static_cast<uint8_t*>(p->dtable) + z0;
+      q.zero_bytes = static_cast<int64_t>(z1 - z0);
+      rc = launch_pass(q, chain, pass > 0);
+      if (rc != AVEY_OK) return rc;
+    }
   }
   avey::EmArgs q = embedding_args(p);
-  q.keys = reinterpret_cast<uint32_t*>(ws + l.keys[(l.passes - 1) & 1]);
-  q.ids = reinterpret_cast<uint32_t*>(ws + l.ids[(l.passes - 1) & 1]);
+  q.keys = words(l.keys[last]);
+  q.ids = words(l.ids[last]);
   q.parts = reinterpret_cast<float*>(ws + l.parts);
-  q.edges = reinterpret_cast<uint32_t*>(ws + l.edges);
-  q.chunks = (p->count + avey::kEmChunk - 1) / avey::kEmChunk;
+  q.edges = edges;
+  q.chunk = static_cast<int>(chunk_places(p->count));
+  q.chunks = (p->count + q.chunk - 1) / q.chunk;
   const int bytes = access_bytes(size, p->width, {p->dy, p->dtable}, {p->dy_ld});
   if (p->dtype == AVEY_F32) return bytes == 16 ? launch_sums<float, 4>(q, chain) : launch_sums<float, 1>(q, chain);
   if (p->dtype == AVEY_F16)

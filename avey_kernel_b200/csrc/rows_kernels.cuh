@@ -281,6 +281,7 @@ struct EmArgs {
   const uint32_t* keys;   // sorted tokens (vocab: no row of the table), and their numbers
   const uint32_t* ids;
   float* parts;           // [chunks][2][width]
+  int chunk;              // places of a chunk
   uint32_t* edges;        // chunks where a run begins that goes on: their number, zero before, and they
   int64_t chunks;
   void* dtable;           // [vocab], contiguous
@@ -322,9 +323,10 @@ __global__ void __launch_bounds__(kRwThreads) em_forward(const EmArgs q, int lan
 // finished there; the parts of one that goes over their edge are kept: slot 0 of a
 // chunk for the run that comes in, slot 1 for one that begins there and goes on. (A frequent
 // token's rows are so shared by many blocks.) em_finish adds the parts up: of the runs that
-// em_sum lists, whose order does not matter. The rows of tokens that do not occur are
-// written beside the sort (st_place), which leaves most of the GPU idle.
-constexpr int kEmChunk = 32;
+// em_sum lists, whose order does not matter. Zeros are written to the whole table before,
+// beside the sort, which leaves most of the GPU idle. 32 places, or 8 where those would be
+// too few blocks.
+constexpr int kEmChunk = 32, kEmSmallChunk = 8;
 constexpr int kEmAhead = 8;  // rows under way for each thread
 
 template <typename T, int N>
@@ -341,18 +343,18 @@ __global__ void __launch_bounds__(256) em_sum(const EmArgs q) {
   griddep_launch_dependents();
   griddep_wait();
   const int threads = blockDim.x;
-  const int64_t p0 = blockIdx.x * static_cast<int64_t>(kEmChunk);
-  const int here = static_cast<int>(min(static_cast<int64_t>(kEmChunk), q.n - p0));
+  const int64_t p0 = blockIdx.x * static_cast<int64_t>(q.chunk);
+  const int here = static_cast<int>(min(static_cast<int64_t>(q.chunk), q.n - p0));
   for (int i = threadIdx.x; i <= here; i += threads) {
     keys[i] = p0 + i < q.n ? __ldg(q.keys + p0 + i) : 0xFFFFFFFFu;  // the last: the next chunk's first
     if (i < here) ids[i] = __ldg(q.ids + p0 + i);
   }
   __syncthreads();
   const bool enters = p0 > 0 && __ldg(q.keys + p0 - 1) == keys[0];
-  if (threadIdx.x == 0 && here == kEmChunk && keys[here] == keys[here - 1] && keys[here] < q.vocab &&
+  if (threadIdx.x == 0 && blockIdx.y == 0 && here == q.chunk && keys[here] == keys[here - 1] && keys[here] < q.vocab &&
       !(enters && keys[0] == keys[here]))
     q.edges[1 + atomicAdd(q.edges, 1u)] = blockIdx.x;
-  for (int c = threadIdx.x * N; c < q.width; c += threads * N) {
+  for (int c = (blockIdx.y * threads + threadIdx.x) * N; c < q.width; c += gridDim.y * threads * N) {
     float z[N];
 #pragma unroll
     for (int n = 0; n < N; ++n) z[n] = 0.f;
@@ -400,13 +402,13 @@ __global__ void __launch_bounds__(kEmGroups * kEmLanes) em_finish(const EmArgs q
   const int64_t items = static_cast<int64_t>(*q.edges) * slabs;
   for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
     const int64_t b = q.edges[1 + item / slabs];
-    const uint32_t token = __ldg(q.keys + b * kEmChunk + kEmChunk);
+    const uint32_t token = __ldg(q.keys + (b + 1) * q.chunk);
     // The last chunk that the run reaches: looked at 256 at a time.
     if (threadIdx.x == 0) last = b;
     __syncthreads();
     for (int64_t c0 = b + 1;; c0 += kEmGroups * kEmLanes) {
       const int64_t c = c0 + threadIdx.x;
-      const bool in = c < q.chunks && __ldg(q.keys + c * kEmChunk) == token;
+      const bool in = c < q.chunks && __ldg(q.keys + c * q.chunk) == token;
       const int n = __syncthreads_count(in);
       if (threadIdx.x == 0) last = c0 - 1 + n;
       if (n < kEmGroups * kEmLanes) break;

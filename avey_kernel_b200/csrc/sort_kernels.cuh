@@ -8,7 +8,8 @@
 // matching digits over the warp). No atomics but on counts: the same input gives the same
 // order. Up to
 // 8192 entries one block does it all; more take a launch that counts and one that places,
-// which counts for the next digit.
+// which counts for the next digit. The places where the rest of the GPU would idle take
+// zeros to write (a table's gradient, of which most rows are zero).
 //
 // Bound: latency, of a few dependent reads a launch: so a warp's keys are loaded eight
 // steps at a time, and the counts of all blocks 16 at a time.
@@ -36,7 +37,6 @@ struct StArgs {
   int64_t limit, skip;    // a raw key outside [0, limit), or equal to skip, counts as limit
   const uint32_t* keys;
   const uint32_t* ids;    // entry numbers that go with keys; null: 0, 1, 2, ...
-  uint8_t* seen;          // [limit + 1], or null: set for every key that occurs
   uint32_t* counts;       // [blocks][buckets]
   int blocks;
   uint32_t* keys_out;     // sorted keys and entry numbers, or
@@ -44,36 +44,28 @@ struct StArgs {
   int32_t* slots;         // the place of every entry
   int32_t* offsets;       // [buckets]: entries with a lower digit; or null
   uint32_t* next_counts;  // the next pass's [blocks][buckets], zero before: counted while placing; or null
-  // Blocks past `blocks` write zeros to the rows of a table whose keys do not occur.
-  uint8_t* table;
-  int64_t row_bytes, row0, row1;
-  int access;             // 16, 4 or 2 bytes
+  uint32_t* more_keys;    // st_sort: room for the passes between, and how many there are
+  uint32_t* more_ids;
+  int passes;
+  uint32_t* clear;        // a word to be cleared, or null
+  // Blocks past `blocks` write zeros to these bytes.
+  uint8_t* zeros;
+  int64_t zero_bytes;
 };
 
-// Zeros for the rows [row0, row1) that are not seen, a warp 32 rows at a time.
-template <typename W>
-__device__ __forceinline__ void st_zero_row(uint8_t* row, int64_t bytes) {
-  W zero{};
-  for (int64_t i = (threadIdx.x & 31) * static_cast<int64_t>(sizeof(W)); i < bytes; i += 32 * sizeof(W))
-    *reinterpret_cast<W*>(row + i) = zero;
+// Zeros by `blocks` blocks, 16 bytes an access but at the ends.
+__device__ __forceinline__ void st_zero(uint8_t* p, int64_t bytes, int64_t block, int64_t blocks) {
+  const int64_t head = min(bytes, static_cast<int64_t>(-reinterpret_cast<uintptr_t>(p) & 15u));
+  const int64_t words = (bytes - head) / 16, tail = bytes - head - 16 * words;
+  uint4* body = reinterpret_cast<uint4*>(p + head);
+  for (int64_t i = block * blockDim.x + threadIdx.x; i < words; i += blocks * blockDim.x)
+    body[i] = make_uint4(0u, 0u, 0u, 0u);
+  if (block != 0) return;
+  if (threadIdx.x < head) p[threadIdx.x] = 0;
+  if (threadIdx.x < tail) p[bytes - tail + threadIdx.x] = 0;
 }
-__device__ __forceinline__ void st_zero_rows(const StArgs& q, int64_t warp, int64_t warps) {
-  const int lane = threadIdx.x & 31;
-  for (int64_t r0 = q.row0 + warp * 32; r0 < q.row1; r0 += warps * 32) {
-    const bool seen = r0 + lane >= q.row1 || q.seen[r0 + lane];
-    unsigned todo = __ballot_sync(0xFFFFFFFFu, !seen);
-    while (todo) {
-      uint8_t* row = q.table + (r0 + __ffs(todo) - 1) * q.row_bytes;
-      todo &= todo - 1;
-      if (q.access == 16) st_zero_row<uint4>(row, q.row_bytes);
-      else if (q.access == 4) st_zero_row<uint32_t>(row, q.row_bytes);
-      else st_zero_row<uint16_t>(row, q.row_bytes);
-    }
-  }
-}
-
 __device__ __forceinline__ uint32_t st_key(const StArgs& q, int64_t i) {
-  if (!q.raw) return __ldg(q.keys + i);
+  if (!q.raw) return __ldcg(q.keys + i);  // (written by this launch's block itself in st_sort)
   const int64_t t = q.raw64 ? __ldg(static_cast<const long long*>(q.raw) + i)
                             : static_cast<int64_t>(__ldg(static_cast<const int32_t*>(q.raw) + i));
   return static_cast<uint32_t>(t < 0 || t >= q.limit || t == q.skip ? q.limit : t);
@@ -102,7 +94,7 @@ __device__ __forceinline__ void st_keys(const StArgs& q, int64_t i0, int64_t w1,
 }
 
 // The digits of a block's entries, counted for each warp: hist [warps][buckets].
-__device__ __forceinline__ void st_count_block(const StArgs& q, uint32_t* hist, const StPart& part, uint8_t* seen) {
+__device__ __forceinline__ void st_count_block(const StArgs& q, uint32_t* hist, const StPart& part) {
   const int lane = threadIdx.x & 31;
   for (int i = threadIdx.x; i < kStWarps * q.buckets; i += kStThreads) hist[i] = 0;
   __syncthreads();
@@ -115,7 +107,6 @@ __device__ __forceinline__ void st_count_block(const StArgs& q, uint32_t* hist, 
       if (i0 + 32 * s >= part.w1) break;
       const bool in = key[s] != 0xFFFFFFFFu;
       const uint32_t d = in ? st_digit(q, key[s]) : 0xFFFFFFFFu;
-      if (in && seen) seen[key[s]] = 1;
       const unsigned peers = __match_any_sync(0xFFFFFFFFu, d);
       if (in && (peers & ((1u << lane) - 1)) == 0) mine[d] += __popc(peers);
       __syncwarp();
@@ -128,8 +119,12 @@ __global__ void __launch_bounds__(kStThreads) st_count(const StArgs q) {
   extern __shared__ uint32_t hist[];
   griddep_launch_dependents();
   griddep_wait();
+  if (static_cast<int>(blockIdx.x) >= q.blocks) {
+    st_zero(q.zeros, q.zero_bytes, blockIdx.x - q.blocks, gridDim.x - q.blocks);
+    return;
+  }
   const int64_t lo = blockIdx.x * q.run, hi = min(q.n, lo + q.run);
-  st_count_block(q, hist, st_part(lo, hi), q.seen);
+  st_count_block(q, hist, st_part(lo, hi));
   for (int d = threadIdx.x; d < q.buckets; d += kStThreads) {
     uint32_t sum = 0;
 #pragma unroll
@@ -138,21 +133,13 @@ __global__ void __launch_bounds__(kStThreads) st_count(const StArgs q) {
   }
 }
 
-__global__ void __launch_bounds__(kStThreads) st_place(const StArgs q) {
-  extern __shared__ uint32_t hist[];  // [warps][buckets], then [buckets]
-  __shared__ uint32_t warp_sums[kStWarps];
-  griddep_launch_dependents();
-  griddep_wait();
-  if (static_cast<int>(blockIdx.x) >= q.blocks) {
-    st_zero_rows(q, (blockIdx.x - q.blocks) * static_cast<int64_t>(kStWarps) + (threadIdx.x >> 5),
-                 (gridDim.x - q.blocks) * static_cast<int64_t>(kStWarps));
-    return;
-  }
+// One pass of a block over its entries. hist: [warps][buckets], then [buckets].
+__device__ __forceinline__ void st_place_block(const StArgs& q, uint32_t* hist, uint32_t* warp_sums) {
   uint32_t* totals = hist + kStWarps * q.buckets;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int64_t lo = blockIdx.x * q.run, hi = min(q.n, lo + q.run);
   const StPart part = st_part(lo, hi);
-  st_count_block(q, hist, part, q.blocks == 1 && q.raw ? q.seen : nullptr);
+  st_count_block(q, hist, part);
   // The digits' totals, and how many of them are in earlier blocks.
   constexpr int kPer = (kStMaxBuckets + kStThreads - 1) / kStThreads;
   uint32_t before[kPer];
@@ -230,7 +217,7 @@ __global__ void __launch_bounds__(kStThreads) st_place(const StArgs q) {
 #pragma unroll
     for (int s = 0; s < kStSteps; ++s) {
       const int64_t i = i0 + 32 * s + lane;
-      id[s] = q.ids && i < part.w1 ? __ldg(q.ids + i) : static_cast<uint32_t>(i);
+      id[s] = q.ids && i < part.w1 ? __ldcg(q.ids + i) : static_cast<uint32_t>(i);
     }
 #pragma unroll
     for (int s = 0; s < kStSteps; ++s) {
@@ -258,10 +245,40 @@ __global__ void __launch_bounds__(kStThreads) st_place(const StArgs q) {
   }
 }
 
-__global__ void __launch_bounds__(kStThreads) st_zeros(const StArgs q) {
+__global__ void __launch_bounds__(kStThreads) st_place(const StArgs q) {
+  extern __shared__ uint32_t hist[];
+  __shared__ uint32_t warp_sums[kStWarps];
   griddep_launch_dependents();
   griddep_wait();
-  st_zero_rows(q, blockIdx.x * static_cast<int64_t>(kStWarps) + (threadIdx.x >> 5), gridDim.x * static_cast<int64_t>(kStWarps));
+  if (static_cast<int>(blockIdx.x) < q.blocks) st_place_block(q, hist, warp_sums);
+  else st_zero(q.zeros, q.zero_bytes, blockIdx.x - q.blocks, gridDim.x - q.blocks);
+}
+
+// All passes of one block, which hands its entries to itself.
+__global__ void __launch_bounds__(kStThreads) st_sort(StArgs q) {
+  extern __shared__ uint32_t hist[];
+  __shared__ uint32_t warp_sums[kStWarps];
+  griddep_launch_dependents();
+  griddep_wait();
+  if (blockIdx.x > 0) {
+    st_zero(q.zeros, q.zero_bytes, blockIdx.x - 1, gridDim.x - 1);
+    return;
+  }
+  if (threadIdx.x == 0 && q.clear) *q.clear = 0u;
+  // The last pass writes to keys_out, those before it to one place and the other in turn.
+  uint32_t* keys[2] = {q.keys_out, q.more_keys};
+  uint32_t* ids[2] = {q.ids_out, q.more_ids};
+  for (int pass = 0; pass < q.passes; ++pass) {
+    const int to = (q.passes - 1 - pass) & 1;
+    q.shift = 10 * pass;
+    q.keys_out = keys[to];
+    q.ids_out = ids[to];
+    st_place_block(q, hist, warp_sums);
+    __syncthreads();
+    q.raw = nullptr;
+    q.keys = keys[to];
+    q.ids = ids[to];
+  }
 }
 
 }  // namespace avey

@@ -17,6 +17,7 @@
 #include <c10/cuda/CUDAGuard.h>
 
 #include <algorithm>
+#include <cmath>
 #include <vector>
 
 #include "avey_b200.h"
@@ -424,6 +425,10 @@ Tensor linear(const Tensor& x, const Tensor& weight, const std::optional<Tensor>
 
 // ------------------------------------------------------------ cross entropy
 
+void check_integers(const Tensor& t, const char* name) {
+  TORCH_CHECK_VALUE(t.scalar_type() == at::kInt || t.scalar_type() == at::kLong, name, " must be int32 or int64");
+}
+
 // The parameter block but for the operands, and for `targets` [rows].
 AveyLossParams loss_params(const Tensor& like, int64_t rows, int64_t width, int64_t vocab, const Tensor& targets,
                            int64_t ignore, int64_t reduction, double z_loss) {
@@ -538,7 +543,12 @@ Tensor cross_entropy(const Tensor& x, const Tensor& weight, const Tensor& target
   TORCH_CHECK_VALUE(x.is_cuda() && (dt == at::kBFloat16 || dt == at::kHalf) && weight.scalar_type() == dt &&
                         weight.device() == x.device(),
                     "the native cross entropy takes bf16 / f16 CUDA tensors of one dtype");
-  TORCH_CHECK_VALUE(targets.device() == x.device(), "targets must be on x's device");
+  TORCH_CHECK_VALUE(x.dim() >= 1 && weight.dim() == 2 && weight.numel() > 0 && weight.size(1) == x.size(-1),
+                    "x must be [..., width] and weight [vocab, width]");
+  check_integers(targets, "targets");
+  TORCH_CHECK_VALUE(targets.device() == x.device() && targets.sizes() == x.sizes().slice(0, x.dim() - 1),
+                    "targets must have shape ", x.sizes().slice(0, x.dim() - 1), " on x's device");
+  TORCH_CHECK_VALUE(std::isfinite(z_loss), "z_loss must be finite");
   if (at::GradMode::is_enabled() && (x.requires_grad() || weight.requires_grad()))
     return LossFunction::apply(x, weight, targets, ignore, reduction, z_loss);
   return loss_forward(x, weight, targets, ignore, reduction, z_loss, false).first;
@@ -546,6 +556,7 @@ Tensor cross_entropy(const Tensor& x, const Tensor& weight, const Tensor& target
 
 // ------------------------------------------------------------ routing
 
+constexpr int64_t kMaxExperts = 1024, kMaxChoices = 32, kMaxGroups = 32;
 void check_floating(const Tensor& t, const char* name) {
   TORCH_CHECK_VALUE(t.is_cuda() && dtype_id(t) >= 0, name, " must be a CUDA tensor of float32, float16 or bfloat16");
 }
@@ -644,9 +655,20 @@ std::pair<Tensor, Tensor> route(const Tensor& logits, const std::optional<Tensor
     if (bias) f(*bias);
   });
   check_floating(logits, "logits");
+  TORCH_CHECK_VALUE(logits.dim() >= 1 && logits.size(-1) >= 1 && logits.size(-1) <= kMaxExperts,
+                    "logits must be [..., experts] with 1 to ", kMaxExperts, " experts");
+  const int64_t experts = logits.size(-1);
+  TORCH_CHECK_VALUE(groups >= 1 && groups <= kMaxGroups && experts % groups == 0 && top_groups >= 1 &&
+                        top_groups <= groups,
+                    "groups must divide the experts and be 1 to ", kMaxGroups, ", top_groups 1 to groups");
+  TORCH_CHECK_VALUE(group_best == 1 || group_best == 2, "group_best must be 1 or 2");
+  TORCH_CHECK_VALUE(k >= 1 && k <= kMaxChoices && k <= experts / groups * top_groups, "k must be 1 to ", kMaxChoices,
+                    " and no more than the experts to choose from");
+  TORCH_CHECK_VALUE(std::isfinite(scale), "scale must be finite");
   if (bias)
-    TORCH_CHECK_VALUE(bias->scalar_type() == at::kFloat && bias->device() == logits.device(),
-                      "bias must be float32 on the logits' device");
+    TORCH_CHECK_VALUE(bias->scalar_type() == at::kFloat && bias->device() == logits.device() && bias->dim() == 1 &&
+                          bias->size(0) == experts,
+                      "bias must be float32 of shape [experts] on the logits' device");
   if (at::GradMode::is_enabled() && logits.requires_grad()) {
     auto out = RouteFunction::apply(logits, bias, k, score, groups, top_groups, group_best,
                                     static_cast<int64_t>(renormalize), scale);
@@ -657,6 +679,8 @@ std::pair<Tensor, Tensor> route(const Tensor& logits, const std::optional<Tensor
 
 std::pair<Tensor, Tensor> arrange(const Tensor& chosen, int64_t experts) {
   refuse_unseen([](auto) {});
+  check_integers(chosen, "chosen");
+  TORCH_CHECK_VALUE(experts >= 1 && experts <= kMaxExperts, "num_experts must be 1 to ", kMaxExperts);
   const c10::cuda::CUDAGuard guard(chosen.device());
   const Tensor c = chosen.contiguous();
   const auto i32 = chosen.options().dtype(at::kInt);
@@ -787,14 +811,17 @@ class CombineFunction : public torch::autograd::Function<CombineFunction> {
 };
 
 void check_slots(const Tensor& slots, const Tensor& like) {
-  TORCH_CHECK_VALUE(slots.dim() == 2 && slots.scalar_type() == at::kInt && slots.device() == like.device(),
-                    "slots must be [tokens, k] int32 on the rows' device");
+  TORCH_CHECK_VALUE(slots.dim() == 2 && slots.scalar_type() == at::kInt && slots.device() == like.device() &&
+                        slots.size(1) >= 1 && slots.size(1) <= kMaxChoices,
+                    "slots must be [tokens, k] in int32 on the rows' device, with k from 1 to ", kMaxChoices);
+  TORCH_CHECK_VALUE(like.dim() == 2 && like.size(1) > 0, "x and rows must be [rows, width]");
 }
 
 Tensor dispatch(const Tensor& x, const Tensor& slots) {
   refuse_unseen([&](auto f) { f(x); });
   check_floating(x, "x");
   check_slots(slots, x);
+  TORCH_CHECK_VALUE(slots.size(0) == x.size(0), "slots must have ", x.size(0), " rows");
   if (at::GradMode::is_enabled() && x.requires_grad()) return DispatchFunction::apply(x, slots);
   return dispatch_rows(x, slots);
 }
@@ -807,11 +834,15 @@ Tensor combine(const Tensor& rows, const Tensor& slots, const Tensor& weights, c
   });
   check_floating(rows, "rows");
   check_slots(slots, rows);
-  TORCH_CHECK_VALUE(weights.scalar_type() == at::kFloat && weights.device() == rows.device(),
-                    "weights must be float32 on the rows' device");
+  TORCH_CHECK_VALUE(rows.size(0) == slots.numel(), "rows must be [", slots.numel(), ", width]");
+  TORCH_CHECK_VALUE(weights.scalar_type() == at::kFloat && weights.device() == rows.device() &&
+                        weights.sizes() == slots.sizes(),
+                    "weights must be float32 of shape ", slots.sizes(), " on the rows' device");
   if (residual)
-    TORCH_CHECK_VALUE(residual->scalar_type() == rows.scalar_type() && residual->device() == rows.device(),
-                      "residual must have the rows' type and device");
+    TORCH_CHECK_VALUE(residual->scalar_type() == rows.scalar_type() && residual->device() == rows.device() &&
+                          residual->dim() == 2 && residual->size(0) == slots.size(0) &&
+                          residual->size(1) == rows.size(1),
+                      "residual must have the rows' type and device and shape [", slots.size(0), ", ", rows.size(1), "]");
   if (at::GradMode::is_enabled() &&
       (rows.requires_grad() || weights.requires_grad() || (residual && residual->requires_grad())))
     return CombineFunction::apply(rows, slots, weights, residual);
@@ -887,7 +918,11 @@ class EmbeddingFunction : public torch::autograd::Function<EmbeddingFunction> {
 Tensor embedding(const Tensor& tokens, const Tensor& weight, double scale, int64_t padding) {
   refuse_unseen([&](auto f) { f(weight); });
   check_floating(weight, "weight");
+  TORCH_CHECK_VALUE(weight.dim() == 2 && weight.numel() > 0, "weight must be [vocab, width]");
+  check_integers(tokens, "tokens");
   TORCH_CHECK_VALUE(tokens.device() == weight.device(), "tokens must be on the weight's device");
+  TORCH_CHECK_VALUE(padding >= -1 && padding < weight.size(0), "padding_idx must be a token of the vocabulary");
+  TORCH_CHECK_VALUE(std::isfinite(scale), "scale must be finite");
   if (at::GradMode::is_enabled() && weight.requires_grad())
     return EmbeddingFunction::apply(tokens, weight, scale, padding);
   return embedding_forward(tokens, weight, scale, padding);

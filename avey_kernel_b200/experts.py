@@ -108,12 +108,15 @@ def route(logits: torch.Tensor, k: int, *, bias: Optional[torch.Tensor] = None,
     CUDA tensors run natively, forward and backward (the weights' gradient goes to the
     logits); forward-mode tangents, traces and second differentiation raise. CPU
     tensors take plain PyTorch."""
+    if score not in _native.SCORE_IDS:
+        raise ValueError("score must be 'softmax' or 'sigmoid'")
+    if logits.is_cuda:
+        return _binding.module().route(logits, bias, k, _native.SCORE_IDS[score], groups, top_groups,
+                                       group_best, renormalize, scale)
     if logits.ndim < 1 or logits.dtype not in _FLOATS or not 1 <= logits.shape[-1] <= _native.MAX_EXPERTS:
         raise ValueError('logits must be [..., experts] in float32, float16 or bfloat16, with 1 to '
                          f'{_native.MAX_EXPERTS} experts')
     experts = logits.shape[-1]
-    if score not in _native.SCORE_IDS:
-        raise ValueError("score must be 'softmax' or 'sigmoid'")
     if not 1 <= groups <= _native.MAX_GROUPS or experts % groups or not 1 <= top_groups <= groups:
         raise ValueError(f'groups must divide the experts and be 1 to {_native.MAX_GROUPS}, top_groups 1 to groups')
     if group_best not in (1, 2):
@@ -124,9 +127,6 @@ def route(logits: torch.Tensor, k: int, *, bias: Optional[torch.Tensor] = None,
         raise ValueError('bias must be float32 of shape [experts]')
     if not math.isfinite(scale):
         raise ValueError('scale must be finite')
-    if logits.is_cuda:
-        return _binding.module().route(logits, bias, k, _native.SCORE_IDS[score], groups, top_groups,
-                                       group_best, renormalize, scale)
     return _route_torch(logits, k, bias, score, groups, top_groups, group_best, renormalize, scale)
 
 
@@ -179,12 +179,12 @@ def arrange(chosen: torch.Tensor, num_experts: int) -> Tuple[torch.Tensor, torch
     ``offsets`` (int32, num_experts + 1) bounds each expert's places, as
     ``expert_linear`` takes them. Choices outside ``[0, num_experts)`` hold the places from
     ``offsets[-1]`` on, where ``expert_linear`` gives zeros: they are dropped."""
+    if chosen.is_cuda:
+        return _binding.module().arrange(chosen, num_experts)
     if chosen.dtype not in (torch.int32, torch.int64):
         raise ValueError('chosen must be int32 or int64 expert numbers')
     if not 1 <= num_experts <= _native.MAX_EXPERTS:
         raise ValueError(f'num_experts must be 1 to {_native.MAX_EXPERTS}')
-    if chosen.is_cuda:
-        return _binding.module().arrange(chosen, num_experts)
     flat = chosen.reshape(-1).long()
     flat = torch.where((flat < 0) | (flat >= num_experts), num_experts, flat)
     order = torch.argsort(flat, stable=True)
@@ -207,11 +207,11 @@ def dispatch(x: torch.Tensor, slots: torch.Tensor) -> torch.Tensor:
     k, width]`` from x ``[tokens, width]`` (fp32, bf16 or f16, any row stride) and the
     slots of ``arrange`` (each place once). CUDA tensors run natively, forward and backward
     (a token's gradient is the sum of its rows', in fp32); CPU tensors take plain PyTorch."""
+    if x.is_cuda:
+        return _binding.module().dispatch(x, slots)
     if x.ndim != 2 or x.shape[1] == 0:
         raise ValueError('x must be [tokens, width]')
     _check_slots(slots, x.shape[0])
-    if x.is_cuda:
-        return _binding.module().dispatch(x, slots)
     # The token of each place; places that no slot names stay zero.
     flat = slots.reshape(-1).long()
     named = (flat >= 0) & (flat < flat.numel())
@@ -229,6 +229,8 @@ def combine(rows: torch.Tensor, slots: torch.Tensor, weights: torch.Tensor, *,
     run natively, forward and backward (gradients of rows, weights and residual);
     forward-mode tangents, traces and second differentiation raise. CPU tensors take
     plain PyTorch."""
+    if rows.is_cuda:
+        return _binding.module().combine(rows, slots, weights, residual)
     _check_slots(slots)
     if rows.ndim != 2 or rows.shape[1] == 0 or rows.shape[0] != slots.numel():
         raise ValueError(f'rows must be [{slots.numel()}, width]')
@@ -236,8 +238,6 @@ def combine(rows: torch.Tensor, slots: torch.Tensor, weights: torch.Tensor, *,
         raise ValueError(f'weights must be float32 of shape {list(slots.shape)}')
     if residual is not None and residual.shape != (slots.shape[0], rows.shape[1]):
         raise ValueError(f'residual must have shape {[slots.shape[0], rows.shape[1]]}')
-    if rows.is_cuda:
-        return _binding.module().combine(rows, slots, weights, residual)
     named = (slots >= 0) & (slots < slots.numel())
     mine = rows.float()[torch.where(named, slots, 0).long()] * (weights * named).unsqueeze(-1)
     out = mine.sum(1)

@@ -280,16 +280,18 @@ def embedding(tokens: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0,
     one order, so it is bitwise reproducible and needs no array in fp32 of the table's size.
     Forward-mode tangents, traces and second differentiation raise. CPU tensors take
     plain PyTorch."""
+    if padding_idx is not None and padding_idx < 0:
+        raise ValueError('padding_idx must be a token of the vocabulary')
+    if weight.is_cuda:
+        return _binding.module().embedding(tokens, weight, scale, -1 if padding_idx is None else padding_idx)
     if weight.ndim != 2 or 0 in weight.shape:
         raise ValueError('weight must be [vocab, width]')
     if tokens.dtype not in (torch.int32, torch.int64):
         raise ValueError('tokens must be int32 or int64')
-    if padding_idx is not None and not 0 <= padding_idx < weight.shape[0]:
+    if padding_idx is not None and padding_idx >= weight.shape[0]:
         raise ValueError('padding_idx must be a token of the vocabulary')
     if not math.isfinite(scale):
         raise ValueError('scale must be finite')
-    if weight.is_cuda:
-        return _binding.module().embedding(tokens, weight, scale, -1 if padding_idx is None else padding_idx)
     inside = (tokens >= 0) & (tokens < weight.shape[0])
     out = F.embedding(torch.where(inside, tokens, 0), weight.float(), padding_idx) * scale
     return torch.where(inside.unsqueeze(-1), out, math.nan).to(weight.dtype)

@@ -41,19 +41,19 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, targets: torch.T
     that f16 keeps small probabilities), and each result rounded once. Tensors with forward-mode tangents, calls under a trace
     (``torch.jit.trace``, ``make_fx``) and second differentiation raise. CPU tensors
     take plain PyTorch."""
+    if reduction not in _native.REDUCTION_IDS:
+        raise ValueError("reduction must be 'none', 'sum' or 'mean'")
+    if x.is_cuda:
+        return _binding.module().cross_entropy(x, weight, targets, ignore_index,
+                                               _native.REDUCTION_IDS[reduction], z_loss)
     if x.ndim < 1 or weight.ndim != 2 or weight.shape[1] != x.shape[-1] or 0 in weight.shape:
         raise ValueError('x must be [..., width] and weight [vocab, width]')
     if targets.shape != x.shape[:-1]:
         raise ValueError(f'targets must have shape {list(x.shape[:-1])}')
     if targets.dtype not in (torch.int32, torch.int64):
         raise ValueError('targets must be int32 or int64')
-    if reduction not in _native.REDUCTION_IDS:
-        raise ValueError("reduction must be 'none', 'sum' or 'mean'")
     if not math.isfinite(z_loss):
         raise ValueError('z_loss must be finite')
-    if x.is_cuda:
-        return _binding.module().cross_entropy(x, weight, targets, ignore_index,
-                                               _native.REDUCTION_IDS[reduction], z_loss)
     return _cross_entropy_torch(x, weight, targets, ignore_index, reduction, z_loss)
 
 

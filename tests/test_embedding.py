@@ -218,7 +218,7 @@ def test_c_workspace_sizes():
                                     count=100, width=8, vocab=1000, scale=1.0, tokens=at, dy=at, dy_ld=8, dtable=at)
     size, lib = ctypes.c_uint64(), _native.lib()
     assert lib.avey_embedding_workspace_size(ctypes.byref(p), ctypes.byref(size)) == 0
-    # Keys and numbers of 100 tokens twice, 5 words of edges, 1001 flags, two parts of 4 pieces of 32.
-    assert size.value == 4 * 512 + 256 + 1024 + 256
+    # Keys and numbers of 100 tokens twice, 14 words of edges, two parts of 13 pieces of 8.
+    assert size.value == 4 * 512 + 256 + 1024
     p.dy = 0
     assert lib.avey_embedding_bwd_v1(ctypes.byref(p), None) == -1 and b'dy' in lib.avey_last_error()
