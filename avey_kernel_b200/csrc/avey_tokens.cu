@@ -232,17 +232,30 @@ int part_lanes(int64_t width, int per) {
   return lanes;
 }
 
+template <typename T, int N, int HOLD>
+int launch_combine(const avey::RwArgs& q, int what, int lanes, Chain& chain) {
+  const int64_t tokens = avey::kRwThreads / lanes;
+  const dim3 grid(static_cast<unsigned>(std::min<int64_t>(
+      (q.tokens + tokens - 1) / tokens, avey_host::multiprocessors() * static_cast<int64_t>(avey::rw_blocks(HOLD)))));
+  if (what == 1) return chain.launch("combine", avey::rw_combine<T, N, HOLD>, grid, avey::kRwThreads, 0, 1, q, lanes);
+  return chain.launch("combine gradient", avey::rw_combine_backward<T, N, HOLD>, grid, avey::kRwThreads, 0, 1, q, lanes);
+}
+
 template <typename T, int N>
 int launch_rows(const avey::RwArgs& q, int what, Chain& chain) {
   if (what == 0)
     return chain.launch("dispatch", avey::rw_dispatch<T, N>, dim3(blocks_for(q.tokens * (q.width / N), 256)), 256, 0, 1,
                         q);
-  const int lanes = part_lanes(q.width, N);
-  const int64_t tokens = avey::kRwThreads / lanes;
-  const dim3 grid(static_cast<unsigned>(
-      std::min<int64_t>((q.tokens + tokens - 1) / tokens, avey_host::multiprocessors() * 3ll)));
-  if (what == 1) return chain.launch("combine", avey::rw_combine<T, N>, grid, avey::kRwThreads, 0, 1, q, lanes);
-  return chain.launch("combine gradient", avey::rw_combine_backward<T, N>, grid, avey::kRwThreads, 0, 1, q, lanes);
+  if constexpr (sizeof(T) * N == 16) {
+    const int lanes = part_lanes(q.width, N);
+    switch ((q.width / N + lanes - 1) / lanes) {
+      case 1: return launch_combine<T, N, 1>(q, what, lanes, chain);
+      case 3: return launch_combine<T, N, 3>(q, what, lanes, chain);
+      case 4: return launch_combine<T, N, 4>(q, what, lanes, chain);
+      default: return launch_combine<T, N, 2>(q, what, lanes, chain);
+    }
+  }
+  return launch_combine<T, N, 2>(q, what, part_lanes(q.width, N), chain);
 }
 
 // what: 0 dispatch, 1 combine, 2 combine's backward.

@@ -231,15 +231,20 @@ __device__ __forceinline__ void st_place_block(const StArgs& q, uint32_t* hist, 
       __syncwarp();
       if (in && lower == 0) place[d] += __popc(peers);
       __syncwarp();
+      if (q.next_counts) {
+        // Lanes that count in one place (those of a frequent token) do so together.
+        const uint32_t to =
+            in ? p / static_cast<uint32_t>(q.run) * q.buckets + ((key[s] >> (q.shift + 10)) & static_cast<uint32_t>(q.mask))
+               : 0xFFFFFFFFu;
+        const unsigned same = __match_any_sync(0xFFFFFFFFu, to);
+        if (in && (same & ((1u << lane) - 1)) == 0) atomicAdd(q.next_counts + to, static_cast<uint32_t>(__popc(same)));
+      }
       if (!in) continue;
       if (q.slots) {
         q.slots[i0 + 32 * s + lane] = static_cast<int32_t>(p);
       } else {
         q.keys_out[p] = key[s];
         q.ids_out[p] = id[s];
-        if (q.next_counts)
-          atomicAdd(q.next_counts + p / static_cast<uint32_t>(q.run) * q.buckets + ((key[s] >> (q.shift + 10)) & static_cast<uint32_t>(q.mask)),
-                    1u);
       }
     }
   }
