@@ -114,11 +114,11 @@ struct Layout {
   uint64_t total = 0;
 };
 
-// Columns of dz kept at a time, twice where there is more than one piece: 256 MB, or
-// four times the width where that is more, so that dx's sums, read and written for
-// every piece, stay small beside its products.
+// Columns of dz kept at a time, twice where there is more than one piece: 256 MB, but
+// 4096 at least (above 32768 rows), where reading and writing dx's fp32 sums for every
+// piece takes a fourteenth of the time of its products.
 int64_t piece_columns(const AveyLossParams* p) {
-  const int64_t most = std::max<int64_t>((256ll << 20) / (2 * p->rows), 4 * p->width);
+  const int64_t most = std::max<int64_t>((256ll << 20) / (2 * p->rows), 4096);
   const int64_t tiles = (p->vocab + 255) / 256, per = std::max<int64_t>(1, most / 256);
   if (2 * per >= tiles) return up(p->vocab, 8);
   const int64_t pieces = (tiles + per - 1) / per;

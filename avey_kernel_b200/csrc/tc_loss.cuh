@@ -924,12 +924,20 @@ __global__ void __launch_bounds__(256) ce_coef(const CeCoef q) {
   }
   if (!q.dirty) return;
   __syncthreads();
-  constexpr uint16_t kTop = std::is_same<T, __half>::value ? 0x7C00 : 0x7F80;
+  // Rows of x are whole 16-byte units here; a warp looks at a row.
+  constexpr uint32_t kTop = std::is_same<T, __half>::value ? 0x7C00u : 0x7F80u;
+  const int lane = tid & 31;
   bool bad = false;
-  for (int i = 0; i < here; ++i) {
-    if (!skip[i]) continue;
+#pragma unroll 4
+  for (int i = tid >> 5; i < kCeCoefRows; i += 8) {
+    if (!skip[i] || i >= here) continue;
     const uint16_t* p = q.x + static_cast<int64_t>(row0 + i) * q.x_ld;
-    for (int j = tid; j < q.width; j += 256) bad |= (p[j] & kTop) == kTop;
+    for (int j = lane * 8; j < q.width; j += 256) {
+      const uint4 v = ln_load8(p + j, q.width - j, true);
+      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) bad |= (w[k] & kTop) == kTop || (w[k] >> 16 & kTop) == kTop;
+    }
   }
   bad = __syncthreads_or(bad);
   if (tid == 0) q.dirty[blockIdx.x] = bad;

@@ -138,6 +138,7 @@ def _route_torch(logits, k, bias, score, groups, top_groups, group_best, renorma
         exact = torch.sigmoid(z) if score == 'sigmoid' else torch.softmax(z, -1)
         rank = z if bias is None else exact + bias.double()
         by = exact if bias is None and group_best == 2 else rank
+        last = rank.isnan()
         rank, by = (torch.where(out, -math.inf, t).nan_to_num(-math.inf, posinf=math.inf, neginf=-math.inf)
                     for t in (rank, by))
         if groups > 1:
@@ -150,7 +151,7 @@ def _route_torch(logits, k, bias, score, groups, top_groups, group_best, renorma
         else:
             kept = torch.ones_like(out)
         # Those out of reach last, before them NaN, before those -inf.
-        tier = torch.where(kept, torch.where(z.isnan() | exact.isnan() & (bias is not None), 1, 0), 2)
+        tier = torch.where(kept, last.long(), 2)
         order = torch.sort(-rank, dim=-1, stable=True).indices
         order = order.gather(-1, torch.sort(tier.gather(-1, order), dim=-1, stable=True).indices)
         chosen = order[..., :k]

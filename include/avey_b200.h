@@ -531,8 +531,9 @@ typedef struct AveyLossParams {
 AVEY_API int avey_loss_fwd_v1(const AveyLossParams* params, void* stream);
 AVEY_API int avey_loss_bwd_v1(const AveyLossParams* params, void* stream);
 
-/* Bytes of `workspace` of the forward (backward == 0) or backward call: about 512
- * MB at most beside a share of the operands' size, whatever rows x vocab is. */
+/* Bytes of `workspace` of the forward (backward == 0) or backward call. The backward
+ * call's holds pieces of dz of 512 MB (16 KB a row above 32768 rows) at most, whatever
+ * the vocabulary, and beside them 6 bytes for every element of x. */
 AVEY_API int avey_loss_workspace_size(const AveyLossParams* params, int backward, uint64_t* bytes);
 
 /*
@@ -746,8 +747,8 @@ AVEY_API uint64_t avey_launch_count(void);
  * wait_limit_cycles: SM cycles after which a bounded wait on an mbarrier gives
  * up (<= 0 restores the default of about one second). stall != 0: later
  * launches of the fused tensor-core kernel start with their TMA and MMA warps
- * issuing nothing, and those of the linear layers with their TMA lane issuing
- * nothing, so the first wait for their work runs out, the kernel
+ * issuing nothing, and those of the linear layers and the cross entropy with their TMA
+ * lanes issuing nothing, so the first wait for their work runs out, the kernel
  * raises AVEY_DEVFLAG_TIMEOUT, unwinds and returns (no trap, the context stays
  * usable). The wait limit applies to the current device; the stall flag to
  * the process. Not for production use. */

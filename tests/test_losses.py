@@ -505,10 +505,10 @@ def test_workspace_stays_small_whatever_the_logits_take():
     back = dict(dloss=at, dx=at, dx_ld=768, dweight=at, width=768, x_ld=768, weight_ld=768)
     for rows, vocab in ((16384, 131072), (65536, 131072), (4096, 50021), (1, 1 << 20)):
         size = _native.loss_workspace_size(_params(rows=rows, vocab=vocab, **back), backward=True)
-        # dz by pieces of 256 MB and their rounding to tiles twice (or 8 widths a row), x's copy,
-        # dx's sums and a few words a row.
-        assert size <= (513 << 20) + rows * 768 * (16 + 2 + 4) + 16 * rows + (1 << 20) + 148 * 4 * 256 * 256 * 4
-        assert size < 3 * rows * vocab or rows * vocab < 1 << 30
+        # dz by pieces of 256 MB, or 4096 columns, twice, in whole tiles of 256 columns; x's copy and
+        # dx's sums; a few words a row; sums of tiles that are shared, eight at most for each of 148 SMs.
+        pieces = 2 * max(256 << 20, rows * 4096 * 2) + 2 * rows * 256 * 2
+        assert size <= pieces + rows * 768 * (2 + 4) + 16 * rows + (1 << 20) + 8 * 148 * 256 * 256 * 4
     assert _native.loss_workspace_size(_params(rows=0)) == 0
 
 
