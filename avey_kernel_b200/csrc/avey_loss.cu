@@ -120,7 +120,7 @@ struct Layout {
 int64_t piece_columns(const AveyLossParams* p) {
   const int64_t most = std::max<int64_t>((256ll << 20) / (2 * p->rows), 4096);
   const int64_t tiles = (p->vocab + 255) / 256, per = std::max<int64_t>(1, most / 256);
-  if (2 * per >= tiles) return up(p->vocab, 8);
+  if (2 * per >= tiles) return up(p->vocab, 16);
   const int64_t pieces = (tiles + per - 1) / per;
   return (tiles + pieces - 1) / pieces * 256;
 }
@@ -173,7 +173,7 @@ Layout layout(const AveyLossParams* p, bool backward) {
       l.dirty = take((p->rows + 63) / 64);
       l.copy = take(p->rows * row);
     }
-    l.dz_bytes = static_cast<uint64_t>(p->rows) * l.piece * 2;
+    l.dz_bytes = (static_cast<uint64_t>(p->rows) * l.piece * 2 + 255) / 256 * 256;
     l.dz = take(l.dz_bytes * (l.pieces > 1 ? 2 : 1));
     if (p->dx) {
       if (l.pieces > 1) l.sums = take(p->rows * up(p->width, 4) * 4);
@@ -407,7 +407,7 @@ int backward(const AveyLossParams* p, cudaStream_t stream) {
     q.coef = k.coef;
     int jobs = 0, splits = 1;
     if (i > 0) {
-      const int64_t v0 = (i - 1) * l.piece, n = std::min(l.piece, p->vocab - v0), ld = up(n, 8);
+      const int64_t v0 = (i - 1) * l.piece, n = std::min(l.piece, p->vocab - v0), ld = up(n, 16);
       const char* dz = ws + l.dz + (i - 1) % 2 * l.dz_bytes;
       const char* wp = static_cast<const char*>(w.p) + v0 * w.ld * 2;
       if (p->dx) {
@@ -449,7 +449,7 @@ int backward(const AveyLossParams* p, cudaStream_t stream) {
       }
     }
     if (i < l.pieces) {
-      const int64_t v0 = i * l.piece, n = std::min(l.piece, p->vocab - v0), ld = up(n, 8);
+      const int64_t v0 = i * l.piece, n = std::min(l.piece, p->vocab - v0), ld = up(n, 16);
       const int cols = logit_cols(n);
       q.job[jobs] = job(avey::kCeGrad, p->rows, n, p->width, cols);
       q.job[jobs].seg = unit_tiles(q.job[jobs].n_mt, q.job[jobs].n_nt);
@@ -460,8 +460,8 @@ int backward(const AveyLossParams* p, cudaStream_t stream) {
       if (rc == AVEY_OK)
         rc = avey_host::encode_rows16(p->dtype, static_cast<const char*>(w.p) + v0 * w.ld * 2, p->width, n, 1, w.ld * 2,
                                       0, cols / 2, &m.w);
-      if (rc == AVEY_OK)
-        rc = avey_host::encode_tiles(p->dtype, ws + l.dz + i % 2 * l.dz_bytes, n, p->rows, 1, ld * 2, 0, &m.dz_out);
+      q.dz = reinterpret_cast<uint16_t*>(ws + l.dz + i % 2 * l.dz_bytes);
+      q.dz_ld = ld;
       if (rc != AVEY_OK) return rc;
     }
     set_ring(q);
