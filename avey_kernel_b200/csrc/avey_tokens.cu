@@ -66,15 +66,18 @@ int validate(const AveyRouteParams* p, bool backward) {
   return AVEY_OK;
 }
 
+// Experts of a lane: `lanes` of a token's each take R of them.
 template <typename T, int R>
-int launch_route(const avey::RtArgs& q, bool backward, Chain& chain) {
-  const dim3 grid(static_cast<unsigned>((q.tokens + avey::kRtWarps - 1) / avey::kRtWarps));
-  if (!backward) {
-    const dim3 some(std::min<unsigned>(grid.x, avey_host::multiprocessors() * 8u));
-    return chain.launch("route", avey::route_forward<T, R>, some, 32 * avey::kRtWarps, 0, 1, q);
-  }
-  return chain.launch("route gradient", avey::route_backward<T, R>, grid, 32 * avey::kRtWarps,
-                      avey::kRtWarps * 32 * R * 4, 1, q);
+int launch_route(const avey::RtArgs& q, bool backward, int lanes, Chain& chain) {
+  const int64_t tokens = 32 * avey::kRtWarps / lanes;
+  const dim3 grid(static_cast<unsigned>((q.tokens + tokens - 1) / tokens));
+  if (backward)
+    return chain.launch("route gradient", avey::route_backward<T, R>, grid, 32 * avey::kRtWarps,
+                        avey::kRtWarps * 32 * (R + 1) * 4, 1, q, lanes);
+  if (!q.bias && q.groups == 1)
+    return chain.launch("route", avey::route_plain<T, R>, grid, 32 * avey::kRtWarps, 0, 1, q, lanes);
+  const dim3 some(std::min<unsigned>(grid.x, avey_host::multiprocessors() * 8u));
+  return chain.launch("route", avey::route_forward<T, R>, some, 32 * avey::kRtWarps, 0, 1, q);
 }
 
 template <typename T>
@@ -99,13 +102,20 @@ int route(const AveyRouteParams* p, bool backward, cudaStream_t stream) {
   q.dlogits = p->dlogits;
   q.dvec = ((address(p->dlogits) | static_cast<uint64_t>(p->experts) * sizeof(T)) & 15u) == 0;
   Chain chain{stream};
-  const int per = (q.experts + 31) / 32;
-  if (per <= 1) return launch_route<T, 1>(q, backward, chain);
-  if (per <= 2) return launch_route<T, 2>(q, backward, chain);
-  if (per <= 4) return launch_route<T, 4>(q, backward, chain);
-  if (per <= 8) return launch_route<T, 8>(q, backward, chain);
-  if (per <= 16) return launch_route<T, 16>(q, backward, chain);
-  return launch_route<T, 32>(q, backward, chain);
+  // A whole warp for the choice by scores; else as many lanes as have 16 experts each, or
+  // one of the chosen.
+  int lanes = 32;
+  if (backward || (!q.bias && q.groups == 1)) {
+    lanes = 1;
+    while (lanes < 32 && (lanes * 16 < q.experts || lanes < q.k)) lanes *= 2;
+  }
+  const int per = (q.experts + lanes - 1) / lanes;
+  if (per <= 1) return launch_route<T, 1>(q, backward, lanes, chain);
+  if (per <= 2) return launch_route<T, 2>(q, backward, lanes, chain);
+  if (per <= 4) return launch_route<T, 4>(q, backward, lanes, chain);
+  if (per <= 8) return launch_route<T, 8>(q, backward, lanes, chain);
+  if (per <= 16) return launch_route<T, 16>(q, backward, lanes, chain);
+  return launch_route<T, 32>(q, backward, lanes, chain);
 }
 
 int run_route(const AveyRouteParams* p, bool backward, void* stream) {
@@ -166,14 +176,12 @@ int launch_pass(avey::StArgs& q, Chain& chain, bool counted = false) {
   if (opted != AVEY_OK) return opted;
   q.run = std::max<int64_t>(1, sort_run(q.n));
   q.blocks = static_cast<int>(sort_blocks(q.n));
-  const dim3 grid(static_cast<unsigned>(q.blocks + zero_blocks(q.zero_bytes)));
   if (q.blocks > 1 && !counted) {
-    avey::StArgs c = q;
-    c.zero_bytes = 0;
     const int rc = chain.launch("sort counts", avey::st_count, dim3(q.blocks), avey::kStThreads, sort_smem(q.buckets),
-                                1, c);
+                                1, q);
     if (rc != AVEY_OK) return rc;
   }
+  const dim3 grid(static_cast<unsigned>(q.blocks + zero_blocks(q.zero_bytes)));
   return chain.launch("sort", avey::st_place, grid, avey::kStThreads, sort_smem(q.buckets), 1, q);
 }
 
@@ -336,7 +344,9 @@ avey::EmArgs embedding_args(const AveyEmbeddingParams* p) {
 
 // Places of a chunk of em_sum.
 int64_t chunk_places(int64_t n) {
-  return n >= avey::kEmChunk * 4ll * avey_host::multiprocessors() ? avey::kEmChunk : avey::kEmSmallChunk;
+  int64_t chunk = avey::kEmChunk;
+  while (chunk > avey::kEmSmallChunk && n < chunk * 4 * avey_host::multiprocessors()) chunk /= 2;
+  return chunk;
 }
 // Workspace of the backward call: [keys, ids] twice, counts, edges, parts.
 struct EmLayout {
@@ -441,9 +451,10 @@ int embedding_backward(const AveyEmbeddingParams* p, cudaStream_t stream) {
       if (pass + 1 < l.passes) q.next_counts = words(l.counts[1] + pass * pass_bytes);
       q.keys_out = words(l.keys[pass & 1]);
       q.ids_out = words(l.ids[pass & 1]);
-      // A share of the table's zeros beside each pass, in whole 256 bytes.
-      const uint64_t z0 = table / l.passes / 256 * 256 * pass;
-      const uint64_t z1 = pass + 1 == l.passes ? table : table / l.passes / 256 * 256 * (pass + 1);
+      // A share of the table's zeros beside each pass, in whole 256 bytes. (With a share beside
+      // the count as well the sort's launches took no longer and the call 5 us more.)
+      const uint64_t share = table / l.passes / 256 * 256;
+      const uint64_t z0 = share * pass, z1 = pass + 1 == l.passes ? table : share * (pass + 1);
       q.zeros = static_cast<uint8_t*>(p->dtable) + z0;
       q.zero_bytes = static_cast<int64_t>(z1 - z0);
       rc = launch_pass(q, chain, pass > 0);

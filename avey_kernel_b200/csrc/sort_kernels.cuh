@@ -119,10 +119,6 @@ __global__ void __launch_bounds__(kStThreads) st_count(const StArgs q) {
   extern __shared__ uint32_t hist[];
   griddep_launch_dependents();
   griddep_wait();
-  if (static_cast<int>(blockIdx.x) >= q.blocks) {
-    st_zero(q.zeros, q.zero_bytes, blockIdx.x - q.blocks, gridDim.x - q.blocks);
-    return;
-  }
   const int64_t lo = blockIdx.x * q.run, hi = min(q.n, lo + q.run);
   st_count_block(q, hist, st_part(lo, hi));
   for (int d = threadIdx.x; d < q.buckets; d += kStThreads) {
