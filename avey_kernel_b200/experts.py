@@ -97,9 +97,9 @@ def route(logits: torch.Tensor, k: int, *, bias: Optional[torch.Tensor] = None,
     bias``. With ``groups`` > 1 (consecutive experts, up to 32 groups) only those of the
     best ``top_groups`` groups are chosen from; a group ranks by the sum of the ranks of
     its best ``group_best`` experts (1 or 2; for 2 without a bias, of their scores).
-    Ties go to the lowest index. ``chosen`` (int32 ``[..., k]``) has them from the best on, ``weights`` (fp32
-    ``[..., k]``) are ``scale * s``, divided by the sum of the chosen scores with
-    ``renormalize``.
+    Ties go to the lowest index. ``chosen`` (int32 ``[..., k]``) has them from the best on,
+    ``weights`` (fp32 ``[..., k]``) are ``scale * s``, divided by the sum of the chosen
+    scores with ``renormalize``.
 
     The choice is the formula's also where scores are nearer than fp32 tells. A logit of
     -inf takes an expert out: it ranks below all others and its weight is 0 (zeros for a
@@ -179,7 +179,8 @@ def arrange(chosen: torch.Tensor, num_experts: int) -> Tuple[torch.Tensor, torch
     all in the order of their experts, those of one expert in their given order, and
     ``offsets`` (int32, num_experts + 1) bounds each expert's places, as
     ``expert_linear`` takes them. Choices outside ``[0, num_experts)`` hold the places from
-    ``offsets[-1]`` on, where ``expert_linear`` gives zeros: they are dropped."""
+    ``offsets[-1]`` on, where ``expert_linear`` gives zeros: so choices are dropped (not by
+    taking slots out, which would leave rows of ``dispatch`` unwritten)."""
     if chosen.is_cuda:
         return _binding.module().arrange(chosen, num_experts)
     if chosen.dtype not in (torch.int32, torch.int64):
@@ -210,8 +211,8 @@ def dispatch(x: torch.Tensor, slots: torch.Tensor) -> torch.Tensor:
     (a token's gradient is the sum of its rows', in fp32); CPU tensors take plain PyTorch."""
     if x.is_cuda:
         return _binding.module().dispatch(x, slots)
-    if x.ndim != 2 or x.shape[1] == 0:
-        raise ValueError('x must be [tokens, width]')
+    if x.ndim != 2 or x.shape[1] == 0 or x.dtype not in _FLOATS:
+        raise ValueError('x must be [tokens, width] in float32, float16 or bfloat16')
     _check_slots(slots, x.shape[0])
     # The token of each place; places that no slot names stay zero.
     flat = slots.reshape(-1).long()
@@ -233,13 +234,13 @@ def combine(rows: torch.Tensor, slots: torch.Tensor, weights: torch.Tensor, *,
     if rows.is_cuda:
         return _binding.module().combine(rows, slots, weights, residual)
     _check_slots(slots)
-    if rows.ndim != 2 or rows.shape[1] == 0 or rows.shape[0] != slots.numel():
-        raise ValueError(f'rows must be [{slots.numel()}, width]')
+    if rows.ndim != 2 or rows.shape[1] == 0 or rows.shape[0] != slots.numel() or rows.dtype not in _FLOATS:
+        raise ValueError(f'rows must be [{slots.numel()}, width] in float32, float16 or bfloat16')
     if weights.shape != slots.shape or weights.dtype != torch.float32:
         raise ValueError(f'weights must be float32 of shape {list(slots.shape)}')
-    if residual is not None and residual.shape != (slots.shape[0], rows.shape[1]):
-        raise ValueError(f'residual must have shape {[slots.shape[0], rows.shape[1]]}')
+    if residual is not None and (residual.shape != (slots.shape[0], rows.shape[1]) or residual.dtype != rows.dtype):
+        raise ValueError(f"residual must have the rows' type and shape {[slots.shape[0], rows.shape[1]]}")
     named = (slots >= 0) & (slots < slots.numel())
-    mine = rows.float()[torch.where(named, slots, 0).long()] * (weights * named).unsqueeze(-1)
-    out = mine.sum(1)
+    mine = rows.float()[torch.where(named, slots, 0).long()] * weights.unsqueeze(-1)
+    out = torch.where(named.unsqueeze(-1), mine, 0.0).sum(1)
     return (out if residual is None else out + residual.float()).to(rows.dtype)

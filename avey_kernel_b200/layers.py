@@ -284,8 +284,8 @@ def embedding(tokens: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0,
         raise ValueError('padding_idx must be a token of the vocabulary')
     if weight.is_cuda:
         return _binding.module().embedding(tokens, weight, scale, -1 if padding_idx is None else padding_idx)
-    if weight.ndim != 2 or 0 in weight.shape:
-        raise ValueError('weight must be [vocab, width]')
+    if weight.ndim != 2 or 0 in weight.shape or weight.dtype not in (torch.float32, torch.float16, torch.bfloat16):
+        raise ValueError('weight must be [vocab, width] in float32, float16 or bfloat16')
     if tokens.dtype not in (torch.int32, torch.int64):
         raise ValueError('tokens must be int32 or int64')
     if padding_idx is not None and padding_idx >= weight.shape[0]:

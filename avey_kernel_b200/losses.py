@@ -38,14 +38,16 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, targets: torch.T
     bf16 / f16 CUDA tensors of one dtype run natively, forward and backward, with
     any row strides: fp32 sums, the gradient at the logits rounded to the operand
     type before its two products (relative to the largest gradient that comes in, so
-    that f16 keeps small probabilities), and each result rounded once. Tensors with forward-mode tangents, calls under a trace
-    (``torch.jit.trace``, ``make_fx``) and second differentiation raise. CPU tensors
-    take plain PyTorch."""
+    that f16 keeps small probabilities), and each result rounded once. Tensors with
+    forward-mode tangents, calls under a trace (``torch.jit.trace``, ``make_fx``) and
+    second differentiation raise. CPU tensors take plain PyTorch."""
     if reduction not in _native.REDUCTION_IDS:
         raise ValueError("reduction must be 'none', 'sum' or 'mean'")
     if x.is_cuda:
         return _binding.module().cross_entropy(x, weight, targets, ignore_index,
                                                _native.REDUCTION_IDS[reduction], z_loss)
+    if weight.dtype != x.dtype or x.dtype not in (torch.float32, torch.float16, torch.bfloat16):
+        raise ValueError('x and weight must be float32, float16 or bfloat16 of one dtype')
     if x.ndim < 1 or weight.ndim != 2 or weight.shape[1] != x.shape[-1] or 0 in weight.shape:
         raise ValueError('x must be [..., width] and weight [vocab, width]')
     if targets.shape != x.shape[:-1]:
@@ -61,7 +63,7 @@ def _cross_entropy_torch(x, weight, targets, ignore_index, reduction, z_loss):
     """The plain PyTorch form (CPU tensors)."""
     used = targets != ignore_index
     inside = (targets >= 0) & (targets < weight.shape[0])
-    z = F.linear(x.masked_fill(~used.unsqueeze(-1), 0), weight).float()
+    z = F.linear(x.masked_fill(~used.unsqueeze(-1), 0).float(), weight.float())
     lse = torch.logsumexp(z, dim=-1)
     picked = z.gather(-1, torch.where(inside, targets, 0).long().unsqueeze(-1)).squeeze(-1)
     each = lse - picked + z_loss * lse.square()

@@ -133,6 +133,19 @@ def test_results_are_bitwise_reproducible_and_whole_numbers_exact():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('n,vocab,width', [(8192, 1000, 24), (8193, 1000, 24), (9500, 1 << 20, 4), (20000, 1 << 20, 1),
+                                           (38000, 777, 300), (40000, (1 << 20) + 7, 2)])
+def test_all_pieces_and_numbers_of_passes(n, vocab, width):
+    """One block's sort and many blocks', of one to three digits, with pieces of 8 to 32 places;
+    tokens from both ends of the vocabulary, one of them a quarter of all."""
+    g = torch.Generator(device='cuda').manual_seed(n)
+    t = torch.randint(0, vocab, (n,), generator=g, device='cuda')
+    t[::4] = vocab - 3
+    t[1:100] = torch.arange(99, device='cuda') - 1
+    check(t, vocab, width, torch.float32, padding=5)
+
+
+@pytest.mark.gpu
 def test_tables_past_2_to_the_31_elements():
     vocab, width = (1 << 21) + 50, 1032  # 2.16 10^9 elements
     w = torch.zeros(vocab, width, dtype=torch.bfloat16, device='cuda')
@@ -170,6 +183,12 @@ def test_streams_and_captured_steps():
         for _ in range(3):
             graph.replay()
         assert all(torch.equal(p, q) for p, q in zip(got, step()))
+
+
+def test_types_that_a_table_may_have():
+    for bad in (torch.double, torch.long):
+        with pytest.raises(ValueError, match='float'):
+            layers.embedding(torch.zeros(3, dtype=torch.int64), torch.ones(5, 4).to(bad))
 
 
 def test_refusals_of_arguments():

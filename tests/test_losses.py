@@ -409,6 +409,13 @@ def test_the_plain_form_on_the_cpu():
             assert (a.double() - b).abs().max() <= 2.0 ** -18 * (1 + b.abs().max())  # sums of 60 terms in fp32
 
 
+@pytest.mark.parametrize('dt', [torch.bfloat16, torch.float16])
+def test_the_plain_form_keeps_the_logits_in_fp32(dt):
+    x, w, t, _ = data(40, 24, 60, dt, 14, 0.2, device='cpu')
+    want = losses.linear_cross_entropy(x.float(), w.float(), t)
+    assert torch.equal(losses.linear_cross_entropy(x, w, t), want)
+
+
 def test_gradient_against_differences():
     """The formula of the gradient that the GPU tests hold the kernels to (``reference``), against
     differences of its loss."""
@@ -434,6 +441,13 @@ def test_gradient_against_differences():
             # Rounding: 2^-52 of sums below 100, over 2 h; the quotient's own error h^2 times the
             # third derivative, below (|step| |w|)^3 = 10^5.
             assert abs(slope - exact) <= 1e-5 + 1e-9 * abs(exact)
+
+
+def test_types_that_rows_may_have():
+    t = torch.zeros(4, dtype=torch.int64)
+    for x, w in ((torch.ones(4, 8).double(), torch.ones(9, 8).double()), (torch.ones(4, 8), torch.ones(9, 8).half())):
+        with pytest.raises(ValueError, match='float'):
+            losses.linear_cross_entropy(x, w, t)
 
 
 def test_refusals_of_arguments():

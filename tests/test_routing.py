@@ -396,6 +396,17 @@ def test_slots_out_of_range_are_left_out(device):
 
 
 @pytest.mark.parametrize('device', DEVICES)
+def test_a_choice_without_a_row_adds_nothing_whatever_its_weight(device):
+    rows = torch.full((4, 8), math.nan, device=device)
+    rows[1] = 2.0
+    slots = torch.tensor([[1, -1], [4, 9]], dtype=torch.int32, device=device)
+    w = torch.tensor([[0.5, math.inf], [math.nan, -math.inf]], device=device)
+    res = torch.arange(16.0, device=device).view(2, 8)
+    want = res + torch.tensor([[1.0], [0.0]], device=device)
+    assert torch.equal(experts.combine(rows, slots, w, residual=res), want)
+
+
+@pytest.mark.parametrize('device', DEVICES)
 def test_only_the_wanted_gradients(device):
     x, y, slots, w, dout, _ = rows_data(10, 2, 16, torch.float32, device)
     full = [t.clone().requires_grad_(True) for t in (y, w, x)]
@@ -410,6 +421,17 @@ def test_only_the_wanted_gradients(device):
 
 
 # ------------------------------------------------------------------ refusals
+
+def test_types_that_rows_may_have():
+    slots, w = torch.zeros(4, 2, dtype=torch.int32), torch.ones(4, 2)
+    for bad in (torch.double, torch.long):
+        with pytest.raises(ValueError, match='float'):
+            experts.dispatch(torch.ones(4, 8).to(bad), slots)
+        with pytest.raises(ValueError, match='float'):
+            experts.combine(torch.ones(8, 8).to(bad), slots, w)
+    with pytest.raises(ValueError, match='residual'):
+        experts.combine(torch.ones(8, 8), slots, w, residual=torch.ones(4, 8).half())
+
 
 def test_refusals_of_arguments():
     z = torch.randn(4, 12)
