@@ -235,8 +235,8 @@ int launch_product(const avey::CeMaps& m, avey::CeGeom& q, Chain& chain) {
   if (attr != cudaSuccess) return fail(AVEY_ERR_CUDA, cudaGetErrorString(attr));
   q.units = 0;
   for (const avey::CeJob& j : q.job) q.units += j.units;
-  return chain.launch("cross entropy product", K, dim3(2 * static_cast<unsigned>(std::min<int64_t>(q.units, pairs()))), avey::kCeThreads,
-                      avey::kCeSmem, 2, m, q);
+  const dim3 grid(2 * static_cast<unsigned>(std::min<int64_t>(q.units, pairs())));
+  return chain.launch("cross entropy product", K, grid, avey::kCeThreads, avey::kCeSmem, 2, m, q);
 }
 
 avey::CeGeom geom(const AveyLossParams* p) {
@@ -308,7 +308,8 @@ int stats_few(const AveyLossParams* p, const Layout& l, Chain& chain) {
   q.ignore = p->ignore_index;
   q.partial = reinterpret_cast<float2*>(ws + l.partial);
   q.picked = reinterpret_cast<float*>(ws + l.picked);
-  return chain.launch("cross entropy of few rows", avey::ce_few<T>, dim3(static_cast<unsigned>(l.segments)), 32 * avey::kCfWarps, 0, 1, q);
+  const dim3 grid(static_cast<unsigned>(l.segments));
+  return chain.launch("cross entropy of few rows", avey::ce_few<T>, grid, 32 * avey::kCfWarps, 0, 1, q);
 }
 
 template <typename T>
@@ -348,7 +349,8 @@ int forward(const AveyLossParams* p, cudaStream_t stream) {
   r.lse = p->saved;
   r.per = 32;
   while (r.per > 1 && r.per / 2 >= p->rows) r.per /= 2;
-  rc = chain.launch("cross entropy rows", avey::ce_rows, dim3(static_cast<unsigned>((p->rows + r.per - 1) / r.per)), 256, 0, 1, r);
+  const dim3 blocks(static_cast<unsigned>((p->rows + r.per - 1) / r.per));
+  rc = chain.launch("cross entropy rows", avey::ce_rows, blocks, 256, 0, 1, r);
   if (rc != AVEY_OK || none) return rc;
   return chain.launch("cross entropy total", avey::ce_total, dim3(1), 1024, 0, 1, r, p->reduction == AVEY_LOSS_MEAN ? 1 : 0,
                       p->loss, p->saved ? p->saved + p->rows : nullptr);
@@ -390,7 +392,8 @@ int backward(const AveyLossParams* p, cudaStream_t stream) {
     k.copy_ld = up(p->width, 8);
     k.dirty = reinterpret_cast<uint8_t*>(ws + l.dirty);
   }
-  rc = chain.launch("cross entropy coefficients", avey::ce_coef<T>, dim3(static_cast<unsigned>((p->rows + 63) / 64)), 256, 0, 1, k);
+  const dim3 blocks(static_cast<unsigned>((p->rows + avey::kCeCoefRows - 1) / avey::kCeCoefRows));
+  rc = chain.launch("cross entropy coefficients", avey::ce_coef<T>, blocks, 256, 0, 1, k);
   if (rc != AVEY_OK) return rc;
   const int64_t sums_ld = up(p->width, 4);
   float* sums = reinterpret_cast<float*>(ws + l.sums);

@@ -8,7 +8,7 @@ import pytest
 import torch
 import torch.nn.functional as F
 
-from avey_kernel_b200 import _native
+from avey_kernel_b200 import _native, experts, layers, losses
 
 PATH = Path(__file__).resolve().parents[1] / 'examples' / 'train_block.py'
 spec = importlib.util.spec_from_file_location('train_block', PATH)
@@ -71,3 +71,58 @@ def test_gradients_of_the_example_model(device, dt):
         model(seq[:, :-1], seq[:, 1:]).backward()
         assert all(torch.equal(a, t.grad) for a, t in zip(first, model.parameters()))
         assert _native.device_status(clear=True) == 0
+
+
+def ends(dt, seed, tokens=300, width=72, vocab=700, num=4):
+    """Tokens in, two experts each, the loss: inputs, and a step that returns it and its gradients."""
+    gen = torch.Generator().manual_seed(seed)
+    new = lambda *shape: (torch.randn(*shape, generator=gen) / shape[-1] ** 0.5).cuda().to(dt).requires_grad_(True)  # noqa: E731
+    leaves = [new(vocab, width), new(num, width), new(num, width, width)]
+    ids = torch.randint(0, vocab, (tokens,), generator=gen).cuda()
+
+    def step(table, router, w):
+        h = layers.embedding(ids, table, scale=4.0)
+        weights, chosen = experts.route(h @ router.t(), 2)
+        slots, offsets = experts.arrange(chosen, num)
+        y = experts.expert_linear(experts.dispatch(h, slots), w, offsets, activation='silu')
+        h = experts.combine(y, slots, weights, residual=h)
+        return losses.linear_cross_entropy(h, table, ids.roll(-1), z_loss=1e-3)
+
+    def train():
+        loss = step(*leaves)
+        return [loss.detach(), *torch.autograd.grad(loss, leaves)]
+
+    return ids, leaves, step, train
+
+
+@pytest.mark.gpu
+def test_two_captured_steps_replayed_at_once():
+    (ids1, _, _, one), (ids2, _, _, two) = ends(torch.bfloat16, 0), ends(torch.float16, 1, tokens=9000, vocab=5000)
+    one(), two()
+    graphs, got = [torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()], []
+    for graph, train in zip(graphs, (one, two)):
+        with torch.cuda.graph(graph):
+            got.append(train())
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for i in range(3):
+        ids1.copy_(ids1.flip(0).roll(i))
+        ids2.copy_(ids2 % (5000 >> i))
+        for stream, graph in zip(streams, graphs):
+            stream.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(stream):
+                for _ in range(4):
+                    graph.replay()
+        for stream in streams:
+            torch.cuda.current_stream().wait_stream(stream)
+        for values, train in zip(got, (one, two)):
+            assert all(torch.equal(p, q) for p, q in zip(values, train()))
+    assert _native.device_status(clear=True) == 0
+
+
+@pytest.mark.gpu
+def test_compiled_functions_call_the_operators():
+    _, leaves, step, train = ends(torch.bfloat16, 2)
+    compiled = torch.compile(step, backend='eager')
+    loss = compiled(*leaves)
+    got = [loss.detach(), *torch.autograd.grad(loss, leaves)]
+    assert all(torch.equal(p, q) for p, q in zip(got, train()))
