@@ -13,15 +13,19 @@
 // all of the chosen at -inf the weights are zero.
 //
 // Scores in fp32 are off by some 10^-7 of themselves, and two experts may be closer than
-// that. Where the order of two that matter is within the error, the token is done again
-// in 64 bits, so the choice is the formula's. (Equal logits with equal biases are equal
-// in any precision and need no second look.)
+// that. Where the order of two that matter is within the error, a second look in 64 bits
+// decides, so the choice is the formula's: at the chosen experts and the next one alone, a lane
+// each, where no other is as near; else, and for groups, at all. (Equal logits with equal biases
+// are equal in any precision and need none.) A few tokens of thousands need one, but the
+// launch waits for them: with all ranks looked at again for each, 4093 tokens of 256 experts in 8
+// groups took 20 us instead of 12.7 (and 11.8 without any such token).
 //
 // Bound: the logits' bytes, or instructions. Without a bias and groups (route_plain) and
 // in the gradient a token takes as many lanes as give each 16 of its experts, so that a
 // warp's shuffles serve several tokens: 65536 tokens of 128 experts, the best 4, 25 us
 // forward and 18 backward, where a warp for each token took 39 and 23. With them a warp
-// takes a token, for the second look: 4093 tokens of 256 experts in 8 groups 22 us.
+// takes a token; few tokens leave it latency-bound, many its instructions (65536 of 256 experts
+// in 8 groups: 123 us; some 15% more with two blocks an SM for R = 8 instead of three).
 #pragma once
 
 #include <math_constants.h>
@@ -80,37 +84,27 @@ __device__ __forceinline__ void rt_load(const T* row, int e, int experts, bool v
   }
 }
 
-template <typename S>
-__device__ __forceinline__ S rt_exp(S x) {
-  if constexpr (sizeof(S) == 8) return exp(x);
-  else return expf(x);
-}
-
 // Scores of a lane's logits: the softmax needs the row's maximum and sum.
-template <typename S, int R>
-__device__ __forceinline__ void rt_scores(const float (&z)[R], bool softmax, S (&s)[R]) {
+template <int R>
+__device__ __forceinline__ void rt_scores(const float (&z)[R], bool softmax, float (&s)[R]) {
   if (softmax) {
     float top = z[0];
 #pragma unroll
     for (int i = 1; i < R; ++i) top = fmaxf(top, z[i]);
 #pragma unroll
     for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
-    const S base = top == -CUDART_INF_F ? S(0) : S(top);
-    S sum = 0;
+    const float base = top == -CUDART_INF_F ? 0.f : top;
+    float sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < R; ++i) sum += s[i] = rt_exp(S(z[i]) - base);
+    for (int i = 0; i < R; ++i) sum += s[i] = expf(z[i] - base);
 #pragma unroll
     for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
-    const S inv = sum > S(0) ? S(1) / sum : sum == S(0) ? S(0) : sum;  // no expert at all: zeros
+    const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;  // no expert at all: zeros
 #pragma unroll
     for (int i = 0; i < R; ++i) s[i] *= inv;
   } else {
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-      const S e = S(1) + rt_exp(-S(z[i]));
-      if constexpr (sizeof(S) == 8) s[i] = S(1) / e;
-      else s[i] = __fdividef(1.f, e);  // 0 past 2^126, as far as any order goes
-    }
+    for (int i = 0; i < R; ++i) s[i] = __fdividef(1.f, 1.f + expf(-z[i]));  // 0 past 2^126, as far as any order goes
   }
 }
 
@@ -228,49 +222,79 @@ __device__ __forceinline__ uint32_t rt_keep(const RtArgs& q, S merit, int lane, 
   return __ballot_sync(0xFFFFFFFFu, there && place < q.top_groups);
 }
 
-// Lane j's expert is the j-th chosen one, by scores in 64 bits. (It reads the logits again:
-// given them, it would have them kept in local memory by every token.)
+// The second looks, in 64 bits. They read the logits again: given them, they would have them kept
+// in local memory by every token.
+//
+// The softmax's maximum and sum.
+struct RtSoft {
+  double base, inv;
+};
 template <typename T, int R>
-__device__ __noinline__ int rt_choose64(const RtArgs& q, int64_t t, int lane) {
-  const int e0 = lane * R;
+__device__ __forceinline__ RtSoft rt_soft64(const RtArgs& q, const T* row, int lane) {
+  if (!q.softmax) return {0.0, 1.0};
   float z[R];
-  rt_load<T, R>(static_cast<const T*>(q.logits) + t * q.ld, e0, q.experts, q.vec, z);
-  const bool scored = q.bias || (q.groups > 1 && q.group_best == 2);
-  double r[R];
-  if (scored) rt_scores<double, R>(z, q.softmax, r);
-  unsigned long long key[R], by[R];  // by: what groups rank by
+  rt_load<T, R>(row, lane * R, q.experts, q.vec, z);
+  float top = z[0];
+#pragma unroll
+  for (int i = 1; i < R; ++i) top = fmaxf(top, z[i]);
+#pragma unroll
+  for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
+  const double base = top == -CUDART_INF_F ? 0.0 : top;
+  double sum = 0.0;
+#pragma unroll
+  for (int i = 0; i < R; ++i) sum += exp(z[i] - base);
+#pragma unroll
+  for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
+  return {base, sum > 0.0 ? 1.0 / sum : sum == 0.0 ? 0.0 : sum};
+}
+// An expert's rank, as a key.
+__device__ __forceinline__ unsigned long long rt_rank64(const RtArgs& q, const RtSoft& soft, float z, int expert) {
+  const double e = exp(q.softmax ? z - soft.base : -static_cast<double>(z));
+  double rank = q.softmax ? e * soft.inv : 1.0 / (1.0 + e);
+  if (q.bias) rank += static_cast<double>(__ldg(q.bias + expert));
+  return z == -CUDART_INF_F ? rt_key64(-CUDART_INF) : z != z ? 1ull : rt_key64(rank);
+}
+
+// The groups to choose from. A group takes as many lanes, a power of two, as there are for each.
+template <typename T, int R>
+__device__ __noinline__ uint32_t rt_keep64(const RtArgs& q, int64_t t, int lane) {
+  const T* row = static_cast<const T*>(q.logits) + t * q.ld;
+  const RtSoft soft = rt_soft64<T, R>(q, row, lane);
+  int lanes = 32;
+  while (lanes * q.groups > 32) lanes >>= 1;
+  const int size = q.experts / q.groups, group = lane / lanes, end = group < q.groups ? (group + 1) * size : 0;
+  unsigned long long first = 0ull, second = 0ull;
+#pragma unroll 4
+  for (int e = group * size + lane % lanes; e < end; e += lanes) {
+    const unsigned long long v = rt_rank64(q, soft, Elem<T>::load(row + e), e);
+    second = max(second, min(first, v));
+    first = max(first, v);
+  }
+  for (int d = lanes >> 1; d; d >>= 1) {
+    const unsigned long long f = __shfl_xor_sync(0xFFFFFFFFu, first, d), s = __shfl_xor_sync(0xFFFFFFFFu, second, d);
+    second = max(min(first, f), max(second, s));
+    first = max(first, f);
+  }
+  const int src = min(lane * lanes, 31);
+  const double best = rt_value64(__shfl_sync(0xFFFFFFFFu, first, src));
+  const double next = rt_value64(__shfl_sync(0xFFFFFFFFu, second, src));
+  int in, out;
+  return rt_keep(q, q.group_best == 2 && next > -CUDART_INF ? best + next : best, lane, in, out);
+}
+
+// Lane j's expert is the j-th chosen one, of the groups in `keep`.
+template <typename T, int R>
+__device__ __noinline__ int rt_choose64(const RtArgs& q, int64_t t, int lane, uint32_t keep) {
+  const int e0 = lane * R, size = q.experts / q.groups;
+  const T* row = static_cast<const T*>(q.logits) + t * q.ld;
+  const RtSoft soft = rt_soft64<T, R>(q, row, lane);
+  float z[R];
+  rt_load<T, R>(row, e0, q.experts, q.vec, z);
+  unsigned long long key[R];
 #pragma unroll
   for (int i = 0; i < R; ++i) {
-    key[i] = by[i] = 0ull;
-    if (e0 + i >= q.experts) continue;
-    const double own = scored ? r[i] : static_cast<double>(z[i]);
-    const double rank = q.bias ? own + static_cast<double>(__ldg(q.bias + e0 + i)) : own;
-    by[i] = z[i] == -CUDART_INF_F ? rt_key64(-CUDART_INF) : z[i] != z[i] ? 1ull : rt_key64(rank);
-    key[i] = q.bias ? by[i] : rt_key64(static_cast<double>(z[i]));
-  }
-  if (q.groups > 1) {
-    const int size = q.experts / q.groups;
-    double merit = -CUDART_INF;
-    for (int g = 0; g < q.groups; ++g) {
-      unsigned long long mine[R];
-#pragma unroll
-      for (int i = 0; i < R; ++i) mine[i] = (e0 + i) / size == g ? by[i] : 0ull;
-      int e;
-      double m = rt_value64(rt_best64<R>(mine, e0, e));
-      if (q.group_best == 2 && m > -CUDART_INF) {
-#pragma unroll
-        for (int i = 0; i < R; ++i)
-          if (e0 + i == e) mine[i] = 0ull;
-        const double second = rt_value64(rt_best64<R>(mine, e0, e));
-        if (second > -CUDART_INF) m += second;
-      }
-      if (lane == g) merit = m;
-    }
-    int in, out;
-    const uint32_t keep = rt_keep(q, merit, lane, in, out);
-#pragma unroll
-    for (int i = 0; i < R; ++i)
-      if (!(keep >> (min((e0 + i) / size, 31)) & 1u)) key[i] = 0ull;
+    const bool there = e0 + i < q.experts && (keep >> min((e0 + i) / size, 31) & 1u);
+    key[i] = there ? rt_rank64(q, soft, z[i], e0 + i) : 0ull;
   }
   int mine = 0;
   for (int j = 0; j < q.k; ++j) {
@@ -284,12 +308,33 @@ __device__ __noinline__ int rt_choose64(const RtArgs& q, int64_t t, int lane) {
   return mine;
 }
 
-// The same choice in 32 bits; false where two ranks that matter are too near to tell.
-// `most`: the largest |bias|; `row`: the logits, to compare two that are near.
+// The order of the experts that lanes 0 to n - 1 hold, a score each.
 template <typename T, int R>
-__device__ __forceinline__ bool rt_choose(const RtArgs& q, const T* row, const float (&z)[R], float most, int lane,
+__device__ __noinline__ int rt_order64(const RtArgs& q, int64_t t, int lane, int n, int expert) {
+  const T* row = static_cast<const T*>(q.logits) + t * q.ld;
+  const RtSoft soft = rt_soft64<T, R>(q, row, lane);
+  const unsigned long long key = lane < n ? rt_rank64(q, soft, Elem<T>::load(row + expert), expert) : 0ull;
+  int place = 0;
+  for (int i = 0; i < n; ++i) {
+    const unsigned long long other = __shfl_sync(0xFFFFFFFFu, key, i);
+    const int other_e = __shfl_sync(0xFFFFFFFFu, expert, i);
+    place += other > key || (other == key && other_e < expert);
+  }
+  int mine = 0;
+  for (int i = 0; i < n; ++i) {
+    const int e = __shfl_sync(0xFFFFFFFFu, expert, i);
+    if (__shfl_sync(0xFFFFFFFFu, place, i) == lane) mine = e;
+  }
+  return mine;
+}
+
+// The choice: lane j's expert is the j-th chosen one, and mz its logit. `most`: the largest |bias|.
+template <typename T, int R>
+__device__ __forceinline__ void rt_choose(const RtArgs& q, int64_t t, const float (&z)[R], float most, int lane,
                                           int& mine, float& mz) {
+  const T* row = static_cast<const T*>(q.logits) + t * q.ld;
   const int e0 = lane * R;
+  uint32_t keep = 0xFFFFFFFFu;
   const bool by_logit = !q.bias, sums = q.groups > 1 && q.group_best == 2;
   // Bounds of the errors of two ranks relative to their terms: the exponential and the
   // division (2^-21), the softmax's common sum of up to 32 + 5 additions (37 2^-24), the
@@ -297,12 +342,11 @@ __device__ __forceinline__ bool rt_choose(const RtArgs& q, const T* row, const f
   const float tol = q.softmax ? 4e-6f : 1e-6f;
   float r[R];
   uint32_t key[R];
-  bool sure = true;
   if (by_logit && !sums) {
 #pragma unroll
     for (int i = 0; i < R; ++i) r[i] = z[i];
   } else {
-    rt_scores<float, R>(z, q.softmax, r);
+    rt_scores<R>(z, q.softmax, r);
 #pragma unroll
     for (int i = 0; i < R; ++i) {
       if (q.bias && e0 + i < q.experts) r[i] += __ldg(q.bias + e0 + i);
@@ -355,12 +399,12 @@ __device__ __forceinline__ bool rt_choose(const RtArgs& q, const T* row, const f
     const bool two = q.group_best == 2 && second > -CUDART_INF_F;
     const float merit = two ? first + second : first;
     int in, out;
-    const uint32_t keep = rt_keep(q, merit, lane, in, out);
+    keep = rt_keep(q, merit, lane, in, out);
     if (q.top_groups < q.groups && !(by_logit && !sums)) {
       const float terms = fabsf(first) + (two ? fabsf(second) : 0.f) + 2.f * most;
       const float bound = tol * (__shfl_sync(0xFFFFFFFFu, terms, in) + __shfl_sync(0xFFFFFFFFu, terms, out));
       const float m_in = __shfl_sync(0xFFFFFFFFu, merit, in), m_out = __shfl_sync(0xFFFFFFFFu, merit, out);
-      sure = m_out == -CUDART_INF_F || !(m_in - m_out <= bound);
+      if (m_out > -CUDART_INF_F && m_in - m_out <= bound) keep = rt_keep64<T, R>(q, t, lane);
     }
     if (lanes) {
       if (!(keep >> min(lane / span, 31) & 1u)) {
@@ -376,29 +420,45 @@ __device__ __forceinline__ bool rt_choose(const RtArgs& q, const T* row, const f
   // The chosen, and with a bias the next one, from the best on.
   RtPool<R> pool;
   pool.fill(key, e0);
-  float before = 0.f;
-  int before_e = 0;
   const int rounds = by_logit ? q.k : min(q.k + 1, q.top_groups * (q.experts / q.groups));
   uint32_t mine_key = 0u;
+  float before = 0.f;
+  int before_e = 0;
+  // Near: two ranks whose order their errors may change. Alike: of equal logits and biases.
+  auto near = [&](float a, float b) { return b > -CUDART_INF_F && a - b <= tol * (fabsf(a) + fabsf(b) + 2.f * most); };
+  auto alike = [&](int a, int b) {
+    return Elem<T>::load(row + a) == Elem<T>::load(row + b) && __ldg(q.bias + a) == __ldg(q.bias + b);
+  };
+  bool order = false, last = false;  // near and not alike: any two, the last two
   for (int j = 0; j < rounds; ++j) {
     int e;
     const uint32_t top = pool.next(lane, e);
     if (!by_logit) {
       const float v = rt_value(top);
-      // Too near, unless they are alike.
-      if (j > 0 && v > -CUDART_INF_F && before - v <= tol * (fabsf(before) + fabsf(v) + 2.f * most))
-        sure = sure && Elem<T>::load(row + before_e) == Elem<T>::load(row + e) &&
-               __ldg(q.bias + before_e) == __ldg(q.bias + e);
+      last = j > 0 && near(before, v);
+      order = order || (last && !alike(before_e, e));
       before = v;
       before_e = e;
     }
-    if (lane == j && j < q.k) {
+    if (lane == j) {
       mine = e;
       mine_key = top;
     }
   }
+  if (!by_logit) {
+    // Where the last one is near the one before it, others that are left may be too.
+    bool full = false;
+    if (last) {
+      bool more = false;
+#pragma unroll
+      for (int i = 0; i < R; ++i)
+        if (near(before, rt_value(pool.key[i]))) more = more || order || !alike(before_e, pool.index[i]);
+      full = __any_sync(0xFFFFFFFFu, more) || (order && rounds > 32);
+    }
+    if (full) mine = rt_choose64<T, R>(q, t, lane, keep);
+    else if (order) mine = rt_order64<T, R>(q, t, lane, min(rounds, 32), mine);
+  }
   if (lane < q.k) mz = by_logit ? (mine_key == 1u ? CUDART_NAN_F : rt_value(mine_key)) : Elem<T>::load(row + mine);
-  return sure;
 }
 
 __device__ __forceinline__ float rt_log_sigmoid(float z) { return fminf(z, 0.f) - log1pf(expf(-fabsf(z))); }
@@ -513,7 +573,8 @@ __global__ void __launch_bounds__(32 * kRtWarps) route_plain(const __grid_consta
 }
 
 template <typename T, int R>
-__global__ void __launch_bounds__(32 * kRtWarps, R <= 4 ? 3 : R <= 8 ? 2 : 1) route_forward(const __grid_constant__ RtArgs q) {
+__global__ void __launch_bounds__(32 * kRtWarps, R <= 4 ? 4 : R <= 8 ? 3 : 1)
+    route_forward(const __grid_constant__ RtArgs q) {
   const int lane = threadIdx.x & 31, e0 = lane * R;
   float most = 0.f;  // the largest |bias|
   if (q.bias) {
@@ -533,11 +594,7 @@ __global__ void __launch_bounds__(32 * kRtWarps, R <= 4 ? 3 : R <= 8 ? 2 : 1) ro
       rt_load<T, R>(static_cast<const T*>(q.logits) + (t + step) * q.ld, e0, q.experts, q.vec, next);
     int mine = 0;
     float mz = 0.f;
-    const T* row = static_cast<const T*>(q.logits) + t * q.ld;
-    if (!rt_choose<T, R>(q, row, z, most, lane, mine, mz)) {
-      mine = rt_choose64<T, R>(q, t, lane);
-      if (lane < q.k) mz = Elem<T>::load(row + mine);
-    }
+    rt_choose<T, R>(q, t, z, most, lane, mine, mz);
     const bool in = lane < q.k;
     float w;
     if (q.softmax && !q.renormalize) {
@@ -642,7 +699,8 @@ __global__ void __launch_bounds__(32 * kRtWarps) route_backward(const __grid_con
           w[j] = __float_as_uint(d[at(i + j)]);
         } else {
           const T lo = Elem<T>::from_f(d[at(i + 2 * j)]), hi = Elem<T>::from_f(d[at(i + 2 * j + 1)]);
-          w[j] = *reinterpret_cast<const uint16_t*>(&lo) | static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(&hi)) << 16;
+          w[j] = *reinterpret_cast<const uint16_t*>(&lo) |
+                 static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(&hi)) << 16;
         }
       }
       *reinterpret_cast<uint4*>(out + i) = make_uint4(w[0], w[1], w[2], w[3]);

@@ -178,6 +178,29 @@ def test_near_scores_keep_the_order_of_exact_arithmetic(score, groups, device):
 
 
 @pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('n,groups,k', [(16, 1, 4), (64, 1, 5), (256, 1, 8), (512, 1, 32), (1000, 1, 3), (64, 4, 6),
+                                        (256, 8, 8), (60, 6, 7), (512, 16, 8)])
+@pytest.mark.parametrize('score', ['softmax', 'sigmoid'])
+def test_clusters_of_near_scores_at_the_border(score, n, groups, k, device):
+    """Rows with a cluster of two to six near ranks, some of them alike, among others that are far
+    apart: inside the chosen ones, over their last place and behind it, and between groups."""
+    g = torch.Generator().manual_seed(n + k)
+    rows = 300
+    z = torch.randn(rows, n, generator=g)
+    bias = torch.randint(0, 3, (n,), generator=g).float() * 2.0 ** -24
+    order = z.argsort(1, descending=True)
+    for t in range(rows):
+        size = 2 + t % 5
+        first = max(0, min(n - size, (k - 4 if groups == 1 else 0) + t // 5 % 8))
+        at = order[t, first:first + size]
+        z[t, at] = z[t, at[0]] * (1 + 2.0 ** -23 * torch.randint(0, 2, (size,), generator=g).float())
+    want = choose64(z, k, bias, score, groups, max(1, groups // 2), 2)
+    _, chosen = experts.route(z.to(device), k, bias=bias.to(device), score=score, groups=groups,
+                              top_groups=max(1, groups // 2), group_best=2)
+    assert torch.equal(chosen.cpu(), want)
+
+
+@pytest.mark.parametrize('device', DEVICES)
 @pytest.mark.parametrize('groups', [1, 4])
 @pytest.mark.parametrize('score', ['softmax', 'sigmoid'])
 @pytest.mark.parametrize('renormalize', [True, False])
