@@ -158,8 +158,6 @@ int sort_opt_in() {
     err[dev] = cudaFuncSetAttribute(avey::st_count, cudaFuncAttributeMaxDynamicSharedMemorySize, avey::kStSmem);
     if (err[dev] == cudaSuccess)
       err[dev] = cudaFuncSetAttribute(avey::st_place, cudaFuncAttributeMaxDynamicSharedMemorySize, avey::kStSmem);
-    if (err[dev] == cudaSuccess)
-      err[dev] = cudaFuncSetAttribute(avey::st_sort, cudaFuncAttributeMaxDynamicSharedMemorySize, avey::kStSmem);
   });
   return err[dev] == cudaSuccess ? AVEY_OK : fail(AVEY_ERR_CUDA, cudaGetErrorString(err[dev]));
 }
@@ -419,22 +417,16 @@ int embedding_backward(const AveyEmbeddingParams* p, cudaStream_t stream) {
   first.skip = p->padding >= 0 ? p->padding : -1;
   first.raw = p->tokens;
   first.raw64 = p->index_bits == 64;
-  if (pass_bytes == 0) {  // one block
-    rc = sort_opt_in();
-    if (rc != AVEY_OK) return rc;
+  if (pass_bytes == 0) {
     avey::StArgs q = first;
-    q.run = p->count;
-    q.blocks = 1;
-    q.passes = l.passes;
+    q.blocks = static_cast<int>((p->count + avey::kStRankEntries - 1) / avey::kStRankEntries);
     q.keys_out = words(l.keys[last]);
     q.ids_out = words(l.ids[last]);
-    q.more_keys = words(l.keys[last ^ 1]);
-    q.more_ids = words(l.ids[last ^ 1]);
     q.clear = edges;
     q.zeros = static_cast<uint8_t*>(p->dtable);
     q.zero_bytes = static_cast<int64_t>(table);
-    rc = chain.launch("sort", avey::st_sort, dim3(1u + zero_blocks(q.zero_bytes)), avey::kStThreads,
-                      sort_smem(q.buckets), 1, q);
+    const dim3 grid(static_cast<unsigned>(q.blocks + zero_blocks(q.zero_bytes)));
+    rc = chain.launch("sort", avey::st_rank, grid, avey::kStRankThreads, static_cast<int>(p->count) * 4, 1, q);
     if (rc != AVEY_OK) return rc;
   } else {
     const cudaError_t e = cudaMemsetAsync(ws + l.counts[1], 0, l.edges + 4 - l.counts[1], stream);

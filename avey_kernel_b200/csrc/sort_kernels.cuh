@@ -6,7 +6,8 @@
 // entry's place is the number of entries with a lower digit, of those with its own in
 // earlier blocks and warps, and of those before it in its warp (found 32 at a time by
 // matching digits over the warp). No atomics but on counts: the same input gives the same
-// order. Up to 8192 entries one block does it all; more take a launch that counts and one
+// order. Up to 8192 entries take one launch: of one block for one digit, or, for keys of more,
+// of blocks that compare each key with all (st_rank). More take a launch that counts and one
 // that places, which counts for the next digit. Blocks beside those, where the rest of the GPU
 // would idle, write zeros (a table's gradient, of which most rows are zero).
 //
@@ -24,7 +25,7 @@ constexpr int kStMaxBuckets = 1025;
 // around them took 295 us instead of 288, an embedding's of 65536 tokens 138 instead of 129;
 // with 1024: 288 and 132.)
 constexpr int kStRun = 2048;
-constexpr int kStOneBlock = 8192;  // entries that one block takes
+constexpr int kStOneBlock = 8192;  // entries that one block, or st_rank, takes
 constexpr int kStSteps = 8;        // keys a lane holds
 constexpr int kStSmem = (kStWarps + 1) * kStMaxBuckets * 4;
 
@@ -46,10 +47,7 @@ struct StArgs {
   int32_t* slots;         // the place of every entry
   int32_t* offsets;       // [buckets]: entries with a lower digit; or null
   uint32_t* next_counts;  // the next pass's [blocks][buckets], zero before: counted while placing; or null
-  uint32_t* more_keys;    // st_sort: room for the passes between, and how many there are
-  uint32_t* more_ids;
-  int passes;
-  uint32_t* clear;        // a word to be cleared, or null
+  uint32_t* clear;        // st_rank: a word to be cleared
   // Blocks past `blocks` write zeros to these bytes.
   uint8_t* zeros;
   int64_t zero_bytes;
@@ -67,7 +65,7 @@ __device__ __forceinline__ void st_zero(uint8_t* p, int64_t bytes, int64_t block
   if (threadIdx.x < tail) p[bytes - tail + threadIdx.x] = 0;
 }
 __device__ __forceinline__ uint32_t st_key(const StArgs& q, int64_t i) {
-  if (!q.raw) return __ldcg(q.keys + i);  // (written by this launch's block itself in st_sort)
+  if (!q.raw) return __ldcg(q.keys + i);
   const int64_t t = q.raw64 ? __ldg(static_cast<const long long*>(q.raw) + i)
                             : static_cast<int64_t>(__ldg(static_cast<const int32_t*>(q.raw) + i));
   return static_cast<uint32_t>(t < 0 || t >= q.limit || t == q.skip ? q.limit : t);
@@ -289,30 +287,51 @@ __global__ void __launch_bounds__(kStThreads) st_place(const StArgs q) {
   else st_zero(q.zeros, q.zero_bytes, blockIdx.x - q.blocks, gridDim.x - q.blocks);
 }
 
-// All passes of one block, which hands its entries to itself.
-__global__ void __launch_bounds__(kStThreads) st_sort(StArgs q) {
-  extern __shared__ uint32_t hist[];
-  __shared__ uint32_t warp_sums[kStWarps];
+// Up to kStOneBlock entries in one launch, whatever the keys: an entry's place is the number of
+// lower keys and of equal ones before it, counted over all keys by a warp for kStEach
+// entries. (Lookup and gradient of 8192 tokens of 768, vocabulary 32768: 39 us, with one block's
+// passes by digits 57; 2047 of 389, 32003: 21 and 27; 64 of 64, 1000: 8.9 and 9.7.)
+constexpr int kStRankThreads = 256, kStEach = 4, kStRankEntries = kStRankThreads / 32 * kStEach;
+__global__ void __launch_bounds__(kStRankThreads) st_rank(const StArgs q) {
+  extern __shared__ uint32_t hist[];  // the keys
   griddep_launch_dependents();
   griddep_wait();
-  if (blockIdx.x > 0) {
-    st_zero(q.zeros, q.zero_bytes, blockIdx.x - 1, gridDim.x - 1);
+  if (static_cast<int>(blockIdx.x) >= q.blocks) {
+    st_zero(q.zeros, q.zero_bytes, blockIdx.x - q.blocks, gridDim.x - q.blocks);
     return;
   }
-  if (threadIdx.x == 0 && q.clear) *q.clear = 0u;
-  // The last pass writes to keys_out, those before it to one place and the other in turn.
-  uint32_t* keys[2] = {q.keys_out, q.more_keys};
-  uint32_t* ids[2] = {q.ids_out, q.more_ids};
-  for (int pass = 0; pass < q.passes; ++pass) {
-    const int to = (q.passes - 1 - pass) & 1;
-    q.shift = 10 * pass;
-    q.keys_out = keys[to];
-    q.ids_out = ids[to];
-    st_place_block(q, hist, warp_sums);
-    __syncthreads();
-    q.raw = nullptr;
-    q.keys = keys[to];
-    q.ids = ids[to];
+  const int tid = threadIdx.x, lane = tid & 31, n = static_cast<int>(q.n);
+  if (blockIdx.x == 0 && tid == 0) *q.clear = 0u;
+#pragma unroll 4
+  for (int i = tid; i < n; i += kStRankThreads) hist[i] = st_key(q, i);
+  __syncthreads();
+  const int i0 = blockIdx.x * kStRankEntries + (tid >> 5) * kStEach, split = min(i0, n);
+  uint32_t mine[kStEach];
+  int count[kStEach] = {};
+#pragma unroll
+  for (int e = 0; e < kStEach; ++e) {
+    mine[e] = hist[min(i0 + e, n - 1)];
+#pragma unroll
+    for (int f = 0; f < e; ++f) count[e] += lane == 0 && mine[f] == mine[e];
+  }
+#pragma unroll 4
+  for (int j = lane; j < split; j += 32) {
+    const uint32_t k = hist[j];
+#pragma unroll
+    for (int e = 0; e < kStEach; ++e) count[e] += k <= mine[e];
+  }
+#pragma unroll 4
+  for (int j = split + lane; j < n; j += 32) {
+    const uint32_t k = hist[j];
+#pragma unroll
+    for (int e = 0; e < kStEach; ++e) count[e] += k < mine[e];
+  }
+#pragma unroll
+  for (int e = 0; e < kStEach; ++e) {
+    const int place = __reduce_add_sync(0xFFFFFFFFu, count[e]);
+    if (lane != e || i0 + e >= n) continue;
+    q.keys_out[place] = mine[e];
+    q.ids_out[place] = static_cast<uint32_t>(i0 + e);
   }
 }
 

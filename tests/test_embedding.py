@@ -136,7 +136,7 @@ def test_results_are_bitwise_reproducible_and_whole_numbers_exact():
 @pytest.mark.parametrize('n,vocab,width', [(8192, 1000, 24), (8193, 1000, 24), (9500, 1 << 20, 4), (20000, 1 << 20, 1),
                                            (38000, 777, 300), (40000, (1 << 20) + 7, 2)])
 def test_all_pieces_and_numbers_of_passes(n, vocab, width):
-    """One block's sort and many blocks', of one to three digits, with pieces of 8 to 32 places;
+    """The sort of one launch and that of many, of one to three digits, with pieces of 8 to 32 places;
     tokens from both ends of the vocabulary, one of them a quarter of all."""
     g = torch.Generator(device='cuda').manual_seed(n)
     t = torch.randint(0, vocab, (n,), generator=g, device='cuda')
