@@ -22,8 +22,8 @@ _FUNCTIONS = ('avey_adamw_v1', 'avey_linear_fwd_v1', 'avey_linear_bwd_v1',
               'avey_linear_workspace_size', 'avey_loss_fwd_v1', 'avey_loss_bwd_v1',
               'avey_loss_workspace_size', 'avey_route_fwd_v1', 'avey_route_bwd_v1', 'avey_arrange_v1',
               'avey_arrange_workspace_size', 'avey_dispatch_v1', 'avey_combine_v1',
-              'avey_combine_bwd_v1', 'avey_embedding_fwd_v1', 'avey_embedding_bwd_v1',
-              'avey_embedding_workspace_size', 'avey_last_error')
+              'avey_combine_bwd_v1', 'avey_rows_workspace_size', 'avey_embedding_fwd_v1',
+              'avey_embedding_bwd_v1', 'avey_embedding_workspace_size', 'avey_last_error')
 
 _lock = threading.Lock()
 _module = None

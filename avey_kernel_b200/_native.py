@@ -31,8 +31,8 @@ EXPORTS = ('avey_fwd_v1', 'avey_fwd_plan', 'avey_fwd_workspace_size', 'avey_fwd_
            'avey_linear_fwd_v1', 'avey_linear_bwd_v1', 'avey_linear_workspace_size',
            'avey_loss_fwd_v1', 'avey_loss_bwd_v1', 'avey_loss_workspace_size',
            'avey_route_fwd_v1', 'avey_route_bwd_v1', 'avey_arrange_v1', 'avey_arrange_workspace_size',
-           'avey_dispatch_v1', 'avey_combine_v1', 'avey_combine_bwd_v1', 'avey_embedding_fwd_v1',
-           'avey_embedding_bwd_v1', 'avey_embedding_workspace_size')
+           'avey_dispatch_v1', 'avey_combine_v1', 'avey_combine_bwd_v1', 'avey_rows_workspace_size',
+           'avey_embedding_fwd_v1', 'avey_embedding_bwd_v1', 'avey_embedding_workspace_size')
 SCORE_IDS = {'softmax': 0, 'sigmoid': 1}
 MAX_EXPERTS, MAX_CHOICES, MAX_GROUPS = 1024, 32, 32
 REDUCTION_IDS = {'none': 0, 'sum': 1, 'mean': 2}
@@ -264,7 +264,7 @@ class AveyRowsParams(ctypes.Structure):
         ('struct_size', ctypes.c_uint32),
         ('dtype', ctypes.c_int32),
         ('k', ctypes.c_int32),
-        ('reserved', ctypes.c_int32),
+        ('clear', ctypes.c_int32),
         ('tokens', ctypes.c_int64),
         ('width', ctypes.c_int64),
         ('slots', ctypes.c_void_p),
@@ -276,6 +276,8 @@ class AveyRowsParams(ctypes.Structure):
         ('out', ctypes.c_void_p),
         ('drows', ctypes.c_void_p),
         ('dweights', ctypes.c_void_p),
+        ('workspace', ctypes.c_void_p),
+        ('workspace_bytes', ctypes.c_uint64),
     ]
 
 
@@ -428,6 +430,7 @@ def lib() -> ctypes.CDLL:
                 getattr(dll, name).argtypes = [ctypes.POINTER(params), ctypes.c_void_p]
                 getattr(dll, name).restype = ctypes.c_int
         for name, params in (('avey_arrange_workspace_size', AveyArrangeParams),
+                             ('avey_rows_workspace_size', AveyRowsParams),
                              ('avey_embedding_workspace_size', AveyEmbeddingParams)):
             getattr(dll, name).argtypes = [ctypes.POINTER(params), ctypes.POINTER(ctypes.c_uint64)]
             getattr(dll, name).restype = ctypes.c_int

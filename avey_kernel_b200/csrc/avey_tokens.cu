@@ -4,6 +4,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <cstddef>
 #include <mutex>
 
 #include "avey_b200.h"
@@ -201,7 +202,8 @@ int validate(const AveyArrangeParams* p) {
 
 int validate(const AveyRowsParams* p, int what) {
   if (!p) return fail(AVEY_ERR_ARGUMENT, "params is NULL");
-  if (p->struct_size != sizeof(AveyRowsParams))
+  // (The block once ended before its workspace.)
+  if (p->struct_size != sizeof(AveyRowsParams) && p->struct_size != offsetof(AveyRowsParams, workspace))
     return fail(AVEY_ERR_ARGUMENT, "struct_size does not match sizeof(AveyRowsParams)");
   if (!known(p->dtype)) return fail(AVEY_ERR_ARGUMENT, "rows are f32, f16 or bf16");
   if (p->tokens < 0 || p->k < 1 || p->k > avey::kRwMaxK || p->tokens > (1ll << 30) / p->k || p->width < 1 ||
@@ -220,6 +222,12 @@ int validate(const AveyRowsParams* p, int what) {
   if (what == 2 && (!p->x || !p->weights || (p->dweights && !p->rows)))
     return fail(AVEY_ERR_ARGUMENT, "x (the gradient of out), weights and, for dweights, rows are required");
   return AVEY_OK;
+}
+
+// Workspace for the places that no slot names.
+uint64_t clear_bytes(const AveyRowsParams* p) {
+  const int64_t places = p->tokens * p->k;
+  return p->clear && places > avey::kRwBlankPlaces ? static_cast<uint64_t>(places) * 4 : 0;
 }
 
 // Bytes of an access that all rows are whole multiples of.
@@ -241,17 +249,18 @@ int part_lanes(int64_t width, int per) {
 template <typename T, int N, int HOLD>
 int launch_combine(const avey::RwArgs& q, int what, int lanes, Chain& chain) {
   const int64_t tokens = avey::kRwThreads / lanes;
-  const dim3 grid(static_cast<unsigned>(std::min<int64_t>(
-      (q.tokens + tokens - 1) / tokens, avey_host::multiprocessors() * static_cast<int64_t>(avey::rw_blocks(HOLD)))));
+  const dim3 grid(static_cast<unsigned>(
+      std::min<int64_t>((q.tokens + tokens - 1) / tokens,
+                        avey_host::multiprocessors() * static_cast<int64_t>(avey::rw_blocks(HOLD))) + q.blanks));
   if (what == 1) return chain.launch("combine", avey::rw_combine<T, N, HOLD>, grid, avey::kRwThreads, 0, 1, q, lanes);
   return chain.launch("combine gradient", avey::rw_combine_backward<T, N, HOLD>, grid, avey::kRwThreads, 0, 1, q, lanes);
 }
 
 template <typename T, int N>
-int launch_rows(const avey::RwArgs& q, int what, Chain& chain) {
+int launch_moves(const avey::RwArgs& q, int what, Chain& chain) {
   if (what == 0)
-    return chain.launch("dispatch", avey::rw_dispatch<T, N>, dim3(blocks_for(q.tokens * (q.width / N), 256)), 256, 0, 1,
-                        q);
+    return chain.launch("dispatch", avey::rw_dispatch<T, N>,
+                        dim3(q.blanks + blocks_for(q.tokens * (q.width / N), 256)), 256, 0, 1, q);
   if constexpr (sizeof(T) * N == 16) {
     const int lanes = part_lanes(q.width, N);
     switch ((q.width / N + lanes - 1) / lanes) {
@@ -264,16 +273,36 @@ int launch_rows(const avey::RwArgs& q, int what, Chain& chain) {
   return launch_combine<T, N, 2>(q, what, part_lanes(q.width, N), chain);
 }
 
+template <typename T, int N>
+int launch_rows(const avey::RwArgs& q, int what, Chain& chain) {
+  const int rc = launch_moves<T, N>(q, what, chain);
+  if (rc != AVEY_OK || !q.namer) return rc;
+  const int places = static_cast<int>(q.tokens * q.k);
+  T* rows = static_cast<T*>(what == 0 ? q.rows : q.out);
+  return chain.launch("clear places", avey::rw_clear<T, N>, dim3(blocks_for(places, 256)), 256, 0, 1, q.slots, q.namer,
+                      places, rows, what == 0 ? q.rows_ld : static_cast<int64_t>(q.width), q.width);
+}
+
 // what: 0 dispatch, 1 combine, 2 combine's backward.
 int run_rows(const AveyRowsParams* p, int what, void* stream) {
   int rc = validate(p, what);
   if (rc != AVEY_OK) return rc;
+  // combine writes no places, and the gradient of rows may not be wanted.
+  const bool clear = p->clear != 0 && (what == 0 || (what == 2 && p->drows));
+  const uint64_t need = clear ? clear_bytes(p) : 0;
+  if (need) {
+    if (p->struct_size != sizeof(AveyRowsParams)) return fail(AVEY_ERR_ARGUMENT, "clear needs the block's workspace");
+    rc = check_workspace(p->workspace, p->workspace_bytes, need);
+    if (rc != AVEY_OK) return rc;
+  }
   rc = avey_host::device_ok();
   if (rc != AVEY_OK || p->tokens == 0) return done(rc);
   avey::RwArgs q{};
   q.tokens = p->tokens;
   q.k = p->k;
   q.width = static_cast<int>(p->width);
+  q.blanks = clear && need == 0;
+  if (need) q.namer = static_cast<int32_t*>(p->workspace);
   q.slots = p->slots;
   q.x = p->x;
   q.x_ld = p->x_ld;
@@ -531,6 +560,20 @@ int avey_arrange_v1(const AveyArrangeParams* p, void* stream) {
   return done(launch_pass(q, chain));
 }
 
+int avey_rows_workspace_size(const AveyRowsParams* p, uint64_t* bytes) {
+  if (!p || !bytes) return fail(AVEY_ERR_ARGUMENT, "params or bytes is NULL");
+  AveyRowsParams sizes{};
+  sizes.struct_size = p->struct_size;
+  sizes.dtype = p->dtype;
+  sizes.k = p->k;
+  sizes.tokens = p->tokens;
+  sizes.width = p->width;
+  sizes.slots = p->slots;
+  const int rc = validate(&sizes, 3);
+  if (rc != AVEY_OK) return rc;
+  *bytes = clear_bytes(p);
+  return avey_host::clear_error();
+}
 int avey_dispatch_v1(const AveyRowsParams* p, void* stream) { return run_rows(p, 0, stream); }
 int avey_combine_v1(const AveyRowsParams* p, void* stream) { return run_rows(p, 1, stream); }
 int avey_combine_bwd_v1(const AveyRowsParams* p, void* stream) { return run_rows(p, 2, stream); }

@@ -108,20 +108,80 @@ struct RwArgs {
   const float* weights;   // [tokens][k], or null: 1
   void* out;              // [tokens], contiguous
   float* dweights;        // combine's backward, or null
+  int blanks;             // 1: the first block clears the places that no slot names (rw_blank)
+  int32_t* namer;         // or: [tokens k], the choice that names a place, for rw_clear
 };
+
+// Rows that no slot names are zeros, not what memory held before. Up to kRwBlankPlaces places:
+// a block ahead of the call's own reads the slots, marks the places that they name in a bit map in
+// shared memory and clears the others, waiting for nothing (16 tokens of two: 1.7 us for the launch
+// instead of 1.6). One block takes 60 us for 131072 slots beside
+// the rows' own traffic, so more places take a launch of their own (rw_clear).
+constexpr int kRwBlankPlaces = 8192;
+template <typename T, int N>
+__device__ __forceinline__ void rw_blank(const RwArgs& q, T* rows, int64_t ld) {
+  __shared__ uint32_t named[kRwBlankPlaces / 32];
+  const int places = static_cast<int>(q.tokens) * q.k, words = (places + 31) / 32;
+  for (int i = threadIdx.x; i < words; i += blockDim.x) named[i] = 0u;
+  __syncthreads();
+#pragma unroll 8
+  for (int i = threadIdx.x; i < places; i += blockDim.x) {
+    const int32_t s = __ldg(q.slots + i);
+    if (s >= 0 && s < places) atomicOr(named + (s >> 5), 1u << (s & 31));
+  }
+  __syncthreads();
+  const int lane = threadIdx.x & 31;
+  for (int w = threadIdx.x >> 5; w < words; w += static_cast<int>(blockDim.x >> 5)) {
+    const int left = places - 32 * w;
+    unsigned blank = ~named[w] & (left >= 32 ? 0xFFFFFFFFu : (1u << left) - 1);
+    for (; blank; blank &= blank - 1) {
+      T* row = rows + static_cast<int64_t>(32 * w + __ffs(blank) - 1) * ld;
+      for (int c = lane * N; c < q.width; c += 32 * N) rw_store<T, N>(row + c, rw_zero<T, N>());
+    }
+  }
+}
+
+// More places: the launch before has left in namer[p] the number of the choice that names p, and
+// where none does, whatever was there: if that is a choice whose slot is p then p is named after all, so
+// nothing has to be set up. A warp looks at 32 places. (131072 places: 2 us of dispatch and of combine's backward pass.)
+template <typename T, int N>
+__global__ void __launch_bounds__(256) rw_clear(const int32_t* slots, const int32_t* namer, int places, T* rows,
+                                                int64_t ld, int width) {
+  griddep_wait();
+  const int lane = threadIdx.x & 31, step = static_cast<int>(gridDim.x) * 256;
+  for (int p0 = static_cast<int>(blockIdx.x) * 256 + threadIdx.x - lane; p0 < places; p0 += step) {
+    const int p = p0 + lane;
+    bool blank = false;
+    if (p < places) {
+      const int32_t i = __ldcg(namer + p);
+      blank = i < 0 || i >= places || __ldg(slots + i) != p;
+    }
+    for (unsigned left = __ballot_sync(0xFFFFFFFFu, blank); left; left &= left - 1) {
+      T* row = rows + static_cast<int64_t>(p0 + __ffs(left) - 1) * ld;
+      for (int c = lane * N; c < width; c += 32 * N) rw_store<T, N>(row + c, rw_zero<T, N>());
+    }
+  }
+}
 
 template <typename T, int N>
 __global__ void __launch_bounds__(256) rw_dispatch(const RwArgs q) {
+  const int block = static_cast<int>(blockIdx.x) - q.blanks, blocks = static_cast<int>(gridDim.x) - q.blanks;
+  if (block < 0) {
+    rw_blank<T, N>(q, static_cast<T*>(q.rows), q.rows_ld);
+    return;
+  }
+  griddep_launch_dependents();
   const int per = q.width / N;
   const int64_t total = q.tokens * per, places = q.tokens * q.k;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < total;
-       i += static_cast<int64_t>(gridDim.x) * 256) {
+  for (int64_t i = static_cast<int64_t>(block) * 256 + threadIdx.x; i < total; i += static_cast<int64_t>(blocks) * 256) {
     const int64_t t = i / per;
     const int c = static_cast<int>(i - t * per) * N;
     const RwVec<T, N> v = rw_load<T, N>(static_cast<const T*>(q.x) + t * q.x_ld + c);
     for (int j = 0; j < q.k; ++j) {
       const int64_t s = __ldg(q.slots + t * q.k + j);
-      if (s >= 0 && s < places) rw_store<T, N>(static_cast<T*>(q.rows) + s * q.rows_ld + c, v);
+      if (s < 0 || s >= places) continue;
+      rw_store<T, N>(static_cast<T*>(q.rows) + s * q.rows_ld + c, v);
+      if (c == 0 && q.namer) q.namer[s] = static_cast<int32_t>(t * q.k + j);
     }
   }
 }
@@ -136,10 +196,10 @@ struct RwPart {
   int64_t t, step;
   int lane;
 };
-__device__ __forceinline__ RwPart rw_part(int lanes) {
+__device__ __forceinline__ RwPart rw_part(int lanes, int blanks = 0) {
   const int parts = kRwThreads / lanes;
-  return {static_cast<int64_t>(blockIdx.x) * parts + threadIdx.x / lanes, static_cast<int64_t>(gridDim.x) * parts,
-          static_cast<int>(threadIdx.x) & (lanes - 1)};
+  return {static_cast<int64_t>(blockIdx.x - blanks) * parts + threadIdx.x / lanes,
+          static_cast<int64_t>(gridDim.x - blanks) * parts, static_cast<int>(threadIdx.x) & (lanes - 1)};
 }
 // Slots and weights of up to kRwRows choices of a token from j0 on (past its last: no row).
 struct RwSlots {
@@ -212,7 +272,12 @@ __global__ void __launch_bounds__(kRwThreads, rw_blocks(HOLD)) rw_combine(const 
 // <dout_t, rows[slot_tj]>.
 template <typename T, int N, int HOLD>
 __global__ void __launch_bounds__(kRwThreads, rw_blocks(HOLD)) rw_combine_backward(const RwArgs q, int lanes) {
-  const RwPart at = rw_part(lanes);
+  if (static_cast<int>(blockIdx.x) < q.blanks) {
+    rw_blank<T, N>(q, static_cast<T*>(q.out), q.width);
+    return;
+  }
+  griddep_launch_dependents();
+  const RwPart at = rw_part(lanes, q.blanks);
   const unsigned mask = lanes == 32 ? 0xFFFFFFFFu : ((1u << lanes) - 1) << (threadIdx.x & 31 & ~(lanes - 1));
   const int64_t places = q.tokens * q.k;
   const T* rows = static_cast<const T*>(q.rows);
@@ -225,6 +290,11 @@ __global__ void __launch_bounds__(kRwThreads, rw_blocks(HOLD)) rw_combine_backwa
     for (int j0 = 0; j0 < q.k; j0 += kRwRows) {
       const RwSlots sl = j0 == 0 ? first : rw_slots(q, t, j0);
       float sum[kRwRows] = {};
+      if (at.lane == 0 && q.namer) {
+#pragma unroll
+        for (int j = 0; j < kRwRows; ++j)
+          if (sl.s[j] >= 0 && sl.s[j] < places) q.namer[sl.s[j]] = static_cast<int32_t>(t * q.k + j0 + j);
+      }
       for (int c0 = at.lane * N; c0 < q.width; c0 += span * HOLD) {
         RwVec<T, N> d[HOLD], v[kRwRows][HOLD];
 #pragma unroll

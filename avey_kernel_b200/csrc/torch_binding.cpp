@@ -41,6 +41,7 @@ struct Library {
   int (*dispatch)(const AveyRowsParams*, void*) = nullptr;
   int (*combine)(const AveyRowsParams*, void*) = nullptr;
   int (*combine_bwd)(const AveyRowsParams*, void*) = nullptr;
+  int (*rows_workspace)(const AveyRowsParams*, uint64_t*) = nullptr;
   int (*embedding_fwd)(const AveyEmbeddingParams*, void*) = nullptr;
   int (*embedding_bwd)(const AveyEmbeddingParams*, void*) = nullptr;
   int (*embedding_workspace)(const AveyEmbeddingParams*, uint64_t*) = nullptr;
@@ -723,6 +724,17 @@ void set_tokens(AveyRowsParams& p, const Tensor& x) {
   p.x_ld = row_ld(x, p.width);
 }
 
+// Places that no slot names get zeros: what a tensor held before never comes out.
+Tensor clear_places(AveyRowsParams& p, const Tensor& like) {
+  p.clear = 1;
+  uint64_t bytes = 0;
+  check_status(lib.rows_workspace(&p, &bytes));
+  const Tensor ws = byte_workspace(bytes, like);
+  if (bytes) p.workspace = ws.data_ptr();
+  p.workspace_bytes = bytes;
+  return ws;
+}
+
 Tensor dispatch_rows(const Tensor& x, const Tensor& slots) {
   const c10::cuda::CUDAGuard guard(x.device());
   const Tensor xr = as_rows(x, x.size(1)), s = slots.contiguous();
@@ -731,6 +743,7 @@ Tensor dispatch_rows(const Tensor& x, const Tensor& slots) {
   set_tokens(p, xr);
   p.rows = rows.data_ptr();
   p.rows_ld = p.width;
+  const Tensor ws = clear_places(p, x);
   check_status(lib.dispatch(&p, stream_of()));
   return rows;
 }
@@ -801,9 +814,11 @@ class CombineFunction : public torch::autograd::Function<CombineFunction> {
       out[2] = at::empty(s.sizes(), w.options());
       p.dweights = out[2].data_ptr<float>();
     }
+    Tensor ws;
     if (need_rows) {
       out[0] = at::empty({s.numel(), p.width}, dy.options());
       p.drows = out[0].data_ptr();
+      ws = clear_places(p, dy);
     }
     check_status(lib.combine_bwd(&p, stream_of()));
     return out;
@@ -945,6 +960,7 @@ void bind(const py::dict& addresses) {
   lib.dispatch = reinterpret_cast<decltype(lib.dispatch)>(at("avey_dispatch_v1"));
   lib.combine = reinterpret_cast<decltype(lib.combine)>(at("avey_combine_v1"));
   lib.combine_bwd = reinterpret_cast<decltype(lib.combine_bwd)>(at("avey_combine_bwd_v1"));
+  lib.rows_workspace = reinterpret_cast<decltype(lib.rows_workspace)>(at("avey_rows_workspace_size"));
   lib.embedding_fwd = reinterpret_cast<decltype(lib.embedding_fwd)>(at("avey_embedding_fwd_v1"));
   lib.embedding_bwd = reinterpret_cast<decltype(lib.embedding_bwd)>(at("avey_embedding_bwd_v1"));
   lib.embedding_workspace = reinterpret_cast<decltype(lib.embedding_workspace)>(at("avey_embedding_workspace_size"));

@@ -179,8 +179,8 @@ def arrange(chosen: torch.Tensor, num_experts: int) -> Tuple[torch.Tensor, torch
     all in the order of their experts, those of one expert in their given order, and
     ``offsets`` (int32, num_experts + 1) bounds each expert's places, as
     ``expert_linear`` takes them. Choices outside ``[0, num_experts)`` hold the places from
-    ``offsets[-1]`` on, where ``expert_linear`` gives zeros: so choices are dropped (not by
-    taking slots out, which would leave rows of ``dispatch`` unwritten)."""
+    ``offsets[-1]`` on, where ``expert_linear`` gives zeros: so choices are dropped (or by
+    slots outside ``[0, tokens k)``; the rows of their places are zeros then)."""
     if chosen.is_cuda:
         return _binding.module().arrange(chosen, num_experts)
     if chosen.dtype not in (torch.int32, torch.int64):
@@ -207,8 +207,10 @@ def _check_slots(slots, tokens=None):
 def dispatch(x: torch.Tensor, slots: torch.Tensor) -> torch.Tensor:
     """The tokens' rows in their experts' order: ``rows[slots[t, j]] = x[t]``, ``[tokens
     k, width]`` from x ``[tokens, width]`` (fp32, bf16 or f16, any row stride) and the
-    slots of ``arrange`` (each place once). CUDA tensors run natively, forward and backward
-    (a token's gradient is the sum of its rows', in fp32); CPU tensors take plain PyTorch."""
+    slots of ``arrange`` (each place once; a slot outside ``[0, tokens k)`` stands for no
+    place, and a place that no slot names gets zeros). CUDA tensors run natively, forward and
+    backward (a token's gradient is the sum of its rows', in fp32); CPU tensors take plain
+    PyTorch."""
     if x.is_cuda:
         return _binding.module().dispatch(x, slots)
     if x.ndim != 2 or x.shape[1] == 0 or x.dtype not in _FLOATS:
@@ -227,7 +229,8 @@ def combine(rows: torch.Tensor, slots: torch.Tensor, weights: torch.Tensor, *,
     """The experts' results back at their tokens: ``out[t] = residual[t] + sum_j
     weights[t, j] rows[slots[t, j]]``, ``[tokens, width]`` from rows ``[tokens k,
     width]`` (fp32, bf16 or f16, any row stride), the slots of ``arrange`` and fp32
-    weights ``[tokens, k]``; sums in fp32, in the order of j, rounded once. CUDA tensors
+    weights ``[tokens, k]``; sums in fp32, in the order of j, rounded once. A slot outside
+    ``[0, tokens k)`` adds nothing, and rows that no slot names get zero gradients. CUDA tensors
     run natively, forward and backward (gradients of rows, weights and residual);
     forward-mode tangents, traces and second differentiation raise. CPU tensors take
     plain PyTorch."""

@@ -602,8 +602,9 @@ AVEY_API int avey_arrange_workspace_size(const AveyArrangeParams* params, uint64
 
 /*
  * Rows of tokens to the places of their choices and back, with slots [tokens][k] that
- * hold each place in [0, tokens k) once (a slot outside it stands for no place: its choice
- * is left out; a place that no slot names is not written):
+ * hold each place in [0, tokens k) at most once (a slot outside it stands for no place: its
+ * choice is left out; a place that no slot names gets zeros with `clear`, and is not written
+ * without):
  *
  *   dispatch      rows[slots[t][j]] = x[t]
  *   combine       out[t] = x[t] (the residual, or 0 where x is NULL)
@@ -618,7 +619,7 @@ typedef struct AveyRowsParams {
   uint32_t struct_size; /* sizeof(AveyRowsParams) */
   int32_t dtype;        /* x, rows, out, drows: AVEY_F32, AVEY_F16 or AVEY_BF16 */
   int32_t k;            /* 1..32 */
-  int32_t reserved;
+  int32_t clear;        /* dispatch, combine_bwd: zeros for the places that no slot names */
   int64_t tokens, width; /* tokens x k up to 2^30, width up to 2^22 */
   const int32_t* slots;
   const void* x;
@@ -629,7 +630,13 @@ typedef struct AveyRowsParams {
   void* out;            /* combine: contiguous [tokens][width] */
   void* drows;          /* combine_bwd: contiguous [tokens k][width], or NULL */
   float* dweights;      /* combine_bwd: contiguous [tokens][k], or NULL */
+  void* workspace;      /* with clear: 256-byte aligned, >= avey_rows_workspace_size() bytes */
+  uint64_t workspace_bytes;
 } AveyRowsParams;
+
+/* Bytes of `workspace`: 0 without `clear` and up to 8192 places, else 4 a place. (A block that ends
+ * before `workspace` is taken too, where it needs none.) */
+AVEY_API int avey_rows_workspace_size(const AveyRowsParams* params, uint64_t* bytes);
 
 AVEY_API int avey_dispatch_v1(const AveyRowsParams* params, void* stream);
 AVEY_API int avey_combine_v1(const AveyRowsParams* params, void* stream);

@@ -443,6 +443,92 @@ def test_only_the_wanted_gradients(device):
         assert torch.equal(got, want[i])
 
 
+def poison(*shapes, dt, device):
+    """The allocator's next blocks of these sizes hold NaN."""
+    if device == 'cuda':
+        gone = [torch.full(shape, math.nan, dtype=dt, device=device) for shape in shapes for _ in range(3)]
+        del gone
+
+
+def check_dropped(tokens, k, width, dt, device, shift=0):
+    """A tenth of the slots out of range (and with them as many places without a name): the rows of
+    dispatch and the gradients are those of all slots where a place has a name, and zeros elsewhere."""
+    x, y, slots, w, dout, _ = rows_data(tokens, k, width, dt, device)
+    slots = torch.cat([slots.reshape(-1)[:shift], slots.reshape(-1)])[shift:].view(tokens, k)  # off 16 bytes
+    g = torch.Generator(device=device).manual_seed(1)
+    out = torch.rand(tokens, k, generator=g, device=device) < 0.1
+    out[-1, -1] = True
+    bad = torch.tensor([-1, tokens * k, 2 ** 31 - 1, -2 ** 31], device=device)[torch.arange(tokens * k, device=device) % 4]
+    gone = torch.cat([bad[:shift], torch.where(out.view(-1), bad, slots.view(-1))]).int()[shift:].view(tokens, k)
+    named = torch.zeros(tokens * k, dtype=torch.bool, device=device)
+    named[gone[~out].long()] = True
+    want = torch.where(named.unsqueeze(1), experts.dispatch(x, slots), 0)
+    leaves = [y.clone().requires_grad_(True), w.clone().requires_grad_(True)]
+    wanted = torch.autograd.grad(experts.combine(*[leaves[0], slots, leaves[1]]), leaves, dout)
+    poison((tokens * k, width), dt=dt, device=device)
+    rows = experts.dispatch(x, gone)
+    assert torch.equal(rows, want)
+    got = experts.combine(leaves[0], gone, leaves[1])
+    poison((tokens * k, width), dt=dt, device=device)
+    dy, dw = torch.autograd.grad(got, leaves, dout)
+    assert torch.equal(dy, torch.where(named.unsqueeze(1), wanted[0], 0))
+    assert torch.equal(dw, torch.where(out, 0, wanted[1]))
+    leaf = x.clone().requires_grad_(True)
+    dx, = torch.autograd.grad(experts.dispatch(leaf, gone), leaf, y)
+    # (Sums of k terms in fp32 in any order, rounded once.)
+    terms = y.double()[torch.where(out, 0, gone).long()].masked_fill(out.unsqueeze(2), 0)
+    value, size = terms.sum(1), terms.abs().sum(1)
+    close(dx, (value, (k + 1) * 2.0 ** -23 * size + UNIT[dt] * value.abs() * (1 + 2.0 ** -7) + TINY[dt]), 'dx')
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('dt', DTYPES)
+@pytest.mark.parametrize('tokens,k,width,shift', [(1, 1, 8, 0), (10, 2, 16, 0), (3, 1, 5, 1), (33, 32, 40, 3), (700, 3, 389, 2),
+                                                  (5000, 2, 64, 0)])
+def test_places_that_no_slot_names_are_zeros(tokens, k, width, shift, dt, device):
+    check_dropped(tokens, k, width, dt, device, shift)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('tokens,k,width,dt', [(33000, 4, 72, torch.float32), (140001, 8, 128, torch.bfloat16),
+                                               (140001, 8, 24, torch.float16), (600001, 2, 1, torch.float32)])
+def test_many_places_that_no_slot_names_are_zeros(tokens, k, width, dt):
+    """Cleared by a launch of its own, with rows of every access size."""
+    check_dropped(tokens, k, width, dt, 'cuda', 1)
+
+
+@pytest.mark.parametrize('device', DEVICES)
+def test_no_slot_names_a_place(device):
+    x, y, slots, w, dout, _ = rows_data(40, 3, 24, torch.float32, device)
+    leaf = y.clone().requires_grad_(True)
+    poison((120, 24), dt=torch.float32, device=device)
+    out = experts.combine(leaf, torch.full_like(slots, -1), w, residual=x)
+    dy, = torch.autograd.grad(out, leaf, dout)
+    assert torch.equal(out, x) and not dy.any()
+    poison((120, 24), dt=torch.float32, device=device)
+    assert not experts.dispatch(x, torch.full_like(slots, 120)).any()
+
+
+@pytest.mark.gpu
+def test_dropped_choices_in_captured_steps():
+    x, y, slots, w, dout, _ = rows_data(500, 4, 64, torch.bfloat16, 'cuda')
+    leaf, at = y.clone().requires_grad_(True), slots.clone()
+
+    def step():
+        return experts.dispatch(x, at), torch.autograd.grad(experts.combine(leaf, at, w), leaf, dout)[0]
+
+    step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for i in range(3):
+        at.copy_(torch.where(torch.arange(2000, device='cuda').view(500, 4) % (3 + i) == 0, -1, slots))
+        for t in got:
+            t.fill_(math.nan)
+        graph.replay()
+        assert all(torch.equal(a, b) and not a.isnan().any() for a, b in zip(got, step()))
+
+
 # ------------------------------------------------------------------ refusals
 
 def test_types_that_rows_may_have():
@@ -654,3 +740,27 @@ def test_c_rows_reject_bad_arguments_before_any_launch(call, change, match):
     lib = _native.lib()
     assert getattr(lib, f'avey_{call}_v1')(ctypes.byref(p), None) == -1
     assert match in lib.avey_last_error().decode()
+
+
+def test_c_rows_workspace():
+    at, lib = 1 << 20, _native.lib()
+
+    def rows(**kw):
+        p = _native.AveyRowsParams(struct_size=ctypes.sizeof(_native.AveyRowsParams), dtype=0, k=2, tokens=4096, width=8, slots=at,
+                                   x=at, x_ld=8, rows=at, rows_ld=8, weights=at, out=at, drows=at, clear=1)
+        for a, b in kw.items():
+            setattr(p, a, b)
+        return p
+
+    size = ctypes.c_uint64()
+    for kw, want in ((dict(), 0), (dict(tokens=4097), 4 * 8194), (dict(tokens=4097, clear=0), 0), (dict(tokens=0), 0),
+                     (dict(tokens=1 << 29), 1 << 32)):
+        assert lib.avey_rows_workspace_size(ctypes.byref(rows(**kw)), ctypes.byref(size)) == 0 and size.value == want
+    assert lib.avey_rows_workspace_size(None, ctypes.byref(size)) == -1
+    assert lib.avey_rows_workspace_size(ctypes.byref(rows(k=33)), ctypes.byref(size)) == -1
+    short = _native.AveyRowsParams.workspace.offset  # a block that ends before its workspace
+    for call in (lib.avey_dispatch_v1, lib.avey_combine_bwd_v1):
+        for kw, match in ((dict(tokens=4097), b'workspace'), (dict(tokens=4097, workspace=at, workspace_bytes=8), b'smaller'),
+                          (dict(tokens=4097, workspace=at + 4, workspace_bytes=1 << 20), b'aligned'),
+                          (dict(tokens=4097, struct_size=short), b'workspace'), (dict(struct_size=short - 8), b'struct_size')):
+            assert call(ctypes.byref(rows(**kw)), None) == -1 and match in lib.avey_last_error()
