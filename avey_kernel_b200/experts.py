@@ -244,6 +244,8 @@ def combine(rows: torch.Tensor, slots: torch.Tensor, weights: torch.Tensor, *,
     if residual is not None and (residual.shape != (slots.shape[0], rows.shape[1]) or residual.dtype != rows.dtype):
         raise ValueError(f"residual must have the rows' type and shape {[slots.shape[0], rows.shape[1]]}")
     named = (slots >= 0) & (slots < slots.numel())
-    mine = rows.float()[torch.where(named, slots, 0).long()] * weights.unsqueeze(-1)
-    out = torch.where(named.unsqueeze(-1), mine, 0.0).sum(1)
+    # A choice without a row: zeros on both sides of the product, so that neither a weight that is infinite nor
+    # the row in its stead reaches a result or a gradient.
+    mine = rows.float()[torch.where(named, slots, 0).long()].masked_fill(~named.unsqueeze(-1), 0.0)
+    out = (mine * weights.masked_fill(~named, 0.0).unsqueeze(-1)).sum(1)
     return (out if residual is None else out + residual.float()).to(rows.dtype)

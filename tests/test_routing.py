@@ -430,6 +430,23 @@ def test_a_choice_without_a_row_adds_nothing_whatever_its_weight(device):
 
 
 @pytest.mark.parametrize('device', DEVICES)
+def test_a_choice_without_a_row_has_no_gradient_whatever_its_weight(device):
+    rows = torch.full((4, 8), math.nan, device=device)
+    rows[1] = 2.0
+    slots = torch.tensor([[1, -1], [4, 9]], dtype=torch.int32, device=device)
+    for filler in (math.nan, 3.0):
+        rows[0] = filler
+        for weight in (math.inf, math.nan, 1.0):
+            leaves = [rows.clone().requires_grad_(True), torch.full((2, 2), weight, device=device)]
+            leaves[1][0, 0] = 0.5
+            leaves[1].requires_grad_(True)
+            dy = torch.tensor([[1.0], [math.nan]], device=device).expand(2, 8)
+            drows, dw = torch.autograd.grad(experts.combine(leaves[0], slots, leaves[1]), leaves, dy)
+            assert torch.equal(drows, torch.tensor([0.0, 0.5, 0.0, 0.0], device=device).unsqueeze(1).expand(4, 8))
+            assert torch.equal(dw, torch.tensor([[16.0, 0.0], [0.0, 0.0]], device=device))
+
+
+@pytest.mark.parametrize('device', DEVICES)
 def test_only_the_wanted_gradients(device):
     x, y, slots, w, dout, _ = rows_data(10, 2, 16, torch.float32, device)
     full = [t.clone().requires_grad_(True) for t in (y, w, x)]
