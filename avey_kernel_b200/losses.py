@@ -33,7 +33,8 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, targets: torch.T
     or the gradients, whatever x holds there, and ``z_loss`` (usually about 1e-4)
     keeps the log sums near zero. ``reduction`` is 'none' (losses of targets'
     shape), 'sum' or 'mean' (over the rows that are not ignored; NaN when all are).
-    A target outside the vocabulary makes its row's loss NaN.
+    A target outside the vocabulary makes its row's loss NaN, and with it the row's gradient and
+    the weight's.
 
     bf16 / f16 CUDA tensors of one dtype run natively, forward and backward, with
     any row strides: fp32 sums, the gradient at the logits rounded to the operand
@@ -67,7 +68,8 @@ def _cross_entropy_torch(x, weight, targets, ignore_index, reduction, z_loss):
     lse = torch.logsumexp(z, dim=-1)
     picked = z.gather(-1, torch.where(inside, targets, 0).long().unsqueeze(-1)).squeeze(-1)
     each = lse - picked + z_loss * lse.square()
-    each = torch.where(used, torch.where(inside, each, math.nan), 0.0)
+    # (A factor, not a choice: the NaN of a bad target goes into the gradients too.)
+    each = torch.where(used, each * torch.where(used & ~inside, math.nan, 1.0), 0.0)
     if reduction == 'none':
         return each
     return each.sum() if reduction == 'sum' else each.sum() / used.sum()

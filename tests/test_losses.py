@@ -253,6 +253,27 @@ def test_bad_targets_and_bad_rows_show_in_their_own_loss(rows, device):
     assert got[1] == 0 and got[2].isnan()
 
 
+@pytest.mark.parametrize('device', ['cpu', pytest.param('cuda', marks=pytest.mark.gpu)])
+@pytest.mark.parametrize('reduction', ['none', 'sum', 'mean'])
+@pytest.mark.parametrize('rows', [8, 300])
+def test_bad_targets_show_in_the_gradients(rows, reduction, device):
+    """NaN in the rows' own dx and in all of dw, which sums over them; the other rows' dx is that of a
+    call that ignores them (but for the mean's count)."""
+    dt = torch.float32 if device == 'cpu' else torch.bfloat16
+    x, w, t, _ = data(rows, 72, 400, dt, 6, ignored=0.2, device=device)
+    t[0], t[5:8] = 3, IGNORE
+    for bad in (400, -1, 1 << 40):
+        t[2], t[rows - 2] = bad, IGNORE
+        dy = torch.ones((rows,) if reduction == 'none' else (), device=device)
+        loss, dx, dw = run(x, w, t, dy, reduction=reduction)
+        _, want, finite = run(x, w, torch.where(t == bad, IGNORE, t), dy, reduction=reduction)
+        assert (loss[2] if reduction == 'none' else loss).isnan()
+        assert dx[2].isnan().all() and dw.isnan().all() and finite.isfinite().all()
+        dx[2] = 0
+        assert torch.equal(dx, want) if reduction != 'mean' else dx.isfinite().all()
+        assert not dx[t == IGNORE].any() and dx[0].any()
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize('dt', DTYPES)
 @pytest.mark.parametrize('rows', [5, 400])
