@@ -103,7 +103,8 @@ def route(logits: torch.Tensor, k: int, *, bias: Optional[torch.Tensor] = None,
 
     The choice is the formula's also where scores are nearer than fp32 tells. A logit of
     -inf takes an expert out: it ranks below all others and its weight is 0 (zeros for a
-    token whose logits all are). NaN ranks last.
+    token whose logits all are). NaN ranks last; it or +inf makes a softmax NaN, in its weights
+    and their gradients, and NaN a sigmoid where it is chosen.
 
     CUDA tensors run natively, forward and backward (the weights' gradient goes to the
     logits); forward-mode tangents, traces and second differentiation raise. CPU
@@ -157,17 +158,18 @@ def _route_torch(logits, k, bias, score, groups, top_groups, group_best, renorma
         chosen = order[..., :k]
     z = logits.float()
     if renormalize:
-        logs = z if score == 'softmax' else F.logsigmoid(z)
-        logs = logs.gather(-1, chosen)
+        logs = z.gather(-1, chosen)
+        logs = logs if score == 'softmax' else F.logsigmoid(logs)
         none = (logs == -math.inf).all(-1, keepdim=True)
         w = torch.softmax(logs.masked_fill(none, 0.0), -1).masked_fill(none, 0.0)
         if score == 'softmax':
-            w = torch.where((z.isnan() | (z == math.inf)).any(-1, keepdim=True), math.nan, w)
+            # (A factor, not a choice: the NaN goes into the gradients too.)
+            w = w * torch.where((z.isnan() | (z == math.inf)).any(-1, keepdim=True), math.nan, 1.0)
     elif score == 'softmax':
         none = (z == -math.inf).all(-1, keepdim=True)
         w = torch.softmax(z.masked_fill(none, 0.0), -1).masked_fill(none, 0.0).gather(-1, chosen)
     else:
-        w = torch.sigmoid(z).gather(-1, chosen)
+        w = torch.sigmoid(z.gather(-1, chosen))
     return w * scale, chosen.to(torch.int32)
 
 

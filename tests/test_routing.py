@@ -242,6 +242,39 @@ def test_infinities_and_nan(score, renormalize, groups, biased, device):
 
 
 @pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('groups', [1, 4])
+@pytest.mark.parametrize('score', ['softmax', 'sigmoid'])
+@pytest.mark.parametrize('renormalize', [True, False])
+def test_gradients_of_nan_and_infinite_logits(score, renormalize, groups, device):
+    """A softmax over a row with NaN or +inf is NaN, and so are its gradients: those of the chosen
+    ones' with renormalised weights, else all. A sigmoid's NaN shows where it is chosen: in all that
+    its sum divides, else in its own. It adds nothing where it is not chosen."""
+    n, k = 16, 5
+    z = torch.randn(7, n, generator=torch.Generator().manual_seed(2))
+    z[0, 7] = math.nan          # not chosen: it ranks last
+    z[1, 2] = INF
+    z[2, 3:] = math.nan         # fewer others than are chosen
+    z[3] = math.nan
+    z[4, 1], z[4, 2:9] = math.nan, -INF
+    z[5, ::2] = -INF
+    leaf = z.to(device).requires_grad_(True)
+    w, chosen = experts.route(leaf, k, score=score, renormalize=renormalize, groups=groups, group_best=2,
+                              top_groups=2 if groups > 1 else 1)
+    dz, = torch.autograd.grad(w, leaf, torch.randn(7, k, generator=torch.Generator().manual_seed(3)).to(device))
+    w, dz, chosen = w.detach().cpu(), dz.cpu(), chosen.cpu().long()
+    mine = torch.zeros_like(z, dtype=torch.bool).scatter_(1, chosen, True)
+    if score == 'softmax':
+        bad = (z.isnan() | (z == INF)).any(1, keepdim=True)
+        want_w, want_z = bad.expand_as(w), bad & mine if renormalize else bad.expand_as(z)
+    else:
+        bad = z.gather(1, chosen).isnan()
+        bad = bad.any(1, keepdim=True).expand_as(bad) if renormalize else bad
+        want_w, want_z = bad, torch.zeros_like(mine).scatter_(1, chosen, bad)
+    assert torch.equal(w.isnan(), want_w) and torch.equal(dz.isnan(), want_z)
+    assert not dz[~mine & ~want_z].any() or (score == 'softmax' and not renormalize)
+
+
+@pytest.mark.parametrize('device', DEVICES)
 def test_renormalised_weights_where_scores_underflow(device):
     z = torch.full((2, 8), -200.0)
     z[1, 0] = 300.0
