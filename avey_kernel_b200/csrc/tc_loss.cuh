@@ -821,13 +821,17 @@ __global__ void __launch_bounds__(256) ce_rows(const CeRows q) {
     __syncthreads();
   }
   if (y != 0 || row >= q.rows) return;
-  constexpr float kLn2 = 0.6931471805599453f;
+  constexpr float kLn2 = 0.6931471805599453f, kLog2e = 1.4426950408889634f;
   const float2 v = part[threadIdx.x];
-  const float lse2 = v.x + log2f(v.y), lse = lse2 * kLn2;
+  const float log2s = log2f(v.y), lse2 = v.x + log2s, lse = lse2 * kLn2;
   const int t = ce_target(q.targets, q.target_stride, q.target64, q.ignore, q.vocab, row);
   float loss = 0.f;
   if (t >= 0) {
-    loss = lse - q.picked[row];
+    // The maximum and the target's z are subtracted before the sum's logarithm is added: the
+    // log sum is rounded at the logits' size (by 10^-5 at 400), the loss of a row that is sure of its
+    // target is far below that. It is never negative, which the rounding of s may make it.
+    loss = kLn2 * (fmaf(-q.picked[row], kLog2e, v.x) + log2s);
+    if (loss < 0.f) loss = 0.f;
     if (q.z_loss != 0.f) loss = fmaf(q.z_loss * lse, lse, loss);
   } else if (t == -2) {
     loss = __int_as_float(0x7fc00000);

@@ -65,9 +65,10 @@ def _cross_entropy_torch(x, weight, targets, ignore_index, reduction, z_loss):
     used = targets != ignore_index
     inside = (targets >= 0) & (targets < weight.shape[0])
     z = F.linear(x.masked_fill(~used.unsqueeze(-1), 0).float(), weight.float())
-    lse = torch.logsumexp(z, dim=-1)
-    picked = z.gather(-1, torch.where(inside, targets, 0).long().unsqueeze(-1)).squeeze(-1)
-    each = lse - picked + z_loss * lse.square()
+    # (log_softmax subtracts the largest logit first: the log sum would be rounded at its size.)
+    each = -F.log_softmax(z, dim=-1).gather(-1, torch.where(inside, targets, 0).long().unsqueeze(-1)).squeeze(-1)
+    if z_loss != 0.0:
+        each = each + z_loss * torch.logsumexp(z, dim=-1).square()
     # (A factor, not a choice: the NaN of a bad target goes into the gradients too.)
     each = torch.where(used, each * torch.where(used & ~inside, math.nan, 1.0), 0.0)
     if reduction == 'none':

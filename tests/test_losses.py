@@ -274,6 +274,35 @@ def test_bad_targets_show_in_the_gradients(rows, reduction, device):
         assert not dx[t == IGNORE].any() and dx[0].any()
 
 
+def sure(rows, top, device, dt, vocab=512, far=10.0, seed=0):
+    """Rows whose target's logit is about `top` and all others' about `far` below it or lower; logits
+    are x itself, bit for bit (the weight is the identity)."""
+    g = torch.Generator(device=device).manual_seed(seed)
+    t = torch.randint(0, vocab, (rows,), generator=g, device=device)
+    x = top - far - 4 * torch.rand(rows, vocab, generator=g, device=device)
+    x = x.masked_fill(torch.rand(rows, vocab, generator=g, device=device) < 0.7, 0.0)
+    x[torch.arange(rows, device=device), t] = top
+    return x.to(dt), torch.eye(vocab, device=device, dtype=dt), t
+
+
+@pytest.mark.parametrize('device', ['cpu', pytest.param('cuda', marks=pytest.mark.gpu)])
+@pytest.mark.parametrize('top', [30, 96, 416, 4096])
+@pytest.mark.parametrize('rows', [8, 300])
+def test_losses_of_sure_rows_keep_their_digits_whatever_the_logits_size(rows, top, device):
+    """The sum of the powers is 1 and a little: its terms are off by 2^-22 of themselves, and
+    some 40 additions at its size by 2^-24 each (16 of a chunk of 32 columns, one for each further one,
+    two for each of the four column parts and eight warps that are joined); the logarithm, the difference and
+    ln 2 by 2^-22 in all. No term grows with the logits."""
+    x, w, t = sure(rows, top, device, torch.float32 if device == 'cpu' else torch.bfloat16)
+    z = x.double()
+    want = torch.logsumexp(z - z.gather(1, t[:, None]), 1)
+    assert float(want.min()) < 2.0 ** -6  # (bf16 rounds the logits' distances)
+    got = losses.linear_cross_entropy(x, w, t, reduction='none')
+    assert (got >= 0).all()
+    bound = 2.0 ** -22 * (1 + want) + 40 * 2.0 ** -24 * (1 + want) + 2.0 ** -22 * (1 + want)
+    assert ((got.double() - want).abs() <= bound).all(), float(((got.double() - want).abs() / bound).max())
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize('dt', DTYPES)
 @pytest.mark.parametrize('rows', [5, 400])
