@@ -219,6 +219,7 @@ class AveyLossParams(ctypes.Structure):
         ('dweight', ctypes.c_void_p),
         ('workspace', ctypes.c_void_p),
         ('workspace_bytes', ctypes.c_uint64),
+        ('saved_low', ctypes.c_void_p),
     ]
 
 

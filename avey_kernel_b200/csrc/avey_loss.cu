@@ -4,6 +4,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <cstddef>
 #include <cstdio>
 #include <mutex>
 
@@ -37,9 +38,12 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) ==
 bool whole_rows(const void* p, int64_t ld) { return aligned16(p) && ld % 8 == 0; }
 int64_t up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
 
+float* saved_low(const AveyLossParams* p) { return p->struct_size == sizeof(AveyLossParams) ? p->saved_low : nullptr; }
+
 int validate(const AveyLossParams* p, bool backward) {
   if (!p) return fail(AVEY_ERR_ARGUMENT, "params is NULL");
-  if (p->struct_size != sizeof(AveyLossParams))
+  // (The block once ended before saved_low.)
+  if (p->struct_size != sizeof(AveyLossParams) && p->struct_size != offsetof(AveyLossParams, saved_low))
     return fail(AVEY_ERR_ARGUMENT, "struct_size does not match sizeof(AveyLossParams)");
   if (p->dtype != AVEY_BF16 && p->dtype != AVEY_F16)
     return fail(AVEY_ERR_ARGUMENT, "the cross entropy takes bf16 or f16 operands");
@@ -57,7 +61,7 @@ int validate(const AveyLossParams* p, bool backward) {
   for (const void* a : {p->x, p->weight, const_cast<const void*>(p->dx), const_cast<const void*>(p->dweight)})
     odd |= reinterpret_cast<uintptr_t>(a) & 1u;
   for (const void* a : {static_cast<const void*>(p->loss), static_cast<const void*>(p->saved),
-                        static_cast<const void*>(p->dloss)})
+                        static_cast<const void*>(saved_low(p)), static_cast<const void*>(p->dloss)})
     odd |= reinterpret_cast<uintptr_t>(a) & 3u;
   if (odd != 0 || (reinterpret_cast<uintptr_t>(p->targets) & (p->target_bits / 8 - 1)) != 0)
     return fail(AVEY_ERR_ARGUMENT, "arrays must be aligned to their elements");
@@ -347,6 +351,7 @@ int forward(const AveyLossParams* p, cudaStream_t stream) {
   const bool none = p->reduction == AVEY_LOSS_NONE;
   r.each = none ? p->loss : reinterpret_cast<float*>(ws + l.each);
   r.lse = p->saved;
+  r.low = saved_low(p);
   r.per = 32;
   while (r.per > 1 && r.per / 2 >= p->rows) r.per /= 2;
   const dim3 blocks(static_cast<unsigned>((p->rows + r.per - 1) / r.per));
@@ -379,6 +384,7 @@ int backward(const AveyLossParams* p, cudaStream_t stream) {
   k.target64 = p->target_bits == 64;
   k.ignore = p->ignore_index;
   k.lse = p->saved;
+  k.low = saved_low(p);
   k.count = p->reduction == AVEY_LOSS_MEAN ? p->saved + p->rows : nullptr;
   k.dy = p->dloss;
   k.dy_stride = p->reduction == AVEY_LOSS_NONE ? p->dloss_stride : 0;

@@ -8,8 +8,8 @@
 //   dX     dx (+)= dz W over the piece       dW    dW = dz^T x for the piece
 //
 // c is the running maximum, so every power is at most 1; lse_i = c + log2 s is
-// kept in base 2, as the hardware's exponential takes it. a_i and b_i hold the
-// gradient that comes in, the z loss's factor and a scale that dX and dW divide by
+// kept in base 2, as the hardware's exponential takes it, with what its rounding left
+// out, which goes into a_i. a_i and b_i hold the gradient that comes in, the z loss's factor and a scale that dX and dW divide by
 // (CeScale). dz is rounded to the operand type once, as the tensor cores need it; all
 // sums are fp32.
 //
@@ -781,6 +781,7 @@ struct CeRows {
   float z_loss;
   float* each;             // losses of the rows
   float* lse;              // [rows], base 2
+  float* low;              // [rows]: what its rounding left of it; or null
   int per;                 // rows of a block, a power of two up to 32
 };
 
@@ -838,6 +839,10 @@ __global__ void __launch_bounds__(256) ce_rows(const CeRows q) {
   }
   q.each[row] = loss;
   if (q.lse) q.lse[row] = lse2;
+  if (q.low) {
+    const float added = lse2 - v.x;
+    q.low[row] = (v.x - (lse2 - added)) + (log2s - added);
+  }
 }
 
 // The sum or mean of the rows' losses, in 64 bits and a fixed order; *count: the
@@ -882,6 +887,7 @@ struct CeCoef {
   int target64;
   int64_t ignore;
   const float* lse;
+  const float* low;        // the log sums' low parts, or null
   const float* count;      // mean: the bits of the number of rows, else null
   const float* dy;
   int64_t dy_stride;       // 0: one value
@@ -920,6 +926,9 @@ __global__ void __launch_bounds__(256) ce_coef(const CeCoef q) {
         if (t == -2) g = __int_as_float(0x7fc00000);
         b = g;
         a = q.z_loss != 0.f ? g * fmaf(2.f * q.z_loss, __ldg(q.lse + row) * kLn2, 1.f) : g;
+        // The powers are relative to the rounded log sum, which is off by 10^-5 at logits of 400: a
+        // row that is sure of its target has a gradient p - 1 far below that.
+        if (q.low) a *= exp2f(-__ldg(q.low + row));
       }
       q.coef[row] = make_float2(a, b);
     }

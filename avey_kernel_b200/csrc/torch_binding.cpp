@@ -469,6 +469,11 @@ struct LossRows {
   }
 };
 
+void set_saved(AveyLossParams& p, const Tensor& saved) {
+  p.saved = saved.data_ptr<float>();
+  p.saved_low = p.saved + p.rows + 1;
+}
+
 // The loss and, with keep, what the backward pass needs of it.
 std::pair<Tensor, Tensor> loss_forward(const Tensor& x, const Tensor& weight, const Tensor& targets, int64_t ignore,
                                        int64_t reduction, double z_loss, bool keep) {
@@ -480,8 +485,8 @@ std::pair<Tensor, Tensor> loss_forward(const Tensor& x, const Tensor& weight, co
   Tensor loss = reduction == AVEY_LOSS_NONE ? at::empty(targets.sizes(), f32) : at::empty({}, f32), saved;
   p.loss = loss.data_ptr<float>();
   if (keep) {
-    saved = at::empty({p.rows + 1}, f32);
-    p.saved = saved.data_ptr<float>();
+    saved = at::empty({2 * p.rows + 1}, f32);
+    set_saved(p, saved);
   }
   const Tensor ws = loss_workspace(p, 0, x);
   check_status(lib.loss_fwd(&p, at::cuda::getCurrentCUDAStream().stream()));
@@ -516,7 +521,7 @@ class LossFunction : public torch::autograd::Function<LossFunction> {
     AveyLossParams p = loss_params(x, t.size(0), weight.size(1), weight.size(0), t, call[0], call[1],
                                    ctx->saved_data["z_loss"].toDouble());
     const LossRows rows(p, x, weight);
-    p.saved = saved[3].data_ptr<float>();
+    set_saved(p, saved[3]);
     p.dloss = g.const_data_ptr<float>();
     p.dloss_stride = g.size(0) > 1 ? g.stride(0) : 1;
     if (need_x) {

@@ -481,9 +481,10 @@ AVEY_API int avey_linear_workspace_size(const AveyLinearParams* params, int back
  * have no part in anything, whatever x holds there, and their dx is zero.
  *
  * The forward call writes `saved` (rows + 1 floats: lse_i / log 2, and the bits of
- * the number of rows that count) for the backward call, which computes z again in
- * pieces of the vocabulary, from dloss (rows values dloss_stride apart for NONE, else
- * one):
+ * the number of rows that count) and `saved_low` (what fp32 leaves out of lse_i / log 2)
+ * for the backward call, which computes z again in pieces of the vocabulary, from dloss
+ * (rows values dloss_stride apart for NONE, else one). Without `saved_low`, p - 1 of a row
+ * that is sure of its target is off by 2^-24 |lse|.
  *
  *   dz_ij = g_i ((1 + 2 z_loss lse_i) exp(z_ij - lse_i) - [j = t_i])
  *   dx = dz W, dweight = dz^T x
@@ -526,6 +527,7 @@ typedef struct AveyLossParams {
 
   void* workspace; /* 256-byte aligned, >= avey_loss_workspace_size() bytes */
   uint64_t workspace_bytes;
+  float* saved_low; /* [rows], or NULL in both calls (or a block that ends before it) */
 } AveyLossParams;
 
 AVEY_API int avey_loss_fwd_v1(const AveyLossParams* params, void* stream);

@@ -303,6 +303,35 @@ def test_losses_of_sure_rows_keep_their_digits_whatever_the_logits_size(rows, to
     assert ((got.double() - want).abs() <= bound).all(), float(((got.double() - want).abs() / bound).max())
 
 
+@pytest.mark.parametrize('device', ['cpu', pytest.param('cuda', marks=pytest.mark.gpu)])
+@pytest.mark.parametrize('top', [30, 96, 416, 4096])
+@pytest.mark.parametrize('rows', [8, 300])
+def test_gradients_of_sure_rows_keep_their_digits_whatever_the_logits_size(rows, top, device):
+    """dx is dz itself (the weight is the identity), rounded to the operands' type twice. A probability is off by
+    the power's and the coefficient's rounding, 3 2^-22, and by that of the sum of powers that the
+    test of the losses counts, 2^-22 + 40 2^-24; p - 1 by as much of 1."""
+    dt = torch.float32 if device == 'cpu' else torch.bfloat16
+    x, w, t = sure(rows, top, device, dt)
+    _, dx, _ = run(x, w, t, torch.ones((), device=device), reduction='sum')
+    z = x.double()
+    p = torch.softmax(z, 1)
+    hit = torch.nn.functional.one_hot(t, 512).bool()
+    want = torch.where(hit, -p.masked_fill(hit, 0).sum(1, keepdim=True), p)
+    unit = 2.0 ** -24 if device == 'cpu' else UNIT[dt]
+    bound = (4 * 2.0 ** -22 + 40 * 2.0 ** -24) * torch.where(hit, 1.0, p) + 2.1 * unit * want.abs() + 2.0 ** -126
+    off = (dx.double() - want).abs() / bound
+    assert float(off.max()) <= 1, float(off.max())
+
+
+def test_c_blocks_that_end_before_the_low_parts_are_taken():
+    short = _native.AveyLossParams.saved_low.offset
+    size = _native.loss_workspace_size(_params(), backward=False)
+    assert _native.loss_workspace_size(_params(struct_size=short), backward=False) == size
+    lib = _native.lib()
+    assert lib.avey_loss_fwd_v1(ctypes.byref(_params(saved_low=(1 << 20) + 2)), None) == -1
+    assert b'aligned' in lib.avey_last_error()
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize('dt', DTYPES)
 @pytest.mark.parametrize('rows', [5, 400])
