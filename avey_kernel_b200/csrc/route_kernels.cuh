@@ -104,7 +104,7 @@ __device__ __forceinline__ void rt_scores(const float (&z)[R], bool softmax, flo
     for (int i = 0; i < R; ++i) s[i] *= inv;
   } else {
 #pragma unroll
-    for (int i = 0; i < R; ++i) s[i] = __fdividef(1.f, 1.f + expf(-z[i]));  // 0 past 2^126, as far as any order goes
+    for (int i = 0; i < R; ++i) s[i] = __fdividef(1.f, 1.f + expf(-z[i]));  // 0 below 2^-126
   }
 }
 
@@ -337,9 +337,10 @@ __device__ __forceinline__ void rt_choose(const RtArgs& q, int64_t t, const floa
   uint32_t keep = 0xFFFFFFFFu;
   const bool by_logit = !q.bias, sums = q.groups > 1 && q.group_best == 2;
   // Bounds of the errors of two ranks relative to their terms: the exponential and the
-  // division (2^-21), the softmax's common sum of up to 32 + 5 additions (37 2^-24), the
-  // addition of the bias (2^-24).
-  const float tol = q.softmax ? 4e-6f : 1e-6f;
+  // division (2^-21), the softmax's common sum of up to 32 + 5 additions (37 2^-24) and
+  // the difference to its maximum (2^-18, half a step below 128; a score further down is 0), the
+  // addition of the bias (2^-24). And in all: scores below 2^-126 have fewer digits, or are 0.
+  const float tol = q.softmax ? 7e-6f : 1e-6f, least = 0x1p-120f;
   float r[R];
   uint32_t key[R];
   if (by_logit && !sums) {
@@ -402,7 +403,7 @@ __device__ __forceinline__ void rt_choose(const RtArgs& q, int64_t t, const floa
     keep = rt_keep(q, merit, lane, in, out);
     if (q.top_groups < q.groups && !(by_logit && !sums)) {
       const float terms = fabsf(first) + (two ? fabsf(second) : 0.f) + 2.f * most;
-      const float bound = tol * (__shfl_sync(0xFFFFFFFFu, terms, in) + __shfl_sync(0xFFFFFFFFu, terms, out));
+      const float bound = tol * (__shfl_sync(0xFFFFFFFFu, terms, in) + __shfl_sync(0xFFFFFFFFu, terms, out)) + least;
       const float m_in = __shfl_sync(0xFFFFFFFFu, merit, in), m_out = __shfl_sync(0xFFFFFFFFu, merit, out);
       if (m_out > -CUDART_INF_F && m_in - m_out <= bound) keep = rt_keep64<T, R>(q, t, lane);
     }
@@ -425,7 +426,9 @@ __device__ __forceinline__ void rt_choose(const RtArgs& q, int64_t t, const floa
   float before = 0.f;
   int before_e = 0;
   // Near: two ranks whose order their errors may change. Alike: of equal logits and biases.
-  auto near = [&](float a, float b) { return b > -CUDART_INF_F && a - b <= tol * (fabsf(a) + fabsf(b) + 2.f * most); };
+  auto near = [&](float a, float b) {
+    return b > -CUDART_INF_F && a - b <= tol * (fabsf(a) + fabsf(b) + 2.f * most) + least;
+  };
   auto alike = [&](int a, int b) {
     return Elem<T>::load(row + a) == Elem<T>::load(row + b) && __ldg(q.bias + a) == __ldg(q.bias + b);
   };

@@ -201,6 +201,30 @@ def test_clusters_of_near_scores_at_the_border(score, n, groups, k, device):
 
 
 @pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('score', ['softmax', 'sigmoid'])
+@pytest.mark.parametrize('depth', [(88.0, 104.0), (64.0, 88.0), (100.0, 140.0)])
+@pytest.mark.parametrize('n,groups', [(32, 8), (24, 8), (256, 16), (60, 10)])
+def test_small_scores_keep_the_order_of_exact_arithmetic(n, groups, depth, score, device):
+    """Scores that fp32 holds with a few bits, or as 0, and those whose distance to the largest logit it rounds by
+    some 10^-6: groups (and with a bias of zeros experts) whose ranks are alike or near."""
+    g = torch.Generator().manual_seed(n)
+    rows, size = 1500, n // groups
+    base = -depth[0] - (depth[1] - depth[0]) * torch.rand(rows, 1, size, generator=g)
+    near = torch.where(torch.rand(rows, groups, 1, generator=g) < 0.5, 2.0 ** -18, 2.0 ** -2)
+    z = base + near * torch.randn(rows, groups, size, generator=g)
+    swap = torch.rand(rows, groups, generator=g).argsort(1)  # which group is how near
+    z = z.gather(1, swap.unsqueeze(-1).expand_as(z)).reshape(rows, n)
+    if score == 'softmax':
+        z[:, 0] = 0.0
+        z = z + 13.37
+    for bias, best in ((None, 2), (torch.zeros(n), 2), (torch.zeros(n), 1)):
+        kw = dict(score=score, groups=groups, top_groups=2, group_best=best)
+        want = choose64(z, min(3, 2 * size), bias, **kw)
+        _, chosen = experts.route(z.to(device), min(3, 2 * size), bias=None if bias is None else bias.to(device), **kw)
+        assert torch.equal(chosen.cpu(), want), int((chosen.cpu() != want).any(1).sum())
+
+
+@pytest.mark.parametrize('device', DEVICES)
 @pytest.mark.parametrize('groups', [1, 4])
 @pytest.mark.parametrize('score', ['softmax', 'sigmoid'])
 @pytest.mark.parametrize('renormalize', [True, False])
