@@ -1,7 +1,7 @@
 // The launches of one call, in order on one stream: all but the first may be set up
-// beside the end of the one before. Every kernel launched so waits for that one
-// (griddepcontrol.wait) ahead of its first read, in every thread, so what an earlier launch
-// wrote is seen by all later ones.
+// beside the end of the one before. Every kernel launched so, those that are the first of
+// all their calls too, waits for that one (griddepcontrol.wait) ahead of its first read, in every
+// thread, so what an earlier launch wrote is seen by all later ones.
 #pragma once
 
 #include <cuda_runtime.h>

@@ -344,6 +344,7 @@ struct LnPack {
 };
 static __global__ void __launch_bounds__(256) ln_pack_rows(const LnPack a, const LnPack b) {
   griddep_launch_dependents();  // the products are set up meanwhile
+  griddep_wait();
   const int64_t na = a.rows * (a.ld / 8), nb = b.rows * (b.ld / 8);
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < na + nb;
        i += static_cast<int64_t>(gridDim.x) * 256) {

@@ -503,6 +503,7 @@ __device__ __forceinline__ float rt_part_sum(float x, int lanes) {
 // j-th chosen one.)
 template <typename T, int R>
 __global__ void __launch_bounds__(32 * kRtWarps) route_plain(const __grid_constant__ RtArgs q, int lanes) {
+  griddep_wait();
   const RtPart p = rt_part(lanes);
   const bool there = p.t < q.tokens;
   const int64_t t = there ? p.t : q.tokens - 1;  // (a part past the end goes along)
@@ -578,6 +579,7 @@ __global__ void __launch_bounds__(32 * kRtWarps) route_plain(const __grid_consta
 template <typename T, int R>
 __global__ void __launch_bounds__(32 * kRtWarps, R <= 4 ? 4 : R <= 8 ? 3 : 1)
     route_forward(const __grid_constant__ RtArgs q) {
+  griddep_wait();
   const int lane = threadIdx.x & 31, e0 = lane * R;
   float most = 0.f;  // the largest |bias|
   if (q.bias) {
@@ -633,6 +635,7 @@ __global__ void __launch_bounds__(32 * kRtWarps, R <= 4 ? 4 : R <= 8 ? 3 : 1)
 template <typename T, int R>
 __global__ void __launch_bounds__(32 * kRtWarps) route_backward(const __grid_constant__ RtArgs q, int lanes) {
   extern __shared__ float rows[];  // R values a thread and one of room, against bank conflicts
+  griddep_wait();
   const RtPart p = rt_part(lanes);
   const bool there = p.t < q.tokens;
   const int64_t t = there ? p.t : q.tokens - 1;  // (a part past the end goes along)

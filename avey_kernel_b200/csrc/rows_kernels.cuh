@@ -165,6 +165,7 @@ __global__ void __launch_bounds__(256) rw_clear(const int32_t* slots, const int3
 
 template <typename T, int N>
 __global__ void __launch_bounds__(256) rw_dispatch(const RwArgs q) {
+  griddep_wait();
   const int block = static_cast<int>(blockIdx.x) - q.blanks, blocks = static_cast<int>(gridDim.x) - q.blanks;
   if (block < 0) {
     rw_blank<T, N>(q, static_cast<T*>(q.rows), q.rows_ld);
@@ -219,6 +220,7 @@ __device__ __forceinline__ RwSlots rw_slots(const RwArgs& q, int64_t t, int j0) 
 
 template <typename T, int N, int HOLD>
 __global__ void __launch_bounds__(kRwThreads, rw_blocks(HOLD)) rw_combine(const RwArgs q, int lanes) {
+  griddep_wait();
   const RwPart at = rw_part(lanes);
   const int64_t places = q.tokens * q.k;
   const T* rows = static_cast<const T*>(q.rows);
@@ -272,6 +274,7 @@ __global__ void __launch_bounds__(kRwThreads, rw_blocks(HOLD)) rw_combine(const 
 // <dout_t, rows[slot_tj]>.
 template <typename T, int N, int HOLD>
 __global__ void __launch_bounds__(kRwThreads, rw_blocks(HOLD)) rw_combine_backward(const RwArgs q, int lanes) {
+  griddep_wait();
   if (static_cast<int>(blockIdx.x) < q.blanks) {
     rw_blank<T, N>(q, static_cast<T*>(q.out), q.width);
     return;
@@ -364,6 +367,7 @@ struct EmArgs {
 // A token outside the vocabulary gives a row of NaN. A part of a warp takes a row.
 template <typename T, int N>
 __global__ void __launch_bounds__(kRwThreads) em_forward(const EmArgs q, int lanes) {
+  griddep_wait();
   const RwPart at = rw_part(lanes);
   if (at.t >= q.n) return;
   const int64_t t = q.tokens64 ? __ldg(static_cast<const long long*>(q.tokens) + at.t)

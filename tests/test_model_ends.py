@@ -2,6 +2,7 @@
 model written in plain torch in 64 bits."""
 
 import importlib.util
+import re
 from pathlib import Path
 
 import pytest
@@ -126,3 +127,30 @@ def test_compiled_functions_call_the_operators():
     loss = compiled(*leaves)
     got = [loss.detach(), *torch.autograd.grad(loss, leaves)]
     assert all(torch.equal(p, q) for p, q in zip(got, train()))
+
+
+def test_chained_kernels_wait_for_the_one_before_ahead_of_their_reads():
+    """Every kernel that a chain of launches (launch_chain.h) names waits before anything that reads: what
+    its body calls ahead of the wait is none of the functions that load."""
+    csrc = Path(_native.__file__).parent / 'csrc'
+    launched = set()
+    for name in ('avey_loss.cu', 'avey_tokens.cu'):
+        source = (csrc / name).read_text()
+        calls = re.findall(r'chain\.launch\(\s*"[^"]*",\s*([\w:<>, ]+?)[,(]', source)
+        assert len(calls) == source.count('chain.launch(') and calls
+        launched |= {re.sub(r'<.*', '', call).split('::')[-1] for call in calls}
+    launched = {'ce_product' if name == 'K' else name for name in launched}  # launch_product's argument
+    seen = set()
+    for name in ('tc_loss.cuh', 'route_kernels.cuh', 'sort_kernels.cuh', 'rows_kernels.cuh', 'linear_steps.cuh'):
+        for part in (csrc / name).read_text().split('__global__')[1:]:
+            kernel = re.search(r'(\w+)\((?:const|CeMaps|float)', part[part.index(')'):] if '__launch_bounds__' in part[:40] else part)
+            if kernel.group(1) not in launched:
+                continue
+            seen.add(kernel.group(1))
+            body = part[part.index('{'):]
+            assert 'griddep_wait();' in body, kernel.group(1)
+            ahead = body[:body.index('griddep_wait();')]
+            for read in ('__ld', 'load', 'atomic', 'ce_target', 'ce_scale', 'st_key', 'st_count', 'st_place_block', 'st_zero', 'rw_blank',
+                         'rw_slots', 'rt_choose', 'q.keys', 'q.ids', 'q.edges', 'q.partial', 'q.each'):
+                assert read not in ahead, (kernel.group(1), read)
+    assert seen == launched, seen ^ launched
