@@ -36,6 +36,11 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, targets: torch.T
     A target outside the vocabulary makes its row's loss NaN, and with it the row's gradient and
     the weight's.
 
+    Memory beside the tensors and their gradients: the backward pass takes up to 512 MB
+    for pieces of the logits' gradient (16 KB a row above 32768 rows) and 6 bytes for
+    every element of x; rows that are not whole 16-byte units (of widths that 8 does not
+    divide, or views off 16 bytes) are copied in either pass, x's and the weight's.
+
     bf16 / f16 CUDA tensors of one dtype run natively, forward and backward, with
     any row strides: fp32 sums, the gradient at the logits rounded to the operand
     type before its two products (relative to the largest gradient that comes in, so

@@ -533,9 +533,13 @@ typedef struct AveyLossParams {
 AVEY_API int avey_loss_fwd_v1(const AveyLossParams* params, void* stream);
 AVEY_API int avey_loss_bwd_v1(const AveyLossParams* params, void* stream);
 
-/* Bytes of `workspace` of the forward (backward == 0) or backward call. The backward
- * call's holds pieces of dz of 512 MB (16 KB a row above 32768 rows) at most, whatever
- * the vocabulary, and beside them 6 bytes for every element of x. */
+/* Bytes of `workspace` of the forward (backward == 0) or backward call, at most:
+ *   backward: 512 MB for pieces of dz, or 16 KB a row above 32768 rows, and 1 KB a row to make them
+ *     whole tiles; 6 bytes for every element of x, its rows filled up to 8; 32 bytes a row; and for
+ *     the sums of dx's tiles that CTAs share 512 KB for each SM (without dweight 2 MB);
+ *   forward: the larger of 5 MB and 8 bytes a row for every 1024 words, and 8 bytes a row;
+ *   either: where the rows of x, or of the weight, are not whole 16-byte units (address, stride or
+ *     width), a copy of that array, 2 bytes an element, its rows filled up to 8. */
 AVEY_API int avey_loss_workspace_size(const AveyLossParams* params, int backward, uint64_t* bytes);
 
 /*
@@ -675,6 +679,10 @@ typedef struct AveyEmbeddingParams {
 
 AVEY_API int avey_embedding_fwd_v1(const AveyEmbeddingParams* params, void* stream);
 AVEY_API int avey_embedding_bwd_v1(const AveyEmbeddingParams* params, void* stream);
+
+/* Bytes of the backward call's `workspace`, at most: 32 a token for the sort, and for the parts of
+ * runs of one token a byte for every element of dy (its tokens filled up to 8), or for every 4 from 18944
+ * tokens on (up to 32); 4 KB. */
 AVEY_API int avey_embedding_workspace_size(const AveyEmbeddingParams* params, uint64_t* bytes);
 
 /*

@@ -241,3 +241,14 @@ def test_c_workspace_sizes():
     assert size.value == 4 * 512 + 256 + 1024
     p.dy = 0
     assert lib.avey_embedding_bwd_v1(ctypes.byref(p), None) == -1 and b'dy' in lib.avey_last_error()
+
+
+@pytest.mark.parametrize('count,width,vocab', [(1, 1, 1), (64, 64, 1000), (8192, 768, 32768), (8193, 1, 1000), (9471, 389, 1 << 30),
+                                               (18943, 5, 1 << 21), (18944, 768, 131072), (65536, 768, 131072), (1 << 20, 64, 1 << 20)])
+def test_workspace_is_what_the_header_says(count, width, vocab):
+    at, size = 1 << 20, ctypes.c_uint64()
+    p = _native.AveyEmbeddingParams(struct_size=ctypes.sizeof(_native.AveyEmbeddingParams), dtype=2, index_bits=64, count=count,
+                                    width=width, vocab=vocab, scale=1.0, tokens=at, dy=at, dy_ld=width, dtable=at)
+    assert _native.lib().avey_embedding_workspace_size(ctypes.byref(p), ctypes.byref(size)) == 0
+    # (The last piece of 8 to 32 places may be short: 8 bytes a column.)
+    assert size.value <= 32 * count + count * width / (4 if count >= 18944 else 1) + 8 * width + 4096

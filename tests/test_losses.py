@@ -605,6 +605,24 @@ def test_workspace_stays_small_whatever_the_logits_take():
     assert _native.loss_workspace_size(_params(rows=0)) == 0
 
 
+@pytest.mark.parametrize('width', [768, 769, 64])
+@pytest.mark.parametrize('rows,vocab', [(1, 131072), (8, 50000), (33, 32768), (100, 131072), (4096, 50021), (16384, 131072),
+                                        (40000, 131072), (262144, 131072), (8192, 1 << 20), (1 << 20, 1000)])
+def test_workspace_is_what_the_header_says(rows, vocab, width):
+    at, mb, sms = 1 << 20, 1 << 20, 148
+    whole = -(-width // 8) * 8
+    copies = 0 if whole == width else 2 * whole * (rows + vocab)
+    kw = dict(rows=rows, vocab=vocab, width=width, x_ld=width, weight_ld=width)
+    room = 256 * 16  # each part begins at a multiple of 256
+    size = _native.loss_workspace_size(_params(**kw), backward=False)
+    few = 0 if rows > 8 else copies  # up to 8 rows are read as they are
+    assert size <= max(8 * rows * (vocab / 1024 + 1), 5 * mb) + 8 * rows + copies - few + room
+    for dweight, share in ((at, mb / 2), (0, 2 * mb)):
+        size = _native.loss_workspace_size(_params(dloss=at, dx=at, dx_ld=width, dweight=dweight, **kw), backward=True)
+        dz = max(512 * mb, 16384 * rows if rows > 32768 else 0) + 1024 * rows
+        assert size <= dz + 6 * whole * rows + 32 * rows + sms * share + copies + room
+
+
 def test_operands_are_read_after_the_wait_for_the_grid_before():
     """Every kernel that may be launched while the step before it runs waits for it, in all of its
     threads, before it reads anything."""
