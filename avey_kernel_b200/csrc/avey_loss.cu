@@ -93,9 +93,9 @@ int unit_tiles(int64_t mt, int64_t nt) {
 // Of a gradient's product over `width` columns (boxes of 64 for each CTA).
 int grad_cols(int64_t width) { return width > 128 ? 256 : 128; }
 
-// Rows up to which the statistics take the kernel for few rows (8 rows, 32768 x 768: 22
-// us against 26 by tiles, 131072 x 1024: 65 against 80, 50021 x 389: 39 against 43; 16
-// rows, which would be two passes of its products: 29, 90 and 76).
+// Rows up to which the statistics take the kernel for few rows (calls with W out of L2: 8 rows of 32768 x
+// 768 25 us, where 9 by tiles take 27; of 131072 x 1024 74 and 76, of 50021 x 389 40 and 44; one row
+// 23, 69 and 38. 16 rows in two passes of its products took longer than by tiles).
 constexpr int64_t kFewRows = 8;
 bool use_few(const AveyLossParams* p) { return p->rows <= kFewRows; }
 // Its CTAs: a warp for 16 rows of W, up to four CTAs an SM.

@@ -23,9 +23,9 @@
 // Bound: the logits' bytes, or instructions. Without a bias and groups (route_plain) and
 // in the gradient a token takes as many lanes as give each 16 of its experts, so that a
 // warp's shuffles serve several tokens: 65536 tokens of 128 experts, the best 4, 25 us
-// forward and 18 backward, where a warp for each token took 39 and 23. With them a warp
+// forward and 18 backward from cold caches, where a warp for each token took 39 and 23. With them a warp
 // takes a token; few tokens leave it latency-bound, many its instructions (65536 of 256 experts
-// in 8 groups: 123 us; some 15% more with two blocks an SM for R = 8 instead of three).
+// in 8 groups: 127 us; some 15% more with two blocks an SM for R = 8 instead of three).
 #pragma once
 
 #include <math_constants.h>

@@ -10,7 +10,7 @@
 // time (less where rows are not whole 16-byte units); a token's rows belong to one warp
 // (or a part of one, for narrow rows), which has up to 16 accesses a lane under way and
 // the next token's slots read ahead. (32768 tokens, four rows of 768 in bf16: combine with
-// a residual 68 us for 302 MB, its backward pass 85 for 453, dispatch 39 for 252; a
+// a residual 71 us for 302 MB, its backward pass 84 for 453, dispatch 40 for 252; a
 // bare sum over 268 MB takes 59 here, over 4.3 GB 666: what memory gives is 17 us and
 // 6.6 TB/s.)
 // Sums are fp32, in the order of the choices, or of the tokens.
@@ -115,8 +115,8 @@ struct RwArgs {
 // Rows that no slot names are zeros, not what memory held before. Up to kRwBlankPlaces places:
 // a block ahead of the call's own reads the slots, marks the places that they name in a bit map in
 // shared memory and clears the others, waiting for nothing (16 tokens of two: 1.7 us for the launch
-// instead of 1.6). One block takes 60 us for 131072 slots beside
-// the rows' own traffic, so more places take a launch of their own (rw_clear).
+// instead of 1.6). One block takes 60 us for 131072 slots beside the rows' own traffic, so more
+// places take a launch of their own (rw_clear).
 constexpr int kRwBlankPlaces = 8192;
 template <typename T, int N>
 __device__ __forceinline__ void rw_blank(const RwArgs& q, T* rows, int64_t ld) {
@@ -143,7 +143,8 @@ __device__ __forceinline__ void rw_blank(const RwArgs& q, T* rows, int64_t ld) {
 
 // More places: the launch before has left in namer[p] the number of the choice that names p, and
 // where none does, whatever was there: if that is a choice whose slot is p then p is named after all, so
-// nothing has to be set up. A warp looks at 32 places. (131072 places: 2 us of dispatch and of combine's backward pass.)
+// nothing has to be set up. A warp looks at 32 places. (131072 places: 4 us by itself, 2 of dispatch and of
+// combine's backward pass each, as it is set up beside their ends.)
 template <typename T, int N>
 __global__ void __launch_bounds__(256) rw_clear(const int32_t* slots, const int32_t* namer, int places, T* rows,
                                                 int64_t ld, int width) {

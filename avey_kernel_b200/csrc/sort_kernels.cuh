@@ -289,8 +289,9 @@ __global__ void __launch_bounds__(kStThreads) st_place(const StArgs q) {
 
 // Up to kStOneBlock entries in one launch, whatever the keys: an entry's place is the number of
 // lower keys and of equal ones before it, counted over all keys by a warp for kStEach
-// entries. (Lookup and gradient of 8192 tokens of 768, vocabulary 32768: 39 us, with one block's
-// passes by digits 57; 2047 of 389, 32003: 21 and 27; 64 of 64, 1000: 8.9 and 9.7.)
+// entries. (The kernels of lookup and gradient, replayed from a graph: 8192 tokens of 768, vocabulary
+// 32768: 39 us, with one block's passes by digits 57; 2047 of 389, 32003: 21 and 27; 64 of 64, 1000: 8.9 and
+// 9.7. Calls as they come take longer up to 8192 tokens, 60 to 70 us: the autograd engine's time on the host.)
 constexpr int kStRankThreads = 256, kStEach = 4, kStRankEntries = kStRankThreads / 32 * kStEach;
 __global__ void __launch_bounds__(kStRankThreads) st_rank(const StArgs q) {
   extern __shared__ uint32_t hist[];  // the keys

@@ -677,7 +677,7 @@ __global__ void __launch_bounds__(kCeThreads, 1)
 // consecutive k (32 bytes) of a 64-wide step for its fragments, so that four lanes read
 // a whole line; the order of k inside a product is free as long as both operands agree. A
 // warp takes 16 rows of W at a time and keeps (c, s) of the rows of x; a CTA's warps are
-// joined at the end. 131072 x 1024: 59 us, 4.5 TB/s.
+// joined at the end. 131072 x 1024: 49 us in calls in a row, 5.5 TB/s.
 constexpr int kCfWarps = 8, kCfRows = 8;
 struct CeFew {
   int rows, vocab, width;
