@@ -224,10 +224,12 @@ int validate(const AveyRowsParams* p, int what) {
   return AVEY_OK;
 }
 
-// Workspace for the places that no slot names.
+// Whether places that no slot names are cleared (a block that ends before its workspace had no such
+// field), and the workspace for it.
+bool clears(const AveyRowsParams* p) { return p->struct_size == sizeof(AveyRowsParams) && p->clear != 0; }
 uint64_t clear_bytes(const AveyRowsParams* p) {
   const int64_t places = p->tokens * p->k;
-  return p->clear && places > avey::kRwBlankPlaces ? static_cast<uint64_t>(places) * 4 : 0;
+  return clears(p) && places > avey::kRwBlankPlaces ? static_cast<uint64_t>(places) * 4 : 0;
 }
 
 // Bytes of an access that all rows are whole multiples of.
@@ -288,13 +290,10 @@ int run_rows(const AveyRowsParams* p, int what, void* stream) {
   int rc = validate(p, what);
   if (rc != AVEY_OK) return rc;
   // combine writes no places, and the gradient of rows may not be wanted.
-  const bool clear = p->clear != 0 && (what == 0 || (what == 2 && p->drows));
+  const bool clear = clears(p) && (what == 0 || (what == 2 && p->drows));
   const uint64_t need = clear ? clear_bytes(p) : 0;
-  if (need) {
-    if (p->struct_size != sizeof(AveyRowsParams)) return fail(AVEY_ERR_ARGUMENT, "clear needs the block's workspace");
-    rc = check_workspace(p->workspace, p->workspace_bytes, need);
-    if (rc != AVEY_OK) return rc;
-  }
+  if (need) rc = check_workspace(p->workspace, p->workspace_bytes, need);
+  if (rc != AVEY_OK) return rc;
   rc = avey_host::device_ok();
   if (rc != AVEY_OK || p->tokens == 0) return done(rc);
   avey::RwArgs q{};

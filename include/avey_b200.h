@@ -641,7 +641,7 @@ typedef struct AveyRowsParams {
 } AveyRowsParams;
 
 /* Bytes of `workspace`: 0 without `clear` and up to 8192 places, else 4 a place. (A block that ends
- * before `workspace` is taken too, where it needs none.) */
+ * before `workspace` is taken too, as one without `clear`.) */
 AVEY_API int avey_rows_workspace_size(const AveyRowsParams* params, uint64_t* bytes);
 
 AVEY_API int avey_dispatch_v1(const AveyRowsParams* params, void* stream);

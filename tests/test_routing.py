@@ -836,5 +836,7 @@ def test_c_rows_workspace():
     for call in (lib.avey_dispatch_v1, lib.avey_combine_bwd_v1):
         for kw, match in ((dict(tokens=4097), b'workspace'), (dict(tokens=4097, workspace=at, workspace_bytes=8), b'smaller'),
                           (dict(tokens=4097, workspace=at + 4, workspace_bytes=1 << 20), b'aligned'),
-                          (dict(tokens=4097, struct_size=short), b'workspace'), (dict(struct_size=short - 8), b'struct_size')):
+                          (dict(struct_size=short - 8), b'struct_size')):
             assert call(ctypes.byref(rows(**kw)), None) == -1 and match in lib.avey_last_error()
+    assert lib.avey_rows_workspace_size(ctypes.byref(rows(tokens=4097, struct_size=short)), ctypes.byref(size)) == 0
+    assert size.value == 0  # what stands where `clear` is now had no meaning there
